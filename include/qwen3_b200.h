@@ -301,6 +301,69 @@ int qk_swiglu_rows(const void* gu, int M, int I, void* h, qk_stream_t stream);
  * lowest index) of bf16 logits row r of [rows][V]; qk_finalize decodes it. The batched decode step's argmax. */
 int qk_argmax_rows(const void* logits, int rows, int V, unsigned long long* best, qk_stream_t stream);
 
+/* Serving from a paged KV cache: many sequences of different lengths, whose caches grow in pages.
+ *
+ * A ragged batch: sequence b owns token rows cu_rows[b] .. cu_rows[b+1]-1 (int32 [batch + 1], ascending from 0) and
+ * ends, with them, at length seq_lens[b] (int32 [batch]), so row cu_rows[b] + i is position
+ * seq_lens[b] - (cu_rows[b+1] - cu_rows[b]) + i. Position p lies in slot p % page_size of page
+ * block_table[b * table_stride + p / page_size] (int32, table_width entries per sequence; entries past a sequence's
+ * end are not read). Lengths and tables are device data: a captured call follows their contents. A position or page
+ * outside the table, the rotary tables or the pool sets the error word's bad-state bit and its row is not written
+ * (attention reads page 0 in its place). Rows past cu_rows[batch] are left alone.
+ * Pages: [n_pages][n_kv][page_size][128], page_size 16, 32, 64 or 128; bf16, or (kv_fp8 = 1) e4m3 bytes with fp32 row
+ * scales [n_pages][n_kv][page_size]: s = max|x| / 448, q = e4m3(x / s), a zero row has s = 0 and zero bytes. Everything
+ * 16-byte aligned. Strides are in elements; rows and heads start on 16-byte boundaries.
+ *
+ * qk_paged_qkv: from the qkv projection's rows [T][(n_q + 2 n_kv) * 128] (qkv_stride apart), per-head RMSNorm with
+ *   q_norm/k_norm [128] (or both NULL: none), then rotary positions from fp32 tables [max_pos][rot_half]: the first
+ *   2 rot_half dims of a head (a multiple of 16) turn, in pairs (i, i + rot_half), or (2i, 2i + 1) where `interleaved`:
+ *   (a, b) -> (a cos - b sin, b cos + a sin). q to q_out, K and V rows to the pages, K also to k_out unless NULL
+ *   (before quantisation). fp32 inside, one rounding at each store. The two layouts, partial rotation and scaled
+ *   frequencies are the tables' and arguments' business; the bf16-table rotation of the decode step is
+ *   qk_prefill_qkv's.
+ * qk_paged_kv_read: positions starts[b] + i (0 + i for starts NULL) of every sequence into row cu_rows[b] + i of k_out
+ *   and v_out (bf16, row_stride between rows, head_stride between heads), dequantised.
+ * qk_paged_attention: out[t][h] = sum over positions j <= pos(t) of softmax_j(scale * q[t][h] . K[g][j]) V[g][j],
+ *   g = h / (n_q / n_kv), 1 to 32 query heads per KV head; a row without a visible position gives zeros. max_q: at
+ *   least the most token rows of a sequence (a longer one sets the bad-state bit and keeps its old output).
+ * qk_packed_attention: the same over whole prompts packed without padding: row t of prompt b sees rows
+ *   cu_rows[b] .. t of k and v (kv_row between rows, kv_head between heads).
+ * workspace: qk_ragged_attention_workspace_bytes() bytes, 256-byte aligned, zeroed once; every call leaves it ready
+ *   for the next. Calls that may overlap need one each. */
+typedef struct {
+  const void *k_pages, *v_pages;
+  const float *k_scale, *v_scale;          /* NULL for bf16 pages */
+  const int *cu_rows, *seq_lens, *block_table;
+  long long batch, n_kv, n_pages, page_size, table_width, table_stride, kv_fp8;
+} qk_paged_cache_t;
+typedef struct {
+  qk_paged_cache_t cache;
+  const void* qkv;
+  void *q_out, *k_out;                     /* k_out NULL: not wanted */
+  const void *q_norm, *k_norm;
+  const float *cos_tab, *sin_tab;
+  long long rows, n_q, qkv_stride, q_stride, k_stride, max_pos, rot_half, interleaved;
+  double eps;
+} qk_paged_qkv_t;
+typedef struct {
+  qk_paged_cache_t cache;                  /* seq_lens unused */
+  const int* starts;                       /* NULL: 0 */
+  void *k_out, *v_out;
+  long long rows, row_stride, head_stride;
+} qk_paged_kv_read_t;
+typedef struct {
+  qk_paged_cache_t cache;                  /* packed prompts: cu_rows, batch and n_kv only */
+  const void *q, *k, *v;                   /* k and v: packed prompts only */
+  void *out, *workspace;
+  long long rows, n_q, max_q, q_row, q_head, kv_row, kv_head, out_row, out_head, workspace_bytes;
+  double scale;
+} qk_ragged_attention_t;
+int qk_paged_qkv(const qk_paged_qkv_t* args, qk_stream_t stream);
+int qk_paged_kv_read(const qk_paged_kv_read_t* args, qk_stream_t stream);
+long long qk_ragged_attention_workspace_bytes(void);
+int qk_paged_attention(const qk_ragged_attention_t* args, qk_stream_t stream);
+int qk_packed_attention(const qk_ragged_attention_t* args, qk_stream_t stream);
+
 /* Tensor-parallel helpers (no counterpart in the single-GPU reference; the TP plan of its decode step):
  * resid[i] = bf16(resid[i] + bf16(sum[i])) for the fp32 all-reduced partial of a row-parallel GEMV (the
  * rounding of the reference's residual epilogue, decode.cu:320-323); and the top-bit flip of packed argmax

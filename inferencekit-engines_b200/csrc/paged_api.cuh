@@ -1,0 +1,183 @@
+// C entry points of the paged-serving operators (paged.cuh, attention_ragged.cuh). Included by qwen3_b200.cu, whose
+// argument-check and launch helpers it uses.
+#pragma once
+
+// the shim packs these structs field by field
+static_assert(sizeof(qk_paged_cache_t) == 14 * 8 && sizeof(qk_paged_qkv_t) == 30 * 8 && sizeof(qk_paged_kv_read_t) == 20 * 8 &&
+                  sizeof(qk_ragged_attention_t) == 30 * 8,
+              "argument structs have 8-byte fields only");
+
+namespace {
+
+// The checks every paged entry point shares, and the cache as the kernels take it.
+int paged_cache(PagedCache* c, const qk_paged_cache_t& a, bool lens) {
+  if (!a.k_pages || !a.v_pages || !a.cu_rows || !a.block_table || (lens && !a.seq_lens)) return fail(QK_EINVAL, "null pointer argument");
+  if (a.kv_fp8 && (!a.k_scale || !a.v_scale)) return fail(QK_EINVAL, "an e4m3 cache needs its row scales");
+  if (a.page_size != 16 && a.page_size != 32 && a.page_size != 64 && a.page_size != 128)
+    return fail(QK_EINVAL, "page_size=%lld (16, 32, 64 or 128)", a.page_size);
+  if (a.n_pages < 1 || a.n_kv < 1 || a.n_kv > 1024 || a.batch < 0 || a.batch > 65536)
+    return fail(QK_EINVAL, "n_pages=%lld n_kv=%lld batch=%lld", a.n_pages, a.n_kv, a.batch);
+  // rows are counted in 32 bits (bytes are not)
+  if (a.n_pages > 0x7fffffffll / (a.n_kv * a.page_size)) return fail(QK_EINVAL, "a pool of more than 2^31 - 1 rows");
+  if (a.table_width < 1 || a.table_stride < a.table_width || a.table_stride > 0x7fffffffll || a.table_width > 0x7fffffffll / a.page_size)
+    return fail(QK_EINVAL, "table_width=%lld table_stride=%lld", a.table_width, a.table_stride);
+  if (!aligned(a.k_pages, 16) || !aligned(a.v_pages, 16) || !aligned(a.k_scale, 16) || !aligned(a.v_scale, 16))
+    return fail(QK_EINVAL, "pages and scales must be 16-byte aligned");
+  c->k = static_cast<uint8_t*>(const_cast<void*>(a.k_pages));
+  c->v = static_cast<uint8_t*>(const_cast<void*>(a.v_pages));
+  c->ks = const_cast<float*>(a.k_scale);
+  c->vs = const_cast<float*>(a.v_scale);
+  c->table = a.block_table;
+  c->cu = a.cu_rows;
+  c->seq_lens = a.seq_lens;
+  c->B = (int)a.batch;
+  c->n_kv = (int)a.n_kv;
+  c->n_pages = (int)a.n_pages;
+  c->page_shift = 31 - __builtin_clz((unsigned)a.page_size);
+  c->table_width = (int)a.table_width;
+  c->table_stride = (int)a.table_stride;
+  return QK_OK;
+}
+
+bool row_strides(long long a, long long b) { return a >= 0 && b >= 0 && a % 8 == 0 && b % 8 == 0 && a < (1ll << 40) && b < (1ll << 40); }
+
+// What both attention entry points check: heads, strides (elements), alignment, scale, workspace.
+int ragged_common(RaggedParams* p, const qk_ragged_attention_t& a) {
+  const long long n_kv = a.cache.n_kv;
+  if (!a.q || !a.out || !a.workspace) return fail(QK_EINVAL, "null pointer argument");
+  if (a.rows < 0 || a.rows > 0x7fffffffll / 64 || n_kv < 1 || n_kv > 1024 || a.n_q < 1 || a.n_q % n_kv || a.n_q / n_kv > 32)
+    return fail(QK_EINVAL, "rows=%lld n_q=%lld n_kv=%lld (1 to 32 query heads per KV head)", a.rows, a.n_q, n_kv);
+  const float scale = (float)a.scale;
+  if (!(scale > 1e-30f) || !(scale < 1e30f)) return fail(QK_EINVAL, "scale=%g must be positive", a.scale);
+  if (a.max_q < 1) return fail(QK_EINVAL, "max_q=%lld", a.max_q);
+  if (!aligned(a.q, 16) || !aligned(a.out, 16) || !row_strides(a.q_row, a.q_head) || !row_strides(a.out_row, a.out_head))
+    return fail(QK_EINVAL, "q and out rows and heads must start on 16-byte boundaries");
+  if (a.workspace_bytes < qk_ragged_attention_workspace_bytes() || !aligned(a.workspace, 256))
+    return fail(QK_EINVAL, "workspace of %lld bytes: %lld needed, 256-byte aligned", a.workspace_bytes, qk_ragged_attention_workspace_bytes());
+  p->q = static_cast<const bf16*>(a.q);
+  p->out = static_cast<bf16*>(a.out);
+  p->q_row = a.q_row;
+  p->q_head = a.q_head;
+  p->out_row = a.out_row;
+  p->out_head = a.out_head;
+  p->T = (int)a.rows;
+  p->n_q = (int)a.n_q;
+  p->group = (int)(a.n_q / n_kv);
+  p->scale = scale;
+  return QK_OK;
+}
+
+int half_warp_grid(long long rows, long long heads, dim3* grid) {   // a warp per row and pair of heads, 8 warps a CTA
+  const long long n = (rows * ((heads + 1) / 2) + 7) / 8;
+  if (n > 0x7fffffff / 8) return fail(QK_EINVAL, "%lld rows are too many", rows);
+  *grid = dim3((unsigned)n);
+  return QK_OK;
+}
+
+template <int SRC>
+int launch_ragged(const RaggedParams& p, cudaStream_t stream) {
+  const long long warps = (long long)p.T * p.n_q;
+  return launch(ragged_attention_kernel<SRC>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int qk_paged_qkv(const qk_paged_qkv_t* args, qk_stream_t stream) {
+  if (!args) return fail(QK_EINVAL, "null pointer argument");
+  const qk_paged_qkv_t& a = *args;
+  PagedQkvParams p = {};
+  if (!a.qkv || !a.cos_tab || !a.sin_tab || !a.q_out) return fail(QK_EINVAL, "null pointer argument");
+  if ((a.q_norm == nullptr) != (a.k_norm == nullptr)) return fail(QK_EINVAL, "q_norm and k_norm go together");
+  if (a.rows < 0 || a.rows > 0x7fffffffll / 64 || a.n_q < 1 || a.n_q > 4096) return fail(QK_EINVAL, "rows=%lld n_q=%lld", a.rows, a.n_q);
+  if (a.rot_half < 8 || a.rot_half > HEAD_DIM / 2 || a.rot_half % 8)
+    return fail(QK_EINVAL, "rotary dims %lld must be a multiple of 16, at most %d", 2 * a.rot_half, HEAD_DIM);
+  if (a.max_pos < 1 || a.max_pos > 0x7fffffffll) return fail(QK_EINVAL, "max_pos=%lld", a.max_pos);
+  if (int r = paged_cache(&p.c, a.cache, true)) return r;
+  if (a.qkv_stride < (a.n_q + 2 * p.c.n_kv) * HEAD_DIM || a.q_stride < a.n_q * HEAD_DIM ||
+      (a.k_out && a.k_stride < (long long)p.c.n_kv * HEAD_DIM) || !row_strides(a.qkv_stride, a.q_stride) || !row_strides(a.k_stride, 0))
+    return fail(QK_EINVAL, "rows overlap or do not start on 16-byte boundaries: qkv_stride=%lld q_stride=%lld k_stride=%lld",
+                a.qkv_stride, a.q_stride, a.k_stride);
+  if (!aligned(a.qkv, 16) || !aligned(a.q_out, 16) || !aligned(a.k_out, 16) || !aligned(a.q_norm, 16) || !aligned(a.k_norm, 16) ||
+      !aligned(a.cos_tab, 16) || !aligned(a.sin_tab, 16))
+    return fail(QK_EINVAL, "qkv, q_out, k_out, norms and tables must start on 16-byte boundaries");
+  if (a.rows == 0 || p.c.B == 0) return QK_OK;
+  p.qkv = static_cast<const bf16*>(a.qkv);
+  p.q_out = static_cast<bf16*>(a.q_out);
+  p.k_out = static_cast<bf16*>(a.k_out);
+  p.q_norm = static_cast<const bf16*>(a.q_norm);
+  p.k_norm = static_cast<const bf16*>(a.k_norm);
+  p.cos = a.cos_tab;
+  p.sin = a.sin_tab;
+  p.qkv_stride = a.qkv_stride;
+  p.q_stride = a.q_stride;
+  p.k_stride = a.k_stride;
+  p.T = (int)a.rows;
+  p.n_q = (int)a.n_q;
+  p.max_pos = (int)a.max_pos;
+  p.half = (int)a.rot_half;
+  p.interleaved = a.interleaved != 0;
+  p.eps = (float)a.eps;
+  dim3 grid;
+  if (int r = half_warp_grid(a.rows, a.n_q + 2 * p.c.n_kv, &grid)) return r;
+  return launch(a.cache.kv_fp8 ? paged_qkv_kernel<true> : paged_qkv_kernel<false>, grid, dim3(256), 0,
+                static_cast<cudaStream_t>(stream), p);
+}
+
+int qk_paged_kv_read(const qk_paged_kv_read_t* args, qk_stream_t stream) {
+  if (!args) return fail(QK_EINVAL, "null pointer argument");
+  const qk_paged_kv_read_t& a = *args;
+  PagedReadParams p = {};
+  if (!a.k_out || !a.v_out) return fail(QK_EINVAL, "null pointer argument");
+  if (a.rows < 0 || a.rows > 0x7fffffffll / 64) return fail(QK_EINVAL, "rows=%lld", a.rows);
+  if (int r = paged_cache(&p.c, a.cache, false)) return r;
+  if (a.row_stride < HEAD_DIM || (a.head_stride < HEAD_DIM && p.c.n_kv > 1) || !row_strides(a.row_stride, a.head_stride) ||
+      !aligned(a.k_out, 16) || !aligned(a.v_out, 16))
+    return fail(QK_EINVAL, "row_stride=%lld head_stride=%lld: rows must not overlap and start on 16-byte boundaries", a.row_stride, a.head_stride);
+  if (a.rows == 0 || p.c.B == 0) return QK_OK;
+  p.starts = a.starts;
+  p.k_out = static_cast<bf16*>(a.k_out);
+  p.v_out = static_cast<bf16*>(a.v_out);
+  p.row_stride = a.row_stride;
+  p.head_stride = a.head_stride;
+  p.T = (int)a.rows;
+  dim3 grid;
+  if (int r = half_warp_grid(a.rows, p.c.n_kv, &grid)) return r;
+  return launch(a.cache.kv_fp8 ? paged_kv_read_kernel<true> : paged_kv_read_kernel<false>, grid, dim3(256), 0,
+                static_cast<cudaStream_t>(stream), p);
+}
+
+long long qk_ragged_attention_workspace_bytes(void) { return 256; }
+
+int qk_paged_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
+  if (!args) return fail(QK_EINVAL, "null pointer argument");
+  RaggedParams p = {};
+  if (int r = ragged_common(&p, *args)) return r;
+  if (int r = paged_cache(&p.c, args->cache, true)) return r;
+  if (p.T == 0 || p.c.B == 0) return QK_OK;
+  return args->cache.kv_fp8 ? launch_ragged<SRC_PAGED_FP8>(p, static_cast<cudaStream_t>(stream))
+                            : launch_ragged<SRC_PAGED>(p, static_cast<cudaStream_t>(stream));
+}
+
+int qk_packed_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
+  if (!args) return fail(QK_EINVAL, "null pointer argument");
+  const qk_ragged_attention_t& a = *args;
+  RaggedParams p = {};
+  if (int r = ragged_common(&p, a)) return r;
+  if (!a.k || !a.v || !a.cache.cu_rows) return fail(QK_EINVAL, "null pointer argument");
+  if (a.cache.batch < 0 || a.cache.batch > 65536) return fail(QK_EINVAL, "batch=%lld", a.cache.batch);
+  if (!aligned(a.k, 16) || !aligned(a.v, 16) || !row_strides(a.kv_row, a.kv_head))
+    return fail(QK_EINVAL, "k and v rows and heads must start on 16-byte boundaries");
+  if (p.T == 0 || a.cache.batch == 0) return QK_OK;
+  p.k = static_cast<const bf16*>(a.k);
+  p.v = static_cast<const bf16*>(a.v);
+  p.kv_row = a.kv_row;
+  p.kv_head = a.kv_head;
+  p.c.cu = a.cache.cu_rows;
+  p.c.B = (int)a.cache.batch;
+  p.c.n_kv = (int)a.cache.n_kv;
+  return launch_ragged<SRC_PACKED>(p, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

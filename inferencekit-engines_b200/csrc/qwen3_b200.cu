@@ -11,9 +11,11 @@
 #include "../../include/qwen3_b200.h"
 #include "attention.cuh"
 #include "attention_fp8kv.cuh"
+#include "attention_ragged.cuh"
 #include "common.cuh"
 #include "gemm_tc.cuh"
 #include "gemv.cuh"
+#include "paged.cuh"
 #include "prefill.cuh"
 #include "step.cuh"
 
@@ -908,3 +910,5 @@ extern "C" int qk_attention_fp8kv(const void* qkv, const void* q_norm_w, const v
   return launch(attn_merge_kernel, dim3(2 * n_kv * GQA, batch), dim3(ATT_MERGE_THREADS), smem_m, stream, m);
 }
 
+// ---- serving from a paged KV cache ----------------------------------------------------------------------------
+#include "paged_api.cuh"

@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -35,7 +36,7 @@ GEMV_QKV, GEMV_O, GEMV_GATE_UP, GEMV_DOWN = 0, 1, 2, 3
 GEMV_PARTIAL, GEMV_QKV_RESADD, GEMV_GATE_UP_RESADD = 5, 6, 7
 SCALE_BLOCK128, SCALE_CHANNEL = 0, 1
 
-_VP, _I, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+_VP, _I, _F, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
 _SIGS = {
     "qk_version": ([], _I),
     "qk_last_error": ([], ctypes.c_char_p),
@@ -75,6 +76,11 @@ _SIGS = {
     "qk_add_rows": ([_VP, _VP, ctypes.c_longlong, _VP], _I),
     "qk_swiglu_rows": ([_VP, _I, _I, _VP, _VP], _I),
     "qk_argmax_rows": ([_VP, _I, _I, _VP, _VP], _I),
+    "qk_paged_qkv": ([_VP, _VP], _I),
+    "qk_paged_kv_read": ([_VP, _VP], _I),
+    "qk_ragged_attention_workspace_bytes": ([], _L),
+    "qk_paged_attention": ([_VP, _VP], _I),
+    "qk_packed_attention": ([_VP, _VP], _I),
 }
 
 
@@ -125,6 +131,16 @@ def _p(t):
 
 def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def _raw_stream(dev: int) -> int:
+    """The current stream of a device as an integer (no stream object: the paged calls' host time is their launch)."""
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+_E4M3 = (torch.float8_e4m3fn, torch.uint8)
+# qk_paged_qkv_t, qk_paged_kv_read_t and qk_ragged_attention_t (the first 14 fields of each: qk_paged_cache_t)
+_QKV_ARGS, _READ_ARGS, _ATTENTION_ARGS = (struct.Struct(f) for f in ("7Q7q7Q8qd", "7Q7q3Q3q", "7Q7q5Q10qd"))
 
 
 class DecodeOps:
@@ -384,6 +400,185 @@ class DecodeOps:
         """best[r] = packed argmax key of bf16 logits row r ([rows, V]; ties to the lowest index)."""
         rows, V = logits.shape
         self._check(self.lib.qk_argmax_rows(_p(logits), rows, V, _p(best), _stream()), "argmax_rows")
+
+    # ---- serving from a paged KV cache ---------------------------------------------------------------------
+    # A ragged batch: sequence b owns rows cu[b] .. cu[b+1]-1 (int32 [B+1]) and ends, with them, at length seq_lens[b]
+    # (int32 [B]); its position p lies in slot p % page_size of page block_table[b, p // page_size] (int32 [B, width]).
+    # k_pages/v_pages: bf16 [pages, n_kv, page_size, 128], or e4m3 (uint8 or float8_e4m3fn) with fp32 row scales
+    # k_scale/v_scale [pages, n_kv, page_size]; page_size 16, 32, 64 or 128. Lengths and tables live on the device
+    # (the calls can be captured); a position or page outside them sets the device error word and is not written.
+    # The arguments go to the library as one packed struct: a ctypes call with 30 arguments costs more host time
+    # than the launch.
+    @staticmethod
+    def _paged(what, k_pages, v_pages, k_scale, v_scale, cu, lens, block_table):
+        """Check the cache and the batch (lens None: none wanted); returns (B, n_kv, device index, the fields of
+        qk_paged_cache_t)."""
+        dev = k_pages.get_device()
+        shape = k_pages.shape
+        if len(shape) != 4 or shape != v_pages.shape or not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+            raise RuntimeError(f"{what}: k_pages and v_pages must be contiguous [pages, n_kv, page_size, 128]")
+        pages, n_kv, page, hd = shape
+        dt = k_pages.dtype
+        fp8 = dt != torch.bfloat16
+        if hd != 128 or dt != v_pages.dtype or (fp8 and dt not in _E4M3):
+            raise RuntimeError(f"{what}: pages must be bf16, or e4m3 bytes (uint8 or float8_e4m3fn), 128 values per row")
+        ks = vs = 0
+        if fp8:
+            for s in (k_scale, v_scale):
+                if s is None or s.dtype != torch.float32 or s.shape != shape[:3] or not s.is_contiguous() or s.get_device() != dev:
+                    raise RuntimeError(f"{what}: an e4m3 cache needs contiguous fp32 k_scale and v_scale [pages, n_kv, page_size]")
+            ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
+        elif k_scale is not None or v_scale is not None:
+            raise RuntimeError(f"{what}: a bf16 cache has no row scales")
+        if cu.dtype != torch.int32 or block_table.dtype != torch.int32 or block_table.dim() != 2 or cu.dim() != 1 \
+                or not cu.is_contiguous():
+            raise RuntimeError(f"{what}: cu must be int32 [B+1] and block_table int32 [B, width]")
+        B, width = block_table.shape
+        stride, inner = block_table.stride()
+        if inner != 1 and width > 1:
+            raise RuntimeError(f"{what}: block_table rows must be contiguous")
+        if len(cu) != B + 1:
+            raise RuntimeError(f"{what}: cu has {len(cu)} entries for {B} sequences (B + 1 wanted)")
+        if dev < 0 or v_pages.get_device() != dev or cu.get_device() != dev or block_table.get_device() != dev:
+            raise RuntimeError(f"{what}: every tensor must be on the same CUDA device")
+        lens_ptr = 0
+        if lens is not None:
+            if lens.dtype != torch.int32 or lens.shape != (B,) or lens.get_device() != dev or not lens.is_contiguous():
+                raise RuntimeError(f"{what}: seq_lens must be int32 [{B}] on the cache's device")
+            lens_ptr = lens.data_ptr()
+        return B, n_kv, dev, (k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, cu.data_ptr(), lens_ptr, block_table.data_ptr(),
+                              B, n_kv, pages, page, width, max(stride, width), fp8)
+
+    @staticmethod
+    def _heads(what, name, t, dev):
+        """(rows, heads, row stride, head stride) of a bf16 [rows, heads, 128] or [rows, heads * 128] tensor."""
+        shape, strides = t.shape, t.stride()
+        if t.dtype == torch.bfloat16 and t.get_device() == dev and strides[-1] == 1:
+            if len(shape) == 3 and shape[2] == 128:
+                return shape[0], shape[1], strides[0], strides[1]
+            if len(shape) == 2 and shape[1] % 128 == 0:
+                return shape[0], shape[1] // 128, strides[0], 128
+        raise RuntimeError(f"{what}: {name} must be bf16 [rows, heads, 128] or [rows, heads * 128] on the call's device, the "
+                           "last dimension contiguous")
+
+    def attention_workspace(self, device) -> torch.Tensor:
+        """A workspace for paged_attention and packed_attention on `device` (zeroed once; every call leaves it
+        ready for the next). Calls that may run at the same time, on two streams, need one each."""
+        return torch.zeros(self.lib.qk_ragged_attention_workspace_bytes(), dtype=torch.uint8, device=device)
+
+    def _workspace(self, what, ws, dev, stream):
+        if ws is None:   # one per device and stream, kept
+            ws = self._scratch.get(("ragged", dev, stream))
+            if ws is None:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError(f"{what}: pass workspace=attention_workspace(device), made before the capture")
+                ws = self._scratch[("ragged", dev, stream)] = self.attention_workspace(torch.device("cuda", dev))
+        elif ws.dtype != torch.uint8 or ws.get_device() != dev or not ws.is_contiguous():
+            raise RuntimeError(f"{what}: workspace must come from attention_workspace() on the call's device")
+        return ws
+
+    def paged_qkv(self, qkv, cu, seq_lens, block_table, k_pages, v_pages, q_out, cos, sin, q_norm=None, k_norm=None,
+                  eps=1e-6, interleaved=False, k_scale=None, v_scale=None, k_out=None):
+        """The qkv projection's rows [T, (n_q + 2 n_kv) * 128] (bf16, any row stride): per-head RMSNorm with q_norm/k_norm
+        (bf16 [128], both or neither), rotary positions, q to q_out ([T, n_q, 128]), K and V rows into their
+        sequences' pages (quantised per row for an e4m3 cache). cos/sin: fp32 [max_pos, r / 2] (`model.rope_angles`);
+        the first r dims of a head turn, in pairs (i, i + r/2) or, interleaved, (2i, 2i + 1). k_out [T, n_kv, 128]
+        also takes the keys before quantisation (for `packed_attention` over the same rows). fp32 inside, one
+        rounding. Rows past cu[B] are left alone."""
+        B, n_kv, dev, cache = self._paged("paged_qkv", k_pages, v_pages, k_scale, v_scale, cu, seq_lens, block_table)
+        T, n_q, q_row, q_head = self._heads("paged_qkv", "q_out", q_out, dev)
+        w = (n_q + 2 * n_kv) * 128
+        if qkv.dtype != torch.bfloat16 or qkv.shape != (T, w) or qkv.stride(1) != 1 or qkv.get_device() != dev:
+            raise RuntimeError(f"paged_qkv: qkv must be bf16 [{T}, {w}], the last dimension contiguous")
+        if q_head != 128:
+            raise RuntimeError("paged_qkv: the heads of a q_out row must be contiguous")
+        k_row = k_ptr = qn = kn = 0
+        if k_out is not None:
+            kT, heads, k_row, k_head = self._heads("paged_qkv", "k_out", k_out, dev)
+            if (kT, heads, k_head) != (T, n_kv, 128):
+                raise RuntimeError(f"paged_qkv: k_out must be [{T}, {n_kv}, 128], the heads of a row contiguous")
+            k_ptr = k_out.data_ptr()
+        tab = cos.shape
+        if cos.dtype != torch.float32 or len(tab) != 2 or tab != sin.shape or sin.dtype != torch.float32 \
+                or not (cos.is_contiguous() and sin.is_contiguous()) or cos.get_device() != dev or sin.get_device() != dev:
+            raise RuntimeError("paged_qkv: cos and sin must be contiguous fp32 [max_pos, rotary dims / 2] tables")
+        if q_norm is not None or k_norm is not None:
+            for t in (q_norm, k_norm):
+                if t is None or t.dtype != torch.bfloat16 or t.shape != (128,) or t.get_device() != dev or t.stride(0) != 1:
+                    raise RuntimeError("paged_qkv: q_norm and k_norm must be bf16 [128], both or neither")
+            qn, kn = q_norm.data_ptr(), k_norm.data_ptr()
+        if T == 0 or B == 0:
+            return
+        st = self.lib.qk_paged_qkv(_QKV_ARGS.pack(*cache, qkv.data_ptr(), q_out.data_ptr(), k_ptr, qn, kn, cos.data_ptr(),
+                                                  sin.data_ptr(), T, n_q, qkv.stride(0), q_row, k_row, tab[0], tab[1],
+                                                  bool(interleaved), eps), _raw_stream(dev))
+        if st:
+            self._check(st, "paged_qkv")
+
+    def paged_kv_read(self, cu, block_table, k_pages, v_pages, k_out, v_out, k_scale=None, v_scale=None, starts=None):
+        """Positions starts[b] .. (0 without starts, int32 [B]) of each sequence out of the pages: row cu[b] + i of
+        k_out and v_out (bf16 [T, n_kv, 128], equal strides, any row and head stride: a contiguous cache's
+        [n_kv, max_seq, 128] transposed will do) is position starts[b] + i, dequantised."""
+        B, n_kv, dev, cache = self._paged("paged_kv_read", k_pages, v_pages, k_scale, v_scale, cu, None, block_table)
+        rows = self._heads("paged_kv_read", "k_out", k_out, dev)
+        if rows[1] != n_kv or self._heads("paged_kv_read", "v_out", v_out, dev) != rows:
+            raise RuntimeError(f"paged_kv_read: k_out and v_out must be [T, {n_kv}, 128] with equal strides")
+        first = 0
+        if starts is not None:
+            if starts.dtype != torch.int32 or starts.shape != (B,) or starts.get_device() != dev or not starts.is_contiguous():
+                raise RuntimeError(f"paged_kv_read: starts must be int32 [{B}] on the cache's device")
+            first = starts.data_ptr()
+        if rows[0] == 0 or B == 0:
+            return
+        st = self.lib.qk_paged_kv_read(_READ_ARGS.pack(*cache, first, k_out.data_ptr(), v_out.data_ptr(), rows[0], rows[2],
+                                                       rows[3]), _raw_stream(dev))
+        if st:
+            self._check(st, "paged_kv_read")
+
+    def paged_attention(self, q, cu, seq_lens, block_table, k_pages, v_pages, out, scale, max_q, k_scale=None,
+                        v_scale=None, workspace=None):
+        """Causal attention of each sequence's new tokens over its paged cache, their own rows included (`paged_qkv`
+        first): row cu[b] + i sees positions 0 .. seq_lens[b] - n_b + i of sequence b; a row that sees none gives zeros.
+        q and out: bf16 [T, n_q, 128] (or [T, n_q * 128]), 1 to 32 query heads per KV head; max_q: at least the most
+        new tokens of a sequence (1 for a decode step). Rows past cu[B] are left alone."""
+        B, n_kv, dev, cache = self._paged("paged_attention", k_pages, v_pages, k_scale, v_scale, cu, seq_lens, block_table)
+        T, n_q, q_row, q_head = self._heads("paged_attention", "q", q, dev)
+        oT, on, o_row, o_head = self._heads("paged_attention", "out", out, dev)
+        if oT != T or on != n_q:
+            raise RuntimeError(f"paged_attention: out must have q's shape, [{T}, {n_q}, 128]")
+        if T == 0 or B == 0:
+            return
+        stream = _raw_stream(dev)
+        ws = self._workspace("paged_attention", workspace, dev, stream)
+        st = self.lib.qk_paged_attention(_ATTENTION_ARGS.pack(*cache, q.data_ptr(), 0, 0, out.data_ptr(), ws.data_ptr(), T, n_q,
+                                                              max_q, q_row, q_head, 0, 0, o_row, o_head, len(ws), scale), stream)
+        if st:
+            self._check(st, "paged_attention")
+
+    def packed_attention(self, q, k, v, cu, out, scale, max_q, workspace=None):
+        """Causal attention of whole prompts packed without padding: prompt b is rows cu[b] .. cu[b+1]-1 (int32 [B+1]) of
+        q [T, n_q, 128], k and v [T, n_kv, 128] (bf16, any 16-byte-aligned row and head strides, k's equal to v's:
+        views of one qkv projection will do) and out; max_q: at least the longest prompt."""
+        dev = q.get_device()
+        T, n_q, q_row, q_head = self._heads("packed_attention", "q", q, dev)
+        kv = self._heads("packed_attention", "k", k, dev)
+        oT, on, o_row, o_head = self._heads("packed_attention", "out", out, dev)
+        if kv[0] != T or self._heads("packed_attention", "v", v, dev) != kv or oT != T or on != n_q:
+            raise RuntimeError("packed_attention: q, k, v and out must have the same rows, k and v equal shapes and strides, "
+                               "out q's shape")
+        if dev < 0 or cu.dtype != torch.int32 or cu.dim() != 1 or len(cu) < 1 or not cu.is_contiguous() or cu.get_device() != dev:
+            raise RuntimeError("packed_attention: cu must be int32 [B+1] on q's CUDA device")
+        B = len(cu) - 1
+        if T == 0 or B == 0:
+            return
+        stream = _raw_stream(dev)
+        ws = self._workspace("packed_attention", workspace, dev, stream)
+        st = self.lib.qk_packed_attention(
+            _ATTENTION_ARGS.pack(0, 0, 0, 0, cu.data_ptr(), 0, 0, B, kv[1], 0, 0, 0, 0, 0, q.data_ptr(), k.data_ptr(),
+                                 v.data_ptr(), out.data_ptr(), ws.data_ptr(), T, n_q, max_q, q_row, q_head, kv[2], kv[3], o_row,
+                                 o_head, len(ws), scale), stream)
+        if st:
+            self._check(st, "packed_attention")
 
     def finalize(self, best, token, out_tokens, state):
         b = token.numel()

@@ -219,6 +219,35 @@ def rope_tables(max_seq: int, head_dim: int, theta: float, device) -> tuple[torc
     return emb.cos().to(torch.bfloat16).contiguous(), emb.sin().to(torch.bfloat16).contiguous()
 
 
+def rope_angles(max_pos: int, rot_dim: int, theta: float, device, scaling: dict | None = None):
+    """fp32 cos and sin tables [max_pos, rot_dim / 2] of the paged path's rotary positions (`DecodeOps.paged_qkv`), the
+    first rot_dim dims of a head turning; angles in 64 bits (fp32 angles at 100k positions are off by 1e-2).
+    scaling, for contexts past the trained length:
+      {"type": "linear", "factor": f}: positions divided by f;
+      {"type": "yarn", "factor": f, "original_max_position": n, "beta_fast": 32, "beta_slow": 1, "attention_factor":
+      0.1 ln f + 1}: a frequency that turns more than beta_fast times over the n trained positions stays, one that
+      turns less than beta_slow times is divided by f, between them a ramp linear in the number of turns; cos and sin
+      times the attention factor (YaRN's interpolation by parts)."""
+    if rot_dim % 16 or not 16 <= rot_dim <= 128:
+        raise ValueError(f"rot_dim must be a multiple of 16 up to 128, got {rot_dim}")
+    inv = theta ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
+    mul = 1.0
+    if scaling is not None:
+        kind, f = scaling.get("type"), float(scaling.get("factor", 1.0))
+        if kind not in ("linear", "yarn") or not f >= 1.0:
+            raise ValueError(f"unsupported rope scaling {scaling!r}")
+        if kind == "linear":
+            inv = inv / f
+        else:
+            fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+            turns = scaling["original_max_position"] * inv / (2 * math.pi)
+            keep = ((turns - slow) / (fast - slow)).clamp(0, 1)
+            inv = inv * keep + inv / f * (1 - keep)
+            mul = float(scaling.get("attention_factor", 0.1 * math.log(f) + 1.0))
+    a = torch.arange(max_pos, device=device, dtype=torch.float64)[:, None] * inv.to(device)[None]
+    return (a.cos() * mul).float().contiguous(), (a.sin() * mul).float().contiguous()
+
+
 # ------------------------------------------------------------------------------------------------------------
 # Model container
 # ------------------------------------------------------------------------------------------------------------
