@@ -4,20 +4,9 @@
 //
 // One pass over the keys with a running maximum m and sum l in fp32; a row that sees no key gives zeros.
 #pragma once
-#include "paged.cuh"
+#include "attention_few.cuh"
 
 namespace qk {
-
-struct RaggedParams {
-  PagedCache c;         // pages, table, cu, seq_lens; packed prompts use cu alone
-  const bf16* q;        // row t, head h at q + t * q_row + h * q_head
-  const bf16* k;        // packed keys: row t, head g at k + t * kv_row + g * kv_head (null for a paged cache)
-  const bf16* v;
-  bf16* out;
-  long long q_row, q_head, kv_row, kv_head, out_row, out_head;
-  int T, n_q, group;
-  float scale;
-};
 
 // A warp per (row, query head): 32 keys a step, a key per lane for the scores, then 4 dims per lane for P.V.
 enum { SRC_PACKED = 0, SRC_PAGED = 1, SRC_PAGED_FP8 = 2 };

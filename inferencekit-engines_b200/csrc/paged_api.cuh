@@ -80,6 +80,48 @@ int launch_ragged(const RaggedParams& p, cudaStream_t stream) {
   return launch(ragged_attention_kernel<SRC>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream, p);
 }
 
+// TMA map of a page pool as [n_pages * n_kv * page_size] rows: box {128 bytes, box_rows}, 128-byte swizzle.
+int encode_pool_map(CUtensorMap* map, const void* pool, long long rows, bool fp8, int box_rows) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return fail(QK_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint64_t dims[2] = {HEAD_DIM, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)HEAD_DIM * (fp8 ? 1 : 2)};
+  const cuuint32_t box[2] = {fp8 ? 128u : 64u, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = enc(map, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(pool),
+                         dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(QK_EINVAL, "cuTensorMapEncodeTiled failed for a page pool (CUresult %d)", (int)r);
+  return QK_OK;
+}
+
+// The attention workspace: the few-row kernel's counters, its partial sums and their (m, l) pairs.
+constexpr int FEW_MAX_CTAS = 160;
+struct FewWorkspace {
+  int counters[256];
+  float ml[FEW_MAX_CTAS * 2 * 32 * 2];
+  float part[FEW_MAX_CTAS * 2 * 32 * HEAD_DIM];
+};
+
+template <bool FP8, int MT>
+int launch_few(const RaggedParams& r, int strict, void* workspace, cudaStream_t stream) {
+  FewParams p = {};
+  const int box = std::min(1 << r.c.page_shift, FEW_KEYS);
+  const long long rows = ((long long)r.c.n_pages * r.c.n_kv) << r.c.page_shift;
+  if (int e = encode_pool_map(&p.tm_k, r.c.k, rows, FP8, box)) return e;
+  if (int e = encode_pool_map(&p.tm_v, r.c.v, rows, FP8, box)) return e;
+  FewWorkspace* ws = static_cast<FewWorkspace*>(workspace);
+  p.r = r;
+  p.part = ws->part;
+  p.ml = ws->ml;
+  p.counters = ws->counters;
+  p.strict = strict;
+  auto k = few_attention_kernel<FP8, MT>;
+  const int smem = (int)sizeof(FewSmem<FP8>);
+  if (int e = ensure_smem((const void*)k, smem)) return e;
+  return launch(k, dim3(std::min(device_sms(), FEW_MAX_CTAS)), dim3(MT == 1 ? 288 : 160), smem, stream, p);
+}
+
 }  // namespace
 
 extern "C" {
@@ -148,7 +190,7 @@ int qk_paged_kv_read(const qk_paged_kv_read_t* args, qk_stream_t stream) {
                 static_cast<cudaStream_t>(stream), p);
 }
 
-long long qk_ragged_attention_workspace_bytes(void) { return 256; }
+long long qk_ragged_attention_workspace_bytes(void) { return sizeof(FewWorkspace); }
 
 int qk_paged_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
   if (!args) return fail(QK_EINVAL, "null pointer argument");
@@ -156,8 +198,12 @@ int qk_paged_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
   if (int r = ragged_common(&p, *args)) return r;
   if (int r = paged_cache(&p.c, args->cache, true)) return r;
   if (p.T == 0 || p.c.B == 0) return QK_OK;
-  return args->cache.kv_fp8 ? launch_ragged<SRC_PAGED_FP8>(p, static_cast<cudaStream_t>(stream))
-                            : launch_ragged<SRC_PAGED>(p, static_cast<cudaStream_t>(stream));
+  const bool fp8 = args->cache.kv_fp8 != 0;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const long long rows = args->max_q * p.group;
+  if (rows <= 16) return fp8 ? launch_few<true, 1>(p, 1, args->workspace, st) : launch_few<false, 1>(p, 1, args->workspace, st);
+  if (rows <= 32) return fp8 ? launch_few<true, 2>(p, 1, args->workspace, st) : launch_few<false, 2>(p, 1, args->workspace, st);
+  return fp8 ? launch_ragged<SRC_PAGED_FP8>(p, st) : launch_ragged<SRC_PAGED>(p, st);
 }
 
 int qk_packed_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
