@@ -211,10 +211,8 @@ __global__ void __launch_bounds__(MT == 1 ? 288 : 160, 1) few_attention_kernel(c
       for (int t = t0; t < t1; ++t, ++it) {
         const int st = it % S, page = next;
         if (t + 1 < t1) next = page_of(t + 1);
-        if (it >= S && !mbar_wait(&sm.empty[st], (uint32_t)((it / S - 1) & 1))) {
-          ok = false;
-          break;
-        }
+        if (it >= S) ok = __all_sync(0xffffffffu, mbar_wait(&sm.empty[st], (uint32_t)((it / S - 1) & 1)));
+        if (!ok) break;
         const int nb = __popc(__ballot_sync(0xffffffffu, page >= 0));
         if (lane == 0) mbar_arrive_expect_tx(&sm.full[st], (uint32_t)(nb * RB) * (2 * bytes_row + (FP8 ? 8 : 0)));
         __syncwarp();

@@ -4,12 +4,11 @@
 //
 // One pass over the keys with a running maximum m and sum l in fp32; a row that sees no key gives zeros.
 #pragma once
-#include "attention_few.cuh"
+#include "attention_tc.cuh"
 
 namespace qk {
 
 // A warp per (row, query head): 32 keys a step, a key per lane for the scores, then 4 dims per lane for P.V.
-enum { SRC_PACKED = 0, SRC_PAGED = 1, SRC_PAGED_FP8 = 2 };
 template <int SRC>
 __global__ void __launch_bounds__(256) ragged_attention_kernel(const __grid_constant__ RaggedParams p) {
   __shared__ float qs[8][HEAD_DIM];

@@ -1,0 +1,622 @@
+// Causal attention on the 5th-generation tensor cores: whole packed prompts, and chunks of new tokens over a paged cache.
+//
+//   out[t][h] = sum over j <= pos(t) of softmax_j(scale * q[t][h] . K[g][j]) V[g][j],   g = h / (n_q / n_kv)
+//
+// Bound by the tensor cores: 2 x 128 x 128 x 128 multiply-adds per (128 query rows, 128 keys), and beside them 128 x 128
+// exponentials, whose unit is as long at it as the two products are at the matrix units.
+//  * The query rows of a KV head are its tokens times its heads, token-major: a tile of 128 rows is 128 / group tokens,
+//    so grouped heads share every K and V tile that is loaded. A CTA (one per SM) works on two such tiles at a time,
+//    whose softmax warps take turns with the matrix unit.
+//  * One pass over the keys in tiles of 128. S = Q K^T (operands in shared memory, accumulator in TMEM); a softmax
+//    thread owns one row: it reads its 128 scores with tcgen05.ld, keeps the running maximum m and sum l, writes
+//    P = exp2(S - m) as bf16 over S in TMEM; O += P V reads P from TMEM and V from shared memory (dims contiguous:
+//    the MN-major operand). P's rounding to bf16 is what the matrix unit takes; l sums the fp32 values.
+//  * O stays in TMEM. Its rows are multiplied by exp2(m_old - m_new) only when a maximum grew by more than 2^8 in
+//    weight: until then the old m serves (P at most 2^8), which changes no result and makes the rescale rare.
+//  * Warps: 0-3 and 4-7 the softmax of the two tiles, 8 the loads (TMA, 128-byte swizzle, a ring of five 32 KB K and V
+//    tiles), 9 issues the MMAs (10 and 11 fill their warpgroup, which gives its registers to the softmax): Q0 K0, Q1 K0, then per tile P0 V, Q0 K', P1 V, Q1 K', so that while one tile's softmax
+//    runs, the matrix unit has the other's two products to do.
+//  * Work: (sequence, KV head, tile pair, key tile) in that order, dealt in equal contiguous ranges to the CTAs: causal
+//    rows and ragged lengths balance by themselves, and a few rows over a long context spread over every SM. A boundary
+//    nearer than TC_MIN_PIECE tiles to the end of a unit moves there. Units cut by one leave fp32 partials (O, m, l) per
+//    piece; the CTA that completes the unit's count adds them in order.
+#pragma once
+#include "attention_few.cuh"
+
+namespace qk {
+
+constexpr int TCA_KEYS = 128;             // keys of a tile
+constexpr int TCA_TILE = TCA_KEYS * HEAD_DIM * 2;   // 32 KB: two 64-dim halves of 128 rows x 128 B
+constexpr int TCA_STAGES = 5;
+constexpr int TCA_MIN_PIECE = 4;          // tiles
+constexpr float TCA_LAZY = 8.f;           // log2 of the growth a stale maximum may hide
+
+enum { SRC_PACKED = 0, SRC_PAGED = 1, SRC_PAGED_FP8 = 2 };
+
+struct TcAttnParams {
+  CUtensorMap tm_q;         // {128 dims, n_q heads, T rows}: box {64, group, 128 / group}
+  CUtensorMap tm_k, tm_v;   // packed: {128 dims, n_kv, T}, box {64, 1, 128}; paged: the pool's rows, box {64, min(page, 128)}
+  RaggedParams r;
+  float* part;              // [grid][2][2 tiles][32 column quads][128 rows][4]
+  float* ml;                // [grid][2][2 tiles][128 rows][2]
+  int* counters;            // [grid], zero between launches
+  int min_rows;             // sequences with fewer query rows per KV head are another kernel's
+};
+
+struct TcSeq {
+  int row0, n, len;         // token rows, keys (n 0: nothing to do here)
+};
+template <int SRC>
+__device__ __forceinline__ TcSeq tc_seq(const TcAttnParams& p, int b) {
+  const RaggedParams& r = p.r;
+  TcSeq s;
+  s.row0 = __ldg(r.c.cu + b);
+  s.n = __ldg(r.c.cu + b + 1) - s.row0;
+  s.len = s.n;
+  if (SRC != SRC_PACKED) {
+    s.len = __ldg(r.c.seq_lens + b);
+    const int cap = r.c.table_width << r.c.page_shift;
+    if (s.len > cap) {
+      atomicOr(&g_dev_error, DEVERR_BAD_STATE);
+      s.len = cap;
+    }
+    s.len = max(s.len, 0);
+  }
+  const bool bad = s.row0 < 0 || s.n < 0 || s.n > r.T - s.row0;
+  if (bad) atomicOr(&g_dev_error, DEVERR_BAD_STATE);
+  if (bad || s.n * r.group < p.min_rows) s.n = 0;
+  return s;
+}
+// sum over i < n of floor((a i + b) / 128), a and b not negative
+__host__ __device__ __forceinline__ long long floor_sum(unsigned n, unsigned a, unsigned b) {
+  long long sum = 0;
+  unsigned m = TCA_KEYS;
+  while (n) {
+    sum += (long long)n * (n - 1) / 2 * (a / m) + (long long)n * (b / m);
+    a %= m;
+    b %= m;
+    const unsigned long long y = (unsigned long long)a * n + b;
+    if (y < m) break;
+    n = (unsigned)(y / m);
+    b = (unsigned)(y % m);
+    const unsigned t = m;
+    m = a;
+    a = t;
+  }
+  return sum;
+}
+// Key tiles of a sequence's tile pairs: pair i covers tokens [i step, (i + 1) step) and the keys its last token sees;
+// a pair that sees none still has rows to set to zero, and counts one.
+struct TcPairs {
+  int n, step, a, len;      // pairs; tokens of a pair; keys before the first token; keys
+  __host__ __device__ __forceinline__ TcPairs(const TcSeq& s, int step_) : n((s.n + step_ - 1) / step_), step(step_), a(s.len - s.n), len(s.len) {}
+  __host__ __device__ __forceinline__ int tiles(int i) const {
+    const int x = i == n - 1 ? len : a + (i + 1) * step;
+    return max(1, (x + TCA_KEYS - 1) / TCA_KEYS);
+  }
+  __host__ __device__ __forceinline__ long long before(int i) const {   // tiles of the pairs 0 .. i - 1
+    const int q = min(i, n - 1), z = a < 0 ? min(q, -a / step) : 0;
+    return q <= 0 && i < n ? 0 : z + floor_sum(q - z, step, a + (z + 1) * step + TCA_KEYS - 1) + (i == n ? tiles(n - 1) : 0);
+  }
+};
+
+struct TcAttnSmem {
+  uint8_t q[2][TCA_TILE];
+  uint8_t kv[TCA_STAGES][TCA_TILE];
+  long long total;
+  struct Place {            // where a range begins
+    int b, g, pair, t;
+    long long u;
+  } at[2];
+  uint64_t q_full, q_empty, full[TCA_STAGES], empty[TCA_STAGES];
+  uint64_t s_full[2], p_full[2], o_full[2];
+  uint32_t tmem;
+  int last;
+};
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+// D fp32, A and B bf16, M = N = 128; b_mn: B is stored with N contiguous
+__host__ __device__ constexpr uint32_t tca_idesc(bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn ? 1u : 0u) << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+}
+// V [128 keys][128 dims]: 64-dim halves TCA_TILE / 2 apart, groups of 8 keys 1024 bytes apart
+__device__ __forceinline__ uint64_t tca_desc_mn(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)((TCA_TILE / 2) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+         ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void tca_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accum), "r"(0)
+      : "memory");
+}
+__device__ __forceinline__ void tca_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accum), "r"(0)
+      : "memory");
+}
+#define QK_R32(r, o)                                                                                                     \
+  r[o], r[o + 1], r[o + 2], r[o + 3], r[o + 4], r[o + 5], r[o + 6], r[o + 7], r[o + 8], r[o + 9], r[o + 10], r[o + 11],  \
+      r[o + 12], r[o + 13], r[o + 14], r[o + 15], r[o + 16], r[o + 17], r[o + 18], r[o + 19], r[o + 20], r[o + 21],      \
+      r[o + 22], r[o + 23], r[o + 24], r[o + 25], r[o + 26], r[o + 27], r[o + 28], r[o + 29], r[o + 30], r[o + 31]
+// 32 consecutive 32-bit columns of this warp's 32 TMEM lanes, one lane a thread
+__device__ __forceinline__ void tca_ld32(uint32_t taddr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+        "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
+        "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+        "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tca_st32(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+      "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+      "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]),
+      "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tca_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A CTA's walk over its pieces; every role walks the same one.
+template <int SRC>
+struct TcWalk {
+  const TcAttnParams& p;
+  int b, g, pair, t0, step;
+  TcSeq s;
+  TcPairs pr;
+  long long u, u1;
+  int n, t1;                // the unit's key tiles; the piece is [t0, t1)
+  __device__ __forceinline__ TcWalk(const TcAttnParams& p_, const TcAttnSmem& sm, int step_)
+      : p(p_), b(sm.at[0].b), g(sm.at[0].g), pair(sm.at[0].pair), t0(sm.at[0].t), step(step_), s(tc_seq<SRC>(p_, sm.at[0].b)), pr(s, step_),
+        u(sm.at[0].u), u1(sm.at[1].u) {
+    piece();
+  }
+  __device__ __forceinline__ void piece() {
+    n = pr.tiles(pair);
+    t1 = (int)min((long long)n, t0 + (u1 - u));
+  }
+  __device__ __forceinline__ bool more() const { return u < u1; }
+  __device__ __forceinline__ void next() {
+    u += t1 - t0;
+    t0 = 0;
+    if (u >= u1) return;
+    if (++pair == pr.n) {
+      pair = 0;
+      if (++g == p.r.c.n_kv) {
+        g = 0;
+        do s = tc_seq<SRC>(p, ++b);
+        while (s.n == 0);
+        pr = TcPairs(s, step);
+      }
+    }
+    piece();
+  }
+  // of tile x of the pair: its first token, whether it has any, and its key tiles in this piece
+  __device__ __forceinline__ int tok0(int x) const { return pair * step + x * (step / 2); }
+  __device__ __forceinline__ int end(int x) const {
+    if (tok0(x) >= s.n) return t0;
+    const int keys = min(s.len, s.len - s.n + min(tok0(x) + step / 2, s.n));
+    return max(t0, min(t1, max(1, (keys + TCA_KEYS - 1) / TCA_KEYS)));
+  }
+};
+
+constexpr int TCA_THREADS = 384;
+// Registers a thread, out of 384 x 168 at launch: 256 x 208 + 128 x 88
+constexpr int TCA_REGS_SOFTMAX = 208, TCA_REGS_OTHER = 88;
+static_assert(256 * TCA_REGS_SOFTMAX + 128 * TCA_REGS_OTHER <= TCA_THREADS * 168, "setmaxnreg would wait for ever");
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+template <int SRC>
+__global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __grid_constant__ TcAttnParams p) {
+  extern __shared__ __align__(1024) uint8_t tca_smem[];
+  TcAttnSmem& sm = *reinterpret_cast<TcAttnSmem*>(tca_smem);
+  const RaggedParams& r = p.r;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x, n_kv = r.c.n_kv;
+  const int step = 2 * (128 / r.group);   // tokens of a tile pair
+  if (tid == 0) {
+    mbar_init(&sm.q_full, 1);
+    mbar_init(&sm.q_empty, 1);
+    for (int i = 0; i < TCA_STAGES; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&sm.s_full[x], 1);
+      mbar_init(&sm.p_full[x], 4);
+      mbar_init(&sm.o_full[x], 1);
+    }
+    fence_mbar_init();
+  }
+  grid_dep_wait();
+  grid_dep_launch();
+
+  // ---- this CTA's range of key tiles (warp 0: sums over the sequences, 32 chunks of them) --------------------------
+  if (warp == 0) {
+    const int per = (r.c.B + 31) / 32;
+    long long mine = 0;
+    for (int b = lane * per; b < min(r.c.B, (lane + 1) * per); ++b) {
+      const TcPairs pr(tc_seq<SRC>(p, b), step);
+      if (pr.n) mine += pr.before(pr.n) * n_kv;
+    }
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const long long W = __shfl_sync(0xffffffffu, incl, 31);
+    const int G = (int)min((long long)gridDim.x, max(1ll, W / TCA_MIN_PIECE));
+    for (int e = 0; e < 2; ++e) {           // both ends of the range
+      const int cc = min(c + e, G);
+      const long long u = cc * W / G;
+      int b = r.c.B, g = 0, pair = 0, t = 0;
+      long long at = W;
+      if (u < W) {
+        const unsigned who = __ballot_sync(0xffffffffu, incl > u);
+        const int first = __ffs(who) - 1;
+        at = __shfl_sync(0xffffffffu, incl - mine, first);
+        b = first * per;
+        TcPairs pr(tc_seq<SRC>(p, b), step);
+        long long tot = pr.n ? pr.before(pr.n) : 0;
+        while (u >= at + tot * n_kv) {
+          at += tot * n_kv;
+          pr = TcPairs(tc_seq<SRC>(p, ++b), step);
+          tot = pr.n ? pr.before(pr.n) : 0;
+        }
+        g = (int)((u - at) / tot);
+        at += g * tot;
+        int lo = 0, hi = pr.n;              // the pair: before(lo) <= u - at < before(hi)
+        while (hi - lo > 1) {
+          const int d = (hi - lo + 31) / 32, i = lo + (lane + 1) * d;
+          const bool le = i < hi && pr.before(i) <= u - at;
+          const int k = __popc(__ballot_sync(0xffffffffu, le));
+          lo += k * d;
+          hi = min(hi, lo + d);
+        }
+        pair = lo;
+        at += pr.before(pair);
+        t = (int)(u - at);
+        const int n = pr.tiles(pair);
+        if (t < TCA_MIN_PIECE) t = 0;
+        else if (n - t < TCA_MIN_PIECE) {   // the range begins with the next unit
+          at += n;
+          t = 0;
+          if (++pair == pr.n) {
+            pair = 0;
+            if (++g == n_kv) {
+              g = 0;
+              do ++b;
+              while (b < r.c.B && tc_seq<SRC>(p, b).n == 0);
+            }
+          }
+        }
+      }
+      if (lane == 0) sm.at[e] = {b, g, pair, t, at + t};
+    }
+    if (lane == 0) sm.total = W;
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+  const long long W = sm.total;
+  const bool work = sm.at[0].u < sm.at[1].u;
+  // TMEM columns: S (and P) of the tiles at 0 and 128, O at 256 and 384
+
+  // the register split stands inside the roles' branches: after a join the compiler would have to take the smaller share
+  if (warp >= 8) {
+  regs_dec<TCA_REGS_OTHER>();
+  if (work && warp == 8) {   // ---- loads ----
+    TcWalk<SRC> w(p, sm, step);
+    const int RB = SRC == SRC_PACKED ? TCA_KEYS : min(1 << r.c.page_shift, TCA_KEYS);
+    const uint32_t q_bytes = (uint32_t)(step / 2) * r.group * HEAD_DIM * 2;
+    int it = 0;
+    bool ok = true;
+    for (int unit = 0; w.more() && ok; w.next(), ++unit) {
+      if (unit) ok = __all_sync(0xffffffffu, mbar_wait(&sm.q_empty, (uint32_t)((unit - 1) & 1)));
+      if (!ok) break;
+      const bool two = w.tok0(1) < w.s.n;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&sm.q_full, two ? 2 * q_bytes : q_bytes);
+        for (int x = 0; x < (two ? 2 : 1); ++x)
+          for (int h = 0; h < 2; ++h)
+            tma_load_3d(sm.q[x] + h * (TCA_TILE / 2), &p.tm_q, 64 * h, w.g * r.group, w.s.row0 + w.tok0(x), &sm.q_full);
+      }
+      auto page_of = [&](int t) {           // this lane's box of tile t: its page, -1 where it holds no key
+        const int j = t * TCA_KEYS + lane * RB;
+        if (lane * RB >= TCA_KEYS || j >= w.s.len) return -1;
+        int pg = __ldg(r.c.table + (size_t)w.b * r.c.table_stride + (j >> r.c.page_shift));
+        if (pg < 0 || pg >= r.c.n_pages) {
+          atomicOr(&g_dev_error, DEVERR_BAD_STATE);
+          pg = 0;
+        }
+        return pg;
+      };
+      int next = SRC == SRC_PACKED ? 0 : page_of(w.t0);
+      for (int t = w.t0; t < w.t1 && ok; ++t) {
+        const int page = next;
+        if (SRC != SRC_PACKED && t + 1 < w.t1) next = page_of(t + 1);
+        for (int v = 0; v < 2; ++v, ++it) {   // K, then V
+          const int st = it % TCA_STAGES;
+          if (it >= TCA_STAGES) ok = __all_sync(0xffffffffu, mbar_wait(&sm.empty[st], (uint32_t)((it / TCA_STAGES - 1) & 1)));
+          if (!ok) break;
+          const CUtensorMap* tm = v ? &p.tm_v : &p.tm_k;
+          if (SRC == SRC_PACKED) {
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&sm.full[st], TCA_TILE);
+              for (int h = 0; h < 2; ++h) tma_load_3d(sm.kv[st] + h * (TCA_TILE / 2), tm, 64 * h, w.g, w.s.row0 + t * TCA_KEYS, &sm.full[st]);
+            }
+          } else {
+            const int nb = __popc(__ballot_sync(0xffffffffu, page >= 0));
+            if (lane == 0) mbar_arrive_expect_tx(&sm.full[st], (uint32_t)(nb * RB) * (2 * HEAD_DIM));
+            __syncwarp();
+            if (page >= 0) {
+              const int row = ((page * n_kv + w.g) << r.c.page_shift) + ((t * TCA_KEYS + lane * RB) & ((1 << r.c.page_shift) - 1));
+              for (int h = 0; h < 2; ++h) tma_load_2d(sm.kv[st] + h * (TCA_TILE / 2) + lane * RB * 128, tm, 64 * h, row, &sm.full[st]);
+            }
+          }
+        }
+      }
+    }
+    if (!ok)   // a wait gave up: let the copies in flight land before the shared memory goes away
+      for (int i = max(0, it - TCA_STAGES); i < it; ++i) mbar_wait(&sm.full[i % TCA_STAGES], (uint32_t)((i / TCA_STAGES) & 1), 1000000ull);
+  } else if (work && warp == 9) {   // ---- MMA issue ----
+    constexpr uint32_t id_s = tca_idesc(false), id_o = tca_idesc(true);
+    TcWalk<SRC> w(p, sm, step);
+    int it = 0, np[2] = {0, 0};
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(bar, parity));
+      tc_fence_after();
+    };
+    auto scores = [&](int x, int st) {      // S of tile x = Q K^T
+      if (lane == 0) {
+        const uint32_t qa = smem_u32(sm.q[x]), ka = smem_u32(sm.kv[st]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t off = (k >> 2) * (TCA_TILE / 2) + (k & 3) * 32;
+          tca_mma_ss(tmem + 128 * x, tc_desc_sw128(qa + off), tc_desc_sw128(ka + off), id_s, k > 0);
+        }
+        tc_commit(&sm.s_full[x]);
+      }
+    };
+    for (int unit = 0; w.more() && ok; w.next(), ++unit) {
+      const int e[2] = {w.end(0), w.end(1)}, cnt = w.t1 - w.t0;
+      wait(&sm.q_full, (uint32_t)(unit & 1));
+      wait(&sm.full[it % TCA_STAGES], (uint32_t)((it / TCA_STAGES) & 1));
+      if (!ok) break;
+      for (int x = 0; x < 2; ++x)
+        if (w.t0 < e[x]) scores(x, it % TCA_STAGES);
+      if (lane == 0) {
+        tc_commit(&sm.empty[it % TCA_STAGES]);
+        if (cnt == 1) tc_commit(&sm.q_empty);
+      }
+      for (int t = w.t0; t < w.t1 && ok; ++t) {
+        const int vs = (it + 1) % TCA_STAGES, ks = (it + 2) % TCA_STAGES;
+        wait(&sm.full[vs], (uint32_t)(((it + 1) / TCA_STAGES) & 1));
+        if (!ok) break;
+        const int tail = w.s.len - t * TCA_KEYS;
+        if (tail < TCA_KEYS) {              // rows past the sequence: another's, or nothing; 0 x NaN must not reach O
+          const uint32_t va = smem_u32(sm.kv[vs]);
+          for (int i = max(tail, 0) * 16 + lane; i < TCA_KEYS * 16; i += 32)
+            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(va + ((i >> 3) & 1) * (TCA_TILE / 2) + (i >> 4) * 128 + (i & 7) * 16), "r"(0) : "memory");
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        for (int x = 0; x < 2 && ok; ++x) {
+          if (t < e[x]) {
+            wait(&sm.p_full[x], (uint32_t)(np[x]++ & 1));
+            if (!ok) break;
+            if (lane == 0) {
+              const uint32_t va = smem_u32(sm.kv[vs]);
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                tca_mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * k, tca_desc_mn(va + k * 2048), id_o, k > 0 || t > w.t0);
+              if (t + 1 == e[x]) tc_commit(&sm.o_full[x]);
+            }
+          }
+          if (t + 1 < e[x]) {
+            wait(&sm.full[ks], (uint32_t)(((it + 2) / TCA_STAGES) & 1));
+            if (!ok) break;
+            scores(x, ks);
+          }
+        }
+        if (!ok) break;
+        if (t + 1 < w.t1) wait(&sm.full[ks], (uint32_t)(((it + 2) / TCA_STAGES) & 1));   // loaded even where no tile reads it
+        if (lane == 0) {
+          tc_commit(&sm.empty[vs]);
+          if (t + 1 < w.t1) tc_commit(&sm.empty[ks]);
+          if (t + 2 == w.t1) tc_commit(&sm.q_empty);
+        }
+        it += 2;
+      }
+    }
+  }
+  } else {
+  regs_inc<TCA_REGS_SOFTMAX>();
+  if (work) {   // ---- softmax: thread = one row of tile x ----
+    const int x = warp >> 2, row = tid & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lanes + 128 * x, to = tmem + lanes + 256 + 128 * x;
+    const float sl2 = r.scale * LOG2E;
+    TcWalk<SRC> w(p, sm, step);
+    int ns = 0, no = 0;
+    bool ok = true;
+    for (; w.more(); w.next()) {
+      const int e = w.end(x), tok = w.tok0(x) + row / r.group, pos = w.s.len - w.s.n + tok;
+      const bool valid = row < (step / 2) * r.group && tok < w.s.n;
+      const int first = w.s.len - w.s.n + w.tok0(x);   // the last key that the tile's first row sees
+      float m = -INFINITY, l = 0.f;
+      for (int t = w.t0; t < e; ++t) {
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(&sm.s_full[x], (uint32_t)(ns++ & 1)));
+        tc_fence_after();
+        uint32_t v[128];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tca_ld32(ts + 32 * i, v + 32 * i);
+        tc_wait_ld();
+        if (t * TCA_KEYS + TCA_KEYS - 1 > first) {
+          const int lim = min(pos, w.s.len - 1) - t * TCA_KEYS;
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (i > lim) v[i] = 0xff800000u;   // -inf
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[i]));
+        const float mn = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), m);
+        // a row's first maximum, or one that grew by more than TCA_LAZY
+        const bool grow = m == -INFINITY ? mn != -INFINITY : (mn - m) * sl2 > TCA_LAZY;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float f = m == -INFINITY ? 0.f : ex2((m - mn) * sl2);
+          m = mn;
+          l *= f;
+          if (t > w.t0) {                   // the products before this tile's scores are done: O is whole
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t o[32];
+              tca_ld32(to + 32 * i, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tca_st32(to + 32 * i, o);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m * sl2;
+        float sum[4] = {};
+#pragma unroll
+        for (int i = 0; i < 128; i += 2) {
+          const float a = ex2(fmaf(__uint_as_float(v[i]), sl2, -base)), b = ex2(fmaf(__uint_as_float(v[i + 1]), sl2, -base));
+          sum[i & 2] += a;
+          sum[(i & 2) + 1] += b;
+          v[i / 2] = pack_bf16(a, b);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tca_st32(ts, v);
+        tca_st32(ts + 32, v + 32);
+        tca_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full[x]);
+      }
+
+      // ---- the piece's end: the output rows, or a partial --------------------------------------------------------
+      const bool any = e > w.t0;
+      if (any) {
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(&sm.o_full[x], (uint32_t)(no++ & 1)));
+        tc_fence_after();
+      }
+      bf16* dst = r.out + (long long)(w.s.row0 + tok) * r.out_row + (long long)(w.g * r.group + row % r.group) * r.out_head;
+      auto store = [&](const float* o, float inv, int col) {   // 32 columns
+#pragma unroll
+        for (int k = 0; k < 32; k += 8) {
+          float y[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = o[k + i] * inv;
+          *reinterpret_cast<uint4*>(dst + col + k) = pack_bf16x8(y);
+        }
+      };
+      if (w.t0 == 0 && w.t1 == w.n) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (any) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t o[32];
+            tca_ld32(to + 32 * i, o);
+            tc_wait_ld();
+            if (valid) store(reinterpret_cast<const float*>(o), inv, 32 * i);
+            __syncwarp();
+          }
+        }
+        continue;
+      }
+      // boundaries inside the unit: c_lo .. c_hi; its first piece is CTA c_lo - 1's last (slot 1), piece i > 0 is CTA
+      // c_lo + i - 1's first (slot 0)
+      const long long a0 = w.u - w.t0;
+      const int G = (int)min((long long)gridDim.x, max(1ll, W / TCA_MIN_PIECE));
+      const int c_lo = (int)(((a0 + TCA_MIN_PIECE) * G + W - 1) / W), c_hi = (int)(((a0 + w.n - TCA_MIN_PIECE + 1) * G + W - 1) / W) - 1;
+      const size_t slot = ((size_t)(c * 2 + (w.t0 == 0 ? 1 : 0)) * 2 + x) * 128;
+      *reinterpret_cast<float2*>(p.ml + (slot + row) * 2) = make_float2(m, l);
+      if (any) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t o[32];
+          tca_ld32(to + 32 * i, o);
+          tc_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 32; k += 4)
+            *reinterpret_cast<uint4*>(p.part + slot * 128 + (size_t)(8 * i + k / 4) * 512 + row * 4) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+        }
+      }
+      __threadfence();
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (tid == 0) {
+        const int before = atomicAdd(p.counters + c_lo - 1, 1);
+        sm.last = before == c_hi - c_lo + 1;
+        if (sm.last) {
+          __threadfence();
+          p.counters[c_lo - 1] = 0;
+        }
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      const bool last = sm.last;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (last && valid) {
+      float M = -INFINITY, L = 0.f;
+      auto slot_of = [&](int cc) { return ((size_t)(cc * 2 + (cc == c_lo - 1 ? 1 : 0)) * 2 + x) * 128; };
+      for (int cc = c_lo - 1; cc <= c_hi; ++cc) M = fmaxf(M, __ldcg(p.ml + (slot_of(cc) + row) * 2));
+#pragma unroll 1
+      for (int col = 0; col < 128; col += 32) {
+        float o[32] = {};
+        L = 0.f;
+        for (int cc = c_lo - 1; cc <= c_hi; ++cc) {
+          const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ml + (slot_of(cc) + row) * 2));
+          if (ml.y == 0.f) continue;        // no key of the piece was visible (and its O may not have been written)
+          const float f = M == -INFINITY ? 1.f : ex2((ml.x - M) * sl2);
+          L += ml.y * f;
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) {
+            const float4 q = __ldcg(reinterpret_cast<const float4*>(p.part + slot_of(cc) * 128 + (size_t)((col + k) / 4) * 512 + row * 4));
+            o[k] += q.x * f, o[k + 1] += q.y * f, o[k + 2] += q.z * f, o[k + 3] += q.w * f;
+          }
+        }
+        store(o, L == 0.f ? 0.f : 1.f / L, col);
+      }
+      }
+      __syncwarp();
+    }
+    if (!ok && lane == 0) atomicOr(&g_dev_error, DEVERR_MBAR_TIMEOUT);
+  }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+}  // namespace qk

@@ -19,7 +19,7 @@ int paged_cache(PagedCache* c, const qk_paged_cache_t& a, bool lens) {
     return fail(QK_EINVAL, "n_pages=%lld n_kv=%lld batch=%lld", a.n_pages, a.n_kv, a.batch);
   // rows are counted in 32 bits (bytes are not)
   if (a.n_pages > 0x7fffffffll / (a.n_kv * a.page_size)) return fail(QK_EINVAL, "a pool of more than 2^31 - 1 rows");
-  if (a.table_width < 1 || a.table_stride < a.table_width || a.table_stride > 0x7fffffffll || a.table_width > 0x7fffffffll / a.page_size)
+  if (a.table_width < 1 || a.table_stride < a.table_width || a.table_stride > 0x7fffffffll || a.table_width > 0x3fffffffll / a.page_size)
     return fail(QK_EINVAL, "table_width=%lld table_stride=%lld", a.table_width, a.table_stride);
   if (!aligned(a.k_pages, 16) || !aligned(a.v_pages, 16) || !aligned(a.k_scale, 16) || !aligned(a.v_scale, 16))
     return fail(QK_EINVAL, "pages and scales must be 16-byte aligned");
@@ -56,8 +56,9 @@ int ragged_common(RaggedParams* p, const qk_ragged_attention_t& a) {
     return fail(QK_EINVAL, "workspace of %lld bytes: %lld needed, 256-byte aligned", a.workspace_bytes, qk_ragged_attention_workspace_bytes());
   p->q = static_cast<const bf16*>(a.q);
   p->out = static_cast<bf16*>(a.out);
-  p->q_row = a.q_row;
-  p->q_head = a.q_head;
+  // a dimension of one has no stride of its own
+  p->q_row = a.rows == 1 ? a.n_q * HEAD_DIM : a.q_row;
+  p->q_head = a.n_q == 1 ? HEAD_DIM : a.q_head;
   p->out_row = a.out_row;
   p->out_head = a.out_head;
   p->T = (int)a.rows;
@@ -65,19 +66,6 @@ int ragged_common(RaggedParams* p, const qk_ragged_attention_t& a) {
   p->group = (int)(a.n_q / n_kv);
   p->scale = scale;
   return QK_OK;
-}
-
-int half_warp_grid(long long rows, long long heads, dim3* grid) {   // a warp per row and pair of heads, 8 warps a CTA
-  const long long n = (rows * ((heads + 1) / 2) + 7) / 8;
-  if (n > 0x7fffffff / 8) return fail(QK_EINVAL, "%lld rows are too many", rows);
-  *grid = dim3((unsigned)n);
-  return QK_OK;
-}
-
-template <int SRC>
-int launch_ragged(const RaggedParams& p, cudaStream_t stream) {
-  const long long warps = (long long)p.T * p.n_q;
-  return launch(ragged_attention_kernel<SRC>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream, p);
 }
 
 // TMA map of a page pool as [n_pages * n_kv * page_size] rows: box {128 bytes, box_rows}, 128-byte swizzle.
@@ -95,12 +83,13 @@ int encode_pool_map(CUtensorMap* map, const void* pool, long long rows, bool fp8
   return QK_OK;
 }
 
-// The attention workspace: the few-row kernel's counters, its partial sums and their (m, l) pairs.
-constexpr int FEW_MAX_CTAS = 160;
-struct FewWorkspace {
-  int counters[256];
-  float ml[FEW_MAX_CTAS * 2 * 32 * 2];
-  float part[FEW_MAX_CTAS * 2 * 32 * HEAD_DIM];
+// The attention workspace: each kernel's counters, then partial sums and their (m, l) pairs, two a CTA, which the two
+// kernels of a call use one after the other.
+constexpr int RAGGED_MAX_CTAS = 160;
+struct RaggedWorkspace {
+  int few_counters[256], tc_counters[256];
+  float ml[RAGGED_MAX_CTAS * 2 * 256 * 2];
+  float part[RAGGED_MAX_CTAS * 2 * 256 * HEAD_DIM];
 };
 
 template <bool FP8, int MT>
@@ -110,16 +99,71 @@ int launch_few(const RaggedParams& r, int strict, void* workspace, cudaStream_t 
   const long long rows = ((long long)r.c.n_pages * r.c.n_kv) << r.c.page_shift;
   if (int e = encode_pool_map(&p.tm_k, r.c.k, rows, FP8, box)) return e;
   if (int e = encode_pool_map(&p.tm_v, r.c.v, rows, FP8, box)) return e;
-  FewWorkspace* ws = static_cast<FewWorkspace*>(workspace);
+  RaggedWorkspace* ws = static_cast<RaggedWorkspace*>(workspace);
   p.r = r;
   p.part = ws->part;
   p.ml = ws->ml;
-  p.counters = ws->counters;
+  p.counters = ws->few_counters;
   p.strict = strict;
   auto k = few_attention_kernel<FP8, MT>;
   const int smem = (int)sizeof(FewSmem<FP8>);
   if (int e = ensure_smem((const void*)k, smem)) return e;
-  return launch(k, dim3(std::min(device_sms(), FEW_MAX_CTAS)), dim3(MT == 1 ? 288 : 160), smem, stream, p);
+  return launch(k, dim3(std::min(device_sms(), RAGGED_MAX_CTAS)), dim3(MT == 1 ? 288 : 160), smem, stream, p);
+}
+
+// TMA map of rows [T][heads][128] bf16 with any strides: box {64 dims, box_heads, box_rows}, 128-byte swizzle, rows past T
+// zero-filled.
+int encode_rows_map(CUtensorMap* map, const void* base, int heads, int T, long long head_stride, long long row_stride, int box_heads, int box_rows) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return fail(QK_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint64_t dims[3] = {HEAD_DIM, (cuuint64_t)heads, (cuuint64_t)T};
+  const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)row_stride * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(QK_EINVAL, "cuTensorMapEncodeTiled failed for rows with strides %lld and %lld (CUresult %d)", row_stride, head_stride, (int)r);
+  return QK_OK;
+}
+
+template <int SRC>
+int launch_tc(const RaggedParams& r, int min_rows, void* workspace, cudaStream_t stream) {
+  TcAttnParams p = {};
+  if (int e = encode_rows_map(&p.tm_q, r.q, r.n_q, r.T, r.q_head, r.q_row, r.group, 128 / r.group)) return e;
+  if (SRC == SRC_PACKED) {
+    if (int e = encode_rows_map(&p.tm_k, r.k, r.c.n_kv, r.T, r.kv_head, r.kv_row, 1, TCA_KEYS)) return e;
+    if (int e = encode_rows_map(&p.tm_v, r.v, r.c.n_kv, r.T, r.kv_head, r.kv_row, 1, TCA_KEYS)) return e;
+  } else {
+    const int box = std::min(1 << r.c.page_shift, TCA_KEYS);
+    const long long rows = ((long long)r.c.n_pages * r.c.n_kv) << r.c.page_shift;
+    if (int e = encode_pool_map(&p.tm_k, r.c.k, rows, SRC == SRC_PAGED_FP8, box)) return e;
+    if (int e = encode_pool_map(&p.tm_v, r.c.v, rows, SRC == SRC_PAGED_FP8, box)) return e;
+  }
+  RaggedWorkspace* ws = static_cast<RaggedWorkspace*>(workspace);
+  p.r = r;
+  p.part = ws->part;
+  p.ml = ws->ml;
+  p.counters = ws->tc_counters;
+  p.min_rows = min_rows;
+  auto k = tc_attention_kernel<SRC>;
+  const int smem = (int)sizeof(TcAttnSmem);
+  if (int e = ensure_smem((const void*)k, smem)) return e;
+  return launch(k, dim3(std::min(device_sms(), RAGGED_MAX_CTAS)), dim3(TCA_THREADS), smem, stream, p);
+}
+
+int half_warp_grid(long long rows, long long heads, dim3* grid) {   // a warp per row and pair of heads, 8 warps a CTA
+  const long long n = (rows * ((heads + 1) / 2) + 7) / 8;
+  if (n > 0x7fffffff / 8) return fail(QK_EINVAL, "%lld rows are too many", rows);
+  *grid = dim3((unsigned)n);
+  return QK_OK;
+}
+
+template <int SRC>
+int launch_ragged(const RaggedParams& p, cudaStream_t stream) {
+  const long long warps = (long long)p.T * p.n_q;
+  return launch(ragged_attention_kernel<SRC>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream, p);
 }
 
 }  // namespace
@@ -190,7 +234,7 @@ int qk_paged_kv_read(const qk_paged_kv_read_t* args, qk_stream_t stream) {
                 static_cast<cudaStream_t>(stream), p);
 }
 
-long long qk_ragged_attention_workspace_bytes(void) { return sizeof(FewWorkspace); }
+long long qk_ragged_attention_workspace_bytes(void) { return sizeof(RaggedWorkspace); }
 
 int qk_paged_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
   if (!args) return fail(QK_EINVAL, "null pointer argument");
@@ -203,7 +247,10 @@ int qk_paged_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
   const long long rows = args->max_q * p.group;
   if (rows <= 16) return fp8 ? launch_few<true, 1>(p, 1, args->workspace, st) : launch_few<false, 1>(p, 1, args->workspace, st);
   if (rows <= 32) return fp8 ? launch_few<true, 2>(p, 1, args->workspace, st) : launch_few<false, 2>(p, 1, args->workspace, st);
-  return fp8 ? launch_ragged<SRC_PAGED_FP8>(p, st) : launch_ragged<SRC_PAGED>(p, st);
+  if (fp8) return launch_ragged<SRC_PAGED_FP8>(p, st);
+  // the sequences with up to 16 query rows per KV head (those that decode beside a chunk), then the others
+  if (int e = launch_few<false, 1>(p, 0, args->workspace, st)) return e;
+  return launch_tc<SRC_PAGED>(p, 17, args->workspace, st);
 }
 
 int qk_packed_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
@@ -218,12 +265,12 @@ int qk_packed_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
   if (p.T == 0 || a.cache.batch == 0) return QK_OK;
   p.k = static_cast<const bf16*>(a.k);
   p.v = static_cast<const bf16*>(a.v);
-  p.kv_row = a.kv_row;
-  p.kv_head = a.kv_head;
+  p.kv_row = a.rows == 1 ? a.cache.n_kv * HEAD_DIM : a.kv_row;
+  p.kv_head = a.cache.n_kv == 1 ? HEAD_DIM : a.kv_head;
   p.c.cu = a.cache.cu_rows;
   p.c.B = (int)a.cache.batch;
   p.c.n_kv = (int)a.cache.n_kv;
-  return launch_ragged<SRC_PACKED>(p, static_cast<cudaStream_t>(stream));
+  return launch_tc<SRC_PACKED>(p, 0, args->workspace, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
