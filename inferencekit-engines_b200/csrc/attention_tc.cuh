@@ -29,6 +29,7 @@ constexpr int TCA_KEYS = 128;             // keys of a tile
 constexpr int TCA_TILE = TCA_KEYS * HEAD_DIM * 2;   // 32 KB: two 64-dim halves of 128 rows x 128 B
 constexpr int TCA_STAGES = 5;
 constexpr int TCA_MIN_PIECE = 4;          // tiles
+constexpr int TCA_UNIT_COST = 2;          // what a unit costs beside its key tiles (Q load, first scores, output), in tiles
 constexpr float TCA_LAZY = 8.f;           // log2 of the growth a stale maximum may hide
 
 enum { SRC_PACKED = 0, SRC_PAGED = 1, SRC_PAGED_FP8 = 2 };
@@ -85,8 +86,8 @@ __host__ __device__ __forceinline__ long long floor_sum(unsigned n, unsigned a, 
   }
   return sum;
 }
-// Key tiles of a sequence's tile pairs: pair i covers tokens [i step, (i + 1) step) and the keys its last token sees;
-// a pair that sees none still has rows to set to zero, and counts one.
+// The cost of a sequence's tile pairs: pair i covers tokens [i step, (i + 1) step) and the keys its last token sees, so
+// many tiles (one where it sees none: there still are rows to set to zero), and TCA_UNIT_COST.
 struct TcPairs {
   int n, step, a, len;      // pairs; tokens of a pair; keys before the first token; keys
   __host__ __device__ __forceinline__ TcPairs(const TcSeq& s, int step_) : n((s.n + step_ - 1) / step_), step(step_), a(s.len - s.n), len(s.len) {}
@@ -94,9 +95,11 @@ struct TcPairs {
     const int x = i == n - 1 ? len : a + (i + 1) * step;
     return max(1, (x + TCA_KEYS - 1) / TCA_KEYS);
   }
-  __host__ __device__ __forceinline__ long long before(int i) const {   // tiles of the pairs 0 .. i - 1
+  __host__ __device__ __forceinline__ int cost(int i) const { return tiles(i) + TCA_UNIT_COST; }
+  __host__ __device__ __forceinline__ long long before(int i) const {   // cost of the pairs 0 .. i - 1
     const int q = min(i, n - 1), z = a < 0 ? min(q, -a / step) : 0;
-    return q <= 0 && i < n ? 0 : z + floor_sum(q - z, step, a + (z + 1) * step + TCA_KEYS - 1) + (i == n ? tiles(n - 1) : 0);
+    if (i <= 0) return 0;
+    return z + floor_sum(q - z, step, a + (z + 1) * step + TCA_KEYS - 1) + (i == n ? tiles(n - 1) : 0) + (long long)i * TCA_UNIT_COST;
   }
 };
 
@@ -109,7 +112,7 @@ struct TcAttnSmem {
     long long u;
   } at[2];
   uint64_t q_full, q_empty, full[TCA_STAGES], empty[TCA_STAGES];
-  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t s_full[2], p_full[2][2], o_full[2];   // per tile; P in two halves
   uint32_t tmem;
   int last;
 };
@@ -170,6 +173,67 @@ __device__ __forceinline__ void tca_st32(uint32_t taddr, const uint32_t* v) {
 }
 __device__ __forceinline__ void tca_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// two fp32 values in a register pair, for the packed instructions (half the issue slots)
+__device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float f32x2_lo(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float f32x2_hi(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// Two exp2 on the FMA pipe, for x >= -126 (smaller ones are taken as that): x = n + f with n the nearest integer (the sum
+// with 1.5 * 2^23 rounds there and leaves n in its low bits), 2^f by the cubic with the least relative error on
+// [-1/2, 1/2] (7.5e-5, found by iterated weighted least squares; a bf16 holds 2^-9 = 2e-3), 2^n added to the exponent.
+__device__ __forceinline__ uint64_t ex2_poly2(uint64_t x) {
+  const float magic = 12582912.f;
+  x = f32x2(fmaxf(f32x2_lo(x), -126.f), fmaxf(f32x2_hi(x), -126.f));
+  const uint64_t t = add2(x, f32x2(magic, magic)), f = fma2(add2(t, f32x2(-magic, -magic)), f32x2(-1.f, -1.f), x);
+  uint64_t y = fma2(f, f32x2(0.05517168343067169f, 0.05517168343067169f), f32x2(0.24261115491390228f, 0.24261115491390228f));
+  y = fma2(y, f, f32x2(0.6932609677314758f, 0.6932609677314758f));
+  y = fma2(y, f, f32x2(0.9999280571937561f, 0.9999280571937561f));
+  const uint32_t lo = (uint32_t)y + ((uint32_t)t << 23), hi = (uint32_t)(y >> 32) + ((uint32_t)(t >> 32) << 23);
+  return f32x2(__uint_as_float(lo), __uint_as_float(hi));
+}
+// P of 64 scores: p = exp2(s * scale + base), bf16 pairs to out (which may be the scores' first half), sums to sum.
+// POLY: TCA_POLY of every 8 pairs go to the FMA pipe: the exponential unit alone would take as long over a tile as the
+// matrix unit over its two products. Not where scores are masked: exp2(-inf) has to be 0.
+constexpr int TCA_POLY = 3;
+template <bool POLY>
+__device__ __forceinline__ void tca_exp(const uint32_t* s, uint32_t* out, uint64_t scale, uint64_t base, uint64_t (&sum)[2]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    uint64_t x = fma2(f32x2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale, base);
+    x = POLY && i % 8 < TCA_POLY ? ex2_poly2(x) : f32x2(ex2(f32x2_lo(x)), ex2(f32x2_hi(x)));
+    sum[i & 1] = add2(sum[i & 1], x);
+    out[i] = pack_bf16(f32x2_lo(x), f32x2_hi(x));
+  }
+}
+
+// One lane of a converged warp, the same one every time. The compiler knows it for a single lane (which `lane == 0` does
+// not tell it), so the MMAs' descriptors go straight to the uniform registers that they are taken from.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
 // A CTA's walk over its pieces; every role walks the same one.
 template <int SRC>
 struct TcWalk {
@@ -180,17 +244,18 @@ struct TcWalk {
   long long u, u1;
   int n, t1;                // the unit's key tiles; the piece is [t0, t1)
   __device__ __forceinline__ TcWalk(const TcAttnParams& p_, const TcAttnSmem& sm, int step_)
-      : p(p_), b(sm.at[0].b), g(sm.at[0].g), pair(sm.at[0].pair), t0(sm.at[0].t), step(step_), s(tc_seq<SRC>(p_, sm.at[0].b)), pr(s, step_),
+      : p(p_), b(sm.at[0].b), g(sm.at[0].g), pair(sm.at[0].pair), t0(max(0, sm.at[0].t - TCA_UNIT_COST)), step(step_), s(tc_seq<SRC>(p_, sm.at[0].b)), pr(s, step_),
         u(sm.at[0].u), u1(sm.at[1].u) {
     piece();
   }
+  __device__ __forceinline__ int cost() const { return t0 ? 0 : TCA_UNIT_COST; }   // a unit's own falls to its first piece
   __device__ __forceinline__ void piece() {
     n = pr.tiles(pair);
-    t1 = (int)min((long long)n, t0 + (u1 - u));
+    t1 = (int)min((long long)n, t0 + (u1 - u) - cost());
   }
   __device__ __forceinline__ bool more() const { return u < u1; }
   __device__ __forceinline__ void next() {
-    u += t1 - t0;
+    u += t1 - t0 + cost();
     t0 = 0;
     if (u >= u1) return;
     if (++pair == pr.n) {
@@ -242,7 +307,8 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&sm.s_full[x], 1);
-      mbar_init(&sm.p_full[x], 4);
+      mbar_init(&sm.p_full[x][0], 4);
+      mbar_init(&sm.p_full[x][1], 4);
       mbar_init(&sm.o_full[x], 1);
     }
     fence_mbar_init();
@@ -295,9 +361,9 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
         }
         pair = lo;
         at += pr.before(pair);
-        t = (int)(u - at);
-        const int n = pr.tiles(pair);
-        if (t < TCA_MIN_PIECE) t = 0;
+        t = (int)(u - at);                  // into the unit's cost: TCA_UNIT_COST, then its tiles
+        const int n = pr.cost(pair);
+        if (t < TCA_UNIT_COST + TCA_MIN_PIECE) t = 0;
         else if (n - t < TCA_MIN_PIECE) {   // the range begins with the next unit
           at += n;
           t = 0;
@@ -311,7 +377,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
           }
         }
       }
-      if (lane == 0) sm.at[e] = {b, g, pair, t, at + t};
+      if (lane == 0) sm.at[e] = {b, g, pair, t, at + t};   // u and t count cost: key tile t - TCA_UNIT_COST
     }
     if (lane == 0) sm.total = W;
   }
@@ -394,7 +460,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
       tc_fence_after();
     };
     auto scores = [&](int x, int st) {      // S of tile x = Q K^T
-      if (lane == 0) {
+      if (elect_one()) {
         const uint32_t qa = smem_u32(sm.q[x]), ka = smem_u32(sm.kv[st]);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -411,7 +477,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
       if (!ok) break;
       for (int x = 0; x < 2; ++x)
         if (w.t0 < e[x]) scores(x, it % TCA_STAGES);
-      if (lane == 0) {
+      if (elect_one()) {
         tc_commit(&sm.empty[it % TCA_STAGES]);
         if (cnt == 1) tc_commit(&sm.q_empty);
       }
@@ -429,15 +495,19 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
         }
         for (int x = 0; x < 2 && ok; ++x) {
           if (t < e[x]) {
-            wait(&sm.p_full[x], (uint32_t)(np[x]++ & 1));
-            if (!ok) break;
-            if (lane == 0) {
-              const uint32_t va = smem_u32(sm.kv[vs]);
+            const uint32_t va = smem_u32(sm.kv[vs]);
+            for (int hh = 0; hh < 2; ++hh) {
+              wait(&sm.p_full[x][hh], (uint32_t)(np[x] & 1));
+              if (!ok) break;
+              if (elect_one()) {
 #pragma unroll
-              for (int k = 0; k < 8; ++k)
-                tca_mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * k, tca_desc_mn(va + k * 2048), id_o, k > 0 || t > w.t0);
-              if (t + 1 == e[x]) tc_commit(&sm.o_full[x]);
+                for (int k = 4 * hh; k < 4 * hh + 4; ++k)
+                  tca_mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * k, tca_desc_mn(va + k * 2048), id_o, k > 0 || t > w.t0);
+              }
             }
+            if (!ok) break;
+            ++np[x];
+            if (t + 1 == e[x] && elect_one()) tc_commit(&sm.o_full[x]);
           }
           if (t + 1 < e[x]) {
             wait(&sm.full[ks], (uint32_t)(((it + 2) / TCA_STAGES) & 1));
@@ -447,7 +517,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
         }
         if (!ok) break;
         if (t + 1 < w.t1) wait(&sm.full[ks], (uint32_t)(((it + 2) / TCA_STAGES) & 1));   // loaded even where no tile reads it
-        if (lane == 0) {
+        if (elect_one()) {
           tc_commit(&sm.empty[vs]);
           if (t + 1 < w.t1) tc_commit(&sm.empty[ks]);
           if (t + 2 == w.t1) tc_commit(&sm.q_empty);
@@ -477,19 +547,19 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
 #pragma unroll
         for (int i = 0; i < 4; ++i) tca_ld32(ts + 32 * i, v + 32 * i);
         tc_wait_ld();
-        if (t * TCA_KEYS + TCA_KEYS - 1 > first) {
+        const bool edge = t * TCA_KEYS + TCA_KEYS - 1 > first;
+        if (edge) {
           const int lim = min(pos, w.s.len - 1) - t * TCA_KEYS;
 #pragma unroll
           for (int i = 0; i < 128; ++i)
             if (i > lim) v[i] = 0xff800000u;   // -inf
         }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float mx[4] = {m, m, m, m};
 #pragma unroll
-        for (int i = 0; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[i]));
-        const float mn = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), m);
-        // a row's first maximum, or one that grew by more than TCA_LAZY
-        const bool grow = m == -INFINITY ? mn != -INFINITY : (mn - m) * sl2 > TCA_LAZY;
-        if (__any_sync(0xffffffffu, grow)) {
+        for (int i = 0; i < 128; i += 2) mx[(i >> 1) & 3] = max3_nan(mx[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+        const float mn = max_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3]);
+        // a row's first maximum, one that grew by more than TCA_LAZY, or a NaN
+        if (__any_sync(0xffffffffu, !((mn - m) * sl2 <= TCA_LAZY))) {
           const float f = m == -INFINITY ? 0.f : ex2((m - mn) * sl2);
           m = mn;
           l *= f;
@@ -505,22 +575,22 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
             }
           }
         }
-        const float base = m == -INFINITY ? 0.f : m * sl2;
-        float sum[4] = {};
+        // an infinite maximum makes the row NaN, as inf - inf does
+        const float base = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7fffffff) : -m * sl2;
+        const bool exact = edge || __any_sync(0xffffffffu, m == -INFINITY);
+        const uint64_t base2 = f32x2(base, base), scale2 = f32x2(sl2, sl2);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
-        for (int i = 0; i < 128; i += 2) {
-          const float a = ex2(fmaf(__uint_as_float(v[i]), sl2, -base)), b = ex2(fmaf(__uint_as_float(v[i + 1]), sl2, -base));
-          sum[i & 2] += a;
-          sum[(i & 2) + 1] += b;
-          v[i / 2] = pack_bf16(a, b);
+        for (int hh = 0; hh < 2; ++hh) {    // the products with the first 64 keys start while the others are computed
+          if (exact) tca_exp<false>(v + 64 * hh, v + 32 * hh, scale2, base2, sum);
+          else tca_exp<true>(v + 64 * hh, v + 32 * hh, scale2, base2, sum);
+          tca_st32(ts + 32 * hh, v + 32 * hh);
+          tca_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.p_full[x][hh]);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tca_st32(ts, v);
-        tca_st32(ts + 32, v + 32);
-        tca_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_full[x]);
+        l += (f32x2_lo(sum[0]) + f32x2_hi(sum[0])) + (f32x2_lo(sum[1]) + f32x2_hi(sum[1]));
       }
 
       // ---- the piece's end: the output rows, or a partial --------------------------------------------------------
@@ -555,9 +625,10 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
       }
       // boundaries inside the unit: c_lo .. c_hi; its first piece is CTA c_lo - 1's last (slot 1), piece i > 0 is CTA
       // c_lo + i - 1's first (slot 0)
-      const long long a0 = w.u - w.t0;
+      const long long a0 = w.u - w.t0 - (w.t0 ? TCA_UNIT_COST : 0);
       const int G = (int)min((long long)gridDim.x, max(1ll, W / TCA_MIN_PIECE));
-      const int c_lo = (int)(((a0 + TCA_MIN_PIECE) * G + W - 1) / W), c_hi = (int)(((a0 + w.n - TCA_MIN_PIECE + 1) * G + W - 1) / W) - 1;
+      const int c_lo = (int)(((a0 + TCA_UNIT_COST + TCA_MIN_PIECE) * G + W - 1) / W);
+      const int c_hi = (int)(((a0 + TCA_UNIT_COST + w.n - TCA_MIN_PIECE + 1) * G + W - 1) / W) - 1;
       const size_t slot = ((size_t)(c * 2 + (w.t0 == 0 ? 1 : 0)) * 2 + x) * 128;
       *reinterpret_cast<float2*>(p.ml + (slot + row) * 2) = make_float2(m, l);
       if (any) {
