@@ -11,10 +11,12 @@
 //    thread owns one row: it reads its 128 scores with tcgen05.ld, keeps the running maximum m and sum l, writes
 //    P = exp2(S - m) as bf16 over S in TMEM; O += P V reads P from TMEM and V from shared memory (dims contiguous:
 //    the MN-major operand). P's rounding to bf16 is what the matrix unit takes; l sums the fp32 values.
-//  * O stays in TMEM. Its rows are multiplied by exp2(m_old - m_new) only when a maximum grew by more than 2^8 in
-//    weight: until then the old m serves (P at most 2^8), which changes no result and makes the rescale rare.
+//  * O stays in TMEM. Its rows are multiplied by exp2(m_old - m_new) only when a maximum grew by more than 2^32 in
+//    weight: until then the old m serves. P, l and O have fp32's exponents, so a P of up to 2^32 is as exact as one of 1;
+//    the rescale becomes rare, and a tile's exponentials need not wait for its maximum.
 //  * Warps: 0-3 and 4-7 the softmax of the two tiles, 8 the loads (TMA, 128-byte swizzle, a ring of five 32 KB K and V
-//    tiles), 9 issues the MMAs (10 and 11 fill their warpgroup, which gives its registers to the softmax): Q0 K0, Q1 K0, then per tile P0 V, Q0 K', P1 V, Q1 K', so that while one tile's softmax
+//    tiles), 9 issues the MMAs (10 clears V rows past a sequence's end, 11 fills the
+//    warpgroup, which gives registers to the softmax): Q0 K0, Q1 K0, then per tile P0 V, Q0 K', P1 V, Q1 K', so that while one tile's softmax
 //    runs, the matrix unit has the other's two products to do.
 //  * Work: (sequence, KV head, tile pair, key tile) in that order, dealt in equal contiguous ranges to the CTAs: causal
 //    rows and ragged lengths balance by themselves, and a few rows over a long context spread over every SM. A boundary
@@ -30,7 +32,7 @@ constexpr int TCA_TILE = TCA_KEYS * HEAD_DIM * 2;   // 32 KB: two 64-dim halves 
 constexpr int TCA_STAGES = 5;
 constexpr int TCA_MIN_PIECE = 4;          // tiles
 constexpr int TCA_UNIT_COST = 2;          // what a unit costs beside its key tiles (Q load, first scores, output), in tiles
-constexpr float TCA_LAZY = 8.f;           // log2 of the growth a stale maximum may hide
+constexpr float TCA_LAZY = 32.f;          // log2 of the growth that a stale maximum may hide
 
 enum { SRC_PACKED = 0, SRC_PAGED = 1, SRC_PAGED_FP8 = 2 };
 
@@ -112,7 +114,7 @@ struct TcAttnSmem {
     long long u;
   } at[2];
   uint64_t q_full, q_empty, full[TCA_STAGES], empty[TCA_STAGES];
-  uint64_t s_full[2], p_full[2][2], o_full[2];   // per tile; P in two halves
+  uint64_t s_full[2], p_full[2][2], o_full[2], v_clean[TCA_STAGES];   // per tile; P in two halves
   uint32_t tmem;
   int last;
 };
@@ -171,6 +173,18 @@ __device__ __forceinline__ void tca_st32(uint32_t taddr, const uint32_t* v) {
       "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tca_ld16(uint32_t taddr, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+                 "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void tca_st16(uint32_t taddr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+               "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(taddr)
+               : "memory");
+}
 __device__ __forceinline__ void tca_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
@@ -196,29 +210,14 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// Two exp2 on the FMA pipe, for x >= -126 (smaller ones are taken as that): x = n + f with n the nearest integer (the sum
-// with 1.5 * 2^23 rounds there and leaves n in its low bits), 2^f by the cubic with the least relative error on
-// [-1/2, 1/2] (7.5e-5, found by iterated weighted least squares; a bf16 holds 2^-9 = 2e-3), 2^n added to the exponent.
-__device__ __forceinline__ uint64_t ex2_poly2(uint64_t x) {
-  const float magic = 12582912.f;
-  x = f32x2(fmaxf(f32x2_lo(x), -126.f), fmaxf(f32x2_hi(x), -126.f));
-  const uint64_t t = add2(x, f32x2(magic, magic)), f = fma2(add2(t, f32x2(-magic, -magic)), f32x2(-1.f, -1.f), x);
-  uint64_t y = fma2(f, f32x2(0.05517168343067169f, 0.05517168343067169f), f32x2(0.24261115491390228f, 0.24261115491390228f));
-  y = fma2(y, f, f32x2(0.6932609677314758f, 0.6932609677314758f));
-  y = fma2(y, f, f32x2(0.9999280571937561f, 0.9999280571937561f));
-  const uint32_t lo = (uint32_t)y + ((uint32_t)t << 23), hi = (uint32_t)(y >> 32) + ((uint32_t)(t >> 32) << 23);
-  return f32x2(__uint_as_float(lo), __uint_as_float(hi));
-}
-// P of 64 scores: p = exp2(s * scale + base), bf16 pairs to out (which may be the scores' first half), sums to sum.
-// POLY: TCA_POLY of every 8 pairs go to the FMA pipe: the exponential unit alone would take as long over a tile as the
-// matrix unit over its two products. Not where scores are masked: exp2(-inf) has to be 0.
-constexpr int TCA_POLY = 3;
-template <bool POLY>
+// P of 2 N scores: p = exp2(s * scale + base), bf16 pairs to out (which may be the scores' first half), sums to sum. The
+// packed instructions halve the issue slots beside the exponential unit, which is what bounds this.
+template <int N>
 __device__ __forceinline__ void tca_exp(const uint32_t* s, uint32_t* out, uint64_t scale, uint64_t base, uint64_t (&sum)[2]) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
+  for (int i = 0; i < N; ++i) {
     uint64_t x = fma2(f32x2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale, base);
-    x = POLY && i % 8 < TCA_POLY ? ex2_poly2(x) : f32x2(ex2(f32x2_lo(x)), ex2(f32x2_hi(x)));
+    x = f32x2(ex2(f32x2_lo(x)), ex2(f32x2_hi(x)));
     sum[i & 1] = add2(sum[i & 1], x);
     out[i] = pack_bf16(f32x2_lo(x), f32x2_hi(x));
   }
@@ -303,7 +302,8 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
     mbar_init(&sm.q_empty, 1);
     for (int i = 0; i < TCA_STAGES; ++i) {
       mbar_init(&sm.full[i], 1);
-      mbar_init(&sm.empty[i], 1);
+      mbar_init(&sm.empty[i], 2);
+      mbar_init(&sm.v_clean[i], 1);
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&sm.s_full[x], 1);
@@ -450,81 +450,94 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
     }
     if (!ok)   // a wait gave up: let the copies in flight land before the shared memory goes away
       for (int i = max(0, it - TCA_STAGES); i < it; ++i) mbar_wait(&sm.full[i % TCA_STAGES], (uint32_t)((i / TCA_STAGES) & 1), 1000000ull);
-  } else if (work && warp == 9) {   // ---- MMA issue ----
-    constexpr uint32_t id_s = tca_idesc(false), id_o = tca_idesc(true);
-    TcWalk<SRC> w(p, sm, step);
-    int it = 0, np[2] = {0, 0};
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(bar, parity));
-      tc_fence_after();
-    };
-    auto scores = [&](int x, int st) {      // S of tile x = Q K^T
-      if (elect_one()) {
-        const uint32_t qa = smem_u32(sm.q[x]), ka = smem_u32(sm.kv[st]);
+  } else if (work && warp == 9) {   // ---- MMA issue: one thread, nothing between the products but its waits ----
+    if (elect_one()) {
+      constexpr uint32_t id_s = tca_idesc(false), id_o = tca_idesc(true);
+      TcWalk<SRC> w(p, sm, step);
+      uint32_t st = 0, par = 0, np[2] = {0, 0}, clean = 0;   // st, par: the next tile's stage, its `full` parity; clean: v_clean's
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        ok = ok && mbar_wait(bar, parity);
+        tc_fence_after();
+      };
+      auto take = [&]() {                   // the next K or V tile of the ring
+        wait(&sm.full[st], par);
+        const uint32_t at = st;
+        if (++st == TCA_STAGES) st = 0, par ^= 1;
+        return at;
+      };
+      auto scores = [&](int x, uint32_t at) {   // S = Q K^T
+        const uint64_t qd = tc_desc_sw128(smem_u32(sm.q[x])), kd = tc_desc_sw128(smem_u32(sm.kv[at]));
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const uint32_t off = (k >> 2) * (TCA_TILE / 2) + (k & 3) * 32;
-          tca_mma_ss(tmem + 128 * x, tc_desc_sw128(qa + off), tc_desc_sw128(ka + off), id_s, k > 0);
+          const uint32_t off = ((k >> 2) * (TCA_TILE / 2) + (k & 3) * 32) >> 4;
+          tca_mma_ss(tmem + 128 * x, qd + off, kd + off, id_s, k > 0);
         }
         tc_commit(&sm.s_full[x]);
-      }
-    };
-    for (int unit = 0; w.more() && ok; w.next(), ++unit) {
-      const int e[2] = {w.end(0), w.end(1)}, cnt = w.t1 - w.t0;
-      wait(&sm.q_full, (uint32_t)(unit & 1));
-      wait(&sm.full[it % TCA_STAGES], (uint32_t)((it / TCA_STAGES) & 1));
-      if (!ok) break;
-      for (int x = 0; x < 2; ++x)
-        if (w.t0 < e[x]) scores(x, it % TCA_STAGES);
-      if (elect_one()) {
-        tc_commit(&sm.empty[it % TCA_STAGES]);
-        if (cnt == 1) tc_commit(&sm.q_empty);
-      }
-      for (int t = w.t0; t < w.t1 && ok; ++t) {
-        const int vs = (it + 1) % TCA_STAGES, ks = (it + 2) % TCA_STAGES;
-        wait(&sm.full[vs], (uint32_t)(((it + 1) / TCA_STAGES) & 1));
+      };
+      for (int unit = 0; w.more() && ok; w.next(), ++unit) {
+        const int e[2] = {w.end(0), w.end(1)};
+        wait(&sm.q_full, (uint32_t)(unit & 1));
+        uint32_t ks = take();
         if (!ok) break;
-        const int tail = w.s.len - t * TCA_KEYS;
-        if (tail < TCA_KEYS) {              // rows past the sequence: another's, or nothing; 0 x NaN must not reach O
-          const uint32_t va = smem_u32(sm.kv[vs]);
-          for (int i = max(tail, 0) * 16 + lane; i < TCA_KEYS * 16; i += 32)
-            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(va + ((i >> 3) & 1) * (TCA_TILE / 2) + (i >> 4) * 128 + (i & 7) * 16), "r"(0) : "memory");
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-        for (int x = 0; x < 2 && ok; ++x) {
-          if (t < e[x]) {
-            const uint32_t va = smem_u32(sm.kv[vs]);
-            for (int hh = 0; hh < 2; ++hh) {
-              wait(&sm.p_full[x][hh], (uint32_t)(np[x] & 1));
-              if (!ok) break;
-              if (elect_one()) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (w.t0 < e[x]) scores(x, ks);
+        tc_commit(&sm.empty[ks]);
+        if (w.t1 - w.t0 == 1) tc_commit(&sm.q_empty);
+        for (int t = w.t0; t < w.t1; ++t) {
+          const uint32_t vs = take();
+          const bool more = t + 1 < w.t1;
+          if (w.s.len - t * TCA_KEYS < TCA_KEYS) {
+            wait(&sm.v_clean[vs], clean >> vs & 1);
+            clean ^= 1u << vs;
+          }
+          if (more) ks = take();
+          if (!ok) break;
+          const uint64_t vd = tca_desc_mn(smem_u32(sm.kv[vs]));
+#pragma unroll                              // (the arrays stay in registers)
+          for (int x = 0; x < 2; ++x) {
+            if (t < e[x]) {
+#pragma unroll
+              for (int hh = 0; hh < 2; ++hh) {
+                wait(&sm.p_full[x][hh], np[x] & 1);
+                if (!ok) break;
 #pragma unroll
                 for (int k = 4 * hh; k < 4 * hh + 4; ++k)
-                  tca_mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * k, tca_desc_mn(va + k * 2048), id_o, k > 0 || t > w.t0);
+                  tca_mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * k, vd + k * (2048 >> 4), id_o, k > 0 || t > w.t0);
               }
+              if (t + 1 == e[x]) tc_commit(&sm.o_full[x]);
+              ++np[x];
             }
-            if (!ok) break;
-            ++np[x];
-            if (t + 1 == e[x] && elect_one()) tc_commit(&sm.o_full[x]);
+            if (t + 1 < e[x] && ok) scores(x, ks);
           }
-          if (t + 1 < e[x]) {
-            wait(&sm.full[ks], (uint32_t)(((it + 2) / TCA_STAGES) & 1));
-            if (!ok) break;
-            scores(x, ks);
-          }
-        }
-        if (!ok) break;
-        if (t + 1 < w.t1) wait(&sm.full[ks], (uint32_t)(((it + 2) / TCA_STAGES) & 1));   // loaded even where no tile reads it
-        if (elect_one()) {
+          if (!ok) break;
           tc_commit(&sm.empty[vs]);
-          if (t + 1 < w.t1) tc_commit(&sm.empty[ks]);
+          if (more) tc_commit(&sm.empty[ks]);
           if (t + 2 == w.t1) tc_commit(&sm.q_empty);
         }
-        it += 2;
       }
     }
+    __syncwarp();
+  } else if (work && warp == 10) {   // ---- V rows past a sequence's end: another's, or nothing; 0 x NaN must not reach O ----
+    TcWalk<SRC> w(p, sm, step);
+    uint32_t st = 0, par = 0;
+    bool ok = true;
+    for (; w.more() && ok; w.next())
+      for (int i = 2 * w.t0; i < 2 * w.t1 && ok; ++i) {   // every tile of the ring in turn, K and V
+        ok = __all_sync(0xffffffffu, mbar_wait(&sm.full[st], par));
+        const int tail = w.s.len - (i >> 1) * TCA_KEYS;
+        if ((i & 1) && tail < TCA_KEYS) {
+          const uint32_t va = smem_u32(sm.kv[st]);
+          for (int k = max(tail, 0) * 16 + lane; k < TCA_KEYS * 16; k += 32)
+            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(va + ((k >> 3) & 1) * (TCA_TILE / 2) + (k >> 4) * 128 + (k & 7) * 16), "r"(0) : "memory");
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.v_clean[st]);
+        }
+        if (lane == 0) mbar_arrive(&sm.empty[st]);
+        if (++st == TCA_STAGES) st = 0, par ^= 1;
+      }
   }
   } else {
   regs_inc<TCA_REGS_SOFTMAX>();
@@ -539,57 +552,65 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
       const int e = w.end(x), tok = w.tok0(x) + row / r.group, pos = w.s.len - w.s.n + tok;
       const bool valid = row < (step / 2) * r.group && tok < w.s.n;
       const int first = w.s.len - w.s.n + w.tok0(x);   // the last key that the tile's first row sees
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, l = 0.f, base = 0.f;   // base = -m * sl2
       for (int t = w.t0; t < e; ++t) {
         ok = __all_sync(0xffffffffu, ok && mbar_wait(&sm.s_full[x], (uint32_t)(ns++ & 1)));
         tc_fence_after();
         uint32_t v[128];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tca_ld32(ts + 32 * i, v + 32 * i);
-        tc_wait_ld();
+        const int lim = t * TCA_KEYS + TCA_KEYS - 1 > first ? min(pos, w.s.len - 1) - t * TCA_KEYS : TCA_KEYS;
         const bool edge = t * TCA_KEYS + TCA_KEYS - 1 > first;
-        if (edge) {
-          const int lim = min(pos, w.s.len - 1) - t * TCA_KEYS;
+        auto load_s = [&](int from, int to_) {
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (i > lim) v[i] = 0xff800000u;   // -inf
-        }
+          for (int i = from; i < to_; ++i) tca_ld32(ts + 32 * i, v + 32 * i);
+          tc_wait_ld();
+          if (edge) {
+#pragma unroll
+            for (int i = 32 * from; i < 32 * to_; ++i)
+              if (i > lim) v[i] = 0xff800000u;   // -inf
+          }
+        };
+        load_s(0, 4);
         float mx[4] = {m, m, m, m};
 #pragma unroll
         for (int i = 0; i < 128; i += 2) mx[(i >> 1) & 3] = max3_nan(mx[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
         const float mn = max_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3]);
-        // a row's first maximum, one that grew by more than TCA_LAZY, or a NaN
+        const uint64_t scale2 = f32x2(sl2, sl2);
+        // The first half's exponentials are computed under the old maximum while the new one is found. It stands unless
+        // some row has none yet, or one that grew by more than TCA_LAZY, or a NaN.
+        uint64_t sum[2] = {0, 0};
+        tca_exp<32>(v, v, scale2, f32x2(base, base), sum);
         if (__any_sync(0xffffffffu, !((mn - m) * sl2 <= TCA_LAZY))) {
           const float f = m == -INFINITY ? 0.f : ex2((m - mn) * sl2);
           m = mn;
           l *= f;
+          // an infinite maximum makes the row NaN, as inf - inf does
+          base = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7fffffff) : -m * sl2;
           if (t > w.t0) {                   // the products before this tile's scores are done: O is whole
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t o[32];
-              tca_ld32(to + 32 * i, o);
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i) {
+              uint32_t o[16];
+              tca_ld16(to + 16 * i, o);
               tc_wait_ld();
 #pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-              tca_st32(to + 32 * i, o);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tca_st16(to + 16 * i, o);
             }
           }
+          load_s(0, 2);
+          sum[0] = sum[1] = 0;
+          tca_exp<32>(v, v, scale2, f32x2(base, base), sum);
         }
-        // an infinite maximum makes the row NaN, as inf - inf does
-        const float base = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7fffffff) : -m * sl2;
-        const bool exact = edge || __any_sync(0xffffffffu, m == -INFINITY);
-        const uint64_t base2 = f32x2(base, base), scale2 = f32x2(sl2, sl2);
-        uint64_t sum[2] = {0, 0};
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {    // the products with the first 64 keys start while the others are computed
-          if (exact) tca_exp<false>(v + 64 * hh, v + 32 * hh, scale2, base2, sum);
-          else tca_exp<true>(v + 64 * hh, v + 32 * hh, scale2, base2, sum);
-          tca_st32(ts + 32 * hh, v + 32 * hh);
+        auto hand_over = [&](int hh) {
           tca_wait_st();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.p_full[x][hh]);
-        }
+        };
+        tca_st32(ts, v);
+        hand_over(0);
+        tca_exp<32>(v + 64, v + 32, scale2, f32x2(base, base), sum);
+        tca_st32(ts + 32, v + 32);
+        hand_over(1);
         l += (f32x2_lo(sum[0]) + f32x2_hi(sum[0])) + (f32x2_lo(sum[1]) + f32x2_hi(sum[1]));
       }
 
