@@ -22,6 +22,9 @@
 //    rows and ragged lengths balance by themselves, and a few rows over a long context spread over every SM. A boundary
 //    nearer than TC_MIN_PIECE tiles to the end of a unit moves there. Units cut by one leave fp32 partials (O, m, l) per
 //    piece; the CTA that completes the unit's count adds them in order.
+//  * An e4m3 cache: the loads bring raw tiles and their row scales, and four more warps write them as bf16 tiles in the
+//    image the MMAs read: value times scale, rounded to bf16. That rounding (2^-9 relative, independent from value to
+//    value) is what a bf16 cache has too; exact scales would cost each softmax thread 256 loads and multiplies a tile.
 #pragma once
 #include "attention_few.cuh"
 
@@ -29,7 +32,6 @@ namespace qk {
 
 constexpr int TCA_KEYS = 128;             // keys of a tile
 constexpr int TCA_TILE = TCA_KEYS * HEAD_DIM * 2;   // 32 KB: two 64-dim halves of 128 rows x 128 B
-constexpr int TCA_STAGES = 5;
 constexpr int TCA_MIN_PIECE = 4;          // tiles
 constexpr int TCA_UNIT_COST = 2;          // what a unit costs beside its key tiles (Q load, first scores, output), in tiles
 constexpr float TCA_LAZY = 32.f;          // log2 of the growth that a stale maximum may hide
@@ -105,16 +107,22 @@ struct TcPairs {
   }
 };
 
+struct TcPlace {              // where a range begins
+  int b, g, pair, t;
+  long long u;
+};
+template <int SRC>
 struct TcAttnSmem {
+  static constexpr int S = SRC == SRC_PAGED_FP8 ? 4 : 5;   // K and V tiles of the ring
+  static constexpr int RAW = SRC == SRC_PAGED_FP8 ? 2 : 0;  // e4m3 tiles on their way to bf16
   uint8_t q[2][TCA_TILE];
-  uint8_t kv[TCA_STAGES][TCA_TILE];
+  uint8_t kv[S][TCA_TILE];
+  uint8_t raw[RAW ? RAW : 1][RAW ? TCA_KEYS * HEAD_DIM : 16];
+  float raw_scale[RAW ? RAW : 1][RAW ? TCA_KEYS : 4];
   long long total;
-  struct Place {            // where a range begins
-    int b, g, pair, t;
-    long long u;
-  } at[2];
-  uint64_t q_full, q_empty, full[TCA_STAGES], empty[TCA_STAGES];
-  uint64_t s_full[2], p_full[2][2], o_full[2], v_clean[TCA_STAGES];   // per tile; P in two halves
+  TcPlace at[2];
+  uint64_t q_full, q_empty, full[S], empty[S], raw_full[2], raw_empty[2];
+  uint64_t s_full[2], p_full[2][2], o_full[2], v_clean[S];   // per tile (P in two halves); per stage
   uint32_t tmem;
   int last;
 };
@@ -242,7 +250,7 @@ struct TcWalk {
   TcPairs pr;
   long long u, u1;
   int n, t1;                // the unit's key tiles; the piece is [t0, t1)
-  __device__ __forceinline__ TcWalk(const TcAttnParams& p_, const TcAttnSmem& sm, int step_)
+  __device__ __forceinline__ TcWalk(const TcAttnParams& p_, const TcAttnSmem<SRC>& sm, int step_)
       : p(p_), b(sm.at[0].b), g(sm.at[0].g), pair(sm.at[0].pair), t0(max(0, sm.at[0].t - TCA_UNIT_COST)), step(step_), s(tc_seq<SRC>(p_, sm.at[0].b)), pr(s, step_),
         u(sm.at[0].u), u1(sm.at[1].u) {
     piece();
@@ -277,10 +285,14 @@ struct TcWalk {
   }
 };
 
-constexpr int TCA_THREADS = 384;
-// Registers a thread, out of 384 x 168 at launch: 256 x 208 + 128 x 88
-constexpr int TCA_REGS_SOFTMAX = 208, TCA_REGS_OTHER = 88;
-static_assert(256 * TCA_REGS_SOFTMAX + 128 * TCA_REGS_OTHER <= TCA_THREADS * 168, "setmaxnreg would wait for ever");
+// Threads, and their registers: 384 x 168 at launch become 256 x 208 + 128 x 88; with four warps more, that turn e4m3
+// tiles into bf16 ones, 512 x 128 become 256 x 184 + 256 x 72.
+template <int SRC>
+struct TcShape {
+  static constexpr int THREADS = SRC == SRC_PAGED_FP8 ? 512 : 384;
+  static constexpr int SOFTMAX = SRC == SRC_PAGED_FP8 ? 184 : 208, OTHER = SRC == SRC_PAGED_FP8 ? 72 : 88;
+  static_assert(256 * SOFTMAX + (THREADS - 256) * OTHER <= THREADS * (SRC == SRC_PAGED_FP8 ? 128 : 168), "setmaxnreg would wait for ever");
+};
 template <int N>
 __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -291,9 +303,12 @@ __device__ __forceinline__ void regs_dec() {
 }
 
 template <int SRC>
-__global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __grid_constant__ TcAttnParams p) {
+__global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(const __grid_constant__ TcAttnParams p) {
   extern __shared__ __align__(1024) uint8_t tca_smem[];
-  TcAttnSmem& sm = *reinterpret_cast<TcAttnSmem*>(tca_smem);
+  using Smem = TcAttnSmem<SRC>;
+  Smem& sm = *reinterpret_cast<Smem*>(tca_smem);
+  constexpr int TCA_STAGES = Smem::S;
+  constexpr bool FP8 = SRC == SRC_PAGED_FP8;
   const RaggedParams& r = p.r;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x, n_kv = r.c.n_kv;
   const int step = 2 * (128 / r.group);   // tokens of a tile pair
@@ -301,9 +316,13 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
     mbar_init(&sm.q_full, 1);
     mbar_init(&sm.q_empty, 1);
     for (int i = 0; i < TCA_STAGES; ++i) {
-      mbar_init(&sm.full[i], 1);
-      mbar_init(&sm.empty[i], 2);
+      mbar_init(&sm.full[i], FP8 ? 4 : 1);    // the converting warps; the copies
+      mbar_init(&sm.empty[i], FP8 ? 1 : 2);   // the MMAs; they and the V cleaner
       mbar_init(&sm.v_clean[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.raw_full[i], 1);
+      mbar_init(&sm.raw_empty[i], 4);
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&sm.s_full[x], 1);
@@ -395,7 +414,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
 
   // the register split stands inside the roles' branches: after a join the compiler would have to take the smaller share
   if (warp >= 8) {
-  regs_dec<TCA_REGS_OTHER>();
+  regs_dec<TcShape<SRC>::OTHER>();
   if (work && warp == 8) {   // ---- loads ----
     TcWalk<SRC> w(p, sm, step);
     const int RB = SRC == SRC_PACKED ? TCA_KEYS : min(1 << r.c.page_shift, TCA_KEYS);
@@ -427,29 +446,37 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
         const int page = next;
         if (SRC != SRC_PACKED && t + 1 < w.t1) next = page_of(t + 1);
         for (int v = 0; v < 2; ++v, ++it) {   // K, then V
-          const int st = it % TCA_STAGES;
-          if (it >= TCA_STAGES) ok = __all_sync(0xffffffffu, mbar_wait(&sm.empty[st], (uint32_t)((it / TCA_STAGES - 1) & 1)));
+          constexpr int N = FP8 ? 2 : TCA_STAGES;
+          const int st = it % N;
+          uint64_t* full = FP8 ? &sm.raw_full[st] : &sm.full[st];
+          if (it >= N) ok = __all_sync(0xffffffffu, mbar_wait(FP8 ? &sm.raw_empty[st] : &sm.empty[st], (uint32_t)((it / N - 1) & 1)));
           if (!ok) break;
           const CUtensorMap* tm = v ? &p.tm_v : &p.tm_k;
           if (SRC == SRC_PACKED) {
             if (lane == 0) {
-              mbar_arrive_expect_tx(&sm.full[st], TCA_TILE);
-              for (int h = 0; h < 2; ++h) tma_load_3d(sm.kv[st] + h * (TCA_TILE / 2), tm, 64 * h, w.g, w.s.row0 + t * TCA_KEYS, &sm.full[st]);
+              mbar_arrive_expect_tx(full, TCA_TILE);
+              for (int h = 0; h < 2; ++h) tma_load_3d(sm.kv[st] + h * (TCA_TILE / 2), tm, 64 * h, w.g, w.s.row0 + t * TCA_KEYS, full);
             }
           } else {
             const int nb = __popc(__ballot_sync(0xffffffffu, page >= 0));
-            if (lane == 0) mbar_arrive_expect_tx(&sm.full[st], (uint32_t)(nb * RB) * (2 * HEAD_DIM));
+            if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(nb * RB) * (FP8 ? HEAD_DIM + 4 : 2 * HEAD_DIM));
             __syncwarp();
             if (page >= 0) {
               const int row = ((page * n_kv + w.g) << r.c.page_shift) + ((t * TCA_KEYS + lane * RB) & ((1 << r.c.page_shift) - 1));
-              for (int h = 0; h < 2; ++h) tma_load_2d(sm.kv[st] + h * (TCA_TILE / 2) + lane * RB * 128, tm, 64 * h, row, &sm.full[st]);
+              if (FP8) {                    // a page's rows of a head and their scales are contiguous
+                bulk_g2s(sm.raw[FP8 ? st : 0] + lane * RB * HEAD_DIM, (v ? r.c.v : r.c.k) + (size_t)row * HEAD_DIM, RB * HEAD_DIM, full);
+                bulk_g2s(&sm.raw_scale[FP8 ? st : 0][lane * RB], (v ? r.c.vs : r.c.ks) + row, RB * 4, full);
+              } else {
+                for (int h = 0; h < 2; ++h) tma_load_2d(sm.kv[st] + h * (TCA_TILE / 2) + lane * RB * 128, tm, 64 * h, row, full);
+              }
             }
           }
         }
       }
     }
     if (!ok)   // a wait gave up: let the copies in flight land before the shared memory goes away
-      for (int i = max(0, it - TCA_STAGES); i < it; ++i) mbar_wait(&sm.full[i % TCA_STAGES], (uint32_t)((i / TCA_STAGES) & 1), 1000000ull);
+      for (int n = FP8 ? 2 : TCA_STAGES, i = max(0, it - n); i < it; ++i)
+        mbar_wait(FP8 ? &sm.raw_full[i % n] : &sm.full[i % n], (uint32_t)((i / n) & 1), 1000000ull);
   } else if (work && warp == 9) {   // ---- MMA issue: one thread, nothing between the products but its waits ----
     if (elect_one()) {
       constexpr uint32_t id_s = tca_idesc(false), id_o = tca_idesc(true);
@@ -488,7 +515,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
         for (int t = w.t0; t < w.t1; ++t) {
           const uint32_t vs = take();
           const bool more = t + 1 < w.t1;
-          if (w.s.len - t * TCA_KEYS < TCA_KEYS) {
+          if (!FP8 && w.s.len - t * TCA_KEYS < TCA_KEYS) {
             wait(&sm.v_clean[vs], clean >> vs & 1);
             clean ^= 1u << vs;
           }
@@ -519,7 +546,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
       }
     }
     __syncwarp();
-  } else if (work && warp == 10) {   // ---- V rows past a sequence's end: another's, or nothing; 0 x NaN must not reach O ----
+  } else if (!FP8 && work && warp == 10) {   // ---- V rows past a sequence's end: another's, or nothing; 0 x NaN must not reach O ----
     TcWalk<SRC> w(p, sm, step);
     uint32_t st = 0, par = 0;
     bool ok = true;
@@ -538,9 +565,51 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) tc_attention_kernel(const __gr
         if (lane == 0) mbar_arrive(&sm.empty[st]);
         if (++st == TCA_STAGES) st = 0, par ^= 1;
       }
+  } else if (FP8 && work && warp >= 12) {   // ---- e4m3 tiles to bf16 ones: value times row scale, rounded once ----
+    TcWalk<SRC> w(p, sm, step);
+    const int th = tid - 384;
+    uint32_t it = 0;
+    bool ok = true;
+    for (; w.more() && ok; w.next())
+      for (int i = 2 * w.t0; i < 2 * w.t1 && ok; ++i, ++it) {   // K and V in turn
+        const uint32_t rs = it & 1, st = it % TCA_STAGES;
+        ok = mbar_wait(&sm.raw_full[rs], (it >> 1) & 1);
+        if (it >= TCA_STAGES) ok = ok && mbar_wait(&sm.empty[st], (it / TCA_STAGES - 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        const int tail = w.s.len - (i >> 1) * TCA_KEYS;   // rows from here on were not loaded, or are not the sequence's
+        const uint32_t src = smem_u32(sm.raw[FP8 ? rs : 0]), dst = smem_u32(sm.kv[st]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {       // 16 bytes: 16 dims of a row, to two swizzled 16-byte chunks
+          const int id = k * 128 + th, row = id >> 3, ch = id & 7, half = ch >> 2;
+          const uint4 q = lds128_at(src + id * 16);
+          const float s = row < tail ? sm.raw_scale[FP8 ? rs : 0][row] : 0.f;
+          uint32_t y[8];
+          const uint32_t words[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t h = e4m3x2_to_f16x2(words[j >> 1] >> (16 * (j & 1)));
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+            y[j] = pack_bf16(f.x * s, f.y * s);
+          }
+          if (row >= tail) y[0] = y[1] = y[2] = y[3] = y[4] = y[5] = y[6] = y[7] = 0;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {     // the second half's lanes begin with their other chunk: no bank conflict
+            const int o = j ^ half, c16 = ((ch & 3) * 2 + o) ^ (row & 7);
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + half * (TCA_TILE / 2) + row * 128 + c16 * 16),
+                         "r"(o ? y[4] : y[0]), "r"(o ? y[5] : y[1]), "r"(o ? y[6] : y[2]), "r"(o ? y[7] : y[3])
+                         : "memory");
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sm.full[st]);
+          mbar_arrive(&sm.raw_empty[rs]);
+        }
+      }
   }
   } else {
-  regs_inc<TCA_REGS_SOFTMAX>();
+  regs_inc<TcShape<SRC>::SOFTMAX>();
   if (work) {   // ---- softmax: thread = one row of tile x ----
     const int x = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lanes + 128 * x, to = tmem + lanes + 256 + 128 * x;

@@ -138,8 +138,10 @@ int launch_tc(const RaggedParams& r, int min_rows, void* workspace, cudaStream_t
   } else {
     const int box = std::min(1 << r.c.page_shift, TCA_KEYS);
     const long long rows = ((long long)r.c.n_pages * r.c.n_kv) << r.c.page_shift;
-    if (int e = encode_pool_map(&p.tm_k, r.c.k, rows, SRC == SRC_PAGED_FP8, box)) return e;
-    if (int e = encode_pool_map(&p.tm_v, r.c.v, rows, SRC == SRC_PAGED_FP8, box)) return e;
+    if (SRC == SRC_PAGED) {   // (e4m3 tiles come by untiled copies)
+      if (int e = encode_pool_map(&p.tm_k, r.c.k, rows, false, box)) return e;
+      if (int e = encode_pool_map(&p.tm_v, r.c.v, rows, false, box)) return e;
+    }
   }
   RaggedWorkspace* ws = static_cast<RaggedWorkspace*>(workspace);
   p.r = r;
@@ -148,9 +150,9 @@ int launch_tc(const RaggedParams& r, int min_rows, void* workspace, cudaStream_t
   p.counters = ws->tc_counters;
   p.min_rows = min_rows;
   auto k = tc_attention_kernel<SRC>;
-  const int smem = (int)sizeof(TcAttnSmem);
+  const int smem = (int)sizeof(TcAttnSmem<SRC>);
   if (int e = ensure_smem((const void*)k, smem)) return e;
-  return launch(k, dim3(std::min(device_sms(), RAGGED_MAX_CTAS)), dim3(TCA_THREADS), smem, stream, p);
+  return launch(k, dim3(std::min(device_sms(), RAGGED_MAX_CTAS)), dim3(TcShape<SRC>::THREADS), smem, stream, p);
 }
 
 int half_warp_grid(long long rows, long long heads, dim3* grid) {   // a warp per row and pair of heads, 8 warps a CTA
@@ -158,12 +160,6 @@ int half_warp_grid(long long rows, long long heads, dim3* grid) {   // a warp pe
   if (n > 0x7fffffff / 8) return fail(QK_EINVAL, "%lld rows are too many", rows);
   *grid = dim3((unsigned)n);
   return QK_OK;
-}
-
-template <int SRC>
-int launch_ragged(const RaggedParams& p, cudaStream_t stream) {
-  const long long warps = (long long)p.T * p.n_q;
-  return launch(ragged_attention_kernel<SRC>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream, p);
 }
 
 }  // namespace
@@ -247,10 +243,9 @@ int qk_paged_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
   const long long rows = args->max_q * p.group;
   if (rows <= 16) return fp8 ? launch_few<true, 1>(p, 1, args->workspace, st) : launch_few<false, 1>(p, 1, args->workspace, st);
   if (rows <= 32) return fp8 ? launch_few<true, 2>(p, 1, args->workspace, st) : launch_few<false, 2>(p, 1, args->workspace, st);
-  if (fp8) return launch_ragged<SRC_PAGED_FP8>(p, st);
   // the sequences with up to 16 query rows per KV head (those that decode beside a chunk), then the others
-  if (int e = launch_few<false, 1>(p, 0, args->workspace, st)) return e;
-  return launch_tc<SRC_PAGED>(p, 17, args->workspace, st);
+  if (int e = fp8 ? launch_few<true, 1>(p, 0, args->workspace, st) : launch_few<false, 1>(p, 0, args->workspace, st)) return e;
+  return fp8 ? launch_tc<SRC_PAGED_FP8>(p, 17, args->workspace, st) : launch_tc<SRC_PAGED>(p, 17, args->workspace, st);
 }
 
 int qk_packed_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {

@@ -11,7 +11,8 @@
 #include "../../include/qwen3_b200.h"
 #include "attention.cuh"
 #include "attention_fp8kv.cuh"
-#include "attention_ragged.cuh"
+#include "attention_few.cuh"
+#include "attention_tc.cuh"
 #include "common.cuh"
 #include "gemm_tc.cuh"
 #include "gemv.cuh"
