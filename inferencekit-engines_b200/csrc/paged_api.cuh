@@ -155,13 +155,16 @@ int launch_tc(const RaggedParams& r, int min_rows, void* workspace, cudaStream_t
   return launch(k, dim3(std::min(device_sms(), RAGGED_MAX_CTAS)), dim3(TcShape<SRC>::THREADS), smem, stream, p);
 }
 
-int half_warp_grid(long long rows, long long heads, dim3* grid) {   // a warp per row and pair of heads, 8 warps a CTA
-  const long long n = (rows * ((heads + 1) / 2) + 7) / 8;
-  if (n > 0x7fffffff / 8) return fail(QK_EINVAL, "%lld rows are too many", rows);
+int warp_grid(long long warps, dim3* grid) {   // 8 warps a CTA
+  const long long n = (warps + 7) / 8;
+  if (n > 0x7fffffff / 8) return fail(QK_EINVAL, "%lld warps are too many", warps);
   *grid = dim3((unsigned)n);
   return QK_OK;
 }
 
+// paged_qkv's warps an SM before a warp takes more than one pair of heads: 1,531 rows of 24 heads take 14.4 us with 16 and
+// 16.4 with 8 or 32; 16 rows of 48 heads have a pair each either way.
+constexpr int QKV_WARPS = 16;
 }  // namespace
 
 extern "C" {
@@ -199,12 +202,14 @@ int qk_paged_qkv(const qk_paged_qkv_t* args, qk_stream_t stream) {
   p.n_q = (int)a.n_q;
   p.max_pos = (int)a.max_pos;
   p.half = (int)a.rot_half;
-  p.interleaved = a.interleaved != 0;
   p.eps = (float)a.eps;
+  const long long pairs = (a.n_q + 1) / 2 + 2 * ((p.c.n_kv + 1) / 2);
+  p.span = (int)std::min(pairs, std::max(1ll, a.rows * pairs / ((long long)device_sms() * QKV_WARPS)));
   dim3 grid;
-  if (int r = half_warp_grid(a.rows, a.n_q + 2 * p.c.n_kv, &grid)) return r;
-  return launch(a.cache.kv_fp8 ? paged_qkv_kernel<true> : paged_qkv_kernel<false>, grid, dim3(256), 0,
-                static_cast<cudaStream_t>(stream), p);
+  if (int r = warp_grid(a.rows * ((pairs + p.span - 1) / p.span), &grid)) return r;
+  auto k = a.cache.kv_fp8 ? (a.interleaved ? paged_qkv_kernel<true, true> : paged_qkv_kernel<true, false>)
+                          : (a.interleaved ? paged_qkv_kernel<false, true> : paged_qkv_kernel<false, false>);
+  return launch(k, grid, dim3(256), 0, static_cast<cudaStream_t>(stream), p);
 }
 
 int qk_paged_kv_read(const qk_paged_kv_read_t* args, qk_stream_t stream) {
@@ -225,7 +230,7 @@ int qk_paged_kv_read(const qk_paged_kv_read_t* args, qk_stream_t stream) {
   p.head_stride = a.head_stride;
   p.T = (int)a.rows;
   dim3 grid;
-  if (int r = half_warp_grid(a.rows, p.c.n_kv, &grid)) return r;
+  if (int r = warp_grid(a.rows, &grid)) return r;
   return launch(a.cache.kv_fp8 ? paged_kv_read_kernel<true> : paged_kv_read_kernel<false>, grid, dim3(256), 0,
                 static_cast<cudaStream_t>(stream), p);
 }
