@@ -10,14 +10,15 @@
 //    order (the same bits every run).
 //  * A producer warp keeps a ring of 192 KB of tiles in flight: TMA boxes of one page's rows each, 128-byte
 //    swizzle, so every shared-memory read below is free of bank conflicts.
-//  * Eight consumer warps (four for 17 to 32 rows): 16 keys of a tile each, and each its own running softmax and
-//    output registers, so nothing waits on a neighbour until the piece ends. Scores and P.V are warp-level MMAs
-//    (m16n8k16) with the query rows as M: the tensor work is some 5 % of what these units do, while a 128-row
-//    tcgen05 tile would hold 4 rows in use and pass every score through TMEM.
+//  * Consumer warps take KW keys of a tile each and keep a running softmax and output registers of their own, so nothing
+//    waits on a neighbour until the piece ends. Products are warp-level MMAs with the keys as M: S^T = K Q^T and
+//    O^T = V^T P^T (m16n8k16), 8 query rows a tile of N, so a decode step's 4 heads fill half of it, where rows as M would
+//    fill a quarter, with twice the MMAs and accumulators. P^T turns from one's result into the other's operand with a
+//    movmatrix. A tcgen05 tile of 128 rows would hold 4 in use and pass every score through TMEM.
 //  * bf16 cache: bf16 MMAs, P rounded to bf16. e4m3 cache: the bytes become f16 exactly; q is scaled to f16 range by
 //    a power of two per row; the K scale multiplies the score in fp32; P times the V scale is brought into f16 range
 //    by a running power of two, 2^15 at most, so what falls below f16's smallest value is below 2^-39 of the row's
-//    largest weight.
+//    largest weight. The conversions (4 issue cycles for two values) are what bounds this path beside HBM.
 #pragma once
 #include "gemm_tc.cuh"     // tma_load_2d
 #include "paged.cuh"
@@ -74,19 +75,36 @@ __device__ __forceinline__ int few_tiles(const FewSeq& s) {
   return s.n > 0 ? max(1, (s.len + FEW_KEYS - 1) / FEW_KEYS) : 0;
 }
 
-template <bool FP8>
-struct FewSmem {
+// NT: 8-row tiles of query rows (1, 2 or 4).
+template <bool FP8, int NT>
+struct FewShape {
+#ifndef FEW_CW
+#define FEW_CW (NT <= 2 ? 8 : 4)
+#endif
+#ifndef FEW_KW
+#define FEW_KW (NT == 1 ? 32 : 16)
+#endif
+  static constexpr int ROWS = 8 * NT;
+  static constexpr int CW = FEW_CW;                      // consumer warps
+  static constexpr int KW = FEW_KW;                      // keys of a tile that a warp takes
+  static constexpr int GROUPS = CW * KW / FEW_KEYS;      // groups of warps, a tile each in turn
   static constexpr int TILE = FEW_KEYS * HEAD_DIM * (FP8 ? 1 : 2);
-  static constexpr int S = FEW_RING / (2 * TILE);
-  // Even, so that tile i and stage i % S belong to the same group of warps (i & 1): a group meets every phase of its
-  // stages' barriers, and a wait by parity cannot mistake one phase for the one two before it.
-  static_assert(S % 2 == 0, "a stage must stay with one group of consumer warps");
-  uint8_t k[S][TILE], v[S][TILE];
-  float sum[2][16][HEAD_DIM + 4];       // the warps' outputs on their way to one
-  float ks[FP8 ? S : 1][FEW_KEYS], vs[FP8 ? S : 1][FEW_KEYS];
-  float wm[8][16], wl[8][16];
-  uint64_t full[S], empty[S];
-  long long chunk[288], total, start_prefix;
+  // Stages: a multiple of GROUPS, so that tile i and stage i % S belong to the same group: a group meets every phase of
+  // its stages' barriers, and a wait by parity cannot mistake one phase for the one two before it.
+  static constexpr int S = FEW_RING / (2 * TILE) / GROUPS * GROUPS;
+  static_assert(S >= GROUPS && S > 0, "every group needs a stage");
+  static constexpr int SUMS = 32 / ROWS;                 // warps that add up at a time
+  static constexpr int THREADS = CW * 32 + 32;
+};
+template <bool FP8, int NT>
+struct FewSmem {
+  using Sh = FewShape<FP8, NT>;
+  uint8_t k[Sh::S][Sh::TILE], v[Sh::S][Sh::TILE];
+  float sum[Sh::SUMS][Sh::ROWS][HEAD_DIM + 4];   // the warps' outputs on their way to one
+  float ks[FP8 ? Sh::S : 1][FEW_KEYS], vs[FP8 ? Sh::S : 1][FEW_KEYS];
+  float wm[Sh::CW][Sh::ROWS], wl[Sh::CW][Sh::ROWS];
+  uint64_t full[Sh::S], empty[Sh::S];
+  long long chunk[Sh::THREADS], total, start_prefix;
   int start_b, last;
 };
 
@@ -99,6 +117,11 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {   // an 8 x 8 tile of 16-bit values across the warp
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
 }
 template <bool FP8>
 __device__ __forceinline__ void few_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -121,16 +144,16 @@ __device__ __forceinline__ int exponent_above(float x) {
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 
-// MT: 16-row M tiles (1 or 2).
 __device__ __forceinline__ void few_sync(int threads) { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); }
 // The CTA whose range holds tile u, for ranges [c * W / G, (c + 1) * W / G).
 __device__ __forceinline__ int owner_of(long long u, long long W, int G) { return (int)(((u + 1) * G - 1) / W); }
 
-template <bool FP8, int MT>
-__global__ void __launch_bounds__(MT == 1 ? 288 : 160, 1) few_attention_kernel(const __grid_constant__ FewParams p) {
-  constexpr int ROWS = 16 * MT, CW = MT == 1 ? 8 : 4, GROUPS = CW / 4, THREADS = CW * 32 + 32;
-  using Smem = FewSmem<FP8>;
-  constexpr int S = Smem::S, TILE = Smem::TILE;
+template <bool FP8, int NT>
+__global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_kernel(const __grid_constant__ FewParams p) {
+  using Sh = FewShape<FP8, NT>;
+  using Smem = FewSmem<FP8, NT>;
+  constexpr int ROWS = Sh::ROWS, CW = Sh::CW, KW = Sh::KW, GROUPS = Sh::GROUPS, THREADS = Sh::THREADS, S = Sh::S, TILE = Sh::TILE;
+  constexpr int KT = KW / 16;               // 16-key tiles of M that a warp takes
   extern __shared__ __align__(1024) uint8_t few_smem[];
   Smem& sm = *reinterpret_cast<Smem*>(few_smem);
   const RaggedParams& r = p.r;
@@ -139,7 +162,7 @@ __global__ void __launch_bounds__(MT == 1 ? 288 : 160, 1) few_attention_kernel(c
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&sm.full[s], 1);
-      mbar_init(&sm.empty[s], 4);
+      mbar_init(&sm.empty[s], FEW_KEYS / KW);
     }
     fence_mbar_init();
   }
@@ -197,9 +220,12 @@ __global__ void __launch_bounds__(MT == 1 ? 288 : 160, 1) few_attention_kernel(c
     bool ok = true;
     for (long long u = u0; u < u1 && ok;) {
       const int t1 = (int)min((long long)n, t0 + (u1 - u));
-      auto page_of = [&](int t) {           // this lane's box of tile t: its page, -1 where it holds no key
-        const int j = t * FEW_KEYS + lane * RB;
-        if (lane >= boxes || j >= s.len) return -1;
+      // page numbers of 32 / boxes tiles a load, the next ones on their way: one load a tile would take as long as the
+      // tile's whole share of HBM's time
+      const int batch = 32 / boxes;
+      auto pages_of = [&](int t) {          // lane: box lane % boxes of tile t + lane / boxes; -1 where it holds no key
+        const int tile = t + lane / boxes, j = tile * FEW_KEYS + (lane % boxes) * RB;
+        if (tile >= t1 || j >= s.len) return -1;
         int pg = __ldg(r.c.table + (size_t)b * r.c.table_stride + (j >> r.c.page_shift));
         if (pg < 0 || pg >= r.c.n_pages) {
           atomicOr(&g_dev_error, DEVERR_BAD_STATE);
@@ -207,10 +233,15 @@ __global__ void __launch_bounds__(MT == 1 ? 288 : 160, 1) few_attention_kernel(c
         }
         return pg;
       };
-      int next = page_of(t0);
-      for (int t = t0; t < t1; ++t, ++it) {
-        const int st = it % S, page = next;
-        if (t + 1 < t1) next = page_of(t + 1);
+      int cur = pages_of(t0), next = pages_of(t0 + batch), in = 0;
+      for (int t = t0; t < t1; ++t, ++it, ++in) {
+        const int st = it % S;
+        if (in == batch) {
+          cur = next;
+          next = pages_of(t + batch);
+          in = 0;
+        }
+        const int of_box = __shfl_sync(0xffffffffu, cur, in * boxes + lane % boxes), page = lane < boxes ? of_box : -1;
         if (it >= S) ok = __all_sync(0xffffffffu, mbar_wait(&sm.empty[st], (uint32_t)((it / S - 1) & 1)));
         if (!ok) break;
         const int nb = __popc(__ballot_sync(0xffffffffu, page >= 0));
@@ -244,204 +275,212 @@ __global__ void __launch_bounds__(MT == 1 ? 288 : 160, 1) few_attention_kernel(c
   }
 
   // ---- consumers ----
-  const int grp = warp / 4, quarter = warp & 3, lg = lane >> 2, lt = lane & 3;   // keys 16 * quarter .. + 15 of a tile
+  const int grp = warp / (FEW_KEYS / KW), part = warp % (FEW_KEYS / KW), lg = lane >> 2, lt = lane & 3;
   const float sl2 = r.scale * LOG2E;
   bool ok = true;
   int it = 0;
   for (long long u = u0; u < u1;) {
     const int t1 = (int)min((long long)n, t0 + (u1 - u));
     const int rows = s.n * r.group;
-    // the query rows as A fragments: thread (lg, lt) holds rows lg and lg + 8; the dims of its MMA k slots are the ones
+    // the query rows as B fragments: thread (lg, lt) holds row lg of each tile; the dims of its MMA k slots are the ones
     // its 16-byte K chunks below hold
-    uint32_t qf[MT][8][4];
-    float qs[MT][2];                        // fp8: the power of two that undoes the row's scaling, times scale * log2 e
+    uint32_t qf[NT][8][2];
+    float qs[NT][2];                        // of rows 2 lt, 2 lt + 1: scale * log2 e, fp8: times the power of two that undoes q's
+    int lim[NT][2];                         // the last key each of them sees
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = nt * 8 + lg;
+      uint4 x[4] = {};
+      if (row < rows) {
+        const bf16* src = r.q + (long long)(s.row0 + row / r.group) * r.q_row + (long long)(g * r.group + row % r.group) * r.q_head;
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        const int row = mt * 16 + hh * 8 + lg;
-        uint4 x[4] = {};
-        if (row < rows) {
-          const bf16* src = r.q + (long long)(s.row0 + row / r.group) * r.q_row + (long long)(g * r.group + row % r.group) * r.q_head;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)       // bf16: chunks 2 lt, 2 lt + 1 of each 64-dim half; e4m3: dims 32 lt .. + 31
-            x[i] = *reinterpret_cast<const uint4*>(src + (FP8 ? 32 * lt + 8 * i : 64 * (i >> 1) + 16 * lt + 8 * (i & 1)));
-        }
-        qs[mt][hh] = sl2;
-        if (FP8) {
-          float f[4][8], mx = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            unpack_bf16x8(x[i], f[i]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(f[i][e]));
-          }
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const int e2 = min(max(exponent_above(mx), -110), 110);
-          const float up = pow2(8 - e2);    // the row's largest value lands in [2^7, 2^8)
-          qs[mt][hh] = sl2 * pow2(e2 - 8);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            x[i] = make_uint4(pack_f16(f[i][0] * up, f[i][1] * up), pack_f16(f[i][2] * up, f[i][3] * up),
-                              pack_f16(f[i][4] * up, f[i][5] * up), pack_f16(f[i][6] * up, f[i][7] * up));
-        }
+        for (int i = 0; i < 4; ++i)         // bf16: chunks 2 lt, 2 lt + 1 of each 64-dim half; e4m3: dims 32 lt .. + 31
+          x[i] = *reinterpret_cast<const uint4*>(src + (FP8 ? 32 * lt + 8 * i : 64 * (i >> 1) + 16 * lt + 8 * (i & 1)));
+      }
+      float own = sl2;
+      if (FP8) {
+        float f[4][8], mx = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          qf[mt][2 * i][hh] = x[i].x, qf[mt][2 * i][2 + hh] = x[i].y;
-          qf[mt][2 * i + 1][hh] = x[i].z, qf[mt][2 * i + 1][2 + hh] = x[i].w;
+          unpack_bf16x8(x[i], f[i]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(f[i][e]));
         }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const int e2 = min(max(exponent_above(mx), -110), 110);
+        const float up = pow2(8 - e2);      // the row's largest value lands in [2^7, 2^8)
+        own = sl2 * pow2(e2 - 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[i] = make_uint4(pack_f16(f[i][0] * up, f[i][1] * up), pack_f16(f[i][2] * up, f[i][3] * up),
+                            pack_f16(f[i][4] * up, f[i][5] * up), pack_f16(f[i][6] * up, f[i][7] * up));
       }
-    int lim[MT][2];                         // the last key each row sees
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+      for (int i = 0; i < 4; ++i) {
+        qf[nt][2 * i][0] = x[i].x, qf[nt][2 * i][1] = x[i].y;
+        qf[nt][2 * i + 1][0] = x[i].z, qf[nt][2 * i + 1][1] = x[i].w;
+      }
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) lim[mt][hh] = min(s.len - 1, s.len - s.n + (mt * 16 + hh * 8 + lg) / r.group);
-    float o[MT][16][4], m[MT][2], l[MT][2];
+      for (int e = 0; e < 2; ++e) {
+        qs[nt][e] = __shfl_sync(0xffffffffu, own, (2 * lt + e) * 4);
+        lim[nt][e] = min(s.len - 1, s.len - s.n + (nt * 8 + 2 * lt + e) / r.group);
+      }
+    }
+    float o[8][NT][4], m[NT][2], l[NT][2];
     int ev = -100;                          // fp8: P is multiplied by the V scale over 2^ev
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[mt][i][0] = o[mt][i][1] = o[mt][i][2] = o[mt][i][3] = 0.f;
-      m[mt][0] = m[mt][1] = -INFINITY;
-      l[mt][0] = l[mt][1] = 0.f;
+      for (int i = 0; i < 8; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
     }
     for (int t = t0; t < t1; ++t, ++it) {
-      if (GROUPS == 2 && (it & 1) != grp) continue;
-      const int st = it % S, j0 = t * FEW_KEYS + quarter * 16;
+      if (GROUPS > 1 && it % GROUPS != grp) continue;
+      const int st = it % S, j0 = t * FEW_KEYS + part * KW;
       ok = __all_sync(0xffffffffu, ok && mbar_wait(&sm.full[st], (uint32_t)((it / S) & 1)));
       if (ok && j0 < s.len) {
-        const uint32_t kb = smem_u32(sm.k[st]) + (quarter * 16) * 128, vb = smem_u32(sm.v[st]) + (quarter * 16) * 128;
-        if (j0 + 16 > s.len) {              // the sequence ends inside: what lies behind it must not reach P.V, as 0 x NaN
-          for (int i = lane; i < (j0 + 16 - s.len) * (FP8 ? 8 : 16); i += 32) {
+        const uint32_t kb = smem_u32(sm.k[st]) + (part * KW) * 128, vb = smem_u32(sm.v[st]) + (part * KW) * 128;
+        if (j0 + KW > s.len) {              // the sequence ends inside: what lies behind it must not reach P.V, as 0 x NaN
+          for (int i = lane; i < (j0 + KW - s.len) * (FP8 ? 8 : 16); i += 32) {
             const int row = (s.len - j0) + i / (FP8 ? 8 : 16), ch = i % (FP8 ? 8 : 16);
             asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(vb + (ch >> 3) * (TILE / 2) + row * 128 + (ch & 7) * 16), "r"(0) : "memory");
           }
           fence_proxy_async_smem();         // the ring's next copy into these rows comes after
           __syncwarp();
         }
-        // scores: two 8-key tiles
-        float sc[MT][2][4];
+        // scores of KT tiles of 16 keys: thread (lg, lt) has keys lg and lg + 8 of query rows 2 lt and 2 lt + 1
+        float sc[KT][NT][4];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < KT; ++j) {
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) sc[mt][j][0] = sc[mt][j][1] = sc[mt][j][2] = sc[mt][j][3] = 0.f;
-          const uint32_t ra = kb + (8 * j + lg) * 128;   // row & 7 == lg
+          for (int nt = 0; nt < NT; ++nt) sc[j][nt][0] = sc[j][nt][1] = sc[j][nt][2] = sc[j][nt][3] = 0.f;
+          const uint32_t ra = kb + (16 * j + lg) * 128;   // row & 7 == lg, of row + 8 too
 #pragma unroll
           for (int i = 0; i < (FP8 ? 2 : 4); ++i) {
-            const int ch = (2 * lt + (i & 1)) ^ lg;
-            const uint4 w = lds128_at(ra + (FP8 ? 0 : (i >> 1) * (TILE / 2)) + ch * 16);
+            const uint32_t at = ra + (FP8 ? 0 : (i >> 1) * (TILE / 2)) + ((2 * lt + (i & 1)) ^ lg) * 16;
+            const uint4 w = lds128_at(at), z = lds128_at(at + 8 * 128);
             if (FP8) {
-              const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+              const uint32_t ww[4] = {w.x, w.y, w.z, w.w}, zz[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const uint32_t b0 = e4m3x2_to_f16x2(ww[e]), b1 = e4m3x2_to_f16x2(ww[e] >> 16);
+                const uint32_t af[4] = {e4m3x2_to_f16x2(ww[e]), e4m3x2_to_f16x2(zz[e]), e4m3x2_to_f16x2(ww[e] >> 16), e4m3x2_to_f16x2(zz[e] >> 16)};
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) few_mma<FP8>(sc[mt][j], qf[mt][4 * i + e], b0, b1);
+                for (int nt = 0; nt < NT; ++nt) few_mma<FP8>(sc[j][nt], af, qf[nt][4 * i + e][0], qf[nt][4 * i + e][1]);
               }
             } else {
+              const uint32_t a0[4] = {w.x, z.x, w.y, z.y}, a1[4] = {w.z, z.z, w.w, z.w};
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                few_mma<FP8>(sc[mt][j], qf[mt][2 * i], w.x, w.y);
-                few_mma<FP8>(sc[mt][j], qf[mt][2 * i + 1], w.z, w.w);
+              for (int nt = 0; nt < NT; ++nt) {
+                few_mma<FP8>(sc[j][nt], a0, qf[nt][2 * i][0], qf[nt][2 * i][1]);
+                few_mma<FP8>(sc[j][nt], a1, qf[nt][2 * i + 1][0], qf[nt][2 * i + 1][1]);
               }
             }
           }
         }
-        float kscale[2][2], vscale[2][2];
+        float kscale[KT][2], vscale[KT][2];
         if (FP8) {
           float vmax = 0.f;
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < KT; ++j)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int key = quarter * 16 + 8 * j + 2 * lt + e;
-              kscale[j][e] = sm.ks[st][key];
-              vscale[j][e] = t * FEW_KEYS + key < s.len ? sm.vs[st][key] : 0.f;
-              vmax = fmaxf(vmax, vscale[j][e]);
+            for (int hh = 0; hh < 2; ++hh) {
+              const int key = part * KW + 16 * j + 8 * hh + lg;
+              kscale[j][hh] = sm.ks[st][key];
+              vscale[j][hh] = t * FEW_KEYS + key < s.len ? sm.vs[st][key] : 0.f;
+              vmax = fmaxf(vmax, vscale[j][hh]);
             }
-          vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 1));
-          vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, d));
           const int e2 = exponent_above(vmax);   // the same in every lane
           if (e2 > ev) {
             const float f = pow2(ev - e2);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[mt][i][0] *= f, o[mt][i][1] *= f, o[mt][i][2] *= f, o[mt][i][3] *= f;
+              for (int nt = 0; nt < NT; ++nt) o[i][nt][0] *= f, o[i][nt][1] *= f, o[i][nt][2] *= f, o[i][nt][3] *= f;
             ev = e2;
           }
-          const float dn = pow2(-ev);
+          const float dn = pow2(-ev) * 32768.f;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) vscale[j][0] *= dn * 32768.f, vscale[j][1] *= dn * 32768.f;
+          for (int j = 0; j < KT; ++j) vscale[j][0] *= dn, vscale[j][1] *= dn;
         }
-        const bool edge = j0 + 15 > s.len - s.n;        // some row does not see some of the 16 keys
-        uint32_t pf[MT][4];
+        const bool edge = j0 + KW - 1 > s.len - s.n;    // some row does not see some of the keys
+        uint32_t pf[KT][NT][2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int nt = 0; nt < NT; ++nt) {
           float f[2];
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            float x[4];
+          for (int e = 0; e < 2; ++e) {
+            float mx = m[nt][e];
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < KT; ++j)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float raw = sc[mt][j][2 * hh + e] * qs[mt][hh];
-                x[2 * j + e] = FP8 ? raw * kscale[j][e] : raw;
-                if (edge && j0 + 8 * j + 2 * lt + e > lim[mt][hh]) x[2 * j + e] = -INFINITY;
+              for (int hh = 0; hh < 2; ++hh) {
+                float& x = sc[j][nt][2 * hh + e];
+                x *= FP8 ? qs[nt][e] * kscale[j][hh] : qs[nt][e];
+                if (edge && j0 + 16 * j + 8 * hh + lg > lim[nt][e]) x = -INFINITY;
+                mx = fmaxf(mx, x);
               }
-            float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float mn = fmaxf(m[mt][hh], mx), base = mn == -INFINITY ? 0.f : mn;
-            f[hh] = ex2(m[mt][hh] - base);
-            m[mt][hh] = mn;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = ex2(x[e] - base);
-            l[mt][hh] = l[mt][hh] * f[hh] + ((x[0] + x[1]) + (x[2] + x[3]));
+            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            const float base = mx == -INFINITY ? 0.f : mx;
+            f[e] = ex2(m[nt][e] - base);
+            m[nt][e] = mx;
+            float add = 0.f;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-              pf[mt][2 * j + hh] = FP8 ? pack_f16(x[2 * j] * vscale[j][0], x[2 * j + 1] * vscale[j][1]) : pack_bf16(x[2 * j], x[2 * j + 1]);
+            for (int j = 0; j < KT; ++j)
+#pragma unroll
+              for (int hh = 0; hh < 2; ++hh) {
+                float& x = sc[j][nt][2 * hh + e];
+                x = ex2(x - base);
+                add += x;
+                if (FP8) x *= vscale[j][hh];
+              }
+            l[nt][e] = l[nt][e] * f[e] + add;
           }
           if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[mt][i][0] *= f[0], o[mt][i][1] *= f[0], o[mt][i][2] *= f[1], o[mt][i][3] *= f[1];
+            for (int i = 0; i < 8; ++i) o[i][nt][0] *= f[0], o[i][nt][1] *= f[1], o[i][nt][2] *= f[0], o[i][nt][3] *= f[1];
           }
+#pragma unroll
+          for (int j = 0; j < KT; ++j)
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh)
+              pf[j][nt][hh] = transpose8x8(FP8 ? pack_f16(sc[j][nt][2 * hh], sc[j][nt][2 * hh + 1]) : pack_bf16(sc[j][nt][2 * hh], sc[j][nt][2 * hh + 1]));
         }
-        // P.V: 16 tiles of 8 output columns
-        if (FP8) {                          // column n of tile i is dim 16 n + i: a thread's chunk lg holds all its tiles
-          uint4 w[4];
+        // O^T: 8 tiles of 16 dims
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int row = 8 * (j >> 1) + 2 * lt + (j & 1);
-            w[j] = lds128_at(vb + row * 128 + ((lg ^ (row & 7)) * 16));
-          }
+        for (int j = 0; j < KT; ++j) {
+          if (FP8) {                        // row lg of tile i is dim 16 lg + 2 i, row lg + 8 the next: a thread's chunk lg holds all its dims
+            uint4 w[4];
 #pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            const uint32_t a[4] = {q4 == 0 ? w[0].x : q4 == 1 ? w[0].y : q4 == 2 ? w[0].z : w[0].w,
-                                   q4 == 0 ? w[1].x : q4 == 1 ? w[1].y : q4 == 2 ? w[1].z : w[1].w,
-                                   q4 == 0 ? w[2].x : q4 == 1 ? w[2].y : q4 == 2 ? w[2].z : w[2].w,
-                                   q4 == 0 ? w[3].x : q4 == 1 ? w[3].y : q4 == 2 ? w[3].z : w[3].w};
-            const uint32_t lo0 = __byte_perm(a[0], a[1], 0x5140), hi0 = __byte_perm(a[0], a[1], 0x7362);
-            const uint32_t lo1 = __byte_perm(a[2], a[3], 0x5140), hi1 = __byte_perm(a[2], a[3], 0x7362);
-            const uint32_t b0[4] = {e4m3x2_to_f16x2(lo0), e4m3x2_to_f16x2(lo0 >> 16), e4m3x2_to_f16x2(hi0), e4m3x2_to_f16x2(hi0 >> 16)};
-            const uint32_t b1[4] = {e4m3x2_to_f16x2(lo1), e4m3x2_to_f16x2(lo1 >> 16), e4m3x2_to_f16x2(hi1), e4m3x2_to_f16x2(hi1 >> 16)};
+            for (int k = 0; k < 4; ++k) {
+              const int row = 8 * (k >> 1) + 2 * lt + (k & 1);
+              w[k] = lds128_at(vb + (16 * j + row) * 128 + ((lg ^ (row & 7)) * 16));
+            }
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int q4 = 0; q4 < 4; ++q4) {
+              uint32_t a[4];
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) few_mma<FP8>(o[mt][4 * q4 + e], pf[mt], b0[e], b1[e]);
-          }
-        } else {
+              for (int k = 0; k < 4; ++k) a[k] = q4 == 0 ? w[k].x : q4 == 1 ? w[k].y : q4 == 2 ? w[k].z : w[k].w;
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const int row = lane & 15, ch = (i + (lane >> 4)) & 7;
-            uint32_t w[4];
-            ldmatrix4_trans(w, vb + (i >> 3) * (TILE / 2) + row * 128 + ((ch ^ (row & 7)) * 16));
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t lo = __byte_perm(a[0], a[1], i ? 0x7362 : 0x5140), hi = __byte_perm(a[2], a[3], i ? 0x7362 : 0x5140);
+                const uint32_t af[4] = {e4m3x2_to_f16x2(lo), e4m3x2_to_f16x2(lo >> 16), e4m3x2_to_f16x2(hi), e4m3x2_to_f16x2(hi >> 16)};
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              few_mma<FP8>(o[mt][i], pf[mt], w[0], w[1]);
-              few_mma<FP8>(o[mt][i + 1], pf[mt], w[2], w[3]);
+                for (int nt = 0; nt < NT; ++nt) few_mma<FP8>(o[2 * q4 + i][nt], af, pf[j][nt][0], pf[j][nt][1]);
+              }
+            }
+          } else {                          // row lg of tile i is dim 16 i + lg
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int row = (lane & 7) + 8 * (lane >> 4), ch = (2 * i + ((lane >> 3) & 1)) & 7;
+              uint32_t af[4];
+              ldmatrix4_trans(af, vb + (i >> 2) * (TILE / 2) + (16 * j + row) * 128 + ((ch ^ (row & 7)) * 16));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) few_mma<FP8>(o[i][nt], af, pf[j][nt][0], pf[j][nt][1]);
             }
           }
         }
@@ -456,67 +495,69 @@ __global__ void __launch_bounds__(MT == 1 ? 288 : 160, 1) few_attention_kernel(c
     const int cf = owner_of(unit0, W, G), cl = owner_of(unit0 + n - 1, W, G);
     const int slot = u == u0 ? 0 : 1;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        l[mt][hh] += __shfl_xor_sync(0xffffffffu, l[mt][hh], 1);
-        l[mt][hh] += __shfl_xor_sync(0xffffffffu, l[mt][hh], 2);
-        if (lt == 0) sm.wm[warp][hh * 8 + lg] = m[mt][hh], sm.wl[warp][hh * 8 + lg] = l[mt][hh];
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], d);
+        if (lg == 0) sm.wm[warp][nt * 8 + 2 * lt + e] = m[nt][e], sm.wl[warp][nt * 8 + 2 * lt + e] = l[nt][e];
       }
-      few_sync(CW * 32);
-      float f[2];
+    few_sync(CW * 32);
+    float f[NT][2];
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
         float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < CW; ++w) M = fmaxf(M, sm.wm[w][hh * 8 + lg]);
-        f[hh] = M == -INFINITY ? 1.f : ex2(m[mt][hh] - M);
-        if (FP8) f[hh] *= pow2(ev) * (1.f / 32768.f);
+        for (int w = 0; w < CW; ++w) M = fmaxf(M, sm.wm[w][nt * 8 + 2 * lt + e]);
+        f[nt][e] = M == -INFINITY ? 1.f : ex2(m[nt][e] - M);
+        if (FP8) f[nt][e] *= pow2(ev) * (1.f / 32768.f);
       }
-      auto put = [&](float (&dst)[16][HEAD_DIM + 4], bool add) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+    for (int w = CW - Sh::SUMS; w >= 0; w -= Sh::SUMS) {   // SUMS warps at a time
+      if (warp >= w && warp < w + Sh::SUMS) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int d = FP8 ? 16 * (2 * lt + (e & 1)) + i : 8 * i + 2 * lt + (e & 1);
-            float& x = dst[(e >> 1) * 8 + lg][d];
-            const float y = o[mt][i][e] * f[e >> 1];
-            x = add ? x + y : y;
-          }
-      };
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int w = CW - 2; w >= 0; w -= 2) {  // two warps at a time
-        if ((warp & ~1) == w) put(sm.sum[warp & 1], w != CW - 2);
-        few_sync(CW * 32);
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int d = FP8 ? 16 * lg + 2 * i + (e >> 1) : 16 * i + 8 * (e >> 1) + lg;
+              float& x = sm.sum[warp - w][nt * 8 + 2 * lt + (e & 1)][d];
+              const float y = o[i][nt][e] * f[nt][e & 1];
+              x = w == CW - Sh::SUMS ? y : x + y;
+            }
       }
-      // thread: 8 dims of a row (16 threads a row)
-      for (int i = tid; i < 16 * 16; i += CW * 32) {
-        const int rr = i >> 4, d0 = (i & 15) * 8, row = mt * 16 + rr;
-        if (row >= rows) continue;
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          x[e] = sm.sum[0][rr][d0 + e] + sm.sum[1][rr][d0 + e];
-        float M = -INFINITY, L = 0.f;
-#pragma unroll
-        for (int w = 0; w < CW; ++w) M = fmaxf(M, sm.wm[w][rr]);
-#pragma unroll
-        for (int w = 0; w < CW; ++w) L += M == -INFINITY ? sm.wl[w][rr] : sm.wl[w][rr] * ex2(sm.wm[w][rr] - M);
-        if (whole) {
-          const float inv = L == 0.f ? 0.f : 1.f / L;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] *= inv;
-          *reinterpret_cast<uint4*>(r.out + (long long)(s.row0 + row / r.group) * r.out_row +
-                                    (long long)(g * r.group + row % r.group) * r.out_head + d0) = pack_bf16x8(x);
-        } else {
-          const size_t at = (size_t)(c * 2 + slot) * ROWS + row;
-          *reinterpret_cast<float4*>(p.part + at * HEAD_DIM + d0) = make_float4(x[0], x[1], x[2], x[3]);
-          *reinterpret_cast<float4*>(p.part + at * HEAD_DIM + d0 + 4) = make_float4(x[4], x[5], x[6], x[7]);
-          if (d0 == 0) *reinterpret_cast<float2*>(p.ml + at * 2) = make_float2(M, L);
-        }
-      }
-      few_sync(CW * 32);                    // sum, wm and wl are free again
+      few_sync(CW * 32);
     }
+    // thread: 8 dims of a row (16 threads a row)
+    for (int i = tid; i < rows * 16; i += CW * 32) {
+      const int row = i >> 4, d0 = (i & 15) * 8;
+      float x[8] = {};
+#pragma unroll
+      for (int w = 0; w < Sh::SUMS; ++w)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] += sm.sum[w][row][d0 + e];
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < CW; ++w) M = fmaxf(M, sm.wm[w][row]);
+#pragma unroll
+      for (int w = 0; w < CW; ++w) L += M == -INFINITY ? sm.wl[w][row] : sm.wl[w][row] * ex2(sm.wm[w][row] - M);
+      if (whole) {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= inv;
+        *reinterpret_cast<uint4*>(r.out + (long long)(s.row0 + row / r.group) * r.out_row +
+                                  (long long)(g * r.group + row % r.group) * r.out_head + d0) = pack_bf16x8(x);
+      } else {
+        const size_t at = (size_t)(c * 2 + slot) * ROWS + row;
+        *reinterpret_cast<float4*>(p.part + at * HEAD_DIM + d0) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(p.part + at * HEAD_DIM + d0 + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        if (d0 == 0) *reinterpret_cast<float2*>(p.ml + at * 2) = make_float2(M, L);
+      }
+    }
+    few_sync(CW * 32);                      // sum, wm and wl are free again
     if (!whole) {
       __threadfence();
       few_sync(CW * 32);

@@ -92,7 +92,7 @@ struct RaggedWorkspace {
   float part[RAGGED_MAX_CTAS * 2 * 256 * HEAD_DIM];
 };
 
-template <bool FP8, int MT>
+template <bool FP8, int NT>
 int launch_few(const RaggedParams& r, int strict, void* workspace, cudaStream_t stream) {
   FewParams p = {};
   const int box = std::min(1 << r.c.page_shift, FEW_KEYS);
@@ -105,10 +105,10 @@ int launch_few(const RaggedParams& r, int strict, void* workspace, cudaStream_t 
   p.ml = ws->ml;
   p.counters = ws->few_counters;
   p.strict = strict;
-  auto k = few_attention_kernel<FP8, MT>;
-  const int smem = (int)sizeof(FewSmem<FP8>);
+  auto k = few_attention_kernel<FP8, NT>;
+  const int smem = (int)sizeof(FewSmem<FP8, NT>);
   if (int e = ensure_smem((const void*)k, smem)) return e;
-  return launch(k, dim3(std::min(device_sms(), RAGGED_MAX_CTAS)), dim3(MT == 1 ? 288 : 160), smem, stream, p);
+  return launch(k, dim3(std::min(device_sms(), RAGGED_MAX_CTAS)), dim3(FewShape<FP8, NT>::THREADS), smem, stream, p);
 }
 
 // TMA map of rows [T][heads][128] bf16 with any strides: box {64 dims, box_heads, box_rows}, 128-byte swizzle, rows past T
@@ -246,10 +246,11 @@ int qk_paged_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
   const bool fp8 = args->cache.kv_fp8 != 0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const long long rows = args->max_q * p.group;
-  if (rows <= 16) return fp8 ? launch_few<true, 1>(p, 1, args->workspace, st) : launch_few<false, 1>(p, 1, args->workspace, st);
-  if (rows <= 32) return fp8 ? launch_few<true, 2>(p, 1, args->workspace, st) : launch_few<false, 2>(p, 1, args->workspace, st);
+  if (rows <= 8) return fp8 ? launch_few<true, 1>(p, 1, args->workspace, st) : launch_few<false, 1>(p, 1, args->workspace, st);
+  if (rows <= 16) return fp8 ? launch_few<true, 2>(p, 1, args->workspace, st) : launch_few<false, 2>(p, 1, args->workspace, st);
+  if (rows <= 32) return fp8 ? launch_few<true, 4>(p, 1, args->workspace, st) : launch_few<false, 4>(p, 1, args->workspace, st);
   // the sequences with up to 16 query rows per KV head (those that decode beside a chunk), then the others
-  if (int e = fp8 ? launch_few<true, 1>(p, 0, args->workspace, st) : launch_few<false, 1>(p, 0, args->workspace, st)) return e;
+  if (int e = fp8 ? launch_few<true, 2>(p, 0, args->workspace, st) : launch_few<false, 2>(p, 0, args->workspace, st)) return e;
   return fp8 ? launch_tc<SRC_PAGED_FP8>(p, 17, args->workspace, st) : launch_tc<SRC_PAGED>(p, 17, args->workspace, st);
 }
 
