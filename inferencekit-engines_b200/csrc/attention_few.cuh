@@ -4,7 +4,7 @@
 //
 // Bound by the cache bytes: up to 32 query rows (tokens x heads of a KV head) meet each K and V row once, so the only
 // aim is to keep HBM busy.
-//  * Work: the (sequence, KV head, 64-key tile) triples, tile-major, are dealt in equal contiguous ranges to one CTA
+//  * Work: the (sequence, KV head, key tile) triples, tile-major, are dealt in equal contiguous ranges to one CTA
 //    per SM, whatever the lengths are: a 32k context beside short ones leaves no SM idle. A unit (sequence, head)
 //    split between CTAs leaves fp32 partials (o, m, l); the CTA that completes the unit's count adds them in CTA
 //    order (the same bits every run).
@@ -25,7 +25,6 @@
 
 namespace qk {
 
-constexpr int FEW_KEYS = 64;          // keys of a tile
 constexpr int FEW_RING = 196608;      // bytes of K and V in the ring
 constexpr int FEW_MIN_TILES = 1;      // a CTA's least share
 constexpr float LOG2E = 1.4426950408889634f;
@@ -71,8 +70,9 @@ __device__ __forceinline__ FewSeq few_seq(const RaggedParams& r, int b, int stri
   return s;
 }
 // Tiles of one of its heads; a sequence without a key still has rows to set to zero.
+template <int KEYS>
 __device__ __forceinline__ int few_tiles(const FewSeq& s) {
-  return s.n > 0 ? max(1, (s.len + FEW_KEYS - 1) / FEW_KEYS) : 0;
+  return s.n > 0 ? max(1, (s.len + KEYS - 1) / KEYS) : 0;
 }
 
 // NT: 8-row tiles of query rows (1, 2 or 4).
@@ -82,13 +82,17 @@ struct FewShape {
 #define FEW_CW (NT <= 2 ? 8 : 4)
 #endif
 #ifndef FEW_KW
-#define FEW_KW (NT == 1 ? 32 : 16)
+#define FEW_KW (FP8 || NT == 1 ? 32 : 16)
+#endif
+#ifndef FEW_K8
+#define FEW_K8 128
 #endif
   static constexpr int ROWS = 8 * NT;
+  static constexpr int KEYS = FP8 ? FEW_K8 : 64;            // keys of a tile
   static constexpr int CW = FEW_CW;                      // consumer warps
   static constexpr int KW = FEW_KW;                      // keys of a tile that a warp takes
-  static constexpr int GROUPS = CW * KW / FEW_KEYS;      // groups of warps, a tile each in turn
-  static constexpr int TILE = FEW_KEYS * HEAD_DIM * (FP8 ? 1 : 2);
+  static constexpr int GROUPS = CW * KW / KEYS;      // groups of warps, a tile each in turn
+  static constexpr int TILE = KEYS * HEAD_DIM * (FP8 ? 1 : 2);
   // Stages: a multiple of GROUPS, so that tile i and stage i % S belong to the same group: a group meets every phase of
   // its stages' barriers, and a wait by parity cannot mistake one phase for the one two before it.
   static constexpr int S = FEW_RING / (2 * TILE) / GROUPS * GROUPS;
@@ -101,7 +105,7 @@ struct FewSmem {
   using Sh = FewShape<FP8, NT>;
   uint8_t k[Sh::S][Sh::TILE], v[Sh::S][Sh::TILE];
   float sum[Sh::SUMS][Sh::ROWS][HEAD_DIM + 4];   // the warps' outputs on their way to one
-  float ks[FP8 ? Sh::S : 1][FEW_KEYS], vs[FP8 ? Sh::S : 1][FEW_KEYS];
+  float ks[FP8 ? Sh::S : 1][Sh::KEYS], vs[FP8 ? Sh::S : 1][Sh::KEYS];
   float wm[Sh::CW][Sh::ROWS], wl[Sh::CW][Sh::ROWS];
   uint64_t full[Sh::S], empty[Sh::S];
   long long chunk[Sh::THREADS], total, start_prefix;
@@ -153,6 +157,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
   using Sh = FewShape<FP8, NT>;
   using Smem = FewSmem<FP8, NT>;
   constexpr int ROWS = Sh::ROWS, CW = Sh::CW, KW = Sh::KW, GROUPS = Sh::GROUPS, THREADS = Sh::THREADS, S = Sh::S, TILE = Sh::TILE;
+  constexpr int FEW_KEYS = Sh::KEYS;
   constexpr int KT = KW / 16;               // 16-key tiles of M that a warp takes
   extern __shared__ __align__(1024) uint8_t few_smem[];
   Smem& sm = *reinterpret_cast<Smem*>(few_smem);
@@ -172,7 +177,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
   // ---- this CTA's range of tiles: the total, then the sequence its first tile lies in -----------------------------
   const int per = (r.c.B + THREADS - 1) / THREADS;
   long long mine = 0;
-  for (int b = tid * per; b < min(r.c.B, (tid + 1) * per); ++b) mine += (long long)few_tiles(few_seq<ROWS>(r, b, p.strict)) * n_kv;
+  for (int b = tid * per; b < min(r.c.B, (tid + 1) * per); ++b) mine += (long long)few_tiles<FEW_KEYS>(few_seq<ROWS>(r, b, p.strict)) * n_kv;
   sm.chunk[tid] = mine;
   __syncthreads();
   if (warp == 0) {                          // inclusive sums over the threads' chunks
@@ -198,7 +203,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
     long long at = sm.chunk[tid] - mine;
     int b = tid * per;
     for (;; ++b) {
-      const long long n = (long long)few_tiles(few_seq<ROWS>(r, b, 0)) * n_kv;
+      const long long n = (long long)few_tiles<FEW_KEYS>(few_seq<ROWS>(r, b, 0)) * n_kv;
       if (u0 < at + n) break;
       at += n;
     }
@@ -210,7 +215,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
   // Every warp walks the same pieces: b, its tiles per head, the head, the tiles [t0, t1) of the head.
   int b = sm.start_b;
   FewSeq s = few_seq<ROWS>(r, b, 0);
-  int n = few_tiles(s);
+  int n = few_tiles<FEW_KEYS>(s);
   int g = (int)((u0 - sm.start_prefix) / n), t0 = (int)((u0 - sm.start_prefix) - (long long)g * n);
   const uint32_t bytes_row = FP8 ? HEAD_DIM : 2 * HEAD_DIM;
 
@@ -263,8 +268,8 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
       if (u < u1 && ++g == n_kv) {
         g = 0;
         do s = few_seq<ROWS>(r, ++b, 0);
-        while (few_tiles(s) == 0);
-        n = few_tiles(s);
+        while (few_tiles<FEW_KEYS>(s) == 0);
+        n = few_tiles<FEW_KEYS>(s);
       }
     }
     if (ok)   // the last stages' copies are waited for by the consumers
@@ -601,8 +606,8 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
     if (u < u1 && ++g == n_kv) {
       g = 0;
       do s = few_seq<ROWS>(r, ++b, 0);
-      while (few_tiles(s) == 0);
-      n = few_tiles(s);
+      while (few_tiles<FEW_KEYS>(s) == 0);
+      n = few_tiles<FEW_KEYS>(s);
     }
   }
   if (!ok && lane == 0) atomicOr(&g_dev_error, DEVERR_MBAR_TIMEOUT);

@@ -95,7 +95,7 @@ struct RaggedWorkspace {
 template <bool FP8, int NT>
 int launch_few(const RaggedParams& r, int strict, void* workspace, cudaStream_t stream) {
   FewParams p = {};
-  const int box = std::min(1 << r.c.page_shift, FEW_KEYS);
+  const int box = std::min(1 << r.c.page_shift, FewShape<FP8, NT>::KEYS);
   const long long rows = ((long long)r.c.n_pages * r.c.n_kv) << r.c.page_shift;
   if (int e = encode_pool_map(&p.tm_k, r.c.k, rows, FP8, box)) return e;
   if (int e = encode_pool_map(&p.tm_v, r.c.v, rows, FP8, box)) return e;
