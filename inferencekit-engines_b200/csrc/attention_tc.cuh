@@ -22,7 +22,7 @@
 //    rows and ragged lengths balance by themselves, and a few rows over a long context spread over every SM. A boundary
 //    nearer than TC_MIN_PIECE tiles to the end of a unit moves there. Units cut by one leave fp32 partials (O, m, l) per
 //    piece; the CTA that completes the unit's count adds them in order.
-//  * An e4m3 cache: the loads bring raw tiles and their row scales, and four more warps write them as bf16 tiles in the
+//  * An e4m3 cache: the loads bring raw tiles and their row scales, and six more warps write them as bf16 tiles in the
 //    image the MMAs read: value times scale, rounded to bf16. That rounding (2^-9 relative, independent from value to
 //    value) is what a bf16 cache has too; exact scales would cost each softmax thread 256 loads and multiplies a tile.
 #pragma once
@@ -262,8 +262,8 @@ struct TcWalk {
   }
 };
 
-// Threads, and their registers: 384 x 168 at launch become 256 x 208 + 128 x 88; with four warps more, that turn e4m3
-// tiles into bf16 ones, 512 x 128 become 256 x 184 + 256 x 72.
+// Threads, and their registers: 384 x 168 at launch become 256 x 208 + 128 x 88; with four warps more (they, 10 and 11 turn
+// e4m3 tiles into bf16 ones), 512 x 128 become 256 x 184 + 256 x 72.
 template <int SRC>
 struct TcShape {
   static constexpr int THREADS = SRC == SRC_PAGED_FP8 ? 512 : 384;
@@ -293,13 +293,13 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
     mbar_init(&sm.q_full, 1);
     mbar_init(&sm.q_empty, 1);
     for (int i = 0; i < TCA_STAGES; ++i) {
-      mbar_init(&sm.full[i], FP8 ? 4 : 1);    // the converting warps; the copies
+      mbar_init(&sm.full[i], FP8 ? 6 : 1);    // the converting warps; the copies
       mbar_init(&sm.empty[i], FP8 ? 1 : 2);   // the MMAs; they and the V cleaner
       mbar_init(&sm.v_clean[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.raw_full[i], 1);
-      mbar_init(&sm.raw_empty[i], 4);
+      mbar_init(&sm.raw_empty[i], 6);
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&sm.s_full[x], 1);
@@ -542,9 +542,9 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         if (lane == 0) mbar_arrive(&sm.empty[st]);
         if (++st == TCA_STAGES) st = 0, par ^= 1;
       }
-  } else if (FP8 && work && warp >= 12) {   // ---- e4m3 tiles to bf16 ones: value times row scale, rounded once ----
+  } else if (FP8 && work) {   // ---- warps 10 to 15: e4m3 tiles to bf16 ones: value times row scale, rounded once ----
     TcWalk<SRC> w(p, sm, step);
-    const int th = tid - 384;
+    const int th = tid - 320, ch = th & 7, half = ch >> 2;   // this thread's 16 dims, of every 24th row
     uint32_t it = 0;
     bool ok = true;
     for (; w.more() && ok; w.next())
@@ -556,24 +556,28 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         const int tail = w.s.len - (i >> 1) * TCA_KEYS;   // rows from here on were not loaded, or are not the sequence's
         const uint32_t src = smem_u32(sm.raw[FP8 ? rs : 0]), dst = smem_u32(sm.kv[st]);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {       // 16 bytes: 16 dims of a row, to two swizzled 16-byte chunks
-          const int id = k * 128 + th, row = id >> 3, ch = id & 7, half = ch >> 2;
-          const uint4 q = lds128_at(src + id * 16);
+        for (int k = 0; k < 6; ++k) {       // 8 bytes and 8 again: two swizzled 16-byte chunks of a row
+          const int row = k * 24 + (th >> 3);
+          if (row >= TCA_KEYS) break;
           const float s = row < tail ? sm.raw_scale[FP8 ? rs : 0][row] : 0.f;
-          uint32_t y[8];
-          const uint32_t words[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint32_t h = e4m3x2_to_f16x2(words[j >> 1] >> (16 * (j & 1)));
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-            y[j] = pack_bf16(f.x * s, f.y * s);
-          }
-          if (row >= tail) y[0] = y[1] = y[2] = y[3] = y[4] = y[5] = y[6] = y[7] = 0;
+          const uint64_t s2 = f32x2(s, s);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {     // the second half's lanes begin with their other chunk: no bank conflict
-            const int o = j ^ half, c16 = ((ch & 3) * 2 + o) ^ (row & 7);
-            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + half * (TCA_TILE / 2) + row * 128 + c16 * 16),
-                         "r"(o ? y[4] : y[0]), "r"(o ? y[5] : y[1]), "r"(o ? y[6] : y[2]), "r"(o ? y[7] : y[3])
+            const int o = j ^ half;
+            uint2 q;
+            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(q.x), "=r"(q.y) : "r"(src + row * HEAD_DIM + ch * 16 + o * 8));
+            uint32_t y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t h = e4m3x2_to_f16x2((i < 2 ? q.x : q.y) >> (16 * (i & 1)));
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+              const uint64_t z = mul2(f32x2(f.x, f.y), s2);
+              y[i] = pack_bf16(f32x2_lo(z), f32x2_hi(z));
+            }
+            if (row >= tail) y[0] = y[1] = y[2] = y[3] = 0;
+            const int c16 = ((ch & 3) * 2 + o) ^ (row & 7);
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + half * (TCA_TILE / 2) + row * 128 + c16 * 16), "r"(y[0]), "r"(y[1]),
+                         "r"(y[2]), "r"(y[3])
                          : "memory");
           }
         }
@@ -622,16 +626,17 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         const float mn = max_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3]);
         const uint64_t scale2 = f32x2(sl2, sl2);
         // The first half's exponentials are computed under the old maximum while the new one is found. It stands unless
-        // some row has none yet, or one that grew by more than TCA_LAZY, or a NaN.
+        // some row has none yet (all of them in the piece's first tile), or one that grew by more than TCA_LAZY, or a NaN.
         uint64_t sum[2] = {0, 0};
-        tca_exp<32>(v, v, scale2, f32x2(base, base), sum);
+        const bool early = t > w.t0;
+        if (early) tca_exp<32>(v, v, scale2, f32x2(base, base), sum);
         if (__any_sync(0xffffffffu, !((mn - m) * sl2 <= TCA_LAZY))) {
           const float f = m == -INFINITY ? 0.f : ex2((m - mn) * sl2);
           m = mn;
           l *= f;
           // an infinite maximum makes the row NaN, as inf - inf does
           base = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7fffffff) : -m * sl2;
-          if (t > w.t0) {                   // the products before this tile's scores are done: O is whole
+          if (early) {                      // the products before this tile's scores are done: O is whole
 #pragma unroll 1
             for (int i = 0; i < 8; ++i) {
               uint32_t o[16];
@@ -642,7 +647,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
               tca_st16(to + 16 * i, o);
             }
           }
-          load_s(0, 2);
+          if (early) load_s(0, 2);
           sum[0] = sum[1] = 0;
           tca_exp<32>(v, v, scale2, f32x2(base, base), sum);
         }
@@ -709,40 +714,39 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
             *reinterpret_cast<uint4*>(p.part + slot * 128 + (size_t)(8 * i + k / 4) * 512 + row * 4) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
         }
       }
-      __threadfence();
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (tid == 0) {
-        const int before = atomicAdd(p.counters + c_lo - 1, 1);
+      if (tid == 0) {                       // releases the CTA's stores (ordered before by the barrier), acquires the others'
+        const int before = add_acq_rel(p.counters + c_lo - 1, 1);
         sm.last = before == c_hi - c_lo + 1;
-        if (sm.last) {
-          __threadfence();
-          p.counters[c_lo - 1] = 0;
-        }
+        if (sm.last) p.counters[c_lo - 1] = 0;
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");
       const bool last = sm.last;
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (last && valid) {
-      float M = -INFINITY, L = 0.f;
-      auto slot_of = [&](int cc) { return ((size_t)(cc * 2 + (cc == c_lo - 1 ? 1 : 0)) * 2 + x) * 128; };
-      for (int cc = c_lo - 1; cc <= c_hi; ++cc) M = fmaxf(M, __ldcg(p.ml + (slot_of(cc) + row) * 2));
+        auto slot_of = [&](int cc) { return ((size_t)(cc * 2 + (cc == c_lo - 1 ? 1 : 0)) * 2 + x) * 128; };
+        float M = -INFINITY;
+#pragma unroll 4
+        for (int cc = c_lo - 1; cc <= c_hi; ++cc) M = fmaxf(M, __ldcg(p.ml + (slot_of(cc) + row) * 2));
 #pragma unroll 1
-      for (int col = 0; col < 128; col += 32) {
-        float o[32] = {};
-        L = 0.f;
-        for (int cc = c_lo - 1; cc <= c_hi; ++cc) {
-          const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ml + (slot_of(cc) + row) * 2));
-          if (ml.y == 0.f) continue;        // no key of the piece was visible (and its O may not have been written)
-          const float f = M == -INFINITY ? 1.f : ex2((ml.x - M) * sl2);
-          L += ml.y * f;
+        for (int col = 0; col < 128; col += 64) {   // 16 loads in flight a piece
+          float o[64] = {}, L = 0.f;
+          for (int cc = c_lo - 1; cc <= c_hi; ++cc) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ml + (slot_of(cc) + row) * 2));
+            float4 q[16];
 #pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            const float4 q = __ldcg(reinterpret_cast<const float4*>(p.part + slot_of(cc) * 128 + (size_t)((col + k) / 4) * 512 + row * 4));
-            o[k] += q.x * f, o[k + 1] += q.y * f, o[k + 2] += q.z * f, o[k + 3] += q.w * f;
+            for (int k = 0; k < 16; ++k) q[k] = __ldcg(reinterpret_cast<const float4*>(p.part + slot_of(cc) * 128 + (size_t)(col / 4 + k) * 512 + row * 4));
+            if (ml.y == 0.f) continue;      // no key of the piece was visible (and its O may not have been written)
+            const float f = M == -INFINITY ? 1.f : ex2((ml.x - M) * sl2);
+            L += ml.y * f;
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              o[4 * k] += q[k].x * f, o[4 * k + 1] += q[k].y * f, o[4 * k + 2] += q[k].z * f, o[4 * k + 3] += q[k].w * f;
           }
+          const float inv = L == 0.f ? 0.f : 1.f / L;
+          store(o, inv, col);
+          store(o + 32, inv, col + 32);
         }
-        store(o, L == 0.f ? 0.f : 1.f / L, col);
-      }
       }
       __syncwarp();
     }

@@ -249,9 +249,10 @@ int qk_paged_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
   if (rows <= 8) return fp8 ? launch_few<true, 1>(p, 1, args->workspace, st) : launch_few<false, 1>(p, 1, args->workspace, st);
   if (rows <= 16) return fp8 ? launch_few<true, 2>(p, 1, args->workspace, st) : launch_few<false, 2>(p, 1, args->workspace, st);
   if (rows <= 32) return fp8 ? launch_few<true, 4>(p, 1, args->workspace, st) : launch_few<false, 4>(p, 1, args->workspace, st);
-  // the sequences with up to 16 query rows per KV head (those that decode beside a chunk), then the others
-  if (int e = fp8 ? launch_few<true, 2>(p, 0, args->workspace, st) : launch_few<false, 2>(p, 0, args->workspace, st)) return e;
-  return fp8 ? launch_tc<SRC_PAGED_FP8>(p, 17, args->workspace, st) : launch_tc<SRC_PAGED>(p, 17, args->workspace, st);
+  // the sequences with up to 8 query rows per KV head (those that decode beside a chunk), then the others: the tensor-core
+  // kernel takes a few rows too, at the matrix unit's time for 128
+  if (int e = fp8 ? launch_few<true, 1>(p, 0, args->workspace, st) : launch_few<false, 1>(p, 0, args->workspace, st)) return e;
+  return fp8 ? launch_tc<SRC_PAGED_FP8>(p, 9, args->workspace, st) : launch_tc<SRC_PAGED>(p, 9, args->workspace, st);
 }
 
 int qk_packed_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
