@@ -139,6 +139,7 @@ def _raw_stream(dev: int) -> int:
 
 
 _E4M3 = (torch.float8_e4m3fn, torch.uint8)
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 # qk_paged_qkv_t, qk_paged_kv_read_t and qk_ragged_attention_t (the first 14 fields of each: qk_paged_cache_t)
 _QKV_ARGS, _READ_ARGS, _ATTENTION_ARGS = (struct.Struct(f) for f in ("7Q7q7Q8qd", "7Q7q3Q3q", "7Q7q5Q10qd"))
 
@@ -414,46 +415,43 @@ class DecodeOps:
         """Check the cache and the batch (lens None: none wanted); returns (B, n_kv, device index, the fields of
         qk_paged_cache_t)."""
         dev = k_pages.get_device()
-        shape = k_pages.shape
+        shape, dt = k_pages.shape, k_pages.dtype
         if len(shape) != 4 or shape != v_pages.shape or not (k_pages.is_contiguous() and v_pages.is_contiguous()):
             raise RuntimeError(f"{what}: k_pages and v_pages must be contiguous [pages, n_kv, page_size, 128]")
         pages, n_kv, page, hd = shape
-        dt = k_pages.dtype
-        fp8 = dt != torch.bfloat16
-        if hd != 128 or dt != v_pages.dtype or (fp8 and dt not in _E4M3):
+        if hd != 128 or v_pages.dtype is not dt or (dt is not _BF16 and dt not in _E4M3):
             raise RuntimeError(f"{what}: pages must be bf16, or e4m3 bytes (uint8 or float8_e4m3fn), 128 values per row")
-        ks = vs = 0
-        if fp8:
+        ks = vs = fp8 = 0
+        if dt is not _BF16:
             for s in (k_scale, v_scale):
-                if s is None or s.dtype != torch.float32 or s.shape != shape[:3] or not s.is_contiguous() or s.get_device() != dev:
+                if s is None or s.dtype is not _F32 or s.shape != shape[:3] or not s.is_contiguous() or s.get_device() != dev:
                     raise RuntimeError(f"{what}: an e4m3 cache needs contiguous fp32 k_scale and v_scale [pages, n_kv, page_size]")
-            ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
+            ks, vs, fp8 = k_scale.data_ptr(), v_scale.data_ptr(), 1
         elif k_scale is not None or v_scale is not None:
             raise RuntimeError(f"{what}: a bf16 cache has no row scales")
-        if cu.dtype != torch.int32 or block_table.dtype != torch.int32 or block_table.dim() != 2 or cu.dim() != 1 \
-                or not cu.is_contiguous():
+        if cu.dtype is not _I32 or block_table.dtype is not _I32 or block_table.dim() != 2 or cu.dim() != 1 or not cu.is_contiguous():
             raise RuntimeError(f"{what}: cu must be int32 [B+1] and block_table int32 [B, width]")
         B, width = block_table.shape
         stride, inner = block_table.stride()
         if inner != 1 and width > 1:
             raise RuntimeError(f"{what}: block_table rows must be contiguous")
-        if len(cu) != B + 1:
-            raise RuntimeError(f"{what}: cu has {len(cu)} entries for {B} sequences (B + 1 wanted)")
+        if cu.numel() != B + 1:
+            raise RuntimeError(f"{what}: cu has {cu.numel()} entries for {B} sequences (B + 1 wanted)")
         if dev < 0 or v_pages.get_device() != dev or cu.get_device() != dev or block_table.get_device() != dev:
             raise RuntimeError(f"{what}: every tensor must be on the same CUDA device")
         lens_ptr = 0
         if lens is not None:
-            if lens.dtype != torch.int32 or lens.shape != (B,) or lens.get_device() != dev or not lens.is_contiguous():
+            if lens.dtype is not _I32 or lens.dim() != 1 or lens.numel() != B or lens.get_device() != dev or not lens.is_contiguous():
                 raise RuntimeError(f"{what}: seq_lens must be int32 [{B}] on the cache's device")
             lens_ptr = lens.data_ptr()
         return B, n_kv, dev, (k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, cu.data_ptr(), lens_ptr, block_table.data_ptr(),
-                              B, n_kv, pages, page, width, max(stride, width), fp8)
+                              B, n_kv, pages, page, width, stride if stride > width else width, fp8)
 
     @staticmethod
     def _heads(what, name, t, dev):
         """(rows, heads, row stride, head stride) of a bf16 [rows, heads, 128] or [rows, heads * 128] tensor."""
         shape, strides = t.shape, t.stride()
-        if t.dtype == torch.bfloat16 and t.get_device() == dev and strides[-1] == 1:
+        if t.dtype is _BF16 and t.get_device() == dev and strides[-1] == 1:
             if len(shape) == 3 and shape[2] == 128:
                 return shape[0], shape[1], strides[0], strides[1]
             if len(shape) == 2 and shape[1] % 128 == 0:
@@ -473,7 +471,7 @@ class DecodeOps:
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError(f"{what}: pass workspace=attention_workspace(device), made before the capture")
                 ws = self._scratch[("ragged", dev, stream)] = self.attention_workspace(torch.device("cuda", dev))
-        elif ws.dtype != torch.uint8 or ws.get_device() != dev or not ws.is_contiguous():
+        elif ws.dtype is not torch.uint8 or ws.get_device() != dev or not ws.is_contiguous():
             raise RuntimeError(f"{what}: workspace must come from attention_workspace() on the call's device")
         return ws
 
@@ -551,7 +549,7 @@ class DecodeOps:
         stream = _raw_stream(dev)
         ws = self._workspace("paged_attention", workspace, dev, stream)
         st = self.lib.qk_paged_attention(_ATTENTION_ARGS.pack(*cache, q.data_ptr(), 0, 0, out.data_ptr(), ws.data_ptr(), T, n_q,
-                                                              max_q, q_row, q_head, 0, 0, o_row, o_head, len(ws), scale), stream)
+                                                              max_q, q_row, q_head, 0, 0, o_row, o_head, ws.numel(), scale), stream)
         if st:
             self._check(st, "paged_attention")
 
@@ -576,7 +574,7 @@ class DecodeOps:
         st = self.lib.qk_packed_attention(
             _ATTENTION_ARGS.pack(0, 0, 0, 0, cu.data_ptr(), 0, 0, B, kv[1], 0, 0, 0, 0, 0, q.data_ptr(), k.data_ptr(),
                                  v.data_ptr(), out.data_ptr(), ws.data_ptr(), T, n_q, max_q, q_row, q_head, kv[2], kv[3], o_row,
-                                 o_head, len(ws), scale), stream)
+                                 o_head, ws.numel(), scale), stream)
         if st:
             self._check(st, "packed_attention")
 
