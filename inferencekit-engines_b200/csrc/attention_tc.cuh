@@ -16,7 +16,7 @@
 //    the rescale becomes rare, and a tile's exponentials need not wait for its maximum.
 //  * Warps: 0-3 and 4-7 the softmax of the two tiles, 8 the loads (TMA, 128-byte swizzle, a ring of five 32 KB K and V
 //    tiles), 9 issues the MMAs (10 clears V rows past a sequence's end, 11 fills the
-//    warpgroup, which gives registers to the softmax): Q0 K0, Q1 K0, then per tile P0 V, Q0 K', P1 V, Q1 K', so that while one tile's softmax
+//    warpgroup, which gives registers to the softmax): Q0 K0, Q1 K0, then per tile P0 V, Q0 K', P1 V, Q1 K' (P in two parts, the first while the second is computed), so that while one tile's softmax
 //    runs, the matrix unit has the other's two products to do.
 //  * Work: (sequence, KV head, tile pair, key tile) in that order, dealt in equal contiguous ranges to the CTAs: causal
 //    rows and ragged lengths balance by themselves, and a few rows over a long context spread over every SM. A boundary
@@ -34,6 +34,7 @@ constexpr int TCA_KEYS = 128;             // keys of a tile
 constexpr int TCA_TILE = TCA_KEYS * HEAD_DIM * 2;   // 32 KB: two 64-dim halves of 128 rows x 128 B
 constexpr int TCA_MIN_PIECE = 4;          // tiles
 constexpr int TCA_UNIT_COST = 2;          // what a unit costs beside its key tiles (Q load, first scores, output), in tiles
+constexpr int TCA_FIRST = 6;              // 16-key steps of P handed over first, of 8 (one prompt of 8,192 tokens: 432 us; 443 with 4, 450 with 2)
 constexpr float TCA_LAZY = 32.f;          // log2 of the growth that a stale maximum may hide
 
 enum { SRC_PACKED = 0, SRC_PAGED = 1, SRC_PAGED_FP8 = 2 };
@@ -193,6 +194,11 @@ __device__ __forceinline__ void tca_st16(uint32_t taddr, const uint32_t* v) {
                "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(taddr)
                : "memory");
 }
+template <int N>
+__device__ __forceinline__ void tca_st(uint32_t taddr, const uint32_t* v) {   // N columns, 16, 32 or 48
+  if (N >= 32) tca_st32(taddr, v);
+  if (N & 16) tca_st16(taddr + (N & 32), v + (N & 32));
+}
 __device__ __forceinline__ void tca_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // P of 2 N scores: p = exp2(s * scale + base), bf16 pairs to out (which may be the scores' first half), sums to sum. The
@@ -208,6 +214,13 @@ __device__ __forceinline__ void tca_exp(const uint32_t* s, uint32_t* out, uint64
   }
 }
 
+// Nothing that uses these values moves before this point (a tcgen05.ld's registers are its own until the wait after it).
+__device__ __forceinline__ void tca_tie32(uint32_t* v) {
+  asm volatile("" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]),
+               "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]),
+               "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]),
+               "+r"(v[30]), "+r"(v[31]));
+}
 // One lane of a converged warp, the same one every time. The compiler knows it for a single lane (which `lane == 0` does
 // not tell it), so the MMAs' descriptors go straight to the uniform registers that they are taken from.
 __device__ __forceinline__ bool elect_one() {
@@ -290,6 +303,8 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x, n_kv = r.c.n_kv;
   const int step = 2 * (128 / r.group);   // tokens of a tile pair
   if (tid == 0) {
+    prefetch_map(&p.tm_q);
+    if (!FP8) prefetch_map(&p.tm_k), prefetch_map(&p.tm_v);
     mbar_init(&sm.q_full, 1);
     mbar_init(&sm.q_empty, 1);
     for (int i = 0; i < TCA_STAGES; ++i) {
@@ -507,7 +522,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
                 wait(&sm.p_full[x][hh], np[x] & 1);
                 if (!ok) break;
 #pragma unroll
-                for (int k = 4 * hh; k < 4 * hh + 4; ++k)
+                for (int k = hh ? TCA_FIRST : 0; k < (hh ? 8 : TCA_FIRST); ++k)
                   tca_mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * k, vd + k * (2048 >> 4), id_o, k > 0 || t > w.t0);
               }
               if (t + 1 == e[x]) tc_commit(&sm.o_full[x]);
@@ -613,6 +628,8 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
 #pragma unroll
           for (int i = from; i < to_; ++i) tca_ld32(ts + 32 * i, v + 32 * i);
           tc_wait_ld();
+#pragma unroll
+          for (int i = from; i < to_; ++i) tca_tie32(v + 32 * i);
           if (edge) {
 #pragma unroll
             for (int i = 32 * from; i < 32 * to_; ++i)
@@ -629,7 +646,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         // some row has none yet (all of them in the piece's first tile), or one that grew by more than TCA_LAZY, or a NaN.
         uint64_t sum[2] = {0, 0};
         const bool early = t > w.t0;
-        if (early) tca_exp<32>(v, v, scale2, f32x2(base, base), sum);
+        if (early) tca_exp<8 * TCA_FIRST>(v, v, scale2, f32x2(base, base), sum);
         if (__any_sync(0xffffffffu, !((mn - m) * sl2 <= TCA_LAZY))) {
           const float f = m == -INFINITY ? 0.f : ex2((m - mn) * sl2);
           m = mn;
@@ -647,9 +664,9 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
               tca_st16(to + 16 * i, o);
             }
           }
-          if (early) load_s(0, 2);
+          if (early) load_s(0, (TCA_FIRST + 1) / 2);
           sum[0] = sum[1] = 0;
-          tca_exp<32>(v, v, scale2, f32x2(base, base), sum);
+          tca_exp<8 * TCA_FIRST>(v, v, scale2, f32x2(base, base), sum);
         }
         auto hand_over = [&](int hh) {
           tca_wait_st();
@@ -657,10 +674,10 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.p_full[x][hh]);
         };
-        tca_st32(ts, v);
+        tca_st<8 * TCA_FIRST>(ts, v);
         hand_over(0);
-        tca_exp<32>(v + 64, v + 32, scale2, f32x2(base, base), sum);
-        tca_st32(ts + 32, v + 32);
+        tca_exp<64 - 8 * TCA_FIRST>(v + 16 * TCA_FIRST, v + 8 * TCA_FIRST, scale2, f32x2(base, base), sum);
+        tca_st<64 - 8 * TCA_FIRST>(ts + 8 * TCA_FIRST, v + 8 * TCA_FIRST);
         hand_over(1);
         l += (f32x2_lo(sum[0]) + f32x2_hi(sum[0])) + (f32x2_lo(sum[1]) + f32x2_hi(sum[1]));
       }
