@@ -8,7 +8,7 @@
 //    per SM, whatever the lengths are: a 32k context beside short ones leaves no SM idle. A unit (sequence, head)
 //    split between CTAs leaves fp32 partials (o, m, l); the CTA that completes the unit's count adds them in CTA
 //    order (the same bits every run).
-//  * A producer warp keeps a ring of 192 KB of tiles in flight: TMA boxes of one page's rows each, 128-byte
+//  * A producer warp keeps a ring of 128 KB of tiles in flight: TMA boxes of one page's rows each, 128-byte
 //    swizzle, so every shared-memory read below is free of bank conflicts.
 //  * Consumer warps take KW keys of a tile each and keep a running softmax and output registers of their own, so nothing
 //    waits on a neighbour until the piece ends. Products are warp-level MMAs with the keys as M: S^T = K Q^T and
@@ -25,7 +25,7 @@
 
 namespace qk {
 
-constexpr int FEW_RING = 196608;      // bytes of K and V in the ring
+constexpr int FEW_RING = 131072;      // bytes of K and V in the ring
 constexpr int FEW_MIN_TILES = 1;      // a CTA's least share (13 tiles of 8 heads: 8.4 us; 10.6 with 2, 11.6 with 4)
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -97,19 +97,36 @@ struct FewShape {
   // its stages' barriers, and a wait by parity cannot mistake one phase for the one two before it.
   static constexpr int S = FEW_RING / (2 * TILE) / GROUPS * GROUPS;
   static_assert(S >= GROUPS && S > 0, "every group needs a stage");
-  static constexpr int SUMS = 32 / ROWS;                 // warps that add up at a time
   static constexpr int THREADS = CW * 32 + 32;
 };
 template <bool FP8, int NT>
 struct FewSmem {
   using Sh = FewShape<FP8, NT>;
   uint8_t k[Sh::S][Sh::TILE], v[Sh::S][Sh::TILE];
-  float sum[Sh::SUMS][Sh::ROWS][HEAD_DIM + 4];   // the warps' outputs on their way to one
+  float sum[Sh::CW][Sh::ROWS][HEAD_DIM + 4];   // the warps' outputs on their way to one
   float ks[FP8 ? Sh::S : 1][Sh::KEYS], vs[FP8 ? Sh::S : 1][Sh::KEYS];
   float wm[Sh::CW][Sh::ROWS], wl[Sh::CW][Sh::ROWS];
   uint64_t full[Sh::S], empty[Sh::S];
   int last;
 };
+
+// mbar_wait in fewer instructions, for kernels with many waits in unrolled code (instructions that are not in the cache cost
+// a short call most): the clock and the error word are looked at every 256 polls, the limits are the same.
+__device__ __forceinline__ bool mbar_wait_small(uint64_t* bar, uint32_t parity, unsigned long long limit_ns = WAIT_LIMIT_NS) {
+  unsigned long long t0 = 0;
+#pragma unroll 1
+  for (uint32_t i = 1; !mbar_try_wait(bar, parity); ++i) {
+    if (i & 255) continue;
+    const unsigned long long now = globaltimer();
+    if (t0 == 0) t0 = now;
+    if (wait_failed()) return false;
+    if (now - t0 > limit_ns) {
+      atomicOr(&g_dev_error, DEVERR_MBAR_TIMEOUT);
+      return false;
+    }
+  }
+  return true;
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float r;
@@ -249,7 +266,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
           in = 0;
         }
         const int of_box = __shfl_sync(0xffffffffu, cur, in * boxes + lane % boxes), page = lane < boxes ? of_box : -1;
-        if (it >= S) ok = __all_sync(0xffffffffu, mbar_wait(&sm.empty[st], (uint32_t)((it / S - 1) & 1)));
+        if (it >= S) ok = __all_sync(0xffffffffu, mbar_wait_small(&sm.empty[st], (uint32_t)((it / S - 1) & 1)));
         if (!ok) break;
         const int nb = __popc(__ballot_sync(0xffffffffu, page >= 0));
         if (lane == 0) mbar_arrive_expect_tx(&sm.full[st], (uint32_t)(nb * RB) * (2 * bytes_row + (FP8 ? 8 : 0)));
@@ -277,7 +294,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
     if (ok)   // the last stages' copies are waited for by the consumers
       return;
     // a wait gave up: let the copies in flight land before the CTA's shared memory goes away
-    for (int i = max(0, it - S); i < it; ++i) mbar_wait(&sm.full[i % S], (uint32_t)((i / S) & 1), 1000000ull);
+    for (int i = max(0, it - S); i < it; ++i) mbar_wait_small(&sm.full[i % S], (uint32_t)((i / S) & 1), 1000000ull);
     return;
   }
 
@@ -346,7 +363,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
     for (int t = t0; t < t1; ++t, ++it) {
       if (GROUPS > 1 && it % GROUPS != grp) continue;
       const int st = it % S, j0 = t * FEW_KEYS + part * KW;
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(&sm.full[st], (uint32_t)((it / S) & 1)));
+      ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.full[st], (uint32_t)((it / S) & 1)));
       if (ok && j0 < s.len) {
         const uint32_t kb = smem_u32(sm.k[st]) + (part * KW) * 128, vb = smem_u32(sm.v[st]) + (part * KW) * 128;
         if (j0 + KW > s.len) {              // the sequence ends inside: what lies behind it must not reach P.V, as 0 x NaN
@@ -522,30 +539,24 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
         if (FP8) f[nt][e] *= pow2(ev) * (1.f / 32768.f);
       }
 #pragma unroll
-    for (int w = CW - Sh::SUMS; w >= 0; w -= Sh::SUMS) {   // SUMS warps at a time
-      if (warp >= w && warp < w + Sh::SUMS) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+      for (int i = 0; i < 8; ++i)
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int d = FP8 ? 16 * lg + 2 * i + (e >> 1) : 16 * i + 8 * (e >> 1) + lg;
-              float& x = sm.sum[warp - w][nt * 8 + 2 * lt + (e & 1)][d];
-              const float y = o[i][nt][e] * f[nt][e & 1];
-              x = w == CW - Sh::SUMS ? y : x + y;
-            }
-      }
-      few_sync(CW * 32);
-    }
+        for (int e = 0; e < 4; ++e) {
+          const int d = FP8 ? 16 * lg + 2 * i + (e >> 1) : 16 * i + 8 * (e >> 1) + lg;
+          sm.sum[warp][nt * 8 + 2 * lt + (e & 1)][d] = o[i][nt][e] * f[nt][e & 1];
+        }
+    few_sync(CW * 32);
     // thread: 8 dims of a row (16 threads a row)
     for (int i = tid; i < rows * 16; i += CW * 32) {
       const int row = i >> 4, d0 = (i & 15) * 8;
       float x[8] = {};
 #pragma unroll
-      for (int w = 0; w < Sh::SUMS; ++w)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] += sm.sum[w][row][d0 + e];
+      for (int w = 0; w < CW; ++w) {
+        const float4 a = *reinterpret_cast<const float4*>(&sm.sum[w][row][d0]), e = *reinterpret_cast<const float4*>(&sm.sum[w][row][d0 + 4]);
+        x[0] += a.x, x[1] += a.y, x[2] += a.z, x[3] += a.w, x[4] += e.x, x[5] += e.y, x[6] += e.z, x[7] += e.w;
+      }
       float M = -INFINITY, L = 0.f;
 #pragma unroll
       for (int w = 0; w < CW; ++w) M = fmaxf(M, sm.wm[w][row]);
@@ -573,7 +584,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
       }
       few_sync(CW * 32);
       if (sm.last) {                        // every piece is there: add them, Q threads a row and 8 dims, in a fixed order
-        const int T = CW * 32, items = rows * 16, Q = max(1, min(Sh::SUMS, T / items));
+        const int T = CW * 32, items = rows * 16, Q = max(1, min(CW, T / items));
         for (int i = tid; i < items * Q; i += T) {
           const int q = i / items, row = i / 16 % rows, d0 = (i & 15) * 8;
           auto at_of = [&](int cc) {        // the unit is CTA cc's first one, unless it begins inside the first owner's range

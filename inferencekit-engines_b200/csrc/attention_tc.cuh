@@ -73,23 +73,33 @@ __device__ __forceinline__ TcSeq tc_seq(const TcAttnParams& p, int b) {
   if (bad || s.n * r.group < p.min_rows) s.n = 0;
   return s;
 }
-// sum over i < n of floor((a i + b) / 128), a and b not negative
+// sum over i < n of floor((a i + b) / 128), a and b not negative (Euclid's scheme: the lattice points under a line)
 __host__ __device__ __forceinline__ long long floor_sum(unsigned n, unsigned a, unsigned b) {
   long long sum = 0;
   unsigned m = TCA_KEYS;
+#pragma unroll 1
   while (n) {
-    sum += (long long)n * (n - 1) / 2 * (a / m) + (long long)n * (b / m);
-    a %= m;
-    b %= m;
+    const unsigned qa = a / m, qb = b / m;
+    sum += (long long)n * (n - 1) / 2 * qa + (long long)n * qb;
+    a -= qa * m;
+    b -= qb * m;
     const unsigned long long y = (unsigned long long)a * n + b;
     if (y < m) break;
-    n = (unsigned)(y / m);
-    b = (unsigned)(y % m);
+    if (y >> 32) {                          // (64-bit divisions are several times slower)
+      n = (unsigned)(y / m);
+      b = (unsigned)(y % m);
+    } else {
+      n = (unsigned)y / m;
+      b = (unsigned)y - n * m;
+    }
     const unsigned t = m;
     m = a;
     a = t;
   }
   return sum;
+}
+__device__ __forceinline__ long long div_short(long long a, long long b) {   // both positive
+  return (a | b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
 }
 // The cost of a sequence's tile pairs: pair i covers tokens [i step, (i + 1) step) and the keys its last token sees, so
 // many tiles (one where it sees none: there still are rows to set to zero), and TCA_UNIT_COST.
@@ -327,13 +337,17 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
   grid_dep_wait();
   grid_dep_launch();
 
-  // ---- this CTA's range of key tiles (warp 0: sums over the sequences, 32 chunks of them) --------------------------
-  if (warp == 0) {
+  // ---- this CTA's range of key tiles: sums over the sequences, 32 chunks of them; warp 0 finds where it begins, warp 1
+  // where the next one does ---------------------------------------------------------------------------------------------
+  if (warp < 2) {
     const int per = (r.c.B + 31) / 32;
-    long long mine = 0;
+    long long mine = 0, tot = 0;
+    TcSeq s = {0, 0, 0};
     for (int b = lane * per; b < min(r.c.B, (lane + 1) * per); ++b) {
-      const TcPairs pr(tc_seq<SRC>(p, b), step);
-      if (pr.n) mine += pr.before(pr.n) * n_kv;
+      s = tc_seq<SRC>(p, b);
+      const TcPairs pr(s, step);
+      tot = pr.n ? pr.before(pr.n) : 0;
+      mine += tot * n_kv;
     }
     long long incl = mine;
 #pragma unroll
@@ -343,54 +357,59 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
     }
     const long long W = __shfl_sync(0xffffffffu, incl, 31);
     const int G = (int)min((long long)gridDim.x, max(1ll, W / TCA_MIN_PIECE));
-    for (int e = 0; e < 2; ++e) {           // both ends of the range
-      const int cc = min(c + e, G);
-      const long long u = cc * W / G;
-      int b = r.c.B, g = 0, pair = 0, t = 0;
-      long long at = W;
-      if (u < W) {
-        const unsigned who = __ballot_sync(0xffffffffu, incl > u);
-        const int first = __ffs(who) - 1;
-        at = __shfl_sync(0xffffffffu, incl - mine, first);
-        b = first * per;
-        TcPairs pr(tc_seq<SRC>(p, b), step);
-        long long tot = pr.n ? pr.before(pr.n) : 0;
-        while (u >= at + tot * n_kv) {
-          at += tot * n_kv;
-          pr = TcPairs(tc_seq<SRC>(p, ++b), step);
+    const long long u = div_short(min(c + warp, G) * W, G);
+    int b = r.c.B, g = 0, pair = 0, t = 0;
+    long long at = W;
+    if (u < W) {
+      const int first = __ffs(__ballot_sync(0xffffffffu, incl > u)) - 1;
+      at = __shfl_sync(0xffffffffu, incl - mine, first);
+      b = first * per;
+      if (per == 1) {                       // the lane's sequence is the one
+        s = {__shfl_sync(0xffffffffu, s.row0, first), __shfl_sync(0xffffffffu, s.n, first), __shfl_sync(0xffffffffu, s.len, first)};
+        tot = __shfl_sync(0xffffffffu, tot, first);
+      } else {
+        for (;; ++b) {
+          s = tc_seq<SRC>(p, b);
+          const TcPairs pr(s, step);
           tot = pr.n ? pr.before(pr.n) : 0;
+          if (u < at + tot * n_kv) break;
+          at += tot * n_kv;
         }
-        g = (int)((u - at) / tot);
-        at += g * tot;
-        int lo = 0, hi = pr.n;              // the pair: before(lo) <= u - at < before(hi)
-        while (hi - lo > 1) {
-          const int d = (hi - lo + 31) / 32, i = lo + (lane + 1) * d;
-          const bool le = i < hi && pr.before(i) <= u - at;
-          const int k = __popc(__ballot_sync(0xffffffffu, le));
-          lo += k * d;
-          hi = min(hi, lo + d);
-        }
-        pair = lo;
-        at += pr.before(pair);
-        t = (int)(u - at);                  // into the unit's cost: TCA_UNIT_COST, then its tiles
-        const int n = pr.cost(pair);
-        if (t < TCA_UNIT_COST + TCA_MIN_PIECE) t = 0;
-        else if (n - t < TCA_MIN_PIECE) {   // the range begins with the next unit
-          at += n;
-          t = 0;
-          if (++pair == pr.n) {
-            pair = 0;
-            if (++g == n_kv) {
-              g = 0;
-              do ++b;
-              while (b < r.c.B && tc_seq<SRC>(p, b).n == 0);
-            }
+      }
+      const TcPairs pr(s, step);
+      g = (int)div_short(u - at, tot);
+      at += g * tot;
+      int lo = 0, hi = pr.n;                // the pair: before(lo) <= u - at < before(hi)
+#pragma unroll 1
+      while (hi - lo > 1) {
+        const int d = (hi - lo + 31) / 32, i = lo + (lane + 1) * d;
+        const bool le = i < hi && pr.before(i) <= u - at;
+        const int k = __popc(__ballot_sync(0xffffffffu, le));
+        lo += k * d;
+        hi = min(hi, lo + d);
+      }
+      pair = lo;
+      at += pr.before(pair);
+      t = (int)(u - at);                    // into the unit's cost: TCA_UNIT_COST, then its tiles
+      const int n = pr.cost(pair);
+      if (t < TCA_UNIT_COST + TCA_MIN_PIECE) t = 0;
+      else if (n - t < TCA_MIN_PIECE) {     // the range begins with the next unit
+        at += n;
+        t = 0;
+        if (++pair == pr.n) {
+          pair = 0;
+          if (++g == n_kv) {
+            g = 0;
+            do ++b;
+            while (b < r.c.B && tc_seq<SRC>(p, b).n == 0);
           }
         }
       }
-      if (lane == 0) sm.at[e] = {b, g, pair, t, at + t};   // u and t count cost: key tile t - TCA_UNIT_COST
     }
-    if (lane == 0) sm.total = W;
+    if (lane == 0) {
+      sm.at[warp] = {b, g, pair, t, at + t};   // u and t count cost: key tile t - TCA_UNIT_COST
+      sm.total = W;
+    }
   }
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
@@ -414,7 +433,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
     int it = 0;
     bool ok = true;
     for (int unit = 0; w.more() && ok; w.next(), ++unit) {
-      if (unit) ok = __all_sync(0xffffffffu, mbar_wait(&sm.q_empty, (uint32_t)((unit - 1) & 1)));
+      if (unit) ok = __all_sync(0xffffffffu, mbar_wait_small(&sm.q_empty, (uint32_t)((unit - 1) & 1)));
       if (!ok) break;
       const bool two = w.tok0(1) < w.s.n;
       if (lane == 0) {
@@ -441,7 +460,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
           constexpr int N = FP8 ? 2 : TCA_STAGES;
           const int st = it % N;
           uint64_t* full = FP8 ? &sm.raw_full[st] : &sm.full[st];
-          if (it >= N) ok = __all_sync(0xffffffffu, mbar_wait(FP8 ? &sm.raw_empty[st] : &sm.empty[st], (uint32_t)((it / N - 1) & 1)));
+          if (it >= N) ok = __all_sync(0xffffffffu, mbar_wait_small(FP8 ? &sm.raw_empty[st] : &sm.empty[st], (uint32_t)((it / N - 1) & 1)));
           if (!ok) break;
           const CUtensorMap* tm = v ? &p.tm_v : &p.tm_k;
           if (SRC == SRC_PACKED) {
@@ -468,7 +487,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
     }
     if (!ok)   // a wait gave up: let the copies in flight land before the shared memory goes away
       for (int n = FP8 ? 2 : TCA_STAGES, i = max(0, it - n); i < it; ++i)
-        mbar_wait(FP8 ? &sm.raw_full[i % n] : &sm.full[i % n], (uint32_t)((i / n) & 1), 1000000ull);
+        mbar_wait_small(FP8 ? &sm.raw_full[i % n] : &sm.full[i % n], (uint32_t)((i / n) & 1), 1000000ull);
   } else if (work && warp == 9) {   // ---- MMA issue: one thread, nothing between the products but its waits ----
     if (elect_one()) {
       constexpr uint32_t id_s = tca_idesc(false), id_o = tca_idesc(true);
@@ -476,7 +495,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
       uint32_t st = 0, par = 0, np[2] = {0, 0}, clean = 0;   // st, par: the next tile's stage, its `full` parity; clean: v_clean's
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
-        ok = ok && mbar_wait(bar, parity);
+        ok = ok && mbar_wait_small(bar, parity);
         tc_fence_after();
       };
       auto take = [&]() {                   // the next K or V tile of the ring
@@ -544,7 +563,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
     bool ok = true;
     for (; w.more() && ok; w.next())
       for (int i = 2 * w.t0; i < 2 * w.t1 && ok; ++i) {   // every tile of the ring in turn, K and V
-        ok = __all_sync(0xffffffffu, mbar_wait(&sm.full[st], par));
+        ok = __all_sync(0xffffffffu, mbar_wait_small(&sm.full[st], par));
         const int tail = w.s.len - (i >> 1) * TCA_KEYS;
         if ((i & 1) && tail < TCA_KEYS) {
           const uint32_t va = smem_u32(sm.kv[st]);
@@ -565,8 +584,8 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
     for (; w.more() && ok; w.next())
       for (int i = 2 * w.t0; i < 2 * w.t1 && ok; ++i, ++it) {   // K and V in turn
         const uint32_t rs = it & 1, st = it % TCA_STAGES;
-        ok = mbar_wait(&sm.raw_full[rs], (it >> 1) & 1);
-        if (it >= TCA_STAGES) ok = ok && mbar_wait(&sm.empty[st], (it / TCA_STAGES - 1) & 1);
+        ok = mbar_wait_small(&sm.raw_full[rs], (it >> 1) & 1);
+        if (it >= TCA_STAGES) ok = ok && mbar_wait_small(&sm.empty[st], (it / TCA_STAGES - 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
         const int tail = w.s.len - (i >> 1) * TCA_KEYS;   // rows from here on were not loaded, or are not the sequence's
         const uint32_t src = smem_u32(sm.raw[FP8 ? rs : 0]), dst = smem_u32(sm.kv[st]);
@@ -619,7 +638,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
       const int first = w.s.len - w.s.n + w.tok0(x);   // the last key that the tile's first row sees
       float m = -INFINITY, l = 0.f, base = 0.f;   // base = -m * sl2
       for (int t = w.t0; t < e; ++t) {
-        ok = __all_sync(0xffffffffu, ok && mbar_wait(&sm.s_full[x], (uint32_t)(ns++ & 1)));
+        ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.s_full[x], (uint32_t)(ns++ & 1)));
         tc_fence_after();
         uint32_t v[128];
         const int lim = t * TCA_KEYS + TCA_KEYS - 1 > first ? min(pos, w.s.len - 1) - t * TCA_KEYS : TCA_KEYS;
@@ -685,7 +704,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
       // ---- the piece's end: the output rows, or a partial --------------------------------------------------------
       const bool any = e > w.t0;
       if (any) {
-        ok = __all_sync(0xffffffffu, ok && mbar_wait(&sm.o_full[x], (uint32_t)(no++ & 1)));
+        ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.o_full[x], (uint32_t)(no++ & 1)));
         tc_fence_after();
       }
       bf16* dst = r.out + (long long)(w.s.row0 + tok) * r.out_row + (long long)(w.g * r.group + row % r.group) * r.out_head;
@@ -701,14 +720,17 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
       if (w.t0 == 0 && w.t1 == w.n) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
         if (any) {
+          uint32_t o[128];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t o[32];
-            tca_ld32(to + 32 * i, o);
-            tc_wait_ld();
-            if (valid) store(reinterpret_cast<const float*>(o), inv, 32 * i);
-            __syncwarp();
+          for (int i = 0; i < 4; ++i) tca_ld32(to + 32 * i, o + 32 * i);
+          tc_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tca_tie32(o + 32 * i);
+          if (valid) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) store(reinterpret_cast<const float*>(o + 32 * i), inv, 32 * i);
           }
+          __syncwarp();
         }
         continue;
       }
@@ -716,8 +738,8 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
       // c_lo + i - 1's first (slot 0)
       const long long a0 = w.u - w.t0 - (w.t0 ? TCA_UNIT_COST : 0);
       const int G = (int)min((long long)gridDim.x, max(1ll, W / TCA_MIN_PIECE));
-      const int c_lo = (int)(((a0 + TCA_UNIT_COST + TCA_MIN_PIECE) * G + W - 1) / W);
-      const int c_hi = (int)(((a0 + TCA_UNIT_COST + w.n - TCA_MIN_PIECE + 1) * G + W - 1) / W) - 1;
+      const int c_lo = (int)div_short((a0 + TCA_UNIT_COST + TCA_MIN_PIECE) * G + W - 1, W);
+      const int c_hi = (int)div_short((a0 + TCA_UNIT_COST + w.n - TCA_MIN_PIECE + 1) * G + W - 1, W) - 1;
       const size_t slot = ((size_t)(c * 2 + (w.t0 == 0 ? 1 : 0)) * 2 + x) * 128;
       *reinterpret_cast<float2*>(p.ml + (slot + row) * 2) = make_float2(m, l);
       if (any) {
