@@ -78,19 +78,11 @@ __device__ __forceinline__ int few_tiles(const FewSeq& s) {
 // NT: 8-row tiles of query rows (1, 2 or 4).
 template <bool FP8, int NT>
 struct FewShape {
-#ifndef FEW_CW
-#define FEW_CW (NT <= 2 ? 8 : 4)
-#endif
-#ifndef FEW_KW
-#define FEW_KW (FP8 || NT == 1 ? 32 : 16)
-#endif
-#ifndef FEW_K8
-#define FEW_K8 128
-#endif
   static constexpr int ROWS = 8 * NT;
-  static constexpr int KEYS = FP8 ? FEW_K8 : 64;            // keys of a tile
-  static constexpr int CW = FEW_CW;                      // consumer warps
-  static constexpr int KW = FEW_KW;                      // keys of a tile that a warp takes
+  static constexpr int KEYS = FP8 ? 128 : 64;            // keys of a tile: 16 KB of K (and of V) either way; e4m3 tiles
+                                                         // of 64 keys cost the loading warp its pace (102 us against 88)
+  static constexpr int CW = NT <= 2 ? 8 : 4;             // consumer warps (their registers: 64 NT for O and q)
+  static constexpr int KW = FP8 || NT == 1 ? 32 : 16;    // keys of a tile that a warp takes (bf16, 16 rows: 16 leaves no spills)
   static constexpr int GROUPS = CW * KW / KEYS;      // groups of warps, a tile each in turn
   static constexpr int TILE = KEYS * HEAD_DIM * (FP8 ? 1 : 2);
   // Stages: a multiple of GROUPS, so that tile i and stage i % S belong to the same group: a group meets every phase of
@@ -181,8 +173,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
   using Sh = FewShape<FP8, NT>;
   using Smem = FewSmem<FP8, NT>;
   constexpr int ROWS = Sh::ROWS, CW = Sh::CW, KW = Sh::KW, GROUPS = Sh::GROUPS, S = Sh::S, TILE = Sh::TILE;
-  constexpr int FEW_KEYS = Sh::KEYS;
-  constexpr int KT = KW / 16;               // 16-key tiles of M that a warp takes
+  constexpr int KEYS = Sh::KEYS, KT = KW / 16;   // 16-key tiles of M that a warp takes
   extern __shared__ __align__(1024) uint8_t few_smem[];
   Smem& sm = *reinterpret_cast<Smem*>(few_smem);
   const RaggedParams& r = p.r;
@@ -193,7 +184,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
     prefetch_map(&p.tm_v);
     for (int s = 0; s < S; ++s) {
       mbar_init(&sm.full[s], 1);
-      mbar_init(&sm.empty[s], FEW_KEYS / KW);
+      mbar_init(&sm.empty[s], KEYS / KW);
     }
     fence_mbar_init();
   }
@@ -206,7 +197,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
   FewSeq s = {0, 0, 0};
   for (int i = lane * per; i < min(r.c.B, (lane + 1) * per); ++i) {
     s = few_seq<ROWS>(r, i, p.strict);
-    mine += (long long)few_tiles<FEW_KEYS>(s) * n_kv;
+    mine += (long long)few_tiles<KEYS>(s) * n_kv;
   }
   long long incl = mine;
 #pragma unroll
@@ -226,7 +217,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
   } else {
     for (;; ++b) {
       s = few_seq<ROWS>(r, b, 0);
-      const long long tiles = (long long)few_tiles<FEW_KEYS>(s) * n_kv;
+      const long long tiles = (long long)few_tiles<KEYS>(s) * n_kv;
       if (u0 < start + tiles) break;
       start += tiles;
     }
@@ -234,12 +225,12 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
   __syncthreads();                          // the barriers are initialised
 
   // Every warp walks the same pieces: b, its tiles per head, the head, the tiles [t0, t1) of the head.
-  int n = few_tiles<FEW_KEYS>(s);
+  int n = few_tiles<KEYS>(s);
   int g = (int)((u0 - start) / n), t0 = (int)((u0 - start) - (long long)g * n);
   const uint32_t bytes_row = FP8 ? HEAD_DIM : 2 * HEAD_DIM;
 
   if (warp == CW) {   // ---- producer ----
-    const int RB = min(1 << r.c.page_shift, FEW_KEYS), boxes = FEW_KEYS / RB;
+    const int RB = min(1 << r.c.page_shift, KEYS), boxes = KEYS / RB;
     int it = 0;
     bool ok = true;
     for (long long u = u0; u < u1 && ok;) {
@@ -248,7 +239,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
       // tile's whole share of HBM's time
       const int batch = 32 / boxes;
       auto pages_of = [&](int t) {          // lane: box lane % boxes of tile t + lane / boxes; -1 where it holds no key
-        const int tile = t + lane / boxes, j = tile * FEW_KEYS + (lane % boxes) * RB;
+        const int tile = t + lane / boxes, j = tile * KEYS + (lane % boxes) * RB;
         if (tile >= t1 || j >= s.len) return -1;
         int pg = __ldg(r.c.table + (size_t)b * r.c.table_stride + (j >> r.c.page_shift));
         if (pg < 0 || pg >= r.c.n_pages) {
@@ -272,7 +263,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
         if (lane == 0) mbar_arrive_expect_tx(&sm.full[st], (uint32_t)(nb * RB) * (2 * bytes_row + (FP8 ? 8 : 0)));
         __syncwarp();
         if (page >= 0) {
-          const int row = ((page * n_kv + g) << r.c.page_shift) + ((t * FEW_KEYS + lane * RB) & ((1 << r.c.page_shift) - 1));
+          const int row = ((page * n_kv + g) << r.c.page_shift) + ((t * KEYS + lane * RB) & ((1 << r.c.page_shift) - 1));
           uint8_t *kd = sm.k[st] + lane * RB * 128, *vd = sm.v[st] + lane * RB * 128;
           tma_load_2d(kd, &p.tm_k, 0, row, &sm.full[st]);
           if (!FP8) tma_load_2d(kd + TILE / 2, &p.tm_k, 64, row, &sm.full[st]);
@@ -287,8 +278,8 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
       if (u < u1 && ++g == n_kv) {
         g = 0;
         do s = few_seq<ROWS>(r, ++b, 0);
-        while (few_tiles<FEW_KEYS>(s) == 0);
-        n = few_tiles<FEW_KEYS>(s);
+        while (few_tiles<KEYS>(s) == 0);
+        n = few_tiles<KEYS>(s);
       }
     }
     if (ok)   // the last stages' copies are waited for by the consumers
@@ -299,7 +290,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
   }
 
   // ---- consumers ----
-  const int grp = warp / (FEW_KEYS / KW), part = warp % (FEW_KEYS / KW), lg = lane >> 2, lt = lane & 3;
+  const int grp = warp / (KEYS / KW), part = warp % (KEYS / KW), lg = lane >> 2, lt = lane & 3;
   const float sl2 = r.scale * LOG2E;
   bool ok = true;
   int it = 0;
@@ -362,7 +353,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
     }
     for (int t = t0; t < t1; ++t, ++it) {
       if (GROUPS > 1 && it % GROUPS != grp) continue;
-      const int st = it % S, j0 = t * FEW_KEYS + part * KW;
+      const int st = it % S, j0 = t * KEYS + part * KW;
       ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.full[st], (uint32_t)((it / S) & 1)));
       if (ok && j0 < s.len) {
         const uint32_t kb = smem_u32(sm.k[st]) + (part * KW) * 128, vb = smem_u32(sm.v[st]) + (part * KW) * 128;
@@ -412,7 +403,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
             for (int hh = 0; hh < 2; ++hh) {
               const int key = part * KW + 16 * j + 8 * hh + lg;
               kscale[j][hh] = sm.ks[st][key];
-              vscale[j][hh] = t * FEW_KEYS + key < s.len ? sm.vs[st][key] : 0.f;
+              vscale[j][hh] = t * KEYS + key < s.len ? sm.vs[st][key] : 0.f;
               vmax = fmaxf(vmax, vscale[j][hh]);
             }
 #pragma unroll
@@ -632,8 +623,8 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
     if (u < u1 && ++g == n_kv) {
       g = 0;
       do s = few_seq<ROWS>(r, ++b, 0);
-      while (few_tiles<FEW_KEYS>(s) == 0);
-      n = few_tiles<FEW_KEYS>(s);
+      while (few_tiles<KEYS>(s) == 0);
+      n = few_tiles<KEYS>(s);
     }
   }
   if (!ok && lane == 0) atomicOr(&g_dev_error, DEVERR_MBAR_TIMEOUT);

@@ -20,7 +20,7 @@
 //    runs, the matrix unit has the other's two products to do.
 //  * Work: (sequence, KV head, tile pair, key tile) in that order, dealt in equal contiguous ranges to the CTAs: causal
 //    rows and ragged lengths balance by themselves, and a few rows over a long context spread over every SM. A boundary
-//    nearer than TC_MIN_PIECE tiles to the end of a unit moves there. Units cut by one leave fp32 partials (O, m, l) per
+//    nearer than TCA_MIN_PIECE tiles to the end of a unit moves there. Units cut by one leave fp32 partials (O, m, l) per
 //    piece; the CTA that completes the unit's count adds them in order.
 //  * An e4m3 cache: the loads bring raw tiles and their row scales, and six more warps write them as bf16 tiles in the
 //    image the MMAs read: value times scale, rounded to bf16. That rounding (2^-9 relative, independent from value to
@@ -47,6 +47,7 @@ struct TcAttnParams {
   float* ml;                // [grid][2][2 tiles][128 rows][2]
   int* counters;            // [grid], zero between launches
   int min_rows;             // sequences with fewer query rows per KV head are another kernel's
+  int after_few;            // launched behind the few-row kernel of the same call, which it need not wait for
 };
 
 struct TcSeq {
@@ -168,10 +169,6 @@ __device__ __forceinline__ void tca_mma_ts(uint32_t d, uint32_t a, uint64_t b, u
       "r"(a), "l"(b), "r"(idesc), "r"(accum), "r"(0)
       : "memory");
 }
-#define QK_R32(r, o)                                                                                                     \
-  r[o], r[o + 1], r[o + 2], r[o + 3], r[o + 4], r[o + 5], r[o + 6], r[o + 7], r[o + 8], r[o + 9], r[o + 10], r[o + 11],  \
-      r[o + 12], r[o + 13], r[o + 14], r[o + 15], r[o + 16], r[o + 17], r[o + 18], r[o + 19], r[o + 20], r[o + 21],      \
-      r[o + 22], r[o + 23], r[o + 24], r[o + 25], r[o + 26], r[o + 27], r[o + 28], r[o + 29], r[o + 30], r[o + 31]
 // 32 consecutive 32-bit columns of this warp's 32 TMEM lanes, one lane a thread
 __device__ __forceinline__ void tca_ld32(uint32_t taddr, uint32_t* v) {
   asm volatile(
@@ -334,7 +331,10 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
     }
     fence_mbar_init();
   }
-  grid_dep_wait();
+  // Behind the few-row kernel: that one let this one start after its own wait, so what came before both is complete, and
+  // the two share neither rows nor scratch. CTAs take the SMs as the other's leave them; this kernel waits for the other
+  // at its end, so that whatever follows it follows both.
+  if (!p.after_few) grid_dep_wait();
   grid_dep_launch();
 
   // ---- this CTA's range of key tiles: sums over the sequences, 32 chunks of them; warp 0 finds where it begins, warp 1
@@ -666,12 +666,16 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         uint64_t sum[2] = {0, 0};
         const bool early = t > w.t0;
         if (early) tca_exp<8 * TCA_FIRST>(v, v, scale2, f32x2(base, base), sum);
-        if (__any_sync(0xffffffffu, !((mn - m) * sl2 <= TCA_LAZY))) {
-          const float f = m == -INFINITY ? 0.f : ex2((m - mn) * sl2);
-          m = mn;
-          l *= f;
-          // an infinite maximum makes the row NaN, as inf - inf does
-          base = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7fffffff) : -m * sl2;
+        const bool grow = valid && !((mn - m) * sl2 <= TCA_LAZY);
+        if (__any_sync(0xffffffffu, grow)) {   // (each row by its own scores: neighbours, and rows that are none, change nothing)
+          float f = 1.f;
+          if (grow) {
+            f = m == -INFINITY ? 0.f : ex2((m - mn) * sl2);
+            m = mn;
+            l *= f;
+            // an infinite maximum makes the row NaN, as inf - inf does
+            base = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7fffffff) : -m * sl2;
+          }
           if (early) {                      // the products before this tile's scores are done: O is whole
 #pragma unroll 1
             for (int i = 0; i < 8; ++i) {
@@ -792,6 +796,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
     if (!ok && lane == 0) atomicOr(&g_dev_error, DEVERR_MBAR_TIMEOUT);
   }
   }
+  if (p.after_few) grid_dep_wait();
   tc_fence_before();
   __syncthreads();
   if (warp == 9) {

@@ -83,13 +83,13 @@ int encode_pool_map(CUtensorMap* map, const void* pool, long long rows, bool fp8
   return QK_OK;
 }
 
-// The attention workspace: each kernel's counters, then partial sums and their (m, l) pairs, two a CTA, which the two
-// kernels of a call use one after the other.
+// The attention workspace: counters, partial sums and their (m, l) pairs, two a CTA, of each kernel (the two of a call
+// overlap).
 constexpr int RAGGED_MAX_CTAS = 160;
 struct RaggedWorkspace {
   int few_counters[256], tc_counters[256];
-  float ml[RAGGED_MAX_CTAS * 2 * 256 * 2];
-  float part[RAGGED_MAX_CTAS * 2 * 256 * HEAD_DIM];
+  float few_ml[RAGGED_MAX_CTAS * 2 * 32 * 2], tc_ml[RAGGED_MAX_CTAS * 2 * 256 * 2];
+  float few_part[RAGGED_MAX_CTAS * 2 * 32 * HEAD_DIM], tc_part[RAGGED_MAX_CTAS * 2 * 256 * HEAD_DIM];
 };
 
 template <bool FP8, int NT>
@@ -101,8 +101,8 @@ int launch_few(const RaggedParams& r, int strict, void* workspace, cudaStream_t 
   if (int e = encode_pool_map(&p.tm_v, r.c.v, rows, FP8, box)) return e;
   RaggedWorkspace* ws = static_cast<RaggedWorkspace*>(workspace);
   p.r = r;
-  p.part = ws->part;
-  p.ml = ws->ml;
+  p.part = ws->few_part;
+  p.ml = ws->few_ml;
   p.counters = ws->few_counters;
   p.strict = strict;
   auto k = few_attention_kernel<FP8, NT>;
@@ -129,7 +129,7 @@ int encode_rows_map(CUtensorMap* map, const void* base, int heads, int T, long l
 }
 
 template <int SRC>
-int launch_tc(const RaggedParams& r, int min_rows, void* workspace, cudaStream_t stream) {
+int launch_tc(const RaggedParams& r, int min_rows, bool after_few, void* workspace, cudaStream_t stream) {
   TcAttnParams p = {};
   if (int e = encode_rows_map(&p.tm_q, r.q, r.n_q, r.T, r.q_head, r.q_row, r.group, 128 / r.group)) return e;
   if (SRC == SRC_PACKED) {
@@ -145,14 +145,15 @@ int launch_tc(const RaggedParams& r, int min_rows, void* workspace, cudaStream_t
   }
   RaggedWorkspace* ws = static_cast<RaggedWorkspace*>(workspace);
   p.r = r;
-  p.part = ws->part;
-  p.ml = ws->ml;
+  p.part = ws->tc_part;
+  p.ml = ws->tc_ml;
   p.counters = ws->tc_counters;
   p.min_rows = min_rows;
+  p.after_few = after_few;
   auto k = tc_attention_kernel<SRC>;
   const int smem = (int)sizeof(TcAttnSmem<SRC>);
   if (int e = ensure_smem((const void*)k, smem)) return e;
-  return launch(k, dim3(std::min(device_sms(), RAGGED_MAX_CTAS)), dim3(TcShape<SRC>::THREADS), smem, stream, p);
+  return launch_as(after_few || g_pdl, k, dim3(std::min(device_sms(), RAGGED_MAX_CTAS)), dim3(TcShape<SRC>::THREADS), smem, stream, p);
 }
 
 int warp_grid(long long warps, dim3* grid) {   // 8 warps a CTA
@@ -252,7 +253,7 @@ int qk_paged_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
   // the sequences with up to 8 query rows per KV head (those that decode beside a chunk), then the others: the tensor-core
   // kernel takes a few rows too, at the matrix unit's time for 128
   if (int e = fp8 ? launch_few<true, 1>(p, 0, args->workspace, st) : launch_few<false, 1>(p, 0, args->workspace, st)) return e;
-  return fp8 ? launch_tc<SRC_PAGED_FP8>(p, 9, args->workspace, st) : launch_tc<SRC_PAGED>(p, 9, args->workspace, st);
+  return fp8 ? launch_tc<SRC_PAGED_FP8>(p, 9, true, args->workspace, st) : launch_tc<SRC_PAGED>(p, 9, true, args->workspace, st);
 }
 
 int qk_packed_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
@@ -272,7 +273,7 @@ int qk_packed_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
   p.c.cu = a.cache.cu_rows;
   p.c.B = (int)a.cache.batch;
   p.c.n_kv = (int)a.cache.n_kv;
-  return launch_tc<SRC_PACKED>(p, 0, args->workspace, static_cast<cudaStream_t>(stream));
+  return launch_tc<SRC_PACKED>(p, 0, false, args->workspace, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

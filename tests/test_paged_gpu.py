@@ -128,6 +128,7 @@ PAGED = {
     "group_32": ([1, 2, 20], [129, 640, 100], 32, 1, 64),
     "long": ([1, 20], [20000, 9000], 8, 2, 64),
     "many": ([1] * 100 + [3] * 40, list(range(1, 141)), 4, 1, 16),
+    "many_mixed": ([1, 30, 0] * 15, [40 + 37 * i for i in range(45)], 8, 2, 16),
 }
 
 
@@ -157,7 +158,7 @@ def test_paged_attention(name, fp8):
 
 
 @pytest.mark.parametrize("lens", [[1], [127], [128], [129], [300], [1, 1, 1], [5, 0, 64, 65], [0, 0, 7], [513, 31, 256],
-                                  [2000, 1, 77]], ids=str)
+                                  [2000, 1, 77], list(range(0, 71))], ids=str)
 @pytest.mark.parametrize("heads", [(32, 8), (8, 8), (12, 4), (10, 2), (28, 4), (16, 1)], ids=str)
 def test_packed_attention(lens, heads):
     n_q, n_kv = heads
@@ -234,6 +235,29 @@ def test_rising_scores_rescale_the_sums():
         out = torch.empty_like(q)
         k.paged_attention(q, ints([0, n]), ints([L]), c["table"], c["k"], c["v"], out, D ** -0.5, n)
         check_attention(out, *attend64(q.double(), K.double(), rows[0][1], L - n, D ** -0.5), False)
+
+
+@pytest.mark.parametrize("group", [3, 4])
+def test_a_row_depends_on_its_own_tokens_only(group):
+    """The same prompt and chunk beside neighbours of ordinary, huge and NaN values: the same bits."""
+    k = ops()
+    g = torch.Generator(device=DEV).manual_seed(group)
+    n_kv, n = 2, 50
+    q, kk, v = (torch.randn(n, h, D, generator=g, device=DEV).to(torch.bfloat16) for h in (n_kv * group, n_kv, n_kv))
+    c, _ = make_cache([n + 400], n_kv, 16, False, g)
+    seen = []
+    for other in (1.0, 1e4, math.nan):
+        def beside(x):
+            return torch.cat([x, torch.randn(n, x.shape[1], D, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).to(torch.bfloat16) * other])
+        qb, kb, vb = beside(q), beside(kk), beside(v)
+        a, b = torch.empty_like(qb), torch.empty_like(qb)
+        k.packed_attention(qb, kb, vb, ints([0, n, 2 * n]), a, D ** -0.5, n)
+        table = c["table"].expand(2, -1).contiguous()
+        k.paged_attention(qb, ints([0, n, 2 * n]), ints([n + 400, 300]), table, c["k"], c["v"], b, D ** -0.5, n)
+        seen.append((a[:n].clone(), b[:n].clone()))
+    for a, b in seen[1:]:
+        assert torch.equal(a.view(torch.int16), seen[0][0].view(torch.int16)) and torch.equal(b.view(torch.int16), seen[0][1].view(torch.int16))
+    assert k.device_error() == 0
 
 
 @pytest.mark.parametrize("n", [1, 64])
