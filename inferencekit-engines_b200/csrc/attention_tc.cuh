@@ -22,9 +22,10 @@
 //    rows and ragged lengths balance by themselves, and a few rows over a long context spread over every SM. A boundary
 //    nearer than TCA_MIN_PIECE tiles to the end of a unit moves there. Units cut by one leave fp32 partials (O, m, l) per
 //    piece; the CTA that completes the unit's count adds them in order.
-//  * An e4m3 cache: the loads bring raw tiles and their row scales, and six more warps write them as bf16 tiles in the
-//    image the MMAs read: value times scale, rounded to bf16. That rounding (2^-9 relative, independent from value to
-//    value) is what a bf16 cache has too; exact scales would cost each softmax thread 256 loads and multiplies a tile.
+//  * An e4m3 cache: the loads bring raw tiles, and six more warps write them as bf16 tiles in the image the MMAs read: the
+//    e4m3 values, exactly. The softmax multiplies each score by its key's K scale and each P by its V scale (packed
+//    multiplications and broadcast loads). Folding the scales into the tiles, rounded to bf16, was a fifth faster and
+//    twice as far off (3.4e-3 against 1.7e-3 for fp32 sums rounded once).
 #pragma once
 #include "attention_few.cuh"
 
@@ -130,7 +131,10 @@ struct TcAttnSmem {
   uint8_t q[2][TCA_TILE];
   uint8_t kv[S][TCA_TILE];
   uint8_t raw[RAW ? RAW : 1][RAW ? TCA_KEYS * HEAD_DIM : 16];
-  float raw_scale[RAW ? RAW : 1][RAW ? TCA_KEYS : 4];
+  // scale * log2 e times the K scales of a key tile, and the V scales, for the softmax. Three tiles of K's: tile j + 3 is
+  // converted into the stage of tile j + 1, which is free once both query tiles' scores of j + 1 are done, behind their
+  // P V of j. Two of V's: tile j + 2 goes into the stage of tile j, free after its P V.
+  float k_scale[RAW ? 3 : 1][RAW ? TCA_KEYS : 4], v_scale[RAW ? 2 : 1][RAW ? TCA_KEYS : 4];
   long long total;
   TcPlace at[2];
   uint64_t q_full, q_empty, full[S], empty[S], raw_full[2], raw_empty[2];
@@ -210,13 +214,19 @@ __device__ __forceinline__ void tca_wait_st() { asm volatile("tcgen05.wait::st.s
 
 // P of 2 N scores: p = exp2(s * scale + base), bf16 pairs to out (which may be the scores' first half), sums to sum. The
 // packed instructions halve the issue slots beside the exponential unit, which is what bounds this.
-template <int N>
-__device__ __forceinline__ void tca_exp(const uint32_t* s, uint32_t* out, uint64_t scale, uint64_t base, uint64_t (&sum)[2]) {
+// With vs, P goes times the keys' V scales (l does not).
+template <int N, bool VS>
+__device__ __forceinline__ void tca_exp(const uint32_t* s, uint32_t* out, uint64_t scale, uint64_t base, uint64_t (&sum)[2], const float* vs) {
+  float4 v4;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     uint64_t x = fma2(f32x2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale, base);
     x = f32x2(ex2(f32x2_lo(x)), ex2(f32x2_hi(x)));
     sum[i & 1] = add2(sum[i & 1], x);
+    if (VS) {
+      if (i % 2 == 0) v4 = *reinterpret_cast<const float4*>(vs + 2 * i);
+      x = mul2(x, i % 2 == 0 ? f32x2(v4.x, v4.y) : f32x2(v4.z, v4.w));
+    }
     out[i] = pack_bf16(f32x2_lo(x), f32x2_hi(x));
   }
 }
@@ -470,13 +480,12 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
             }
           } else {
             const int nb = __popc(__ballot_sync(0xffffffffu, page >= 0));
-            if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(nb * RB) * (FP8 ? HEAD_DIM + 4 : 2 * HEAD_DIM));
+            if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(nb * RB) * (FP8 ? HEAD_DIM : 2 * HEAD_DIM));
             __syncwarp();
             if (page >= 0) {
               const int row = ((page * n_kv + w.g) << r.c.page_shift) + ((t * TCA_KEYS + lane * RB) & ((1 << r.c.page_shift) - 1));
-              if (FP8) {                    // a page's rows of a head and their scales are contiguous
+              if (FP8) {                    // a page's rows of a head are contiguous
                 bulk_g2s(sm.raw[FP8 ? st : 0] + lane * RB * HEAD_DIM, (v ? r.c.v : r.c.k) + (size_t)row * HEAD_DIM, RB * HEAD_DIM, full);
-                bulk_g2s(&sm.raw_scale[FP8 ? st : 0][lane * RB], (v ? r.c.vs : r.c.ks) + row, RB * 4, full);
               } else {
                 for (int h = 0; h < 2; ++h) tma_load_2d(sm.kv[st] + h * (TCA_TILE / 2) + lane * RB * 128, tm, 64 * h, row, full);
               }
@@ -576,25 +585,43 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         if (lane == 0) mbar_arrive(&sm.empty[st]);
         if (++st == TCA_STAGES) st = 0, par ^= 1;
       }
-  } else if (FP8 && work) {   // ---- warps 10 to 15: e4m3 tiles to bf16 ones: value times row scale, rounded once ----
+  } else if (FP8 && work) {   // ---- warps 10 to 15: e4m3 tiles to bf16 ones (exact), and their rows' scales ----
     TcWalk<SRC> w(p, sm, step);
     const int th = tid - 320, ch = th & 7, half = ch >> 2;   // this thread's 16 dims, of every 24th row
+    // the scales of key th of tile t: fetched a tile ahead
+    auto scales_of = [&](int t) {
+      const int j = t * TCA_KEYS + th;
+      float2 y = make_float2(0.f, 0.f);
+      if (th < TCA_KEYS && t < w.t1 && j < w.s.len) {
+        int pg = __ldg(r.c.table + (size_t)w.b * r.c.table_stride + (j >> r.c.page_shift));
+        if (pg < 0 || pg >= r.c.n_pages) pg = 0;   // (the loads say so)
+        const int at = ((pg * n_kv + w.g) << r.c.page_shift) + (j & ((1 << r.c.page_shift) - 1));
+        y = make_float2(__ldg(r.c.ks + at) * (r.scale * LOG2E), __ldg(r.c.vs + at));
+      }
+      return y;
+    };
     uint32_t it = 0;
     bool ok = true;
-    for (; w.more() && ok; w.next())
+    for (; w.more() && ok; w.next()) {
+      float2 scales = scales_of(w.t0), ahead = make_float2(0.f, 0.f);
       for (int i = 2 * w.t0; i < 2 * w.t1 && ok; ++i, ++it) {   // K and V in turn
         const uint32_t rs = it & 1, st = it % TCA_STAGES;
+        const bool is_v = i & 1;
+        if (!is_v) ahead = scales_of((i >> 1) + 1);
         ok = mbar_wait_small(&sm.raw_full[rs], (it >> 1) & 1);
         if (it >= TCA_STAGES) ok = ok && mbar_wait_small(&sm.empty[st], (it / TCA_STAGES - 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
         const int tail = w.s.len - (i >> 1) * TCA_KEYS;   // rows from here on were not loaded, or are not the sequence's
         const uint32_t src = smem_u32(sm.raw[FP8 ? rs : 0]), dst = smem_u32(sm.kv[st]);
+        if (th < TCA_KEYS) {
+          if (is_v) sm.v_scale[FP8 ? (it >> 1) & 1 : 0][FP8 ? th : 0] = scales.y;
+          else sm.k_scale[FP8 ? (it >> 1) % 3 : 0][FP8 ? th : 0] = scales.x;
+        }
+        if (is_v) scales = ahead;
 #pragma unroll
         for (int k = 0; k < 6; ++k) {       // 8 bytes and 8 again: two swizzled 16-byte chunks of a row
           const int row = k * 24 + (th >> 3);
           if (row >= TCA_KEYS) break;
-          const float s = row < tail ? sm.raw_scale[FP8 ? rs : 0][row] : 0.f;
-          const uint64_t s2 = f32x2(s, s);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {     // the second half's lanes begin with their other chunk: no bank conflict
             const int o = j ^ half;
@@ -602,11 +629,10 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
             asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(q.x), "=r"(q.y) : "r"(src + row * HEAD_DIM + ch * 16 + o * 8));
             uint32_t y[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t h = e4m3x2_to_f16x2((i < 2 ? q.x : q.y) >> (16 * (i & 1)));
+            for (int i2 = 0; i2 < 4; ++i2) {
+              const uint32_t h = e4m3x2_to_f16x2((i2 < 2 ? q.x : q.y) >> (16 * (i2 & 1)));
               const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-              const uint64_t z = mul2(f32x2(f.x, f.y), s2);
-              y[i] = pack_bf16(f32x2_lo(z), f32x2_hi(z));
+              y[i2] = pack_bf16(f.x, f.y);
             }
             if (row >= tail) y[0] = y[1] = y[2] = y[3] = 0;
             const int c16 = ((ch & 3) * 2 + o) ^ (row & 7);
@@ -622,15 +648,16 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
           mbar_arrive(&sm.raw_empty[rs]);
         }
       }
+    }
   }
   } else {
   regs_inc<TcShape<SRC>::SOFTMAX>();
   if (work) {   // ---- softmax: thread = one row of tile x ----
     const int x = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lanes + 128 * x, to = tmem + lanes + 256 + 128 * x;
-    const float sl2 = r.scale * LOG2E;
+    const float sl2 = FP8 ? 1.f : r.scale * LOG2E;   // (an e4m3 cache: already in the keys' scales)
     TcWalk<SRC> w(p, sm, step);
-    int ns = 0, no = 0;
+    int ns = 0, no = 0, kt = 0;             // kt: key tiles of the pieces before
     bool ok = true;
     for (; w.more(); w.next()) {
       const int e = w.end(x), tok = w.tok0(x) + row / r.group, pos = w.s.len - w.s.n + tok;
@@ -649,6 +676,16 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
           tc_wait_ld();
 #pragma unroll
           for (int i = from; i < to_; ++i) tca_tie32(v + 32 * i);
+          if (FP8) {                        // the K scales, exactly
+            const float* ks = sm.k_scale[FP8 ? (kt + t - w.t0) % 3 : 0];
+#pragma unroll
+            for (int i = 32 * from; i < 32 * to_; i += 4) {
+              const float4 k4 = *reinterpret_cast<const float4*>(ks + (FP8 ? i : 0));
+              const uint64_t a = mul2(f32x2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), f32x2(k4.x, k4.y));
+              const uint64_t b = mul2(f32x2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), f32x2(k4.z, k4.w));
+              v[i] = (uint32_t)a, v[i + 1] = (uint32_t)(a >> 32), v[i + 2] = (uint32_t)b, v[i + 3] = (uint32_t)(b >> 32);
+            }
+          }
           if (edge) {
 #pragma unroll
             for (int i = 32 * from; i < 32 * to_; ++i)
@@ -656,6 +693,11 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
           }
         };
         load_s(0, 4);
+        const float* vs = sm.v_scale[FP8 ? (kt + t - w.t0) & 1 : 0];
+        if (FP8) {                          // V's tile, and with it the scales, is there (its stage waits for this P)
+          const uint32_t i = 2 * (kt + t - w.t0) + 1;
+          ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.full[i % TCA_STAGES], (i / TCA_STAGES) & 1));
+        }
         float mx[4] = {m, m, m, m};
 #pragma unroll
         for (int i = 0; i < 128; i += 2) mx[(i >> 1) & 3] = max3_nan(mx[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
@@ -665,7 +707,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         // some row has none yet (all of them in the piece's first tile), or one that grew by more than TCA_LAZY, or a NaN.
         uint64_t sum[2] = {0, 0};
         const bool early = t > w.t0;
-        if (early) tca_exp<8 * TCA_FIRST>(v, v, scale2, f32x2(base, base), sum);
+        if (early) tca_exp<8 * TCA_FIRST, FP8>(v, v, scale2, f32x2(base, base), sum, vs);
         const bool grow = valid && !((mn - m) * sl2 <= TCA_LAZY);
         if (__any_sync(0xffffffffu, grow)) {   // (each row by its own scores: neighbours, and rows that are none, change nothing)
           float f = 1.f;
@@ -689,7 +731,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
           }
           if (early) load_s(0, (TCA_FIRST + 1) / 2);
           sum[0] = sum[1] = 0;
-          tca_exp<8 * TCA_FIRST>(v, v, scale2, f32x2(base, base), sum);
+          tca_exp<8 * TCA_FIRST, FP8>(v, v, scale2, f32x2(base, base), sum, vs);
         }
         auto hand_over = [&](int hh) {
           tca_wait_st();
@@ -699,12 +741,13 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         };
         tca_st<8 * TCA_FIRST>(ts, v);
         hand_over(0);
-        tca_exp<64 - 8 * TCA_FIRST>(v + 16 * TCA_FIRST, v + 8 * TCA_FIRST, scale2, f32x2(base, base), sum);
+        tca_exp<64 - 8 * TCA_FIRST, FP8>(v + 16 * TCA_FIRST, v + 8 * TCA_FIRST, scale2, f32x2(base, base), sum, vs + (FP8 ? 16 * TCA_FIRST : 0));
         tca_st<64 - 8 * TCA_FIRST>(ts + 8 * TCA_FIRST, v + 8 * TCA_FIRST);
         hand_over(1);
         l += (f32x2_lo(sum[0]) + f32x2_hi(sum[0])) + (f32x2_lo(sum[1]) + f32x2_hi(sum[1]));
       }
 
+      kt += w.t1 - w.t0;
       // ---- the piece's end: the output rows, or a partial --------------------------------------------------------
       const bool any = e > w.t0;
       if (any) {

@@ -204,14 +204,20 @@ __global__ void __launch_bounds__(256, 4) paged_qkv_kernel(const __grid_constant
   const size_t row0 = (((size_t)page * n_kv) << p.c.page_shift) + slot;
   // pairs [from, to) of one kind, whose heads begin at src and end at n
   auto rows = [&](auto kind, int from, int to, int n, const bf16* src) {
-    constexpr int KIND = decltype(kind)::value, AHEAD = 4;
+    constexpr int KIND = decltype(kind)::value, AHEAD = 2;
+    auto load = [&](int pair) {
+      const int h = 2 * pair + side;
+      return pair < to && h < n ? ldg_stream(src + h * HEAD_DIM) : make_uint4(0, 0, 0, 0);
+    };
+    uint4 next[AHEAD];                        // two pairs' rows are on their way while two are computed
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) next[i] = load(from + i);
     for (int pair = from; pair < to; pair += AHEAD) {
       uint4 in[AHEAD];
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        const int h = 2 * (pair + i) + side;
-        in[i] = pair + i < to && h < n ? ldg_stream(src + h * HEAD_DIM) : make_uint4(0, 0, 0, 0);
-      }
+      for (int i = 0; i < AHEAD; ++i) in[i] = next[i];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) next[i] = load(pair + AHEAD + i);
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
         if (pair + i >= to) break;

@@ -248,6 +248,14 @@ class PagedEngine:
             self.k.paged_kv_read(cu, table, self.k_pages[li], self.v_pages[li], k_cache[li, :, :n].transpose(0, 1),
                                  v_cache[li, :, :n].transpose(0, 1), k_scale=self.k_scale[li], v_scale=self.v_scale[li])
 
+    def recover(self):
+        """After a failed pass, with no launch in flight: zero the attention workspace's counters and clear the error word. The
+        sequences of the failed pass have to be prefilled again."""
+        torch.cuda.synchronize()
+        self.ws.zero_()
+        torch.cuda.synchronize()
+        self.k.device_error()
+
     def check(self):
         """Raise RuntimeError if a kernel recorded a device error since the last check (see `generate.Engine.check`)."""
         err = self.k.device_error()
