@@ -214,20 +214,28 @@ __device__ __forceinline__ void tca_wait_st() { asm volatile("tcgen05.wait::st.s
 
 // P of 2 N scores: p = exp2(s * scale + base), bf16 pairs to out (which may be the scores' first half), sums to sum. The
 // packed instructions halve the issue slots beside the exponential unit, which is what bounds this.
-// With vs, P goes times the keys' V scales (l does not).
-template <int N, bool VS>
-__device__ __forceinline__ void tca_exp(const uint32_t* s, uint32_t* out, uint64_t scale, uint64_t base, uint64_t (&sum)[2], const float* vs) {
-  float4 v4;
+// With F32 it stays as fp32 in the scores' place (out unused), for tca_pack.
+template <int N, bool F32>
+__device__ __forceinline__ void tca_exp(uint32_t* s, uint32_t* out, uint64_t scale, uint64_t base, uint64_t (&sum)[2]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     uint64_t x = fma2(f32x2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale, base);
     x = f32x2(ex2(f32x2_lo(x)), ex2(f32x2_hi(x)));
     sum[i & 1] = add2(sum[i & 1], x);
-    if (VS) {
-      if (i % 2 == 0) v4 = *reinterpret_cast<const float4*>(vs + 2 * i);
-      x = mul2(x, i % 2 == 0 ? f32x2(v4.x, v4.y) : f32x2(v4.z, v4.w));
-    }
-    out[i] = pack_bf16(f32x2_lo(x), f32x2_hi(x));
+    if (F32) s[2 * i] = (uint32_t)x, s[2 * i + 1] = (uint32_t)(x >> 32);
+    else out[i] = pack_bf16(f32x2_lo(x), f32x2_hi(x));
+  }
+}
+// P times the keys' V scales (l is without them), to bf16 pairs.
+template <int N>
+__device__ __forceinline__ void tca_pack(const uint32_t* s, uint32_t* out, const float* vs) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const float4 v4 = *reinterpret_cast<const float4*>(vs + 2 * i);
+    const uint64_t a = mul2(f32x2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), f32x2(v4.x, v4.y));
+    const uint64_t b = mul2(f32x2(__uint_as_float(s[2 * i + 2]), __uint_as_float(s[2 * i + 3])), f32x2(v4.z, v4.w));
+    out[i] = pack_bf16(f32x2_lo(a), f32x2_hi(a));
+    out[i + 1] = pack_bf16(f32x2_lo(b), f32x2_hi(b));
   }
 }
 
@@ -293,11 +301,11 @@ struct TcWalk {
 };
 
 // Threads, and their registers: 384 x 168 at launch become 256 x 208 + 128 x 88; with four warps more (they, 10 and 11 turn
-// e4m3 tiles into bf16 ones), 512 x 128 become 256 x 184 + 256 x 72.
+// e4m3 tiles into bf16 ones), 512 x 128 become 256 x 200 + 256 x 56.
 template <int SRC>
 struct TcShape {
   static constexpr int THREADS = SRC == SRC_PAGED_FP8 ? 512 : 384;
-  static constexpr int SOFTMAX = SRC == SRC_PAGED_FP8 ? 184 : 208, OTHER = SRC == SRC_PAGED_FP8 ? 72 : 88;
+  static constexpr int SOFTMAX = SRC == SRC_PAGED_FP8 ? 200 : 208, OTHER = SRC == SRC_PAGED_FP8 ? 56 : 88;
   static_assert(256 * SOFTMAX + (THREADS - 256) * OTHER <= THREADS * (SRC == SRC_PAGED_FP8 ? 128 : 168), "setmaxnreg would wait for ever");
 };
 template <int N>
@@ -693,11 +701,6 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
           }
         };
         load_s(0, 4);
-        const float* vs = sm.v_scale[FP8 ? (kt + t - w.t0) & 1 : 0];
-        if (FP8) {                          // V's tile, and with it the scales, is there (its stage waits for this P)
-          const uint32_t i = 2 * (kt + t - w.t0) + 1;
-          ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.full[i % TCA_STAGES], (i / TCA_STAGES) & 1));
-        }
         float mx[4] = {m, m, m, m};
 #pragma unroll
         for (int i = 0; i < 128; i += 2) mx[(i >> 1) & 3] = max3_nan(mx[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
@@ -707,7 +710,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         // some row has none yet (all of them in the piece's first tile), or one that grew by more than TCA_LAZY, or a NaN.
         uint64_t sum[2] = {0, 0};
         const bool early = t > w.t0;
-        if (early) tca_exp<8 * TCA_FIRST, FP8>(v, v, scale2, f32x2(base, base), sum, vs);
+        if (early) tca_exp<8 * TCA_FIRST, FP8>(v, v, scale2, f32x2(base, base), sum);
         const bool grow = valid && !((mn - m) * sl2 <= TCA_LAZY);
         if (__any_sync(0xffffffffu, grow)) {   // (each row by its own scores: neighbours, and rows that are none, change nothing)
           float f = 1.f;
@@ -731,7 +734,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
           }
           if (early) load_s(0, (TCA_FIRST + 1) / 2);
           sum[0] = sum[1] = 0;
-          tca_exp<8 * TCA_FIRST, FP8>(v, v, scale2, f32x2(base, base), sum, vs);
+          tca_exp<8 * TCA_FIRST, FP8>(v, v, scale2, f32x2(base, base), sum);
         }
         auto hand_over = [&](int hh) {
           tca_wait_st();
@@ -739,9 +742,16 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.p_full[x][hh]);
         };
+        const float* vs = sm.v_scale[FP8 ? (kt + t - w.t0) & 1 : 0];
+        if (FP8) {                          // V's tile, and with it the scales, is there (its stage waits for this P)
+          const uint32_t i = 2 * (kt + t - w.t0) + 1;
+          ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.full[i % TCA_STAGES], (i / TCA_STAGES) & 1));
+          tca_pack<8 * TCA_FIRST>(v, v, vs);
+        }
         tca_st<8 * TCA_FIRST>(ts, v);
         hand_over(0);
-        tca_exp<64 - 8 * TCA_FIRST, FP8>(v + 16 * TCA_FIRST, v + 8 * TCA_FIRST, scale2, f32x2(base, base), sum, vs + (FP8 ? 16 * TCA_FIRST : 0));
+        tca_exp<64 - 8 * TCA_FIRST, FP8>(v + 16 * TCA_FIRST, v + 8 * TCA_FIRST, scale2, f32x2(base, base), sum);
+        if (FP8) tca_pack<64 - 8 * TCA_FIRST>(v + 16 * TCA_FIRST, v + 8 * TCA_FIRST, vs + (FP8 ? 16 * TCA_FIRST : 0));
         tca_st<64 - 8 * TCA_FIRST>(ts + 8 * TCA_FIRST, v + 8 * TCA_FIRST);
         hand_over(1);
         l += (f32x2_lo(sum[0]) + f32x2_hi(sum[0])) + (f32x2_lo(sum[1]) + f32x2_hi(sum[1]));
