@@ -2,7 +2,7 @@
 //
 //   out[t][h] = sum over j <= pos(t) of softmax_j(scale * q[t][h] . K[g][j]) V[g][j]
 //
-// Bound by the cache bytes: up to 32 query rows (tokens x heads of a KV head) meet each K and V row once, so the only
+// Bound by the cache bytes: up to 16 query rows (tokens x heads of a KV head) meet each K and V row once, so the only
 // aim is to keep HBM busy.
 //  * Work: the (sequence, KV head, key tile) triples, tile-major, are dealt in equal contiguous ranges to one CTA
 //    per SM, whatever the lengths are: a 32k context beside short ones leaves no SM idle. A unit (sequence, head)
@@ -26,7 +26,7 @@
 namespace qk {
 
 constexpr int FEW_RING = 131072;      // bytes of K and V in the ring
-constexpr int FEW_MIN_TILES = 1;      // a CTA's least share (13 tiles of 8 heads: 8.4 us; 10.6 with 2, 11.6 with 4)
+constexpr int FEW_MIN_TILES = 1;      // a CTA's least share (one sequence of 13 tiles and 8 heads: 8.4 us; 10.6 with 2, 11.6 with 4)
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct RaggedParams {
@@ -75,13 +75,13 @@ __device__ __forceinline__ int few_tiles(const FewSeq& s) {
   return s.n > 0 ? max(1, (s.len + KEYS - 1) / KEYS) : 0;
 }
 
-// NT: 8-row tiles of query rows (1, 2 or 4).
+// NT: 8-row tiles of query rows (1 or 2).
 template <bool FP8, int NT>
 struct FewShape {
   static constexpr int ROWS = 8 * NT;
   static constexpr int KEYS = FP8 ? 128 : 64;            // keys of a tile: 16 KB of K (and of V) either way; e4m3 tiles
                                                          // of 64 keys cost the loading warp its pace (102 us against 88)
-  static constexpr int CW = NT <= 2 ? 8 : 4;             // consumer warps (their registers: 64 NT for O and q)
+  static constexpr int CW = 8;                           // consumer warps
   static constexpr int KW = FP8 || NT == 1 ? 32 : 16;    // keys of a tile that a warp takes (bf16, 16 rows: 16 leaves no spills)
   static constexpr int GROUPS = CW * KW / KEYS;      // groups of warps, a tile each in turn
   static constexpr int TILE = KEYS * HEAD_DIM * (FP8 ? 1 : 2);

@@ -88,8 +88,8 @@ int encode_pool_map(CUtensorMap* map, const void* pool, long long rows, bool fp8
 constexpr int RAGGED_MAX_CTAS = 160;
 struct RaggedWorkspace {
   int few_counters[256], tc_counters[256];
-  float few_ml[RAGGED_MAX_CTAS * 2 * 32 * 2], tc_ml[RAGGED_MAX_CTAS * 2 * 256 * 2];
-  float few_part[RAGGED_MAX_CTAS * 2 * 32 * HEAD_DIM], tc_part[RAGGED_MAX_CTAS * 2 * 256 * HEAD_DIM];
+  float few_ml[RAGGED_MAX_CTAS * 2 * 16 * 2], tc_ml[RAGGED_MAX_CTAS * 2 * 256 * 2];
+  float few_part[RAGGED_MAX_CTAS * 2 * 16 * HEAD_DIM], tc_part[RAGGED_MAX_CTAS * 2 * 256 * HEAD_DIM];
 };
 
 template <bool FP8, int NT>
@@ -249,9 +249,10 @@ int qk_paged_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
   const long long rows = args->max_q * p.group;
   if (rows <= 8) return fp8 ? launch_few<true, 1>(p, 1, args->workspace, st) : launch_few<false, 1>(p, 1, args->workspace, st);
   if (rows <= 16) return fp8 ? launch_few<true, 2>(p, 1, args->workspace, st) : launch_few<false, 2>(p, 1, args->workspace, st);
-  if (rows <= 32) return fp8 ? launch_few<true, 4>(p, 1, args->workspace, st) : launch_few<false, 4>(p, 1, args->workspace, st);
-  // the sequences with up to 8 query rows per KV head (those that decode beside a chunk), then the others: the tensor-core
-  // kernel takes a few rows too, at the matrix unit's time for 128
+  // More: the sequences with up to 8 query rows per KV head (those that decode beside a chunk), and the others behind them on
+  // the tensor cores, which take a few rows too at the matrix unit's time for 128. 17 to 32 rows in the few-row kernel
+  // took longer (16 sequences of up to 8 tokens at up to 16k: 183 us against 117; 8 at up to 400: 22 against 14), 9 to 16
+  // take less (102 against 115, 20 against 34 for 4 sequences at up to 4k).
   if (int e = fp8 ? launch_few<true, 1>(p, 0, args->workspace, st) : launch_few<false, 1>(p, 0, args->workspace, st)) return e;
   return fp8 ? launch_tc<SRC_PAGED_FP8>(p, 9, true, args->workspace, st) : launch_tc<SRC_PAGED>(p, 9, true, args->workspace, st);
 }
