@@ -15,9 +15,14 @@
 //    weight: until then the old m serves. P, l and O have fp32's exponents, so a P of up to 2^32 is as exact as one of 1;
 //    the rescale becomes rare, and a tile's exponentials need not wait for its maximum.
 //  * Warps: 0-3 and 4-7 the softmax of the two tiles, 8 the loads (TMA, 128-byte swizzle, a ring of five 32 KB K and V
-//    tiles), 9 issues the MMAs (10 clears V rows past a sequence's end, 11 fills the
-//    warpgroup, which gives registers to the softmax): Q0 K0, Q1 K0, then per tile P0 V, Q0 K', P1 V, Q1 K' (P in two parts, the first while the second is computed), so that while one tile's softmax
-//    runs, the matrix unit has the other's two products to do.
+//    tiles), 9 issues the MMAs from one thread (10 clears V rows past a sequence's end, 11 fills the warpgroup, which
+//    gives registers to the softmax): Q0 K0, Q1 K0, then per key tile P0 V, Q0 K', P1 V, Q1 K', with P in two parts, the
+//    first multiplied while the second is computed. While one tile's softmax runs, the matrix unit has the other's two
+//    products to do.
+//  * Measured (one prompt of 8,192 tokens, 32 heads on 8): 432 us in a burst, 1,270 TFLOP/s; some 510 us under the 1,000 W
+//    cap. A period of a pair of tiles is 3,150 cycles, the matrix unit's share 2,130: the chain of one tile's softmax
+//    (2,060), its last P V and next S (800) is longer than half of it. Slower were: exponentials partly on the FMA pipe,
+//    halves of S loaded apart, an issuing warp per tile, P in halves (443 us), 128-byte transposed output stores.
 //  * Work: (sequence, KV head, tile pair, key tile) in that order, dealt in equal contiguous ranges to the CTAs: causal
 //    rows and ragged lengths balance by themselves, and a few rows over a long context spread over every SM. A boundary
 //    nearer than TCA_MIN_PIECE tiles to the end of a unit moves there. Units cut by one leave fp32 partials (O, m, l) per
@@ -443,411 +448,411 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
 
   // the register split stands inside the roles' branches: after a join the compiler would have to take the smaller share
   if (warp >= 8) {
-  regs_dec<TcShape<SRC>::OTHER>();
-  if (work && warp == 8) {   // ---- loads ----
-    TcWalk<SRC> w(p, sm, step);
-    const int RB = SRC == SRC_PACKED ? TCA_KEYS : min(1 << r.c.page_shift, TCA_KEYS);
-    const uint32_t q_bytes = (uint32_t)(step / 2) * r.group * HEAD_DIM * 2;
-    int it = 0;
-    bool ok = true;
-    for (int unit = 0; w.more() && ok; w.next(), ++unit) {
-      if (unit) ok = __all_sync(0xffffffffu, mbar_wait_small(&sm.q_empty, (uint32_t)((unit - 1) & 1)));
-      if (!ok) break;
-      const bool two = w.tok0(1) < w.s.n;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&sm.q_full, two ? 2 * q_bytes : q_bytes);
-        for (int x = 0; x < (two ? 2 : 1); ++x)
-          for (int h = 0; h < 2; ++h)
-            tma_load_3d(sm.q[x] + h * (TCA_TILE / 2), &p.tm_q, 64 * h, w.g * r.group, w.s.row0 + w.tok0(x), &sm.q_full);
-      }
-      auto page_of = [&](int t) {           // this lane's box of tile t: its page, -1 where it holds no key
-        const int j = t * TCA_KEYS + lane * RB;
-        if (lane * RB >= TCA_KEYS || j >= w.s.len) return -1;
-        int pg = __ldg(r.c.table + (size_t)w.b * r.c.table_stride + (j >> r.c.page_shift));
-        if (pg < 0 || pg >= r.c.n_pages) {
-          atomicOr(&g_dev_error, DEVERR_BAD_STATE);
-          pg = 0;
-        }
-        return pg;
-      };
-      int next = SRC == SRC_PACKED ? 0 : page_of(w.t0);
-      for (int t = w.t0; t < w.t1 && ok; ++t) {
-        const int page = next;
-        if (SRC != SRC_PACKED && t + 1 < w.t1) next = page_of(t + 1);
-        for (int v = 0; v < 2; ++v, ++it) {   // K, then V
-          constexpr int N = FP8 ? 2 : TCA_STAGES;
-          const int st = it % N;
-          uint64_t* full = FP8 ? &sm.raw_full[st] : &sm.full[st];
-          if (it >= N) ok = __all_sync(0xffffffffu, mbar_wait_small(FP8 ? &sm.raw_empty[st] : &sm.empty[st], (uint32_t)((it / N - 1) & 1)));
-          if (!ok) break;
-          const CUtensorMap* tm = v ? &p.tm_v : &p.tm_k;
-          if (SRC == SRC_PACKED) {
-            if (lane == 0) {
-              mbar_arrive_expect_tx(full, TCA_TILE);
-              for (int h = 0; h < 2; ++h) tma_load_3d(sm.kv[st] + h * (TCA_TILE / 2), tm, 64 * h, w.g, w.s.row0 + t * TCA_KEYS, full);
-            }
-          } else {
-            const int nb = __popc(__ballot_sync(0xffffffffu, page >= 0));
-            if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(nb * RB) * (FP8 ? HEAD_DIM : 2 * HEAD_DIM));
-            __syncwarp();
-            if (page >= 0) {
-              const int row = ((page * n_kv + w.g) << r.c.page_shift) + ((t * TCA_KEYS + lane * RB) & ((1 << r.c.page_shift) - 1));
-              if (FP8) {                    // a page's rows of a head are contiguous
-                bulk_g2s(sm.raw[FP8 ? st : 0] + lane * RB * HEAD_DIM, (v ? r.c.v : r.c.k) + (size_t)row * HEAD_DIM, RB * HEAD_DIM, full);
-              } else {
-                for (int h = 0; h < 2; ++h) tma_load_2d(sm.kv[st] + h * (TCA_TILE / 2) + lane * RB * 128, tm, 64 * h, row, full);
-              }
-            }
-          }
-        }
-      }
-    }
-    if (!ok)   // a wait gave up: let the copies in flight land before the shared memory goes away
-      for (int n = FP8 ? 2 : TCA_STAGES, i = max(0, it - n); i < it; ++i)
-        mbar_wait_small(FP8 ? &sm.raw_full[i % n] : &sm.full[i % n], (uint32_t)((i / n) & 1), 1000000ull);
-  } else if (work && warp == 9) {   // ---- MMA issue: one thread, nothing between the products but its waits ----
-    if (elect_one()) {
-      constexpr uint32_t id_s = tca_idesc(false), id_o = tca_idesc(true);
+    regs_dec<TcShape<SRC>::OTHER>();
+    if (work && warp == 8) {   // ---- loads ----
       TcWalk<SRC> w(p, sm, step);
-      uint32_t st = 0, par = 0, np[2] = {0, 0}, clean = 0;   // st, par: the next tile's stage, its `full` parity; clean: v_clean's
+      const int RB = SRC == SRC_PACKED ? TCA_KEYS : min(1 << r.c.page_shift, TCA_KEYS);
+      const uint32_t q_bytes = (uint32_t)(step / 2) * r.group * HEAD_DIM * 2;
+      int it = 0;
       bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        ok = ok && mbar_wait_small(bar, parity);
-        tc_fence_after();
-      };
-      auto take = [&]() {                   // the next K or V tile of the ring
-        wait(&sm.full[st], par);
-        const uint32_t at = st;
-        if (++st == TCA_STAGES) st = 0, par ^= 1;
-        return at;
-      };
-      auto scores = [&](int x, uint32_t at) {   // S = Q K^T
-        const uint64_t qd = tc_desc_sw128(smem_u32(sm.q[x])), kd = tc_desc_sw128(smem_u32(sm.kv[at]));
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t off = ((k >> 2) * (TCA_TILE / 2) + (k & 3) * 32) >> 4;
-          tca_mma_ss(tmem + 128 * x, qd + off, kd + off, id_s, k > 0);
-        }
-        tc_commit(&sm.s_full[x]);
-      };
       for (int unit = 0; w.more() && ok; w.next(), ++unit) {
-        const int e[2] = {w.end(0), w.end(1)};
-        wait(&sm.q_full, (uint32_t)(unit & 1));
-        uint32_t ks = take();
+        if (unit) ok = __all_sync(0xffffffffu, mbar_wait_small(&sm.q_empty, (uint32_t)((unit - 1) & 1)));
         if (!ok) break;
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (w.t0 < e[x]) scores(x, ks);
-        tc_commit(&sm.empty[ks]);
-        if (w.t1 - w.t0 == 1) tc_commit(&sm.q_empty);
-        for (int t = w.t0; t < w.t1; ++t) {
-          const uint32_t vs = take();
-          const bool more = t + 1 < w.t1;
-          if (!FP8 && w.s.len - t * TCA_KEYS < TCA_KEYS) {
-            wait(&sm.v_clean[vs], clean >> vs & 1);
-            clean ^= 1u << vs;
-          }
-          if (more) ks = take();
-          if (!ok) break;
-          const uint64_t vd = tca_desc_mn(smem_u32(sm.kv[vs]));
-#pragma unroll                              // (the arrays stay in registers)
-          for (int x = 0; x < 2; ++x) {
-            if (t < e[x]) {
-#pragma unroll
-              for (int hh = 0; hh < 2; ++hh) {
-                wait(&sm.p_full[x][hh], np[x] & 1);
-                if (!ok) break;
-#pragma unroll
-                for (int k = hh ? TCA_FIRST : 0; k < (hh ? 8 : TCA_FIRST); ++k)
-                  tca_mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * k, vd + k * (2048 >> 4), id_o, k > 0 || t > w.t0);
-              }
-              if (t + 1 == e[x]) tc_commit(&sm.o_full[x]);
-              ++np[x];
-            }
-            if (t + 1 < e[x] && ok) scores(x, ks);
-          }
-          if (!ok) break;
-          tc_commit(&sm.empty[vs]);
-          if (more) tc_commit(&sm.empty[ks]);
-          if (t + 2 == w.t1) tc_commit(&sm.q_empty);
-        }
-      }
-    }
-    __syncwarp();
-  } else if (!FP8 && work && warp == 10) {   // ---- V rows past a sequence's end: another's, or nothing; 0 x NaN must not reach O ----
-    TcWalk<SRC> w(p, sm, step);
-    uint32_t st = 0, par = 0;
-    bool ok = true;
-    for (; w.more() && ok; w.next())
-      for (int i = 2 * w.t0; i < 2 * w.t1 && ok; ++i) {   // every tile of the ring in turn, K and V
-        ok = __all_sync(0xffffffffu, mbar_wait_small(&sm.full[st], par));
-        const int tail = w.s.len - (i >> 1) * TCA_KEYS;
-        if ((i & 1) && tail < TCA_KEYS) {
-          const uint32_t va = smem_u32(sm.kv[st]);
-          for (int k = max(tail, 0) * 16 + lane; k < TCA_KEYS * 16; k += 32)
-            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(va + ((k >> 3) & 1) * (TCA_TILE / 2) + (k >> 4) * 128 + (k & 7) * 16), "r"(0) : "memory");
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.v_clean[st]);
-        }
-        if (lane == 0) mbar_arrive(&sm.empty[st]);
-        if (++st == TCA_STAGES) st = 0, par ^= 1;
-      }
-  } else if (FP8 && work) {   // ---- warps 10 to 15: e4m3 tiles to bf16 ones (exact), and their rows' scales ----
-    TcWalk<SRC> w(p, sm, step);
-    const int th = tid - 320, ch = th & 7, half = ch >> 2;   // this thread's 16 dims, of every 24th row
-    // the scales of key th of tile t: fetched a tile ahead
-    auto scales_of = [&](int t) {
-      const int j = t * TCA_KEYS + th;
-      float2 y = make_float2(0.f, 0.f);
-      if (th < TCA_KEYS && t < w.t1 && j < w.s.len) {
-        int pg = __ldg(r.c.table + (size_t)w.b * r.c.table_stride + (j >> r.c.page_shift));
-        if (pg < 0 || pg >= r.c.n_pages) pg = 0;   // (the loads say so)
-        const int at = ((pg * n_kv + w.g) << r.c.page_shift) + (j & ((1 << r.c.page_shift) - 1));
-        y = make_float2(__ldg(r.c.ks + at) * (r.scale * LOG2E), __ldg(r.c.vs + at));
-      }
-      return y;
-    };
-    uint32_t it = 0;
-    bool ok = true;
-    for (; w.more() && ok; w.next()) {
-      float2 scales = scales_of(w.t0), ahead = make_float2(0.f, 0.f);
-      for (int i = 2 * w.t0; i < 2 * w.t1 && ok; ++i, ++it) {   // K and V in turn
-        const uint32_t rs = it & 1, st = it % TCA_STAGES;
-        const bool is_v = i & 1;
-        if (!is_v) ahead = scales_of((i >> 1) + 1);
-        ok = mbar_wait_small(&sm.raw_full[rs], (it >> 1) & 1);
-        if (it >= TCA_STAGES) ok = ok && mbar_wait_small(&sm.empty[st], (it / TCA_STAGES - 1) & 1);
-        ok = __all_sync(0xffffffffu, ok);
-        const int tail = w.s.len - (i >> 1) * TCA_KEYS;   // rows from here on were not loaded, or are not the sequence's
-        const uint32_t src = smem_u32(sm.raw[FP8 ? rs : 0]), dst = smem_u32(sm.kv[st]);
-        if (th < TCA_KEYS) {
-          if (is_v) sm.v_scale[FP8 ? (it >> 1) & 1 : 0][FP8 ? th : 0] = scales.y;
-          else sm.k_scale[FP8 ? (it >> 1) % 3 : 0][FP8 ? th : 0] = scales.x;
-        }
-        if (is_v) scales = ahead;
-#pragma unroll
-        for (int k = 0; k < 6; ++k) {       // 8 bytes and 8 again: two swizzled 16-byte chunks of a row
-          const int row = k * 24 + (th >> 3);
-          if (row >= TCA_KEYS) break;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {     // the second half's lanes begin with their other chunk: no bank conflict
-            const int o = j ^ half;
-            uint2 q;
-            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(q.x), "=r"(q.y) : "r"(src + row * HEAD_DIM + ch * 16 + o * 8));
-            uint32_t y[4];
-#pragma unroll
-            for (int i2 = 0; i2 < 4; ++i2) {
-              const uint32_t h = e4m3x2_to_f16x2((i2 < 2 ? q.x : q.y) >> (16 * (i2 & 1)));
-              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-              y[i2] = pack_bf16(f.x, f.y);
-            }
-            if (row >= tail) y[0] = y[1] = y[2] = y[3] = 0;
-            const int c16 = ((ch & 3) * 2 + o) ^ (row & 7);
-            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + half * (TCA_TILE / 2) + row * 128 + c16 * 16), "r"(y[0]), "r"(y[1]),
-                         "r"(y[2]), "r"(y[3])
-                         : "memory");
-          }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
+        const bool two = w.tok0(1) < w.s.n;
         if (lane == 0) {
-          mbar_arrive(&sm.full[st]);
-          mbar_arrive(&sm.raw_empty[rs]);
+          mbar_arrive_expect_tx(&sm.q_full, two ? 2 * q_bytes : q_bytes);
+          for (int x = 0; x < (two ? 2 : 1); ++x)
+            for (int h = 0; h < 2; ++h)
+              tma_load_3d(sm.q[x] + h * (TCA_TILE / 2), &p.tm_q, 64 * h, w.g * r.group, w.s.row0 + w.tok0(x), &sm.q_full);
         }
-      }
-    }
-  }
-  } else {
-  regs_inc<TcShape<SRC>::SOFTMAX>();
-  if (work) {   // ---- softmax: thread = one row of tile x ----
-    const int x = warp >> 2, row = tid & 127;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lanes + 128 * x, to = tmem + lanes + 256 + 128 * x;
-    const float sl2 = FP8 ? 1.f : r.scale * LOG2E;   // (an e4m3 cache: already in the keys' scales)
-    TcWalk<SRC> w(p, sm, step);
-    int ns = 0, no = 0, kt = 0;             // kt: key tiles of the pieces before
-    bool ok = true;
-    for (; w.more(); w.next()) {
-      const int e = w.end(x), tok = w.tok0(x) + row / r.group, pos = w.s.len - w.s.n + tok;
-      const bool valid = row < (step / 2) * r.group && tok < w.s.n;
-      const int first = w.s.len - w.s.n + w.tok0(x);   // the last key that the tile's first row sees
-      float m = -INFINITY, l = 0.f, base = 0.f;   // base = -m * sl2
-      for (int t = w.t0; t < e; ++t) {
-        ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.s_full[x], (uint32_t)(ns++ & 1)));
-        tc_fence_after();
-        uint32_t v[128];
-        const int lim = t * TCA_KEYS + TCA_KEYS - 1 > first ? min(pos, w.s.len - 1) - t * TCA_KEYS : TCA_KEYS;
-        const bool edge = t * TCA_KEYS + TCA_KEYS - 1 > first;
-        auto load_s = [&](int from, int to_) {
-#pragma unroll
-          for (int i = from; i < to_; ++i) tca_ld32(ts + 32 * i, v + 32 * i);
-          tc_wait_ld();
-#pragma unroll
-          for (int i = from; i < to_; ++i) tca_tie32(v + 32 * i);
-          if (FP8) {                        // the K scales, exactly
-            const float* ks = sm.k_scale[FP8 ? (kt + t - w.t0) % 3 : 0];
-#pragma unroll
-            for (int i = 32 * from; i < 32 * to_; i += 4) {
-              const float4 k4 = *reinterpret_cast<const float4*>(ks + (FP8 ? i : 0));
-              const uint64_t a = mul2(f32x2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), f32x2(k4.x, k4.y));
-              const uint64_t b = mul2(f32x2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), f32x2(k4.z, k4.w));
-              v[i] = (uint32_t)a, v[i + 1] = (uint32_t)(a >> 32), v[i + 2] = (uint32_t)b, v[i + 3] = (uint32_t)(b >> 32);
+        auto page_of = [&](int t) {           // this lane's box of tile t: its page, -1 where it holds no key
+          const int j = t * TCA_KEYS + lane * RB;
+          if (lane * RB >= TCA_KEYS || j >= w.s.len) return -1;
+          int pg = __ldg(r.c.table + (size_t)w.b * r.c.table_stride + (j >> r.c.page_shift));
+          if (pg < 0 || pg >= r.c.n_pages) {
+            atomicOr(&g_dev_error, DEVERR_BAD_STATE);
+            pg = 0;
+          }
+          return pg;
+        };
+        int next = SRC == SRC_PACKED ? 0 : page_of(w.t0);
+        for (int t = w.t0; t < w.t1 && ok; ++t) {
+          const int page = next;
+          if (SRC != SRC_PACKED && t + 1 < w.t1) next = page_of(t + 1);
+          for (int v = 0; v < 2; ++v, ++it) {   // K, then V
+            constexpr int N = FP8 ? 2 : TCA_STAGES;
+            const int st = it % N;
+            uint64_t* full = FP8 ? &sm.raw_full[st] : &sm.full[st];
+            if (it >= N) ok = __all_sync(0xffffffffu, mbar_wait_small(FP8 ? &sm.raw_empty[st] : &sm.empty[st], (uint32_t)((it / N - 1) & 1)));
+            if (!ok) break;
+            const CUtensorMap* tm = v ? &p.tm_v : &p.tm_k;
+            if (SRC == SRC_PACKED) {
+              if (lane == 0) {
+                mbar_arrive_expect_tx(full, TCA_TILE);
+                for (int h = 0; h < 2; ++h) tma_load_3d(sm.kv[st] + h * (TCA_TILE / 2), tm, 64 * h, w.g, w.s.row0 + t * TCA_KEYS, full);
+              }
+            } else {
+              const int nb = __popc(__ballot_sync(0xffffffffu, page >= 0));
+              if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(nb * RB) * (FP8 ? HEAD_DIM : 2 * HEAD_DIM));
+              __syncwarp();
+              if (page >= 0) {
+                const int row = ((page * n_kv + w.g) << r.c.page_shift) + ((t * TCA_KEYS + lane * RB) & ((1 << r.c.page_shift) - 1));
+                if (FP8) {                    // a page's rows of a head are contiguous
+                  bulk_g2s(sm.raw[FP8 ? st : 0] + lane * RB * HEAD_DIM, (v ? r.c.v : r.c.k) + (size_t)row * HEAD_DIM, RB * HEAD_DIM, full);
+                } else {
+                  for (int h = 0; h < 2; ++h) tma_load_2d(sm.kv[st] + h * (TCA_TILE / 2) + lane * RB * 128, tm, 64 * h, row, full);
+                }
+              }
             }
           }
-          if (edge) {
-#pragma unroll
-            for (int i = 32 * from; i < 32 * to_; ++i)
-              if (i > lim) v[i] = 0xff800000u;   // -inf
-          }
+        }
+      }
+      if (!ok)   // a wait gave up: let the copies in flight land before the shared memory goes away
+        for (int n = FP8 ? 2 : TCA_STAGES, i = max(0, it - n); i < it; ++i)
+          mbar_wait_small(FP8 ? &sm.raw_full[i % n] : &sm.full[i % n], (uint32_t)((i / n) & 1), 1000000ull);
+    } else if (work && warp == 9) {   // ---- MMA issue: one thread, nothing between the products but its waits ----
+      if (elect_one()) {
+        constexpr uint32_t id_s = tca_idesc(false), id_o = tca_idesc(true);
+        TcWalk<SRC> w(p, sm, step);
+        uint32_t st = 0, par = 0, np[2] = {0, 0}, clean = 0;   // st, par: the next tile's stage, its `full` parity; clean: v_clean's
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+          ok = ok && mbar_wait_small(bar, parity);
+          tc_fence_after();
         };
-        load_s(0, 4);
-        float mx[4] = {m, m, m, m};
+        auto take = [&]() {                   // the next K or V tile of the ring
+          wait(&sm.full[st], par);
+          const uint32_t at = st;
+          if (++st == TCA_STAGES) st = 0, par ^= 1;
+          return at;
+        };
+        auto scores = [&](int x, uint32_t at) {   // S = Q K^T
+          const uint64_t qd = tc_desc_sw128(smem_u32(sm.q[x])), kd = tc_desc_sw128(smem_u32(sm.kv[at]));
 #pragma unroll
-        for (int i = 0; i < 128; i += 2) mx[(i >> 1) & 3] = max3_nan(mx[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-        const float mn = max_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3]);
-        const uint64_t scale2 = f32x2(sl2, sl2);
-        // The first half's exponentials are computed under the old maximum while the new one is found. It stands unless
-        // some row has none yet (all of them in the piece's first tile), or one that grew by more than TCA_LAZY, or a NaN.
-        uint64_t sum[2] = {0, 0};
-        const bool early = t > w.t0;
-        if (early) tca_exp<8 * TCA_FIRST, FP8>(v, v, scale2, f32x2(base, base), sum);
-        const bool grow = valid && !((mn - m) * sl2 <= TCA_LAZY);
-        if (__any_sync(0xffffffffu, grow)) {   // (each row by its own scores: neighbours, and rows that are none, change nothing)
-          float f = 1.f;
-          if (grow) {
-            f = m == -INFINITY ? 0.f : ex2((m - mn) * sl2);
-            m = mn;
-            l *= f;
-            // an infinite maximum makes the row NaN, as inf - inf does
-            base = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7fffffff) : -m * sl2;
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t off = ((k >> 2) * (TCA_TILE / 2) + (k & 3) * 32) >> 4;
+            tca_mma_ss(tmem + 128 * x, qd + off, kd + off, id_s, k > 0);
           }
-          if (early) {                      // the products before this tile's scores are done: O is whole
-#pragma unroll 1
-            for (int i = 0; i < 8; ++i) {
-              uint32_t o[16];
-              tca_ld16(to + 16 * i, o);
-              tc_wait_ld();
+          tc_commit(&sm.s_full[x]);
+        };
+        for (int unit = 0; w.more() && ok; w.next(), ++unit) {
+          const int e[2] = {w.end(0), w.end(1)};
+          wait(&sm.q_full, (uint32_t)(unit & 1));
+          uint32_t ks = take();
+          if (!ok) break;
 #pragma unroll
-              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-              tca_st16(to + 16 * i, o);
+          for (int x = 0; x < 2; ++x)
+            if (w.t0 < e[x]) scores(x, ks);
+          tc_commit(&sm.empty[ks]);
+          if (w.t1 - w.t0 == 1) tc_commit(&sm.q_empty);
+          for (int t = w.t0; t < w.t1; ++t) {
+            const uint32_t vs = take();
+            const bool more = t + 1 < w.t1;
+            if (!FP8 && w.s.len - t * TCA_KEYS < TCA_KEYS) {
+              wait(&sm.v_clean[vs], clean >> vs & 1);
+              clean ^= 1u << vs;
             }
+            if (more) ks = take();
+            if (!ok) break;
+            const uint64_t vd = tca_desc_mn(smem_u32(sm.kv[vs]));
+#pragma unroll                              // (the arrays stay in registers)
+            for (int x = 0; x < 2; ++x) {
+              if (t < e[x]) {
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                  wait(&sm.p_full[x][hh], np[x] & 1);
+                  if (!ok) break;
+#pragma unroll
+                  for (int k = hh ? TCA_FIRST : 0; k < (hh ? 8 : TCA_FIRST); ++k)
+                    tca_mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * k, vd + k * (2048 >> 4), id_o, k > 0 || t > w.t0);
+                }
+                if (t + 1 == e[x]) tc_commit(&sm.o_full[x]);
+                ++np[x];
+              }
+              if (t + 1 < e[x] && ok) scores(x, ks);
+            }
+            if (!ok) break;
+            tc_commit(&sm.empty[vs]);
+            if (more) tc_commit(&sm.empty[ks]);
+            if (t + 2 == w.t1) tc_commit(&sm.q_empty);
           }
-          if (early) load_s(0, (TCA_FIRST + 1) / 2);
-          sum[0] = sum[1] = 0;
-          tca_exp<8 * TCA_FIRST, FP8>(v, v, scale2, f32x2(base, base), sum);
-        }
-        auto hand_over = [&](int hh) {
-          tca_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.p_full[x][hh]);
-        };
-        const float* vs = sm.v_scale[FP8 ? (kt + t - w.t0) & 1 : 0];
-        if (FP8) {                          // V's tile, and with it the scales, is there (its stage waits for this P)
-          const uint32_t i = 2 * (kt + t - w.t0) + 1;
-          ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.full[i % TCA_STAGES], (i / TCA_STAGES) & 1));
-          tca_pack<8 * TCA_FIRST>(v, v, vs);
-        }
-        tca_st<8 * TCA_FIRST>(ts, v);
-        hand_over(0);
-        tca_exp<64 - 8 * TCA_FIRST, FP8>(v + 16 * TCA_FIRST, v + 8 * TCA_FIRST, scale2, f32x2(base, base), sum);
-        if (FP8) tca_pack<64 - 8 * TCA_FIRST>(v + 16 * TCA_FIRST, v + 8 * TCA_FIRST, vs + (FP8 ? 16 * TCA_FIRST : 0));
-        tca_st<64 - 8 * TCA_FIRST>(ts + 8 * TCA_FIRST, v + 8 * TCA_FIRST);
-        hand_over(1);
-        l += (f32x2_lo(sum[0]) + f32x2_hi(sum[0])) + (f32x2_lo(sum[1]) + f32x2_hi(sum[1]));
-      }
-
-      kt += w.t1 - w.t0;
-      // ---- the piece's end: the output rows, or a partial --------------------------------------------------------
-      const bool any = e > w.t0;
-      if (any) {
-        ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.o_full[x], (uint32_t)(no++ & 1)));
-        tc_fence_after();
-      }
-      bf16* dst = r.out + (long long)(w.s.row0 + tok) * r.out_row + (long long)(w.g * r.group + row % r.group) * r.out_head;
-      auto store = [&](const float* o, float inv, int col) {   // 32 columns
-#pragma unroll
-        for (int k = 0; k < 32; k += 8) {
-          float y[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = o[k + i] * inv;
-          *reinterpret_cast<uint4*>(dst + col + k) = pack_bf16x8(y);
-        }
-      };
-      if (w.t0 == 0 && w.t1 == w.n) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        if (any) {
-          uint32_t o[128];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) tca_ld32(to + 32 * i, o + 32 * i);
-          tc_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 4; ++i) tca_tie32(o + 32 * i);
-          if (valid) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) store(reinterpret_cast<const float*>(o + 32 * i), inv, 32 * i);
-          }
-          __syncwarp();
-        }
-        continue;
-      }
-      // boundaries inside the unit: c_lo .. c_hi; its first piece is CTA c_lo - 1's last (slot 1), piece i > 0 is CTA
-      // c_lo + i - 1's first (slot 0)
-      const long long a0 = w.u - w.t0 - (w.t0 ? TCA_UNIT_COST : 0);
-      const int G = (int)min((long long)gridDim.x, max(1ll, W / TCA_MIN_PIECE));
-      const int c_lo = (int)div_short((a0 + TCA_UNIT_COST + TCA_MIN_PIECE) * G + W - 1, W);
-      const int c_hi = (int)div_short((a0 + TCA_UNIT_COST + w.n - TCA_MIN_PIECE + 1) * G + W - 1, W) - 1;
-      const size_t slot = ((size_t)(c * 2 + (w.t0 == 0 ? 1 : 0)) * 2 + x) * 128;
-      *reinterpret_cast<float2*>(p.ml + (slot + row) * 2) = make_float2(m, l);
-      if (any) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t o[32];
-          tca_ld32(to + 32 * i, o);
-          tc_wait_ld();
-#pragma unroll
-          for (int k = 0; k < 32; k += 4)
-            *reinterpret_cast<uint4*>(p.part + slot * 128 + (size_t)(8 * i + k / 4) * 512 + row * 4) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-        }
-      }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (tid == 0) {                       // releases the CTA's stores (ordered before by the barrier), acquires the others'
-        const int before = add_acq_rel(p.counters + c_lo - 1, 1);
-        sm.last = before == c_hi - c_lo + 1;
-        if (sm.last) p.counters[c_lo - 1] = 0;
-      }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      const bool last = sm.last;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (last && valid) {
-        auto slot_of = [&](int cc) { return ((size_t)(cc * 2 + (cc == c_lo - 1 ? 1 : 0)) * 2 + x) * 128; };
-        float M = -INFINITY;
-#pragma unroll 4
-        for (int cc = c_lo - 1; cc <= c_hi; ++cc) M = fmaxf(M, __ldcg(p.ml + (slot_of(cc) + row) * 2));
-#pragma unroll 1
-        for (int col = 0; col < 128; col += 64) {   // 16 loads in flight a piece
-          float o[64] = {}, L = 0.f;
-          for (int cc = c_lo - 1; cc <= c_hi; ++cc) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ml + (slot_of(cc) + row) * 2));
-            float4 q[16];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) q[k] = __ldcg(reinterpret_cast<const float4*>(p.part + slot_of(cc) * 128 + (size_t)(col / 4 + k) * 512 + row * 4));
-            if (ml.y == 0.f) continue;      // no key of the piece was visible (and its O may not have been written)
-            const float f = M == -INFINITY ? 1.f : ex2((ml.x - M) * sl2);
-            L += ml.y * f;
-#pragma unroll
-            for (int k = 0; k < 16; ++k)
-              o[4 * k] += q[k].x * f, o[4 * k + 1] += q[k].y * f, o[4 * k + 2] += q[k].z * f, o[4 * k + 3] += q[k].w * f;
-          }
-          const float inv = L == 0.f ? 0.f : 1.f / L;
-          store(o, inv, col);
-          store(o + 32, inv, col + 32);
         }
       }
       __syncwarp();
+    } else if (!FP8 && work && warp == 10) {   // ---- V rows past a sequence's end: another's, or nothing; 0 x NaN must not reach O ----
+      TcWalk<SRC> w(p, sm, step);
+      uint32_t st = 0, par = 0;
+      bool ok = true;
+      for (; w.more() && ok; w.next())
+        for (int i = 2 * w.t0; i < 2 * w.t1 && ok; ++i) {   // every tile of the ring in turn, K and V
+          ok = __all_sync(0xffffffffu, mbar_wait_small(&sm.full[st], par));
+          const int tail = w.s.len - (i >> 1) * TCA_KEYS;
+          if ((i & 1) && tail < TCA_KEYS) {
+            const uint32_t va = smem_u32(sm.kv[st]);
+            for (int k = max(tail, 0) * 16 + lane; k < TCA_KEYS * 16; k += 32)
+              asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(va + ((k >> 3) & 1) * (TCA_TILE / 2) + (k >> 4) * 128 + (k & 7) * 16), "r"(0) : "memory");
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.v_clean[st]);
+          }
+          if (lane == 0) mbar_arrive(&sm.empty[st]);
+          if (++st == TCA_STAGES) st = 0, par ^= 1;
+        }
+    } else if (FP8 && work) {   // ---- warps 10 to 15: e4m3 tiles to bf16 ones (exact), and their rows' scales ----
+      TcWalk<SRC> w(p, sm, step);
+      const int th = tid - 320, ch = th & 7, half = ch >> 2;   // this thread's 16 dims, of every 24th row
+      // the scales of key th of tile t: fetched a tile ahead
+      auto scales_of = [&](int t) {
+        const int j = t * TCA_KEYS + th;
+        float2 y = make_float2(0.f, 0.f);
+        if (th < TCA_KEYS && t < w.t1 && j < w.s.len) {
+          int pg = __ldg(r.c.table + (size_t)w.b * r.c.table_stride + (j >> r.c.page_shift));
+          if (pg < 0 || pg >= r.c.n_pages) pg = 0;   // (the loads say so)
+          const int at = ((pg * n_kv + w.g) << r.c.page_shift) + (j & ((1 << r.c.page_shift) - 1));
+          y = make_float2(__ldg(r.c.ks + at) * (r.scale * LOG2E), __ldg(r.c.vs + at));
+        }
+        return y;
+      };
+      uint32_t it = 0;
+      bool ok = true;
+      for (; w.more() && ok; w.next()) {
+        float2 scales = scales_of(w.t0), ahead = make_float2(0.f, 0.f);
+        for (int i = 2 * w.t0; i < 2 * w.t1 && ok; ++i, ++it) {   // K and V in turn
+          const uint32_t rs = it & 1, st = it % TCA_STAGES;
+          const bool is_v = i & 1;
+          if (!is_v) ahead = scales_of((i >> 1) + 1);
+          ok = mbar_wait_small(&sm.raw_full[rs], (it >> 1) & 1);
+          if (it >= TCA_STAGES) ok = ok && mbar_wait_small(&sm.empty[st], (it / TCA_STAGES - 1) & 1);
+          ok = __all_sync(0xffffffffu, ok);
+          const int tail = w.s.len - (i >> 1) * TCA_KEYS;   // rows from here on were not loaded, or are not the sequence's
+          const uint32_t src = smem_u32(sm.raw[FP8 ? rs : 0]), dst = smem_u32(sm.kv[st]);
+          if (th < TCA_KEYS) {
+            if (is_v) sm.v_scale[FP8 ? (it >> 1) & 1 : 0][FP8 ? th : 0] = scales.y;
+            else sm.k_scale[FP8 ? (it >> 1) % 3 : 0][FP8 ? th : 0] = scales.x;
+          }
+          if (is_v) scales = ahead;
+#pragma unroll
+          for (int k = 0; k < 6; ++k) {       // 8 bytes and 8 again: two swizzled 16-byte chunks of a row
+            const int row = k * 24 + (th >> 3);
+            if (row >= TCA_KEYS) break;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {     // the second half's lanes begin with their other chunk: no bank conflict
+              const int o = j ^ half;
+              uint2 q;
+              asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(q.x), "=r"(q.y) : "r"(src + row * HEAD_DIM + ch * 16 + o * 8));
+              uint32_t y[4];
+#pragma unroll
+              for (int i2 = 0; i2 < 4; ++i2) {
+                const uint32_t h = e4m3x2_to_f16x2((i2 < 2 ? q.x : q.y) >> (16 * (i2 & 1)));
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+                y[i2] = pack_bf16(f.x, f.y);
+              }
+              if (row >= tail) y[0] = y[1] = y[2] = y[3] = 0;
+              const int c16 = ((ch & 3) * 2 + o) ^ (row & 7);
+              asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + half * (TCA_TILE / 2) + row * 128 + c16 * 16), "r"(y[0]), "r"(y[1]),
+                           "r"(y[2]), "r"(y[3])
+                           : "memory");
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&sm.full[st]);
+            mbar_arrive(&sm.raw_empty[rs]);
+          }
+        }
+      }
     }
-    if (!ok && lane == 0) atomicOr(&g_dev_error, DEVERR_MBAR_TIMEOUT);
-  }
+  } else {
+    regs_inc<TcShape<SRC>::SOFTMAX>();
+    if (work) {   // ---- softmax: thread = one row of tile x ----
+      const int x = warp >> 2, row = tid & 127;
+      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lanes + 128 * x, to = tmem + lanes + 256 + 128 * x;
+      const float sl2 = FP8 ? 1.f : r.scale * LOG2E;   // (an e4m3 cache: already in the keys' scales)
+      TcWalk<SRC> w(p, sm, step);
+      int ns = 0, no = 0, kt = 0;             // kt: key tiles of the pieces before
+      bool ok = true;
+      for (; w.more(); w.next()) {
+        const int e = w.end(x), tok = w.tok0(x) + row / r.group, pos = w.s.len - w.s.n + tok;
+        const bool valid = row < (step / 2) * r.group && tok < w.s.n;
+        const int first = w.s.len - w.s.n + w.tok0(x);   // the last key that the tile's first row sees
+        float m = -INFINITY, l = 0.f, base = 0.f;   // base = -m * sl2
+        for (int t = w.t0; t < e; ++t) {
+          ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.s_full[x], (uint32_t)(ns++ & 1)));
+          tc_fence_after();
+          uint32_t v[128];
+          const int lim = t * TCA_KEYS + TCA_KEYS - 1 > first ? min(pos, w.s.len - 1) - t * TCA_KEYS : TCA_KEYS;
+          const bool edge = t * TCA_KEYS + TCA_KEYS - 1 > first;
+          auto load_s = [&](int from, int to_) {
+#pragma unroll
+            for (int i = from; i < to_; ++i) tca_ld32(ts + 32 * i, v + 32 * i);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = from; i < to_; ++i) tca_tie32(v + 32 * i);
+            if (FP8) {                        // the K scales, exactly
+              const float* ks = sm.k_scale[FP8 ? (kt + t - w.t0) % 3 : 0];
+#pragma unroll
+              for (int i = 32 * from; i < 32 * to_; i += 4) {
+                const float4 k4 = *reinterpret_cast<const float4*>(ks + (FP8 ? i : 0));
+                const uint64_t a = mul2(f32x2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), f32x2(k4.x, k4.y));
+                const uint64_t b = mul2(f32x2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), f32x2(k4.z, k4.w));
+                v[i] = (uint32_t)a, v[i + 1] = (uint32_t)(a >> 32), v[i + 2] = (uint32_t)b, v[i + 3] = (uint32_t)(b >> 32);
+              }
+            }
+            if (edge) {
+#pragma unroll
+              for (int i = 32 * from; i < 32 * to_; ++i)
+                if (i > lim) v[i] = 0xff800000u;   // -inf
+            }
+          };
+          load_s(0, 4);
+          float mx[4] = {m, m, m, m};
+#pragma unroll
+          for (int i = 0; i < 128; i += 2) mx[(i >> 1) & 3] = max3_nan(mx[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+          const float mn = max_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3]);
+          const uint64_t scale2 = f32x2(sl2, sl2);
+          // The first half's exponentials are computed under the old maximum while the new one is found. It stands unless
+          // some row has none yet (all of them in the piece's first tile), or one that grew by more than TCA_LAZY, or a NaN.
+          uint64_t sum[2] = {0, 0};
+          const bool early = t > w.t0;
+          if (early) tca_exp<8 * TCA_FIRST, FP8>(v, v, scale2, f32x2(base, base), sum);
+          const bool grow = valid && !((mn - m) * sl2 <= TCA_LAZY);
+          if (__any_sync(0xffffffffu, grow)) {   // (each row by its own scores: neighbours, and rows that are none, change nothing)
+            float f = 1.f;
+            if (grow) {
+              f = m == -INFINITY ? 0.f : ex2((m - mn) * sl2);
+              m = mn;
+              l *= f;
+              // an infinite maximum makes the row NaN, as inf - inf does
+              base = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7fffffff) : -m * sl2;
+            }
+            if (early) {                      // the products before this tile's scores are done: O is whole
+#pragma unroll 1
+              for (int i = 0; i < 8; ++i) {
+                uint32_t o[16];
+                tca_ld16(to + 16 * i, o);
+                tc_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                tca_st16(to + 16 * i, o);
+              }
+            }
+            if (early) load_s(0, (TCA_FIRST + 1) / 2);
+            sum[0] = sum[1] = 0;
+            tca_exp<8 * TCA_FIRST, FP8>(v, v, scale2, f32x2(base, base), sum);
+          }
+          auto hand_over = [&](int hh) {
+            tca_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.p_full[x][hh]);
+          };
+          const float* vs = sm.v_scale[FP8 ? (kt + t - w.t0) & 1 : 0];
+          if (FP8) {                          // V's tile, and with it the scales, is there (its stage waits for this P)
+            const uint32_t i = 2 * (kt + t - w.t0) + 1;
+            ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.full[i % TCA_STAGES], (i / TCA_STAGES) & 1));
+            tca_pack<8 * TCA_FIRST>(v, v, vs);
+          }
+          tca_st<8 * TCA_FIRST>(ts, v);
+          hand_over(0);
+          tca_exp<64 - 8 * TCA_FIRST, FP8>(v + 16 * TCA_FIRST, v + 8 * TCA_FIRST, scale2, f32x2(base, base), sum);
+          if (FP8) tca_pack<64 - 8 * TCA_FIRST>(v + 16 * TCA_FIRST, v + 8 * TCA_FIRST, vs + (FP8 ? 16 * TCA_FIRST : 0));
+          tca_st<64 - 8 * TCA_FIRST>(ts + 8 * TCA_FIRST, v + 8 * TCA_FIRST);
+          hand_over(1);
+          l += (f32x2_lo(sum[0]) + f32x2_hi(sum[0])) + (f32x2_lo(sum[1]) + f32x2_hi(sum[1]));
+        }
+
+        kt += w.t1 - w.t0;
+        // ---- the piece's end: the output rows, or a partial --------------------------------------------------------
+        const bool any = e > w.t0;
+        if (any) {
+          ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.o_full[x], (uint32_t)(no++ & 1)));
+          tc_fence_after();
+        }
+        bf16* dst = r.out + (long long)(w.s.row0 + tok) * r.out_row + (long long)(w.g * r.group + row % r.group) * r.out_head;
+        auto store = [&](const float* o, float inv, int col) {   // 32 columns
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = o[k + i] * inv;
+            *reinterpret_cast<uint4*>(dst + col + k) = pack_bf16x8(y);
+          }
+        };
+        if (w.t0 == 0 && w.t1 == w.n) {
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          if (any) {
+            uint32_t o[128];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tca_ld32(to + 32 * i, o + 32 * i);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tca_tie32(o + 32 * i);
+            if (valid) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) store(reinterpret_cast<const float*>(o + 32 * i), inv, 32 * i);
+            }
+            __syncwarp();
+          }
+          continue;
+        }
+        // boundaries inside the unit: c_lo .. c_hi; its first piece is CTA c_lo - 1's last (slot 1), piece i > 0 is CTA
+        // c_lo + i - 1's first (slot 0)
+        const long long a0 = w.u - w.t0 - (w.t0 ? TCA_UNIT_COST : 0);
+        const int G = (int)min((long long)gridDim.x, max(1ll, W / TCA_MIN_PIECE));
+        const int c_lo = (int)div_short((a0 + TCA_UNIT_COST + TCA_MIN_PIECE) * G + W - 1, W);
+        const int c_hi = (int)div_short((a0 + TCA_UNIT_COST + w.n - TCA_MIN_PIECE + 1) * G + W - 1, W) - 1;
+        const size_t slot = ((size_t)(c * 2 + (w.t0 == 0 ? 1 : 0)) * 2 + x) * 128;
+        *reinterpret_cast<float2*>(p.ml + (slot + row) * 2) = make_float2(m, l);
+        if (any) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t o[32];
+            tca_ld32(to + 32 * i, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              *reinterpret_cast<uint4*>(p.part + slot * 128 + (size_t)(8 * i + k / 4) * 512 + row * 4) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          }
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (tid == 0) {                       // releases the CTA's stores (ordered before by the barrier), acquires the others'
+          const int before = add_acq_rel(p.counters + c_lo - 1, 1);
+          sm.last = before == c_hi - c_lo + 1;
+          if (sm.last) p.counters[c_lo - 1] = 0;
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const bool last = sm.last;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (last && valid) {
+          auto slot_of = [&](int cc) { return ((size_t)(cc * 2 + (cc == c_lo - 1 ? 1 : 0)) * 2 + x) * 128; };
+          float M = -INFINITY;
+#pragma unroll 4
+          for (int cc = c_lo - 1; cc <= c_hi; ++cc) M = fmaxf(M, __ldcg(p.ml + (slot_of(cc) + row) * 2));
+#pragma unroll 1
+          for (int col = 0; col < 128; col += 64) {   // 16 loads in flight a piece
+            float o[64] = {}, L = 0.f;
+            for (int cc = c_lo - 1; cc <= c_hi; ++cc) {
+              const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ml + (slot_of(cc) + row) * 2));
+              float4 q[16];
+#pragma unroll
+              for (int k = 0; k < 16; ++k) q[k] = __ldcg(reinterpret_cast<const float4*>(p.part + slot_of(cc) * 128 + (size_t)(col / 4 + k) * 512 + row * 4));
+              if (ml.y == 0.f) continue;      // no key of the piece was visible (and its O may not have been written)
+              const float f = M == -INFINITY ? 1.f : ex2((ml.x - M) * sl2);
+              L += ml.y * f;
+#pragma unroll
+              for (int k = 0; k < 16; ++k)
+                o[4 * k] += q[k].x * f, o[4 * k + 1] += q[k].y * f, o[4 * k + 2] += q[k].z * f, o[4 * k + 3] += q[k].w * f;
+            }
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            store(o, inv, col);
+            store(o + 32, inv, col + 32);
+          }
+        }
+        __syncwarp();
+      }
+      if (!ok && lane == 0) atomicOr(&g_dev_error, DEVERR_MBAR_TIMEOUT);
+    }
   }
   if (p.after_few) grid_dep_wait();
   tc_fence_before();

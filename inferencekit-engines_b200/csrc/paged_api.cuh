@@ -163,7 +163,7 @@ int warp_grid(long long warps, dim3* grid) {   // 8 warps a CTA
   return QK_OK;
 }
 
-// paged_qkv's warps an SM before a warp takes more than one pair of heads: 1,531 rows of 24 heads take 14.4 us with 16 and
+// paged_qkv's warps an SM before a warp takes more than one pair of heads: 1,655 rows of 24 heads take 14.4 us with 16 and
 // 16.4 with 8 or 32; 16 rows of 48 heads have a pair each either way.
 constexpr int QKV_WARPS = 16;
 }  // namespace
