@@ -301,10 +301,10 @@ struct PagedReadParams {
 
 // Rows back out of the pages: output row cu[b] + i is position starts[b] + i of sequence b, dequantised in fp32 and
 // rounded to bf16 once. A warp takes all 2 n_kv rows (K, then V) of one position, 16 bytes a lane: two bf16 rows or four
-// e4m3 rows at a time, two such loads in flight (four cost occupancy: 166 us against 148 for 131,000 positions of 8 heads
-// out of e4m3 pages, 5.5 TB/s).
+// e4m3 rows at a time, two such loads in flight, 48 warps an SM: 139 us for 131,000 positions of 8 heads out of e4m3 pages
+// (5.9 TB/s). Four loads cost occupancy (166 us), one leaves too little in flight (154), 64 warps too few registers (160).
 template <bool FP8>
-__global__ void __launch_bounds__(256) paged_kv_read_kernel(const __grid_constant__ PagedReadParams p) {
+__global__ void __launch_bounds__(256, 6) paged_kv_read_kernel(const __grid_constant__ PagedReadParams p) {
   constexpr int LANES = FP8 ? 8 : 16, ROWS = 32 / LANES, AHEAD = 2;
   const int lane = threadIdx.x & 31, sub = lane % LANES;
   const int n_kv = p.c.n_kv;

@@ -147,6 +147,22 @@ def test_longer_contexts_by_scaled_angles():
         assert torch.equal(plain.logits[0], yarn.logits[0]) == same
 
 
+def test_a_bad_page_is_reported_and_recovered_from():
+    """A page id outside the pool sets the error word: the pass raises, and after recover() passes run as before."""
+    from paged import PagedEngine
+    eng = PagedEngine(model(), pages=8, page_size=64, max_rows=64)
+    s = eng.new()
+    want = eng.step([(s, [1, 2, 3])])
+    t = eng.new()
+    eng.tables[t], eng.lens[t] = [99], 1
+    with pytest.raises(RuntimeError, match="error word 0x2"):
+        eng.step([(t, [5])])
+    eng.recover()
+    del eng.tables[t], eng.lens[t]
+    u = eng.new()
+    assert eng.step([(u, [1, 2, 3])]) == want
+
+
 def test_refusals():
     from paged import PagedEngine
     m = model()

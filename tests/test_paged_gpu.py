@@ -333,6 +333,18 @@ def test_attention_in_a_graph_follows_the_lengths():
     assert k.device_error() == 0
 
 
+def test_capture_needs_a_workspace_of_the_callers():
+    k = ops()
+    c, _ = make_cache([40], 8, 16, False, torch.Generator(device=DEV).manual_seed(1))
+    q = torch.zeros(1, 32, D, dtype=torch.bfloat16, device=DEV)
+    cu, lens = ints([0, 1]), ints([40])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        k._scratch.pop(("ragged", q.get_device(), torch.cuda.current_stream().cuda_stream), None)
+        with pytest.raises(RuntimeError, match="before the capture"):
+            k.paged_attention(q, cu, lens, c["table"], c["k"], c["v"], q, 0.1, 1)
+
+
 # ---- the cache's rows ----------------------------------------------------------------------------------------
 def rotate64(x, cos, sin, interleaved):
     x = x.clone()
