@@ -306,8 +306,8 @@ int qk_argmax_rows(const void* logits, int rows, int V, unsigned long long* best
  * A ragged batch: sequence b owns token rows cu_rows[b] .. cu_rows[b+1]-1 (int32 [batch + 1], ascending from 0) and
  * ends, with them, at length seq_lens[b] (int32 [batch]), so row cu_rows[b] + i is position
  * seq_lens[b] - (cu_rows[b+1] - cu_rows[b]) + i. Position p lies in slot p % page_size of page
- * block_table[b * table_stride + p / page_size] (int32, table_width entries per sequence; entries past a sequence's
- * end are not read). Lengths and tables are device data: a captured call follows their contents. A position or page
+ * block_table[b * table_stride + p / page_size] (int32, table_width entries per sequence, table_stride 0, one row for
+ * all, or at least table_width; entries past a sequence's end are not read). Lengths and tables are device data: a captured call follows their contents. A position or page
  * outside the table, the rotary tables or the pool sets the error word's bad-state bit and its row is not written
  * (attention reads page 0 in its place). Rows past cu_rows[batch] are left alone.
  * Pages: [n_pages][n_kv][page_size][128], page_size 16, 32, 64 or 128; bf16, or (kv_fp8 = 1) e4m3 bytes with fp32 row

@@ -19,7 +19,9 @@ int paged_cache(PagedCache* c, const qk_paged_cache_t& a, bool lens) {
     return fail(QK_EINVAL, "n_pages=%lld n_kv=%lld batch=%lld", a.n_pages, a.n_kv, a.batch);
   // rows are counted in 32 bits (bytes are not)
   if (a.n_pages > 0x7fffffffll / (a.n_kv * a.page_size)) return fail(QK_EINVAL, "a pool of more than 2^31 - 1 rows");
-  if (a.table_width < 1 || a.table_stride < a.table_width || a.table_stride > 0x7fffffffll || a.table_width > 0x3fffffffll / a.page_size)
+  // (stride 0: every sequence reads the one row)
+  if (a.table_width < 1 || (a.table_stride != 0 && a.table_stride < a.table_width) || a.table_stride > 0x7fffffffll ||
+      a.table_width > 0x3fffffffll / a.page_size)
     return fail(QK_EINVAL, "table_width=%lld table_stride=%lld", a.table_width, a.table_stride);
   if (!aligned(a.k_pages, 16) || !aligned(a.v_pages, 16) || !aligned(a.k_scale, 16) || !aligned(a.v_scale, 16))
     return fail(QK_EINVAL, "pages and scales must be 16-byte aligned");

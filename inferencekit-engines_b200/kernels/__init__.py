@@ -404,7 +404,8 @@ class DecodeOps:
 
     # ---- serving from a paged KV cache ---------------------------------------------------------------------
     # A ragged batch: sequence b owns rows cu[b] .. cu[b+1]-1 (int32 [B+1]) and ends, with them, at length seq_lens[b]
-    # (int32 [B]); its position p lies in slot p % page_size of page block_table[b, p // page_size] (int32 [B, width]).
+    # (int32 [B]); its position p lies in slot p % page_size of page block_table[b, p // page_size] (int32 [B, width], the
+    # rows any distance of at least `width` apart, or one row for all: an expanded table).
     # k_pages/v_pages: bf16 [pages, n_kv, page_size, 128], or e4m3 (uint8 or float8_e4m3fn) with fp32 row scales
     # k_scale/v_scale [pages, n_kv, page_size]; page_size 16, 32, 64 or 128. Lengths and tables live on the device
     # (the calls can be captured); a position or page outside them sets the device error word and is not written.
@@ -445,7 +446,7 @@ class DecodeOps:
                 raise RuntimeError(f"{what}: seq_lens must be int32 [{B}] on the cache's device")
             lens_ptr = lens.data_ptr()
         return B, n_kv, dev, (k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, cu.data_ptr(), lens_ptr, block_table.data_ptr(),
-                              B, n_kv, pages, page, width, stride if stride > width else width, fp8)
+                              B, n_kv, pages, page, width, stride if B > 1 else width, fp8)
 
     @staticmethod
     def _heads(what, name, t, dev):

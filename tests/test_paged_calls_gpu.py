@@ -1,0 +1,32 @@
+"""The paged operators on the GPU, called in ways of their own: shared tables, several host threads, captures, orders and
+strides. Outputs are compared bit for bit with those of the ordinary call."""
+import pytest
+import torch
+
+from test_paged_gpu import D, DEV, cumulative, ints, make_cache, ops
+
+pytestmark = pytest.mark.gpu
+
+
+def same(a, b):
+    return torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "e4m3"])
+@pytest.mark.parametrize("n", [1, 3, 40])
+def test_one_table_for_every_sequence(n, fp8):
+    """An expanded table: several queries over one context, several ranges of one sequence."""
+    k = ops()
+    c, _ = make_cache([300], 4, 32, fp8, torch.Generator(device=DEV).manual_seed(n))
+    B, lens = 3, [300, 190, n]
+    q = torch.randn(B * n, 16, D, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).to(torch.bfloat16)
+    cu = ints(cumulative([n] * B))
+    got = []
+    for table in (c["table"].expand(B, -1), c["table"].expand(B, -1).contiguous()):
+        out = torch.empty_like(q)
+        k.paged_attention(q, cu, ints(lens), table, c["k"], c["v"], out, D ** -0.5, n, k_scale=c["ks"], v_scale=c["vs"])
+        ko, vo = (torch.empty(B * n, 4, D, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+        k.paged_kv_read(cu, table, c["k"], c["v"], ko, vo, k_scale=c["ks"], v_scale=c["vs"], starts=ints([0, 100, 300 - n]))
+        got.append((out, ko, vo))
+    assert all(same(a, b) for a, b in zip(*got))
+    assert k.device_error() == 0

@@ -1,0 +1,96 @@
+"""What the paged operators' shim sends to the library, without a GPU: CPU tensors that say they are on device 0, and a
+library that records its arguments."""
+import pytest
+import torch
+
+
+class OnGpu(torch.Tensor):
+    """A CPU tensor that says it is on GPU `index`."""
+    index = 0
+
+    def get_device(self):
+        return self.index
+
+
+def gpu(t):
+    return t.as_subclass(OnGpu)
+
+
+class Library:
+    """Stands in for the C library: every entry point unpacks its argument struct, records it and succeeds."""
+
+    def __init__(self, kernels):
+        self.calls = []
+        for name, fmt in (("qk_paged_qkv", kernels._QKV_ARGS), ("qk_paged_kv_read", kernels._READ_ARGS),
+                          ("qk_paged_attention", kernels._ATTENTION_ARGS), ("qk_packed_attention", kernels._ATTENTION_ARGS)):
+            setattr(self, name, self.entry(name, fmt))
+
+    def entry(self, name, fmt):
+        def call(args, stream):
+            self.calls.append((name, fmt.unpack(args)))
+            return 0
+        return call
+
+    def qk_ragged_attention_workspace_bytes(self):
+        return 512
+
+
+@pytest.fixture
+def shim(monkeypatch):
+    import kernels
+    monkeypatch.setattr(kernels, "_raw_stream", lambda dev: 0)
+    return kernels.DecodeOps(Library(kernels))
+
+
+def ints(v):
+    return gpu(torch.tensor(v, dtype=torch.int32))
+
+
+def bf16(*shape):
+    return gpu(torch.zeros(*shape, dtype=torch.bfloat16))
+
+
+TABLE_STRIDE = 12   # the field of qk_paged_cache_t
+
+
+def table_calls(shim, table, lens):
+    """Each call that takes a block table, with one new row a sequence; the row strides that were sent."""
+    B = len(lens)
+    pages, cu = bf16(8, 2, 16, 128), ints(list(range(B + 1)))
+    q, kv = bf16(B, 4, 128), bf16(B, 2, 128)
+    tab = gpu(torch.zeros(64, 64))
+    ws = gpu(torch.zeros(512, dtype=torch.uint8))
+    shim.paged_attention(q, cu, ints(lens), table, pages, pages, q, 0.1, 1, workspace=ws)
+    shim.paged_kv_read(cu, table, pages, pages, kv, kv)
+    shim.paged_qkv(bf16(B, 8 * 128), cu, ints(lens), table, pages, pages, q, tab, tab)
+    return [args[TABLE_STRIDE] for _, args in shim.lib.calls]
+
+
+def test_a_table_is_sent_with_its_own_row_stride(shim):
+    """One table for several ranges of a sequence is an expanded one: stride 0, not the width (rows past its end)."""
+    row = torch.tensor([[1, 2, 3]], dtype=torch.int32)
+    assert table_calls(shim, gpu(row.expand(3, -1)), [40, 41, 42]) == [0, 0, 0]
+    shim.lib.calls.clear()
+    wide = torch.zeros(4, 10, dtype=torch.int32)
+    assert table_calls(shim, gpu(wide[:, :3]), [40] * 4) == [10] * 3
+    shim.lib.calls.clear()
+    overlapping = torch.zeros(8, dtype=torch.int32).as_strided((3, 3), (2, 1))   # the library refuses it
+    assert table_calls(shim, gpu(overlapping), [40] * 3) == [2] * 3
+    shim.lib.calls.clear()
+    assert table_calls(shim, gpu(torch.zeros(8, dtype=torch.int32).as_strided((1, 3), (1, 1))), [40]) == [3] * 3
+
+
+def test_the_library_takes_shared_tables_and_refuses_overlapping_ones():
+    import os
+    import kernels
+    if not os.path.exists(kernels.LIB_PATH):
+        pytest.skip("library not built (run __graft_entry__.build())")
+    lib = kernels.load_library()
+
+    def read(batch, width, stride):   # no rows: the checks, and no launch
+        return lib.qk_paged_kv_read(kernels._READ_ARGS.pack(256, 256, 0, 0, 256, 0, 256, batch, 8, 10, 16, width, stride, 0,
+                                                            0, 256, 256, 0, 1024, 128), 0)
+
+    assert read(3, 4, 0) == 0 and read(3, 4, 4) == 0 and read(3, 4, 9) == 0
+    for stride in (1, 3, -1, -4):
+        assert read(3, 4, stride) == 1 and b"table_stride" in lib.qk_last_error()
