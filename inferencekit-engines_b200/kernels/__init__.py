@@ -152,6 +152,7 @@ class DecodeOps:
     def __init__(self, lib: ctypes.CDLL):
         self.lib = lib
         self._scratch = {}
+        self._outgrown = []          # scratch that larger calls replaced: a captured graph may still run on it
         self.timeline_names = None   # launch names in timeline-slot order while a timeline is set
 
     # ---- helpers ------------------------------------------------------------------------------------------
@@ -166,6 +167,8 @@ class DecodeOps:
         if part is None or part.numel() < part_floats or counters.numel() < units:
             n_part = max(part_floats, 0 if part is None else part.numel())
             n_cnt = max(units, 0 if counters is None else counters.numel())
+            if part is not None:
+                self._outgrown.append((part, counters))
             part = torch.empty(n_part, dtype=torch.float32, device=device)
             counters = torch.zeros(n_cnt, dtype=torch.int32, device=device)
             self._scratch[key] = (part, counters)
@@ -336,12 +339,21 @@ class DecodeOps:
         b = token.numel()
         self._check(self.lib.qk_embed(_p(token), _p(table), _p(resid), table.shape[0], b, _stream()), "embed")
 
-    def fp8_gemm_rows(self, x, w, w_scale, out, norm_w=None, eps=1e-6):
+    def gemm_scratch(self, device, rows: int, shapes) -> torch.Tensor:
+        """A scratch for fp8_gemm_rows calls of up to `rows` rows and weights of any of these (N, K) shapes (zeroed once;
+        every call leaves it ready for the next). Calls that may run at the same time need one each."""
+        need = [self.lib.qk_fp8_gemm_rows_scratch_bytes(rows, N, K) for N, K in shapes]
+        if not need or min(need) < 0:
+            raise RuntimeError(f"gemm_scratch: unsupported rows={rows} or shapes {list(shapes)}")
+        return torch.zeros(max(need), dtype=torch.uint8, device=device)
+
+    def fp8_gemm_rows(self, x, w, w_scale, out, norm_w=None, eps=1e-6, scratch=None):
         """Batched FP8 linear on the tcgen05 tensor cores: out[m] = bf16 W8A8 linear of x[m] (optionally
         RMS-normalised with norm_w first), for M = 1..128 rows (K <= 12288 above 64). x bf16 [M, K]; w fp8 [N, K],
         either a plain row-major matrix (read through TMA boxes) or a `PackedTiles` tensor from
         `model.pack_fp8_tiles` (read as contiguous tiles; not the GEMV's pack_fp8 layout); w_scale fp32 [N] or
-        [N/128, K/128]; out bf16 [M, N]. Scratch is owned by this object (zeroed once per size and device)."""
+        [N/128, K/128]; out bf16 [M, N]. scratch: from gemm_scratch; by default this object's own, one per device, which
+        every caller without one shares."""
         tiles = isinstance(w, PackedTiles)
         if (isinstance(w, PackedFP8) or w.dtype != torch.float8_e4m3fn or w.dim() != 2 or not w.is_contiguous()):
             raise RuntimeError("fp8_gemm_rows: w must be a row-major float8_e4m3fn [N, K] matrix or "
@@ -352,11 +364,16 @@ class DecodeOps:
         if nbytes < 0:
             raise RuntimeError(f"fp8_gemm_rows: unsupported shape M={M} N={N} K={K} (M 1..128; N, K multiples of "
                                "128; K at most 16384, or 12288 above 64 rows)")
-        key = ("gemm", x.device.index if x.device.index is not None else torch.cuda.current_device())
-        sc = self._scratch.get(key)
-        if sc is None or sc.numel() < nbytes:
-            sc = torch.zeros(nbytes, dtype=torch.uint8, device=x.device)
-            self._scratch[key] = sc
+        sc = scratch
+        if sc is None:
+            key = ("gemm", x.device.index if x.device.index is not None else torch.cuda.current_device())
+            sc = self._scratch.get(key)
+            if sc is None or sc.numel() < nbytes:
+                if sc is not None:
+                    self._outgrown.append(sc)
+                sc = self._scratch[key] = torch.zeros(nbytes, dtype=torch.uint8, device=x.device)
+        elif sc.dtype != torch.uint8 or sc.device != x.device or not sc.is_contiguous() or sc.numel() < nbytes:
+            raise RuntimeError(f"fp8_gemm_rows: scratch must come from gemm_scratch() for these rows, on x's device ({nbytes} bytes)")
         scale_mode = SCALE_CHANNEL if w_scale.dim() == 1 else SCALE_BLOCK128
         fn = self.lib.qk_fp8_gemm_tiles if tiles else self.lib.qk_fp8_gemm_rows
         st = fn(_p(x), _p(norm_w), M, K, _p(w), _p(w_scale), scale_mode, N, float(eps), _p(out), _p(sc), sc.numel(),

@@ -59,7 +59,11 @@ class PagedEngine:
         self.h = torch.empty(max_rows, cfg.inter, **bf)
         self.logits = torch.empty(max_seqs, cfg.vocab, **bf)
         self.best = torch.zeros(max_seqs, dtype=torch.int64, device=dev)
+        # scratch of its own: the decode graph runs on it, beside passes of any number of rows
         self.ws = self.k.attention_workspace(dev)
+        self.linear_ws = self.k.gemm_scratch(dev, min(max_rows, GEMM_ROWS),
+                                             [((nq + 2 * nkv) * hd, cfg.hidden), (cfg.hidden, nq * hd), (2 * cfg.inter, cfg.hidden),
+                                              (cfg.hidden, cfg.inter), (cfg.vocab, cfg.hidden)])
         self.w = [tuple(pack_fp8_tiles(unpack_fp8(lin.packed, lin.N, lin.K, lin.pairs)) for lin in (L.qkv, L.o, L.gu, L.down))
                   for L in m.layers]
         self.head_w = pack_fp8_tiles(unpack_fp8(m.lm_head.packed, m.lm_head.N, m.lm_head.K))
@@ -101,7 +105,8 @@ class PagedEngine:
     # ---- the pass ----------------------------------------------------------------------------------------------
     def _linear(self, x, w, scale, out, norm_w=None):
         for r in range(0, x.shape[0], GEMM_ROWS):
-            self.k.fp8_gemm_rows(x[r:r + GEMM_ROWS], w, scale, out[r:r + GEMM_ROWS], norm_w=norm_w, eps=self.m.cfg.eps)
+            self.k.fp8_gemm_rows(x[r:r + GEMM_ROWS], w, scale, out[r:r + GEMM_ROWS], norm_w=norm_w, eps=self.m.cfg.eps,
+                                 scratch=self.linear_ws)
 
     def _forward(self, tokens, cu, lens, table, max_q, whole, last):
         """One pass over T packed rows (device tensors); `whole`: every sequence begins in this pass. Leaves each

@@ -1,5 +1,7 @@
 """What the paged operators' shim sends to the library, without a GPU: CPU tensors that say they are on device 0, and a
 library that records its arguments."""
+import weakref
+
 import pytest
 import torch
 
@@ -94,3 +96,66 @@ def test_the_library_takes_shared_tables_and_refuses_overlapping_ones():
     assert read(3, 4, 0) == 0 and read(3, 4, 4) == 0 and read(3, 4, 9) == 0
     for stride in (1, 3, -1, -4):
         assert read(3, 4, stride) == 1 and b"table_stride" in lib.qk_last_error()
+
+
+class Linears:
+    """The batched linear's entry points: a scratch that grows with the rows, and the scratch pointers of the calls."""
+
+    def __init__(self):
+        self.seen = []
+
+    def qk_fp8_gemm_rows_scratch_bytes(self, M, N, K):
+        return 1024 * M
+
+    def qk_fp8_gemm_rows(self, x, norm, M, K, w, ws, mode, N, eps, out, scratch, nbytes, stream):
+        assert nbytes >= 1024 * M
+        self.seen.append(scratch.value)
+        return 0
+
+
+@pytest.fixture
+def linear(monkeypatch):
+    import kernels
+    monkeypatch.setattr(kernels, "_stream", lambda: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    k = kernels.DecodeOps(Linears())
+    w = torch.zeros(128, 128, dtype=torch.uint8).view(torch.float8_e4m3fn)
+
+    def call(rows, **kw):
+        x = torch.zeros(rows, 128, dtype=torch.bfloat16)
+        k.fp8_gemm_rows(x, w, torch.zeros(128), x.clone(), **kw)
+    return k, call
+
+
+def test_a_scratch_that_a_graph_may_hold_outlives_a_larger_one(linear):
+    k, call = linear
+    call(4)
+    held = weakref.ref(k._scratch[("gemm", 0)])
+    call(128)
+    call(4)
+    first, second, third = k.lib.seen
+    assert first != second and third == second and held() is not None and held().data_ptr() == first
+
+
+def test_the_gemvs_scratch_outlives_a_larger_one(monkeypatch):
+    import kernels
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    k = kernels.DecodeOps(Linears())
+    held = [weakref.ref(t) for t in k.scratch(torch.device("cpu"), 64, 4)]
+    assert [weakref.ref(t) for t in k.scratch(torch.device("cpu"), 32, 4)] == held
+    k.scratch(torch.device("cpu"), 65, 4)
+    assert all(r() is not None for r in held)
+
+
+def test_a_scratch_of_the_callers(linear):
+    k, call = linear
+    own = k.gemm_scratch("cpu", 64, [(128, 128)])
+    assert own.numel() == 64 * 1024 and not own.any()
+    call(64, scratch=own)
+    call(4, scratch=own)
+    assert k.lib.seen == [own.data_ptr()] * 2 and not k._scratch
+    for bad in (own.float(), own[::2]):
+        with pytest.raises(RuntimeError, match="scratch"):
+            call(4, scratch=bad)
+    with pytest.raises(RuntimeError, match="scratch"):
+        call(65, scratch=own)
