@@ -204,7 +204,9 @@ class PagedEngine:
             raise ValueError(f"1 to {min(self.max_seqs, self.max_rows, GEMM_ROWS)} sequences")
         for s in seqs:
             self.reserve(s, self.lens[s] + steps)
+        self.graph = None
         self.g_seqs, self.g_steps, self.g_done = list(seqs), steps, 0
+        self.g_at = {s: self.lens[s] for s in seqs}                     # where the next replay finds them
         self.token = self._int32(tokens)
         self.state = self._int32([[self.lens[s], 0] for s in seqs])     # [position of the next row, step]
         self.out_tokens = torch.zeros(B, steps, dtype=torch.int32, device=dev)
@@ -230,14 +232,22 @@ class PagedEngine:
             one()
 
     def decode(self, steps: int):
-        """Replay `steps` captured steps; returns the new tokens of each sequence (host lists)."""
-        if self.g_done + steps > self.g_steps:
-            raise ValueError(f"{self.g_steps - self.g_done} steps left of the capture")
+        """Replay `steps` captured steps; returns the new tokens of each sequence (host lists). The graph holds its own copy of
+        the sequences' pages and positions: once one of them was released, or went on in a `step`, ValueError (and nothing
+        is replayed) until the next capture."""
+        if self.graph is None:
+            raise ValueError("no capture to replay")
+        if not 0 <= steps <= self.g_steps - self.g_done:
+            raise ValueError(f"{steps} steps: {self.g_steps - self.g_done} steps left of the capture")
+        gone = [s for s in self.g_seqs if self.lens.get(s) != self.g_at[s]]
+        if gone:
+            raise ValueError(f"sequences {gone} of the capture were released or went on since: capture again")
         for _ in range(steps):
             self.graph.replay()
         self.g_done += steps
         for s in self.g_seqs:
-            self.lens[s] += steps
+            self.g_at[s] += steps
+            self.lens[s] = self.g_at[s]
         t = self.out_tokens[:, self.g_done - steps:self.g_done].tolist()
         self.check()
         return t

@@ -1,0 +1,166 @@
+"""paged.PagedEngine's bookkeeping without a GPU: a model without layers, stand-ins for the kernels and for CUDA graphs. The
+"model" answers each sequence with its last token plus one, and a write of a row is recorded as (sequence's page, slot)."""
+from contextlib import contextmanager
+
+import pytest
+import torch
+
+import model as M
+import paged
+
+VOCAB = 256
+
+
+class Ops:
+    error = 0
+
+    def set_pdl(self, on):
+        pass
+
+    def attention_workspace(self, device):
+        return torch.zeros(64, dtype=torch.uint8)
+
+    def gemm_scratch(self, device, rows, shapes):
+        return torch.zeros(64, dtype=torch.uint8)
+
+    def finalize(self, best, token, out_tokens, state):
+        nxt = 0xFFFFFFFF - (best & 0xFFFFFFFF)
+        token.copy_(nxt)
+        out_tokens[torch.arange(len(nxt)), state[:, 1].long()] = nxt.to(torch.int32)
+        state += 1
+
+    def device_error(self):
+        e, self.error = self.error, 0
+        return e
+
+
+class Engine(paged.PagedEngine):
+    """Records what each pass writes: (page, slot) of every new row, by the arguments that the kernels get."""
+
+    def _forward(self, tokens, cu, lens, table, max_q, whole, last):
+        self.passes = getattr(self, "passes", 0) + 1
+        self.batches = getattr(self, "batches", []) + [(cu[1:] - cu[:-1]).tolist()]
+        P = self.page_size
+        for b in range(len(lens)):
+            n = int(cu[b + 1] - cu[b])
+            for i in range(n):
+                pos = int(lens[b]) - n + i
+                page = int(table[b, pos // P]) if pos // P < table.shape[1] else -1
+                if not 0 <= page < self.pages:
+                    self.k.error = 2
+                else:
+                    self.written.append((page, pos % P))
+            self.best[b] = 0xFFFFFFFF - (int(tokens[cu[b + 1] - 1]) + 1) % VOCAB
+
+
+class Graph:
+    recording = None
+
+    def replay(self):
+        self.body()
+
+
+@pytest.fixture(scope="module")
+def model():
+    return M.Qwen3FP8Decode.synthetic(M.Config(vocab=VOCAB), max_seq=64, device="cpu", n_layers=0)
+
+
+@pytest.fixture
+def make(model, monkeypatch):
+    """make(pages, ...): an engine on the CPU."""
+    ops = Ops()
+    monkeypatch.setattr(paged, "ops", lambda: ops)
+
+    class Stream:
+        def wait_stream(self, other):
+            pass
+
+    @contextmanager
+    def on(stream):
+        yield
+
+    monkeypatch.setattr(torch.cuda, "Stream", Stream)
+    monkeypatch.setattr(torch.cuda, "current_stream", Stream)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda: None)
+    monkeypatch.setattr(torch.cuda, "stream", on)
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", Graph)
+
+    def build(pages, **kw):
+        kw = {**dict(page_size=16, max_rows=64, max_seqs=8), **kw}
+        eng = Engine(model, pages, **kw)
+        eng.pages, eng.written, eng.k.error = pages, [], 0
+
+        @contextmanager
+        def capture(graph):
+            """The body of the capture, run again by a replay. (The recording run's own effects are undone.)"""
+            keep = [t.clone() for t in (eng.token, eng.state, eng.out_tokens)]
+            written, batches = list(eng.written), list(eng.batches)
+            yield
+            for t, old in zip((eng.token, eng.state, eng.out_tokens), keep):
+                t.copy_(old)
+            eng.written, eng.batches = written, batches
+
+            def body():
+                torch.add(eng.state[:, 0], 1, out=eng.g_lens)
+                eng._forward(eng.token, eng.g_cu, eng.g_lens, eng.g_table, 1, False, None)
+                eng.k.finalize(eng.best[:len(eng.g_lens)], eng.token, eng.out_tokens, eng.state)
+            graph.body = body
+        monkeypatch.setattr(torch.cuda, "graph", capture)
+        return eng
+    return build
+
+
+def captured(eng, prompts=((1, 2, 3), (50,)), steps=4):
+    seqs = [eng.new() for _ in prompts]
+    toks = eng.step(list(zip(seqs, prompts)))
+    eng.capture(seqs, toks, steps)
+    return seqs, toks
+
+
+def test_decode_goes_on_from_the_capture(make):
+    eng = make(8)
+    seqs, toks = captured(eng)
+    assert toks == [4, 51]
+    assert eng.decode(2) == [[5, 6], [52, 53]] and eng.decode(2) == [[7, 8], [54, 55]]
+    assert [eng.lens[s] for s in seqs] == [7, 5]
+
+
+def test_decode_refuses_a_sequence_that_was_released(make):
+    """Its pages may be another's by then: nothing is replayed."""
+    eng = make(4)
+    (a, b), _ = captured(eng)
+    eng.decode(1)
+    eng.release(a)
+    other = eng.new()
+    eng.step([(other, [9] * 40)])                    # takes the released page too
+    written, lens = list(eng.written), dict(eng.lens)
+    with pytest.raises(ValueError, match="capture"):
+        eng.decode(1)
+    assert eng.written == written and eng.lens == lens
+
+
+def test_decode_refuses_a_sequence_that_went_on(make):
+    """A pass on a captured sequence leaves the graph's position behind it."""
+    eng = make(8)
+    (a, b), _ = captured(eng)
+    eng.decode(1)
+    nxt = eng.step([(b, [70])])
+    assert nxt == [71]
+    written, lens = list(eng.written), dict(eng.lens)
+    with pytest.raises(ValueError, match="capture"):
+        eng.decode(1)
+    assert eng.written == written and eng.lens == lens
+    eng.capture([a, b], [6, 71], 2)                  # a new capture goes on from there
+    assert eng.decode(2) == [[7, 8], [72, 73]]
+
+
+def test_decode_refuses_before_a_capture_and_steps_that_are_none(make):
+    eng = make(8)
+    with pytest.raises(ValueError, match="capture"):
+        eng.decode(1)
+    seqs, _ = captured(eng)
+    before = dict(eng.lens)
+    for n in (-1, 5):
+        with pytest.raises(ValueError):
+            eng.decode(n)
+    assert eng.lens == before and eng.decode(0) == [[], []]
