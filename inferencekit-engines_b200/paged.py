@@ -100,7 +100,8 @@ class PagedEngine:
         return torch.tensor(rows, dtype=torch.int32).to(self.m.device, non_blocking=True)
 
     def _table(self, seqs):
-        return self._int32([(self.tables[s] + [0] * self.width)[:self.width] for s in seqs])
+        """The sequences' pages; -1, which no kernel takes for a page, past them."""
+        return self._int32([(self.tables[s] + [-1] * self.width)[:self.width] for s in seqs])
 
     # ---- the pass ----------------------------------------------------------------------------------------------
     def _linear(self, x, w, scale, out, norm_w=None):

@@ -164,3 +164,12 @@ def test_decode_refuses_before_a_capture_and_steps_that_are_none(make):
         with pytest.raises(ValueError):
             eng.decode(n)
     assert eng.lens == before and eng.decode(0) == [[], []]
+
+
+def test_a_table_names_no_page_past_a_sequences_own(make):
+    """Entries past the reservation are -1, which the kernels refuse, not page 0, which may be another sequence's."""
+    eng = make(8, max_len=64)
+    s = eng.new()
+    eng.reserve(s, 17)
+    table = eng._table([s])
+    assert table.tolist() == [eng.tables[s] + [-1, -1]]
