@@ -88,13 +88,19 @@ class PagedEngine:
 
     def reserve(self, seq: int, length: int):
         """Pages for `length` positions; RuntimeError (and nothing taken) where the pool has too few."""
-        if length > self.max_len:
-            raise RuntimeError(f"sequence of {length} positions: the engine was built for {self.max_len}")
-        need = -(-length // self.page_size) - len(self.tables[seq])
-        if need > len(self.free):
-            raise RuntimeError(f"out of pages: {need} wanted, {len(self.free)} free")
-        for _ in range(need):
-            self.tables[seq].append(self.free.pop())
+        self._reserve([(seq, length)])
+
+    def _reserve(self, wants):
+        """Pages for all of [(sequence, positions)], or none."""
+        top = max(length for _, length in wants)
+        if top > self.max_len:
+            raise RuntimeError(f"sequence of {top} positions: the engine was built for {self.max_len}")
+        need = [max(0, -(-length // self.page_size) - len(self.tables[s])) for s, length in wants]
+        if sum(need) > len(self.free):
+            raise RuntimeError(f"out of pages: {sum(need)} wanted, {len(self.free)} free")
+        for (s, _), n in zip(wants, need):
+            for _ in range(n):
+                self.tables[s].append(self.free.pop())
 
     def _int32(self, rows):
         return torch.tensor(rows, dtype=torch.int32).to(self.m.device, non_blocking=True)
@@ -150,8 +156,7 @@ class PagedEngine:
         n = [len(t) for t in toks]
         if not batch or min(n) < 1 or sum(n) > self.max_rows or len(batch) > self.max_seqs or len(set(seqs)) < len(seqs):
             raise ValueError(f"a pass takes 1 to {self.max_seqs} different sequences with 1 to {self.max_rows} tokens together")
-        for s, c in zip(seqs, n):
-            self.reserve(s, self.lens[s] + c)
+        self._reserve([(s, self.lens[s] + c) for s, c in zip(seqs, n)])
         whole = all(self.lens[s] == 0 for s in seqs)
         cu = [0]
         for s, c in zip(seqs, n):
@@ -203,8 +208,7 @@ class PagedEngine:
         B, dev = len(seqs), self.m.device
         if not 0 < B <= min(self.max_seqs, self.max_rows, GEMM_ROWS):
             raise ValueError(f"1 to {min(self.max_seqs, self.max_rows, GEMM_ROWS)} sequences")
-        for s in seqs:
-            self.reserve(s, self.lens[s] + steps)
+        self._reserve([(s, self.lens[s] + steps) for s in seqs])
         self.graph = None
         self.g_seqs, self.g_steps, self.g_done = list(seqs), steps, 0
         self.g_at = {s: self.lens[s] for s in seqs}                     # where the next replay finds them

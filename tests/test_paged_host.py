@@ -173,3 +173,20 @@ def test_a_table_names_no_page_past_a_sequences_own(make):
     eng.reserve(s, 17)
     table = eng._table([s])
     assert table.tolist() == [eng.tables[s] + [-1, -1]]
+
+
+def test_capture_takes_no_pages_where_the_pool_has_too_few(make):
+    eng = make(3)
+    seqs = [eng.new(), eng.new()]
+    toks = eng.step([(seqs[0], [1] * 16), (seqs[1], [2] * 16)])
+    with pytest.raises(RuntimeError, match="out of pages"):
+        eng.capture(seqs, toks, 4)                   # a page each: one is left
+    assert len(eng.free) == 1
+
+
+def test_a_pass_takes_no_pages_where_the_pool_has_too_few(make):
+    eng = make(3)
+    a, b = eng.new(), eng.new()
+    with pytest.raises(RuntimeError, match="out of pages"):
+        eng.step([(a, [1] * 16), (b, [1] * 33)])
+    assert len(eng.free) == 3 and eng.lens == {a: 0, b: 0} and eng.step([(b, [1] * 33)]) == [2]
