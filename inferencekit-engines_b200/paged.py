@@ -208,6 +208,10 @@ class PagedEngine:
         B, dev = len(seqs), self.m.device
         if not 0 < B <= min(self.max_seqs, self.max_rows, GEMM_ROWS):
             raise ValueError(f"1 to {min(self.max_seqs, self.max_rows, GEMM_ROWS)} sequences")
+        if steps < 1:                            # (the warm-up writes the next position, which has to be reserved)
+            raise ValueError(f"{steps} steps to capture")
+        if len(set(seqs)) < B or len(tokens) != B:
+            raise ValueError(f"{B} sequences, {len(set(seqs))} of them different, and {len(tokens)} tokens")
         self._reserve([(s, self.lens[s] + steps) for s in seqs])
         self.graph = None
         self.g_seqs, self.g_steps, self.g_done = list(seqs), steps, 0

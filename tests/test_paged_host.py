@@ -175,6 +175,20 @@ def test_a_table_names_no_page_past_a_sequences_own(make):
     assert table.tolist() == [eng.tables[s] + [-1, -1]]
 
 
+@pytest.mark.parametrize("bad", ["no steps", "negative steps", "one sequence twice", "a token short", "a token over"])
+def test_capture_refuses(make, bad):
+    """Nothing is written and no page taken: the warm-up step needs a reserved position, and a row a token."""
+    eng = make(8)
+    seqs = [eng.new(), eng.new()]
+    toks = eng.step([(seqs[0], [1] * 16), (seqs[1], [2] * 16)])      # both end with their page
+    args = {"no steps": (seqs, toks, 0), "negative steps": (seqs, toks, -1), "one sequence twice": (seqs[:1] * 2, toks, 2),
+            "a token short": (seqs, toks[:1], 2), "a token over": (seqs, toks + [1], 2)}[bad]
+    free, written = list(eng.free), list(eng.written)
+    with pytest.raises(ValueError):
+        eng.capture(*args)
+    assert eng.free == free and eng.written == written and eng.k.error == 0
+
+
 def test_capture_takes_no_pages_where_the_pool_has_too_few(make):
     eng = make(3)
     seqs = [eng.new(), eng.new()]
