@@ -178,7 +178,19 @@ class PagedEngine:
         """Greedy generation of gen_len tokens for each prompt (lists of ids): prompts enter in chunks of at most `chunk`
         tokens (default: what a pass takes) beside the sequences that already decode. Returns the lists of ids."""
         chunk = min(chunk or self.max_rows, self.max_rows)
+        if chunk < 1 or not all(len(p) for p in prompts):
+            raise ValueError(f"chunks of {chunk} tokens, {sum(not len(p) for p in prompts)} empty prompts")
+        longest = max((len(p) for p in prompts), default=0) + gen_len - 1
+        if longest > self.max_len:
+            raise RuntimeError(f"sequence of {longest} positions: the engine was built for {self.max_len}")
         seqs = [self.new() for _ in prompts]
+        try:
+            return self._generate(seqs, prompts, gen_len, chunk)
+        finally:
+            for s in seqs:
+                self.release(s)
+
+    def _generate(self, seqs, prompts, gen_len, chunk):
         todo = {s: list(p) for s, p in zip(seqs, prompts)}
         out: dict[int, list[int]] = {s: [] for s in seqs}
         while any(len(out[s]) < gen_len for s in seqs):
@@ -196,8 +208,6 @@ class PagedEngine:
             for (s, _), tok in zip(batch, self.step(batch)):
                 if not todo[s]:
                     out[s].append(tok)
-        for s in seqs:
-            self.release(s)
         return [out[s] for s in seqs]
 
     # ---- decode graph ------------------------------------------------------------------------------------------

@@ -204,3 +204,23 @@ def test_a_pass_takes_no_pages_where_the_pool_has_too_few(make):
     with pytest.raises(RuntimeError, match="out of pages"):
         eng.step([(a, [1] * 16), (b, [1] * 33)])
     assert len(eng.free) == 3 and eng.lens == {a: 0, b: 0} and eng.step([(b, [1] * 33)]) == [2]
+
+
+@pytest.mark.parametrize("bad", ["empty prompt", "too long", "a failing pass"])
+def test_generate_gives_its_pages_back_when_it_fails(make, bad):
+    eng = make(8, max_len=48)
+    kept = eng.new()
+    eng.step([(kept, [3])])
+    prompts = [[1, 2], list(range(20))]
+    if bad == "empty prompt":
+        prompts.append([])
+    elif bad == "too long":
+        prompts.append([1] * 47)
+    else:
+        step = eng.step
+        eng.step = lambda batch: step(batch) if eng.passes < 3 else (_ for _ in ()).throw(RuntimeError("pass failed"))
+    with pytest.raises(ValueError if bad == "empty prompt" else RuntimeError):
+        eng.generate(prompts, 4)
+    assert len(eng.free) == 7 and list(eng.lens) == [kept]
+    if bad != "a failing pass":
+        assert eng.passes == 1                       # refused before anything ran
