@@ -176,30 +176,44 @@ class PagedEngine:
     @torch.no_grad()
     def generate(self, prompts, gen_len: int, chunk: int | None = None):
         """Greedy generation of gen_len tokens for each prompt (lists of ids): prompts enter in chunks of at most `chunk`
-        tokens (default: what a pass takes) beside the sequences that already decode. Returns the lists of ids."""
+        tokens (default: what a pass takes) beside the sequences that already decode, in their order and as soon as the pool
+        has pages for a prompt and its gen_len tokens; a finished sequence's pages go to those that wait. Returns the lists
+        of ids."""
         chunk = min(chunk or self.max_rows, self.max_rows)
         if chunk < 1 or not all(len(p) for p in prompts):
             raise ValueError(f"chunks of {chunk} tokens, {sum(not len(p) for p in prompts)} empty prompts")
+        if gen_len < 1:
+            return [[] for _ in prompts]
         longest = max((len(p) for p in prompts), default=0) + gen_len - 1
         if longest > self.max_len:
             raise RuntimeError(f"sequence of {longest} positions: the engine was built for {self.max_len}")
-        seqs = [self.new() for _ in prompts]
+        need = [-(-(len(p) + gen_len - 1) // self.page_size) for p in prompts]
+        if max(need, default=0) > len(self.free):
+            raise RuntimeError(f"out of pages: {max(need)} wanted by one prompt, {len(self.free)} free")
+        running: list[int] = []
         try:
-            return self._generate(seqs, prompts, gen_len, chunk)
+            return self._generate(running, prompts, need, gen_len, chunk)
         finally:
-            for s in seqs:
+            for s in running:
                 self.release(s)
 
-    def _generate(self, seqs, prompts, gen_len, chunk):
-        todo = {s: list(p) for s, p in zip(seqs, prompts)}
-        out: dict[int, list[int]] = {s: [] for s in seqs}
-        while any(len(out[s]) < gen_len for s in seqs):
+    def _generate(self, running, prompts, need, gen_len, chunk):
+        """`running`: the sequences that hold pages, kept up to date for the caller."""
+        out: list[list[int]] = [[] for _ in prompts]
+        waiting = list(range(len(prompts)))
+        todo, of = {}, {}                        # sequence -> tokens still to enter; its prompt's place
+        while waiting or running:
+            while waiting and need[waiting[0]] <= len(self.free):
+                i, s = waiting.pop(0), self.new()
+                running.append(s)
+                todo[s], of[s] = list(prompts[i]), i
+                self.reserve(s, len(prompts[i]) + gen_len - 1)   # to its end: it cannot run out on the way
             batch, room = [], self.max_rows
-            for s in seqs:                       # those that decode, then prompts
-                if not todo[s] and len(out[s]) < gen_len and len(batch) < self.max_seqs and room:
-                    batch.append((s, out[s][-1:]))
+            for s in running:                    # those that decode, then prompts
+                if not todo[s] and len(batch) < self.max_seqs and room:
+                    batch.append((s, out[of[s]][-1:]))
                     room -= 1
-            for s in seqs:
+            for s in running:
                 if todo[s] and room and len(batch) < self.max_seqs:
                     take = todo[s][:min(chunk, room)]
                     todo[s] = todo[s][len(take):]
@@ -207,8 +221,11 @@ class PagedEngine:
                     room -= len(take)
             for (s, _), tok in zip(batch, self.step(batch)):
                 if not todo[s]:
-                    out[s].append(tok)
-        return [out[s] for s in seqs]
+                    out[of[s]].append(tok)
+                    if len(out[of[s]]) == gen_len:
+                        running.remove(s)
+                        self.release(s)
+        return out
 
     # ---- decode graph ------------------------------------------------------------------------------------------
     @torch.no_grad()

@@ -224,3 +224,27 @@ def test_generate_gives_its_pages_back_when_it_fails(make, bad):
     assert len(eng.free) == 7 and list(eng.lens) == [kept]
     if bad != "a failing pass":
         assert eng.passes == 1                       # refused before anything ran
+
+
+def test_generate_serves_in_turn_what_does_not_fit_together(make):
+    """Finished sequences give their pages to those that wait; a prompt waits until its whole length has pages."""
+    eng = make(4, max_len=64)
+    prompts = [[10 * i + 1] * (17 + i) for i in range(5)]            # two pages each, with four new tokens
+    assert eng.generate(prompts, 4) == [[10 * i + 1 + j for j in range(1, 5)] for i in range(5)]
+    assert len(eng.free) == 4 and not eng.lens
+    assert max(len(b) for b in eng.batches) == 2
+    with pytest.raises(RuntimeError, match="out of pages"):
+        make(3, max_len=64).generate(prompts + [[1] * 50], 4)
+    kept = eng.new()
+    eng.step([(kept, [5] * 33)])
+    with pytest.raises(RuntimeError, match="out of pages"):          # one page is left, and nothing to wait for
+        eng.generate(prompts[:1], 4)
+    assert len(eng.free) == 1 and list(eng.lens) == [kept]
+
+
+def test_generate_admits_everything_that_fits_at_once(make):
+    """As many sequences as there is room for begin together, in the order they came."""
+    eng = make(16, max_rows=40)
+    prompts = [[1] * 30, [2] * 25, [3]]
+    assert eng.generate(prompts, 3, chunk=16) == [[2, 3, 4], [3, 4, 5], [4, 5, 6]]
+    assert eng.batches[:3] == [[16, 16, 1], [1, 14, 9], [1, 1, 1]]
