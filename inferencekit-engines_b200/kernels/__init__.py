@@ -138,6 +138,13 @@ def _raw_stream(dev: int) -> int:
     return torch._C._cuda_getCurrentRawStream(dev)
 
 
+def _launch_stream(what: str, dev: int) -> int:
+    """The stream for a call on tensors of GPU `dev`, which has to be the current one: the library launches there."""
+    if torch.cuda.current_device() != dev:
+        raise RuntimeError(f"{what}: the tensors are on GPU {dev}, the current device is {torch.cuda.current_device()}")
+    return _raw_stream(dev)
+
+
 _E4M3 = (torch.float8_e4m3fn, torch.uint8)
 _BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 # qk_paged_qkv_t, qk_paged_kv_read_t and qk_ragged_attention_t (the first 14 fields of each: qk_paged_cache_t)
@@ -527,7 +534,7 @@ class DecodeOps:
             return
         st = self.lib.qk_paged_qkv(_QKV_ARGS.pack(*cache, qkv.data_ptr(), q_out.data_ptr(), k_ptr, qn, kn, cos.data_ptr(),
                                                   sin.data_ptr(), T, n_q, qkv.stride(0), q_row, k_row, tab[0], tab[1],
-                                                  bool(interleaved), eps), _raw_stream(dev))
+                                                  bool(interleaved), eps), _launch_stream("paged_qkv", dev))
         if st:
             self._check(st, "paged_qkv")
 
@@ -547,7 +554,7 @@ class DecodeOps:
         if rows[0] == 0 or B == 0:
             return
         st = self.lib.qk_paged_kv_read(_READ_ARGS.pack(*cache, first, k_out.data_ptr(), v_out.data_ptr(), rows[0], rows[2],
-                                                       rows[3]), _raw_stream(dev))
+                                                       rows[3]), _launch_stream("paged_kv_read", dev))
         if st:
             self._check(st, "paged_kv_read")
 
@@ -564,7 +571,7 @@ class DecodeOps:
             raise RuntimeError(f"paged_attention: out must have q's shape, [{T}, {n_q}, 128]")
         if T == 0 or B == 0:
             return
-        stream = _raw_stream(dev)
+        stream = _launch_stream("paged_attention", dev)
         ws = self._workspace("paged_attention", workspace, dev, stream)
         st = self.lib.qk_paged_attention(_ATTENTION_ARGS.pack(*cache, q.data_ptr(), 0, 0, out.data_ptr(), ws.data_ptr(), T, n_q,
                                                               max_q, q_row, q_head, 0, 0, o_row, o_head, ws.numel(), scale), stream)
@@ -587,7 +594,7 @@ class DecodeOps:
         B = len(cu) - 1
         if T == 0 or B == 0:
             return
-        stream = _raw_stream(dev)
+        stream = _launch_stream("packed_attention", dev)
         ws = self._workspace("packed_attention", workspace, dev, stream)
         st = self.lib.qk_packed_attention(
             _ATTENTION_ARGS.pack(0, 0, 0, 0, cu.data_ptr(), 0, 0, B, kv[1], 0, 0, 0, 0, 0, q.data_ptr(), k.data_ptr(),

@@ -41,6 +41,7 @@ class Library:
 def shim(monkeypatch):
     import kernels
     monkeypatch.setattr(kernels, "_raw_stream", lambda dev: 0)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     return kernels.DecodeOps(Library(kernels))
 
 
@@ -159,3 +160,36 @@ def test_a_scratch_of_the_callers(linear):
             call(4, scratch=bad)
     with pytest.raises(RuntimeError, match="scratch"):
         call(65, scratch=own)
+
+
+def paged_calls(k, index):
+    """Every paged operator with tensors of GPU `index`."""
+    def on(t):
+        t = gpu(t)
+        t.index = index
+        return t
+
+    def zeros(*shape, dtype=torch.bfloat16):
+        return on(torch.zeros(*shape, dtype=dtype))
+
+    cu, lens, table = (on(torch.tensor(v, dtype=torch.int32)) for v in ([0, 1], [5], [[1, 2]]))
+    pages, q, kv, tab = zeros(8, 2, 16, 128), zeros(1, 4, 128), zeros(1, 2, 128), zeros(64, 64, dtype=torch.float32)
+    ws = zeros(512, dtype=torch.uint8)
+    return [lambda: k.paged_attention(q, cu, lens, table, pages, pages, q, 0.1, 1, workspace=ws),
+            lambda: k.packed_attention(q, kv, kv, cu, q, 0.1, 1, workspace=ws),
+            lambda: k.paged_kv_read(cu, table, pages, pages, kv, kv),
+            lambda: k.paged_qkv(zeros(1, 8 * 128), cu, lens, table, pages, pages, q, tab, tab)]
+
+
+def test_tensors_of_a_device_that_is_not_current_are_refused(shim, monkeypatch):
+    """The library launches on the current device, where another device's pointers mean nothing."""
+    for current in (0, 1):
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: current)
+        shim.lib.calls.clear()
+        for call in paged_calls(shim, current):
+            call()
+        assert len(shim.lib.calls) == 4
+        for call in paged_calls(shim, 1 - current):
+            with pytest.raises(RuntimeError, match="current"):
+                call()
+        assert len(shim.lib.calls) == 4
