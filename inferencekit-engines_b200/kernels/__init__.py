@@ -490,11 +490,11 @@ class DecodeOps:
         return torch.zeros(self.lib.qk_ragged_attention_workspace_bytes(), dtype=torch.uint8, device=device)
 
     def _workspace(self, what, ws, dev, stream):
-        if ws is None:   # one per device and stream, kept
+        if ws is None:   # one per device and stream, kept; never a graph's, whose replays may run beside the stream's calls
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"{what}: pass workspace=attention_workspace(device), made before the capture")
             ws = self._scratch.get(("ragged", dev, stream))
             if ws is None:
-                if torch.cuda.is_current_stream_capturing():
-                    raise RuntimeError(f"{what}: pass workspace=attention_workspace(device), made before the capture")
                 ws = self._scratch[("ragged", dev, stream)] = self.attention_workspace(torch.device("cuda", dev))
         elif ws.dtype is not torch.uint8 or ws.get_device() != dev or not ws.is_contiguous():
             raise RuntimeError(f"{what}: workspace must come from attention_workspace() on the call's device")

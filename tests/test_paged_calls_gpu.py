@@ -30,3 +30,25 @@ def test_one_table_for_every_sequence(n, fp8):
         got.append((out, ko, vo))
     assert all(same(a, b) for a, b in zip(*got))
     assert k.device_error() == 0
+
+
+def test_a_capture_needs_a_workspace_of_its_own():
+    """Also on a stream that an earlier call has given one."""
+    k = ops()
+    c, _ = make_cache([40], 8, 16, False, torch.Generator(device=DEV).manual_seed(1))
+    q, out = torch.zeros(1, 32, D, dtype=torch.bfloat16, device=DEV), torch.empty(1, 32, D, dtype=torch.bfloat16, device=DEV)
+    call = (q, ints([0, 1]), ints([40]), c["table"], c["k"], c["v"], out, 0.1, 1)
+    ws, side = k.attention_workspace(DEV), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        k.paged_attention(*call)
+        assert ("ragged", q.get_device(), side.cuda_stream) in k._scratch
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        with pytest.raises(RuntimeError, match="before the capture"):
+            k.paged_attention(*call)
+        k.paged_attention(*call, workspace=ws)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert k.device_error() == 0

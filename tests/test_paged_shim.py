@@ -193,3 +193,21 @@ def test_tensors_of_a_device_that_is_not_current_are_refused(shim, monkeypatch):
             with pytest.raises(RuntimeError, match="current"):
                 call()
         assert len(shim.lib.calls) == 4
+
+
+def test_a_capture_never_takes_the_streams_own_workspace(shim, monkeypatch):
+    """Not even where an earlier call on the stream has made it: its replays may run beside calls that use it."""
+    capturing = False
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    monkeypatch.setattr(shim, "attention_workspace", lambda device: gpu(torch.zeros(512, dtype=torch.uint8)))
+    q, kv, pages = bf16(1, 4, 128), bf16(1, 2, 128), bf16(8, 2, 16, 128)
+    attend = [lambda **kw: shim.paged_attention(q, ints([0, 1]), ints([5]), ints([[1, 2]]), pages, pages, q, 0.1, 1, **kw),
+              lambda **kw: shim.packed_attention(q, kv, kv, ints([0, 1]), q, 0.1, 1, **kw)]
+    for call in attend:
+        call()
+    capturing = True
+    for call in attend:
+        with pytest.raises(RuntimeError, match="before the capture"):
+            call()
+        call(workspace=gpu(torch.zeros(512, dtype=torch.uint8)))
+    assert len(shim.lib.calls) == 4
