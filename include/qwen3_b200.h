@@ -329,7 +329,8 @@ int qk_argmax_rows(const void* logits, int rows, int V, unsigned long long* best
  * qk_packed_attention: the same over whole prompts packed without padding: row t of prompt b sees rows
  *   cu_rows[b] .. t of k and v (kv_row between rows, kv_head between heads).
  * workspace: qk_ragged_attention_workspace_bytes() bytes, 256-byte aligned, zeroed once; every call leaves it ready
- *   for the next. Calls that may overlap need one each. */
+ *   for the next. Calls that may overlap on the device (two streams, a graph beside a stream) need one each; calls on one
+ *   stream may share one, from several host threads too. */
 typedef struct {
   const void *k_pages, *v_pages;
   const float *k_scale, *v_scale;          /* NULL for bf16 pages */

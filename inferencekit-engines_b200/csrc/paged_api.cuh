@@ -1,6 +1,7 @@
 // C entry points of the paged-serving operators (paged.cuh, attention_ragged.cuh). Included by qwen3_b200.cu, whose
 // argument-check and launch helpers it uses.
 #pragma once
+#include <mutex>
 
 // the shim packs these structs field by field
 static_assert(sizeof(qk_paged_cache_t) == 14 * 8 && sizeof(qk_paged_qkv_t) == 30 * 8 && sizeof(qk_paged_kv_read_t) == 20 * 8 &&
@@ -93,6 +94,13 @@ struct RaggedWorkspace {
   float few_ml[RAGGED_MAX_CTAS * 2 * 16 * 2], tc_ml[RAGGED_MAX_CTAS * 2 * 256 * 2];
   float few_part[RAGGED_MAX_CTAS * 2 * 16 * HEAD_DIM], tc_part[RAGGED_MAX_CTAS * 2 * 256 * HEAD_DIM];
 };
+
+// Held over the launches of a call. The tensor-core kernel of a mixed batch skips its wait for what precedes the few-row
+// kernel: another thread's call on the same stream must not get in between, or two of them would run at once on one workspace.
+std::mutex& workspace_mutex(const void* workspace) {
+  static std::mutex mu[16];
+  return mu[(reinterpret_cast<uintptr_t>(workspace) >> 8) % 16];
+}
 
 template <bool FP8, int NT>
 int launch_few(const RaggedParams& r, int strict, void* workspace, cudaStream_t stream) {
@@ -249,6 +257,7 @@ int qk_paged_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
   const bool fp8 = args->cache.kv_fp8 != 0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const long long rows = args->max_q * p.group;
+  std::lock_guard<std::mutex> together(workspace_mutex(args->workspace));
   if (rows <= 8) return fp8 ? launch_few<true, 1>(p, 1, args->workspace, st) : launch_few<false, 1>(p, 1, args->workspace, st);
   if (rows <= 16) return fp8 ? launch_few<true, 2>(p, 1, args->workspace, st) : launch_few<false, 2>(p, 1, args->workspace, st);
   // More: the sequences with up to 8 query rows per KV head (those that decode beside a chunk), and the others behind them on
@@ -276,6 +285,7 @@ int qk_packed_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
   p.c.cu = a.cache.cu_rows;
   p.c.B = (int)a.cache.batch;
   p.c.n_kv = (int)a.cache.n_kv;
+  std::lock_guard<std::mutex> together(workspace_mutex(a.workspace));
   return launch_tc<SRC_PACKED>(p, 0, false, args->workspace, static_cast<cudaStream_t>(stream));
 }
 

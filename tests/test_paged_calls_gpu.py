@@ -52,3 +52,46 @@ def test_a_capture_needs_a_workspace_of_its_own():
     graph.replay()
     torch.cuda.synchronize()
     assert k.device_error() == 0
+
+
+def test_host_threads_share_a_stream():
+    """Mixed batches (two launches a call), packed prompts and decode steps from several threads on one stream and its one
+    workspace: each call's output as from a call alone."""
+    import threading
+    k = ops()
+    work = []
+    for i in range(4):
+        g = torch.Generator(device=DEV).manual_seed(i)
+        n = [1, 30 + 17 * i, 1, 2]
+        lens = [900 + 100 * i, 700, 50, 400]
+        c, _ = make_cache(lens, 4, 32, i % 2 == 1, g)
+        q = torch.randn(sum(n), 16, D, generator=g, device=DEV).to(torch.bfloat16)
+        kv = torch.randn(2, sum(n), 4, D, generator=g, device=DEV).to(torch.bfloat16)
+        work.append((q, kv, c, ints(cumulative(n)), ints(lens), max(n), ints(list(range(5)))))
+
+    def calls(i, outs):
+        q, kv, c, cu, lens, top, ones = work[i]
+        for a, b, d in outs:
+            k.paged_attention(q, cu, lens, c["table"], c["k"], c["v"], a, D ** -0.5, top, k_scale=c["ks"], v_scale=c["vs"])
+            k.packed_attention(q, kv[0], kv[1], cu, b, D ** -0.5, top)
+            k.paged_attention(q[:4], ones, lens, c["table"], c["k"], c["v"], d, D ** -0.5, 1, k_scale=c["ks"], v_scale=c["vs"])
+
+    def outputs(i, n):
+        q = work[i][0]
+        return [(torch.empty_like(q), torch.empty_like(q), torch.empty_like(q[:4])) for _ in range(n)]
+
+    want = [outputs(i, 1) for i in range(4)]
+    for i in range(4):
+        calls(i, want[i])
+    torch.cuda.synchronize()
+    got = [outputs(i, 50) for i in range(4)]
+    threads = [threading.Thread(target=calls, args=(i, got[i])) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert k.device_error() == 0
+    for i in range(4):
+        for outs in got[i]:
+            assert all(same(a, b) for a, b in zip(outs, want[i][0]))
