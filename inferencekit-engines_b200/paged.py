@@ -300,10 +300,11 @@ class PagedEngine:
                                  v_cache[li, :, :n].transpose(0, 1), k_scale=self.k_scale[li], v_scale=self.v_scale[li])
 
     def recover(self):
-        """After a failed pass, with no launch in flight: zero the attention workspace's counters and clear the error word. The
-        sequences of the failed pass have to be prefilled again."""
+        """After a failed pass, with no launch in flight: zero the counters of the attention workspace and of the linears'
+        scratch, and clear the error word. The sequences of the failed pass have to be prefilled again."""
         torch.cuda.synchronize()
         self.ws.zero_()
+        self.linear_ws.zero_()
         torch.cuda.synchronize()
         self.k.device_error()
 

@@ -248,3 +248,14 @@ def test_generate_admits_everything_that_fits_at_once(make):
     prompts = [[1] * 30, [2] * 25, [3]]
     assert eng.generate(prompts, 3, chunk=16) == [[2, 3, 4], [3, 4, 5], [4, 5, 6]]
     assert eng.batches[:3] == [[16, 16, 1], [1, 14, 9], [1, 1, 1]]
+
+
+def test_recover_resets_every_counter_of_a_pass(make):
+    """A wait that gave up leaves the counters of the attention or of the linears mid-count."""
+    eng = make(4)
+    eng.ws.fill_(1)
+    eng.linear_ws.fill_(1)
+    eng.k.error = 1
+    eng.recover()
+    assert not eng.ws.any() and not eng.linear_ws.any()
+    eng.check()
