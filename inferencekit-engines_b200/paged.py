@@ -159,12 +159,13 @@ class PagedEngine:
         self._reserve([(s, self.lens[s] + c) for s, c in zip(seqs, n)])
         whole = all(self.lens[s] == 0 for s in seqs)
         cu = [0]
-        for s, c in zip(seqs, n):
+        for c in n:
             cu.append(cu[-1] + c)
-            self.lens[s] += c
+        lens = [self.lens[s] + c for s, c in zip(seqs, n)]
         last = None if max(n) == 1 else torch.tensor([c - 1 for c in cu[1:]]).to(self.m.device, non_blocking=True)
-        self._forward(self._int32([t for x in toks for t in x]), self._int32(cu), self._int32([self.lens[s] for s in seqs]),
-                      self._table(seqs), max(n), whole, last)
+        self._forward(self._int32([t for x in toks for t in x]), self._int32(cu), self._int32(lens), self._table(seqs), max(n),
+                      whole, last)
+        self.lens.update(zip(seqs, lens))
         return self._tokens(len(batch))
 
     def _tokens(self, B):

@@ -259,3 +259,15 @@ def test_recover_resets_every_counter_of_a_pass(make):
     eng.recover()
     assert not eng.ws.any() and not eng.linear_ws.any()
     eng.check()
+
+
+def test_a_pass_that_was_not_launched_leaves_the_lengths(make):
+    """A refusal on the host (a table, a shape) wrote no rows: the sequences go on from where they were."""
+    eng = make(4)
+    s = eng.new()
+    eng.step([(s, [1, 2])])
+    forward, eng._forward = eng._forward, lambda *a: (_ for _ in ()).throw(RuntimeError("refused"))
+    with pytest.raises(RuntimeError, match="refused"):
+        eng.step([(s, [3])])
+    eng._forward = forward
+    assert eng.lens[s] == 2 and eng.step([(s, [3])]) == [4]
