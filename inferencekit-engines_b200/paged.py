@@ -294,7 +294,11 @@ class PagedEngine:
     def export(self, seq: int, k_cache: torch.Tensor, v_cache: torch.Tensor):
         """A sequence's rows into one sequence of a contiguous bf16 cache, [layers, n_kv, max_seq, 128] (a `Qwen3FP8Decode`'s
         k_cache[:, b]), from where the contiguous engines go on."""
-        n = self.lens[seq]
+        n, cfg = self.lens[seq], self.m.cfg
+        for t in (k_cache, v_cache):
+            if t.dim() != 4 or tuple(t.shape[:2]) != (len(self.m.layers), cfg.n_kv_heads) or t.shape[2] < n or t.shape[3] != cfg.head_dim:
+                raise ValueError(f"export wants caches [{len(self.m.layers)}, {cfg.n_kv_heads}, {n} or more, {cfg.head_dim}], got "
+                                 f"{tuple(t.shape)}")
         cu, table = self._int32([0, n]), self._table([seq])
         for li in range(len(self.m.layers)):
             self.k.paged_kv_read(cu, table, self.k_pages[li], self.v_pages[li], k_cache[li, :, :n].transpose(0, 1),

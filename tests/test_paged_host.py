@@ -271,3 +271,15 @@ def test_a_pass_that_was_not_launched_leaves_the_lengths(make):
         eng.step([(s, [3])])
     eng._forward = forward
     assert eng.lens[s] == 2 and eng.step([(s, [3])]) == [4]
+
+
+def test_export_refuses_a_cache_that_cannot_hold_the_sequence(make):
+    eng = make(4)
+    s = eng.new()
+    eng.step([(s, [1] * 20)])
+    cache = torch.zeros(0, 8, 64, 128, dtype=torch.bfloat16)
+    eng.export(s, cache, cache.clone())
+    for bad in (cache[:, :, :19], cache[:, :4], torch.zeros(1, 8, 64, 128, dtype=torch.bfloat16), cache[..., :64]):
+        for k, v in ((bad, cache), (cache, bad)):
+            with pytest.raises(ValueError, match="export"):
+                eng.export(s, k, v)
