@@ -44,6 +44,19 @@ int paged_cache(PagedCache* c, const qk_paged_cache_t& a, bool lens) {
 
 bool row_strides(long long a, long long b) { return a >= 0 && b >= 0 && a % 8 == 0 && b % 8 == 0 && a < (1ll << 40) && b < (1ll << 40); }
 
+// Whether no two of an output's rows of 128 values share one: row t, head h at t * row + h * head. Strides that are not
+// negative meet only where t grows and h shrinks, so each distance of heads is held against the nearest of rows.
+bool rows_apart(long long rows, long long heads, long long row, long long head) {
+  if (rows > 1 && row < HEAD_DIM) return false;
+  if (head >= HEAD_DIM && (rows <= 1 || row >= (heads - 1) * head + HEAD_DIM)) return true;   // heads within rows
+  for (long long h = 1; h < heads; ++h) {
+    const long long at = h * head, t = rows > 1 ? std::min(at / row, rows - 1) : 0;
+    if (at - t * row < HEAD_DIM) return false;
+    if (t + 1 < rows && (t + 1) * row - at < HEAD_DIM) return false;
+  }
+  return true;
+}
+
 // What both attention entry points check: heads, strides (elements), alignment, scale, workspace.
 int ragged_common(RaggedParams* p, const qk_ragged_attention_t& a) {
   const long long n_kv = a.cache.n_kv;
@@ -55,6 +68,8 @@ int ragged_common(RaggedParams* p, const qk_ragged_attention_t& a) {
   if (a.max_q < 1) return fail(QK_EINVAL, "max_q=%lld", a.max_q);
   if (!aligned(a.q, 16) || !aligned(a.out, 16) || !row_strides(a.q_row, a.q_head) || !row_strides(a.out_row, a.out_head))
     return fail(QK_EINVAL, "q and out rows and heads must start on 16-byte boundaries");
+  if (!rows_apart(a.rows, a.n_q, a.out_row, a.out_head))
+    return fail(QK_EINVAL, "rows of out overlap: row stride %lld, head stride %lld", a.out_row, a.out_head);
   if (a.workspace_bytes < qk_ragged_attention_workspace_bytes() || !aligned(a.workspace, 256))
     return fail(QK_EINVAL, "workspace of %lld bytes: %lld needed, 256-byte aligned", a.workspace_bytes, qk_ragged_attention_workspace_bytes());
   p->q = static_cast<const bf16*>(a.q);
@@ -230,7 +245,7 @@ int qk_paged_kv_read(const qk_paged_kv_read_t* args, qk_stream_t stream) {
   if (!a.k_out || !a.v_out) return fail(QK_EINVAL, "null pointer argument");
   if (a.rows < 0 || a.rows > 0x7fffffffll / 64) return fail(QK_EINVAL, "rows=%lld", a.rows);
   if (int r = paged_cache(&p.c, a.cache, false)) return r;
-  if (a.row_stride < HEAD_DIM || (a.head_stride < HEAD_DIM && p.c.n_kv > 1) || !row_strides(a.row_stride, a.head_stride) ||
+  if (a.row_stride < HEAD_DIM || !row_strides(a.row_stride, a.head_stride) || !rows_apart(a.rows, p.c.n_kv, a.row_stride, a.head_stride) ||
       !aligned(a.k_out, 16) || !aligned(a.v_out, 16))
     return fail(QK_EINVAL, "row_stride=%lld head_stride=%lld: rows must not overlap and start on 16-byte boundaries", a.row_stride, a.head_stride);
   if (a.rows == 0 || p.c.B == 0) return QK_OK;

@@ -95,3 +95,38 @@ def test_host_threads_share_a_stream():
     for i in range(4):
         for outs in got[i]:
             assert all(same(a, b) for a, b in zip(outs, want[i][0]))
+
+
+def test_outputs_of_any_order():
+    """Rows within heads, heads within rows, and the two laid between each other (rows 256 apart, heads 384): the same
+    bits; expanded outputs are refused."""
+    k = ops()
+    g = torch.Generator(device=DEV).manual_seed(3)
+    lens, n_q, n_kv = [100], 8, 2
+    c, _ = make_cache(lens, n_kv, 16, False, g)
+    cu, sl = ints([0, 3]), ints(lens)
+    q = torch.randn(3, n_q, D, generator=g, device=DEV).to(torch.bfloat16)
+    kv = torch.randn(2, 3, n_kv, D, generator=g, device=DEV).to(torch.bfloat16)
+
+    def run(out, ko, vo):
+        k.paged_attention(q, cu, sl, c["table"], c["k"], c["v"], out, D ** -0.5, 3)
+        k.paged_kv_read(cu, c["table"], c["k"], c["v"], ko, vo)
+        both = torch.empty_like(q).copy_(out)
+        k.packed_attention(q, kv[0], kv[1], cu, out, D ** -0.5, 3)
+        return both, torch.empty_like(q).copy_(out), ko.contiguous(), vo.contiguous()
+
+    def empty(heads, row, head):
+        return torch.empty(3 * row + heads * head, dtype=torch.bfloat16, device=DEV).as_strided((3, heads, D), (row, head, 1))
+
+    want = run(*(empty(h, h * D, D) for h in (n_q, n_kv, n_kv)))
+    for row, head in ((D, 3 * D), (1200, D), (D, 400), (256, 384 * 2)):
+        got = run(*(empty(h, row, head) for h in (n_q, n_kv, n_kv)))
+        assert all(same(a, b) for a, b in zip(got, want))
+    between = [torch.empty(4096, dtype=torch.bfloat16, device=DEV).as_strided((3, n_kv, D), (256, 384, 1)) for _ in range(2)]
+    k.paged_kv_read(cu, c["table"], c["k"], c["v"], *between)
+    assert all(same(a.contiguous(), b) for a, b in zip(between, want[2:]))
+    with pytest.raises(RuntimeError, match="overlap"):
+        k.paged_attention(q, cu, sl, c["table"], c["k"], c["v"], q[:1].expand(3, -1, -1), D ** -0.5, 3)
+    with pytest.raises(RuntimeError, match="overlap"):
+        k.packed_attention(q, kv[0], kv[1], cu, q[:, :1].expand(-1, n_q, -1), D ** -0.5, 3)
+    assert k.device_error() == 0

@@ -211,3 +211,23 @@ def test_a_capture_never_takes_the_streams_own_workspace(shim, monkeypatch):
             call()
         call(workspace=gpu(torch.zeros(512, dtype=torch.uint8)))
     assert len(shim.lib.calls) == 4
+
+
+OVERLAPS = [dict(row=0, head=128), dict(row=4096, head=0), dict(row=64, head=4096), dict(row=128, head=128), dict(row=4096, head=64),
+            dict(row=512, head=128), dict(row=128, head=256), dict(row=384, head=256)]
+
+
+@pytest.mark.parametrize("bad", OVERLAPS, ids=str)
+def test_outputs_whose_rows_overlap_are_refused(bad):
+    """An expanded output, or one whose rows and heads run into each other: what it would hold depends on the order of
+    the stores. (8 rows of 8 heads; every call is refused before a launch.)"""
+    import os
+    import kernels
+    if not os.path.exists(kernels.LIB_PATH):
+        pytest.skip("library not built (run __graft_entry__.build())")
+    lib, (row, head) = kernels.load_library(), bad.values()
+    cache = (256, 256, 0, 0, 256, 256, 256, 2, 8, 10, 16, 4, 4, 0)
+    att = kernels._ATTENTION_ARGS.pack(*cache, 256, 256, 256, 256, 256, 8, 8, 8, 1024, 128, 1024, 128, row, head, 1 << 40, 0.1)
+    for f, args in ((lib.qk_paged_attention, att), (lib.qk_packed_attention, att),
+                    (lib.qk_paged_kv_read, kernels._READ_ARGS.pack(*cache, 0, 256, 256, 8, row, head))):
+        assert f(args, 0) == 1 and b"overlap" in lib.qk_last_error()
