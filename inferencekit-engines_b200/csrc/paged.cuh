@@ -39,21 +39,6 @@ __device__ __forceinline__ int seq_of_row(const int* cu, int B, int t, int lane)
   return lo;
 }
 
-// 8 floats of a row whose largest magnitude is amax, s = amax / 448 -> 8 e4m3 bytes x / s, round to nearest even (a zero
-// row gives zeros). One division a row: x * (448 / amax) is x / s to an ulp and a half of fp32, which can move a value
-// across a rounding boundary of e4m3 (2^20 times coarser) only where it lay on it but for fp32's own rounding of s.
-__device__ __forceinline__ uint2 quant8(const float (&x)[8], float amax, float s) {
-  const bool plain = amax >= 1e-30f;          // 448 / amax is finite; otherwise tiny, zero or NaN rows
-  const float inv = plain ? __fdiv_rn(448.f, amax) : 0.f;
-  uint32_t h[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float a = x[2 * j] * inv, b = x[2 * j + 1] * inv;
-    if (!plain) a = s != 0.f ? __fdiv_rn(x[2 * j], s) : 0.f, b = s != 0.f ? __fdiv_rn(x[2 * j + 1], s) : 0.f;
-    h[j] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-  }
-  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
-}
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -113,6 +98,27 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+
+// 8 floats (as packed pairs) of a row whose largest magnitude is amax, s = amax / 448 -> 8 e4m3 bytes: the fp32 quotients x / s,
+// rounded to nearest even (a zero row gives zeros). bf16 rows lie on ties of e4m3 often, so the quotient has to be the
+// rounded one: x * (1 / s) is off by an ulp here and there, and a correction by its remainder x - q s, which an fma
+// gives exactly, makes it right (Markstein, IBM J. Res. Dev. 34, 1990). Rows whose remainders could fall below fp32's
+// range, and those with an infinity or NaN, are divided.
+__device__ __forceinline__ uint2 quant8(const uint64_t (&x)[4], float amax, float s) {
+  uint32_t h[4];
+  const bool plain = amax >= 1e-20f && amax < INFINITY;
+  const float r = plain ? __frcp_rn(s) : 0.f;
+  const uint64_t inv = f32x2(r, r), neg = f32x2(-s, -s);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint64_t q = mul2(x[j], inv);
+    q = fma2(fma2(q, neg, x[j]), inv, q);
+    float a = f32x2_lo(q), b = f32x2_hi(q);
+    if (!plain) a = s != 0.f ? __fdiv_rn(f32x2_lo(x[j]), s) : 0.f, b = s != 0.f ? __fdiv_rn(f32x2_hi(x[j]), s) : 0.f;
+    h[j] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  }
+  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
 
 struct PagedQkvParams {
@@ -268,7 +274,7 @@ __global__ void __launch_bounds__(256, 4) paged_qkv_kernel(const __grid_constant
           for (int j = 0; j < 8; j += 2) a = max3_nan(a, fabsf(x[j]), fabsf(x[j + 1]));
           a = half_max(a);
           const float s = __fdiv_rn(a, 448.f);
-          const uint2 q = quant8(x, a, s);
+          const uint2 q = quant8(x2, a, s);
           if (on) *reinterpret_cast<uint2*>(pool + row * HEAD_DIM + d0) = q;
           if (on && sub == 0) (KIND == ROW_K ? p.c.ks : p.c.vs)[row] = s;
         } else if (on) {
