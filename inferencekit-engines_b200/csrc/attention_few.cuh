@@ -16,9 +16,10 @@
 //    fill a quarter, with twice the MMAs and accumulators. P^T turns from one's result into the other's operand with a
 //    movmatrix. A tcgen05 tile of 128 rows would hold 4 in use and pass every score through TMEM.
 //  * bf16 cache: bf16 MMAs, P rounded to bf16. e4m3 cache: the bytes become f16 exactly; q is scaled to f16 range by
-//    a power of two per row; the K scale multiplies the score in fp32; P times the V scale is brought into f16 range
-//    by a running power of two, 2^15 at most, so what falls below f16's smallest value is below 2^-39 of the row's
-//    largest weight. The conversions (4 issue cycles for two values) are what bounds this path beside HBM.
+//    a power of two per row; the K scale multiplies the score in fp32; P times the V scale is brought into f16 range,
+//    to at most 2^15, by a running power of two per row, so what falls below f16's smallest value is below 2^-39 of the row's
+//    largest weight times V scale, whatever the scales are. The conversions (4 issue cycles for two values) are what
+//    bounds this path beside HBM.
 #pragma once
 #include "gemm_tc.cuh"     // tma_load_2d
 #include "paged.cuh"
@@ -89,8 +90,22 @@ struct FewShape {
   // its stages' barriers, and a wait by parity cannot mistake one phase for the one two before it.
   static constexpr int S = FEW_RING / (2 * TILE) / GROUPS * GROUPS;
   static_assert(S >= GROUPS && S > 0, "every group needs a stage");
-  static constexpr int THREADS = CW * 32 + 32;
+  // 16 rows need more registers than nine warps can have (168 each: three of them share a scheduler's); with three idle
+  // warps beside the loading one the three warpgroups have 384 x 168, which become 256 x 208 and 128 x 88 (16 sequences
+  // of 4 tokens at 16k, e4m3: 114 us; 135 without). 8 rows fit.
+  static constexpr bool SPLIT = NT == 2;
+  static constexpr int THREADS = CW * 32 + (SPLIT ? 128 : 32);
+  static constexpr int CONSUMER = 208, PRODUCER = 88;
+  static_assert(256 * CONSUMER + 128 * PRODUCER <= 384 * 168, "setmaxnreg would wait for ever");
 };
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 template <bool FP8, int NT>
 struct FewSmem {
   using Sh = FewShape<FP8, NT>;
@@ -229,7 +244,9 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
   int g = (int)((u0 - start) / n), t0 = (int)((u0 - start) - (long long)g * n);
   const uint32_t bytes_row = FP8 ? HEAD_DIM : 2 * HEAD_DIM;
 
-  if (warp == CW) {   // ---- producer ----
+  if (warp >= CW) {   // ---- producer ----
+    if constexpr (Sh::SPLIT) regs_dec<Sh::PRODUCER>();
+    if (warp > CW) return;
     const int RB = min(1 << r.c.page_shift, KEYS), boxes = KEYS / RB;
     int it = 0;
     bool ok = true;
@@ -290,6 +307,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
   }
 
   // ---- consumers ----
+  if constexpr (Sh::SPLIT) regs_inc<Sh::CONSUMER>();
   const int grp = warp / (KEYS / KW), part = warp % (KEYS / KW), lg = lane >> 2, lt = lane & 3;
   const float sl2 = r.scale * LOG2E;
   bool ok = true;
@@ -343,13 +361,17 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
       }
     }
     float o[8][NT][4], m[NT][2], l[NT][2];
-    int ev = -100;                          // fp8: P is multiplied by the V scale over 2^ev
+    // fp8: the largest weight times V scale of each row so far, under the running maximum; P times the V scale is taken over
+    // the power of two above it
+    float big[NT][2];
+    auto unit = [](float x) { return max(exponent_above(x), -100); };
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
       m[nt][0] = m[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = 0.f;
+      big[nt][0] = big[nt][1] = 0.f;
     }
     for (int t = t0; t < t1; ++t, ++it) {
       if (GROUPS > 1 && it % GROUPS != grp) continue;
@@ -396,7 +418,6 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
         }
         float kscale[KT][2], vscale[KT][2];
         if (FP8) {
-          float vmax = 0.f;
 #pragma unroll
           for (int j = 0; j < KT; ++j)
 #pragma unroll
@@ -404,22 +425,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
               const int key = part * KW + 16 * j + 8 * hh + lg;
               kscale[j][hh] = sm.ks[st][key];
               vscale[j][hh] = t * KEYS + key < s.len ? sm.vs[st][key] : 0.f;
-              vmax = fmaxf(vmax, vscale[j][hh]);
             }
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, d));
-          const int e2 = exponent_above(vmax);   // the same in every lane
-          if (e2 > ev) {
-            const float f = pow2(ev - e2);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) o[i][nt][0] *= f, o[i][nt][1] *= f, o[i][nt][2] *= f, o[i][nt][3] *= f;
-            ev = e2;
-          }
-          const float dn = pow2(-ev) * 32768.f;
-#pragma unroll
-          for (int j = 0; j < KT; ++j) vscale[j][0] *= dn, vscale[j][1] *= dn;
         }
         const bool edge = j0 + KW - 1 > s.len - s.n;    // some row does not see some of the keys
         uint32_t pf[KT][NT][2];
@@ -454,6 +460,20 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
                 if (FP8) x *= vscale[j][hh];
               }
             l[nt][e] = l[nt][e] * f[e] + add;
+            if (FP8) {                      // into f16's range, each row by what its own sum is made of
+              float top = 0.f;
+#pragma unroll
+              for (int j = 0; j < KT; ++j) top = fmaxf(top, fmaxf(sc[j][nt][e], sc[j][nt][2 + e]));
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+              const int before = unit(big[nt][e]);
+              big[nt][e] = fmaxf(big[nt][e] * f[e], top);
+              const int now = unit(big[nt][e]);
+              f[e] *= pow2(before - now);   // (the exponent falls only as far as f does)
+              const float dn = pow2(-now) * 32768.f;
+#pragma unroll
+              for (int j = 0; j < KT; ++j) sc[j][nt][e] *= dn, sc[j][nt][2 + e] *= dn;
+            }
           }
           if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
 #pragma unroll
@@ -527,7 +547,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
 #pragma unroll
         for (int w = 0; w < CW; ++w) M = fmaxf(M, sm.wm[w][nt * 8 + 2 * lt + e]);
         f[nt][e] = M == -INFINITY ? 1.f : ex2(m[nt][e] - M);
-        if (FP8) f[nt][e] *= pow2(ev) * (1.f / 32768.f);
+        if (FP8) f[nt][e] *= pow2(unit(big[nt][e])) * (1.f / 32768.f);
       }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)

@@ -313,15 +313,6 @@ struct TcShape {
   static constexpr int SOFTMAX = SRC == SRC_PAGED_FP8 ? 200 : 208, OTHER = SRC == SRC_PAGED_FP8 ? 56 : 88;
   static_assert(256 * SOFTMAX + (THREADS - 256) * OTHER <= THREADS * (SRC == SRC_PAGED_FP8 ? 128 : 168), "setmaxnreg would wait for ever");
 };
-template <int N>
-__device__ __forceinline__ void regs_inc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void regs_dec() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
 template <int SRC>
 __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(const __grid_constant__ TcAttnParams p) {
   extern __shared__ __align__(1024) uint8_t tca_smem[];

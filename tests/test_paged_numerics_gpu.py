@@ -69,6 +69,32 @@ def set_rows(c, table, page, pos, K=None, V=None):
 
 
 @pytest.mark.parametrize("n", [1, 4, 70])
+@pytest.mark.parametrize("big", ["first", "middle", "last", "scattered"])
+def test_value_rows_of_very_different_size(n, big):
+    """e4m3 value rows 2^45 times the others', whose own weights are nearly zero (2^-60 and less): what the others give must
+    not be lost beside them."""
+    k = ops()
+    L, n_kv, n_q, page = 700, 2, 8, 32
+    g = torch.Generator(device=DEV).manual_seed(n)
+    c, _ = make_cache([L], n_kv, page, True, g)
+    K, V = (torch.randn(L, n_kv, D, generator=g, device=DEV) for _ in range(2))
+    K[:, :, 0] = 3.0
+    at = {"first": [0], "middle": [333], "last": [L - n], "scattered": [5, 130, 131, 400, 601]}[big]
+    V[at] *= 2.0 ** 45
+    K[at, :, 0] = -3.0
+    pos = torch.arange(L, device=DEV)
+    K, V = set_rows(c, c["table"], page, pos, K.to(torch.bfloat16), V.to(torch.bfloat16))
+    q = torch.randn(n, n_q, D, generator=g, device=DEV)
+    q[:, :, 0] = 90.0                                # 6 x 90 / sqrt(128) = 47.7, a factor of 2^-68 before the rest's few
+    q = q.to(torch.bfloat16)
+    out = torch.empty_like(q)
+    k.paged_attention(q, ints([0, n]), ints([L]), c["table"], c["k"], c["v"], out, D ** -0.5, n, k_scale=c["ks"], v_scale=c["vs"])
+    want, A, reach = attend64(q.double(), K, V, L - n, D ** -0.5)
+    assert (want.abs() / 2.0 ** 30).max() < 1        # (the large rows are not what the answer is)
+    check(out, want, A, reach, 11 if n * n_q // n_kv <= 16 else 8)
+
+
+@pytest.mark.parametrize("n", [1, 4, 70])
 def test_weights_and_value_rows_that_balance(n):
     """Scores that rise by 40 in steps while the value rows fall by as much: every step counts alike in the output."""
     k = ops()
