@@ -11,9 +11,10 @@
 //    thread owns one row: it reads its 128 scores with tcgen05.ld, keeps the running maximum m and sum l, writes
 //    P = exp2(S - m) as bf16 over S in TMEM; O += P V reads P from TMEM and V from shared memory (dims contiguous:
 //    the MN-major operand). P's rounding to bf16 is what the matrix unit takes; l sums the fp32 values.
-//  * O stays in TMEM. Its rows are multiplied by exp2(m_old - m_new) only when a maximum grew by more than 2^32 in
-//    weight: until then the old m serves. P, l and O have fp32's exponents, so a P of up to 2^32 is as exact as one of 1;
-//    the rescale becomes rare, and a tile's exponentials need not wait for its maximum.
+//  * O stays in TMEM. Its rows are multiplied by exp2(m_old - m_new) only when a maximum grew by more than 2^8 in
+//    weight: until then the old m serves. P, l and O have fp32's exponents, so a P of up to 2^8 is as exact as one of 1;
+//    the rescale becomes rare, and a tile's exponentials need not wait for its maximum. Sums before the division by l
+//    can pass fp32's largest value where V's values times the keys that count are above 2^120.
 //  * Warps: 0-3 and 4-7 the softmax of the two tiles, 8 the loads (TMA, 128-byte swizzle, a ring of five 32 KB K and V
 //    tiles), 9 issues the MMAs from one thread (10 clears V rows past a sequence's end, 11 fills the warpgroup, which
 //    gives registers to the softmax): Q0 K0, Q1 K0, then per key tile P0 V, Q0 K', P1 V, Q1 K', with P in two parts, the
@@ -41,7 +42,7 @@ constexpr int TCA_TILE = TCA_KEYS * HEAD_DIM * 2;   // 32 KB: two 64-dim halves 
 constexpr int TCA_MIN_PIECE = 4;          // tiles
 constexpr int TCA_UNIT_COST = 2;          // what a unit costs beside its key tiles (Q load, first scores, output), in tiles
 constexpr int TCA_FIRST = 6;              // 16-key steps of P handed over first, of 8 (one prompt of 8,192 tokens: 432 us; 443 with 4, 450 with 2)
-constexpr float TCA_LAZY = 32.f;          // log2 of the growth that a stale maximum may hide
+constexpr float TCA_LAZY = 8.f;           // log2 of the growth that a stale maximum may hide
 
 enum { SRC_PACKED = 0, SRC_PAGED = 1, SRC_PAGED_FP8 = 2 };
 

@@ -115,6 +115,30 @@ def test_weights_and_value_rows_that_balance(n):
     check(out, *attend64(q.double(), K, V, L - n, D ** -0.5), 11 if n * n_q // n_kv <= 16 else 8)
 
 
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "e4m3"])
+@pytest.mark.parametrize("n", [1, 4, 200])
+def test_large_values_under_rising_scores(n, fp8):
+    """Values of 2^100 while the running maximum rises by 2^26 in weight a tile: sums stay finite."""
+    k = ops()
+    L, n_kv, n_q, page = 1500, 2, 8, 64
+    g = torch.Generator(device=DEV).manual_seed(n)
+    c, _ = make_cache([L], n_kv, page, fp8, g)
+    K, V = (torch.randn(L, n_kv, D, generator=g, device=DEV) for _ in range(2))
+    K[:, :, 0] = torch.linspace(-40, 40, L, device=DEV)[:, None]
+    pos = torch.arange(L, device=DEV)
+    K, V = set_rows(c, c["table"], page, pos, K.to(torch.bfloat16), (V * 2.0 ** 100).to(torch.bfloat16))
+    q = torch.randn(n, n_q, D, generator=g, device=DEV)
+    q[:, :, 0] = 30
+    q = q.to(torch.bfloat16)
+    out = torch.empty_like(q)
+    k.paged_attention(q, ints([0, n]), ints([L]), c["table"], c["k"], c["v"], out, D ** -0.5, n, k_scale=c["ks"], v_scale=c["vs"])
+    check(out, *attend64(q.double(), K, V, L - n, D ** -0.5), 11 if fp8 and n * n_q // n_kv <= 16 else 8)
+    if not fp8:
+        q, kk, v = (x.to(torch.bfloat16) for x in (q.expand(n, -1, -1), K[:n].contiguous(), V[:n].contiguous()))
+        k.packed_attention(q, kk, v, ints([0, n]), out, D ** -0.5, n)
+        check(out, *attend64(q.double(), kk.double(), v.double(), 0, D ** -0.5), 8)
+
+
 @pytest.mark.parametrize("amax", ["normal", "multiples of 7", "tiny", "huge"])
 def test_e4m3_rows_are_the_rounded_quotients(amax):
     """Stored rows to the bit: s = max|x| / 448 and q = e4m3(x / s), each rounded once from fp32 quotients. bf16 rows lie on
