@@ -15,11 +15,13 @@
 //    O^T = V^T P^T (m16n8k16), 8 query rows a tile of N, so a decode step's 4 heads fill half of it, where rows as M would
 //    fill a quarter, with twice the MMAs and accumulators. P^T turns from one's result into the other's operand with a
 //    movmatrix. A tcgen05 tile of 128 rows would hold 4 in use and pass every score through TMEM.
-//  * bf16 cache: bf16 MMAs, P rounded to bf16. e4m3 cache: the bytes become f16 exactly; q is scaled to f16 range by
-//    a power of two per row; the K scale multiplies the score in fp32; P times the V scale is brought into f16 range,
-//    to at most 2^15, by a running power of two per row, so what falls below f16's smallest value is below 2^-39 of the row's
-//    largest weight times V scale, whatever the scales are. The conversions (4 issue cycles for two values) are what
-//    bounds this path beside HBM.
+//  * bf16 cache: bf16 MMAs, P in two parts, its rounding to bf16 and what that leaves: 16 bits of P, more than the output
+//    shows, as in the contiguous cache's attention, whose P is fp32. 1 % more time (16 sequences at up to 32k).
+//  * e4m3 cache: the bytes become f16 exactly; q is scaled to f16 range by a power of two per row; the K scale multiplies
+//    the score in fp32; P times the V scale is rounded to f16 (11 bits: an eighth of the output's own rounding),
+//    brought to at most 2^15 by a running power of two per row, so that what falls below f16's smallest value is below 2^-39
+//    of the row's largest weight times V scale, whatever the scales are. The conversions (4 issue cycles for two values)
+//    are what bounds this path beside HBM.
 #pragma once
 #include "gemm_tc.cuh"     // tma_load_2d
 #include "paged.cuh"
@@ -428,7 +430,7 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
             }
         }
         const bool edge = j0 + KW - 1 > s.len - s.n;    // some row does not see some of the keys
-        uint32_t pf[KT][NT][2];
+        uint32_t pf[KT][NT][2], pl[FP8 ? 1 : KT][NT][2];   // bf16: and what rounding P to it leaves
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float f[2];
@@ -482,8 +484,12 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
 #pragma unroll
           for (int j = 0; j < KT; ++j)
 #pragma unroll
-            for (int hh = 0; hh < 2; ++hh)
-              pf[j][nt][hh] = transpose8x8(FP8 ? pack_f16(sc[j][nt][2 * hh], sc[j][nt][2 * hh + 1]) : pack_bf16(sc[j][nt][2 * hh], sc[j][nt][2 * hh + 1]));
+            for (int hh = 0; hh < 2; ++hh) {
+              const float a = sc[j][nt][2 * hh], e = sc[j][nt][2 * hh + 1];
+              const uint32_t p2 = FP8 ? pack_f16(a, e) : pack_bf16(a, e);
+              pf[j][nt][hh] = transpose8x8(p2);
+              if (!FP8) pl[FP8 ? 0 : j][nt][hh] = transpose8x8(pack_bf16(a - bf16lo(p2), e - bf16hi(p2)));
+            }
         }
         // O^T: 8 tiles of 16 dims
 #pragma unroll
@@ -515,7 +521,10 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
               uint32_t af[4];
               ldmatrix4_trans(af, vb + (i >> 2) * (TILE / 2) + (16 * j + row) * 128 + ((ch ^ (row & 7)) * 16));
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) few_mma<FP8>(o[i][nt], af, pf[j][nt][0], pf[j][nt][1]);
+              for (int nt = 0; nt < NT; ++nt) {
+                few_mma<FP8>(o[i][nt], af, pf[j][nt][0], pf[j][nt][1]);
+                few_mma<FP8>(o[i][nt], af, pl[FP8 ? 0 : j][nt][0], pl[FP8 ? 0 : j][nt][1]);
+              }
             }
           }
         }

@@ -10,7 +10,9 @@
 //  * One pass over the keys in tiles of 128. S = Q K^T (operands in shared memory, accumulator in TMEM); a softmax
 //    thread owns one row: it reads its 128 scores with tcgen05.ld, keeps the running maximum m and sum l, writes
 //    P = exp2(S - m) as bf16 over S in TMEM; O += P V reads P from TMEM and V from shared memory (dims contiguous:
-//    the MN-major operand). P's rounding to bf16 is what the matrix unit takes; l sums the fp32 values.
+//    the MN-major operand). P is rounded to bf16, the type of V's tile, which costs an output about as much as its own
+//    rounding (2.2e-3 together, of its norm, against 1.5e-3); P in two parts would be half as many products again, of what
+//    bounds this. l sums the fp32 values.
 //  * O stays in TMEM. Its rows are multiplied by exp2(m_old - m_new) only when a maximum grew by more than 2^8 in
 //    weight: until then the old m serves. P, l and O have fp32's exponents, so a P of up to 2^8 is as exact as one of 1;
 //    the rescale becomes rare, and a tile's exponentials need not wait for its maximum. Sums before the division by l
@@ -30,7 +32,7 @@
 //    piece; the CTA that completes the unit's count adds them in order.
 //  * An e4m3 cache: the loads bring raw tiles, and six more warps write them as bf16 tiles in the image the MMAs read: the
 //    e4m3 values, exactly. The softmax multiplies each score by its key's K scale and each P by its V scale (packed
-//    multiplications and broadcast loads). Folding the scales into the tiles, rounded to bf16, was a fifth faster and
+//    multiplications and broadcast loads); P times the V scale is what is rounded to bf16. Folding the scales into the tiles, rounded to bf16, was a fifth faster and
 //    twice as far off (3.4e-3 against 1.7e-3 for fp32 sums rounded once).
 #pragma once
 #include "attention_few.cuh"

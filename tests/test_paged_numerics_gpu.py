@@ -52,6 +52,22 @@ def test_attention_rounds_only_probabilities_and_outputs(name, fp8):
     assert rel < (1.9e-3 if few else 2.7e-3), rel
 
 
+@pytest.mark.parametrize("name", ["decode", "few_tokens"])
+def test_few_rows_over_bf16_pages_keep_their_probabilities(name):
+    """P goes to the bf16 products in two parts, its rounding and what that leaves (2^-16 of it at most is lost): the
+    output's own rounding is all that counts, as in the contiguous cache's attention."""
+    n, lens, n_q, n_kv, page = SIZES[name]
+    k = ops()
+    g = torch.Generator(device=DEV).manual_seed(len(name))
+    c, rows = make_cache(lens, n_kv, page, False, g)
+    q = (torch.randn(sum(n), n_q, D, generator=g, device=DEV) * 1.5).to(torch.bfloat16)
+    out, cu = torch.empty_like(q), cumulative(n)
+    k.paged_attention(q, ints(cu), ints(lens), c["table"], c["k"], c["v"], out, D ** -0.5, max(n))
+    want = [attend64(q[a:b].double(), *rows[i], lens[i] - n[i], D ** -0.5) for i, (a, b) in enumerate(zip(cu, cu[1:]))]
+    rel = check(out, *(torch.cat(x) for x in zip(*want)), 16)
+    assert rel < 1.9e-3, rel
+
+
 def set_rows(c, table, page, pos, K=None, V=None):
     """Overwrite positions of sequence 0; returns the rows as the cache holds them, in 64 bits."""
     pg, slot = table[0, pos // page].long(), pos % page
