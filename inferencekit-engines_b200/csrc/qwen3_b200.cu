@@ -55,6 +55,13 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
         q == cudaDriverEntryPointSuccess)
       fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
   });
+  // The encoder is a driver call and wants a context, which a host thread has only after its first runtime call that needs
+  // one. Selecting the thread's device makes it (allowed while a stream is captured).
+  static thread_local bool has_context = false;
+  if (!has_context) {
+    int dev = 0;
+    has_context = cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
+  }
   return fn;
 }
 

@@ -130,3 +130,43 @@ def test_outputs_of_any_order():
     with pytest.raises(RuntimeError, match="overlap"):
         k.packed_attention(q, kv[0], kv[1], cu, q[:, :1].expand(-1, n_q, -1), D ** -0.5, 3)
     assert k.device_error() == 0
+
+
+@pytest.mark.parametrize("what", ["decode", "mixed", "packed", "linear"])
+def test_a_call_may_be_a_threads_first(what):
+    """A new host thread whose first use of the GPU is one of the calls that build tensor maps."""
+    import threading
+    import model as M
+    k = ops()
+    g = torch.Generator(device=DEV).manual_seed(7)
+    c, _ = make_cache([300], 2, 16, False, g)
+    n = 1 if what == "decode" else 40
+    q = torch.randn(n, 8, D, generator=g, device=DEV).to(torch.bfloat16)
+    kv = torch.randn(2, n, 2, D, generator=g, device=DEV).to(torch.bfloat16)
+    cu, lens, ws = ints([0, n]), ints([300]), k.attention_workspace(DEV)
+    w = torch.randn(256, 256, generator=g, device=DEV).to(torch.float8_e4m3fn)
+    scale, x = torch.ones(256, device=DEV), torch.randn(4, 256, generator=g, device=DEV).to(torch.bfloat16)
+
+    def call(out):
+        if what == "linear":
+            k.fp8_gemm_rows(x, w, scale, out)
+        elif what == "packed":
+            k.packed_attention(q, kv[0], kv[1], cu, out, D ** -0.5, n, workspace=ws)
+        else:
+            k.paged_attention(q, cu, lens, c["table"], c["k"], c["v"], out, D ** -0.5, n, workspace=ws)
+
+    want, got = (torch.zeros_like(x if what == "linear" else q) for _ in range(2))
+    call(want)
+    failed = []
+
+    def first():
+        try:
+            call(got)
+        except RuntimeError as e:
+            failed.append(e)
+
+    t = threading.Thread(target=first)
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert not failed and same(got, want) and k.device_error() == 0
