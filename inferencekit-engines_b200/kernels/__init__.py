@@ -133,16 +133,13 @@ def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def _raw_stream(dev: int) -> int:
-    """The current stream of a device as an integer (no stream object: the paged calls' host time is their launch)."""
-    return torch._C._cuda_getCurrentRawStream(dev)
-
-
 def _launch_stream(what: str, dev: int) -> int:
-    """The stream for a call on tensors of GPU `dev`, which has to be the current one: the library launches there."""
-    if torch.cuda.current_device() != dev:
-        raise RuntimeError(f"{what}: the tensors are on GPU {dev}, the current device is {torch.cuda.current_device()}")
-    return _raw_stream(dev)
+    """The stream for a call on tensors of GPU `dev`, which has to be the current one: the library launches there; as an
+    integer (no stream object, and the bindings behind torch.cuda's functions: the paged calls' host time is their launch)."""
+    current = torch._C._cuda_getDevice()
+    if current != dev:
+        raise RuntimeError(f"{what}: the tensors are on GPU {dev}, the current device is {current}")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 _E4M3 = (torch.float8_e4m3fn, torch.uint8)
@@ -491,7 +488,7 @@ class DecodeOps:
 
     def _workspace(self, what, ws, dev, stream):
         if ws is None:   # one per device and stream, kept; never a graph's, whose replays may run beside the stream's calls
-            if torch.cuda.is_current_stream_capturing():
+            if stream and torch._C._cuda_isCurrentStreamCapturing():   # (stream 0 cannot be captured)
                 raise RuntimeError(f"{what}: pass workspace=attention_workspace(device), made before the capture")
             ws = self._scratch.get(("ragged", dev, stream))
             if ws is None:

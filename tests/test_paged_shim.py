@@ -40,8 +40,9 @@ class Library:
 @pytest.fixture
 def shim(monkeypatch):
     import kernels
-    monkeypatch.setattr(kernels, "_raw_stream", lambda dev: 0)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: 0x100)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: False)
     return kernels.DecodeOps(Library(kernels))
 
 
@@ -184,7 +185,7 @@ def paged_calls(k, index):
 def test_tensors_of_a_device_that_is_not_current_are_refused(shim, monkeypatch):
     """The library launches on the current device, where another device's pointers mean nothing."""
     for current in (0, 1):
-        monkeypatch.setattr(torch.cuda, "current_device", lambda: current)
+        monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current)
         shim.lib.calls.clear()
         for call in paged_calls(shim, current):
             call()
@@ -198,7 +199,7 @@ def test_tensors_of_a_device_that_is_not_current_are_refused(shim, monkeypatch):
 def test_a_capture_never_takes_the_streams_own_workspace(shim, monkeypatch):
     """Not even where an earlier call on the stream has made it: its replays may run beside calls that use it."""
     capturing = False
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: capturing)
     monkeypatch.setattr(shim, "attention_workspace", lambda device: gpu(torch.zeros(512, dtype=torch.uint8)))
     q, kv, pages = bf16(1, 4, 128), bf16(1, 2, 128), bf16(8, 2, 16, 128)
     attend = [lambda **kw: shim.paged_attention(q, ints([0, 1]), ints([5]), ints([[1, 2]]), pages, pages, q, 0.1, 1, **kw),
