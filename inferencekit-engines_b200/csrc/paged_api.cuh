@@ -279,8 +279,11 @@ int qk_paged_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
   // the tensor cores, which take a few rows too at the matrix unit's time for 128. 17 to 32 rows in the few-row kernel
   // took longer (16 sequences of up to 8 tokens at up to 16k: 183 us against 117; 8 at up to 400: 22 against 14), 9 to 16
   // take less (102 against 115, 20 against 34 for 4 sequences at up to 4k).
-  if (int e = fp8 ? launch_few<true, 1>(p, 0, args->workspace, st) : launch_few<false, 1>(p, 0, args->workspace, st)) return e;
-  return fp8 ? launch_tc<SRC_PAGED_FP8>(p, 9, true, args->workspace, st) : launch_tc<SRC_PAGED>(p, 9, true, args->workspace, st);
+  // From 9 query heads per KV head on no sequence has that few.
+  const bool few = p.group <= 8;
+  if (few)
+    if (int e = fp8 ? launch_few<true, 1>(p, 0, args->workspace, st) : launch_few<false, 1>(p, 0, args->workspace, st)) return e;
+  return fp8 ? launch_tc<SRC_PAGED_FP8>(p, 9, few, args->workspace, st) : launch_tc<SRC_PAGED>(p, 9, few, args->workspace, st);
 }
 
 int qk_packed_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {

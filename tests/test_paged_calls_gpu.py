@@ -170,3 +170,26 @@ def test_a_call_may_be_a_threads_first(what):
     t.join()
     torch.cuda.synchronize()
     assert not failed and same(got, want) and k.device_error() == 0
+
+
+@pytest.mark.parametrize("n_q,n,launches", [(8, 1, 1), (16, 1, 1), (8, 40, 2), (9, 2, 1), (16, 2, 1), (32, 1, 1), (32, 40, 1)])
+def test_launches_of_a_call(n_q, n, launches):
+    """One KV head. A mixed batch is two launches where some sequence can have few rows: one token has more than 8 of them
+    from 9 query heads per KV head on."""
+    import ctypes
+    k = ops()
+    g = torch.Generator(device=DEV).manual_seed(n_q)
+    c, _ = make_cache([300, 70], 1, 16, False, g)
+    q = torch.randn(2 * n, n_q, D, generator=g, device=DEV).to(torch.bfloat16)
+    out, cu, lens, ws = torch.empty_like(q), ints([0, n, 2 * n]), ints([300, 70]), k.attention_workspace(DEV)
+
+    def call():
+        k.paged_attention(q, cu, lens, c["table"], c["k"], c["v"], out, D ** -0.5, n, workspace=ws)
+
+    call()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    nodes = ctypes.c_size_t(0)
+    assert ctypes.CDLL("libcudart.so.12").cudaGraphGetNodes(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(nodes)) == 0
+    assert nodes.value == launches
