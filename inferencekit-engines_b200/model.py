@@ -225,9 +225,11 @@ def rope_angles(max_pos: int, rot_dim: int, theta: float, device, scaling: dict 
     scaling, for contexts past the trained length:
       {"type": "linear", "factor": f}: positions divided by f;
       {"type": "yarn", "factor": f, "original_max_position": n, "beta_fast": 32, "beta_slow": 1, "attention_factor":
-      0.1 ln f + 1}: a frequency that turns more than beta_fast times over the n trained positions stays, one that
-      turns less than beta_slow times is divided by f, between them a ramp linear in the number of turns; cos and sin
-      times the attention factor (YaRN's interpolation by parts)."""
+      0.1 ln f + 1, "ramp": "turns"}: a frequency that turns more than beta_fast times over the n trained positions stays, one
+      that turns less than beta_slow times is divided by f, a mixture between them, linear in the number of turns (the
+      paper's interpolation by parts) or, with "ramp": "dims", in the pair's index between the two corners, rounded
+      outwards to whole indices: what models whose configuration says "yarn" (Qwen3's factor 4 from 32,768) are commonly
+      served with. At theta 1e6 and 128 dims the two differ in pairs 24 to 39. cos and sin times the attention factor."""
     if rot_dim % 16 or not 16 <= rot_dim <= 128:
         raise ValueError(f"rot_dim must be a multiple of 16 up to 128, got {rot_dim}")
     inv = theta ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
@@ -239,11 +241,19 @@ def rope_angles(max_pos: int, rot_dim: int, theta: float, device, scaling: dict 
         if kind == "linear":
             inv = inv / f
         else:
-            fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
-            turns = scaling["original_max_position"] * inv / (2 * math.pi)
-            keep = ((turns - slow) / (fast - slow)).clamp(0, 1)
+            n, fast, slow = (scaling.get(k, d) for k, d in (("original_max_position", 0), ("beta_fast", 32.0), ("beta_slow", 1.0)))
+            ramp, mul = scaling.get("ramp", "turns"), scaling.get("attention_factor", 0.1 * math.log(f) + 1.0)
+            known = {"type", "factor", "original_max_position", "beta_fast", "beta_slow", "attention_factor", "ramp"}
+            if set(scaling) - known or ramp not in ("turns", "dims") or None in (n, fast, slow, mul) or not (n > 0 and fast > slow > 0):
+                raise ValueError(f"unsupported rope scaling {scaling!r}")
+            if ramp == "turns":
+                keep = ((n * inv / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+            else:   # pair i turns n theta^(-2i / rot_dim) / 2 pi times: the indices of `fast` and `slow` turns
+                first, last = (rot_dim * math.log(n / (2 * math.pi * t)) / (2 * math.log(theta)) for t in (fast, slow))
+                first = max(0, math.floor(first))
+                last = max(first, min(rot_dim - 1, math.ceil(last)))
+                keep = 1 - ((torch.arange(rot_dim // 2, dtype=torch.float64) - first) / max(last - first, 1e-3)).clamp(0, 1)
             inv = inv * keep + inv / f * (1 - keep)
-            mul = float(scaling.get("attention_factor", 0.1 * math.log(f) + 1.0))
     a = torch.arange(max_pos, device=device, dtype=torch.float64)[:, None] * inv.to(device)[None]
     return (a.cos() * mul).float().contiguous(), (a.sin() * mul).float().contiguous()
 
