@@ -38,3 +38,46 @@ def test_the_decode_graph_beside_larger_passes():
         out.append((toks, other, eng.k_pages.clone()))
     assert out[0][:2] == out[1][:2]
     assert torch.equal(out[0][2].view(torch.int16), out[1][2].view(torch.int16))
+
+
+def test_export_follows_the_contiguous_engine():
+    """The exported rows under the reference's own tokens, one by one: its logits at every step."""
+    from generate import Engine
+    from paged import PagedEngine
+    prompt, steps = [(11 * i + 3) % 4096 for i in range(137)], 5
+    e = Engine(model())
+    e.prefill(prompt, use_graph=False)
+    toks, logits = [int(e.token)], []
+    for _ in range(steps):
+        e.decode_step()
+        toks.append(int(e.token))
+        logits.append(e.logits.float().clone())
+    e.check()
+    eng = PagedEngine(model(), pages=16, page_size=32, max_rows=256)
+    s = eng.new()
+    eng.step([(s, prompt)])
+    m = model()
+    eng.export(s, m.k_cache[:, 0], m.v_cache[:, 0])
+    eng.check()
+    e = Engine(m)
+    e.state.copy_(torch.tensor([len(prompt), 0], dtype=torch.int32))
+    for t, want in zip(toks, logits):
+        e.token.fill_(t)
+        e.decode_step()
+        rel = ((e.logits.float() - want).norm() / want.norm()).item()
+        assert rel < 0.1, rel            # W8A8 under other summation orders and fp32 angles
+    e.check()
+
+
+@pytest.mark.parametrize("cut", [1, 50, 136])
+def test_a_prompt_in_two_passes(cut):
+    """bf16 pages: the logits of a prompt do not depend on where it was cut but for the summation order."""
+    from paged import PagedEngine
+    prompt = [(17 * i + 5) % 4096 for i in range(137)]
+    eng = PagedEngine(model(), pages=16, page_size=32, max_rows=256)
+    a, b = eng.new(), eng.new()
+    eng.step([(a, prompt)])
+    want = eng.logits[0].float().clone()
+    eng.step([(b, prompt[:cut])])
+    eng.step([(b, prompt[cut:])])
+    assert ((eng.logits[0].float() - want).norm() / want.norm()).item() < 0.1
