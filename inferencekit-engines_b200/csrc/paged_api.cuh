@@ -42,6 +42,8 @@ int paged_cache(PagedCache* c, const qk_paged_cache_t& a, bool lens) {
   return QK_OK;
 }
 
+// A dimension of one has no stride of its own: whatever it says, it is taken for that of contiguous rows.
+long long own_stride(long long size, long long stride, long long contiguous) { return size == 1 ? contiguous : stride; }
 bool row_strides(long long a, long long b) { return a >= 0 && b >= 0 && a % 8 == 0 && b % 8 == 0 && a < (1ll << 40) && b < (1ll << 40); }
 
 // Whether no two of an output's rows of 128 values share one: row t, head h at t * row + h * head. Strides that are not
@@ -66,19 +68,18 @@ int ragged_common(RaggedParams* p, const qk_ragged_attention_t& a) {
   const float scale = (float)a.scale;
   if (!(scale > 1e-30f) || !(scale < 1e30f)) return fail(QK_EINVAL, "scale=%g must be positive", a.scale);
   if (a.max_q < 1) return fail(QK_EINVAL, "max_q=%lld", a.max_q);
-  if (!aligned(a.q, 16) || !aligned(a.out, 16) || !row_strides(a.q_row, a.q_head) || !row_strides(a.out_row, a.out_head))
+  p->q_row = own_stride(a.rows, a.q_row, a.n_q * HEAD_DIM);
+  p->q_head = own_stride(a.n_q, a.q_head, HEAD_DIM);
+  p->out_row = own_stride(a.rows, a.out_row, a.n_q * HEAD_DIM);
+  p->out_head = own_stride(a.n_q, a.out_head, HEAD_DIM);
+  if (!aligned(a.q, 16) || !aligned(a.out, 16) || !row_strides(p->q_row, p->q_head) || !row_strides(p->out_row, p->out_head))
     return fail(QK_EINVAL, "q and out rows and heads must start on 16-byte boundaries");
-  if (!rows_apart(a.rows, a.n_q, a.out_row, a.out_head))
-    return fail(QK_EINVAL, "rows of out overlap: row stride %lld, head stride %lld", a.out_row, a.out_head);
+  if (!rows_apart(a.rows, a.n_q, p->out_row, p->out_head))
+    return fail(QK_EINVAL, "rows of out overlap: row stride %lld, head stride %lld", p->out_row, p->out_head);
   if (a.workspace_bytes < qk_ragged_attention_workspace_bytes() || !aligned(a.workspace, 256))
     return fail(QK_EINVAL, "workspace of %lld bytes: %lld needed, 256-byte aligned", a.workspace_bytes, qk_ragged_attention_workspace_bytes());
   p->q = static_cast<const bf16*>(a.q);
   p->out = static_cast<bf16*>(a.out);
-  // a dimension of one has no stride of its own
-  p->q_row = a.rows == 1 ? a.n_q * HEAD_DIM : a.q_row;
-  p->q_head = a.n_q == 1 ? HEAD_DIM : a.q_head;
-  p->out_row = a.out_row;
-  p->out_head = a.out_head;
   p->T = (int)a.rows;
   p->n_q = (int)a.n_q;
   p->group = (int)(a.n_q / n_kv);
@@ -206,8 +207,12 @@ int qk_paged_qkv(const qk_paged_qkv_t* args, qk_stream_t stream) {
     return fail(QK_EINVAL, "rotary dims %lld must be a multiple of 16, at most %d", 2 * a.rot_half, HEAD_DIM);
   if (a.max_pos < 1 || a.max_pos > 0x7fffffffll) return fail(QK_EINVAL, "max_pos=%lld", a.max_pos);
   if (int r = paged_cache(&p.c, a.cache, true)) return r;
-  if (a.qkv_stride < (a.n_q + 2 * p.c.n_kv) * HEAD_DIM || a.q_stride < a.n_q * HEAD_DIM ||
-      (a.k_out && a.k_stride < (long long)p.c.n_kv * HEAD_DIM) || !row_strides(a.qkv_stride, a.q_stride) || !row_strides(a.k_stride, 0))
+  const long long w_qkv = (a.n_q + 2 * p.c.n_kv) * HEAD_DIM, w_q = a.n_q * HEAD_DIM, w_k = (long long)p.c.n_kv * HEAD_DIM;
+  p.qkv_stride = own_stride(a.rows, a.qkv_stride, w_qkv);
+  p.q_stride = own_stride(a.rows, a.q_stride, w_q);
+  p.k_stride = own_stride(a.rows, a.k_stride, w_k);
+  if (p.qkv_stride < w_qkv || p.q_stride < w_q || (a.k_out && p.k_stride < w_k) || !row_strides(p.qkv_stride, p.q_stride) ||
+      !row_strides(p.k_stride, 0))
     return fail(QK_EINVAL, "rows overlap or do not start on 16-byte boundaries: qkv_stride=%lld q_stride=%lld k_stride=%lld",
                 a.qkv_stride, a.q_stride, a.k_stride);
   if (!aligned(a.qkv, 16) || !aligned(a.q_out, 16) || !aligned(a.k_out, 16) || !aligned(a.q_norm, 16) || !aligned(a.k_norm, 16) ||
@@ -221,9 +226,6 @@ int qk_paged_qkv(const qk_paged_qkv_t* args, qk_stream_t stream) {
   p.k_norm = static_cast<const bf16*>(a.k_norm);
   p.cos = a.cos_tab;
   p.sin = a.sin_tab;
-  p.qkv_stride = a.qkv_stride;
-  p.q_stride = a.q_stride;
-  p.k_stride = a.k_stride;
   p.T = (int)a.rows;
   p.n_q = (int)a.n_q;
   p.max_pos = (int)a.max_pos;
@@ -245,15 +247,15 @@ int qk_paged_kv_read(const qk_paged_kv_read_t* args, qk_stream_t stream) {
   if (!a.k_out || !a.v_out) return fail(QK_EINVAL, "null pointer argument");
   if (a.rows < 0 || a.rows > 0x7fffffffll / 64) return fail(QK_EINVAL, "rows=%lld", a.rows);
   if (int r = paged_cache(&p.c, a.cache, false)) return r;
-  if (a.row_stride < HEAD_DIM || !row_strides(a.row_stride, a.head_stride) || !rows_apart(a.rows, p.c.n_kv, a.row_stride, a.head_stride) ||
+  p.row_stride = own_stride(a.rows, a.row_stride, (long long)p.c.n_kv * HEAD_DIM);
+  p.head_stride = own_stride(p.c.n_kv, a.head_stride, HEAD_DIM);
+  if (p.row_stride < HEAD_DIM || !row_strides(p.row_stride, p.head_stride) || !rows_apart(a.rows, p.c.n_kv, p.row_stride, p.head_stride) ||
       !aligned(a.k_out, 16) || !aligned(a.v_out, 16))
     return fail(QK_EINVAL, "row_stride=%lld head_stride=%lld: rows must not overlap and start on 16-byte boundaries", a.row_stride, a.head_stride);
   if (a.rows == 0 || p.c.B == 0) return QK_OK;
   p.starts = a.starts;
   p.k_out = static_cast<bf16*>(a.k_out);
   p.v_out = static_cast<bf16*>(a.v_out);
-  p.row_stride = a.row_stride;
-  p.head_stride = a.head_stride;
   p.T = (int)a.rows;
   dim3 grid;
   if (int r = warp_grid(a.rows, &grid)) return r;
@@ -293,13 +295,13 @@ int qk_packed_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
   if (int r = ragged_common(&p, a)) return r;
   if (!a.k || !a.v || !a.cache.cu_rows) return fail(QK_EINVAL, "null pointer argument");
   if (a.cache.batch < 0 || a.cache.batch > 65536) return fail(QK_EINVAL, "batch=%lld", a.cache.batch);
-  if (!aligned(a.k, 16) || !aligned(a.v, 16) || !row_strides(a.kv_row, a.kv_head))
+  p.kv_row = own_stride(a.rows, a.kv_row, a.cache.n_kv * HEAD_DIM);
+  p.kv_head = own_stride(a.cache.n_kv, a.kv_head, HEAD_DIM);
+  if (!aligned(a.k, 16) || !aligned(a.v, 16) || !row_strides(p.kv_row, p.kv_head))
     return fail(QK_EINVAL, "k and v rows and heads must start on 16-byte boundaries");
   if (p.T == 0 || a.cache.batch == 0) return QK_OK;
   p.k = static_cast<const bf16*>(a.k);
   p.v = static_cast<const bf16*>(a.v);
-  p.kv_row = a.rows == 1 ? a.cache.n_kv * HEAD_DIM : a.kv_row;
-  p.kv_head = a.cache.n_kv == 1 ? HEAD_DIM : a.kv_head;
   p.c.cu = a.cache.cu_rows;
   p.c.B = (int)a.cache.batch;
   p.c.n_kv = (int)a.cache.n_kv;

@@ -193,3 +193,31 @@ def test_launches_of_a_call(n_q, n, launches):
     nodes = ctypes.c_size_t(0)
     assert ctypes.CDLL("libcudart.so.12").cudaGraphGetNodes(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(nodes)) == 0
     assert nodes.value == launches
+
+
+def one_row(heads, row):
+    """[1, heads, D] whose row stride means nothing (a transposed vector has 1)."""
+    return torch.zeros(heads * D, dtype=torch.bfloat16, device=DEV).as_strided((1, heads, D), (row, D, 1))
+
+
+@pytest.mark.parametrize("row", [1, 0, 4100])
+def test_a_single_row_has_no_stride(row):
+    k = ops()
+    g = torch.Generator(device=DEV).manual_seed(5)
+    c, _ = make_cache([70], 2, 16, False, g)
+    cos, sin = torch.rand(2, 128, 64, generator=g, device=DEV)
+    x = torch.randn(12 * D, generator=g, device=DEV).to(torch.bfloat16)
+    cu, lens = ints([0, 1]), ints([70])
+
+    def run(row):
+        q, ko, kr, vr, o, op = (one_row(h, r) for h, r in ((8, row), (2, row), (2, row), (2, row), (8, row), (8, row)))
+        qkv = torch.empty_like(x).copy_(x).as_strided((1, 12 * D), (row, 1))
+        k.paged_qkv(qkv, cu, lens, c["table"], c["k"], c["v"], q, cos, sin, k_out=ko)
+        k.paged_kv_read(cu, c["table"], c["k"], c["v"], kr, vr, starts=ints([69]))
+        k.paged_attention(q, cu, lens, c["table"], c["k"], c["v"], o, D ** -0.5, 1)
+        k.packed_attention(q, ko, vr, cu, op, D ** -0.5, 1)
+        return [t.flatten() for t in (q, ko, kr, vr, o, op)]
+
+    want = run(12 * D)
+    assert all(same(a, b) for a, b in zip(run(row), want))
+    assert same(want[1], want[2]) and k.device_error() == 0
