@@ -221,3 +221,28 @@ def test_a_single_row_has_no_stride(row):
     want = run(12 * D)
     assert all(same(a, b) for a, b in zip(run(row), want))
     assert same(want[1], want[2]) and k.device_error() == 0
+
+
+def test_broadcast_inputs():
+    """Queries, keys and values expanded over rows or heads give what their copies give."""
+    k = ops()
+    g = torch.Generator(device=DEV).manual_seed(6)
+    c, _ = make_cache([300], 4, 32, False, g)
+    cu, lens = ints([0, 50]), ints([300])
+    x = torch.randn(50, 8, D, generator=g, device=DEV).to(torch.bfloat16)
+    rows, heads = x[:1].expand(50, -1, -1), x[:, :1].expand(-1, 8, -1)
+    for q in (rows, heads):
+        got = []
+        for t in (q, q.contiguous()):
+            out = torch.empty(50, 8, D, dtype=torch.bfloat16, device=DEV)
+            k.paged_attention(t, cu, lens, c["table"], c["k"], c["v"], out, D ** -0.5, 50)
+            got.append(out.clone())
+        assert same(*got)
+    for kv in (rows[:, :4], heads[:, :4]):
+        got = []
+        for t in (kv, kv.contiguous()):
+            out = torch.empty(50, 8, D, dtype=torch.bfloat16, device=DEV)
+            k.packed_attention(x, t, t, cu, out, D ** -0.5, 50)
+            got.append(out)
+        assert same(*got)
+    assert k.device_error() == 0
