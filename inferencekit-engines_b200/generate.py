@@ -254,14 +254,12 @@ class Engine:
     def recover(self):
         """Reset the step's scratch counters after a failed step (a wait that gave up leaves them mid-count):
         the fused step's grid-barrier, GEMV-unit and attention counters and the argmax key, or the op path's
-        counters. Call it between steps, with no launch in flight; clears the device error word."""
+        counters, and the ops' own scratch. Call it between steps, with no launch in flight; clears the device error
+        word."""
         torch.cuda.synchronize()
         for t in (self.counters, self.best) + ((self.sync, self.gemv_counters, self.part) if self.fused else ()):
             t.zero_()
-        if not self.fused:
-            for key, val in self.k._scratch.items():
-                if isinstance(val, tuple):   # the GEMV's (block dots, unit counters)
-                    val[1].zero_()
+        self.k.reset_scratch()
         torch.cuda.synchronize()
         self.k.device_error()
 

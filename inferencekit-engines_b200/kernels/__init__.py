@@ -178,6 +178,11 @@ class DecodeOps:
             self._scratch[key] = (part, counters)
         return part, counters
 
+    def reset_scratch(self):
+        """Zero the counters of every scratch and workspace of this object's, after a failed launch and with none in flight."""
+        for s in [*self._scratch.values(), *self._outgrown]:
+            (s[1] if isinstance(s, tuple) else s).zero_()   # the GEMV's (block dots, unit counters); a whole buffer
+
     def device_error(self) -> int:
         """Read and clear the device error word (bounded waits that gave up, bad state)."""
         v = ctypes.c_int(0)

@@ -232,3 +232,22 @@ def test_outputs_whose_rows_overlap_are_refused(bad):
     for f, args in ((lib.qk_paged_attention, att), (lib.qk_packed_attention, att),
                     (lib.qk_paged_kv_read, kernels._READ_ARGS.pack(*cache, 0, 256, 256, 8, row, head))):
         assert f(args, 0) == 1 and b"overlap" in lib.qk_last_error()
+
+
+def test_recovery_resets_every_scratch(linear):
+    """Counters that a timed-out wait left mid-count: of the GEMV's and the linears' scratch, and of those that larger calls
+    replaced and a graph may still run on."""
+    k, call = linear
+    tensors = []
+    for units in (4, 8):
+        tensors.append(k.scratch(torch.device("cpu"), 64, units)[1])
+    call(4)
+    tensors.append(k._scratch[("gemm", 0)])
+    call(128)
+    tensors.append(k._scratch[("gemm", 0)])
+    k._scratch[("ragged", 0, 0)] = torch.zeros(64, dtype=torch.uint8)
+    tensors.append(k._scratch[("ragged", 0, 0)])
+    for t in tensors:
+        t.fill_(1)
+    k.reset_scratch()
+    assert not any(t.any() for t in tensors)
