@@ -100,15 +100,15 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// 8 floats (as packed pairs) of a row whose largest magnitude is amax, s = amax / 448 -> 8 e4m3 bytes: the fp32 quotients x / s,
-// rounded to nearest even (a zero row gives zeros). bf16 rows lie on ties of e4m3 often, so the quotient has to be the
-// rounded one: x * (1 / s) is off by an ulp here and there, and a correction by its remainder x - q s, which an fma
-// gives exactly, makes it right (Markstein, IBM J. Res. Dev. 34, 1990). Rows whose remainders could fall below fp32's
-// range, and those with an infinity or NaN, are divided.
+// 8 floats (as packed pairs) of a row whose largest magnitude is amax, s = amax / 448 -> 8 e4m3 bytes: the fp32 quotients
+// x / s, rounded to nearest even (a zero row gives zeros). bf16 rows lie on ties of e4m3 often, so the quotient has to be the
+// rounded one: x * (448 / amax) is off by an ulp here and there, and a correction by its remainder x - q s, which an fma
+// gives without rounding the product, makes it right (Markstein, IBM J. Res. Dev. 34, 1990), for two packed fmas a pair.
+// Rows whose remainders could fall below fp32's range, and those with an infinity or NaN, are divided.
 __device__ __forceinline__ uint2 quant8(const uint64_t (&x)[4], float amax, float s) {
   uint32_t h[4];
   const bool plain = amax >= 1e-20f && amax < INFINITY;
-  const float r = plain ? __frcp_rn(s) : 0.f;
+  const float r = plain ? __fdiv_rn(448.f, amax) : 0.f;   // 1 / s to an ulp or two, beside s and not behind it
   const uint64_t inv = f32x2(r, r), neg = f32x2(-s, -s);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
