@@ -325,7 +325,9 @@ int qk_argmax_rows(const void* logits, int rows, int V, unsigned long long* best
  *   and v_out (bf16, row_stride between rows, head_stride between heads), dequantised.
  * qk_paged_attention: out[t][h] = sum over positions j <= pos(t) of softmax_j(scale * q[t][h] . K[g][j]) V[g][j],
  *   g = h / (n_q / n_kv), 1 to 32 query heads per KV head; a row without a visible position gives zeros. max_q: at
- *   least the most token rows of a sequence (a longer one sets the bad-state bit and keeps its old output).
+ *   least the most token rows of a sequence. It chooses the kernels: where max_q * n_q / n_kv is at most 16, the kernel that
+ *   is launched takes that many query rows (8 or 16) of a sequence, and one with more sets the bad-state bit and keeps its
+ *   old output; otherwise sequences of any number of rows are computed.
  * qk_packed_attention: the same over whole prompts packed without padding: row t of prompt b sees rows
  *   cu_rows[b] .. t of k and v (kv_row between rows, kv_head between heads).
  * workspace: qk_ragged_attention_workspace_bytes() bytes, 256-byte aligned, zeroed once; every call leaves it ready

@@ -29,7 +29,7 @@
 namespace qk {
 
 constexpr int FEW_RING = 131072;      // bytes of K and V in the ring
-constexpr int FEW_MIN_TILES = 1;      // a CTA's least share (one sequence of 13 tiles and 8 heads: 8.4 us; 10.6 with 2, 11.6 with 4)
+constexpr int FEW_MIN_TILES = 1;      // a CTA's least share (one sequence of 13 tiles and 8 heads: 9.0 us in a graph; 10.7 with 2, 11.7 with 4)
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct RaggedParams {
@@ -44,7 +44,7 @@ struct RaggedParams {
 };
 
 struct FewParams {
-  CUtensorMap tm_k, tm_v;   // the pools as [n_pages * n_kv * page_size] rows: box {128 bytes, min(page_size, 64) rows}
+  CUtensorMap tm_k, tm_v;   // the pools as [n_pages * n_kv * page_size] rows: box {128 bytes, min(page_size, keys of a tile) rows}
   RaggedParams r;
   float* part;              // [grid][2][rows][128]
   float* ml;                // [grid][2][rows][2]

@@ -22,18 +22,19 @@
 //    gives registers to the softmax): Q0 K0, Q1 K0, then per key tile P0 V, Q0 K', P1 V, Q1 K', with P in two parts, the
 //    first multiplied while the second is computed. While one tile's softmax runs, the matrix unit has the other's two
 //    products to do.
-//  * Measured (one prompt of 8,192 tokens, 32 heads on 8): 432 us in a burst, 1,270 TFLOP/s; some 510 us under the 1,000 W
-//    cap. A period of a pair of tiles is 3,150 cycles, the matrix unit's share 2,130: the chain of one tile's softmax
-//    (2,060), its last P V and next S (800) is longer than half of it. Slower were: exponentials partly on the FMA pipe,
-//    halves of S loaded apart, an issuing warp per tile, P in halves (443 us), 128-byte transposed output stores.
+//  * Measured (one prompt of 8,192 tokens, 32 heads on 8): 444 us in a burst of four calls, 1,239 TFLOP/s; some
+//    505 us under the 1,000 W cap. A period of a pair of tiles is 3,150 cycles, the matrix unit's share 2,130: the chain of
+//    one tile's softmax (2,060), its last P V and next S (800) is longer than half of it. Slower were: exponentials partly on
+//    the FMA pipe, halves of S loaded apart, an issuing warp per tile, P in halves (452 us), 128-byte transposed output
+//    stores.
 //  * Work: (sequence, KV head, tile pair, key tile) in that order, dealt in equal contiguous ranges to the CTAs: causal
 //    rows and ragged lengths balance by themselves, and a few rows over a long context spread over every SM. A boundary
 //    nearer than TCA_MIN_PIECE tiles to the end of a unit moves there. Units cut by one leave fp32 partials (O, m, l) per
 //    piece; the CTA that completes the unit's count adds them in order.
 //  * An e4m3 cache: the loads bring raw tiles, and six more warps write them as bf16 tiles in the image the MMAs read: the
 //    e4m3 values, exactly. The softmax multiplies each score by its key's K scale and each P by its V scale (packed
-//    multiplications and broadcast loads); P times the V scale is what is rounded to bf16. Folding the scales into the tiles, rounded to bf16, was a fifth faster and
-//    twice as far off (3.4e-3 against 1.7e-3 for fp32 sums rounded once).
+//    multiplications and broadcast loads); P times the V scale is what is rounded to bf16. Folding the scales into the tiles,
+//    rounded to bf16, was a fifth faster and half as far off again (3.4e-3 against 2.3e-3; fp32 sums rounded once: 1.7e-3).
 #pragma once
 #include "attention_few.cuh"
 
@@ -43,7 +44,7 @@ constexpr int TCA_KEYS = 128;             // keys of a tile
 constexpr int TCA_TILE = TCA_KEYS * HEAD_DIM * 2;   // 32 KB: two 64-dim halves of 128 rows x 128 B
 constexpr int TCA_MIN_PIECE = 4;          // tiles
 constexpr int TCA_UNIT_COST = 2;          // what a unit costs beside its key tiles (Q load, first scores, output), in tiles
-constexpr int TCA_FIRST = 6;              // 16-key steps of P handed over first, of 8 (one prompt of 8,192 tokens: 432 us; 443 with 4, 450 with 2)
+constexpr int TCA_FIRST = 6;              // 16-key steps of P handed over first, of 8 (one prompt of 8,192 tokens, in a burst: 444 us; 452 with 4, 464 with 2)
 constexpr float TCA_LAZY = 8.f;           // log2 of the growth that a stale maximum may hide
 
 enum { SRC_PACKED = 0, SRC_PAGED = 1, SRC_PAGED_FP8 = 2 };

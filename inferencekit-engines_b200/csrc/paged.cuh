@@ -143,7 +143,7 @@ struct PagedQkvParams {
 // partner, A_j = w_j c and B_j = +-w_j' s, both computed once per warp: two products and a multiplication per value.
 // Pairs of heads: ceil(n_q / 2) of queries, then ceil(n_kv / 2) of keys and as many of values; a pair has one kind.
 // Bound by issue slots, not bytes, when written head by head with its own angles (160 us for 16,384 rows of 32 + 16
-// heads into e4m3 pages, 2.4 TB/s); 84 us, 4.5 TB/s so.
+// heads into e4m3 pages, 2.4 TB/s); 80 us in a graph, 4.7 TB/s so.
 enum { ROW_Q, ROW_K, ROW_V };
 template <bool FP8, bool INTER>
 __global__ void __launch_bounds__(256, 4) paged_qkv_kernel(const __grid_constant__ PagedQkvParams p) {
@@ -307,8 +307,9 @@ struct PagedReadParams {
 
 // Rows back out of the pages: output row cu[b] + i is position starts[b] + i of sequence b, dequantised in fp32 and
 // rounded to bf16 once. A warp takes all 2 n_kv rows (K, then V) of one position, 16 bytes a lane: two bf16 rows or four
-// e4m3 rows at a time, two such loads in flight, 48 warps an SM: 139 us for 131,000 positions of 8 heads out of e4m3 pages
-// (5.9 TB/s). Four loads cost occupancy (166 us), one leaves too little in flight (154), 64 warps too few registers (160).
+// e4m3 rows at a time, two such loads in flight, 48 warps an SM: 134 us in a graph for 131,000 positions of 8 heads out of
+// e4m3 pages (6.1 TB/s). Four loads a lane take 160 us (registers), one 144 (too little in flight), 64 warps 154 (too few
+// registers), 40 warps 137.
 template <bool FP8>
 __global__ void __launch_bounds__(256, 6) paged_kv_read_kernel(const __grid_constant__ PagedReadParams p) {
   constexpr int LANES = FP8 ? 8 : 16, ROWS = 32 / LANES, AHEAD = 2;

@@ -1,4 +1,4 @@
-// C entry points of the paged-serving operators (paged.cuh, attention_ragged.cuh). Included by qwen3_b200.cu, whose
+// C entry points of the paged-serving operators (paged.cuh, attention_few.cuh, attention_tc.cuh). Included by qwen3_b200.cu, whose
 // argument-check and launch helpers it uses.
 #pragma once
 #include <mutex>
@@ -189,8 +189,8 @@ int warp_grid(long long warps, dim3* grid) {   // 8 warps a CTA
   return QK_OK;
 }
 
-// paged_qkv's warps an SM before a warp takes more than one pair of heads: 1,655 rows of 24 heads take 14.4 us with 16 and
-// 16.4 with 8 or 32; 16 rows of 48 heads have a pair each either way.
+// paged_qkv's warps an SM before a warp takes more than one pair of heads: 1,655 rows of 24 heads take 6.4 us in a graph with
+// 16, 8.5 with 8 and 9.1 with 32; 16 rows of 48 heads have a pair each either way.
 constexpr int QKV_WARPS = 16;
 }  // namespace
 
@@ -279,8 +279,9 @@ int qk_paged_attention(const qk_ragged_attention_t* args, qk_stream_t stream) {
   if (rows <= 16) return fp8 ? launch_few<true, 2>(p, 1, args->workspace, st) : launch_few<false, 2>(p, 1, args->workspace, st);
   // More: the sequences with up to 8 query rows per KV head (those that decode beside a chunk), and the others behind them on
   // the tensor cores, which take a few rows too at the matrix unit's time for 128. 17 to 32 rows in the few-row kernel
-  // took longer (16 sequences of up to 8 tokens at up to 16k: 183 us against 117; 8 at up to 400: 22 against 14), 9 to 16
-  // take less (102 against 115, 20 against 34 for 4 sequences at up to 4k).
+  // took longer (16 sequences of up to 8 tokens at up to 16k: 183 us against 118; 8 at up to 400: 22 against 15), 9 to 16
+  // take less (103 against 115 for 16 sequences of up to 4 tokens at up to 16k, 82 against 126 over e4m3 pages; 21 against 34
+  // for 4 at up to 4k; 15 against 14 for 8 at up to 400).
   // From 9 query heads per KV head on no sequence has that few.
   const bool few = p.group <= 8;
   if (few)

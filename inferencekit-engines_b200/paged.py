@@ -25,8 +25,11 @@ GEMM_ROWS = 128   # rows of one batched-linear call
 class PagedEngine:
     """pages: pages of the pool (each page_size positions of every layer); max_rows: token rows of one pass; max_seqs:
     sequences of one pass; max_len: the longest sequence (the rotary tables' length); kv_dtype: "bf16" or "fp8";
-    rope_scaling: see `model.rope_angles` (contexts past the trained length). The model's own contiguous cache is not
-    used."""
+    rope_scaling: see `model.rope_angles` (contexts past the trained length; "ramp": "dims" for what Qwen3's configurations
+    mean). The model's own contiguous cache is not used.
+
+    A pass in which every sequence begins attends over the projection's own rows, any other over the cache: with an fp8
+    cache a prompt's logits depend on whether it entered whole (unquantised keys and values) or in chunks."""
 
     def __init__(self, model: Qwen3FP8Decode, pages: int, page_size: int = 64, max_rows: int = 512, max_seqs: int = 64,
                  max_len: int | None = None, kv_dtype: str = "bf16", rope_scaling: dict | None = None, pdl: bool = True):
