@@ -9,21 +9,23 @@
 //    whose softmax warps take turns with the matrix unit.
 //  * One pass over the keys in tiles of 128. S = Q K^T (operands in shared memory, accumulator in TMEM); a softmax
 //    thread owns one row: it reads its 128 scores with tcgen05.ld, keeps the running maximum m and sum l, writes
-//    P = exp2(S - m) as bf16 over S in TMEM; O += P V reads P from TMEM and V from shared memory (dims contiguous:
-//    the MN-major operand). P is rounded to bf16, the type of V's tile, which costs an output about as much as its own
-//    rounding (2.2e-3 together, of its norm, against 1.5e-3); P in two parts would be half as many products again, of what
-//    bounds this. l sums the fp32 values.
-//  * O stays in TMEM. Its rows are multiplied by exp2(m_old - m_new) only when a maximum grew by more than 2^8 in
-//    weight: until then the old m serves. P, l and O have fp32's exponents, so a P of up to 2^8 is as exact as one of 1;
-//    the rescale becomes rare, and a tile's exponentials need not wait for its maximum. Sums before the division by l
-//    can pass fp32's largest value where V's values times the keys that count are above 2^120.
+//    P = exp2(S - m), but for a constant, as bf16 over S in TMEM; O += P V reads P from TMEM and V from shared memory
+//    (dims contiguous: the MN-major operand). P is rounded to bf16, the type of V's tile, which costs an output about as
+//    much as its own rounding (2.2e-3 together, of its norm, against 1.5e-3); P in two parts would be half as many products
+//    again, of what bounds this. l sums the fp32 values.
+//  * O stays in TMEM. Its rows are multiplied by exp2(m_old - m_new) only when a maximum grew by more than 2^32 in
+//    weight: until then the old m serves. P, l and O have fp32's exponents, so a P of 2^16 is as exact as one of 1; the
+//    rescale becomes rare, and a tile's exponentials need not wait for its maximum. (A limit of 2^8 costs nothing where scores
+//    deviate by 1 or 2, but 40 % where they deviate by 4: 630 us for one prompt of 8,192 tokens.) P is exp2(S - m - 16), so
+//    that it stays below 2^16 under a stale maximum; the sums pass fp32's range where V's values times the keys that count
+//    are above 2^112, and lose bits where V's values are below 2^-110.
 //  * Warps: 0-3 and 4-7 the softmax of the two tiles, 8 the loads (TMA, 128-byte swizzle, a ring of five 32 KB K and V
 //    tiles), 9 issues the MMAs from one thread (10 clears V rows past a sequence's end, 11 fills the warpgroup, which
 //    gives registers to the softmax): Q0 K0, Q1 K0, then per key tile P0 V, Q0 K', P1 V, Q1 K', with P in two parts, the
 //    first multiplied while the second is computed. While one tile's softmax runs, the matrix unit has the other's two
 //    products to do.
-//  * Measured (one prompt of 8,192 tokens, 32 heads on 8): 444 us in a burst of four calls, 1,239 TFLOP/s; some
-//    505 us under the 1,000 W cap. A period of a pair of tiles is 3,150 cycles, the matrix unit's share 2,130: the chain of
+//  * Measured (one prompt of 8,192 tokens, 32 heads on 8): 437 to 445 us in bursts of four calls, 1,235 to
+//    1,258 TFLOP/s; some 505 us under the 1,000 W cap. A period of a pair of tiles is 3,150 cycles, the matrix unit's share 2,130: the chain of
 //    one tile's softmax (2,060), its last P V and next S (800) is longer than half of it. Slower were: exponentials partly on
 //    the FMA pipe, halves of S loaded apart, an issuing warp per tile, P in halves (452 us), 128-byte transposed output
 //    stores.
@@ -45,7 +47,8 @@ constexpr int TCA_TILE = TCA_KEYS * HEAD_DIM * 2;   // 32 KB: two 64-dim halves 
 constexpr int TCA_MIN_PIECE = 4;          // tiles
 constexpr int TCA_UNIT_COST = 2;          // what a unit costs beside its key tiles (Q load, first scores, output), in tiles
 constexpr int TCA_FIRST = 6;              // 16-key steps of P handed over first, of 8 (one prompt of 8,192 tokens, in a burst: 444 us; 452 with 4, 464 with 2)
-constexpr float TCA_LAZY = 8.f;           // log2 of the growth that a stale maximum may hide
+constexpr float TCA_LAZY = 32.f;          // log2 of the growth that a stale maximum may hide
+constexpr float TCA_SHIFT = 16.f;         // P's largest value under a fresh maximum is 2^-16, under a stale one 2^16
 
 enum { SRC_PACKED = 0, SRC_PAGED = 1, SRC_PAGED_FP8 = 2 };
 
@@ -671,7 +674,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         const int e = w.end(x), tok = w.tok0(x) + row / r.group, pos = w.s.len - w.s.n + tok;
         const bool valid = row < (step / 2) * r.group && tok < w.s.n;
         const int first = w.s.len - w.s.n + w.tok0(x);   // the last key that the tile's first row sees
-        float m = -INFINITY, l = 0.f, base = 0.f;   // base = -m * sl2
+        float m = -INFINITY, l = 0.f, base = 0.f;   // base = -m * sl2 - TCA_SHIFT
         for (int t = w.t0; t < e; ++t) {
           ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.s_full[x], (uint32_t)(ns++ & 1)));
           tc_fence_after();
@@ -719,7 +722,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
               m = mn;
               l *= f;
               // an infinite maximum makes the row NaN, as inf - inf does
-              base = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7fffffff) : -m * sl2;
+              base = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7fffffff) : -m * sl2 - TCA_SHIFT;
             }
             if (early) {                      // the products before this tile's scores are done: O is whole
 #pragma unroll 1
