@@ -183,6 +183,7 @@ class PagedEngine:
         tokens (default: what a pass takes) beside the sequences that already decode, in their order and as soon as the pool
         has pages for a prompt and its gen_len tokens; a finished sequence's pages go to those that wait. Returns the lists
         of ids."""
+        prompts = [list(p) for p in prompts]
         chunk = min(chunk or self.max_rows, self.max_rows)
         if chunk < 1 or not all(len(p) for p in prompts):
             raise ValueError(f"chunks of {chunk} tokens, {sum(not len(p) for p in prompts)} empty prompts")
@@ -210,7 +211,7 @@ class PagedEngine:
             while waiting and need[waiting[0]] <= len(self.free):
                 i, s = waiting.pop(0), self.new()
                 running.append(s)
-                todo[s], of[s] = list(prompts[i]), i
+                todo[s], of[s] = prompts[i], i
                 self.reserve(s, len(prompts[i]) + gen_len - 1)   # to its end: it cannot run out on the way
             batch, room = [], self.max_rows
             for s in running:                    # those that decode, then prompts

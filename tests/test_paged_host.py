@@ -283,3 +283,12 @@ def test_export_refuses_a_cache_that_cannot_hold_the_sequence(make):
         for k, v in ((bad, cache), (cache, bad)):
             with pytest.raises(ValueError, match="export"):
                 eng.export(s, k, v)
+
+
+def test_generate_takes_prompts_of_any_kind_once(make):
+    eng = make(8)
+    prompts = [range(5), (7, 8), iter([20, 30])]
+    assert eng.generate(prompts, 2) == [[5, 6], [9, 10], [31, 32]]
+    kept = [[1, 2], [3]]
+    eng.generate(kept, 2)
+    assert kept == [[1, 2], [3]]
