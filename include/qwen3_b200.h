@@ -324,7 +324,9 @@ int qk_argmax_rows(const void* logits, int rows, int V, unsigned long long* best
  * qk_paged_kv_read: positions starts[b] + i (0 + i for starts NULL) of every sequence into row cu_rows[b] + i of k_out
  *   and v_out (bf16, row_stride between rows, head_stride between heads), dequantised.
  * qk_paged_attention: out[t][h] = sum over positions j <= pos(t) of softmax_j(scale * q[t][h] . K[g][j]) V[g][j],
- *   g = h / (n_q / n_kv), 1 to 32 query heads per KV head; a row without a visible position gives zeros. max_q: at
+ *   g = h / (n_q / n_kv), 1 to 32 query heads per KV head; a row without a visible position gives zeros. What lies in
+ *   the pages past a sequence's end, and in other sequences, has no influence; a NaN or an infinity in a V row of the
+ *   sequence itself also reaches the rows before it that share its 128-key tile. max_q: at
  *   least the most token rows of a sequence. It chooses the kernels: where max_q * n_q / n_kv is at most 16, the kernel that
  *   is launched takes that many query rows (8 or 16) of a sequence, and one with more sets the bad-state bit and keeps its
  *   old output; otherwise sequences of any number of rows are computed.

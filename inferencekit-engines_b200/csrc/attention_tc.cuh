@@ -25,10 +25,10 @@
 //    first multiplied while the second is computed. While one tile's softmax runs, the matrix unit has the other's two
 //    products to do.
 //  * Measured (one prompt of 8,192 tokens, 32 heads on 8): 437 to 445 us in bursts of four calls, 1,235 to
-//    1,258 TFLOP/s; some 505 us under the 1,000 W cap. A period of a pair of tiles is 3,150 cycles, the matrix unit's share 2,130: the chain of
-//    one tile's softmax (2,060), its last P V and next S (800) is longer than half of it. Slower were: exponentials partly on
-//    the FMA pipe, halves of S loaded apart, an issuing warp per tile, P in halves (452 us), 128-byte transposed output
-//    stores.
+//    1,258 TFLOP/s; some 505 us under the 1,000 W cap. A period of a pair of tiles is 3,150 cycles, the matrix unit's share
+//    2,130: the chain of one tile's softmax (2,060), its last P V and next S (800) is longer than half of it. Slower were:
+//    exponentials partly on the FMA pipe, halves of S loaded apart, an issuing warp per tile, P in halves (452 us),
+//    128-byte transposed output stores.
 //  * Work: (sequence, KV head, tile pair, key tile) in that order, dealt in equal contiguous ranges to the CTAs: causal
 //    rows and ragged lengths balance by themselves, and a few rows over a long context spread over every SM. A boundary
 //    nearer than TCA_MIN_PIECE tiles to the end of a unit moves there. Units cut by one leave fp32 partials (O, m, l) per
