@@ -369,6 +369,70 @@ long long qk_ragged_attention_workspace_bytes(void);
 int qk_paged_attention(const qk_ragged_attention_t* args, qk_stream_t stream);
 int qk_packed_attention(const qk_ragged_attention_t* args, qk_stream_t stream);
 
+/* Sequences that share pages: beams, samples of one prompt, requests behind one system prompt. The page pool's state is
+ * refs (int32 [n_pages]: the sequences that hold a page, 0 for a free one) beside the block tables; a sequence of length n holds the
+ * first ceil(n / page_size) entries of its row, and what lies behind them means nothing. Everything is device data, and what the
+ * calls leave depends on their inputs alone: free pages are taken lowest first, in the order of the sequences.
+ *
+ * qk_paged_plan: the pass in which fresh[b] >= 0 tokens enter sequence b, which has lens[b] positions in the cache: cu_rows
+ *   [batch + 1] (prefix sums of fresh), seq_lens = lens + fresh, free pages into the new entries of the tables, their refs 1.
+ *   slots and positions [rows] (each may be NULL): of token row t, page * page_size + position % page_size, and the position; rows
+ *   past cu_rows[batch] are left alone. groups [n_groups + 1] and shared [n_groups] (both or neither): group g is the sequences
+ *   groups[g] .. groups[g+1]-1; shared[g] = the leading positions that its tables have in the same pages, at most its smallest lens.
+ *   All or nothing: with too few free pages (error word 8), or more rows than `rows` (error word 2; rows -1: any number), nothing is taken,
+ *   cu_rows is 0 and seq_lens is lens. info (NULL, or [2]): pages missing (0: done), free pages left. A sequence with a negative length or
+ *   one past its table sits the pass out (error word 2). table_out and refs_out may be the inputs (then only what changes is
+ *   written) or memory apart from them (copied). At most 16,384 sequences.
+ * qk_paged_fork: the sequences in a new order: row i (of `rows`) continues row parents[i] of the old ones (-1: it is empty). table_out and
+ *   lens_out (apart from the inputs) are the new rows, -1 behind their pages; refs counts the new rows in place of the old ones. A
+ *   partly filled last page stays with its row's first child, unless a sequence outside the call holds it too; the
+ *   other children get a free page and a copy of the filled rows, in every layer: pools [layers][n_pages][n_kv][page_size][128].
+ *   With one old row and many new ones it spreads a prompt, with parents -1 it ends sequences. All or nothing: with too few free pages
+ *   (error word 8) the refs are as they were and the new rows are empty. At most 16,384 rows on either side.
+ * qk_beam_select: request b's beams are the rows cu_rows[b] .. cu_rows[b+1]-1 (at most 128) of logits [rows][vocab] (bf16, or fp32 = 1;
+ *   row_stride elements apart, vocab at most 1,048,576) with their scores so far. Out of all (beam r, token v) the k <= 64 largest
+ *   scores[r] + logits[r][v] - logsumexp(logits[r]), in order, equal ones by r, then v: out_scores, out_parents (r) and out_tokens
+ *   [batch][k]; -inf, -1, -1 where fewer have a score above -inf. A logit of -inf excludes a token, a score of -inf a beam (its logits
+ *   are not read). A row with a NaN or +inf in logits or score sets error word 2 and gives no candidates. Sums of exponentials in fp32,
+ *   scores and their order in 64 bits. workspace: qk_beam_workspace_bytes(rows, vocab, k), 256-byte aligned, zeroed once; calls that may overlap
+ *   need one each.
+ * qk_shared_attention: qk_paged_attention over sequences of which group g (as above, device data) has its first shared[g] positions in
+ *   common: in the same pages, or in pages of equal contents. They are read through the group's first row, once for all its
+ *   query rows. Every new token of a group comes after them (lens >= shared: else error word 2, and the group's rows are unspecified).
+ *   Sequences in no group are on their own. workspace: qk_shared_attention_workspace_bytes(rows, n_q). */
+typedef struct {
+  const int *refs, *lens, *fresh, *block_table, *groups;
+  int *refs_out, *table_out, *cu_rows, *seq_lens, *slots, *positions, *shared, *info;
+  long long batch, table_width, table_stride, out_stride, n_pages, page_size, rows, n_groups;
+} qk_paged_plan_t;
+typedef struct {
+  const int *refs, *lens, *parents, *block_table;
+  int *refs_out, *table_out, *lens_out, *info;
+  void *k_pages, *v_pages;
+  float *k_scale, *v_scale;                /* NULL for bf16 pages */
+  long long batch, rows, table_width, table_stride, out_stride, layers, n_pages, n_kv, page_size, kv_fp8;
+} qk_paged_fork_t;
+typedef struct {
+  const void* logits;
+  const float* scores;
+  const int* cu_rows;
+  float* out_scores;
+  int *out_parents, *out_tokens;
+  void* workspace;
+  long long rows, batch, vocab, k, row_stride, fp32, workspace_bytes;
+} qk_beam_select_t;
+typedef struct {
+  qk_ragged_attention_t att;               /* as for qk_paged_attention */
+  const int *groups, *shared;
+  long long n_groups;
+} qk_shared_attention_t;
+int qk_paged_plan(const qk_paged_plan_t* args, qk_stream_t stream);
+int qk_paged_fork(const qk_paged_fork_t* args, qk_stream_t stream);
+long long qk_beam_workspace_bytes(long long rows, long long vocab, long long k);
+int qk_beam_select(const qk_beam_select_t* args, qk_stream_t stream);
+long long qk_shared_attention_workspace_bytes(long long rows, long long n_q);
+int qk_shared_attention(const qk_shared_attention_t* args, qk_stream_t stream);
+
 /* Tensor-parallel helpers (no counterpart in the single-GPU reference; the TP plan of its decode step):
  * resid[i] = bf16(resid[i] + bf16(sum[i])) for the fp32 all-reduced partial of a row-parallel GEMV (the
  * rounding of the reference's residual epilogue, decode.cu:320-323); and the top-bit flip of packed argmax

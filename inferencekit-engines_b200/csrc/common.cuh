@@ -16,7 +16,7 @@ constexpr int QB = 128;         // quantization block (weights and activations)
 
 // Device-side error word: bounded waits that give up set a bit here instead of hanging; the host reads
 // and clears it with qk_get_device_error().
-enum : int { DEVERR_MBAR_TIMEOUT = 1, DEVERR_BAD_STATE = 2, DEVERR_GRID_TIMEOUT = 4 };
+enum : int { DEVERR_MBAR_TIMEOUT = 1, DEVERR_BAD_STATE = 2, DEVERR_GRID_TIMEOUT = 4, DEVERR_NO_PAGES = 8 };
 // Once a wait has timed out anywhere, every later wait gives up at once instead of waiting its own limit,
 // so a failure ends the launch quickly (the host reads and clears the word with qk_get_device_error).
 constexpr int DEVERR_WAIT_FAILED = DEVERR_MBAR_TIMEOUT | DEVERR_GRID_TIMEOUT;

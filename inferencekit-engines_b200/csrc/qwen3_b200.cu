@@ -13,10 +13,12 @@
 #include "attention_fp8kv.cuh"
 #include "attention_few.cuh"
 #include "attention_tc.cuh"
+#include "beam.cuh"
 #include "common.cuh"
 #include "gemm_tc.cuh"
 #include "gemv.cuh"
 #include "paged.cuh"
+#include "paged_plan.cuh"
 #include "prefill.cuh"
 #include "step.cuh"
 
@@ -924,3 +926,4 @@ extern "C" int qk_attention_fp8kv(const void* qkv, const void* q_norm_w, const v
 
 // ---- serving from a paged KV cache ----------------------------------------------------------------------------
 #include "paged_api.cuh"
+#include "sharing_api.cuh"

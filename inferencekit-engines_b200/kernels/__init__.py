@@ -81,6 +81,12 @@ _SIGS = {
     "qk_ragged_attention_workspace_bytes": ([], _L),
     "qk_paged_attention": ([_VP, _VP], _I),
     "qk_packed_attention": ([_VP, _VP], _I),
+    "qk_paged_plan": ([_VP, _VP], _I),
+    "qk_paged_fork": ([_VP, _VP], _I),
+    "qk_beam_workspace_bytes": ([_L, _L, _L], _L),
+    "qk_beam_select": ([_VP, _VP], _I),
+    "qk_shared_attention_workspace_bytes": ([_L, _L], _L),
+    "qk_shared_attention": ([_VP, _VP], _I),
 }
 
 
@@ -146,6 +152,8 @@ _E4M3 = (torch.float8_e4m3fn, torch.uint8)
 _BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 # qk_paged_qkv_t, qk_paged_kv_read_t and qk_ragged_attention_t (the first 14 fields of each: qk_paged_cache_t)
 _QKV_ARGS, _READ_ARGS, _ATTENTION_ARGS = (struct.Struct(f) for f in ("7Q7q7Q8qd", "7Q7q3Q3q", "7Q7q5Q10qd"))
+# qk_paged_plan_t, qk_paged_fork_t, qk_beam_select_t and qk_shared_attention_t
+_PLAN_ARGS, _FORK_ARGS, _BEAM_ARGS, _SHARED_ARGS = (struct.Struct(f) for f in ("13Q8q", "12Q10q", "7Q7q", "7Q7q5Q10qd2Qq"))
 
 
 class DecodeOps:
@@ -491,15 +499,19 @@ class DecodeOps:
         ready for the next). Calls that may run at the same time, on two streams, need one each."""
         return torch.zeros(self.lib.qk_ragged_attention_workspace_bytes(), dtype=torch.uint8, device=device)
 
-    def _workspace(self, what, ws, dev, stream):
+    def _workspace(self, what, ws, dev, stream, maker="attention_workspace", nbytes=0):
         if ws is None:   # one per device and stream, kept; never a graph's, whose replays may run beside the stream's calls
             if stream and torch._C._cuda_isCurrentStreamCapturing():   # (stream 0 cannot be captured)
-                raise RuntimeError(f"{what}: pass workspace=attention_workspace(device), made before the capture")
-            ws = self._scratch.get(("ragged", dev, stream))
-            if ws is None:
-                ws = self._scratch[("ragged", dev, stream)] = self.attention_workspace(torch.device("cuda", dev))
+                raise RuntimeError(f"{what}: pass workspace={maker}(device), made before the capture")
+            key = ("ragged" if maker == "attention_workspace" else maker, dev, stream)
+            ws = self._scratch.get(key)
+            if ws is None or ws.numel() < nbytes:
+                if ws is not None:
+                    self._outgrown.append(ws)
+                dest = torch.device("cuda", dev)
+                ws = self._scratch[key] = torch.zeros(nbytes, dtype=torch.uint8, device=dest) if nbytes else self.attention_workspace(dest)
         elif ws.dtype is not torch.uint8 or ws.get_device() != dev or not ws.is_contiguous():
-            raise RuntimeError(f"{what}: workspace must come from attention_workspace() on the call's device")
+            raise RuntimeError(f"{what}: workspace must come from {maker}() on the call's device")
         return ws
 
     def paged_qkv(self, qkv, cu, seq_lens, block_table, k_pages, v_pages, q_out, cos, sin, q_norm=None, k_norm=None,
@@ -604,6 +616,176 @@ class DecodeOps:
                                  o_head, ws.numel(), scale), stream)
         if st:
             self._check(st, "packed_attention")
+
+    # ---- sequences that share pages ------------------------------------------------------------------------
+    # refs (int32 [pages]) counts the sequences that hold a page, 0 for a free one; a sequence of length n holds the first
+    # ceil(n / page_size) entries of its block-table row. Free pages are taken lowest first, in the order of the sequences.
+    # With too few of them a call takes nothing and sets the device error word (8).
+    @staticmethod
+    def _ints(what, name, t, shape, dev):
+        """The address of a contiguous int32 tensor of `shape` (None: any one-dimensional) on GPU dev; 0 for None."""
+        if t is None:
+            return 0
+        if t.dtype is not _I32 or t.get_device() != dev or not t.is_contiguous() or (t.dim() != 1 if shape is None else tuple(t.shape) != shape):
+            raise RuntimeError(f"{what}: {name} must be contiguous int32 {list(shape) if shape else '[n]'} on the call's CUDA device")
+        return t.data_ptr()
+
+    @staticmethod
+    def _table(what, name, t, rows, width, dev):
+        """(address, row stride) of an int32 [rows, width] block table on GPU dev (width None: any)."""
+        if t.dtype is not _I32 or t.dim() != 2 or t.shape[0] != rows or t.get_device() != dev or (width is not None and t.shape[1] != width) \
+                or (t.stride(1) != 1 and t.shape[1] > 1):
+            raise RuntimeError(f"{what}: {name} must be int32 [{rows}, {'width' if width is None else width}] on the call's CUDA device, "
+                               "rows contiguous")
+        return t.data_ptr(), t.stride(0)
+
+    def paged_plan(self, refs, lens, new, block_table, cu, seq_lens, page_size, refs_out=None, table_out=None, slots=None,
+                   positions=None, groups=None, shared=None, info=None):
+        """The pass in which new[b] tokens enter sequence b, which has lens[b] positions in the cache (int32 [B]): writes cu [B+1]
+        and seq_lens [B] (what the paged calls take), free pages into the new entries of block_table, their refs 1. slots and
+        positions (int32 [T]): of every token row, page * page_size + slot in the page, and the position. groups (int32
+        [G+1], group g is the sequences groups[g] .. groups[g+1]-1) and shared (int32 [G]): how many leading positions a group's
+        sequences have in the same pages (for `shared_attention`). info (int32 [2]): pages missing (0: done), free pages left.
+        All or nothing: where pages are missing, or slots are too few for the rows, cu is 0 and seq_lens is lens.
+        refs_out and table_out: where the new state goes (default: in place)."""
+        what, dev = "paged_plan", refs.get_device()
+        if dev < 0:
+            raise RuntimeError("paged_plan: every tensor must be on the same CUDA device")
+        refs_ptr, lens_ptr = self._ints(what, "refs", refs, None, dev), self._ints(what, "lens", lens, None, dev)
+        B = lens.shape[0]
+        table_ptr, stride = self._table(what, "block_table", block_table, B, None, dev)
+        width = block_table.shape[1]
+        out_ptr, out_stride = (table_ptr, stride) if table_out is None else self._table(what, "table_out", table_out, B, width, dev)
+        if (groups is None) != (shared is None):
+            raise RuntimeError("paged_plan: groups and shared go together")
+        G = 0 if groups is None else len(groups) - 1
+        if G < 0:
+            raise RuntimeError("paged_plan: groups must have at least one entry")
+        T = -1 if slots is None and positions is None else len(positions if slots is None else slots)
+        st = self.lib.qk_paged_plan(
+            _PLAN_ARGS.pack(refs_ptr, lens_ptr, self._ints(what, "new", new, (B,), dev), table_ptr,
+                            self._ints(what, "groups", groups, None, dev),
+                            refs_ptr if refs_out is None else self._ints(what, "refs_out", refs_out, tuple(refs.shape), dev), out_ptr,
+                            self._ints(what, "cu", cu, (B + 1,), dev), self._ints(what, "seq_lens", seq_lens, (B,), dev),
+                            self._ints(what, "slots", slots, (T,), dev), self._ints(what, "positions", positions, (T,), dev),
+                            self._ints(what, "shared", shared, (G,), dev), self._ints(what, "info", info, (2,), dev),
+                            B, width, stride, out_stride, refs.shape[0], page_size, T, G), _launch_stream(what, dev))
+        if st:
+            self._check(st, what)
+
+    def paged_fork(self, refs, lens, parents, block_table, table_out, lens_out, k_pages, v_pages, k_scale=None, v_scale=None,
+                   refs_out=None, info=None):
+        """The sequences in a new order: row i of table_out [N, width] and lens_out [N] (not the inputs) continues row parents[i]
+        (int32 [N]; -1: an empty row) of block_table [B, width] and lens [B]. Whole pages are shared by count; a partly filled last
+        page stays with its row's first child, the others get a free page and a copy of the filled rows. Pools: [pages, n_kv,
+        page_size, 128] or [layers, pages, n_kv, page_size, 128] (bf16, or e4m3 with scales of the leading dimensions), whose
+        pages are copied in every layer. One row into many spreads a prompt over its beams, parents of -1 end sequences. refs_out:
+        where the counts go (default: in place). info (int32 [2]): pages missing (0: done; else refs is as it was and the new rows are
+        empty), free pages left."""
+        what, dev, shape, dt = "paged_fork", refs.get_device(), k_pages.shape, k_pages.dtype
+        if dev < 0 or k_pages.get_device() != dev or v_pages.get_device() != dev:
+            raise RuntimeError("paged_fork: every tensor must be on the same CUDA device")
+        if len(shape) not in (4, 5) or shape != v_pages.shape or not (k_pages.is_contiguous() and v_pages.is_contiguous()) or shape[-1] != 128 \
+                or v_pages.dtype is not dt or (dt is not _BF16 and dt not in _E4M3):
+            raise RuntimeError("paged_fork: k_pages and v_pages must be contiguous [pages, n_kv, page_size, 128] or [layers, ...] pools, bf16 "
+                               "or e4m3 bytes")
+        ks = vs = fp8 = 0
+        if dt is not _BF16:
+            for s in (k_scale, v_scale):
+                if s is None or s.dtype is not _F32 or s.shape != shape[:-1] or not s.is_contiguous() or s.get_device() != dev:
+                    raise RuntimeError("paged_fork: an e4m3 cache needs contiguous fp32 k_scale and v_scale, the pools' leading dimensions")
+            ks, vs, fp8 = k_scale.data_ptr(), v_scale.data_ptr(), 1
+        elif k_scale is not None or v_scale is not None:
+            raise RuntimeError("paged_fork: a bf16 cache has no row scales")
+        pages, n_kv, page = shape[-4:-1]
+        refs_ptr, lens_ptr = self._ints(what, "refs", refs, (pages,), dev), self._ints(what, "lens", lens, None, dev)
+        parents_ptr = self._ints(what, "parents", parents, None, dev)
+        B, N = lens.shape[0], parents.shape[0]
+        table_ptr, stride = self._table(what, "block_table", block_table, B, None, dev)
+        width = block_table.shape[1]
+        out_ptr, out_stride = self._table(what, "table_out", table_out, N, width, dev)
+        st = self.lib.qk_paged_fork(
+            _FORK_ARGS.pack(refs_ptr, lens_ptr, parents_ptr, table_ptr,
+                            refs_ptr if refs_out is None else self._ints(what, "refs_out", refs_out, (pages,), dev), out_ptr,
+                            self._ints(what, "lens_out", lens_out, (N,), dev), self._ints(what, "info", info, (2,), dev),
+                            k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, B, N, width, stride, out_stride,
+                            shape[0] if len(shape) == 5 else 1, pages, n_kv, page, fp8), _launch_stream(what, dev))
+        if st:
+            self._check(st, what)
+
+    def beam_workspace(self, device, rows: int, vocab: int, k: int) -> torch.Tensor:
+        """A workspace for beam_select calls of up to these sizes (zeroed once). Calls that may run at the same time need one each."""
+        nbytes = self.lib.qk_beam_workspace_bytes(rows, vocab, k)
+        if nbytes < 0:
+            raise RuntimeError(f"beam_workspace: unsupported rows={rows} vocab={vocab} k={k} (vocab at most 1048576, k at most 64)")
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+
+    def beam_select(self, logits, scores, cu, out_scores, out_parents, out_tokens, workspace=None):
+        """The k best continuations of each request: its beams are rows cu[b] .. cu[b+1]-1 (int32 [B+1], at most 128 a request) of
+        logits [R, V] (bf16 or fp32, any row stride) with their scores so far (fp32 [R]). out_scores (fp32), out_parents (the
+        row) and out_tokens (int32), all [B, k] with k <= 64: the largest scores[r] + log_softmax(logits[r])[v], in order,
+        equal ones by row, then token; -inf, -1, -1 where fewer have a score above -inf. A logit of -inf excludes a token, a score of
+        -inf a beam. A NaN or +inf among a row's logits (or as its score) sets the device error word (2) and excludes the row."""
+        what, dev = "beam_select", logits.get_device()
+        if dev < 0 or logits.dim() != 2 or logits.dtype not in (_BF16, _F32) or (logits.stride(1) != 1 and logits.shape[1] > 1):
+            raise RuntimeError("beam_select: logits must be bf16 or fp32 [rows, vocab] on a CUDA device, rows contiguous")
+        R, V = logits.shape
+        if scores.dtype is not _F32 or tuple(scores.shape) != (R,) or scores.get_device() != dev or not scores.is_contiguous():
+            raise RuntimeError(f"beam_select: scores must be fp32 [{R}] on the logits' device")
+        cu_ptr = self._ints(what, "cu", cu, None, dev)
+        B = len(cu) - 1
+        if B < 0 or out_scores.dim() != 2 or out_scores.dtype is not _F32 or out_scores.shape[0] != B or out_scores.get_device() != dev \
+                or not out_scores.is_contiguous():
+            raise RuntimeError("beam_select: out_scores must be contiguous fp32 [requests, k] on the logits' device, cu [requests + 1]")
+        k = out_scores.shape[1]
+        nbytes = self.lib.qk_beam_workspace_bytes(R, V, k)
+        if nbytes < 0:
+            raise RuntimeError(f"beam_select: unsupported rows={R} vocab={V} k={k} (vocab at most 1048576, k 1 to 64)")
+        stream = _launch_stream(what, dev)
+        ws = self._workspace(what, workspace, dev, stream, "beam_workspace", nbytes)
+        st = self.lib.qk_beam_select(
+            _BEAM_ARGS.pack(logits.data_ptr(), scores.data_ptr(), cu_ptr, out_scores.data_ptr(),
+                            self._ints(what, "out_parents", out_parents, (B, k), dev), self._ints(what, "out_tokens", out_tokens, (B, k), dev),
+                            ws.data_ptr(), R, B, V, k, logits.stride(0), logits.dtype is _F32, ws.numel()), stream)
+        if st:
+            self._check(st, what)
+
+    def shared_workspace(self, device, rows: int, n_q: int) -> torch.Tensor:
+        """A workspace for shared_attention calls of up to `rows` token rows and n_q query heads (zeroed once; every call leaves it
+        ready for the next). Calls that may run at the same time need one each."""
+        nbytes = self.lib.qk_shared_attention_workspace_bytes(rows, n_q)
+        if nbytes < 0:
+            raise RuntimeError(f"shared_workspace: unsupported rows={rows} n_q={n_q}")
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+
+    def shared_attention(self, q, cu, seq_lens, block_table, groups, shared, k_pages, v_pages, out, scale, max_q, k_scale=None,
+                         v_scale=None, workspace=None):
+        """`paged_attention` over sequences that share their first positions: group g, the sequences groups[g] .. groups[g+1]-1
+        (int32 [G+1]), has its first shared[g] positions (int32 [G]; `paged_plan` finds them) in the same pages, or in pages of equal
+        contents, all of them before its new tokens. They are read once for the whole group, through its first sequence's table.
+        Sequences in no group are on their own."""
+        what = "shared_attention"
+        B, n_kv, dev, cache = self._paged(what, k_pages, v_pages, k_scale, v_scale, cu, seq_lens, block_table)
+        T, n_q, q_row, q_head = self._heads(what, "q", q, dev)
+        oT, on, o_row, o_head = self._heads(what, "out", out, dev)
+        if oT != T or on != n_q:
+            raise RuntimeError(f"shared_attention: out must have q's shape, [{T}, {n_q}, 128]")
+        groups_ptr = self._ints(what, "groups", groups, None, dev)
+        G = len(groups) - 1
+        if G < 0:
+            raise RuntimeError("shared_attention: groups must have at least one entry")
+        shared_ptr = self._ints(what, "shared", shared, (G,), dev)
+        nbytes = self.lib.qk_shared_attention_workspace_bytes(T, n_q)
+        if nbytes < 0:
+            raise RuntimeError(f"shared_attention: unsupported rows={T} n_q={n_q}")
+        if T == 0 or B == 0:
+            return
+        stream = _launch_stream(what, dev)
+        ws = self._workspace(what, workspace, dev, stream, "shared_workspace", nbytes)
+        st = self.lib.qk_shared_attention(_SHARED_ARGS.pack(*cache, q.data_ptr(), 0, 0, out.data_ptr(), ws.data_ptr(), T, n_q, max_q, q_row,
+                                                            q_head, 0, 0, o_row, o_head, ws.numel(), scale, groups_ptr, shared_ptr, G), stream)
+        if st:
+            self._check(st, what)
 
     def finalize(self, best, token, out_tokens, state):
         b = token.numel()
