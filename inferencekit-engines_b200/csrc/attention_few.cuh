@@ -185,6 +185,241 @@ __device__ __forceinline__ void few_sync(int threads) { asm volatile("bar.sync 1
 // The CTA whose range holds tile u, for ranges [c * W / G, (c + 1) * W / G).
 __device__ __forceinline__ int owner_of(long long u, long long W, int G) { return (int)(((u + 1) * G - 1) / W); }
 
+// A warp's query rows (8 or 16) and their running sums: KT tiles of 16 keys a step, keys as the MMAs' M.
+template <bool FP8, int NT, int KT>
+struct FewRows {
+  static constexpr int KW = 16 * KT;      // keys of a step
+  uint32_t qf[NT][8][2];
+  float qs[NT][2];                        // of rows 2 lt, 2 lt + 1: scale * log2 e, fp8: times the power of two that undoes q's
+  int lim[NT][2];                         // the last key each of them sees
+  float o[8][NT][4], m[NT][2], l[NT][2];
+  // fp8: the largest weight times V scale of each row so far, under the running maximum; P times the V scale is taken over
+  // the power of two above it
+  float big[NT][2];
+  static __device__ __forceinline__ int unit(float x) { return max(exponent_above(x), -100); }
+
+  // Rows from, from + 1, .. of the sequence's n * group (token-major) for KV head g; `rows` of them exist.
+  __device__ __forceinline__ void begin(const RaggedParams& r, int row0, int n, int len, int from, int rows, int g, int lane) {
+    const int lg = lane >> 2, lt = lane & 3;
+    const float sl2 = r.scale * LOG2E;
+    // the query rows as B fragments: thread (lg, lt) holds row lg of each tile; the dims of its MMA k slots are the ones
+    // its 16-byte K chunks below hold
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = nt * 8 + lg;
+      uint4 x[4] = {};
+      if (row < rows) {
+        const bf16* src = r.q + (long long)(row0 + (from + row) / r.group) * r.q_row + (long long)(g * r.group + (from + row) % r.group) * r.q_head;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)         // bf16: chunks 2 lt, 2 lt + 1 of each 64-dim half; e4m3: dims 32 lt .. + 31
+          x[i] = *reinterpret_cast<const uint4*>(src + (FP8 ? 32 * lt + 8 * i : 64 * (i >> 1) + 16 * lt + 8 * (i & 1)));
+      }
+      float own = sl2;
+      if (FP8) {
+        float f[4][8], mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          unpack_bf16x8(x[i], f[i]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(f[i][e]));
+        }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const int e2 = min(max(exponent_above(mx), -110), 110);
+        const float up = pow2(8 - e2);      // the row's largest value lands in [2^7, 2^8)
+        own = sl2 * pow2(e2 - 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[i] = make_uint4(pack_f16(f[i][0] * up, f[i][1] * up), pack_f16(f[i][2] * up, f[i][3] * up),
+                            pack_f16(f[i][4] * up, f[i][5] * up), pack_f16(f[i][6] * up, f[i][7] * up));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        qf[nt][2 * i][0] = x[i].x, qf[nt][2 * i][1] = x[i].y;
+        qf[nt][2 * i + 1][0] = x[i].z, qf[nt][2 * i + 1][1] = x[i].w;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        qs[nt][e] = __shfl_sync(0xffffffffu, own, (2 * lt + e) * 4);
+        lim[nt][e] = min(len - 1, len - n + (from + nt * 8 + 2 * lt + e) / r.group);
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+      big[nt][0] = big[nt][1] = 0.f;
+    }
+  }
+
+  // The step's keys j0 .. j0 + KW - 1 of the sequence: rows kb and vb of swizzled tiles, whose second 64 dims (bf16) lie `half`
+  // bytes on; ks, vs: their scales. first: the last key that the first row sees.
+  __device__ __forceinline__ void step(uint32_t kb, uint32_t vb, int half, const float* ks, const float* vs, int j0, int len, int first, int lane) {
+    const int lg = lane >> 2, lt = lane & 3;
+    if (j0 + KW > len) {              // the sequence ends inside: what lies behind it must not reach P.V, as 0 x NaN
+      for (int i = lane; i < (j0 + KW - len) * (FP8 ? 8 : 16); i += 32) {
+        const int row = (len - j0) + i / (FP8 ? 8 : 16), ch = i % (FP8 ? 8 : 16);
+        asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(vb + (ch >> 3) * half + row * 128 + (ch & 7) * 16), "r"(0) : "memory");
+      }
+      fence_proxy_async_smem();         // the ring's next copy into these rows comes after
+      __syncwarp();
+    }
+    // scores of KT tiles of 16 keys: thread (lg, lt) has keys lg and lg + 8 of query rows 2 lt and 2 lt + 1
+    float sc[KT][NT][4];
+#pragma unroll
+    for (int j = 0; j < KT; ++j) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) sc[j][nt][0] = sc[j][nt][1] = sc[j][nt][2] = sc[j][nt][3] = 0.f;
+      const uint32_t ra = kb + (16 * j + lg) * 128;   // row & 7 == lg, of row + 8 too
+#pragma unroll
+      for (int i = 0; i < (FP8 ? 2 : 4); ++i) {
+        const uint32_t at = ra + (FP8 ? 0 : (i >> 1) * half) + ((2 * lt + (i & 1)) ^ lg) * 16;
+        const uint4 w = lds128_at(at), z = lds128_at(at + 8 * 128);
+        if (FP8) {
+          const uint32_t ww[4] = {w.x, w.y, w.z, w.w}, zz[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t af[4] = {e4m3x2_to_f16x2(ww[e]), e4m3x2_to_f16x2(zz[e]), e4m3x2_to_f16x2(ww[e] >> 16), e4m3x2_to_f16x2(zz[e] >> 16)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) few_mma<FP8>(sc[j][nt], af, qf[nt][4 * i + e][0], qf[nt][4 * i + e][1]);
+          }
+        } else {
+          const uint32_t a0[4] = {w.x, z.x, w.y, z.y}, a1[4] = {w.z, z.z, w.w, z.w};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            few_mma<FP8>(sc[j][nt], a0, qf[nt][2 * i][0], qf[nt][2 * i][1]);
+            few_mma<FP8>(sc[j][nt], a1, qf[nt][2 * i + 1][0], qf[nt][2 * i + 1][1]);
+          }
+        }
+      }
+    }
+    float kscale[KT][2], vscale[KT][2];
+    if (FP8) {
+#pragma unroll
+      for (int j = 0; j < KT; ++j)
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const int key = 16 * j + 8 * hh + lg;
+          kscale[j][hh] = ks[key];
+          vscale[j][hh] = j0 + key < len ? vs[key] : 0.f;
+        }
+    }
+    const bool edge = j0 + KW - 1 > first;    // some row does not see some of the keys
+    uint32_t pf[KT][NT][2], pl[FP8 ? 1 : KT][NT][2];   // bf16: and what rounding P to it leaves
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float f[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float mx = m[nt][e];
+#pragma unroll
+        for (int j = 0; j < KT; ++j)
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            float& x = sc[j][nt][2 * hh + e];
+            x *= FP8 ? qs[nt][e] * kscale[j][hh] : qs[nt][e];
+            if (edge && j0 + 16 * j + 8 * hh + lg > lim[nt][e]) x = -INFINITY;
+            mx = fmaxf(mx, x);
+          }
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        const float base = mx == -INFINITY ? 0.f : mx;
+        f[e] = ex2(m[nt][e] - base);
+        m[nt][e] = mx;
+        float add = 0.f;
+#pragma unroll
+        for (int j = 0; j < KT; ++j)
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            float& x = sc[j][nt][2 * hh + e];
+            x = ex2(x - base);
+            add += x;
+            if (FP8) x *= vscale[j][hh];
+          }
+        l[nt][e] = l[nt][e] * f[e] + add;
+        if (FP8) {                      // into f16's range, each row by what its own sum is made of
+          float top = 0.f;
+#pragma unroll
+          for (int j = 0; j < KT; ++j) top = fmaxf(top, fmaxf(sc[j][nt][e], sc[j][nt][2 + e]));
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+          const int before = unit(big[nt][e]);
+          big[nt][e] = fmaxf(big[nt][e] * f[e], top);
+          const int now = unit(big[nt][e]);
+          f[e] *= pow2(before - now);   // (the exponent falls only as far as f does)
+          const float dn = pow2(-now) * 32768.f;
+#pragma unroll
+          for (int j = 0; j < KT; ++j) sc[j][nt][e] *= dn, sc[j][nt][2 + e] *= dn;
+        }
+      }
+      if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i][nt][0] *= f[0], o[i][nt][1] *= f[1], o[i][nt][2] *= f[0], o[i][nt][3] *= f[1];
+      }
+#pragma unroll
+      for (int j = 0; j < KT; ++j)
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const float a = sc[j][nt][2 * hh], e = sc[j][nt][2 * hh + 1];
+          const uint32_t p2 = FP8 ? pack_f16(a, e) : pack_bf16(a, e);
+          pf[j][nt][hh] = transpose8x8(p2);
+          if (!FP8) pl[FP8 ? 0 : j][nt][hh] = transpose8x8(pack_bf16(a - bf16lo(p2), e - bf16hi(p2)));
+        }
+    }
+    // O^T: 8 tiles of 16 dims
+#pragma unroll
+    for (int j = 0; j < KT; ++j) {
+      if (FP8) {                        // row lg of tile i is dim 16 lg + 2 i, row lg + 8 the next: a thread's chunk lg holds all its dims
+        uint4 w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int row = 8 * (k >> 1) + 2 * lt + (k & 1);
+          w[k] = lds128_at(vb + (16 * j + row) * 128 + ((lg ^ (row & 7)) * 16));
+        }
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          uint32_t a[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) a[k] = q4 == 0 ? w[k].x : q4 == 1 ? w[k].y : q4 == 2 ? w[k].z : w[k].w;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t lo = __byte_perm(a[0], a[1], i ? 0x7362 : 0x5140), hi = __byte_perm(a[2], a[3], i ? 0x7362 : 0x5140);
+            const uint32_t af[4] = {e4m3x2_to_f16x2(lo), e4m3x2_to_f16x2(lo >> 16), e4m3x2_to_f16x2(hi), e4m3x2_to_f16x2(hi >> 16)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) few_mma<FP8>(o[2 * q4 + i][nt], af, pf[j][nt][0], pf[j][nt][1]);
+          }
+        }
+      } else {                          // row lg of tile i is dim 16 i + lg
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = (lane & 7) + 8 * (lane >> 4), ch = (2 * i + ((lane >> 3) & 1)) & 7;
+          uint32_t af[4];
+          ldmatrix4_trans(af, vb + (i >> 2) * half + (16 * j + row) * 128 + ((ch ^ (row & 7)) * 16));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            few_mma<FP8>(o[i][nt], af, pf[j][nt][0], pf[j][nt][1]);
+            few_mma<FP8>(o[i][nt], af, pl[FP8 ? 0 : j][nt][0], pl[FP8 ? 0 : j][nt][1]);
+          }
+        }
+      }
+    }
+  }
+
+  // After the last step: l is the whole row's; what the row's outputs are to be multiplied by, beside the weight of its maximum.
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], d);
+  }
+  __device__ __forceinline__ float unscale(int nt, int e) const { return FP8 ? pow2(unit(big[nt][e])) * (1.f / 32768.f) : 1.f; }
+  static __device__ __forceinline__ int dim(int i, int e, int lg) { return FP8 ? 16 * lg + 2 * i + (e >> 1) : 16 * i + 8 * (e >> 1) + lg; }
+};
+
 template <bool FP8, int NT>
 __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_kernel(const __grid_constant__ FewParams p) {
   using Sh = FewShape<FP8, NT>;
@@ -311,223 +546,20 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
   // ---- consumers ----
   if constexpr (Sh::SPLIT) regs_inc<Sh::CONSUMER>();
   const int grp = warp / (KEYS / KW), part = warp % (KEYS / KW), lg = lane >> 2, lt = lane & 3;
-  const float sl2 = r.scale * LOG2E;
   bool ok = true;
   int it = 0;
   for (long long u = u0; u < u1;) {
     const int t1 = (int)min((long long)n, t0 + (u1 - u));
     const int rows = s.n * r.group;
-    // the query rows as B fragments: thread (lg, lt) holds row lg of each tile; the dims of its MMA k slots are the ones
-    // its 16-byte K chunks below hold
-    uint32_t qf[NT][8][2];
-    float qs[NT][2];                        // of rows 2 lt, 2 lt + 1: scale * log2 e, fp8: times the power of two that undoes q's
-    int lim[NT][2];                         // the last key each of them sees
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int row = nt * 8 + lg;
-      uint4 x[4] = {};
-      if (row < rows) {
-        const bf16* src = r.q + (long long)(s.row0 + row / r.group) * r.q_row + (long long)(g * r.group + row % r.group) * r.q_head;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)         // bf16: chunks 2 lt, 2 lt + 1 of each 64-dim half; e4m3: dims 32 lt .. + 31
-          x[i] = *reinterpret_cast<const uint4*>(src + (FP8 ? 32 * lt + 8 * i : 64 * (i >> 1) + 16 * lt + 8 * (i & 1)));
-      }
-      float own = sl2;
-      if (FP8) {
-        float f[4][8], mx = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          unpack_bf16x8(x[i], f[i]);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(f[i][e]));
-        }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const int e2 = min(max(exponent_above(mx), -110), 110);
-        const float up = pow2(8 - e2);      // the row's largest value lands in [2^7, 2^8)
-        own = sl2 * pow2(e2 - 8);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          x[i] = make_uint4(pack_f16(f[i][0] * up, f[i][1] * up), pack_f16(f[i][2] * up, f[i][3] * up),
-                            pack_f16(f[i][4] * up, f[i][5] * up), pack_f16(f[i][6] * up, f[i][7] * up));
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        qf[nt][2 * i][0] = x[i].x, qf[nt][2 * i][1] = x[i].y;
-        qf[nt][2 * i + 1][0] = x[i].z, qf[nt][2 * i + 1][1] = x[i].w;
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        qs[nt][e] = __shfl_sync(0xffffffffu, own, (2 * lt + e) * 4);
-        lim[nt][e] = min(s.len - 1, s.len - s.n + (nt * 8 + 2 * lt + e) / r.group);
-      }
-    }
-    float o[8][NT][4], m[NT][2], l[NT][2];
-    // fp8: the largest weight times V scale of each row so far, under the running maximum; P times the V scale is taken over
-    // the power of two above it
-    float big[NT][2];
-    auto unit = [](float x) { return max(exponent_above(x), -100); };
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
-      m[nt][0] = m[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = 0.f;
-      big[nt][0] = big[nt][1] = 0.f;
-    }
+    FewRows<FP8, NT, KT> w;
+    w.begin(r, s.row0, s.n, s.len, 0, rows, g, lane);
     for (int t = t0; t < t1; ++t, ++it) {
       if (GROUPS > 1 && it % GROUPS != grp) continue;
       const int st = it % S, j0 = t * KEYS + part * KW;
       ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.full[st], (uint32_t)((it / S) & 1)));
       if (ok && j0 < s.len) {
-        const uint32_t kb = smem_u32(sm.k[st]) + (part * KW) * 128, vb = smem_u32(sm.v[st]) + (part * KW) * 128;
-        if (j0 + KW > s.len) {              // the sequence ends inside: what lies behind it must not reach P.V, as 0 x NaN
-          for (int i = lane; i < (j0 + KW - s.len) * (FP8 ? 8 : 16); i += 32) {
-            const int row = (s.len - j0) + i / (FP8 ? 8 : 16), ch = i % (FP8 ? 8 : 16);
-            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(vb + (ch >> 3) * (TILE / 2) + row * 128 + (ch & 7) * 16), "r"(0) : "memory");
-          }
-          fence_proxy_async_smem();         // the ring's next copy into these rows comes after
-          __syncwarp();
-        }
-        // scores of KT tiles of 16 keys: thread (lg, lt) has keys lg and lg + 8 of query rows 2 lt and 2 lt + 1
-        float sc[KT][NT][4];
-#pragma unroll
-        for (int j = 0; j < KT; ++j) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) sc[j][nt][0] = sc[j][nt][1] = sc[j][nt][2] = sc[j][nt][3] = 0.f;
-          const uint32_t ra = kb + (16 * j + lg) * 128;   // row & 7 == lg, of row + 8 too
-#pragma unroll
-          for (int i = 0; i < (FP8 ? 2 : 4); ++i) {
-            const uint32_t at = ra + (FP8 ? 0 : (i >> 1) * (TILE / 2)) + ((2 * lt + (i & 1)) ^ lg) * 16;
-            const uint4 w = lds128_at(at), z = lds128_at(at + 8 * 128);
-            if (FP8) {
-              const uint32_t ww[4] = {w.x, w.y, w.z, w.w}, zz[4] = {z.x, z.y, z.z, z.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t af[4] = {e4m3x2_to_f16x2(ww[e]), e4m3x2_to_f16x2(zz[e]), e4m3x2_to_f16x2(ww[e] >> 16), e4m3x2_to_f16x2(zz[e] >> 16)};
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) few_mma<FP8>(sc[j][nt], af, qf[nt][4 * i + e][0], qf[nt][4 * i + e][1]);
-              }
-            } else {
-              const uint32_t a0[4] = {w.x, z.x, w.y, z.y}, a1[4] = {w.z, z.z, w.w, z.w};
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                few_mma<FP8>(sc[j][nt], a0, qf[nt][2 * i][0], qf[nt][2 * i][1]);
-                few_mma<FP8>(sc[j][nt], a1, qf[nt][2 * i + 1][0], qf[nt][2 * i + 1][1]);
-              }
-            }
-          }
-        }
-        float kscale[KT][2], vscale[KT][2];
-        if (FP8) {
-#pragma unroll
-          for (int j = 0; j < KT; ++j)
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-              const int key = part * KW + 16 * j + 8 * hh + lg;
-              kscale[j][hh] = sm.ks[st][key];
-              vscale[j][hh] = t * KEYS + key < s.len ? sm.vs[st][key] : 0.f;
-            }
-        }
-        const bool edge = j0 + KW - 1 > s.len - s.n;    // some row does not see some of the keys
-        uint32_t pf[KT][NT][2], pl[FP8 ? 1 : KT][NT][2];   // bf16: and what rounding P to it leaves
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float f[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float mx = m[nt][e];
-#pragma unroll
-            for (int j = 0; j < KT; ++j)
-#pragma unroll
-              for (int hh = 0; hh < 2; ++hh) {
-                float& x = sc[j][nt][2 * hh + e];
-                x *= FP8 ? qs[nt][e] * kscale[j][hh] : qs[nt][e];
-                if (edge && j0 + 16 * j + 8 * hh + lg > lim[nt][e]) x = -INFINITY;
-                mx = fmaxf(mx, x);
-              }
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-            const float base = mx == -INFINITY ? 0.f : mx;
-            f[e] = ex2(m[nt][e] - base);
-            m[nt][e] = mx;
-            float add = 0.f;
-#pragma unroll
-            for (int j = 0; j < KT; ++j)
-#pragma unroll
-              for (int hh = 0; hh < 2; ++hh) {
-                float& x = sc[j][nt][2 * hh + e];
-                x = ex2(x - base);
-                add += x;
-                if (FP8) x *= vscale[j][hh];
-              }
-            l[nt][e] = l[nt][e] * f[e] + add;
-            if (FP8) {                      // into f16's range, each row by what its own sum is made of
-              float top = 0.f;
-#pragma unroll
-              for (int j = 0; j < KT; ++j) top = fmaxf(top, fmaxf(sc[j][nt][e], sc[j][nt][2 + e]));
-#pragma unroll
-              for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-              const int before = unit(big[nt][e]);
-              big[nt][e] = fmaxf(big[nt][e] * f[e], top);
-              const int now = unit(big[nt][e]);
-              f[e] *= pow2(before - now);   // (the exponent falls only as far as f does)
-              const float dn = pow2(-now) * 32768.f;
-#pragma unroll
-              for (int j = 0; j < KT; ++j) sc[j][nt][e] *= dn, sc[j][nt][2 + e] *= dn;
-            }
-          }
-          if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[i][nt][0] *= f[0], o[i][nt][1] *= f[1], o[i][nt][2] *= f[0], o[i][nt][3] *= f[1];
-          }
-#pragma unroll
-          for (int j = 0; j < KT; ++j)
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-              const float a = sc[j][nt][2 * hh], e = sc[j][nt][2 * hh + 1];
-              const uint32_t p2 = FP8 ? pack_f16(a, e) : pack_bf16(a, e);
-              pf[j][nt][hh] = transpose8x8(p2);
-              if (!FP8) pl[FP8 ? 0 : j][nt][hh] = transpose8x8(pack_bf16(a - bf16lo(p2), e - bf16hi(p2)));
-            }
-        }
-        // O^T: 8 tiles of 16 dims
-#pragma unroll
-        for (int j = 0; j < KT; ++j) {
-          if (FP8) {                        // row lg of tile i is dim 16 lg + 2 i, row lg + 8 the next: a thread's chunk lg holds all its dims
-            uint4 w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int row = 8 * (k >> 1) + 2 * lt + (k & 1);
-              w[k] = lds128_at(vb + (16 * j + row) * 128 + ((lg ^ (row & 7)) * 16));
-            }
-#pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-              uint32_t a[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) a[k] = q4 == 0 ? w[k].x : q4 == 1 ? w[k].y : q4 == 2 ? w[k].z : w[k].w;
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const uint32_t lo = __byte_perm(a[0], a[1], i ? 0x7362 : 0x5140), hi = __byte_perm(a[2], a[3], i ? 0x7362 : 0x5140);
-                const uint32_t af[4] = {e4m3x2_to_f16x2(lo), e4m3x2_to_f16x2(lo >> 16), e4m3x2_to_f16x2(hi), e4m3x2_to_f16x2(hi >> 16)};
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) few_mma<FP8>(o[2 * q4 + i][nt], af, pf[j][nt][0], pf[j][nt][1]);
-              }
-            }
-          } else {                          // row lg of tile i is dim 16 i + lg
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int row = (lane & 7) + 8 * (lane >> 4), ch = (2 * i + ((lane >> 3) & 1)) & 7;
-              uint32_t af[4];
-              ldmatrix4_trans(af, vb + (i >> 2) * (TILE / 2) + (16 * j + row) * 128 + ((ch ^ (row & 7)) * 16));
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                few_mma<FP8>(o[i][nt], af, pf[j][nt][0], pf[j][nt][1]);
-                few_mma<FP8>(o[i][nt], af, pl[FP8 ? 0 : j][nt][0], pl[FP8 ? 0 : j][nt][1]);
-              }
-            }
-          }
-        }
+        w.step(smem_u32(sm.k[st]) + (part * KW) * 128, smem_u32(sm.v[st]) + (part * KW) * 128, TILE / 2, &sm.ks[FP8 ? st : 0][FP8 ? part * KW : 0],
+               &sm.vs[FP8 ? st : 0][FP8 ? part * KW : 0], j0, s.len, s.len - s.n, lane);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.empty[st]);
@@ -538,14 +570,12 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
     const bool whole = t1 - t0 == n;
     const int cf = owner_of(unit0, W, G), cl = owner_of(unit0 + n - 1, W, G);
     const int slot = u == u0 ? 0 : 1;
+    w.finish();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], d);
-        if (lg == 0) sm.wm[warp][nt * 8 + 2 * lt + e] = m[nt][e], sm.wl[warp][nt * 8 + 2 * lt + e] = l[nt][e];
-      }
+      for (int e = 0; e < 2; ++e)
+        if (lg == 0) sm.wm[warp][nt * 8 + 2 * lt + e] = w.m[nt][e], sm.wl[warp][nt * 8 + 2 * lt + e] = w.l[nt][e];
     few_sync(CW * 32);
     float f[NT][2];
 #pragma unroll
@@ -554,19 +584,16 @@ __global__ void __launch_bounds__(FewShape<FP8, NT>::THREADS, 1) few_attention_k
       for (int e = 0; e < 2; ++e) {
         float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < CW; ++w) M = fmaxf(M, sm.wm[w][nt * 8 + 2 * lt + e]);
-        f[nt][e] = M == -INFINITY ? 1.f : ex2(m[nt][e] - M);
-        if (FP8) f[nt][e] *= pow2(unit(big[nt][e])) * (1.f / 32768.f);
+        for (int k = 0; k < CW; ++k) M = fmaxf(M, sm.wm[k][nt * 8 + 2 * lt + e]);
+        f[nt][e] = M == -INFINITY ? 1.f : ex2(w.m[nt][e] - M);
+        if (FP8) f[nt][e] *= w.unscale(nt, e);
       }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int d = FP8 ? 16 * lg + 2 * i + (e >> 1) : 16 * i + 8 * (e >> 1) + lg;
-          sm.sum[warp][nt * 8 + 2 * lt + (e & 1)][d] = o[i][nt][e] * f[nt][e & 1];
-        }
+        for (int e = 0; e < 4; ++e) sm.sum[warp][nt * 8 + 2 * lt + (e & 1)][w.dim(i, e, lg)] = w.o[i][nt][e] * f[nt][e & 1];
     few_sync(CW * 32);
     // thread: 8 dims of a row (16 threads a row)
     for (int i = tid; i < rows * 16; i += CW * 32) {

@@ -38,7 +38,7 @@
 //    multiplications and broadcast loads); P times the V scale is what is rounded to bf16. Folding the scales into the tiles,
 //    rounded to bf16, was a fifth faster and half as far off again (3.4e-3 against 2.3e-3; fp32 sums rounded once: 1.7e-3).
 #pragma once
-#include "attention_few.cuh"
+#include "attention_own.cuh"
 
 namespace qk {
 
@@ -51,6 +51,9 @@ constexpr float TCA_LAZY = 32.f;          // log2 of the growth that a stale max
 constexpr float TCA_SHIFT = 16.f;         // P's largest value under a fresh maximum is 2^-16, under a stale one 2^16
 
 enum { SRC_PACKED = 0, SRC_PAGED = 1, SRC_PAGED_FP8 = 2 };
+// What the kernel's sequences are: whole ones; the groups of shared_attention, whose rows all see all of the prefix and whose
+// sums it leaves to the next launches; or what follows a sequence's prefix, whose sums are added.
+enum { TC_WHOLE = 0, TC_PREFIX = 1, TC_OWN = 2 };
 
 struct TcAttnParams {
   CUtensorMap tm_q;         // {128 dims, n_q heads, T rows}: box {64, group, 128 / group}
@@ -60,16 +63,35 @@ struct TcAttnParams {
   float* ml;                // [grid][2][2 tiles][128 rows][2]
   int* counters;            // [grid], zero between launches
   int min_rows;             // sequences with fewer query rows per KV head are another kernel's
-  int after_few;            // launched behind the few-row kernel of the same call, which it need not wait for
+  int after;                // launched behind another kernel of the same call, which it need not wait for at its start
+  int seqs;                 // sequences, or groups
+  SharedParams x;           // (prefixes: part and ml are its)
 };
 
 struct TcSeq {
   int row0, n, len;         // token rows, keys (n 0: nothing to do here)
+  int table, start;         // the row of the block table; keys before these that a shared prefix has
 };
-template <int SRC>
+template <int SRC, int MODE>
 __device__ __forceinline__ TcSeq tc_seq(const TcAttnParams& p, int b) {
   const RaggedParams& r = p.r;
   TcSeq s;
+  s.table = b;
+  s.start = 0;
+  if (MODE == TC_PREFIX) {
+    const SharedGroup g = shared_group(p.x, r.c, b);
+    s.table = g.first;
+    s.row0 = s.n = 0;
+    s.len = g.keys;
+    if (g.keys) {
+      s.row0 = __ldg(r.c.cu + g.first);
+      s.n = __ldg(r.c.cu + g.end) - s.row0;
+      const bool bad = s.row0 < 0 || s.n < 0 || s.n > r.T - s.row0;
+      if (bad) atomicOr(&g_dev_error, DEVERR_BAD_STATE);
+      if (bad) s.n = 0;
+    }
+    return s;
+  }
   s.row0 = __ldg(r.c.cu + b);
   s.n = __ldg(r.c.cu + b + 1) - s.row0;
   s.len = s.n;
@@ -85,6 +107,12 @@ __device__ __forceinline__ TcSeq tc_seq(const TcAttnParams& p, int b) {
   const bool bad = s.row0 < 0 || s.n < 0 || s.n > r.T - s.row0;
   if (bad) atomicOr(&g_dev_error, DEVERR_BAD_STATE);
   if (bad || s.n * r.group < p.min_rows) s.n = 0;
+  if (MODE == TC_OWN && s.n) {
+    s.start = shared_keys(p.x, r.c, b);
+    s.len -= s.start;
+    if (s.start && s.len < s.n) atomicOr(&g_dev_error, DEVERR_BAD_STATE);
+    s.len = max(s.len, 0);
+  }
   return s;
 }
 // sum over i < n of floor((a i + b) / 128), a and b not negative (Euclid's scheme: the lattice points under a line)
@@ -117,15 +145,18 @@ __device__ __forceinline__ long long div_short(long long a, long long b) {   // 
 }
 // The cost of a sequence's tile pairs: pair i covers tokens [i step, (i + 1) step) and the keys its last token sees, so
 // many tiles (one where it sees none: there still are rows to set to zero), and TCA_UNIT_COST.
+// FLAT: every token sees all keys.
+template <bool FLAT>
 struct TcPairs {
   int n, step, a, len;      // pairs; tokens of a pair; keys before the first token; keys
   __host__ __device__ __forceinline__ TcPairs(const TcSeq& s, int step_) : n((s.n + step_ - 1) / step_), step(step_), a(s.len - s.n), len(s.len) {}
   __host__ __device__ __forceinline__ int tiles(int i) const {
-    const int x = i == n - 1 ? len : a + (i + 1) * step;
+    const int x = FLAT || i == n - 1 ? len : a + (i + 1) * step;
     return max(1, (x + TCA_KEYS - 1) / TCA_KEYS);
   }
   __host__ __device__ __forceinline__ int cost(int i) const { return tiles(i) + TCA_UNIT_COST; }
   __host__ __device__ __forceinline__ long long before(int i) const {   // cost of the pairs 0 .. i - 1
+    if (FLAT) return (long long)i * cost(0);
     const int q = min(i, n - 1), z = a < 0 ? min(q, -a / step) : 0;
     if (i <= 0) return 0;
     return z + floor_sum(q - z, step, a + (z + 1) * step + TCA_KEYS - 1) + (i == n ? tiles(n - 1) : 0) + (long long)i * TCA_UNIT_COST;
@@ -136,10 +167,11 @@ struct TcPlace {              // where a range begins
   int b, g, pair, t;
   long long u;
 };
-template <int SRC>
+template <int SRC, int MODE>
 struct TcAttnSmem {
-  static constexpr int S = SRC == SRC_PAGED_FP8 ? 4 : 5;   // K and V tiles of the ring
-  static constexpr int RAW = SRC == SRC_PAGED_FP8 ? 2 : 0;  // e4m3 tiles on their way to bf16
+  // K and V tiles of the ring; e4m3 tiles on their way to bf16 (prefixes are bound by what is on its way from memory)
+  static constexpr int S = SRC != SRC_PAGED_FP8 ? 5 : MODE == TC_PREFIX ? 3 : 4;
+  static constexpr int RAW = SRC != SRC_PAGED_FP8 ? 0 : MODE == TC_PREFIX ? 4 : 2;
   uint8_t q[2][TCA_TILE];
   uint8_t kv[S][TCA_TILE];
   uint8_t raw[RAW ? RAW : 1][RAW ? TCA_KEYS * HEAD_DIM : 16];
@@ -149,7 +181,7 @@ struct TcAttnSmem {
   float k_scale[RAW ? 3 : 1][RAW ? TCA_KEYS : 4], v_scale[RAW ? 2 : 1][RAW ? TCA_KEYS : 4];
   long long total;
   TcPlace at[2];
-  uint64_t q_full, q_empty, full[S], empty[S], raw_full[2], raw_empty[2];
+  uint64_t q_full, q_empty, full[S], empty[S], raw_full[RAW ? RAW : 1], raw_empty[RAW ? RAW : 1];
   uint64_t s_full[2], p_full[2][2], o_full[2], v_clean[S];   // per tile (P in two halves); per stage
   uint32_t tmem;
   int last;
@@ -268,17 +300,22 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
+// A prefix with few rows: a tile's four warps of 32 rows hold them 2 or 4 times (`parts`), each part for its own half or quarter of
+// every key tile. What a tile costs then is the chain from its scores to its product with V, and a thread's 128 exponentials
+// are the longest part of that: 128 / parts remain (and zeros for the other parts' keys).
+__device__ __forceinline__ int prefix_parts(int n, int tpq) { return n <= tpq ? 4 : n <= 2 * tpq ? 2 : 1; }
+
 // A CTA's walk over its pieces; every role walks the same one.
-template <int SRC>
+template <int SRC, int MODE>
 struct TcWalk {
   const TcAttnParams& p;
   int b, g, pair, t0, step;
   TcSeq s;
-  TcPairs pr;
+  TcPairs<MODE == TC_PREFIX> pr;
   long long u, u1;
   int n, t1;                // the unit's key tiles; the piece is [t0, t1)
-  __device__ __forceinline__ TcWalk(const TcAttnParams& p_, const TcAttnSmem<SRC>& sm, int step_)
-      : p(p_), b(sm.at[0].b), g(sm.at[0].g), pair(sm.at[0].pair), t0(max(0, sm.at[0].t - TCA_UNIT_COST)), step(step_), s(tc_seq<SRC>(p_, sm.at[0].b)), pr(s, step_),
+  __device__ __forceinline__ TcWalk(const TcAttnParams& p_, const TcAttnSmem<SRC, MODE>& sm, int step_)
+      : p(p_), b(sm.at[0].b), g(sm.at[0].g), pair(sm.at[0].pair), t0(max(0, sm.at[0].t - TCA_UNIT_COST)), step(step_), s(tc_seq<SRC, MODE>(p_, sm.at[0].b)), pr(s, step_),
         u(sm.at[0].u), u1(sm.at[1].u) {
     piece();
   }
@@ -296,9 +333,9 @@ struct TcWalk {
       pair = 0;
       if (++g == p.r.c.n_kv) {
         g = 0;
-        do s = tc_seq<SRC>(p, ++b);
+        do s = tc_seq<SRC, MODE>(p, ++b);
         while (s.n == 0);
-        pr = TcPairs(s, step);
+        pr = TcPairs<MODE == TC_PREFIX>(s, step);
       }
     }
     piece();
@@ -307,7 +344,7 @@ struct TcWalk {
   __device__ __forceinline__ int tok0(int x) const { return pair * step + x * (step / 2); }
   __device__ __forceinline__ int end(int x) const {
     if (tok0(x) >= s.n) return t0;
-    const int keys = min(s.len, s.len - s.n + min(tok0(x) + step / 2, s.n));
+    const int keys = MODE == TC_PREFIX ? s.len : min(s.len, s.len - s.n + min(tok0(x) + step / 2, s.n));
     return max(t0, min(t1, max(1, (keys + TCA_KEYS - 1) / TCA_KEYS)));
   }
 };
@@ -320,16 +357,19 @@ struct TcShape {
   static constexpr int SOFTMAX = SRC == SRC_PAGED_FP8 ? 200 : 208, OTHER = SRC == SRC_PAGED_FP8 ? 56 : 88;
   static_assert(256 * SOFTMAX + (THREADS - 256) * OTHER <= THREADS * (SRC == SRC_PAGED_FP8 ? 128 : 168), "setmaxnreg would wait for ever");
 };
-template <int SRC>
+template <int SRC, int MODE>
 __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(const __grid_constant__ TcAttnParams p) {
   extern __shared__ __align__(1024) uint8_t tca_smem[];
-  using Smem = TcAttnSmem<SRC>;
+  using Smem = TcAttnSmem<SRC, MODE>;
+  using Pairs = TcPairs<MODE == TC_PREFIX>;
+  using Walk = TcWalk<SRC, MODE>;
   Smem& sm = *reinterpret_cast<Smem*>(tca_smem);
-  constexpr int TCA_STAGES = Smem::S;
+  constexpr int TCA_STAGES = Smem::S, RAW = Smem::RAW ? Smem::RAW : 1;
   constexpr bool FP8 = SRC == SRC_PAGED_FP8;
   const RaggedParams& r = p.r;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x, n_kv = r.c.n_kv;
-  const int step = 2 * (128 / r.group);   // tokens of a tile pair
+  const int tpq = 32 / r.group;           // prefixes: tokens of a warp's 32 rows
+  const int step = MODE == TC_PREFIX ? 8 * tpq : 2 * (128 / r.group);   // tokens of a tile pair
   if (tid == 0) {
     prefetch_map(&p.tm_q);
     if (!FP8) prefetch_map(&p.tm_k), prefetch_map(&p.tm_v);
@@ -340,7 +380,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
       mbar_init(&sm.empty[i], FP8 ? 1 : 2);   // the MMAs; they and the V cleaner
       mbar_init(&sm.v_clean[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < RAW; ++i) {
       mbar_init(&sm.raw_full[i], 1);
       mbar_init(&sm.raw_empty[i], 6);
     }
@@ -355,18 +395,18 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
   // Behind the few-row kernel: that one let this one start after its own wait, so what came before both is complete, and
   // the two share neither rows nor scratch. CTAs take the SMs as the other's leave them; this kernel waits for the other
   // at its end, so that whatever follows it follows both.
-  if (!p.after_few) grid_dep_wait();
+  if (!p.after) grid_dep_wait();
   grid_dep_launch();
 
   // ---- this CTA's range of key tiles: sums over the sequences, 32 chunks of them; warp 0 finds where it begins, warp 1
   // where the next one does ---------------------------------------------------------------------------------------------
   if (warp < 2) {
-    const int per = (r.c.B + 31) / 32;
+    const int per = (p.seqs + 31) / 32;
     long long mine = 0, tot = 0;
-    TcSeq s = {0, 0, 0};
-    for (int b = lane * per; b < min(r.c.B, (lane + 1) * per); ++b) {
-      s = tc_seq<SRC>(p, b);
-      const TcPairs pr(s, step);
+    TcSeq s = {0, 0, 0, 0, 0};
+    for (int b = lane * per; b < min(p.seqs, (lane + 1) * per); ++b) {
+      s = tc_seq<SRC, MODE>(p, b);
+      const Pairs pr(s, step);
       tot = pr.n ? pr.before(pr.n) : 0;
       mine += tot * n_kv;
     }
@@ -379,25 +419,25 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
     const long long W = __shfl_sync(0xffffffffu, incl, 31);
     const int G = (int)min((long long)gridDim.x, max(1ll, W / TCA_MIN_PIECE));
     const long long u = div_short(min(c + warp, G) * W, G);
-    int b = r.c.B, g = 0, pair = 0, t = 0;
+    int b = p.seqs, g = 0, pair = 0, t = 0;
     long long at = W;
     if (u < W) {
       const int first = __ffs(__ballot_sync(0xffffffffu, incl > u)) - 1;
       at = __shfl_sync(0xffffffffu, incl - mine, first);
       b = first * per;
       if (per == 1) {                       // the lane's sequence is the one
-        s = {__shfl_sync(0xffffffffu, s.row0, first), __shfl_sync(0xffffffffu, s.n, first), __shfl_sync(0xffffffffu, s.len, first)};
+        s = {__shfl_sync(0xffffffffu, s.row0, first), __shfl_sync(0xffffffffu, s.n, first), __shfl_sync(0xffffffffu, s.len, first), 0, 0};
         tot = __shfl_sync(0xffffffffu, tot, first);
       } else {
         for (;; ++b) {
-          s = tc_seq<SRC>(p, b);
-          const TcPairs pr(s, step);
+          s = tc_seq<SRC, MODE>(p, b);
+          const Pairs pr(s, step);
           tot = pr.n ? pr.before(pr.n) : 0;
           if (u < at + tot * n_kv) break;
           at += tot * n_kv;
         }
       }
-      const TcPairs pr(s, step);
+      const Pairs pr(s, step);
       g = (int)div_short(u - at, tot);
       at += g * tot;
       int lo = 0, hi = pr.n;                // the pair: before(lo) <= u - at < before(hi)
@@ -422,7 +462,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
           if (++g == n_kv) {
             g = 0;
             do ++b;
-            while (b < r.c.B && tc_seq<SRC>(p, b).n == 0);
+            while (b < p.seqs && tc_seq<SRC, MODE>(p, b).n == 0);
           }
         }
       }
@@ -448,7 +488,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
   if (warp >= 8) {
     regs_dec<TcShape<SRC>::OTHER>();
     if (work && warp == 8) {   // ---- loads ----
-      TcWalk<SRC> w(p, sm, step);
+      Walk w(p, sm, step);
       const int RB = SRC == SRC_PACKED ? TCA_KEYS : min(1 << r.c.page_shift, TCA_KEYS);
       const uint32_t q_bytes = (uint32_t)(step / 2) * r.group * HEAD_DIM * 2;
       int it = 0;
@@ -460,13 +500,20 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         if (lane == 0) {
           mbar_arrive_expect_tx(&sm.q_full, two ? 2 * q_bytes : q_bytes);
           for (int x = 0; x < (two ? 2 : 1); ++x)
-            for (int h = 0; h < 2; ++h)
-              tma_load_3d(sm.q[x] + h * (TCA_TILE / 2), &p.tm_q, 64 * h, w.g * r.group, w.s.row0 + w.tok0(x), &sm.q_full);
+            for (int h = 0; h < 2; ++h) {
+              if (MODE == TC_PREFIX) {
+                const int per = 4 / prefix_parts(w.s.n, tpq);   // a part's quarters
+                for (int k = 0; k < 4; ++k)
+                  tma_load_3d(sm.q[x] + h * (TCA_TILE / 2) + k * 32 * 128, &p.tm_q, 64 * h, w.g * r.group, w.s.row0 + w.tok0(x) + k % per * tpq, &sm.q_full);
+              } else {
+                tma_load_3d(sm.q[x] + h * (TCA_TILE / 2), &p.tm_q, 64 * h, w.g * r.group, w.s.row0 + w.tok0(x), &sm.q_full);
+              }
+            }
         }
         auto page_of = [&](int t) {           // this lane's box of tile t: its page, -1 where it holds no key
           const int j = t * TCA_KEYS + lane * RB;
           if (lane * RB >= TCA_KEYS || j >= w.s.len) return -1;
-          int pg = __ldg(r.c.table + (size_t)w.b * r.c.table_stride + (j >> r.c.page_shift));
+          int pg = __ldg(r.c.table + (size_t)(MODE == TC_PREFIX ? w.s.table : w.b) * r.c.table_stride + ((MODE == TC_OWN ? j + w.s.start : j) >> r.c.page_shift));
           if (pg < 0 || pg >= r.c.n_pages) {
             atomicOr(&g_dev_error, DEVERR_BAD_STATE);
             pg = 0;
@@ -478,7 +525,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
           const int page = next;
           if (SRC != SRC_PACKED && t + 1 < w.t1) next = page_of(t + 1);
           for (int v = 0; v < 2; ++v, ++it) {   // K, then V
-            constexpr int N = FP8 ? 2 : TCA_STAGES;
+            constexpr int N = FP8 ? RAW : TCA_STAGES;
             const int st = it % N;
             uint64_t* full = FP8 ? &sm.raw_full[st] : &sm.full[st];
             if (it >= N) ok = __all_sync(0xffffffffu, mbar_wait_small(FP8 ? &sm.raw_empty[st] : &sm.empty[st], (uint32_t)((it / N - 1) & 1)));
@@ -506,12 +553,12 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         }
       }
       if (!ok)   // a wait gave up: let the copies in flight land before the shared memory goes away
-        for (int n = FP8 ? 2 : TCA_STAGES, i = max(0, it - n); i < it; ++i)
+        for (int n = FP8 ? RAW : TCA_STAGES, i = max(0, it - n); i < it; ++i)
           mbar_wait_small(FP8 ? &sm.raw_full[i % n] : &sm.full[i % n], (uint32_t)((i / n) & 1), 1000000ull);
     } else if (work && warp == 9) {   // ---- MMA issue: one thread, nothing between the products but its waits ----
       if (elect_one()) {
         constexpr uint32_t id_s = tca_idesc(false), id_o = tca_idesc(true);
-        TcWalk<SRC> w(p, sm, step);
+        Walk w(p, sm, step);
         uint32_t st = 0, par = 0, np[2] = {0, 0}, clean = 0;   // st, par: the next tile's stage, its `full` parity; clean: v_clean's
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -578,7 +625,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
       }
       __syncwarp();
     } else if (!FP8 && work && warp == 10) {   // ---- V rows past a sequence's end: another's, or nothing; 0 x NaN must not reach O ----
-      TcWalk<SRC> w(p, sm, step);
+      Walk w(p, sm, step);
       uint32_t st = 0, par = 0;
       bool ok = true;
       for (; w.more() && ok; w.next())
@@ -597,14 +644,19 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
           if (++st == TCA_STAGES) st = 0, par ^= 1;
         }
     } else if (FP8 && work) {   // ---- warps 10 to 15: e4m3 tiles to bf16 ones (exact), and their rows' scales ----
-      TcWalk<SRC> w(p, sm, step);
+      Walk w(p, sm, step);
       const int th = tid - 320, ch = th & 7, half = ch >> 2;   // this thread's 16 dims, of every 24th row
-      // the scales of key th of tile t: fetched a tile ahead
-      auto scales_of = [&](int t) {
+      // the scales of key th of tile t: fetched a tile ahead, and the number of the page that they are in two
+      auto page_of = [&](int t) {
+        const int j = t * TCA_KEYS + th;
+        return th < TCA_KEYS && t < w.t1 && j < w.s.len
+                   ? __ldg(r.c.table + (size_t)(MODE == TC_PREFIX ? w.s.table : w.b) * r.c.table_stride + ((MODE == TC_OWN ? j + w.s.start : j) >> r.c.page_shift))
+                   : -1;
+      };
+      auto scales_of = [&](int t, int pg) {
         const int j = t * TCA_KEYS + th;
         float2 y = make_float2(0.f, 0.f);
         if (th < TCA_KEYS && t < w.t1 && j < w.s.len) {
-          int pg = __ldg(r.c.table + (size_t)w.b * r.c.table_stride + (j >> r.c.page_shift));
           if (pg < 0 || pg >= r.c.n_pages) pg = 0;   // (the loads say so)
           const int at = ((pg * n_kv + w.g) << r.c.page_shift) + (j & ((1 << r.c.page_shift) - 1));
           y = make_float2(__ldg(r.c.ks + at) * (r.scale * LOG2E), __ldg(r.c.vs + at));
@@ -614,12 +666,16 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
       uint32_t it = 0;
       bool ok = true;
       for (; w.more() && ok; w.next()) {
-        float2 scales = scales_of(w.t0), ahead = make_float2(0.f, 0.f);
+        int page = page_of(w.t0 + 1);
+        float2 scales = scales_of(w.t0, page_of(w.t0)), ahead = make_float2(0.f, 0.f);
         for (int i = 2 * w.t0; i < 2 * w.t1 && ok; ++i, ++it) {   // K and V in turn
-          const uint32_t rs = it & 1, st = it % TCA_STAGES;
+          const uint32_t rs = it % RAW, st = it % TCA_STAGES;
           const bool is_v = i & 1;
-          if (!is_v) ahead = scales_of((i >> 1) + 1);
-          ok = mbar_wait_small(&sm.raw_full[rs], (it >> 1) & 1);
+          if (!is_v) {
+            ahead = scales_of((i >> 1) + 1, page);
+            page = page_of((i >> 1) + 2);
+          }
+          ok = mbar_wait_small(&sm.raw_full[rs], (it / RAW) & 1);
           if (it >= TCA_STAGES) ok = ok && mbar_wait_small(&sm.empty[st], (it / TCA_STAGES - 1) & 1);
           ok = __all_sync(0xffffffffu, ok);
           const int tail = w.s.len - (i >> 1) * TCA_KEYS;   // rows from here on were not loaded, or are not the sequence's
@@ -667,14 +723,87 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
       const int x = warp >> 2, row = tid & 127;
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lanes + 128 * x, to = tmem + lanes + 256 + 128 * x;
       const float sl2 = FP8 ? 1.f : r.scale * LOG2E;   // (an e4m3 cache: already in the keys' scales)
-      TcWalk<SRC> w(p, sm, step);
+      Walk w(p, sm, step);
       int ns = 0, no = 0, kt = 0;             // kt: key tiles of the pieces before
       bool ok = true;
       for (; w.more(); w.next()) {
-        const int e = w.end(x), tok = w.tok0(x) + row / r.group, pos = w.s.len - w.s.n + tok;
-        const bool valid = row < (step / 2) * r.group && tok < w.s.n;
-        const int first = w.s.len - w.s.n + w.tok0(x);   // the last key that the tile's first row sees
+        const int parts = MODE == TC_PREFIX ? prefix_parts(w.s.n, tpq) : 1, per = 4 / parts;
+        const int own = MODE == TC_PREFIX ? lane / r.group : row / r.group, hq = MODE == TC_PREFIX ? lane % r.group : row % r.group;
+        const int e = w.end(x), tok = w.tok0(x) + own + (MODE == TC_PREFIX ? (warp & 3) % per * tpq : 0), pos = MODE == TC_PREFIX ? w.s.len - 1 : w.s.len - w.s.n + tok;
+        const bool valid = (MODE == TC_PREFIX ? own < tpq : row < (step / 2) * r.group) && tok < w.s.n;
+        const int first = MODE == TC_PREFIX ? w.s.len - 1 : w.s.len - w.s.n + w.tok0(x);   // the last key that the tile's first row sees
         float m = -INFINITY, l = 0.f, base = 0.f;   // base = -m * sl2 - TCA_SHIFT
+        if (MODE == TC_PREFIX && parts > 1) {
+          auto tiles = [&](auto n_parts) {
+            constexpr int N = 128 / decltype(n_parts)::value;   // keys of a tile that are this part's: from k0 on
+            const int part = (warp & 3) / per, k0 = part * N;
+            for (int t = w.t0; t < e; ++t) {
+              ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.s_full[x], (uint32_t)(ns++ & 1)));
+              tc_fence_after();
+              uint32_t v[N];
+#pragma unroll
+              for (int i = 0; i < N; i += 32) tca_ld32(ts + k0 + i, v + i);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < N; i += 32) tca_tie32(v + i);
+              if (FP8) {
+                const float* ks = sm.k_scale[FP8 ? (kt + t - w.t0) % 3 : 0] + (FP8 ? k0 : 0);
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * ks[FP8 ? i : 0]);
+              }
+              float mx[2] = {m, m};
+#pragma unroll
+              for (int i = 0; i < N; i += 2) mx[(i >> 1) & 1] = max3_nan(mx[(i >> 1) & 1], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+              const float mn = max_nan(mx[0], mx[1]);
+              const bool grow = valid && !((mn - m) * sl2 <= TCA_LAZY);
+              if (__any_sync(0xffffffffu, grow)) {
+                float f = 1.f;
+                if (grow) {
+                  f = m == -INFINITY ? 0.f : ex2((m - mn) * sl2);
+                  m = mn;
+                  l *= f;
+                  base = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7fffffff) : -m * sl2 - TCA_SHIFT;
+                }
+                if (t > w.t0) {               // the products before this tile's scores are done: O is whole
+#pragma unroll 1
+                  for (int i = 0; i < 8; ++i) {
+                    uint32_t o[16];
+                    tca_ld16(to + 16 * i, o);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                    tca_st16(to + 16 * i, o);
+                  }
+                }
+              }
+              uint64_t sum[2] = {0, 0};
+              tca_exp<N / 2, FP8>(v, v, f32x2(sl2, sl2), f32x2(base, base), sum);
+              if (FP8) {                      // V's tile, and with it the scales, is there (its stage waits for this P)
+                const uint32_t i = 2 * (kt + t - w.t0) + 1;
+                ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.full[i % TCA_STAGES], (i / TCA_STAGES) & 1));
+                tca_pack<N / 2>(v, v, sm.v_scale[FP8 ? (kt + t - w.t0) & 1 : 0] + (FP8 ? k0 : 0));
+              }
+              uint32_t none[N / 2];
+#pragma unroll
+              for (int i = 0; i < N / 2; ++i) none[i] = 0;
+#pragma unroll
+              for (int k = 0; k < 128 / N; ++k) {
+                if (k == part) tca_st<N / 2>(ts + k * (N / 2), v);
+                else tca_st<N / 2>(ts + k * (N / 2), none);
+              }
+              tca_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) {
+                mbar_arrive(&sm.p_full[x][0]);
+                mbar_arrive(&sm.p_full[x][1]);
+              }
+              l += (f32x2_lo(sum[0]) + f32x2_hi(sum[0])) + (f32x2_lo(sum[1]) + f32x2_hi(sum[1]));
+            }
+          };
+          if (parts == 4) tiles(std::integral_constant<int, 4>{});
+          else tiles(std::integral_constant<int, 2>{});
+        } else
         for (int t = w.t0; t < e; ++t) {
           ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.s_full[x], (uint32_t)(ns++ & 1)));
           tc_fence_after();
@@ -767,7 +896,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
           ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.o_full[x], (uint32_t)(no++ & 1)));
           tc_fence_after();
         }
-        bf16* dst = r.out + (long long)(w.s.row0 + tok) * r.out_row + (long long)(w.g * r.group + row % r.group) * r.out_head;
+        bf16* dst = r.out + (long long)(w.s.row0 + tok) * r.out_row + (long long)(w.g * r.group + hq) * r.out_head;
         auto store = [&](const float* o, float inv, int col) {   // 32 columns
 #pragma unroll
           for (int k = 0; k < 32; k += 8) {
@@ -777,6 +906,34 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
             *reinterpret_cast<uint4*>(dst + col + k) = pack_bf16x8(y);
           }
         };
+        // sums for prefix_merge_kernel: of the own keys, or of a prefix that no other CTA has keys of, in parts
+        const int row_at = (w.s.row0 + tok) * r.n_q + w.g * r.group + hq, part = MODE == TC_PREFIX ? (warp & 3) / per : 0;
+        const int split = parts == 4 ? 2 : parts - 1;
+        const float m2 = m == -INFINITY ? m : m * sl2 + TCA_SHIFT;
+        if ((MODE == TC_PREFIX || (MODE == TC_OWN && w.s.start)) && w.t0 == 0 && w.t1 == w.n) {
+          if (any) {
+            float* sums = MODE == TC_PREFIX ? p.x.o + ((size_t)row_at * 4 + part) * HEAD_DIM : p.x.own_o + (size_t)row_at * HEAD_DIM;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t o[32];
+              tca_ld32(to + 32 * i, o);
+              tc_wait_ld();
+              tca_tie32(o);
+              if (valid) {
+#pragma unroll
+                for (int k = 0; k < 32; k += 4) *reinterpret_cast<uint4*>(sums + 32 * i + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+              }
+              __syncwarp();
+            }
+            if (valid) {
+              *(MODE == TC_PREFIX ? p.x.ml + (size_t)row_at * 4 + part : p.x.own_ml + row_at) = make_float2(m2, l);
+              if (MODE == TC_OWN) p.x.own_info[row_at] = OWN_SUMS;
+              else if (part == 0) p.x.info[row_at] = PREFIX_WHOLE | split << 24;
+            }
+            __syncwarp();
+          }
+          continue;
+        }
         if (w.t0 == 0 && w.t1 == w.n) {
           const float inv = l == 0.f ? 0.f : 1.f / l;
           if (any) {
@@ -801,7 +958,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         const int c_lo = (int)div_short((a0 + TCA_UNIT_COST + TCA_MIN_PIECE) * G + W - 1, W);
         const int c_hi = (int)div_short((a0 + TCA_UNIT_COST + w.n - TCA_MIN_PIECE + 1) * G + W - 1, W) - 1;
         const size_t slot = ((size_t)(c * 2 + (w.t0 == 0 ? 1 : 0)) * 2 + x) * 128;
-        *reinterpret_cast<float2*>(p.ml + (slot + row) * 2) = make_float2(m, l);
+        *reinterpret_cast<float2*>(p.ml + (slot + row) * 2) = make_float2(MODE == TC_PREFIX ? m2 : m, l);
         if (any) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -812,6 +969,11 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
             for (int k = 0; k < 32; k += 4)
               *reinterpret_cast<uint4*>(p.part + slot * 128 + (size_t)(8 * i + k / 4) * 512 + row * 4) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
           }
+        }
+        if (MODE == TC_PREFIX) {              // (the merge adds the pieces)
+          if (valid && w.t0 == 0 && part == 0) p.x.info[row_at] = PREFIX_PIECES | (c_lo - 1) | c_hi << 8 | (x * 128 + row) << 16 | split << 24;
+          __syncwarp();
+          continue;
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (tid == 0) {                       // releases the CTA's stores (ordered before by the barrier), acquires the others'
@@ -842,6 +1004,12 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
               for (int k = 0; k < 16; ++k)
                 o[4 * k] += q[k].x * f, o[4 * k + 1] += q[k].y * f, o[4 * k + 2] += q[k].z * f, o[4 * k + 3] += q[k].w * f;
             }
+            if (MODE == TC_OWN && w.s.start) {
+#pragma unroll
+              for (int k = 0; k < 64; k += 4) *reinterpret_cast<float4*>(p.x.own_o + (size_t)row_at * HEAD_DIM + col + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+              if (col == 0) p.x.own_ml[row_at] = make_float2(M == -INFINITY ? M : M * sl2 + TCA_SHIFT, L), p.x.own_info[row_at] = OWN_SUMS;
+              continue;
+            }
             const float inv = L == 0.f ? 0.f : 1.f / L;
             store(o, inv, col);
             store(o + 32, inv, col + 32);
@@ -852,7 +1020,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
       if (!ok && lane == 0) atomicOr(&g_dev_error, DEVERR_MBAR_TIMEOUT);
     }
   }
-  if (p.after_few) grid_dep_wait();
+  if (p.after) grid_dep_wait();
   tc_fence_before();
   __syncthreads();
   if (warp == 9) {

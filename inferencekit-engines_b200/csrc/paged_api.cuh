@@ -154,10 +154,10 @@ int encode_rows_map(CUtensorMap* map, const void* base, int heads, int T, long l
   return QK_OK;
 }
 
-template <int SRC>
-int launch_tc(const RaggedParams& r, int min_rows, bool after_few, void* workspace, cudaStream_t stream) {
+template <int SRC, int MODE = TC_WHOLE>
+int launch_tc(const RaggedParams& r, int min_rows, bool after, void* workspace, cudaStream_t stream, const SharedParams& x = {}) {
   TcAttnParams p = {};
-  if (int e = encode_rows_map(&p.tm_q, r.q, r.n_q, r.T, r.q_head, r.q_row, r.group, 128 / r.group)) return e;
+  if (int e = encode_rows_map(&p.tm_q, r.q, r.n_q, r.T, r.q_head, r.q_row, r.group, (MODE == TC_PREFIX ? 32 : 128) / r.group)) return e;
   if (SRC == SRC_PACKED) {
     if (int e = encode_rows_map(&p.tm_k, r.k, r.c.n_kv, r.T, r.kv_head, r.kv_row, 1, TCA_KEYS)) return e;
     if (int e = encode_rows_map(&p.tm_v, r.v, r.c.n_kv, r.T, r.kv_head, r.kv_row, 1, TCA_KEYS)) return e;
@@ -175,11 +175,14 @@ int launch_tc(const RaggedParams& r, int min_rows, bool after_few, void* workspa
   p.ml = ws->tc_ml;
   p.counters = ws->tc_counters;
   p.min_rows = min_rows;
-  p.after_few = after_few;
-  auto k = tc_attention_kernel<SRC>;
-  const int smem = (int)sizeof(TcAttnSmem<SRC>);
+  p.after = after;
+  p.seqs = MODE == TC_PREFIX ? x.G : r.c.B;
+  p.x = x;
+  if (MODE == TC_PREFIX) p.part = x.part, p.ml = x.part_ml;
+  auto k = tc_attention_kernel<SRC, MODE>;
+  const int smem = (int)sizeof(TcAttnSmem<SRC, MODE>);
   if (int e = ensure_smem((const void*)k, smem)) return e;
-  return launch_as(after_few || g_pdl, k, dim3(std::min(device_sms(), RAGGED_MAX_CTAS)), dim3(TcShape<SRC>::THREADS), smem, stream, p);
+  return launch_as(after || g_pdl, k, dim3(std::min(device_sms(), RAGGED_MAX_CTAS)), dim3(TcShape<SRC>::THREADS), smem, stream, p);
 }
 
 int warp_grid(long long warps, dim3* grid) {   // 8 warps a CTA

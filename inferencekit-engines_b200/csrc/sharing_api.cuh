@@ -29,6 +29,51 @@ int table_shape(long long rows, long long width, long long stride, long long pag
   return QK_OK;
 }
 
+// The attention workspace, the prefixes' pieces and the own keys'; then the rows' sums.
+struct SharedWorkspace {
+  RaggedWorkspace base;
+  float prefix_ml[RAGGED_MAX_CTAS * 2 * 256 * 2], prefix_part[RAGGED_MAX_CTAS * 2 * 256 * HEAD_DIM];
+  float2 own_ml[OWN_MAX_GRID * 2 * 16];
+  float own_part[OWN_MAX_GRID * 2 * 16 * HEAD_DIM];
+};
+constexpr long long SHARED_ROW = 5 * (HEAD_DIM * 4 + 8) + 8;   // bytes of a row and head: sums, and info
+constexpr long long shared_fixed_bytes() { return ((long long)sizeof(SharedWorkspace) + 255) / 256 * 256; }
+
+template <bool FP8, int NT>
+int launch_own(const RaggedParams& r, int strict, const SharedParams& x, cudaStream_t stream) {
+  OwnParams p = {};
+  const int box = std::min(1 << r.c.page_shift, OwnShape<FP8, NT>::KEYS);
+  const long long rows = ((long long)r.c.n_pages * r.c.n_kv) << r.c.page_shift;
+  if (int e = encode_pool_map(&p.tm_k, r.c.k, rows, FP8, box)) return e;
+  if (int e = encode_pool_map(&p.tm_v, r.c.v, rows, FP8, box)) return e;
+  p.r = r;
+  p.x = x;
+  p.strict = strict;
+  auto k = own_attention_kernel<FP8, NT>;
+  const int smem = (int)sizeof(OwnSmem<FP8, NT>);
+  if (int e = ensure_smem((const void*)k, smem)) return e;
+  return launch(k, dim3(std::min(std::min(device_sms(), RAGGED_MAX_CTAS) * OWN_WARPS, OWN_MAX_GRID)), dim3(32), smem, stream, p);
+}
+
+// The sequences' own keys, the prefixes, their sums: each launch starts beside its forerunner.
+template <bool FP8>
+int shared_launches(const RaggedParams& p, const qk_ragged_attention_t& a, const SharedParams& x, cudaStream_t st) {
+  constexpr int SRC = FP8 ? SRC_PAGED_FP8 : SRC_PAGED;
+  void* ws = a.workspace;
+  const long long rows = a.max_q * p.group;
+  std::lock_guard<std::mutex> together(workspace_mutex(ws));
+  // sequences of up to OWN_MAX_ROWS query rows a KV head, and the others on the tensor cores
+  const int strict = rows <= OWN_MAX_ROWS;
+  if (int e = rows <= 8 ? launch_own<FP8, 1>(p, strict, x, st) : launch_own<FP8, 2>(p, strict, x, st)) return e;
+  if (!strict)
+    if (int e = launch_tc<SRC, TC_OWN>(p, OWN_MAX_ROWS + 1, true, ws, st, x)) return e;
+  if (int e = launch_tc<SRC, TC_PREFIX>(p, 0, true, ws, st, x)) return e;
+  MergeParams m = {};
+  m.x = x;
+  m.out = p.out, m.out_row = p.out_row, m.out_head = p.out_head, m.n_q = p.n_q, m.rows = p.T * p.n_q;
+  return launch_as(true, prefix_merge_kernel, dim3((m.rows + 3) / 4), dim3(256), 0, st, m);
+}
+
 }  // namespace
 
 extern "C" {
@@ -140,18 +185,38 @@ int qk_beam_select(const qk_beam_select_t* args, qk_stream_t stream) {
 }
 
 long long qk_shared_attention_workspace_bytes(long long rows, long long n_q) {
-  if (rows < 0 || rows > 0x7fffffffll / 64 || n_q < 1 || n_q > 32768) return -1;
-  return qk_ragged_attention_workspace_bytes();
+  if (rows < 0 || rows > 0x7fffffffll / 64 || n_q < 1 || n_q > 32768 || rows > 0x7fffffffll / n_q) return -1;
+  return shared_fixed_bytes() + (rows * n_q + 3) / 4 * 4 * SHARED_ROW;
 }
 
 int qk_shared_attention(const qk_shared_attention_t* args, qk_stream_t stream) {
   if (!args) return fail(QK_EINVAL, "null pointer argument");
   const qk_shared_attention_t& a = *args;
+  RaggedParams p = {};
   if (a.n_groups && (!a.groups || !a.shared)) return fail(QK_EINVAL, "null pointer argument");
   if (a.n_groups < 0 || a.n_groups > 65536) return fail(QK_EINVAL, "n_groups=%lld", a.n_groups);
+  if (int r = ragged_common(&p, a.att)) return r;
+  if (int r = paged_cache(&p.c, a.att.cache, true)) return r;
   const long long need = qk_shared_attention_workspace_bytes(a.att.rows, a.att.n_q);
   if (need < 0 || a.att.workspace_bytes < need) return fail(QK_EINVAL, "workspace of %lld bytes: %lld needed", a.att.workspace_bytes, need);
-  return qk_paged_attention(&a.att, stream);
+  if (p.T == 0 || p.c.B == 0) return QK_OK;
+  if (a.n_groups == 0) return qk_paged_attention(&a.att, stream);
+  SharedParams x = {};
+  x.groups = a.groups, x.shared = a.shared, x.G = (int)a.n_groups;
+  char* ws = static_cast<char*>(a.att.workspace);
+  SharedWorkspace* fixed = static_cast<SharedWorkspace*>(a.att.workspace);
+  x.part = fixed->prefix_part, x.part_ml = fixed->prefix_ml;
+  x.own_part = fixed->own_part, x.own_part_ml = fixed->own_ml;
+  // where the rows' sums are goes by the workspace's size: calls of any shape find info as the last one left it
+  const size_t room = (size_t)(a.att.workspace_bytes - shared_fixed_bytes()) / (4 * SHARED_ROW) * 4;
+  x.own_o = reinterpret_cast<float*>(ws + shared_fixed_bytes());
+  x.o = x.own_o + room * HEAD_DIM;
+  x.own_ml = reinterpret_cast<float2*>(x.o + room * 4 * HEAD_DIM);
+  x.ml = x.own_ml + room;
+  x.info = reinterpret_cast<int*>(x.ml + room * 4);
+  x.own_info = x.info + room;
+  return a.att.cache.kv_fp8 ? shared_launches<true>(p, a.att, x, static_cast<cudaStream_t>(stream))
+                            : shared_launches<false>(p, a.att, x, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
