@@ -685,28 +685,38 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
             else sm.k_scale[FP8 ? (it >> 1) % 3 : 0][FP8 ? th : 0] = scales.x;
           }
           if (is_v) scales = ahead;
+          // 8 bytes and 8 again: two swizzled 16-byte chunks of a row. Three rows' loads before their stores: one at a time a
+          // tile took 2,500 cycles, each load's latency and each conversion's in turn
 #pragma unroll
-          for (int k = 0; k < 6; ++k) {       // 8 bytes and 8 again: two swizzled 16-byte chunks of a row
-            const int row = k * 24 + (th >> 3);
-            if (row >= TCA_KEYS) break;
+          for (int k0 = 0; k0 < 6; k0 += 3) {
+            uint2 q[3][2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {     // the second half's lanes begin with their other chunk: no bank conflict
-              const int o = j ^ half;
-              uint2 q;
-              asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(q.x), "=r"(q.y) : "r"(src + row * HEAD_DIM + ch * 16 + o * 8));
-              uint32_t y[4];
+            for (int k = 0; k < 3; ++k)
 #pragma unroll
-              for (int i2 = 0; i2 < 4; ++i2) {
-                const uint32_t h = e4m3x2_to_f16x2((i2 < 2 ? q.x : q.y) >> (16 * (i2 & 1)));
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-                y[i2] = pack_bf16(f.x, f.y);
+              for (int j = 0; j < 2; ++j) {   // the second half's lanes begin with their other chunk: no bank conflict
+                const int row = (k0 + k) * 24 + (th >> 3);
+                if (row < TCA_KEYS)
+                  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(q[k][j].x), "=r"(q[k][j].y) : "r"(src + row * HEAD_DIM + ch * 16 + (j ^ half) * 8));
               }
-              if (row >= tail) y[0] = y[1] = y[2] = y[3] = 0;
-              const int c16 = ((ch & 3) * 2 + o) ^ (row & 7);
-              asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + half * (TCA_TILE / 2) + row * 128 + c16 * 16), "r"(y[0]), "r"(y[1]),
-                           "r"(y[2]), "r"(y[3])
-                           : "memory");
-            }
+#pragma unroll
+            for (int k = 0; k < 3; ++k)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const int row = (k0 + k) * 24 + (th >> 3);
+                if (row >= TCA_KEYS) break;
+                uint32_t y[4];
+#pragma unroll
+                for (int i2 = 0; i2 < 4; ++i2) {
+                  const uint32_t h = e4m3x2_to_f16x2((i2 < 2 ? q[k][j].x : q[k][j].y) >> (16 * (i2 & 1)));
+                  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+                  y[i2] = pack_bf16(f.x, f.y);
+                }
+                if (row >= tail) y[0] = y[1] = y[2] = y[3] = 0;
+                const int c16 = ((ch & 3) * 2 + (j ^ half)) ^ (row & 7);
+                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + half * (TCA_TILE / 2) + row * 128 + c16 * 16), "r"(y[0]), "r"(y[1]),
+                             "r"(y[2]), "r"(y[3])
+                             : "memory");
+              }
           }
           fence_proxy_async_smem();
           __syncwarp();

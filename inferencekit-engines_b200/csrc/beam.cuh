@@ -7,6 +7,9 @@
 //  * The order inside a row is the order of its logits, which needs no logsumexp: a chunk leaves (max, sum) and its k best keys,
 //    value and ~index, in order. The CTA that completes a request's count merges the chunks' lists: row sums and scores in 64
 //    bits there, so that two beams' candidates are ordered by more than fp32 shows.
+//  * k best of many, twice: the k-th largest of some of them (the largest value of each of 64 or 128 groups; the heads of lists)
+//    is a lower bound of the k-th largest of all, which few more than k reach; those are ranked by counting. Where too many
+//    reach it (ties, sorted rows), k rounds of a maximum take their place.
 //  * exp in fp32, a thread's 64 terms under its own maximum; a row's sum is off by some 2^-22 of itself.
 #pragma once
 #include "paged.cuh"
@@ -52,131 +55,46 @@ __device__ __forceinline__ int beam_index(unsigned long long key) { return (int)
 struct BeamBest {            // a candidate of the merge: its score, then its flat place in the request (row * V + token)
   double s;
   unsigned at;
-  int list;
+  int list;                 // where it is from; -1: none
 };
 __device__ __forceinline__ bool beam_better(double a, unsigned ia, double b, unsigned ib) { return a > b || (a == b && ia < ib); }
 
+constexpr int BEAM_CAP = 512;              // candidates that are ranked by counting
+
+// exp2 of x - m, both already in units of log2 e
+__device__ __forceinline__ float beam_ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 template <typename T>
-__global__ void __launch_bounds__(BEAM_THREADS) beam_select_kernel(const __grid_constant__ BeamParams p) {
-  constexpr int PER = 16 / sizeof(T), N = BEAM_VECTORS * PER;   // values of a vector; of a thread
-  __shared__ unsigned long long red[BEAM_WARPS];
-  __shared__ float red_m[BEAM_WARPS], red_l[BEAM_WARPS];
-  __shared__ int s_b, s_last;
-  __shared__ double lse[BEAM_MAX_ROWS];
-  __shared__ BeamBest red_c[BEAM_WARPS];
-  __shared__ uint8_t head[BEAM_MAX_LISTS];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = blockIdx.x / p.chunks, chunk = blockIdx.x - row * p.chunks;
-  grid_dep_wait();
-  grid_dep_launch();
-  // ---- the rows' requests: all or nothing, so that every CTA comes to the same count ------------------------------------------
-  if (tid == 0) s_b = -1;
-  __syncthreads();
-  bool bad = false;
-  for (int b = tid; b < p.B; b += BEAM_THREADS) {
-    const int lo = __ldg(p.cu + b), hi = __ldg(p.cu + b + 1);
-    bad |= lo < 0 || hi < lo || hi > p.R || hi - lo > BEAM_MAX_ROWS;
-    if (lo <= row && row < hi) s_b = b;
-    if (lo == hi && b == (int)blockIdx.x)   // (the grid has a CTA for each request) without beams
-      for (int i = 0; i < p.K; ++i) {
-        const size_t at = (size_t)b * p.K + i;
-        p.out_scores[at] = -INFINITY, p.out_parents[at] = p.out_tokens[at] = -1;
-      }
-  }
-  if (__syncthreads_or(bad)) {
-    if (tid == 0) atomicOr(&g_dev_error, DEVERR_BAD_STATE);
-    return;
-  }
-  const int b = s_b;
-  if (b < 0 || row >= p.R) return;
+__device__ __forceinline__ float beam_value_of(uint32_t w, int j) {   // value j (0 or 1; fp32: 0) of a word
+  return sizeof(T) == 4 ? __uint_as_float(w) : j ? bf16hi(w) : bf16lo(w);
+}
 
-  // ---- the chunk ----------------------------------------------------------------------------------------------------------------
-  const float score = __ldg(p.scores + row);
-  const uintptr_t base = reinterpret_cast<uintptr_t>(p.logits) + (size_t)row * p.row_stride * sizeof(T);
-  const int lead = (int)(base & 15) / (int)sizeof(T);       // values of the first vector before the row
-  const uint4* vec = reinterpret_cast<const uint4*>(base & ~(uintptr_t)15);
-  const T* x0 = reinterpret_cast<const T*>(base);
-  const int g0 = chunk * p.granules;
-  alignas(16) T x[N];
-  auto index = [&](int i) { return (g0 + (i / PER) * BEAM_THREADS + tid) * PER - lead + i % PER; };
-#pragma unroll
-  for (int i = 0; i < BEAM_VECTORS; ++i) {
-    const int in_chunk = i * BEAM_THREADS + tid, first = index(i * PER);
-    uint4 w;
-    if (score != -INFINITY && in_chunk < p.granules && first >= 0 && first + PER <= p.V) {
-      w = ldg_stream(vec + g0 + in_chunk);
-      *reinterpret_cast<uint4*>(x + i * PER) = w;
-    } else {
-#pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const bool in = score != -INFINITY && in_chunk < p.granules && first + j >= 0 && first + j < p.V;
-        x[i * PER + j] = in ? x0[first + j] : (T)-INFINITY;
-      }
-    }
-  }
-  float m = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < N; ++i) m = fmaxf(m, (float)x[i]);
-  const float under = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) l += exp2f(((float)x[i] - under) * 1.4426950408889634f);
-  // the k best, one a round: the thread that gave it looks for its next
-  auto next_best = [&](unsigned long long below) {
-    unsigned long long best = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float v = (float)x[i];
-      const unsigned long long key = v > -INFINITY ? beam_key(v, index(i)) : 0;   // (a NaN is none)
-      if (key < below && key > best) best = key;
-    }
-    return best;
+struct BeamSmem {
+  union {
+    unsigned long long keys[BEAM_CAP];     // a chunk's candidates
+    struct {                               // the merge's
+      double score[BEAM_CAP];
+      unsigned at[BEAM_CAP];
+    } c;
   };
-  unsigned long long mine = next_best(~0ull);
-  unsigned long long* keys = p.keys + ((size_t)row * p.chunks + chunk) * p.K;
-  for (int k = 0; k < p.K; ++k) {
-    unsigned long long best = mine;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (lane == 0) red[warp] = best;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < BEAM_WARPS; ++w) best = max(best, red[w]);
-    if (tid == 0) keys[k] = best;
-    if (best && best == mine) mine = next_best(mine);
-    __syncthreads();
-  }
-  // (max, sum) of the chunk
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float om = __shfl_xor_sync(0xffffffffu, m, o), ol = __shfl_xor_sync(0xffffffffu, l, o), to = fmaxf(m, om);
-    const float z = to == -INFINITY ? 0.f : to;
-    l = l * exp2f((m - z) * 1.4426950408889634f) + ol * exp2f((om - z) * 1.4426950408889634f);
-    m = to;
-  }
-  if (lane == 0) red_m[warp] = m, red_l[warp] = l;
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < BEAM_WARPS; ++w) {
-      const float to = fmaxf(m, red_m[w]), z = to == -INFINITY ? 0.f : to;
-      l = l * exp2f((m - z) * 1.4426950408889634f) + red_l[w] * exp2f((red_m[w] - z) * 1.4426950408889634f);
-      m = to;
-    }
-    p.ml[(size_t)row * p.chunks + chunk] = make_float2(m, l);
-  }
-  __syncthreads();
-  const int r0 = __ldg(p.cu + b), rows = __ldg(p.cu + b + 1) - r0;
-  if (tid == 0) {
-    __threadfence();
-    const int before = atomicAdd(p.counters + b, 1);
-    s_last = before == rows * p.chunks - 1;
-    if (s_last) p.counters[b] = 0;
-    __threadfence();
-  }
-  __syncthreads();
-  if (!s_last) return;
+  float group[128];
+  double heads[BEAM_THREADS];
+  unsigned long long red[BEAM_WARPS];
+  float red_m[BEAM_WARPS], red_l[BEAM_WARPS];
+  double lse[BEAM_MAX_ROWS];
+  BeamBest red_c[BEAM_WARPS];
+  uint8_t head[BEAM_MAX_LISTS];
+  float border;
+  double border_s;
+  int b, last, count;
+};
 
-  // ---- the request is complete: its lists, merged -------------------------------------------------------------------------------
+// The merge of a request's lists, by the CTA that completed it.
+__device__ __forceinline__ void beam_merge(const BeamParams& p, BeamSmem& sm, int b, int r0, int rows) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int r = warp; r < rows; r += BEAM_WARPS) {
     const float2* ml = p.ml + (size_t)(r0 + r) * p.chunks;
     float M = -INFINITY;
@@ -193,22 +111,68 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_select_kernel(const __grid_
     const bool none = s == -INFINITY || (L == 0. && M == -INFINITY), wrong = !none && !(fabsf(s) < INFINITY && L > 0. && L < 1e300);
     if (lane == 0) {
       if (wrong) atomicOr(&g_dev_error, DEVERR_BAD_STATE);   // a NaN or +infinity among its logits, or as its score
-      lse[r] = none || wrong ? INFINITY : (double)M + log(L);
+      sm.lse[r] = none || wrong ? INFINITY : (double)M + log(L);
     }
   }
   const int lists = rows * p.chunks;
-  for (int i = tid; i < lists; i += BEAM_THREADS) head[i] = 0;
+  if (tid == 0) sm.count = 0, sm.border_s = -INFINITY;
   __syncthreads();
-  auto pick = [&]() {                       // the best head of this thread's lists
+  auto get = [&](int list, int i) {         // candidate i of a list
+    BeamBest c = {-INFINITY, 0xffffffffu, -1};
+    const int r = list / p.chunks;
+    const unsigned long long key = i < p.K && sm.lse[r] != INFINITY ? __ldcg(p.keys + ((size_t)r0 * p.chunks + list) * p.K + i) : 0;
+    if (key) c = {(double)__ldg(p.scores + r0 + r) + ((double)beam_value(key) - sm.lse[r]), (unsigned)r * (unsigned)p.V + (unsigned)beam_index(key), list};
+    return c;
+  };
+  // a lower bound of the k-th best: the k-th best of the first `depth` of every list, or of the best heads of each thread's lists
+  const int depth = lists >= p.K ? 1 : (p.K + lists - 1) / lists, n_set = min(lists * depth, BEAM_THREADS);
+  double mine = -INFINITY;
+  if (depth == 1) {
+    for (int i = tid; i < lists; i += BEAM_THREADS) mine = fmax(mine, get(i, 0).s);
+  } else if (tid < n_set) {
+    mine = get(tid / depth, tid % depth).s;
+  }
+  sm.heads[tid] = mine;
+  __syncthreads();
+  if (tid < n_set) {
+    int rank = 0;
+    for (int i = 0; i < n_set; ++i) rank += sm.heads[i] > mine || (sm.heads[i] == mine && i < tid);
+    if (rank == p.K - 1) sm.border_s = mine;
+  }
+  __syncthreads();
+  for (int i = tid; i < lists; i += BEAM_THREADS)
+    for (int k = 0;; ++k) {
+      const BeamBest c = get(i, k);
+      if (c.list < 0 || c.s < sm.border_s) break;
+      const int at = atomicAdd(&sm.count, 1);
+      if (at < BEAM_CAP) sm.c.score[at] = c.s, sm.c.at[at] = c.at;
+    }
+  __syncthreads();
+  const size_t out = (size_t)b * p.K;
+  auto write = [&](int k, bool any, double s, unsigned at) {
+    p.out_scores[out + k] = any ? (float)s : -INFINITY;
+    p.out_parents[out + k] = any ? r0 + (int)(at / (unsigned)p.V) : -1;
+    p.out_tokens[out + k] = any ? (int)(at % (unsigned)p.V) : -1;
+  };
+  const int n = sm.count;
+  if (n <= BEAM_CAP) {
+    for (int i = tid; i < n; i += BEAM_THREADS) {
+      const double s = sm.c.score[i];
+      const unsigned at = sm.c.at[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += beam_better(sm.c.score[j], sm.c.at[j], s, at);
+      if (rank < p.K) write(rank, true, s, at);
+    }
+    for (int k = n + tid; k < p.K; k += BEAM_THREADS) write(k, false, 0., 0u);
+    return;
+  }
+  // many equal ones: a round each, among the heads of the lists
+  for (int i = tid; i < lists; i += BEAM_THREADS) sm.head[i] = 0;
+  auto pick = [&]() {                       // (a thread's own lists)
     BeamBest best = {-INFINITY, 0xffffffffu, -1};
     for (int i = tid; i < lists; i += BEAM_THREADS) {
-      const int r = i / p.chunks;
-      if (head[i] >= p.K || lse[r] == INFINITY) continue;
-      const unsigned long long key = __ldcg(p.keys + ((size_t)r0 * p.chunks + i) * p.K + head[i]);
-      if (!key) continue;
-      const double s = (double)__ldg(p.scores + r0 + r) + ((double)beam_value(key) - lse[r]);
-      const unsigned at = (unsigned)r * (unsigned)p.V + (unsigned)beam_index(key);
-      if (best.list < 0 || beam_better(s, at, best.s, best.at)) best = {s, at, i};
+      const BeamBest c = get(i, sm.head[i]);
+      if (c.list >= 0 && (best.list < 0 || beam_better(c.s, c.at, best.s, best.at))) best = c;
     }
     return best;
   };
@@ -222,26 +186,203 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_select_kernel(const __grid_
       const int list = __shfl_xor_sync(0xffffffffu, best.list, o);
       if (list >= 0 && (best.list < 0 || beam_better(s, at, best.s, best.at))) best = {s, at, list};
     }
-    if (lane == 0) red_c[warp] = best;
+    if (lane == 0) sm.red_c[warp] = best;
     __syncthreads();
-    best = red_c[0];
+    best = sm.red_c[0];
     for (int w = 1; w < BEAM_WARPS; ++w) {
-      const BeamBest o = red_c[w];
+      const BeamBest o = sm.red_c[w];
       if (o.list >= 0 && (best.list < 0 || beam_better(o.s, o.at, best.s, best.at))) best = o;
     }
-    if (tid == 0) {
-      const size_t at = (size_t)b * p.K + k;
-      const bool any = best.list >= 0;
-      p.out_scores[at] = any ? (float)best.s : -INFINITY;
-      p.out_parents[at] = any ? r0 + (int)(best.at / (unsigned)p.V) : -1;
-      p.out_tokens[at] = any ? (int)(best.at % (unsigned)p.V) : -1;
-    }
+    if (tid == 0) write(k, best.list >= 0, best.s, best.at);
     if (best.list >= 0 && best.list == own.list) {
-      ++head[best.list];
+      ++sm.head[best.list];
       own = pick();
     }
     __syncthreads();
   }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(BEAM_THREADS, 4) beam_select_kernel(const __grid_constant__ BeamParams p) {
+  constexpr int PER = 16 / sizeof(T), PW = 4 / sizeof(T), WORDS = BEAM_VECTORS * 4;   // values of a vector and a word; words of a thread
+  __shared__ BeamSmem sm;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row = blockIdx.x / p.chunks, chunk = blockIdx.x - row * p.chunks;
+  grid_dep_wait();
+  grid_dep_launch();
+  // ---- the chunk: on its way before anything else is looked at ------------------------------------------------------------------
+  const uintptr_t base = reinterpret_cast<uintptr_t>(p.logits) + (size_t)row * p.row_stride * sizeof(T);
+  const int lead = (int)(base & 15) / (int)sizeof(T);       // values of the first vector before the row
+  const uint4* vec = reinterpret_cast<const uint4*>(base & ~(uintptr_t)15);
+  const int g0 = chunk * p.granules;
+  constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;   // -inf
+  uint32_t x[WORDS];
+  auto index = [&](int word) { return (g0 + (word / 4) * BEAM_THREADS + tid) * PER - lead + (word % 4) * PW; };   // of its first value
+#pragma unroll
+  for (int i = 0; i < BEAM_VECTORS; ++i) {
+    const int at = i * BEAM_THREADS + tid, first = index(4 * i);
+    uint4 w = make_uint4(NONE, NONE, NONE, NONE);
+    if (row < p.R && at < p.granules && first < p.V && first > -PER) {
+      if (first >= 0 && first + PER <= p.V) {
+        w = ldg_stream(vec + g0 + at);
+      } else {                              // a row's first and last vector: its own values only
+        uint64_t half[2] = {(uint64_t)NONE << 32 | NONE, (uint64_t)NONE << 32 | NONE};
+        const T* src = reinterpret_cast<const T*>(base);
+#pragma unroll 1
+        for (int j = max(0, -first); j < min(PER, p.V - first); ++j) {
+          const uint32_t v = sizeof(T) == 4 ? __float_as_uint((float)src[first + j]) : (uint32_t)__bfloat16_as_ushort((bf16)src[first + j]);
+          const int bit = j * (int)sizeof(T) * 8;
+          const uint64_t mask = (sizeof(T) == 4 ? 0xffffffffull : 0xffffull) << (bit & 63);
+          if (bit < 64) half[0] = (half[0] & ~mask) | (uint64_t)v << (bit & 63);
+          else half[1] = (half[1] & ~mask) | (uint64_t)v << (bit & 63);
+        }
+        w = make_uint4((uint32_t)half[0], (uint32_t)(half[0] >> 32), (uint32_t)half[1], (uint32_t)(half[1] >> 32));
+      }
+    }
+    x[4 * i] = w.x, x[4 * i + 1] = w.y, x[4 * i + 2] = w.z, x[4 * i + 3] = w.w;
+  }
+  // ---- the rows' requests: all or nothing, so that every CTA comes to the same count ------------------------------------------
+  if (tid == 0) sm.b = -1, sm.count = 0, sm.border = -INFINITY;
+  __syncthreads();
+  bool bad = false;
+  for (int b = tid; b < p.B; b += BEAM_THREADS) {
+    const int lo = __ldg(p.cu + b), hi = __ldg(p.cu + b + 1);
+    bad |= lo < 0 || hi < lo || hi > p.R || hi - lo > BEAM_MAX_ROWS;
+    if (lo <= row && row < hi) sm.b = b;
+    if (lo == hi && b == (int)blockIdx.x)   // (the grid has a CTA for each request) without beams
+      for (int i = 0; i < p.K; ++i) {
+        const size_t at = (size_t)b * p.K + i;
+        p.out_scores[at] = -INFINITY, p.out_parents[at] = p.out_tokens[at] = -1;
+      }
+  }
+  if (__syncthreads_or(bad)) {
+    if (tid == 0) atomicOr(&g_dev_error, DEVERR_BAD_STATE);
+    return;
+  }
+  const int b = sm.b;
+  if (b < 0 || row >= p.R) return;
+  const int r0 = __ldg(p.cu + b), rows = __ldg(p.cu + b + 1) - r0;
+  if (__ldg(p.scores + row) == -INFINITY) {   // a beam that is none: whatever its logits are
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) x[i] = NONE;
+  }
+
+  // ---- maximum, sum ---------------------------------------------------------------------------------------------------------------
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < WORDS; ++i)
+#pragma unroll
+    for (int j = 0; j < PW; ++j) m = fmaxf(m, beam_value_of<T>(x[i], j));
+  const float own = m;
+  constexpr float LOG2E_ = 1.4426950408889634f;
+  const float under = m == -INFINITY ? 0.f : -m * LOG2E_;
+  float l = 0.f, l1 = 0.f;
+#pragma unroll
+  for (int i = 0; i < WORDS; ++i) {
+    l += beam_ex2(fmaf(beam_value_of<T>(x[i], 0), LOG2E_, under));
+    if (PW == 2) l1 += beam_ex2(fmaf(beam_value_of<T>(x[i], 1), LOG2E_, under));
+  }
+  l += l1;
+  // ---- the k best ---------------------------------------------------------------------------------------------------------------
+  const int share = p.K > 16 ? 2 : 4;       // threads of a group
+  float top = own;
+  for (int o = 1; o < share; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const int groups = BEAM_THREADS / share;
+  if (tid % share == 0) sm.group[tid / share] = top;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float om = __shfl_xor_sync(0xffffffffu, m, o), ol = __shfl_xor_sync(0xffffffffu, l, o), to = fmaxf(m, om), z = to == -INFINITY ? 0.f : to;
+    l = l * beam_ex2((m - z) * LOG2E_) + ol * beam_ex2((om - z) * LOG2E_);
+    m = to;
+  }
+  if (lane == 0) sm.red_m[warp] = m, sm.red_l[warp] = l;
+  __syncthreads();
+  if (tid < groups) {                       // the k-th largest of the groups' maxima
+    const float v = sm.group[tid];
+    int rank = 0;
+    for (int i = 0; i < groups; i += 4) {
+      const float4 o = *reinterpret_cast<const float4*>(&sm.group[i]);
+      rank += (o.x > v || (o.x == v && i < tid)) + (o.y > v || (o.y == v && i + 1 < tid)) + (o.z > v || (o.z == v && i + 2 < tid)) +
+              (o.w > v || (o.w == v && i + 3 < tid));
+    }
+    if (rank == p.K - 1) sm.border = v;
+  }
+  if (tid == BEAM_THREADS - 1) {            // (max, sum) of the chunk
+    m = sm.red_m[0], l = sm.red_l[0];
+    for (int w = 1; w < BEAM_WARPS; ++w) {
+      const float to = fmaxf(m, sm.red_m[w]), z = to == -INFINITY ? 0.f : to;
+      l = l * beam_ex2((m - z) * LOG2E_) + sm.red_l[w] * beam_ex2((sm.red_m[w] - z) * LOG2E_);
+      m = to;
+    }
+    p.ml[(size_t)row * p.chunks + chunk] = make_float2(m, l);
+  }
+  __syncthreads();
+  const float border = sm.border;
+  if (own >= border && own > -INFINITY) {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i)
+#pragma unroll
+      for (int j = 0; j < PW; ++j) {
+        const float v = beam_value_of<T>(x[i], j);
+        if (v >= border && v > -INFINITY) {
+          const int at = atomicAdd(&sm.count, 1);
+          if (at < BEAM_CAP) sm.keys[at] = beam_key(v, index(i) + j);
+        }
+      }
+  }
+  __syncthreads();
+  unsigned long long* keys = p.keys + ((size_t)row * p.chunks + chunk) * p.K;
+  const int n = sm.count;
+  if (n <= BEAM_CAP) {
+    for (int i = tid; i < n; i += BEAM_THREADS) {
+      const unsigned long long key = sm.keys[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += sm.keys[j] > key;
+      if (rank < p.K) keys[rank] = key;
+    }
+    for (int k = n + tid; k < p.K; k += BEAM_THREADS) keys[k] = 0;
+  } else {                                  // one a round: the thread that gave it looks for its next
+    const T* src = reinterpret_cast<const T*>(base);   // (read again: registers have no index)
+    auto next_best = [&](unsigned long long below) {
+      unsigned long long best = 0;
+#pragma unroll 1
+      for (int i = 0; i < BEAM_VECTORS; ++i) {
+        const int at = index(4 * i);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          const bool in = i * BEAM_THREADS + tid < p.granules && at + j >= 0 && at + j < p.V;
+          const float v = in ? (float)src[at + j] : -INFINITY;
+          const unsigned long long key = v > -INFINITY ? beam_key(v, at + j) : 0;   // (a NaN is none)
+          if (key < below && key > best) best = key;
+        }
+      }
+      return best;
+    };
+    unsigned long long mine = ~0ull;
+    bool stale = true;
+    for (int k = 0; k < p.K; ++k) {
+      if (stale) mine = next_best(mine);
+      unsigned long long best = mine;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+      if (lane == 0) sm.red[warp] = best;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < BEAM_WARPS; ++w) best = max(best, sm.red[w]);
+      if (tid == 0) keys[k] = best;
+      stale = best && best == mine;
+      __syncthreads();
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {                           // releases the CTA's stores (ordered before by the barrier), acquires the others'
+    int before;
+    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.counters + b) : "memory");
+    sm.last = before == rows * p.chunks - 1;
+    if (sm.last) p.counters[b] = 0;
+  }
+  __syncthreads();
+  if (sm.last) beam_merge(p, sm, b, r0, rows);
 }
 
 }  // namespace qk
