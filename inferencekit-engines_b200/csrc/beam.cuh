@@ -7,12 +7,12 @@
 //  * The order inside a row is the order of its logits, which needs no logsumexp: a chunk leaves (max, sum) and its k best keys,
 //    value and ~index, in order. The CTA that completes a request's count merges the chunks' lists: row sums and scores in 64
 //    bits there, so that two beams' candidates are ordered by more than fp32 shows.
-//  * k best of many, twice: the k-th largest of some of them (the largest value of each of 64 or 128 groups; the heads of lists)
-//    is a lower bound of the k-th largest of all, which few more than k reach; those are ranked by counting. Where too many
-//    reach it (ties, sorted rows), k rounds of a maximum take their place.
+//  * k best of many, twice: the k-th largest of some of them (the largest value of each thread or group of threads) is a lower
+//    bound of the k-th largest of all, which few more than k reach; those are ranked by counting. Where too many reach it (ties,
+//    sorted rows), k rounds of a maximum take their place.
 //  * exp in fp32, a thread's 64 terms under its own maximum; a row's sum is off by some 2^-22 of itself.
 #pragma once
-#include "paged.cuh"
+#include "attention_few.cuh"   // LOG2E
 
 namespace qk {
 
@@ -80,73 +80,106 @@ struct BeamSmem {
       unsigned at[BEAM_CAP];
     } c;
   };
-  float group[128];
-  double heads[BEAM_THREADS];
+  float top[BEAM_THREADS];                 // the groups' largest
+  unsigned short lists[BEAM_CAP];          // the merge: lists that can hold one of the k best
   unsigned long long red[BEAM_WARPS];
   float red_m[BEAM_WARPS], red_l[BEAM_WARPS];
   double lse[BEAM_MAX_ROWS];
   BeamBest red_c[BEAM_WARPS];
   uint8_t head[BEAM_MAX_LISTS];
   float border;
-  double border_s;
-  int b, last, count;
+  int b, r0, rows, last, count, n_lists;
 };
+
+// sm.border: the k-th largest of the first n of sm.top (a multiple of 4, at most the threads), -inf where there are fewer. Two barriers.
+__device__ __forceinline__ void beam_border(BeamSmem& sm, int n, int k) {
+  const int tid = threadIdx.x;
+  if (tid == 0) sm.border = -INFINITY;
+  __syncthreads();
+  if (tid < n) {
+    const float v = sm.top[tid];
+    int rank = 0;
+#pragma unroll 4
+    for (int i = 0; i < n; i += 4) {
+      const float4 o = *reinterpret_cast<const float4*>(&sm.top[i]);
+      rank += (o.x > v || (o.x == v && i < tid)) + (o.y > v || (o.y == v && i + 1 < tid)) + (o.z > v || (o.z == v && i + 2 < tid)) +
+              (o.w > v || (o.w == v && i + 3 < tid));
+    }
+    if (rank == k - 1) sm.border = v;
+  }
+  __syncthreads();
+}
 
 // The merge of a request's lists, by the CTA that completed it.
 __device__ __forceinline__ void beam_merge(const BeamParams& p, BeamSmem& sm, int b, int r0, int rows) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) sm.count = sm.n_lists = 0;
   for (int r = warp; r < rows; r += BEAM_WARPS) {
     const float2* ml = p.ml + (size_t)(r0 + r) * p.chunks;
+    const float s = __ldg(p.scores + r0 + r);
     float M = -INFINITY;
-    for (int c = lane; c < p.chunks; c += 32) M = fmaxf(M, __ldcg(&ml[c].x));
-    M = warp_max(M);
     double L = 0.;
-    for (int c = lane; c < p.chunks; c += 32) {
-      const float2 v = __ldcg(ml + c);
-      if (v.x != -INFINITY) L += (double)v.y * exp((double)v.x - (double)M);
+    for (int c0 = 0; c0 < p.chunks; c0 += 32) {
+      const float2 v = c0 + lane < p.chunks ? __ldcg(ml + c0 + lane) : make_float2(-INFINITY, 0.f);
+      const float to = fmaxf(M, warp_max(v.x)), z = to == -INFINITY ? 0.f : to;
+      L = L * beam_ex2((M - z) * LOG2E) + (double)v.y * beam_ex2((v.x - z) * LOG2E);
+      M = to;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    const float s = __ldg(p.scores + r0 + r);
     const bool none = s == -INFINITY || (L == 0. && M == -INFINITY), wrong = !none && !(fabsf(s) < INFINITY && L > 0. && L < 1e300);
     if (lane == 0) {
       if (wrong) atomicOr(&g_dev_error, DEVERR_BAD_STATE);   // a NaN or +infinity among its logits, or as its score
       sm.lse[r] = none || wrong ? INFINITY : (double)M + log(L);
     }
   }
+  __syncthreads();
   const int lists = rows * p.chunks;
-  if (tid == 0) sm.count = 0, sm.border_s = -INFINITY;
-  __syncthreads();
-  auto get = [&](int list, int i) {         // candidate i of a list
-    BeamBest c = {-INFINITY, 0xffffffffu, -1};
+  auto key_of = [&](int list, int i) { return __ldcg(p.keys + ((size_t)r0 * p.chunks + list) * p.K + i); };
+  auto score_of = [&](int list, unsigned long long key) {   // -inf: none
     const int r = list / p.chunks;
-    const unsigned long long key = i < p.K && sm.lse[r] != INFINITY ? __ldcg(p.keys + ((size_t)r0 * p.chunks + list) * p.K + i) : 0;
-    if (key) c = {(double)__ldg(p.scores + r0 + r) + ((double)beam_value(key) - sm.lse[r]), (unsigned)r * (unsigned)p.V + (unsigned)beam_index(key), list};
-    return c;
+    return key && sm.lse[r] != INFINITY ? (double)__ldg(p.scores + r0 + r) + ((double)beam_value(key) - sm.lse[r]) : -INFINITY;
   };
-  // a lower bound of the k-th best: the k-th best of the first `depth` of every list, or of the best heads of each thread's lists
-  const int depth = lists >= p.K ? 1 : (p.K + lists - 1) / lists, n_set = min(lists * depth, BEAM_THREADS);
-  double mine = -INFINITY;
-  if (depth == 1) {
-    for (int i = tid; i < lists; i += BEAM_THREADS) mine = fmax(mine, get(i, 0).s);
-  } else if (tid < n_set) {
-    mine = get(tid / depth, tid % depth).s;
-  }
-  sm.heads[tid] = mine;
-  __syncthreads();
-  if (tid < n_set) {
-    int rank = 0;
-    for (int i = 0; i < n_set; ++i) rank += sm.heads[i] > mine || (sm.heads[i] == mine && i < tid);
-    if (rank == p.K - 1) sm.border_s = mine;
-  }
-  __syncthreads();
-  for (int i = tid; i < lists; i += BEAM_THREADS)
-    for (int k = 0;; ++k) {
-      const BeamBest c = get(i, k);
-      if (c.list < 0 || c.s < sm.border_s) break;
-      const int at = atomicAdd(&sm.count, 1);
-      if (at < BEAM_CAP) sm.c.score[at] = c.s, sm.c.at[at] = c.at;
+  auto place_of = [&](int list, unsigned long long key) { return (unsigned)(list / p.chunks) * (unsigned)p.V + (unsigned)beam_index(key); };
+  // (scores rounded down to fp32 for the borders: what reaches a border of theirs is a lower bound too)
+  // ---- which lists: with many, those whose first candidate is among the k best firsts (or equal to the last of them) --------------
+  const bool few = lists * p.K <= BEAM_CAP * 8 || lists <= p.K;
+  if (!few) {
+    float top = -INFINITY;
+    for (int i = tid; i < lists; i += BEAM_THREADS) top = fmaxf(top, __double2float_rd(score_of(i, key_of(i, 0))));
+    sm.top[tid] = top;
+    beam_border(sm, BEAM_THREADS, p.K);
+    for (int i = tid; i < lists; i += BEAM_THREADS) {
+      const float s = __double2float_rd(score_of(i, key_of(i, 0)));
+      if (s < sm.border || s == -INFINITY) continue;
+      const int at = atomicAdd(&sm.n_lists, 1);
+      if (at < BEAM_CAP) sm.lists[at] = (unsigned short)i;
     }
+    __syncthreads();
+  }
+  const int n_lists = few ? lists : sm.n_lists;
+  if (n_lists <= BEAM_CAP) {
+    // ---- their candidates, by depth, so that a list's go to different threads ------------------------------------------------------
+    auto each = [&](auto f) {
+#pragma unroll 4
+      for (int c = tid; c < n_lists * p.K; c += BEAM_THREADS) {
+        const int i = c / n_lists, list = few ? c - i * n_lists : sm.lists[c - i * n_lists];
+        f(list, key_of(list, i));
+      }
+    };
+    float top = -INFINITY;
+    each([&](int list, unsigned long long key) { top = fmaxf(top, __double2float_rd(score_of(list, key))); });
+    sm.top[tid] = top;
+    beam_border(sm, BEAM_THREADS, p.K);
+    each([&](int list, unsigned long long key) {
+      const double s = score_of(list, key);
+      if (s == -INFINITY || __double2float_rd(s) < sm.border) return;
+      const int at = atomicAdd(&sm.count, 1);
+      if (at < BEAM_CAP) sm.c.score[at] = s, sm.c.at[at] = place_of(list, key);
+    });
+  } else if (tid == 0) {
+    sm.count = BEAM_CAP + 1;
+  }
   __syncthreads();
   const size_t out = (size_t)b * p.K;
   auto write = [&](int k, bool any, double s, unsigned at) {
@@ -171,8 +204,10 @@ __device__ __forceinline__ void beam_merge(const BeamParams& p, BeamSmem& sm, in
   auto pick = [&]() {                       // (a thread's own lists)
     BeamBest best = {-INFINITY, 0xffffffffu, -1};
     for (int i = tid; i < lists; i += BEAM_THREADS) {
-      const BeamBest c = get(i, sm.head[i]);
-      if (c.list >= 0 && (best.list < 0 || beam_better(c.s, c.at, best.s, best.at))) best = c;
+      if (sm.head[i] >= p.K) continue;
+      const unsigned long long key = key_of(i, sm.head[i]);
+      const BeamBest c = {score_of(i, key), place_of(i, key), i};
+      if (c.s > -INFINITY && (best.list < 0 || beam_better(c.s, c.at, best.s, best.at))) best = c;
     }
     return best;
   };
@@ -216,6 +251,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4) beam_select_kernel(const __gr
   const uint4* vec = reinterpret_cast<const uint4*>(base & ~(uintptr_t)15);
   const int g0 = chunk * p.granules;
   constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;   // -inf
+  const float beam = row < p.R ? __ldg(p.scores + row) : 0.f;
   uint32_t x[WORDS];
   auto index = [&](int word) { return (g0 + (word / 4) * BEAM_THREADS + tid) * PER - lead + (word % 4) * PW; };   // of its first value
 #pragma unroll
@@ -242,13 +278,13 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4) beam_select_kernel(const __gr
     x[4 * i] = w.x, x[4 * i + 1] = w.y, x[4 * i + 2] = w.z, x[4 * i + 3] = w.w;
   }
   // ---- the rows' requests: all or nothing, so that every CTA comes to the same count ------------------------------------------
-  if (tid == 0) sm.b = -1, sm.count = 0, sm.border = -INFINITY;
+  if (tid == 0) sm.b = -1, sm.count = 0;
   __syncthreads();
   bool bad = false;
   for (int b = tid; b < p.B; b += BEAM_THREADS) {
     const int lo = __ldg(p.cu + b), hi = __ldg(p.cu + b + 1);
     bad |= lo < 0 || hi < lo || hi > p.R || hi - lo > BEAM_MAX_ROWS;
-    if (lo <= row && row < hi) sm.b = b;
+    if (lo <= row && row < hi) sm.b = b, sm.r0 = lo, sm.rows = hi - lo;
     if (lo == hi && b == (int)blockIdx.x)   // (the grid has a CTA for each request) without beams
       for (int i = 0; i < p.K; ++i) {
         const size_t at = (size_t)b * p.K + i;
@@ -259,10 +295,9 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4) beam_select_kernel(const __gr
     if (tid == 0) atomicOr(&g_dev_error, DEVERR_BAD_STATE);
     return;
   }
-  const int b = sm.b;
+  const int b = sm.b, r0 = sm.r0, rows = sm.rows;
   if (b < 0 || row >= p.R) return;
-  const int r0 = __ldg(p.cu + b), rows = __ldg(p.cu + b + 1) - r0;
-  if (__ldg(p.scores + row) == -INFINITY) {   // a beam that is none: whatever its logits are
+  if (beam == -INFINITY) {   // a beam that is none: whatever its logits are
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) x[i] = NONE;
   }
@@ -273,62 +308,51 @@ __global__ void __launch_bounds__(BEAM_THREADS, 4) beam_select_kernel(const __gr
   for (int i = 0; i < WORDS; ++i)
 #pragma unroll
     for (int j = 0; j < PW; ++j) m = fmaxf(m, beam_value_of<T>(x[i], j));
-  const float own = m;
-  constexpr float LOG2E_ = 1.4426950408889634f;
-  const float under = m == -INFINITY ? 0.f : -m * LOG2E_;
+  const float under = m == -INFINITY ? 0.f : -m * LOG2E;
   float l = 0.f, l1 = 0.f;
 #pragma unroll
   for (int i = 0; i < WORDS; ++i) {
-    l += beam_ex2(fmaf(beam_value_of<T>(x[i], 0), LOG2E_, under));
-    if (PW == 2) l1 += beam_ex2(fmaf(beam_value_of<T>(x[i], 1), LOG2E_, under));
+    l += beam_ex2(fmaf(beam_value_of<T>(x[i], 0), LOG2E, under));
+    if (PW == 2) l1 += beam_ex2(fmaf(beam_value_of<T>(x[i], 1), LOG2E, under));
   }
   l += l1;
   // ---- the k best ---------------------------------------------------------------------------------------------------------------
   const int share = p.K > 16 ? 2 : 4;       // threads of a group
-  float top = own;
+  float top = m;
   for (int o = 1; o < share; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const int groups = BEAM_THREADS / share;
-  if (tid % share == 0) sm.group[tid / share] = top;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float om = __shfl_xor_sync(0xffffffffu, m, o), ol = __shfl_xor_sync(0xffffffffu, l, o), to = fmaxf(m, om), z = to == -INFINITY ? 0.f : to;
-    l = l * beam_ex2((m - z) * LOG2E_) + ol * beam_ex2((om - z) * LOG2E_);
-    m = to;
+  if (tid % share == 0) sm.top[tid / share] = top;
+  float M = warp_max(m);                    // the warp's sum under its maximum
+  l = warp_sum(M == -INFINITY ? 0.f : l * beam_ex2((m - M) * LOG2E));
+  if (lane == 0) sm.red_m[warp] = M, sm.red_l[warp] = l;
+  beam_border(sm, BEAM_THREADS / share, p.K);
+  if (warp == BEAM_WARPS - 1) {             // (max, sum) of the chunk
+    const float wm = lane < BEAM_WARPS ? sm.red_m[lane] : -INFINITY;
+    M = warp_max(wm);
+    l = warp_sum(wm == -INFINITY ? 0.f : sm.red_l[lane] * beam_ex2((wm - M) * LOG2E));
+    if (lane == 0) p.ml[(size_t)row * p.chunks + chunk] = make_float2(M, l);
   }
-  if (lane == 0) sm.red_m[warp] = m, sm.red_l[warp] = l;
-  __syncthreads();
-  if (tid < groups) {                       // the k-th largest of the groups' maxima
-    const float v = sm.group[tid];
-    int rank = 0;
-    for (int i = 0; i < groups; i += 4) {
-      const float4 o = *reinterpret_cast<const float4*>(&sm.group[i]);
-      rank += (o.x > v || (o.x == v && i < tid)) + (o.y > v || (o.y == v && i + 1 < tid)) + (o.z > v || (o.z == v && i + 2 < tid)) +
-              (o.w > v || (o.w == v && i + 3 < tid));
-    }
-    if (rank == p.K - 1) sm.border = v;
-  }
-  if (tid == BEAM_THREADS - 1) {            // (max, sum) of the chunk
-    m = sm.red_m[0], l = sm.red_l[0];
-    for (int w = 1; w < BEAM_WARPS; ++w) {
-      const float to = fmaxf(m, sm.red_m[w]), z = to == -INFINITY ? 0.f : to;
-      l = l * beam_ex2((m - z) * LOG2E_) + sm.red_l[w] * beam_ex2((sm.red_m[w] - z) * LOG2E_);
-      m = to;
-    }
-    p.ml[(size_t)row * p.chunks + chunk] = make_float2(m, l);
-  }
-  __syncthreads();
   const float border = sm.border;
-  if (own >= border && own > -INFINITY) {
+  if (m >= border && m > -INFINITY) {
+    uint32_t hits = 0;                      // words with a value that reaches the border
 #pragma unroll
-    for (int i = 0; i < WORDS; ++i)
+    for (int i = 0; i < WORDS; ++i) {
+      const float v0 = beam_value_of<T>(x[i], 0), v1 = PW == 2 ? beam_value_of<T>(x[i], 1) : v0;
+      hits |= (fmaxf(v0, v1) >= border ? 1u : 0u) << i;
+    }
+    const T* src = reinterpret_cast<const T*>(base);   // (few, and read again: registers have no index)
+    while (hits) {
+      const int i = __ffs(hits) - 1;
+      hits &= hits - 1;
+      const int first = index(i);
 #pragma unroll
       for (int j = 0; j < PW; ++j) {
-        const float v = beam_value_of<T>(x[i], j);
+        const float v = first + j >= 0 && first + j < p.V ? (float)src[first + j] : -INFINITY;
         if (v >= border && v > -INFINITY) {
           const int at = atomicAdd(&sm.count, 1);
-          if (at < BEAM_CAP) sm.keys[at] = beam_key(v, index(i) + j);
+          if (at < BEAM_CAP) sm.keys[at] = beam_key(v, first + j);
         }
       }
+    }
   }
   __syncthreads();
   unsigned long long* keys = p.keys + ((size_t)row * p.chunks + chunk) * p.K;
