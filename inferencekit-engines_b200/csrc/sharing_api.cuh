@@ -146,11 +146,10 @@ int qk_paged_fork(const qk_paged_fork_t* args, qk_stream_t stream) {
   return launch(paged_copy_kernel, dim3(p.N, p.parts), dim3(256), 0, st, p);
 }
 
-// Counters of every request a call may have, then the chunks' sums and lists.
-constexpr long long BEAM_COUNTERS = 4ll * PLAN_MAX_BATCH;
+// The chunks' sums and lists; as many chunks as a call of these sizes may make, of rows of either type.
 long long qk_beam_workspace_bytes(long long rows, long long vocab, long long k) {
   if (rows < 0 || rows > 65536 || vocab < 1 || vocab > BEAM_MAX_VOCAB || k < 1 || k > BEAM_MAX_K) return -1;
-  return BEAM_COUNTERS + rows * beam_chunks((int)vocab, 4) * (8 * k + 8);   // (fp32 rows have the more chunks)
+  return std::max(256ll, rows * beam_min_chunks((int)vocab, 4) * (8 * k + 8));
 }
 
 int qk_beam_select(const qk_beam_select_t* args, qk_stream_t stream) {
@@ -172,16 +171,18 @@ int qk_beam_select(const qk_beam_select_t* args, qk_stream_t stream) {
   p.logits = a.logits, p.scores = a.scores, p.cu = a.cu_rows;
   p.out_scores = a.out_scores, p.out_parents = a.out_parents, p.out_tokens = a.out_tokens;
   p.B = (int)a.batch, p.R = (int)a.rows, p.V = (int)a.vocab, p.K = (int)a.k;
-  p.chunks = beam_chunks(p.V, size);
-  const int per = 16 / size, granules = (p.V + per - 1 + per - 1) / per;
-  p.granules = (granules + p.chunks - 1) / p.chunks;
-  char* ws = static_cast<char*>(a.workspace);
-  p.counters = reinterpret_cast<int*>(ws);
-  p.keys = reinterpret_cast<unsigned long long*>(ws + BEAM_COUNTERS);
-  p.ml = reinterpret_cast<float2*>(p.keys + (size_t)p.R * p.chunks * p.K);
-  const long long grid = std::max((long long)p.R * p.chunks, (long long)p.B);
-  return launch(a.fp32 ? beam_select_kernel<float> : beam_select_kernel<bf16>, dim3((unsigned)grid), dim3(BEAM_THREADS), 0,
-                static_cast<cudaStream_t>(stream), p);
+  p.chunks = beam_min_chunks(p.V, size);
+  p.granules = (beam_granules(p.V, size) + p.chunks - 1) / p.chunks;
+  const size_t all = (size_t)p.R * p.chunks;
+  p.grid = (int)std::max((size_t)1, std::min(all, (size_t)device_sms() * 2));
+  p.keys = static_cast<unsigned long long*>(a.workspace);
+  p.ml = reinterpret_cast<float2*>(p.keys + all * p.K);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (all)
+    if (int r = launch(a.fp32 ? beam_chunk_kernel<float> : beam_chunk_kernel<bf16>, dim3(p.grid), dim3(BEAM_THREADS), 0, st, p)) return r;
+  const int lists = (int)std::min((size_t)BEAM_MAX_USED, (size_t)std::min(p.R, BEAM_MAX_ROWS) * p.chunks), smem = (int)sizeof(BeamMergeSmem) + lists * (p.K + 1) * 4;
+  if (int r = ensure_smem((const void*)beam_merge_kernel, smem)) return r;
+  return launch_as(all || g_pdl, beam_merge_kernel, dim3(p.B), dim3(BEAM_THREADS), smem, st, p);
 }
 
 long long qk_shared_attention_workspace_bytes(long long rows, long long n_q) {

@@ -375,11 +375,19 @@ def test_select_strides_and_alignment():
 
 
 def test_select_offsets_that_are_none():
-    logits, scores = torch.zeros(4, 100, device=DEV), torch.zeros(4, device=DEV)
-    for cu in ([0, 5], [2, 1, 4], [-1, 4]):
+    """A request whose rows are not the call's is empty and sets the error word; the others are as they would be alone."""
+    g = torch.Generator(device=DEV).manual_seed(4)
+    logits, scores = torch.randn(4, 100, generator=g, device=DEV), torch.zeros(4, device=DEV)
+    for cu, bad in (([0, 5], {0}), ([2, 1, 4], {0}), ([-1, 4], {0}), ([0, 4, 300], {1}), ([0, 2, 4], set())):
         err, got = select(logits, scores, cu, 3)
-        assert err == 2 and all(v in (7, -1) for row in got[1] for v in row)
-    assert select(logits, scores, [0, 4], 3)[0] == 0   # and the workspace is as it was
+        assert err == (2 if bad else 0)
+        for b in range(len(cu) - 1):
+            one = [[t[b]] for t in got]
+            if b in bad:
+                assert one == [[[-math.inf] * 3], [[-1] * 3], [[-1] * 3]]
+            else:
+                lo, hi = cu[b], cu[b + 1]
+                check_select(logits[lo:hi], scores[lo:hi], [0, hi - lo], 3, (one[0], [[v - lo for v in one[1][0]]], one[2]))
 
 
 # ---- shared_attention --------------------------------------------------------------------------------------
