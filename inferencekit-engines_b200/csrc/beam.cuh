@@ -45,9 +45,11 @@ struct BeamParams {
   long long row_stride;
   int B, R, V, K, chunks, granules, grid;   // granules: 16-byte vectors of a chunk; grid: of the chunks' kernel
 };
-// CTA c has the chunks from beam_first(c) to beam_first(c + 1).
-__device__ __forceinline__ int beam_first(const BeamParams& p, int c) { return (int)((long long)c * p.R * p.chunks / p.grid); }
-__device__ __forceinline__ int beam_owner(const BeamParams& p, int u) { return owner_of(u, (long long)p.R * p.chunks, p.grid); }
+// CTA c has the chunks from beam_first(c) to beam_first(c + 1). (At most 2^23 chunks, 2^9 CTAs.)
+__device__ __forceinline__ int beam_first(const BeamParams& p, int c) { return (int)((unsigned)c * (unsigned)(p.R * p.chunks) / (unsigned)p.grid); }
+__device__ __forceinline__ int beam_owner(const BeamParams& p, int u) {
+  return (int)(((unsigned)(u + 1) * (unsigned)p.grid - 1) / (unsigned)(p.R * p.chunks));
+}
 
 // A value's place in the order: larger values first, then lower indices; 0 is less than every one of them.
 __device__ __forceinline__ unsigned long long beam_key(float x, int v) { return argmax_key(x + 0.f, v); }   // (-0 is 0)
@@ -212,16 +214,21 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) beam_chunk_kernel(const __gri
     // (equal values of later chunks have higher indices than k that are kept already)
     auto reaches = [&](float v) { return begins ? v >= border && v > -INFINITY : v > border; };
     if (reaches(top)) {
-      const T* src = reinterpret_cast<const T*>(c.base);   // (few, and read again: registers have no index)
       uint32_t hits = 0;
 #pragma unroll
       for (int i = 0; i < BEAM_VECTORS; ++i) hits |= (reaches(vm[i]) ? 1u : 0u) << i;
       while (hits) {
-        const int first = index(c, 4 * (__ffs(hits) - 1));
+        const int i = __ffs(hits) - 1, first = index(c, 4 * i);
         hits &= hits - 1;
+        uint32_t w[4];                      // (registers have no index)
+#pragma unroll
+        for (int k = 0; k < BEAM_VECTORS; ++k)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (k == 0 || k == i) w[j] = x[4 * k + j];
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-          const float v = first + j >= 0 && first + j < p.V ? (float)src[first + j] : -INFINITY;
+          const float v = sizeof(T) == 4 ? __uint_as_float(w[j & 3]) : j & 1 ? bf16hi(w[j / 2 & 3]) : bf16lo(w[j / 2 & 3]);
           if (!reaches(v)) continue;
           const int at = atomicAdd(&count, 1);
           if (at < BEAM_CAP) cand[at] = beam_key(v, first + j);
@@ -310,9 +317,11 @@ struct BeamMergeSmem {
   unsigned cand_at[BEAM_CAP];
   BeamBorder border;
   double off[BEAM_MAX_ROWS];               // score - logsumexp; -inf: the row has nothing
+  float2 ml[BEAM_MAX_USED];
   BeamBest red[BEAM_WARPS];
   int list_at[BEAM_MAX_ROWS + 4];          // lists of the rows before
-  unsigned short of[BEAM_MAX_USED];        // lists that can hold one of the k best
+  int chunk[BEAM_MAX_USED];                // of the lists that can hold one of the k best: the first chunk, the row
+  uint8_t row[BEAM_MAX_USED];
   uint8_t head[BEAM_MAX_LISTS];
   int count, n_of, reach;
 };
@@ -320,19 +329,10 @@ struct BeamMergeSmem {
 __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const __grid_constant__ BeamParams p) {
   extern __shared__ __align__(16) uint8_t beam_smem[];
   BeamMergeSmem& sm = *reinterpret_cast<BeamMergeSmem*>(beam_smem);
-  float* score = reinterpret_cast<float*>(beam_smem + sizeof(BeamMergeSmem));   // [lists][K + 1]: the candidates', rounded
-  auto &cand_s = sm.cand_s;
-  auto &cand_at = sm.cand_at;
-  auto &off = sm.off;
-  auto &list_at = sm.list_at;
-  auto &of = sm.of;
-  auto &red = sm.red;
-  auto &head = sm.head;
-  int &count = sm.count, &n_of = sm.n_of, &reach = sm.reach;
+  float* value = reinterpret_cast<float*>(beam_smem + sizeof(BeamMergeSmem));   // [lists][K]: the candidates' logits, -inf: none
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.x;
-  if (tid == 0) count = n_of = reach = 0;
-  grid_dep_wait();
-  grid_dep_launch();
+  if (tid == 0) sm.count = sm.n_of = sm.reach = 0;
+  if (p.R * p.chunks == 0) grid_dep_wait();   // (else the chunks' kernel waited for what precedes it before it let this one start)
   const int r0 = __ldg(p.cu + b);
   int rows = __ldg(p.cu + b + 1) - r0;
   if (r0 < 0 || rows < 0 || rows > BEAM_MAX_ROWS || r0 > p.R - rows) {
@@ -357,116 +357,141 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const __grid_c
         const int v = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += v;
       }
-      if (r + lane < rows) list_at[r + lane] = before + incl - n;
+      if (r + lane < rows) sm.list_at[r + lane] = before + incl - n;
       before += __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (lane == 0) list_at[rows] = before;
+    if (lane == 0) sm.list_at[rows] = before;
   }
+  const float score = tid < rows ? __ldg(p.scores + r0 + tid) : -INFINITY;   // of row tid
   __syncthreads();
-  const int lists = list_at[rows];
+  const int lists = sm.list_at[rows];
   auto row_of = [&](int list) {
     int lo = 0, hi = rows;                  // list_at[lo] <= list
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2;
-      if (list_at[mid] <= list) lo = mid;
+      if (sm.list_at[mid] <= list) lo = mid;
       else hi = mid;
     }
     return lo;
   };
   auto chunk_of = [&](int r, int list) {    // the first chunk of a list of row r
-    const int u = (r0 + r) * p.chunks, i = list - list_at[r];
+    const int u = (r0 + r) * p.chunks, i = list - sm.list_at[r];
     return i == 0 ? u : beam_first(p, beam_owner(p, u) + i);
   };
-  for (int r = warp; r < rows; r += BEAM_WARPS) {
-    const float s = __ldg(p.scores + r0 + r);
+  const bool few = lists <= BEAM_MAX_USED;
+  if (few && tid < lists) {
+    const int r = row_of(tid);
+    sm.row[tid] = (uint8_t)r;
+    sm.chunk[tid] = chunk_of(r, tid);
+  }
+  __syncthreads();
+  grid_dep_wait();                          // the chunks' lists are there
+  grid_dep_launch();
+  // ---- the lists' values on their way, the rows' sums ------------------------------------------------------------------------------
+  auto key_at = [&](int chunk, int i) { return __ldcg(p.keys + (size_t)chunk * p.K + i); };
+  auto fetch = [&](int n) {
+#pragma unroll 4
+    for (int at = warp; at < n; at += BEAM_WARPS)
+#pragma unroll
+      for (int i = lane; i < BEAM_MAX_K; i += 32)
+        if (i < p.K) {
+          const unsigned long long key = key_at(sm.chunk[at], i);
+          value[at * p.K + i] = key ? beam_value(key) : -INFINITY;
+        }
+  };
+  if (few) {
+    if (tid < lists) sm.ml[tid] = __ldcg(p.ml + sm.chunk[tid]);
+    fetch(lists);
+  }
+  __syncthreads();
+  if (tid < rows) {
     float M = -INFINITY;
     double L = 0.;
-    for (int i0 = list_at[r]; i0 < list_at[r + 1]; i0 += 32) {
-      const float2 v = i0 + lane < list_at[r + 1] ? __ldcg(p.ml + chunk_of(r, i0 + lane)) : make_float2(-INFINITY, 0.f);
-      const float to = fmaxf(M, warp_max(v.x)), z = to == -INFINITY ? 0.f : to;
+    for (int i = sm.list_at[tid]; i < sm.list_at[tid + 1]; ++i) {
+      const float2 v = few ? sm.ml[i] : __ldcg(p.ml + chunk_of(tid, i));
+      const float to = fmaxf(M, v.x), z = to == -INFINITY ? 0.f : to;
       L = L * ex2((M - z) * LOG2E) + (double)v.y * (v.x == z ? 1.f : ex2((v.x - z) * LOG2E));
       M = to;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    const bool none = s == -INFINITY || (L == 0. && M == -INFINITY), wrong = !none && !(fabsf(s) < INFINITY && L > 0. && L < 1e300);
-    if (lane == 0) {
-      if (wrong) atomicOr(&g_dev_error, DEVERR_BAD_STATE);   // a NaN or +infinity among its logits, or as its score
-      off[r] = none || wrong ? -INFINITY : (double)s - ((double)M + log(L));
-      if (!none && !wrong) atomicMax(&reach, __float_as_int(fabsf((float)off[r])));
-    }
+    const bool none = score == -INFINITY || (L == 0. && M == -INFINITY), wrong = !none && !(fabsf(score) < INFINITY && L > 0. && L < 1e300);
+    if (wrong) atomicOr(&g_dev_error, DEVERR_BAD_STATE);   // a NaN or +infinity among its logits, or as its score
+    const double off = none || wrong ? -INFINITY : (double)score - ((double)M + log(L));
+    sm.off[tid] = off;
+    if (off != -INFINITY) atomicMax(&sm.reach, __float_as_int(fabsf((float)off)));
   }
   __syncthreads();
-  auto key_at = [&](int r, int list, int i) { return __ldcg(p.keys + (size_t)chunk_of(r, list) * p.K + i); };
   // Borders are found among fp32 scores, each within 2^-23 of |score| + |off| of the 64-bit one; what may be among the k best reaches
   // the border less twice that.
-  auto score32 = [&](int r, unsigned long long key) { return key ? beam_value(key) + (float)off[r] : -INFINITY; };
-  auto lowered = [&](float border) { return border == -INFINITY ? border : border - 0x1p-21f * (fabsf(border) + __int_as_float(reach)); };
+  auto lowered = [&](float border) { return border == -INFINITY ? border : border - 0x1p-21f * (fabsf(border) + __int_as_float(sm.reach)); };
   // ---- which lists: with many, those whose first candidate can be among the k best firsts -----------------------------------------
-  const bool few = lists <= BEAM_MAX_USED;
   if (!few) {
-    auto first = [&](int list) {
-      const int r = row_of(list);
-      return score32(r, key_at(r, list, 0));
+    auto first = [&](int list, int& r, int& chunk) {
+      r = row_of(list);
+      chunk = chunk_of(r, list);
+      const unsigned long long key = key_at(chunk, 0);
+      return key ? beam_value(key) + (float)sm.off[r] : -INFINITY;
     };
+    int r, chunk;
     float top = -INFINITY;
-    for (int i = tid; i < lists; i += BEAM_THREADS) top = fmaxf(top, first(i));
+    for (int i = tid; i < lists; i += BEAM_THREADS) top = fmaxf(top, first(i, r, chunk));
     const float border = lowered(beam_border(sm.border, top, p.K));
     for (int i = tid; i < lists; i += BEAM_THREADS) {
-      const float s = first(i);
+      const float s = first(i, r, chunk);
       if (!(s >= border && s > -INFINITY)) continue;
-      const int at = atomicAdd(&n_of, 1);
-      if (at < BEAM_MAX_USED) of[at] = (unsigned short)i;
+      const int at = atomicAdd(&sm.n_of, 1);
+      if (at < BEAM_MAX_USED) sm.row[at] = (uint8_t)r, sm.chunk[at] = chunk;
     }
+    __syncthreads();
+    if (sm.n_of <= BEAM_MAX_USED) fetch(sm.n_of);
     __syncthreads();
   }
-  const int n_lists = few ? lists : n_of, width = p.K + 1;   // (an odd place more: the lists' firsts fall to different threads)
+  const int n_lists = few ? lists : sm.n_of;
   if (n_lists <= BEAM_MAX_USED) {
-    // ---- their candidates ---------------------------------------------------------------------------------------------------------
-#pragma unroll 4
-    for (int at = warp; at < n_lists; at += BEAM_WARPS) {
-      const int list = few ? at : of[at], r = row_of(list);
-      for (int i = lane; i < width; i += 32) score[at * width + i] = i < p.K ? score32(r, key_at(r, list, i)) : -INFINITY;
-    }
-    __syncthreads();
-    const int all = n_lists * width;
+    // ---- their candidates: a warp a list, its first one another lane's in each ------------------------------------------------------
+    auto each = [&](auto f) {
+      for (int at = warp; at < n_lists; at += BEAM_WARPS) {
+        const float off = (float)sm.off[sm.row[at]];
+        for (int i = (lane - 5 * (at / BEAM_WARPS)) & 31; i < p.K; i += 32) f(at, i, value[at * p.K + i] + off);
+      }
+    };
     float top = -INFINITY;
-    for (int c = tid; c < all; c += BEAM_THREADS) top = fmaxf(top, score[c]);
+    each([&](int, int, float s) { top = fmaxf(top, s); });
     const float border = lowered(beam_border(sm.border, top, p.K));
-    for (int c = tid; c < all; c += BEAM_THREADS) {
-      if (!(score[c] >= border && score[c] > -INFINITY)) continue;   // (nor what an infinite logit makes NaN)
-      const int at = atomicAdd(&count, 1);
-      if (at >= BEAM_CAP) break;
-      const int l = c / width, list = few ? l : of[l], r = row_of(list);
-      const unsigned long long key = key_at(r, list, c - l * width);
-      cand_s[at] = (double)beam_value(key) + off[r];
-      cand_at[at] = (unsigned)r * (unsigned)p.V + (unsigned)beam_index(key);
-    }
+    each([&](int at, int i, float s) {
+      if (!(s >= border && s > -INFINITY)) return;   // (nor what an infinite logit makes NaN)
+      const int to = atomicAdd(&sm.count, 1);
+      if (to >= BEAM_CAP) return;
+      const int r = sm.row[at];
+      const unsigned long long key = key_at(sm.chunk[at], i);
+      sm.cand_s[to] = (double)beam_value(key) + sm.off[r];
+      sm.cand_at[to] = (unsigned)r * (unsigned)p.V + (unsigned)beam_index(key);
+    });
   } else if (tid == 0) {
-    count = BEAM_CAP + 1;
+    sm.count = BEAM_CAP + 1;
   }
   __syncthreads();
-  const int n = count;
+  const int n = sm.count;
   if (n <= BEAM_CAP) {
     for (int i = tid; i < n; i += BEAM_THREADS) {
-      const double s = cand_s[i];
-      const unsigned at = cand_at[i];
+      const double s = sm.cand_s[i];
+      const unsigned at = sm.cand_at[i];
       int rank = 0;
-      for (int j = 0; j < n; ++j) rank += beam_better(cand_s[j], cand_at[j], s, at);
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) rank += beam_better(sm.cand_s[j], sm.cand_at[j], s, at);
       if (rank < p.K) write(rank, true, s, at);
     }
     for (int k = n + tid; k < p.K; k += BEAM_THREADS) write(k, false, 0., 0u);
     return;
   }
   // many equal ones: a round each, among the heads of the lists
-  for (int i = tid; i < lists; i += BEAM_THREADS) head[i] = 0;
+  for (int i = tid; i < lists; i += BEAM_THREADS) sm.head[i] = 0;
   auto pick = [&]() {                       // (a thread's own lists)
     BeamBest best = {-INFINITY, 0xffffffffu, -1};
     for (int i = tid; i < lists; i += BEAM_THREADS) {
-      if (head[i] >= p.K) continue;
+      if (sm.head[i] >= p.K) continue;
       const int r = row_of(i);
-      const unsigned long long key = key_at(r, i, head[i]);
-      const BeamBest c = {key ? (double)beam_value(key) + off[r] : -INFINITY, (unsigned)r * (unsigned)p.V + (unsigned)beam_index(key), i};
+      const unsigned long long key = key_at(chunk_of(r, i), sm.head[i]);
+      const BeamBest c = {key ? (double)beam_value(key) + sm.off[r] : -INFINITY, (unsigned)r * (unsigned)p.V + (unsigned)beam_index(key), i};
       if (c.s > -INFINITY && (best.list < 0 || beam_better(c.s, c.at, best.s, best.at))) best = c;
     }
     return best;
@@ -481,16 +506,16 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const __grid_c
       const int list = __shfl_xor_sync(0xffffffffu, best.list, o);
       if (list >= 0 && (best.list < 0 || beam_better(s, at, best.s, best.at))) best = {s, at, list};
     }
-    if (lane == 0) red[warp] = best;
+    if (lane == 0) sm.red[warp] = best;
     __syncthreads();
-    best = red[0];
+    best = sm.red[0];
     for (int w = 1; w < BEAM_WARPS; ++w) {
-      const BeamBest o = red[w];
+      const BeamBest o = sm.red[w];
       if (o.list >= 0 && (best.list < 0 || beam_better(o.s, o.at, best.s, best.at))) best = o;
     }
     if (tid == 0) write(k, best.list >= 0, best.s, best.at);
     if (best.list >= 0 && best.list == own.list) {
-      ++head[best.list];
+      ++sm.head[best.list];
       own = pick();
     }
     __syncthreads();
