@@ -4,12 +4,12 @@
 // Bound by the logits' bytes, which are read once, and nearly as much by their exponentials (16 a cycle and SM: 70 % of the time
 // that bf16 logits take to arrive).
 //  * beam_chunk_kernel: the order inside a row is the order of its logits, which needs no logsumexp. The rows' chunks are dealt in
-//    equal contiguous ranges to two CTAs an SM. A CTA holds a chunk in registers (8 16-byte vectors a thread: 16,384 bf16 or
-//    8,192 fp32 values) while the next one is on its way into others, and leaves, for its part of a row, (max, sum of
-//    exponentials) and the k best keys, value and ~index, in order.
+//    equal contiguous ranges to two CTAs an SM. A chunk (16,384 bf16 or 8,192 fp32 values) comes by a bulk copy into a ring of
+//    three, so that up to 192 KB an SM are on their way. A CTA leaves, for its part of a row, (max, sum of exponentials) and the
+//    k best keys, value and ~index, in order. (Vectors in registers, unrolled: no faster, and twice the code.)
 //  * k best of many: the k-th largest of some of them (the largest of each group of threads, in a part's first chunk) is a lower
-//    bound of the k-th largest of all. What reaches it is collected, chunk after chunk, and ranked by counting at the end. A
-//    chunk in which too many reach it (ties, rising rows) takes k rounds of a maximum instead.
+//    bound of the k-th largest of all. What reaches it is collected, chunk after chunk, and ranked by counting at the end. Chunks
+//    in which too many reach it (ties, rising rows) take k rounds of a maximum instead.
 //  * beam_merge_kernel: a CTA per request makes its rows' logsumexps and merges their parts' lists, in the same way. Row sums and
 //    scores are in 64 bits there, so that two beams' candidates are ordered by more than fp32 shows.
 //  * exp in fp32, a thread's terms under its own maximum; a row's sum is off by some 2^-22 of itself.
@@ -51,6 +51,10 @@ __device__ __forceinline__ int beam_owner(const BeamParams& p, int u) {
   return (int)(((unsigned)(u + 1) * (unsigned)p.grid - 1) / (unsigned)(p.R * p.chunks));
 }
 
+template <typename T>
+__device__ __forceinline__ float beam_value_of(uint32_t w, int j) {   // value j (0 or 1; fp32: 0) of a word
+  return sizeof(T) == 4 ? __uint_as_float(w) : j ? bf16hi(w) : bf16lo(w);
+}
 // A value's place in the order: larger values first, then lower indices; 0 is less than every one of them.
 __device__ __forceinline__ unsigned long long beam_key(float x, int v) { return argmax_key(x + 0.f, v); }   // (-0 is 0)
 __device__ __forceinline__ float beam_value(unsigned long long key) {
@@ -86,58 +90,91 @@ __device__ __forceinline__ float beam_border(BeamBorder& sm, float top, int k) {
   return sm.border;
 }
 
+constexpr int BEAM_STAGES = 3, BEAM_CHECK = 4;   // chunks in the ring; chunks between looks at the number of candidates
+struct BeamChunkSmem {
+  uint4 ring[BEAM_STAGES][BEAM_THREADS * BEAM_VECTORS];
+  unsigned long long cand[BEAM_CAP];       // keys
+  uint32_t hit[BEAM_CAP];                  // vectors with a value that reaches the border: vector of the row, top bit: of the first chunk
+  BeamBorder border;
+  unsigned long long red[BEAM_WARPS];
+  float red_m[BEAM_WARPS], red_l[BEAM_WARPS];
+  uint64_t full[BEAM_STAGES], empty[BEAM_STAGES];
+  int count, hits;
+};
+
 template <typename T>
 __global__ void __launch_bounds__(BEAM_THREADS, 2) beam_chunk_kernel(const __grid_constant__ BeamParams p) {
-  constexpr int PER = 16 / sizeof(T), PW = 4 / sizeof(T), WORDS = BEAM_VECTORS * 4;   // values of a vector and a word; words of a thread
+  constexpr int PER = 16 / sizeof(T), PW = 4 / sizeof(T);   // values of a vector and a word
   constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;   // -inf
-  __shared__ __align__(16) unsigned long long cand[BEAM_CAP];
-  __shared__ __align__(16) BeamBorder sm_border;
-  __shared__ unsigned long long red[BEAM_WARPS];
-  __shared__ float red_m[BEAM_WARPS], red_l[BEAM_WARPS];
-  __shared__ int count;
+  extern __shared__ __align__(128) uint8_t beam_smem[];
+  BeamChunkSmem& sm = *reinterpret_cast<BeamChunkSmem*>(beam_smem);
+  auto &cand = sm.cand;
+  int &count = sm.count, &hits = sm.hits;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) {
+    for (int i = 0; i < BEAM_STAGES; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], BEAM_WARPS);
+    }
+    fence_mbar_init();
+  }
+  __syncthreads();
   grid_dep_wait();
   grid_dep_launch();
   const int u0 = beam_first(p, blockIdx.x), u1 = beam_first(p, blockIdx.x + 1);
 
-  // chunk u: its row's address, the values of that row's first vector that lie before it, its first vector
+  // chunk u: its row's address, the values of that row's first vector that lie before it, its first vector, and those of its
+  // vectors (from .. to - 1 of the row) that lie whole within the tensor, which are copied
   struct Chunk {
     uintptr_t base;
-    int lead, g0;
+    int lead, g0, from, to;
   };
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(p.logits), hi = lo + ((size_t)(p.R - 1) * p.row_stride + p.V) * sizeof(T);
   auto chunk_of = [&](int u) {
     const int row = u / p.chunks;
     Chunk c;
-    c.base = reinterpret_cast<uintptr_t>(p.logits) + (size_t)row * p.row_stride * sizeof(T);
+    c.base = lo + (size_t)row * p.row_stride * sizeof(T);
     c.lead = (int)(c.base & 15) / (int)sizeof(T);
     c.g0 = (u - row * p.chunks) * p.granules;
+    const uintptr_t v0 = c.base & ~(uintptr_t)15;
+    const int all = (c.lead + p.V + PER - 1) / PER;
+    c.from = c.g0 == 0 && v0 < lo ? 1 : c.g0;
+    c.to = min(c.g0 + p.granules, all);
+    if (c.to == all && v0 + (size_t)all * 16 > hi) --c.to;
     return c;
   };
-  auto index = [&](const Chunk& c, int word) { return (c.g0 + (word / 4) * BEAM_THREADS + tid) * PER - c.lead + (word % 4) * PW; };   // of its first value
-  auto load = [&](const Chunk& c, uint32_t (&x)[WORDS]) {
-#pragma unroll
-    for (int i = 0; i < BEAM_VECTORS; ++i) {
-      const int first = index(c, 4 * i);
-      uint4 w = make_uint4(NONE, NONE, NONE, NONE);
-      if (i * BEAM_THREADS + tid < p.granules && first < p.V && first > -PER) {
-        if (first >= 0 && first + PER <= p.V) {
-          w = ldg_stream(reinterpret_cast<const T*>(c.base) + first);
-        } else {                            // a row's first and last vector: its own values only
-          uint64_t half[2] = {(uint64_t)NONE << 32 | NONE, (uint64_t)NONE << 32 | NONE};
-          const T* src = reinterpret_cast<const T*>(c.base);
+  auto copy = [&](int u) {                  // thread 0
+    const Chunk c = chunk_of(u);
+    const int st = (u - u0) % BEAM_STAGES, n = max(0, c.to - c.from);
+    mbar_arrive_expect_tx(&sm.full[st], (uint32_t)n * 16);
+    if (n) bulk_g2s(&sm.ring[st][c.from - c.g0], reinterpret_cast<const void*>((c.base & ~(uintptr_t)15) + (size_t)c.from * 16), (uint32_t)n * 16, &sm.full[st]);
+  };
+  // vector v of a row at its edge: its own values only
+  auto gather = [&](uintptr_t base, int first) {
+    uint64_t half[2] = {(uint64_t)NONE << 32 | NONE, (uint64_t)NONE << 32 | NONE};
+    const T* src = reinterpret_cast<const T*>(base);
 #pragma unroll 1
-          for (int j = max(0, -first); j < min(PER, p.V - first); ++j) {
-            const uint32_t v = sizeof(T) == 4 ? __float_as_uint((float)src[first + j]) : (uint32_t)__bfloat16_as_ushort((bf16)src[first + j]);
-            const int bit = j * (int)sizeof(T) * 8;
-            const uint64_t mask = (sizeof(T) == 4 ? 0xffffffffull : 0xffffull) << (bit & 63);
-            if (bit < 64) half[0] = (half[0] & ~mask) | (uint64_t)v << (bit & 63);
-            else half[1] = (half[1] & ~mask) | (uint64_t)v << (bit & 63);
-          }
-          w = make_uint4((uint32_t)half[0], (uint32_t)(half[0] >> 32), (uint32_t)half[1], (uint32_t)(half[1] >> 32));
-        }
-      }
-      x[4 * i] = w.x, x[4 * i + 1] = w.y, x[4 * i + 2] = w.z, x[4 * i + 3] = w.w;
+    for (int j = max(0, -first); j < min(PER, p.V - first); ++j) {
+      const uint32_t v = sizeof(T) == 4 ? __float_as_uint((float)src[first + j]) : (uint32_t)__bfloat16_as_ushort((bf16)src[first + j]);
+      const int bit = j * (int)sizeof(T) * 8;
+      const uint64_t mask = (sizeof(T) == 4 ? 0xffffffffull : 0xffffull) << (bit & 63);
+      if (bit < 64) half[0] = (half[0] & ~mask) | (uint64_t)v << (bit & 63);
+      else half[1] = (half[1] & ~mask) | (uint64_t)v << (bit & 63);
     }
+    return make_uint4((uint32_t)half[0], (uint32_t)(half[0] >> 32), (uint32_t)half[1], (uint32_t)(half[1] >> 32));
+  };
+  // this thread's vector i of the chunk; what is not the row's is -inf
+  auto take = [&](const Chunk& c, int st, int i) {
+    const int at = i * BEAM_THREADS + tid, first = (c.g0 + at) * PER - c.lead;
+    uint4 w = make_uint4(NONE, NONE, NONE, NONE);
+    if (at < p.granules && first < p.V && first > -PER) w = first >= 0 && first + PER <= p.V ? sm.ring[st][at] : gather(c.base, first);
+    return w;
+  };
+  auto largest = [&](const uint4& w) {      // (a NaN is none, but for a vector of them)
+    if (sizeof(T) == 4) return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+    const __nv_bfloat162 mx = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(mx), __high2float(mx));
   };
   // cand[0 .. n): the k best of them to the front, in order (0 where there are fewer)
   auto rank_all = [&](int n) {
@@ -165,94 +202,97 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) beam_chunk_kernel(const __gri
     for (int k = n + tid; k < p.K; k += BEAM_THREADS) cand[k] = 0;
     __syncthreads();
   };
-  uint32_t next[WORDS];
-  if (u0 < u1) load(chunk_of(u0), next);
+  if (tid == 0)
+    for (int u = u0; u < min(u1, u0 + BEAM_STAGES); ++u) copy(u);
   int first_u = u0;                         // the part's first chunk
   float m = -INFINITY, border = -INFINITY;
-  uint64_t sum[2] = {0, 0};
-  int kept = 0;                             // candidates of the chunks before
+  float sum = 0.f;
+  int kept = 0, since = 0, looked = u0;     // candidates at the last look; chunks since; the next one
+  bool ok = true;
   for (int u = u0; u < u1; ++u) {
     const Chunk c = chunk_of(u);
     const bool ends = u + 1 == u1 || (u + 1) % p.chunks == 0;
-    uint32_t x[WORDS];
-#pragma unroll
-    for (int i = 0; i < WORDS; ++i) x[i] = next[i];
-    if (u + 1 < u1) load(chunk_of(u + 1), next);
-    // ---- maximum, sum -------------------------------------------------------------------------------------------------------------
-    float vm[BEAM_VECTORS], top = -INFINITY;   // of each vector, of them all
-#pragma unroll
-    for (int i = 0; i < BEAM_VECTORS; ++i) {
-      if (sizeof(T) == 2) {
-        const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(&x[4 * i]);
-        const __nv_bfloat162 mx = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
-        vm[i] = fmaxf(__low2float(mx), __high2float(mx));
-      } else {
-        vm[i] = fmaxf(fmaxf(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1])), fmaxf(__uint_as_float(x[4 * i + 2]), __uint_as_float(x[4 * i + 3])));
-      }
-      top = fmaxf(top, vm[i]);              // (NaN only: none)
-    }
-    if (top > m) {
-      const float f = ex2((m - top) * LOG2E);   // (m -inf: 0)
-      sum[0] = mul2(sum[0], f32x2(f, f)), sum[1] = mul2(sum[1], f32x2(f, f));
-      m = top;
-    }
-    const float under = m == -INFINITY ? 0.f : -m * LOG2E;
-    const uint64_t scale2 = f32x2(LOG2E, LOG2E), under2 = f32x2(under, under);
-#pragma unroll
-    for (int i = 0; i < WORDS; i += 3 - PW) {   // two values
-      const uint64_t v = sizeof(T) == 4 ? f32x2(__uint_as_float(x[i]), __uint_as_float(x[i + 2 - PW])) : f32x2(bf16lo(x[i]), bf16hi(x[i]));
-      const uint64_t e = fma2(v, scale2, under2);
-      sum[i >> (2 - PW) & 1] = add2(sum[i >> (2 - PW) & 1], f32x2(ex2(f32x2_lo(e)), ex2(f32x2_hi(e))));
-    }
-    // ---- the k best ---------------------------------------------------------------------------------------------------------------
+    const int st = (u - u0) % BEAM_STAGES, turn = (u - u0) / BEAM_STAGES;
     const bool begins = u == first_u;
-    if (begins) {
-      if (tid == 0) count = 0;
-      kept = 0;
-      border = beam_border(sm_border, top, p.K);
+    ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.full[st], (uint32_t)(turn & 1)));
+    auto push = [&](int i) {
+      const int at = atomicAdd(&hits, 1);
+      if (at < BEAM_CAP) sm.hit[at] = (uint32_t)(c.g0 + i * BEAM_THREADS + tid) | (begins ? 1u << 31 : 0);
+    };
+    // ---- maximum, sum, what reaches the border (equal values of later chunks have higher indices than k that are kept already) -------
+    float top = -INFINITY;
+#pragma unroll 2
+    for (int i = 0; i < BEAM_VECTORS; ++i) {
+      const uint4 w = take(c, st, i);
+      const float vm = largest(w), mn = fmaxf(m, vm), z = mn == -INFINITY ? 0.f : mn;   // (x - z first: its product's rounding goes by it)
+      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+      float e[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        e[j] = ex2((beam_value_of<T>(words[j], 0) - z) * LOG2E);
+        if (PW == 2) e[j] += ex2((beam_value_of<T>(words[j], 1) - z) * LOG2E);
+      }
+      sum = sum * ex2((m - z) * LOG2E) + ((e[0] + e[1]) + (e[2] + e[3]));
+      m = mn;
+      top = fmaxf(top, vm);
+      if (!begins && vm > border) push(i);
     }
-    // (equal values of later chunks have higher indices than k that are kept already)
-    auto reaches = [&](float v) { return begins ? v >= border && v > -INFINITY : v > border; };
-    if (reaches(top)) {
-      uint32_t hits = 0;
-#pragma unroll
-      for (int i = 0; i < BEAM_VECTORS; ++i) hits |= (reaches(vm[i]) ? 1u : 0u) << i;
-      while (hits) {
-        const int i = __ffs(hits) - 1, first = index(c, 4 * i);
-        hits &= hits - 1;
-        uint32_t w[4];                      // (registers have no index)
-#pragma unroll
-        for (int k = 0; k < BEAM_VECTORS; ++k)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (k == 0 || k == i) w[j] = x[4 * k + j];
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          const float v = sizeof(T) == 4 ? __uint_as_float(w[j & 3]) : j & 1 ? bf16hi(w[j / 2 & 3]) : bf16lo(w[j / 2 & 3]);
-          if (!reaches(v)) continue;
-          const int at = atomicAdd(&count, 1);
-          if (at < BEAM_CAP) cand[at] = beam_key(v, first + j);
+    if (begins) {
+      if (tid == 0) count = hits = 0;
+      kept = 0;
+      border = beam_border(sm.border, top, p.K);
+      if (top >= border && top > -INFINITY)
+#pragma unroll 1
+        for (int i = 0; i < BEAM_VECTORS; ++i) {
+          const float vm = largest(take(c, st, i));
+          if (vm >= border && vm > -INFINITY) push(i);
         }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.empty[st]);
+    if (tid == 0 && u + BEAM_STAGES < u1 && ok) {
+      ok = mbar_wait_small(&sm.empty[st], (uint32_t)(turn & 1));
+      if (ok) copy(u + BEAM_STAGES);
+    }
+    if (!ends && ++since < BEAM_CHECK) continue;
+    since = 0;
+    __syncthreads();
+    const int vectors = hits;
+    if (!ends && vectors <= BEAM_CAP / 2) continue;
+    // ---- the vectors' values that reach the border, the k best of them and of those before -----------------------------------------
+    for (int i = tid; i < min(vectors, BEAM_CAP); i += BEAM_THREADS) {
+      const int first = (int)(sm.hit[i] & 0x7fffffffu) * PER - c.lead;
+      const bool in_first = sm.hit[i] >> 31;
+      const uint4 w = first >= 0 && first + PER <= p.V ? *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(c.base) + first) : gather(c.base, first);
+      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+      uint32_t reach = 0;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const float v = beam_value_of<T>(words[j / PW], j % PW);
+        reach |= ((in_first ? v >= border && v > -INFINITY : v > border) ? 1u : 0u) << j;
+      }
+      while (reach) {
+        const int j = __ffs(reach) - 1, at = atomicAdd(&count, 1);
+        reach &= reach - 1;
+        if (at < BEAM_CAP) cand[at] = beam_key((float)reinterpret_cast<const T*>(c.base)[first + j], first + j);
       }
     }
     __syncthreads();
-    int n = count;
-    if (n > BEAM_CAP) {                     // one a round: the thread that gave it looks for its next, among the kept and the chunk's
+    int n = vectors > BEAM_CAP ? BEAM_CAP + 1 : count;
+    if (n > BEAM_CAP) {
+      // one a round: the thread that gave it looks for its next, among those kept at the last look and the values since
       const T* src = reinterpret_cast<const T*>(c.base);
+      const int row_u = u / p.chunks * p.chunks, v0 = max(0, (max(first_u, looked) - row_u) * p.granules * PER - c.lead);
+      const int v1 = min(p.V, (u + 1 - row_u) * p.granules * PER - c.lead);
       auto next_best = [&](unsigned long long below) {
         unsigned long long best = 0;
         for (int i = tid; i < kept; i += BEAM_THREADS)
           if (cand[i] < below && cand[i] > best) best = cand[i];
-#pragma unroll 1
-        for (int i = 0; i < BEAM_VECTORS; ++i) {
-          const int at = index(c, 4 * i);
-#pragma unroll
-          for (int j = 0; j < PER; ++j) {
-            const bool in = i * BEAM_THREADS + tid < p.granules && at + j >= 0 && at + j < p.V;
-            const float v = in ? (float)src[at + j] : -INFINITY;
-            const unsigned long long key = v > -INFINITY ? beam_key(v, at + j) : 0;   // (a NaN is none)
-            if (key < below && key > best) best = key;
-          }
+#pragma unroll 8
+        for (int i = v0 + tid; i < v1; i += BEAM_THREADS) {
+          const float v = (float)src[i];
+          const unsigned long long key = v > -INFINITY ? beam_key(v, i) : 0;   // (a NaN is none)
+          if (key < below && key > best) best = key;
         }
         return best;
       };
@@ -263,44 +303,45 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) beam_chunk_kernel(const __gri
         unsigned long long best = mine;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-        if (lane == 0) red[warp] = best;
+        if (lane == 0) sm.red[warp] = best;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < BEAM_WARPS; ++w) best = max(best, red[w]);
-        if (tid == 0) cand[BEAM_CAP - BEAM_MAX_K + k] = best;   // (kept are at most half of them)
+        for (int w = 0; w < BEAM_WARPS; ++w) best = max(best, sm.red[w]);
+        if (tid == 0) cand[BEAM_CAP - BEAM_MAX_K + k] = best;   // (those kept are in front)
         stale = best && best == mine;
         __syncthreads();
       }
       if (tid < p.K) cand[tid] = cand[BEAM_CAP - BEAM_MAX_K + tid];
       __syncthreads();
-    } else if (ends || n > BEAM_CAP / 2) {
+    } else {
       rank_all(n);
     }
-    if (n > BEAM_CAP / 2 || ends) {         // the k best are in front
-      n = min(n, p.K);
-      if (n == p.K) border = fmaxf(border, beam_value(cand[p.K - 1]));
-      if (tid == 0) count = n;
-    }
-    kept = n;
+    kept = min(n, p.K);                     // the k best are in front
+    if (kept == p.K) border = fmaxf(border, beam_value(cand[p.K - 1]));
+    if (tid == 0) count = kept, hits = 0;
+    looked = u + 1;
     if (ends) {
       const float M = warp_max(m);          // the warp's sum under its maximum
-      float l = (f32x2_lo(sum[0]) + f32x2_hi(sum[0])) + (f32x2_lo(sum[1]) + f32x2_hi(sum[1]));
-      l = warp_sum(M == -INFINITY ? l : l * ex2((m - M) * LOG2E));   // (a NaN stays)
-      if (lane == 0) red_m[warp] = M, red_l[warp] = l;
+      float l = warp_sum(M == -INFINITY ? sum : sum * ex2((m - M) * LOG2E));   // (a NaN stays)
+      if (lane == 0) sm.red_m[warp] = M, sm.red_l[warp] = l;
       unsigned long long* keys = p.keys + (size_t)first_u * p.K;
       if (tid < p.K) keys[tid] = cand[tid];
       __syncthreads();
       if (warp == 0) {
-        const float wm = lane < BEAM_WARPS ? red_m[lane] : -INFINITY, wl = lane < BEAM_WARPS ? red_l[lane] : 0.f, top_m = warp_max(wm);
+        const float wm = lane < BEAM_WARPS ? sm.red_m[lane] : -INFINITY, wl = lane < BEAM_WARPS ? sm.red_l[lane] : 0.f, top_m = warp_max(wm);
         l = warp_sum(top_m == -INFINITY ? wl : wl * ex2((wm - top_m) * LOG2E));
         if (lane == 0) p.ml[first_u] = make_float2(top_m, l);
       }
       first_u = u + 1;
       m = -INFINITY;
-      sum[0] = sum[1] = 0;
+      sum = 0.f;
     }
     __syncthreads();                        // the next chunk's candidates come behind, or in the place of these
   }
+  if (!ok && lane == 0) atomicOr(&g_dev_error, DEVERR_MBAR_TIMEOUT);
+  if (__syncthreads_or(!ok) && tid == 0)    // a wait gave up: the copies in flight land before the shared memory goes away
+    for (int u = max(u0, u1 - BEAM_STAGES); u < u1; ++u)
+      mbar_wait_small(&sm.full[(u - u0) % BEAM_STAGES], (uint32_t)((u - u0) / BEAM_STAGES & 1), 1000000ull);
 }
 
 constexpr int BEAM_MAX_USED = 256;         // lists that are merged side by side
@@ -387,17 +428,22 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const __grid_c
   __syncthreads();
   grid_dep_wait();                          // the chunks' lists are there
   grid_dep_launch();
-  // ---- the lists' values on their way, the rows' sums ------------------------------------------------------------------------------
   auto key_at = [&](int chunk, int i) { return __ldcg(p.keys + (size_t)chunk * p.K + i); };
+  // ---- the lists' values on their way, the rows' sums ------------------------------------------------------------------------------
   auto fetch = [&](int n) {
-#pragma unroll 4
-    for (int at = warp; at < n; at += BEAM_WARPS)
+    const float per_k = 1.f / p.K;
+#pragma unroll 1
+    for (int c0 = tid; c0 < n * p.K; c0 += 8 * BEAM_THREADS) {
+      unsigned long long key[8];
 #pragma unroll
-      for (int i = lane; i < BEAM_MAX_K; i += 32)
-        if (i < p.K) {
-          const unsigned long long key = key_at(sm.chunk[at], i);
-          value[at * p.K + i] = key ? beam_value(key) : -INFINITY;
-        }
+      for (int j = 0; j < 8; ++j) {
+        const int c = min(c0 + j * BEAM_THREADS, n * p.K - 1), at = (int)(((float)c + 0.5f) * per_k);   // c / K (c < 2^14, K <= 64)
+        key[j] = key_at(sm.chunk[at], c - at * p.K);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c0 + j * BEAM_THREADS < n * p.K) value[c0 + j * BEAM_THREADS] = key[j] ? beam_value(key[j]) : -INFINITY;
+    }
   };
   if (few) {
     if (tid < lists) sm.ml[tid] = __ldcg(p.ml + sm.chunk[tid]);

@@ -178,8 +178,11 @@ int qk_beam_select(const qk_beam_select_t* args, qk_stream_t stream) {
   p.keys = static_cast<unsigned long long*>(a.workspace);
   p.ml = reinterpret_cast<float2*>(p.keys + all * p.K);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (all)
-    if (int r = launch(a.fp32 ? beam_chunk_kernel<float> : beam_chunk_kernel<bf16>, dim3(p.grid), dim3(BEAM_THREADS), 0, st, p)) return r;
+  if (all) {
+    auto k = a.fp32 ? beam_chunk_kernel<float> : beam_chunk_kernel<bf16>;
+    if (int r = ensure_smem((const void*)k, (int)sizeof(BeamChunkSmem))) return r;
+    if (int r = launch(k, dim3(p.grid), dim3(BEAM_THREADS), sizeof(BeamChunkSmem), st, p)) return r;
+  }
   const int lists = (int)std::min((size_t)BEAM_MAX_USED, (size_t)std::min(p.R, BEAM_MAX_ROWS) * p.chunks), smem = (int)sizeof(BeamMergeSmem) + lists * p.K * 4;
   if (int r = ensure_smem((const void*)beam_merge_kernel, smem)) return r;
   return launch_as(all || g_pdl, beam_merge_kernel, dim3(p.B), dim3(BEAM_THREADS), smem, st, p);
