@@ -9,6 +9,9 @@ and one pass mixes whole prompts, chunks of long prompts and decode steps:
   into the pages) -> packed_attention (every sequence of the pass begins here) or paged_attention -> W_o, residual, W_gu,
   SwiGLU, W_down, residual -> the last row of each sequence through the final norm, the FP8 head and the argmax.
 
+`beam_search` lets beams share their pages: `paged_plan` (pages, offsets) -> the pass with `shared_attention` -> `beam_select` ->
+`paged_fork` (the beams in their new order), all on the device, a captured graph a step.
+
 `paged_kv_read` hands a sequence to a contiguous-cache engine (`export`). `capture` records the decode step of a fixed set
 of sequences as a CUDA graph: their lengths and tables are device data.
 """
@@ -75,6 +78,7 @@ class PagedEngine:
         self.lens: dict[int, int] = {}            # sequence -> positions in the cache
         self._next = 0
         self.graph = None
+        self.beam_graph = True                    # beam_search replays a graph for each step
 
     # ---- sequences ---------------------------------------------------------------------------------------------
     def new(self) -> int:
@@ -118,10 +122,10 @@ class PagedEngine:
             self.k.fp8_gemm_rows(x[r:r + GEMM_ROWS], w, scale, out[r:r + GEMM_ROWS], norm_w=norm_w, eps=self.m.cfg.eps,
                                  scratch=self.linear_ws)
 
-    def _forward(self, tokens, cu, lens, table, max_q, whole, last):
+    def _forward(self, tokens, cu, lens, table, max_q, whole, last, sharing=None):
         """One pass over T packed rows (device tensors); `whole`: every sequence begins in this pass. Leaves each
         sequence's logits and argmax key in rows 0 .. B-1 of `logits` and `best`; last: its last row, or None where
-        every row is one."""
+        every row is one. sharing: (groups, shared, workspace) of sequences that share their first positions."""
         m, k, cfg = self.m, self.k, self.m.cfg
         T, B = tokens.shape[0], lens.shape[0]
         nq, nkv, hd = cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
@@ -137,6 +141,8 @@ class PagedEngine:
                         k_scale=ks, v_scale=vs, k_out=kb if whole else None)
             if whole:
                 k.packed_attention(q, kb, v, cu, attn, scale, max_q, workspace=self.ws)
+            elif sharing:
+                k.shared_attention(q, cu, lens, table, *sharing[:2], kp, vp, attn, scale, max_q, k_scale=ks, v_scale=vs, workspace=sharing[2])
             else:
                 k.paged_attention(q, cu, lens, table, kp, vp, attn, scale, max_q, k_scale=ks, v_scale=vs, workspace=self.ws)
             self._linear(attn, wo, L.o.scale, y)
@@ -232,6 +238,148 @@ class PagedEngine:
                         self.release(s)
         return out
 
+    # ---- beam search -------------------------------------------------------------------------------------------
+    @torch.no_grad()
+    def beam_search(self, prompts, beams: int, gen_len: int, eos: int | None = None, length_penalty: float = 1.0):
+        """The `beams` best continuations of each prompt (lists of ids) by beam search, of up to gen_len tokens: per prompt a
+        list of (ids, score), best first, score = sum of log-probabilities / (number of ids) ** length_penalty (at least 0).
+        Each step takes the 2 * beams best candidates of a prompt's beams: those of the first `beams` that are `eos` become
+        hypotheses (the eos is their last id), the first `beams` others go on. Prompts enter as many at a time as passes and
+        pool can hold; the beams of a prompt share its pages, and each other's."""
+        prompts, K = [list(p) for p in prompts], 2 * beams
+        limit = min(self.max_seqs, self.max_rows)
+        if not 1 <= beams <= min(32, limit) or gen_len < 1 or not length_penalty >= 0:
+            raise ValueError(f"{beams} beams (1 to {min(32, limit)}), {gen_len} tokens, length penalty {length_penalty}")
+        if not all(len(p) for p in prompts) or self.m.cfg.vocab < K:
+            raise ValueError(f"{sum(not len(p) for p in prompts)} empty prompts, {beams} beams over {self.m.cfg.vocab} tokens")
+        longest = max((len(p) for p in prompts), default=0) + gen_len - 1
+        if longest > self.max_len:
+            raise RuntimeError(f"sequence of {longest} positions: the engine was built for {self.max_len}")
+        # a prompt's pages, and for each beam what it writes: from the page that the prompt ends in, which forks copy
+        need = [len(p) // self.page_size + beams * (-(-(len(p) + gen_len - 1) // self.page_size) - len(p) // self.page_size + 1)
+                for p in prompts]
+        if max(need, default=0) > len(self.free):
+            raise RuntimeError(f"out of pages: {max(need)} wanted by one prompt, {len(self.free)} free")
+        out, at = [], 0
+        while at < len(prompts):
+            n = 1
+            while at + n < len(prompts) and (n + 1) * beams <= limit and sum(need[at:at + n + 1]) <= len(self.free):
+                n += 1
+            out += self._beam_batch(prompts[at:at + n], sum(need[at:at + n]), beams, gen_len, eos, length_penalty)
+            at += n
+        return out
+
+    def _beam_batch(self, prompts, pages, beams, gen_len, eos, alpha):
+        N, K, R, V, dev = len(prompts), 2 * beams, len(prompts) * beams, self.m.cfg.vocab, self.m.device
+        k, seqs, pool = self.k, [], []
+        i32 = dict(dtype=torch.int32, device=dev)
+        try:
+            logits = torch.empty(N, V, dtype=torch.bfloat16, device=dev)
+            for i, p in enumerate(prompts):      # prompts alone or in chunks
+                seqs.append(self.new())
+                for c in range(0, len(p), self.max_rows):
+                    self.step([(seqs[i], p[c:c + self.max_rows])])
+                logits[i] = self.logits[0]
+            held = [x for s in seqs for x in self.tables[s]]
+            pool = [self.free.pop() for _ in range(pages - len(held))]
+            refs = torch.ones(self.k_pages.shape[1], **i32)
+            if pool:
+                refs[torch.tensor(pool, device=dev)] = 0
+            table, table2 = self._table(seqs), torch.empty(R, self.width, **i32)
+            lens = self._int32([len(p) for p in prompts])
+            lens2, info = torch.empty(R, **i32), torch.zeros(2, **i32)
+            # per request: the candidates of a step, the hypotheses that ended; per step: each beam's parent and token
+            cand = (torch.empty(N, K, device=dev), torch.empty(N, K, **i32), torch.empty(N, K, **i32))
+            ws = k.beam_workspace(dev, R, V, K)
+            scores, token, parents = torch.empty(R, device=dev), torch.empty(R, **i32), torch.empty(R, **i32)
+            ended = torch.full((N, beams), -float("inf"), device=dev)
+            ended_at = torch.zeros(N, beams, dtype=torch.int64, device=dev)   # step * R + parent row
+            hist = torch.zeros(2, gen_len, R, **i32)
+            step = torch.zeros(1, dtype=torch.int64, device=dev)
+            rank = torch.arange(K, device=dev)
+            weight = torch.arange(1, gen_len + 1, device=dev, dtype=torch.float64).pow(-alpha).float()   # of a hypothesis of n tokens
+            first_row = (torch.arange(N, device=dev, dtype=torch.int32) * beams)[:, None]
+
+            def choose(rows_logits, rows_scores, cu, parent_of):
+                """The candidates of a step -> hypotheses that ended, the beams that go on (their parents, tokens and scores)."""
+                k.beam_select(rows_logits, rows_scores, cu, *cand, workspace=ws)
+                s, parent, tok = cand
+                none = parent < 0
+                over = torch.zeros_like(none) if eos is None else (tok == eos) & ~none
+                new = torch.where(over & (rank < beams), s * weight[step], -float("inf"))
+                best, i = torch.cat((ended, new), 1).topk(beams, dim=1)
+                ended.copy_(best)
+                ended_at.copy_(torch.cat((ended_at, step * R + parent_of(parent)), 1).gather(1, i))
+                on = torch.where(over, rank + K, rank).topk(beams, dim=1, largest=False, sorted=True).indices   # (keys are all different)
+                scores.copy_(s.gather(1, on).flatten())
+                parents.copy_(parent_of(parent).gather(1, on).flatten())
+                token.copy_(tok.clamp(min=0).gather(1, on).flatten())   # (a beam without a candidate: score -inf)
+                hist[0].index_copy_(0, step, parents[None])
+                hist[1].index_copy_(0, step, token[None])
+                step.add_(1)
+
+            # the prompts' own logits: the first tokens; every beam of a request continues its prompt
+            choose(logits, torch.zeros(N, device=dev), torch.arange(N + 1, **i32),
+                   lambda p: torch.arange(N, **i32)[:, None].expand(N, K).contiguous())
+            k.paged_fork(refs, lens, parents, table, table2, lens2, self.k_pages, self.v_pages, *self._scales(), info=info)
+            table = torch.empty_like(table2)
+            cu, cu_new, ones = torch.arange(N + 1, **i32) * beams, torch.empty(R + 1, **i32), torch.ones(R, **i32)
+            seq_lens, shared = torch.empty(R, **i32), torch.empty(N, **i32)
+            sharing = (cu, shared, k.shared_workspace(dev, R, self.m.cfg.n_heads))
+
+            def one():
+                k.paged_plan(refs, lens2, ones, table2, cu_new, seq_lens, self.page_size, groups=cu, shared=shared, info=info)
+                table.copy_(table2)
+                self._forward(token, cu_new, seq_lens, table, 1, False, None, sharing)
+                choose(self.logits[:R], scores, cu, lambda p: torch.where(p < 0, first_row, p))
+                k.paged_fork(refs, seq_lens, parents, table, table2, lens2, self.k_pages, self.v_pages, *self._scales(), info=info)
+
+            graph, done = None, 1
+            while done < gen_len:
+                if graph is None and done > 1 and self.beam_graph:   # (the first step warmed everything up)
+                    graph = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(graph):
+                        one()
+                graph.replay() if graph else one()
+                done += 1
+                if eos is not None and done % 8 == 0:   # a beam's score only falls, its weight ends at weight[-1]
+                    top = scores.view(N, beams).amax(1)
+                    if bool((ended.amin(1) >= torch.maximum(top * weight[-1], top * weight[done - 1])).all()):
+                        break
+            live = scores.view(N, beams) * weight[done - 1]
+            result = self._hypotheses(hist[:, :done].tolist(), ended.tolist(), ended_at.tolist(), live.tolist(), done, beams, eos)
+            self.check()
+            return result
+        finally:
+            torch.cuda.synchronize()
+            self.free.extend(reversed(pool))
+            for s in seqs:
+                self.release(s)
+
+    def _scales(self):
+        return (self.k_scale, self.v_scale) if isinstance(self.k_scale, torch.Tensor) else (None, None)
+
+    @staticmethod
+    def _hypotheses(hist, ended, ended_at, live, steps, beams, eos):
+        """Beams and what ended, followed back through the steps' parents: the best of each request, [(ids, score)]."""
+        parents, tokens = hist
+        R = len(parents[0])
+
+        def back(step, row):                     # the ids of beam `row` after the first `step` steps
+            ids = []
+            for t in range(step - 1, -1, -1):
+                ids.append(tokens[t][row])
+                row = parents[t][row]
+            return ids[::-1]
+
+        out = []
+        for b in range(len(ended)):
+            found = [(s, 0, back(at // R, at % R) + [eos]) for s, at in zip(ended[b], ended_at[b]) if s > -float("inf")]
+            found += [(s, 1, back(steps, b * beams + w)) for w, s in enumerate(live[b]) if s > -float("inf")]
+            found.sort(key=lambda h: -h[0])
+            out.append([(ids, s) for s, _, ids in found[:beams]])
+        return out
+
     # ---- decode graph ------------------------------------------------------------------------------------------
     @torch.no_grad()
     def capture(self, seqs, tokens, steps: int):
@@ -322,4 +470,4 @@ class PagedEngine:
         err = self.k.device_error()
         if err:
             raise RuntimeError(f"paged pass failed on the device (error word {err:#x}: 1 = a wait timed out, 2 = a bad position, "
-                               "page or token)")
+                               "page, token or logit, 8 = too few pages)")
