@@ -74,6 +74,27 @@ int shared_launches(const RaggedParams& p, const qk_ragged_attention_t& a, const
   return launch_as(true, prefix_merge_kernel, dim3((m.rows + 3) / 4), dim3(256), 0, st, m);
 }
 
+// A launch of one cluster of `ctas` CTAs.
+template <typename... KArgs, typename... Args>
+int launch_cluster(void (*kernel)(KArgs...), int ctas, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)ctas, 1, 1};
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = g_pdl ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  return e == cudaSuccess ? QK_OK : cuda_fail(e, "kernel launch");
+}
+// One CTA for small work, eight for what takes longer than their barriers cost.
+int plan_ctas(long long pages, long long batch, long long rows) { return pages > 8192 || batch > 128 || rows > 4096 ? 8 : 1; }
+
 }  // namespace
 
 extern "C" {
@@ -107,7 +128,7 @@ int qk_paged_plan(const qk_paged_plan_t* args, qk_stream_t stream) {
   p.B = (int)a.batch, p.width = (int)a.table_width, p.pages = (int)a.n_pages, p.T = (int)a.rows, p.G = (int)a.n_groups;
   const int smem = (2 * p.B + 1) * 4;
   if (int r = ensure_smem((const void*)paged_plan_kernel, smem)) return r;
-  return launch(paged_plan_kernel, dim3(1), dim3(PLAN_THREADS), smem, static_cast<cudaStream_t>(stream), p);
+  return launch_cluster(paged_plan_kernel, plan_ctas(p.pages, p.B, p.T), dim3(PLAN_THREADS), smem, static_cast<cudaStream_t>(stream), p);
 }
 
 int qk_paged_fork(const qk_paged_fork_t* args, qk_stream_t stream) {

@@ -626,9 +626,9 @@ class DecodeOps:
         """The address of a contiguous int32 tensor of `shape` (None: any one-dimensional) on GPU dev; 0 for None."""
         if t is None:
             return 0
-        if t.dtype is not _I32 or t.get_device() != dev or not t.is_contiguous() or (t.dim() != 1 if shape is None else tuple(t.shape) != shape):
-            raise RuntimeError(f"{what}: {name} must be contiguous int32 {list(shape) if shape else '[n]'} on the call's CUDA device")
-        return t.data_ptr()
+        if t.dtype is _I32 and t.get_device() == dev and (t.shape == shape or (shape is None and t.dim() == 1)) and t.is_contiguous():
+            return t.data_ptr()
+        raise RuntimeError(f"{what}: {name} must be contiguous int32 {list(shape) if shape else '[n]'} on the call's CUDA device")
 
     @staticmethod
     def _table(what, name, t, rows, width, dev):
