@@ -143,12 +143,18 @@ struct OwnShape {
   static constexpr int TILE = KEYS * HEAD_DIM * (FP8 ? 1 : 2);   // bytes of K (and of V)
   static constexpr int S = FP8 ? 4 : 2;    // 32 KB
 };
+// Up to so many sequences, and groups, are looked up once, side by side, and kept in shared memory: a warp would else come to
+// its first tile by a chain of some ten loads from memory (64 sequences of up to 500 keys: XX us of launch, XX now).
+constexpr int OWN_KEPT = 128, OWN_KEPT_GROUPS = 32;
+
 template <bool FP8, int NT>
 struct OwnSmem {
   using Sh = OwnShape<FP8, NT>;
   uint8_t k[Sh::S][Sh::TILE], v[Sh::S][Sh::TILE];
   float ks[FP8 ? Sh::S : 1][Sh::KEYS], vs[FP8 ? Sh::S : 1][Sh::KEYS];
   uint64_t full[Sh::S];
+  int4 seq[OWN_KEPT];        // OwnSeq
+  int4 group[OWN_KEPT_GROUPS];   // SharedGroup
 };
 
 struct OwnParams {
@@ -161,13 +167,10 @@ struct OwnParams {
 struct OwnSeq {
   int row0, n, len, start;  // token rows (n 0: not this kernel's), own keys, keys of the prefix before them
 };
-__device__ __forceinline__ OwnSeq own_seq(const OwnParams& p, int b) {
+// Of sequence b, with row0 = cu[b], end = cu[b + 1], len and its group's keys
+__device__ __forceinline__ OwnSeq own_seq(const OwnParams& p, int row0, int end, int len, int keys) {
   const RaggedParams& r = p.r;
-  OwnSeq s;
-  s.row0 = __ldg(r.c.cu + b);
-  s.n = __ldg(r.c.cu + b + 1) - s.row0;
-  s.len = __ldg(r.c.seq_lens + b);
-  s.start = 0;
+  OwnSeq s = {row0, end - row0, len, 0};
   const long long cap = (long long)r.c.table_width << r.c.page_shift;
   bool wrong = s.len > cap;
   if (wrong) s.len = (int)cap;
@@ -175,23 +178,31 @@ __device__ __forceinline__ OwnSeq own_seq(const OwnParams& p, int b) {
   wrong |= bad || (more && p.strict);
   if (bad || more) s.n = 0;
   if (s.n) {
-    s.start = shared_keys(p.x, r.c, b);
+    s.start = keys;
     s.len -= s.start;
     wrong |= s.start && s.len < s.n;        // a new token among the prefix's
   }
   if (wrong) atomicOr(&g_dev_error, DEVERR_BAD_STATE);
   return s;
 }
-
+__device__ __forceinline__ OwnSeq own_seq(const OwnParams& p, int b) {
+  return own_seq(p, __ldg(p.r.c.cu + b), __ldg(p.r.c.cu + b + 1), __ldg(p.r.c.seq_lens + b), shared_keys(p.x, p.r.c, b));
+}
 // The walk over a warp's range of tiles: sequences, their blocks of rows, KV heads, tiles of 32 keys.
 template <int ROWS, int KEYS>
 struct OwnWalk {
   const OwnParams& p;
+  const int4* kept;                         // sequences in shared memory, or null
   OwnSeq s;
   int b, block, g, t, n, blocks;            // t: the next tile of the unit's n
-  __device__ __forceinline__ OwnWalk(const OwnParams& p_, int b_) : p(p_), b(b_), block(0), g(0), t(0) { seq(); }
+  __device__ __forceinline__ OwnWalk(const OwnParams& p_, const int4* kept_, int b_) : p(p_), kept(kept_), b(b_), block(0), g(0), t(0) { seq(); }
   __device__ __forceinline__ void seq() {
-    s = own_seq(p, b);
+    if (kept) {
+      const int4 v = kept[b];
+      s = {v.x, v.y, v.z, v.w};
+    } else {
+      s = own_seq(p, b);
+    }
     blocks = (s.n * p.r.group + ROWS - 1) / ROWS;
     n = max(1, (s.len + KEYS - 1) / KEYS);   // (a sequence without a key still has rows to be written)
   }
@@ -228,8 +239,38 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
   grid_dep_launch();
   // ---- this warp's range: the total, then the sequence its first tile lies in -------------------------------------------------
   const int per = (r.c.B + 31) / 32;
+  const int4* kept = r.c.B <= OWN_KEPT && p.x.G <= OWN_KEPT_GROUPS ? sm.seq : nullptr;
+  if (kept) {
+    int row0[OWN_KEPT / 32], end[OWN_KEPT / 32], len[OWN_KEPT / 32];
+#pragma unroll
+    for (int i = 0; i < OWN_KEPT / 32; ++i) {
+      const int b = 32 * i + lane;
+      row0[i] = end[i] = len[i] = 0;
+      if (b < r.c.B) row0[i] = __ldg(r.c.cu + b), end[i] = __ldg(r.c.cu + b + 1), len[i] = __ldg(r.c.seq_lens + b);
+    }
+    if (lane < p.x.G) {
+      const SharedGroup g = shared_group(p.x, r.c, lane);
+      sm.group[lane] = make_int4(g.first, g.end, g.keys, 0);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < OWN_KEPT / 32; ++i) {
+      const int b = 32 * i + lane;
+      if (b >= r.c.B) break;
+      int lo = 0, hi = p.x.G;               // (as shared_keys)
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (sm.group[mid].x <= b) lo = mid;
+        else hi = mid;
+      }
+      const int4 g = sm.group[lo];
+      const OwnSeq s = own_seq(p, row0[i], end[i], len[i], g.x <= b && b < g.y ? g.z : 0);
+      sm.seq[b] = make_int4(s.row0, s.n, s.len, s.start);
+    }
+    __syncwarp();
+  }
   long long mine = 0;
-  for (int i = lane * per; i < min(r.c.B, (lane + 1) * per); ++i) mine += Walk(p, i).tiles();
+  for (int i = lane * per; i < min(r.c.B, (lane + 1) * per); ++i) mine += Walk(p, kept, i).tiles();
   long long incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -242,7 +283,7 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
   const long long u0 = c * W / G, u1 = (c + 1) * W / G;
   const int owner = __ffs(__ballot_sync(0xffffffffu, incl > u0)) - 1;
   long long start = __shfl_sync(0xffffffffu, incl - mine, owner);
-  Walk at(p, owner * per);
+  Walk at(p, kept, owner * per);
   while (u0 >= start + at.tiles()) {
     start += at.tiles();
     ++at.b;
@@ -303,7 +344,7 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
   for (long long u = u0; u < u1;) {
     const int n = at.n, t0 = at.t, t1 = (int)min((long long)n, t0 + (u1 - u)), from = at.block * ROWS;
     const OwnSeq s = at.s;
-    const int rows = min(ROWS, s.n * r.group - from), first = s.len - s.n + from / r.group;
+    const int rows = min(ROWS, s.n * r.group - from), first = s.len - s.n + by_group(from, r.group);
     w.begin(r, s.row0, s.n, s.len, from, rows, at.g, lane);
     for (int t = t0; t < t1; ++t) {
       const int it = (int)(u - u0) + t - t0, st = it % S;
@@ -334,7 +375,7 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
         for (int e = 0; e < 2; ++e) {
           const int row = nt * 8 + 2 * lt + e;
           if (row >= rows) continue;
-          const int sum_at = (s.row0 + (from + row) / r.group) * r.n_q + at.g * r.group + (from + row) % r.group;
+          const int sum_at = (s.row0 + by_group(from + row, r.group)) * r.n_q + at.g * r.group + from + row - by_group(from + row, r.group) * r.group;
           if (lg == 0) {
             *(whole ? p.x.own_ml + sum_at : p.x.own_part_ml + slot + row) = make_float2(w.m[nt][e], w.l[nt][e]);
             if (t0 == 0) p.x.own_info[sum_at] = code | row << 20;
@@ -360,7 +401,8 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
           for (int i = 0; i < 8; ++i) w.o[i][nt][e] *= inv, w.o[i][nt][2 + e] *= inv;
         }
         auto row_of = [&](int row) {
-          return r.out + (long long)(s.row0 + (from + row) / r.group) * r.out_row + (long long)(at.g * r.group + (from + row) % r.group) * r.out_head;
+          const int tok = by_group(from + row, r.group);
+          return r.out + (long long)(s.row0 + tok) * r.out_row + (long long)(at.g * r.group + from + row - tok * r.group) * r.out_head;
         };
         if (FP8) {                          // 16 dims of rows 2 lt and 2 lt + 1
 #pragma unroll
