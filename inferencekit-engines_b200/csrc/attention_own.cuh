@@ -137,6 +137,7 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const __grid_constant
 // A sequence's part here: up to OWN_MAX_ROWS query rows per KV head, in blocks of 8 or 16.
 constexpr int OWN_MAX_ROWS = 64;
 constexpr int OWN_MIN_TILES = 1;           // a warp's least share
+constexpr int OWN_UNIT_COST = 2;           // what a unit costs beside its tiles (rows of q, the sums' way out), in tiles
 template <bool FP8, int NT>
 struct OwnShape {
   static constexpr int ROWS = 8 * NT, KEYS = 32;
@@ -206,7 +207,7 @@ struct OwnWalk {
     blocks = (s.n * p.r.group + ROWS - 1) / ROWS;
     n = max(1, (s.len + KEYS - 1) / KEYS);   // (a sequence without a key still has rows to be written)
   }
-  __device__ __forceinline__ long long tiles() const { return (long long)blocks * p.r.c.n_kv * n; }
+  __device__ __forceinline__ long long cost() const { return (long long)blocks * p.r.c.n_kv * (n + OWN_UNIT_COST); }
   __device__ __forceinline__ void next_unit() {   // (there is one)
     t = 0;
     if (++g < p.r.c.n_kv) return;
@@ -270,7 +271,7 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
     __syncwarp();
   }
   long long mine = 0;
-  for (int i = lane * per; i < min(r.c.B, (lane + 1) * per); ++i) mine += Walk(p, kept, i).tiles();
+  for (int i = lane * per; i < min(r.c.B, (lane + 1) * per); ++i) mine += Walk(p, kept, i).cost();
   long long incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -284,14 +285,16 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
   const int owner = __ffs(__ballot_sync(0xffffffffu, incl > u0)) - 1;
   long long start = __shfl_sync(0xffffffffu, incl - mine, owner);
   Walk at(p, kept, owner * per);
-  while (u0 >= start + at.tiles()) {
-    start += at.tiles();
+  while (u0 >= start + at.cost()) {
+    start += at.cost();
     ++at.b;
     at.seq();
   }
+  long long unit0;                          // where the unit begins: its cost, then its tiles
   {
-    const long long unit = (u0 - start) / at.n;
-    at.t = (int)((u0 - start) - unit * at.n);
+    const long long unit = (u0 - start) / (at.n + OWN_UNIT_COST);
+    unit0 = start + unit * (at.n + OWN_UNIT_COST);
+    at.t = max(0, (int)(u0 - unit0) - OWN_UNIT_COST);
     at.block = (int)(unit / r.c.n_kv);
     at.g = (int)(unit - (long long)at.block * r.c.n_kv);
   }
@@ -300,10 +303,11 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
   // ---- loads: S tiles ahead of the products, page numbers 32 boxes at a time ---------------------------------------------------
   Walk ld = at;
   const int RB = min(1 << r.c.page_shift, KEYS), boxes = KEYS / RB, batch = 32 / boxes;
-  long long loaded = u0;
+  long long next = unit0 + OWN_UNIT_COST + at.t;   // where the next tile to load is
+  int loaded = 0;
   int pages = -1, in = batch;               // this lane's box of tile (first of the batch) + lane / boxes; the place in the batch
   auto load = [&]() {                       // the next tile of the range
-    const int st = (int)((loaded - u0) % S);
+    const int st = loaded % S;
     if (in == batch) {
       const int j = (ld.t + lane / boxes) * KEYS + (lane % boxes) * RB;
       pages = -1;
@@ -332,28 +336,31 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
     }
     ++loaded;
     ++in;
-    if (++ld.t == ld.n && loaded < u1) {
-      ld.next_unit();
+    ++next;
+    if (++ld.t == ld.n) {
+      next += OWN_UNIT_COST;
+      if (next < u1) ld.next_unit();
       in = batch;
     }
   };
-  for (int i = 0; i < S && loaded < u1; ++i) load();
+  for (int i = 0; i < S && next < u1; ++i) load();
 
   FewRows<FP8, NT, KEYS / 16> w;
   bool ok = true;
-  for (long long u = u0; u < u1;) {
-    const int n = at.n, t0 = at.t, t1 = (int)min((long long)n, t0 + (u1 - u)), from = at.block * ROWS;
+  for (int it = 0;;) {
+    const int n = at.n, t0 = at.t, t1 = (int)min((long long)n, u1 - unit0 - OWN_UNIT_COST), from = at.block * ROWS;
+    if (t1 <= t0) break;                    // (the range ends before the unit's first tile)
     const OwnSeq s = at.s;
     const int rows = min(ROWS, s.n * r.group - from), first = s.len - s.n + by_group(from, r.group);
     w.begin(r, s.row0, s.n, s.len, from, rows, at.g, lane);
-    for (int t = t0; t < t1; ++t) {
-      const int it = (int)(u - u0) + t - t0, st = it % S;
+    for (int t = t0; t < t1; ++t, ++it) {
+      const int st = it % S;
       ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.full[st], (uint32_t)((it / S) & 1)));
       if (!ok) break;
       if (t * KEYS < s.len)
         w.step(smem_u32(sm.k[st]), smem_u32(sm.v[st]), TILE / 2, sm.ks[FP8 ? st : 0], sm.vs[FP8 ? st : 0], t * KEYS, s.len, first, lane);
       __syncwarp();
-      if (loaded < u1) load();
+      if (next < u1) load();
     }
     if (!ok) break;
     w.finish();
@@ -365,10 +372,10 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
         for (int e = 0; e < 4; ++e) w.o[i][nt][e] *= w.unscale(nt, e & 1);
     const bool whole = t1 - t0 == n;
     if (!whole || s.start) {                // sums, for the merge with the other pieces' and the prefix's
-      const long long unit0 = u - t0;
-      const int cf = owner_of(unit0, W, G), cl = owner_of(unit0 + n - 1, W, G);
-      const int code = whole ? OWN_SUMS : OWN_PIECES | (cf * W / G != unit0 ? 1 << 24 : 0) | cl << 10 | cf;
-      const size_t slot = (size_t)(c * 2 + (u == u0 ? 0 : 1)) * 16;
+      const long long tile0 = unit0 + OWN_UNIT_COST;
+      const int cf = owner_of(tile0, W, G), cl = owner_of(tile0 + n - 1, W, G);
+      const int code = whole ? OWN_SUMS : OWN_PIECES | (cf * W / G < unit0 ? 1 << 24 : 0) | cl << 10 | cf;
+      const size_t slot = (size_t)(c * 2 + (u0 < unit0 ? 1 : 0)) * 16;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -428,13 +435,13 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
         }
       }
     }
-    u += t1 - t0;
-    if (u < u1) at.next_unit();
+    unit0 += n + OWN_UNIT_COST;
+    if (unit0 + OWN_UNIT_COST >= u1) break;
+    at.next_unit();
   }
   if (!ok) {                                // a wait gave up: the copies in flight land before the shared memory goes away
     if (lane == 0) atomicOr(&g_dev_error, DEVERR_MBAR_TIMEOUT);
-    const int it = (int)(loaded - u0);
-    for (int i = max(0, it - S); i < it; ++i) mbar_wait_small(&sm.full[i % S], (uint32_t)((i / S) & 1), 1000000ull);
+    for (int i = max(0, loaded - S); i < loaded; ++i) mbar_wait_small(&sm.full[i % S], (uint32_t)((i / S) & 1), 1000000ull);
   }
 }
 
