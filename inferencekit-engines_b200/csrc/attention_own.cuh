@@ -71,7 +71,7 @@ struct MergeParams {
   int n_q, rows;            // T * n_q
 };
 // Four warps for two rows, whose 16-byte columns lie beside each other in a piece, so that every 32-byte sector is used; each
-// warp takes every fourth part, all of them in flight at once for up to 16.
+// warp takes every fourth part, up to 24 of them on their way at once.
 __global__ void __launch_bounds__(256) prefix_merge_kernel(const __grid_constant__ MergeParams p) {
   __shared__ float4 sum[8][2][32];
   __shared__ float2 sum_ml[8][32];
@@ -97,26 +97,38 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const __grid_constant
     o[0].x = o[0].x * f0 + a.x * f, o[0].y = o[0].y * f0 + a.y * f, o[0].z = o[0].z * f0 + a.z * f, o[0].w = o[0].w * f0 + a.w * f;
     o[1].x = o[1].x * f0 + b.x * f, o[1].y = o[1].y * f0 + b.y * f, o[1].z = o[1].z * f0 + b.z * f, o[1].w = o[1].w * f0 + b.w * f;
   };
-#pragma unroll 4
-  for (int i = quarter; i < parts; i += 4) {
-    const float2* ml;
-    const float* src;
-    int step = 64;                          // to the second 64 dims
-    if (i < own_parts) {
-      const int c = own_first + i;
-      const size_t at_row = (size_t)(c * 2 + (i == 0 ? own >> 24 & 1 : 0)) * 16 + (own >> 20 & 15);
-      ml = own & OWN_SUMS ? x.own_ml + at : x.own_part_ml + at_row;
-      src = (own & OWN_SUMS ? x.own_o + (size_t)at * HEAD_DIM : x.own_part + at_row * HEAD_DIM) + 4 * q0;
-    } else {
-      const int k = i - own_parts, part = k & ((1 << split) - 1), c = first + (k >> split), r = (row & 127) + part * (128 >> split);
-      const size_t slot = ((size_t)(c * 2 + (c == first ? 1 : 0)) * 2 + (row >> 7)) * 128;
-      ml = whole ? x.ml + (size_t)at * 4 + part : reinterpret_cast<const float2*>(x.part_ml) + slot + (r & 127);
-      src = whole ? x.o + ((size_t)at * 4 + part) * HEAD_DIM + 4 * q0 : x.part + slot * 128 + (size_t)q0 * 512 + (r & 127) * 4;
-      if (!whole) step = 16 * 512;
+  constexpr int BATCH = 6;                  // parts of a warp that are on their way at once
+#pragma unroll 1
+  for (int i0 = quarter; i0 < parts; i0 += 4 * BATCH) {
+    float2 v[BATCH];
+    float4 a[BATCH], b[BATCH];
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      const int i = i0 + 4 * j;
+      v[j] = make_float2(-INFINITY, 0.f);
+      if (i >= parts) continue;
+      const float2* ml;
+      const float* src;
+      int step = 64;                        // to the second 64 dims
+      if (i < own_parts) {
+        const int c = own_first + i;
+        const size_t at_row = (size_t)(c * 2 + (i == 0 ? own >> 24 & 1 : 0)) * 16 + (own >> 20 & 15);
+        ml = own & OWN_SUMS ? x.own_ml + at : x.own_part_ml + at_row;
+        src = (own & OWN_SUMS ? x.own_o + (size_t)at * HEAD_DIM : x.own_part + at_row * HEAD_DIM) + 4 * q0;
+      } else {
+        const int k = i - own_parts, part = k & ((1 << split) - 1), c = first + (k >> split), r = (row & 127) + part * (128 >> split);
+        const size_t slot = ((size_t)(c * 2 + (c == first ? 1 : 0)) * 2 + (row >> 7)) * 128;
+        ml = whole ? x.ml + (size_t)at * 4 + part : reinterpret_cast<const float2*>(x.part_ml) + slot + (r & 127);
+        src = whole ? x.o + ((size_t)at * 4 + part) * HEAD_DIM + 4 * q0 : x.part + slot * 128 + (size_t)q0 * 512 + (r & 127) * 4;
+        if (!whole) step = 16 * 512;
+      }
+      v[j] = __ldcg(ml);
+      a[j] = __ldcg(reinterpret_cast<const float4*>(src));
+      b[j] = __ldcg(reinterpret_cast<const float4*>(src + step));
     }
-    const float2 v = __ldcg(ml);
-    const float4 a = __ldcg(reinterpret_cast<const float4*>(src)), b = __ldcg(reinterpret_cast<const float4*>(src + step));
-    add(v, a, b);
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j)
+      if (i0 + 4 * j < parts) add(v[j], a[j], b[j]);
   }
   if (quarter) {
     sum[warp][0][lane] = o[0], sum[warp][1][lane] = o[1];

@@ -300,6 +300,45 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
+// A tile of e4m3 rows to bf16 ones in the image the MMAs read, exactly; 8 threads a row, ROWS rows at a time, from `tail` on zeros.
+// 8 bytes and 8 again: two swizzled 16-byte chunks of a row. Three rows' loads go before their stores: one at a time, each load's
+// latency and each conversion's in turn, a tile took 2,500 cycles of six warps.
+template <int ROWS>
+__device__ __forceinline__ void tca_convert(uint32_t src, uint32_t dst, int th, int tail) {
+  const int ch = th & 7, half = ch >> 2;    // this thread's 16 dims
+#pragma unroll
+  for (int k0 = 0; k0 * ROWS < TCA_KEYS; k0 += 3) {
+    uint2 q[3][2];
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {         // the second half's lanes begin with their other chunk: no bank conflict
+        const int row = (k0 + k) * ROWS + (th >> 3);
+        if ((k0 + k) * ROWS < TCA_KEYS && row < TCA_KEYS)
+          asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(q[k][j].x), "=r"(q[k][j].y) : "r"(src + row * HEAD_DIM + ch * 16 + (j ^ half) * 8));
+      }
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = (k0 + k) * ROWS + (th >> 3);
+        if ((k0 + k) * ROWS >= TCA_KEYS || row >= TCA_KEYS) break;
+        uint32_t y[4];
+#pragma unroll
+        for (int i2 = 0; i2 < 4; ++i2) {
+          const uint32_t h = e4m3x2_to_f16x2((i2 < 2 ? q[k][j].x : q[k][j].y) >> (16 * (i2 & 1)));
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+          y[i2] = pack_bf16(f.x, f.y);
+        }
+        if (row >= tail) y[0] = y[1] = y[2] = y[3] = 0;
+        const int c16 = ((ch & 3) * 2 + (j ^ half)) ^ (row & 7);
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + half * (TCA_TILE / 2) + row * 128 + c16 * 16), "r"(y[0]), "r"(y[1]),
+                     "r"(y[2]), "r"(y[3])
+                     : "memory");
+      }
+  }
+}
+
 // A prefix with few rows: a tile's four warps of 32 rows hold them 2 or 4 times (`parts`), each part for its own half or quarter of
 // every key tile. What a tile costs then is the chain from its scores to its product with V, and a thread's 128 exponentials
 // are the longest part of that: 128 / parts remain (and zeros for the other parts' keys).
@@ -376,13 +415,13 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
     mbar_init(&sm.q_full, 1);
     mbar_init(&sm.q_empty, 1);
     for (int i = 0; i < TCA_STAGES; ++i) {
-      mbar_init(&sm.full[i], FP8 ? 6 : 1);    // the converting warps; the copies
+      mbar_init(&sm.full[i], !FP8 ? 1 : MODE == TC_PREFIX ? 10 : 6);   // the copies; the converting warps
       mbar_init(&sm.empty[i], FP8 ? 1 : 2);   // the MMAs; they and the V cleaner
       mbar_init(&sm.v_clean[i], 1);
     }
     for (int i = 0; i < RAW; ++i) {
       mbar_init(&sm.raw_full[i], 1);
-      mbar_init(&sm.raw_empty[i], 6);
+      mbar_init(&sm.raw_empty[i], MODE == TC_PREFIX ? 10 : 6);
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&sm.s_full[x], 1);
@@ -645,7 +684,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         }
     } else if (FP8 && work) {   // ---- warps 10 to 15: e4m3 tiles to bf16 ones (exact), and their rows' scales ----
       Walk w(p, sm, step);
-      const int th = tid - 320, ch = th & 7, half = ch >> 2;   // this thread's 16 dims, of every 24th row
+      const int th = tid - 320;
       // the scales of key th of tile t: fetched a tile ahead, and the number of the page that they are in two
       auto page_of = [&](int t) {
         const int j = t * TCA_KEYS + th;
@@ -685,44 +724,15 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
             else sm.k_scale[FP8 ? (it >> 1) % 3 : 0][FP8 ? th : 0] = scales.x;
           }
           if (is_v) scales = ahead;
-          // 8 bytes and 8 again: two swizzled 16-byte chunks of a row. Three rows' loads before their stores: one at a time a
-          // tile took 2,500 cycles, each load's latency and each conversion's in turn
-#pragma unroll
-          for (int k0 = 0; k0 < 6; k0 += 3) {
-            uint2 q[3][2];
-#pragma unroll
-            for (int k = 0; k < 3; ++k)
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {   // the second half's lanes begin with their other chunk: no bank conflict
-                const int row = (k0 + k) * 24 + (th >> 3);
-                if (row < TCA_KEYS)
-                  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(q[k][j].x), "=r"(q[k][j].y) : "r"(src + row * HEAD_DIM + ch * 16 + (j ^ half) * 8));
-              }
-#pragma unroll
-            for (int k = 0; k < 3; ++k)
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const int row = (k0 + k) * 24 + (th >> 3);
-                if (row >= TCA_KEYS) break;
-                uint32_t y[4];
-#pragma unroll
-                for (int i2 = 0; i2 < 4; ++i2) {
-                  const uint32_t h = e4m3x2_to_f16x2((i2 < 2 ? q[k][j].x : q[k][j].y) >> (16 * (i2 & 1)));
-                  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-                  y[i2] = pack_bf16(f.x, f.y);
-                }
-                if (row >= tail) y[0] = y[1] = y[2] = y[3] = 0;
-                const int c16 = ((ch & 3) * 2 + (j ^ half)) ^ (row & 7);
-                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + half * (TCA_TILE / 2) + row * 128 + c16 * 16), "r"(y[0]), "r"(y[1]),
-                             "r"(y[2]), "r"(y[3])
-                             : "memory");
-              }
-          }
+          const bool ten = MODE == TC_PREFIX && prefix_parts(w.s.n, tpq) > 1;
+          if (ten) tca_convert<40>(src, dst, th, TCA_KEYS);
+          else tca_convert<24>(src, dst, th, tail);
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&sm.full[st]);
-            mbar_arrive(&sm.raw_empty[rs]);
+          if (lane == 0) {                    // (a prefix's barriers wait for ten warps)
+            const uint32_t n = MODE == TC_PREFIX && !ten && warp == 10 ? 5 : 1;
+            mbar_arrive_n(&sm.full[st], n);
+            mbar_arrive_n(&sm.raw_empty[rs], n);
           }
         }
       }
@@ -743,7 +753,22 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         const bool valid = (MODE == TC_PREFIX ? own < tpq : row < (step / 2) * r.group) && tok < w.s.n;
         const int first = MODE == TC_PREFIX ? w.s.len - 1 : w.s.len - w.s.n + w.tok0(x);   // the last key that the tile's first row sees
         float m = -INFINITY, l = 0.f, base = 0.f;   // base = -m * sl2 - TCA_SHIFT
-        if (MODE == TC_PREFIX && parts > 1) {
+        if (FP8 && MODE == TC_PREFIX && parts > 1 && x == 1) {   // no rows here: a third of the tiles' conversion
+          for (uint32_t it = 2 * kt; it < (uint32_t)(2 * (kt + w.t1 - w.t0)); ++it) {
+            const uint32_t rs = it % RAW, st = it % TCA_STAGES;
+            ok = ok && mbar_wait_small(&sm.raw_full[rs], (it / RAW) & 1);
+            if (it >= TCA_STAGES) ok = ok && mbar_wait_small(&sm.empty[st], (it / TCA_STAGES - 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tca_convert<40>(smem_u32(sm.raw[FP8 ? rs : 0]), smem_u32(sm.kv[st]), 192 + row, TCA_KEYS);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(&sm.full[st]);
+              mbar_arrive(&sm.raw_empty[rs]);
+            }
+          }
+        } else if (MODE == TC_PREFIX && parts > 1) {
           auto tiles = [&](auto n_parts) {
             constexpr int N = 128 / decltype(n_parts)::value;   // keys of a tile that are this part's: from k0 on
             const int part = (warp & 3) / per, k0 = part * N;
