@@ -300,29 +300,30 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
-// A tile of e4m3 rows to bf16 ones in the image the MMAs read, exactly; 8 threads a row, ROWS rows at a time, from `tail` on zeros.
+// Rows FIRST to LAST - 1 of a tile of e4m3 rows to bf16 ones in the image the MMAs read, exactly; 8 threads a row, ROWS rows at a
+// time, from `tail` on zeros.
 // 8 bytes and 8 again: two swizzled 16-byte chunks of a row. Three rows' loads go before their stores: one at a time, each load's
 // latency and each conversion's in turn, a tile took 2,500 cycles of six warps.
-template <int ROWS>
+template <int ROWS, int FIRST, int LAST>
 __device__ __forceinline__ void tca_convert(uint32_t src, uint32_t dst, int th, int tail) {
   const int ch = th & 7, half = ch >> 2;    // this thread's 16 dims
 #pragma unroll
-  for (int k0 = 0; k0 * ROWS < TCA_KEYS; k0 += 3) {
+  for (int k0 = 0; FIRST + k0 * ROWS < LAST; k0 += 3) {
     uint2 q[3][2];
 #pragma unroll
     for (int k = 0; k < 3; ++k)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {         // the second half's lanes begin with their other chunk: no bank conflict
-        const int row = (k0 + k) * ROWS + (th >> 3);
-        if ((k0 + k) * ROWS < TCA_KEYS && row < TCA_KEYS)
+        const int row = FIRST + (k0 + k) * ROWS + (th >> 3);
+        if (FIRST + (k0 + k) * ROWS < LAST && row < LAST)
           asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(q[k][j].x), "=r"(q[k][j].y) : "r"(src + row * HEAD_DIM + ch * 16 + (j ^ half) * 8));
       }
 #pragma unroll
     for (int k = 0; k < 3; ++k)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int row = (k0 + k) * ROWS + (th >> 3);
-        if ((k0 + k) * ROWS >= TCA_KEYS || row >= TCA_KEYS) break;
+        const int row = FIRST + (k0 + k) * ROWS + (th >> 3);
+        if (FIRST + (k0 + k) * ROWS >= LAST || row >= LAST) break;
         uint32_t y[4];
 #pragma unroll
         for (int i2 = 0; i2 < 4; ++i2) {
@@ -725,8 +726,8 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
           }
           if (is_v) scales = ahead;
           const bool ten = MODE == TC_PREFIX && prefix_parts(w.s.n, tpq) > 1;
-          if (ten) tca_convert<40>(src, dst, th, TCA_KEYS);
-          else tca_convert<24>(src, dst, th, tail);
+          if (ten) tca_convert<24, 80, TCA_KEYS>(src, dst, th, TCA_KEYS);
+          else tca_convert<24, 0, TCA_KEYS>(src, dst, th, tail);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {                    // (a prefix's barriers wait for ten warps)
@@ -753,14 +754,14 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         const bool valid = (MODE == TC_PREFIX ? own < tpq : row < (step / 2) * r.group) && tok < w.s.n;
         const int first = MODE == TC_PREFIX ? w.s.len - 1 : w.s.len - w.s.n + w.tok0(x);   // the last key that the tile's first row sees
         float m = -INFINITY, l = 0.f, base = 0.f;   // base = -m * sl2 - TCA_SHIFT
-        if (FP8 && MODE == TC_PREFIX && parts > 1 && x == 1) {   // no rows here: a third of the tiles' conversion
+        if (FP8 && MODE == TC_PREFIX && parts > 1 && x == 1) {   // no rows here: most of the tiles' conversion
           for (uint32_t it = 2 * kt; it < (uint32_t)(2 * (kt + w.t1 - w.t0)); ++it) {
             const uint32_t rs = it % RAW, st = it % TCA_STAGES;
             ok = ok && mbar_wait_small(&sm.raw_full[rs], (it / RAW) & 1);
             if (it >= TCA_STAGES) ok = ok && mbar_wait_small(&sm.empty[st], (it / TCA_STAGES - 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            tca_convert<40>(smem_u32(sm.raw[FP8 ? rs : 0]), smem_u32(sm.kv[st]), 192 + row, TCA_KEYS);
+            tca_convert<16, 0, 80>(smem_u32(sm.raw[FP8 ? rs : 0]), smem_u32(sm.kv[st]), row, TCA_KEYS);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
