@@ -38,7 +38,11 @@ constexpr int PREFIX_WHOLE = 1 << 26, PREFIX_PIECES = 1 << 27;
 // second piece (24), and one of these. 0: the output is written.
 constexpr int OWN_SUMS = 1 << 25, OWN_PIECES = 1 << 26;
 constexpr int SHARED_TILE = 128;      // a prefix is cut to whole key tiles: what is left of it is read with a sequence's own keys
-constexpr int SHARED_MIN_KEYS = 256;  // shorter ones too
+// Sharing pays where it saves so many reads of a key (for one KV head) in all: the prefixes' launch and the merge of their sums take
+// some 10 us, and a shared page that is read again comes out of the L2 cache. A group by itself is held against its part of them.
+// Measured, shared against not: 4 sequences behind 8,192 keys (197,000 reads) 38 us against 29; 16 behind 2,048 (246,000) 25 against 27;
+// 64 behind 512 (258,000) 33 against 32; 8 groups of 8 behind 512 (229,000) 31 against 33, behind 1,024 38 against 47; e4m3 pages alike.
+constexpr long long SHARED_MIN_READS = 240000;
 struct SharedGroup {
   int first, end, keys;               // its sequences; the keys that are read once
 };
@@ -46,7 +50,9 @@ __device__ __forceinline__ SharedGroup shared_group(const SharedParams& x, const
   SharedGroup s = {__ldg(x.groups + g), __ldg(x.groups + g + 1), __ldg(x.shared + g)};
   const bool bad = s.first < 0 || s.end < s.first || s.end > c.B || s.keys < 0 || s.keys > (long long)c.table_width << c.page_shift;
   if (bad) atomicOr(&g_dev_error, DEVERR_BAD_STATE);
-  s.keys = bad || s.end - s.first < 2 || s.keys < SHARED_MIN_KEYS ? 0 : s.keys / SHARED_TILE * SHARED_TILE;
+  s.keys = bad ? 0 : s.keys / SHARED_TILE * SHARED_TILE;
+  const long long saved = (long long)(s.end - s.first - 1) * s.keys * c.n_kv;
+  if (saved <= 0 || saved * x.G < SHARED_MIN_READS) s.keys = 0;
   return s;
 }
 // The keys of sequence b that its group's prefix has.

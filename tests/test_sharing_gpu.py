@@ -411,6 +411,9 @@ SHARED = {   # members and prefix of each group (prefix None: its sequences are 
     "long": ([(3, 20480), (2, 8192)], [1], [77, 1500], 8, 2, 64),
     "many_groups": ([(2, 128 * (i % 4)) for i in range(60)], [1], [5, 18, 140], 8, 2, 16),
     "no_tokens": ([(4, 512)], [1, 0], [20], 32, 8, 16),
+    "two_quarters": ([(13, 512), (9, 256)], [1], [3, 90], 32, 8, 32),
+    "large": ([(30, 1280), (2, 1024), (17, 2048)], [1], [33, 1], 32, 8, 64),
+    "large_drafts": ([(20, 2048), (11, 3968)], [4, 1, 3], [33, 6], 32, 8, 32),
 }
 
 
@@ -445,10 +448,21 @@ def shared_case(name, fp8, seed=0):
     return dict(c, table=table, q=q, n=n, lens=lens, cu=cumulative(n), groups=groups, shared=shared, rows=full, page=page)
 
 
+def all_shared(s, n_kv):
+    """The case's groups, and empty ones behind them: what sharing has to save is a group's part of a sum over the groups, so
+    with enough of them every prefix of 128 keys or more is read once."""
+    saved = [(b - a - 1) * (keys // 128 * 128) * n_kv for a, b, keys in zip(s["groups"], s["groups"][1:], s["shared"])]
+    n = -(-240_001 // min([x for x in saved if x > 0] or [1 << 20]))
+    return s["groups"] + [len(s["n"])] * n, s["shared"] + [0] * n
+
+
+@pytest.mark.parametrize("every", [False, True], ids=["large_ones", "every_prefix"])
 @pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "e4m3"])
 @pytest.mark.parametrize("name", SHARED)
-def test_shared_attention(name, fp8):
+def test_shared_attention(name, fp8, every):
     s = shared_case(name, fp8)
+    if every:
+        s["groups"], s["shared"] = all_shared(s, SHARED[name][4])
     out = torch.full_like(s["q"], 3.0)
     k = ops()
     k.device_error()
