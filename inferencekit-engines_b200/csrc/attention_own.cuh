@@ -8,7 +8,8 @@
 //    pages, rows of q, the first tile, the sums' way out). So a warp is a CTA of its own here, with a ring of its own: six on an SM
 //    hide each other's chains. (The few-row kernel, whose eight warps take each unit together: 40 us for 64 sequences of up to
 //    500 keys and 8 KV heads out of a cold cache, against XX.)
-//  * the prefixes (attention_tc.cuh): a group's rows, as one sequence's, over the keys they share, read once;
+//    Prefixes of groups with few query rows are sequences like these, in blocks of 16 rows.
+//  * the prefixes of larger groups (attention_tc.cuh): a group's rows, as one sequence's, over the keys they share, read once;
 //  * prefix_merge_kernel: a row's sums over its own keys and its prefix, in pieces where CTAs or warps shared them out, become the output.
 #pragma once
 #include "attention_few.cuh"
@@ -33,30 +34,57 @@ struct SharedParams {
 };
 // info: the CTAs first .. last that have pieces (bits 0-7 and 8-15; the first one's second piece, the others' first), the row of a
 // tile pair that has the row's first part (16-23), parts as a power of two (24-25), and one of these. 0: nothing.
-constexpr int PREFIX_WHOLE = 1 << 26, PREFIX_PIECES = 1 << 27;
+constexpr int PREFIX_WHOLE = 1 << 26, PREFIX_PIECES = 1 << 27, PREFIX_WARPS = 1 << 28;   // the last: the rest is as in own_info
 // own_info: the warps first .. last that have pieces (0-9 and 10-19), the row of the block (20-23), whether the first one's is its
 // second piece (24), and one of these. 0: the output is written.
 constexpr int OWN_SUMS = 1 << 25, OWN_PIECES = 1 << 26;
 constexpr int SHARED_TILE = 128;      // a prefix is cut to whole key tiles: what is left of it is read with a sequence's own keys
-// Sharing pays where it saves so many reads of a key (for one KV head) in all: the prefixes' launch and the merge of their sums take
-// some 10 us, and a shared page that is read again comes out of the L2 cache. A group by itself is held against its part of them.
-// Measured, shared against not: 4 sequences behind 8,192 keys (197,000 reads) 38 us against 29; 16 behind 2,048 (246,000) 25 against 27;
-// 64 behind 512 (258,000) 33 against 32; 8 groups of 8 behind 512 (229,000) 31 against 33, behind 1,024 38 against 47; e4m3 pages alike.
+constexpr int SHARED_MIN_KEYS = 256;  // shorter ones too
+// The tensor cores' launch pays where it saves so many reads of a key (for one KV head) in all: it and the merge of its sums take some
+// 10 us, and a shared page that is read again comes out of the L2 cache. Measured, shared against not: 16 sequences behind
+// 2,048 keys (246,000 reads) 25 us against 27; 64 behind 512 (258,000) 33 against 32; 8 groups of 8 behind 512 (229,000) 31
+// against 33, behind 1,024 38 against 47; e4m3 pages alike.
 constexpr long long SHARED_MIN_READS = 240000;
+// A prefix that the warps take is read once for every 16 rows (the second time out of the L2 cache): those of one block of rows, and of
+// up to four where that is few reads in all. Measured, warps against tensor cores: 8 sequences behind 4,096 keys (65,000 reads) 25 us against
+// 33, 16 (131,000) 27 against 31, 8 groups of 8 (524,000) 71 against 59, 8 of 4 (one block) 48 against 55.
+constexpr long long OWN_PREFIX_READS = 200000;
 struct SharedGroup {
   int first, end, keys;               // its sequences; the keys that are read once
+  int row0, n;                        // their rows
+  bool warps;                         // whether the prefix is the warps'
 };
-__device__ __forceinline__ SharedGroup shared_group(const SharedParams& x, const PagedCache& c, int g) {
-  SharedGroup s = {__ldg(x.groups + g), __ldg(x.groups + g + 1), __ldg(x.shared + g)};
-  const bool bad = s.first < 0 || s.end < s.first || s.end > c.B || s.keys < 0 || s.keys > (long long)c.table_width << c.page_shift;
+// `large`: whether prefixes that are not the warps' are shared at all.
+__device__ __forceinline__ SharedGroup shared_group(const SharedParams& x, const RaggedParams& r, int g, bool large) {
+  const PagedCache& c = r.c;
+  SharedGroup s = {__ldg(x.groups + g), __ldg(x.groups + g + 1), __ldg(x.shared + g), 0, 0, false};
+  bool bad = s.first < 0 || s.end < s.first || s.end > c.B || s.keys < 0 || s.keys > (long long)c.table_width << c.page_shift;
+  s.keys = bad || s.end - s.first < 2 || s.keys < SHARED_MIN_KEYS ? 0 : s.keys / SHARED_TILE * SHARED_TILE;
+  if (s.keys) {
+    s.row0 = __ldg(c.cu + s.first);
+    s.n = __ldg(c.cu + s.end) - s.row0;
+    if (s.row0 < 0 || s.n < 0 || s.n > r.T - s.row0) bad = true, s.keys = s.n = 0;
+    const int blocks = (s.n * r.group + 15) / 16;
+    s.warps = blocks <= 1 || (blocks <= 4 && (long long)blocks * s.keys * c.n_kv * x.G <= OWN_PREFIX_READS);
+    if (!s.warps && !large) s.keys = 0;
+  }
   if (bad) atomicOr(&g_dev_error, DEVERR_BAD_STATE);
-  s.keys = bad ? 0 : s.keys / SHARED_TILE * SHARED_TILE;
-  const long long saved = (long long)(s.end - s.first - 1) * s.keys * c.n_kv;
-  if (saved <= 0 || saved * x.G < SHARED_MIN_READS) s.keys = 0;
   return s;
 }
+// Whether what the large prefixes save is worth their launch; a whole warp.
+__device__ __forceinline__ bool large_prefixes(const SharedParams& x, const RaggedParams& r, int lane) {
+  long long reads = 0;
+  for (int g = lane; g < x.G; g += 32) {
+    const SharedGroup s = shared_group(x, r, g, true);
+    if (s.keys && !s.warps)                 // (a sequence's own keys are read once for each 16 of its rows)
+      reads += (long long)(max(s.end - s.first, s.n * r.group / 16) - 1) * s.keys * r.c.n_kv;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) reads += __shfl_xor_sync(0xffffffffu, reads, o);
+  return reads >= SHARED_MIN_READS;
+}
 // The keys of sequence b that its group's prefix has.
-__device__ __forceinline__ int shared_keys(const SharedParams& x, const PagedCache& c, int b) {
+__device__ __forceinline__ int shared_keys(const SharedParams& x, const RaggedParams& r, int b, bool large) {
   int lo = 0, hi = x.G;                // the group: the last one that begins at or before b
   if (hi == 0) return 0;
   while (hi - lo > 1) {
@@ -64,7 +92,7 @@ __device__ __forceinline__ int shared_keys(const SharedParams& x, const PagedCac
     if (__ldg(x.groups + mid) <= b) lo = mid;
     else hi = mid;
   }
-  const SharedGroup s = shared_group(x, c, lo);
+  const SharedGroup s = shared_group(x, r, lo, large);
   return s.first <= b && b < s.end ? s.keys : 0;
 }
 
@@ -88,11 +116,21 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const __grid_constant
   grid_dep_launch();
   const int info = at < p.rows ? __ldcg(x.info + at) : 0, own = at < p.rows ? __ldcg(x.own_info + at) : 0;
   if (__syncthreads_or(info | own) == 0) return;
-  const bool whole = info & PREFIX_WHOLE;
+  const bool whole = info & PREFIX_WHOLE && !(info & PREFIX_WARPS);
   const int split = info >> 24 & 3, first = min(info & 255, 159), last = min(info >> 8 & 255, 159), row = info >> 16 & 255;
-  const int own_first = min(own & 1023, OWN_MAX_GRID - 1), own_last = min(own >> 10 & 1023, OWN_MAX_GRID - 1);
-  const int own_parts = own & OWN_SUMS ? 1 : own & OWN_PIECES ? own_last - own_first + 1 : 0;
-  const int parts = own_parts + (info == 0 ? 0 : (whole ? 1 : last - first + 1) << split);
+  // what warps left: the own keys' sums, or pieces; a prefix's likewise
+  struct Warps {
+    int first, parts, code;
+  };
+  auto warps_of = [&](int code) {
+    Warps w = {min(code & 1023, OWN_MAX_GRID - 1), 0, code};
+    w.parts = code & OWN_SUMS ? 1 : code & OWN_PIECES ? max(0, min(code >> 10 & 1023, OWN_MAX_GRID - 1) - w.first + 1) : 0;
+    return w;
+  };
+  const bool prefix_by_warps = info & PREFIX_WARPS;
+  const Warps w_own = warps_of(own), w_pre = warps_of(prefix_by_warps ? info & (PREFIX_WARPS - 1) : 0);
+  const int by_warp = w_own.parts + w_pre.parts;
+  const int parts = by_warp + (info == 0 || prefix_by_warps ? 0 : (whole ? 1 : last - first + 1) << split);
   float M = -INFINITY, L = 0.f;
   float4 o[2] = {};
   auto add = [&](float2 v, float4 a, float4 b) {
@@ -116,13 +154,16 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const __grid_constant
       const float2* ml;
       const float* src;
       int step = 64;                        // to the second 64 dims
-      if (i < own_parts) {
-        const int c = own_first + i;
-        const size_t at_row = (size_t)(c * 2 + (i == 0 ? own >> 24 & 1 : 0)) * 16 + (own >> 20 & 15);
-        ml = own & OWN_SUMS ? x.own_ml + at : x.own_part_ml + at_row;
-        src = (own & OWN_SUMS ? x.own_o + (size_t)at * HEAD_DIM : x.own_part + at_row * HEAD_DIM) + 4 * q0;
+      if (i < by_warp) {
+        const bool pre = i >= w_own.parts;
+        const Warps& w = pre ? w_pre : w_own;
+        const int k = pre ? i - w_own.parts : i;
+        const size_t at_row = (size_t)((w.first + k) * 2 + (k == 0 ? w.code >> 24 & 1 : 0)) * 16 + (w.code >> 20 & 15);
+        const bool sums = w.code & OWN_SUMS;
+        ml = !sums ? x.own_part_ml + at_row : pre ? x.ml + (size_t)at * 4 : x.own_ml + at;
+        src = (!sums ? x.own_part + at_row * HEAD_DIM : pre ? x.o + (size_t)at * 4 * HEAD_DIM : x.own_o + (size_t)at * HEAD_DIM) + 4 * q0;
       } else {
-        const int k = i - own_parts, part = k & ((1 << split) - 1), c = first + (k >> split), r = (row & 127) + part * (128 >> split);
+        const int k = i - by_warp, part = k & ((1 << split) - 1), c = first + (k >> split), r = (row & 127) + part * (128 >> split);
         const size_t slot = ((size_t)(c * 2 + (c == first ? 1 : 0)) * 2 + (row >> 7)) * 128;
         ml = whole ? x.ml + (size_t)at * 4 + part : reinterpret_cast<const float2*>(x.part_ml) + slot + (r & 127);
         src = whole ? x.o + ((size_t)at * 4 + part) * HEAD_DIM + 4 * q0 : x.part + slot * 128 + (size_t)q0 * 512 + (r & 127) * 4;
@@ -173,7 +214,7 @@ struct OwnSmem {
   float ks[FP8 ? Sh::S : 1][Sh::KEYS], vs[FP8 ? Sh::S : 1][Sh::KEYS];
   uint64_t full[Sh::S];
   int4 seq[OWN_KEPT];        // OwnSeq
-  int4 group[OWN_KEPT_GROUPS];   // SharedGroup
+  int4 group[OWN_KEPT_GROUPS], prefix[OWN_KEPT_GROUPS];   // its sequences and keys; OwnSeq
 };
 
 struct OwnParams {
@@ -184,7 +225,7 @@ struct OwnParams {
 };
 
 struct OwnSeq {
-  int row0, n, len, start;  // token rows (n 0: not this kernel's), own keys, keys of the prefix before them
+  int row0, n, len, start;  // token rows (n 0: not this kernel's), own keys, keys of the prefix before them (-1 - table row: a prefix)
 };
 // Of sequence b, with row0 = cu[b], end = cu[b + 1], len and its group's keys
 __device__ __forceinline__ OwnSeq own_seq(const OwnParams& p, int row0, int end, int len, int keys) {
@@ -204,23 +245,30 @@ __device__ __forceinline__ OwnSeq own_seq(const OwnParams& p, int row0, int end,
   if (wrong) atomicOr(&g_dev_error, DEVERR_BAD_STATE);
   return s;
 }
-__device__ __forceinline__ OwnSeq own_seq(const OwnParams& p, int b) {
-  return own_seq(p, __ldg(p.r.c.cu + b), __ldg(p.r.c.cu + b + 1), __ldg(p.r.c.seq_lens + b), shared_keys(p.x, p.r.c, b));
+__device__ __forceinline__ OwnSeq own_seq(const OwnParams& p, int b, bool large) {
+  return own_seq(p, __ldg(p.r.c.cu + b), __ldg(p.r.c.cu + b + 1), __ldg(p.r.c.seq_lens + b), shared_keys(p.x, p.r, b, large));
+}
+// A group's prefix as a sequence: every row sees all of its keys.
+__device__ __forceinline__ OwnSeq own_prefix(const SharedGroup& g) {
+  return {g.row0, g.keys && g.warps ? g.n : 0, g.keys, -1 - g.first};
 }
 // The walk over a warp's range of tiles: sequences, their blocks of rows, KV heads, tiles of 32 keys.
 template <int ROWS, int KEYS>
 struct OwnWalk {
   const OwnParams& p;
-  const int4* kept;                         // sequences in shared memory, or null
+  const int4 *kept, *kept_prefix;           // sequences and prefixes in shared memory, or null
+  bool large;                               // large_prefixes
   OwnSeq s;
   int b, block, g, t, n, blocks;            // t: the next tile of the unit's n
-  __device__ __forceinline__ OwnWalk(const OwnParams& p_, const int4* kept_, int b_) : p(p_), kept(kept_), b(b_), block(0), g(0), t(0) { seq(); }
+  __device__ __forceinline__ OwnWalk(const OwnParams& p_, const int4* kept_, const int4* prefix_, bool large_, int b_)
+      : p(p_), kept(kept_), kept_prefix(prefix_), large(large_), b(b_), block(0), g(0), t(0) { seq(); }
   __device__ __forceinline__ void seq() {
+    const int g = b - p.r.c.B;              // the prefixes come behind the sequences
     if (kept) {
-      const int4 v = kept[b];
+      const int4 v = g < 0 ? kept[b] : kept_prefix[g];
       s = {v.x, v.y, v.z, v.w};
     } else {
-      s = own_seq(p, b);
+      s = g < 0 ? own_seq(p, b, large) : own_prefix(shared_group(p.x, p.r, g, large));
     }
     blocks = (s.n * p.r.group + ROWS - 1) / ROWS;
     n = max(1, (s.len + KEYS - 1) / KEYS);   // (a sequence without a key still has rows to be written)
@@ -257,8 +305,9 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
   grid_dep_wait();
   grid_dep_launch();
   // ---- this warp's range: the total, then the sequence its first tile lies in -------------------------------------------------
-  const int per = (r.c.B + 31) / 32;
+  const int seqs = r.c.B + p.x.G, per = (seqs + 31) / 32;
   const int4* kept = r.c.B <= OWN_KEPT && p.x.G <= OWN_KEPT_GROUPS ? sm.seq : nullptr;
+  bool large = false;
   if (kept) {
     int row0[OWN_KEPT / 32], end[OWN_KEPT / 32], len[OWN_KEPT / 32];
 #pragma unroll
@@ -267,9 +316,12 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
       row0[i] = end[i] = len[i] = 0;
       if (b < r.c.B) row0[i] = __ldg(r.c.cu + b), end[i] = __ldg(r.c.cu + b + 1), len[i] = __ldg(r.c.seq_lens + b);
     }
+    large = large_prefixes(p.x, r, lane);
     if (lane < p.x.G) {
-      const SharedGroup g = shared_group(p.x, r.c, lane);
+      const SharedGroup g = shared_group(p.x, r, lane, large);   // (the loads are in the L1 cache by now)
+      const OwnSeq s = own_prefix(g);
       sm.group[lane] = make_int4(g.first, g.end, g.keys, 0);
+      sm.prefix[lane] = make_int4(s.row0, s.n, s.len, s.start);
     }
     __syncwarp();
 #pragma unroll
@@ -288,8 +340,9 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
     }
     __syncwarp();
   }
+  if (!kept) large = large_prefixes(p.x, r, lane);
   long long mine = 0;
-  for (int i = lane * per; i < min(r.c.B, (lane + 1) * per); ++i) mine += Walk(p, kept, i).cost();
+  for (int i = lane * per; i < min(seqs, (lane + 1) * per); ++i) mine += Walk(p, kept, sm.prefix, large, i).cost();
   long long incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -302,7 +355,7 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
   const long long u0 = c * W / G, u1 = (c + 1) * W / G;
   const int owner = __ffs(__ballot_sync(0xffffffffu, incl > u0)) - 1;
   long long start = __shfl_sync(0xffffffffu, incl - mine, owner);
-  Walk at(p, kept, owner * per);
+  Walk at(p, kept, sm.prefix, large, owner * per);
   while (u0 >= start + at.cost()) {
     start += at.cost();
     ++at.b;
@@ -330,7 +383,8 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
       const int j = (ld.t + lane / boxes) * KEYS + (lane % boxes) * RB;
       pages = -1;
       if (j < ld.s.len) {
-        pages = __ldg(r.c.table + (size_t)ld.b * r.c.table_stride + ((j + ld.s.start) >> r.c.page_shift));
+        const int start = ld.s.start;
+        pages = __ldg(r.c.table + (size_t)(start < 0 ? -1 - start : ld.b) * r.c.table_stride + ((j + max(start, 0)) >> r.c.page_shift));
         if (pages < 0 || pages >= r.c.n_pages) {
           atomicOr(&g_dev_error, DEVERR_BAD_STATE);
           pages = 0;
@@ -369,8 +423,10 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
     const int n = at.n, t0 = at.t, t1 = (int)min((long long)n, u1 - unit0 - OWN_UNIT_COST), from = at.block * ROWS;
     if (t1 <= t0) break;                    // (the range ends before the unit's first tile)
     const OwnSeq s = at.s;
-    const int rows = min(ROWS, s.n * r.group - from), first = s.len - s.n + by_group(from, r.group);
-    w.begin(r, s.row0, s.n, s.len, from, rows, at.g, lane);
+    const bool prefix = s.start < 0;
+    const int after = prefix ? 1 : s.n;     // tokens that do not see all of the keys, and the last one
+    const int rows = min(ROWS, s.n * r.group - from), first = s.len - after + by_group(from, r.group);
+    w.begin(r, s.row0, after, s.len, from, rows, at.g, lane);
     for (int t = t0; t < t1; ++t, ++it) {
       const int st = it % S;
       ok = __all_sync(0xffffffffu, ok && mbar_wait_small(&sm.full[st], (uint32_t)((it / S) & 1)));
@@ -389,7 +445,7 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
 #pragma unroll
         for (int e = 0; e < 4; ++e) w.o[i][nt][e] *= w.unscale(nt, e & 1);
     const bool whole = t1 - t0 == n;
-    if (!whole || s.start) {                // sums, for the merge with the other pieces' and the prefix's
+    if (!whole || s.start) {                // sums, for the merge with other pieces' and the prefix's, or the own keys'
       const long long tile0 = unit0 + OWN_UNIT_COST;
       const int cf = owner_of(tile0, W, G), cl = owner_of(tile0 + n - 1, W, G);
       const int code = whole ? OWN_SUMS : OWN_PIECES | (cf * W / G < unit0 ? 1 << 24 : 0) | cl << 10 | cf;
@@ -402,10 +458,10 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
           if (row >= rows) continue;
           const int sum_at = (s.row0 + by_group(from + row, r.group)) * r.n_q + at.g * r.group + from + row - by_group(from + row, r.group) * r.group;
           if (lg == 0) {
-            *(whole ? p.x.own_ml + sum_at : p.x.own_part_ml + slot + row) = make_float2(w.m[nt][e], w.l[nt][e]);
-            if (t0 == 0) p.x.own_info[sum_at] = code | row << 20;
+            *(!whole ? p.x.own_part_ml + slot + row : prefix ? p.x.ml + (size_t)sum_at * 4 : p.x.own_ml + sum_at) = make_float2(w.m[nt][e], w.l[nt][e]);
+            if (t0 == 0) *(prefix ? p.x.info + sum_at : p.x.own_info + sum_at) = code | row << 20 | (prefix ? PREFIX_WARPS : 0);
           }
-          float* dst = whole ? p.x.own_o + (size_t)sum_at * HEAD_DIM : p.x.own_part + (slot + row) * HEAD_DIM;
+          float* dst = !whole ? p.x.own_part + (slot + row) * HEAD_DIM : prefix ? p.x.o + (size_t)sum_at * 4 * HEAD_DIM : p.x.own_o + (size_t)sum_at * HEAD_DIM;
 #pragma unroll
           for (int i = 0; i < 8; i += 2) {
             if (FP8) {                      // 16 dims in a row

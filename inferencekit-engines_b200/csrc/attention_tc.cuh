@@ -73,23 +73,17 @@ struct TcSeq {
   int table, start;         // the row of the block table; keys before these that a shared prefix has
 };
 template <int SRC, int MODE>
-__device__ __forceinline__ TcSeq tc_seq(const TcAttnParams& p, int b) {
+__device__ __forceinline__ TcSeq tc_seq(const TcAttnParams& p, int b, bool large) {   // large: large_prefixes
   const RaggedParams& r = p.r;
   TcSeq s;
   s.table = b;
   s.start = 0;
   if (MODE == TC_PREFIX) {
-    const SharedGroup g = shared_group(p.x, r.c, b);
+    const SharedGroup g = shared_group(p.x, r, b, large);
     s.table = g.first;
-    s.row0 = s.n = 0;
+    s.row0 = g.row0;
+    s.n = g.keys && !g.warps ? g.n : 0;
     s.len = g.keys;
-    if (g.keys) {
-      s.row0 = __ldg(r.c.cu + g.first);
-      s.n = __ldg(r.c.cu + g.end) - s.row0;
-      const bool bad = s.row0 < 0 || s.n < 0 || s.n > r.T - s.row0;
-      if (bad) atomicOr(&g_dev_error, DEVERR_BAD_STATE);
-      if (bad) s.n = 0;
-    }
     return s;
   }
   s.row0 = __ldg(r.c.cu + b);
@@ -108,7 +102,7 @@ __device__ __forceinline__ TcSeq tc_seq(const TcAttnParams& p, int b) {
   if (bad) atomicOr(&g_dev_error, DEVERR_BAD_STATE);
   if (bad || s.n * r.group < p.min_rows) s.n = 0;
   if (MODE == TC_OWN && s.n) {
-    s.start = shared_keys(p.x, r.c, b);
+    s.start = shared_keys(p.x, r, b, large);
     s.len -= s.start;
     if (s.start && s.len < s.n) atomicOr(&g_dev_error, DEVERR_BAD_STATE);
     s.len = max(s.len, 0);
@@ -185,6 +179,7 @@ struct TcAttnSmem {
   uint64_t s_full[2], p_full[2][2], o_full[2], v_clean[S];   // per tile (P in two halves); per stage
   uint32_t tmem;
   int last;
+  bool large;
 };
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, int x, int y, int z, uint64_t* bar) {
@@ -350,12 +345,13 @@ template <int SRC, int MODE>
 struct TcWalk {
   const TcAttnParams& p;
   int b, g, pair, t0, step;
+  bool large;
   TcSeq s;
   TcPairs<MODE == TC_PREFIX> pr;
   long long u, u1;
   int n, t1;                // the unit's key tiles; the piece is [t0, t1)
   __device__ __forceinline__ TcWalk(const TcAttnParams& p_, const TcAttnSmem<SRC, MODE>& sm, int step_)
-      : p(p_), b(sm.at[0].b), g(sm.at[0].g), pair(sm.at[0].pair), t0(max(0, sm.at[0].t - TCA_UNIT_COST)), step(step_), s(tc_seq<SRC, MODE>(p_, sm.at[0].b)), pr(s, step_),
+      : p(p_), b(sm.at[0].b), g(sm.at[0].g), pair(sm.at[0].pair), t0(max(0, sm.at[0].t - TCA_UNIT_COST)), step(step_), large(sm.large), s(tc_seq<SRC, MODE>(p_, sm.at[0].b, sm.large)), pr(s, step_),
         u(sm.at[0].u), u1(sm.at[1].u) {
     piece();
   }
@@ -373,7 +369,7 @@ struct TcWalk {
       pair = 0;
       if (++g == p.r.c.n_kv) {
         g = 0;
-        do s = tc_seq<SRC, MODE>(p, ++b);
+        do s = tc_seq<SRC, MODE>(p, ++b, large);
         while (s.n == 0);
         pr = TcPairs<MODE == TC_PREFIX>(s, step);
       }
@@ -441,11 +437,12 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
   // ---- this CTA's range of key tiles: sums over the sequences, 32 chunks of them; warp 0 finds where it begins, warp 1
   // where the next one does ---------------------------------------------------------------------------------------------
   if (warp < 2) {
+    const bool large = MODE != TC_WHOLE && large_prefixes(p.x, r, lane);
     const int per = (p.seqs + 31) / 32;
     long long mine = 0, tot = 0;
     TcSeq s = {0, 0, 0, 0, 0};
     for (int b = lane * per; b < min(p.seqs, (lane + 1) * per); ++b) {
-      s = tc_seq<SRC, MODE>(p, b);
+      s = tc_seq<SRC, MODE>(p, b, large);
       const Pairs pr(s, step);
       tot = pr.n ? pr.before(pr.n) : 0;
       mine += tot * n_kv;
@@ -470,7 +467,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         tot = __shfl_sync(0xffffffffu, tot, first);
       } else {
         for (;; ++b) {
-          s = tc_seq<SRC, MODE>(p, b);
+          s = tc_seq<SRC, MODE>(p, b, large);
           const Pairs pr(s, step);
           tot = pr.n ? pr.before(pr.n) : 0;
           if (u < at + tot * n_kv) break;
@@ -502,7 +499,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
           if (++g == n_kv) {
             g = 0;
             do ++b;
-            while (b < p.seqs && tc_seq<SRC, MODE>(p, b).n == 0);
+            while (b < p.seqs && tc_seq<SRC, MODE>(p, b, large).n == 0);
           }
         }
       }
@@ -510,6 +507,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
     if (lane == 0) {
       sm.at[warp] = {b, g, pair, t, at + t};   // u and t count cost: key tile t - TCA_UNIT_COST
       sm.total = W;
+      sm.large = large;
     }
   }
   if (warp == 9) {

@@ -64,7 +64,9 @@ int shared_launches(const RaggedParams& p, const qk_ragged_attention_t& a, const
   std::lock_guard<std::mutex> together(workspace_mutex(ws));
   // sequences of up to OWN_MAX_ROWS query rows a KV head, and the others on the tensor cores
   const int strict = rows <= OWN_MAX_ROWS;
-  if (int e = rows <= 8 ? launch_own<FP8, 1>(p, strict, x, st) : launch_own<FP8, 2>(p, strict, x, st)) return e;
+  // (blocks of 8 rows are the quicker ones; a second block of a prefix's 16 comes out of the L2 cache, which several groups fill:
+  // one group of 4 behind 4,096 keys takes 23 us with 8 and 25 with 16, 8 such groups over e4m3 pages 49 and 41)
+  if (int e = rows <= 8 && x.G == 1 ? launch_own<FP8, 1>(p, strict, x, st) : launch_own<FP8, 2>(p, strict, x, st)) return e;
   if (!strict)
     if (int e = launch_tc<SRC, TC_OWN>(p, OWN_MAX_ROWS + 1, true, ws, st, x)) return e;
   if (int e = launch_tc<SRC, TC_PREFIX>(p, 0, true, ws, st, x)) return e;

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from test_paged_gpu import D, DEV, attend64, check_attention, cumulative, ints, make_cache, ops
-from test_sharing_gpu import SHARED, all_shared, check_select, fork, plan, shared_case
+from test_sharing_gpu import check_select, fork, plan, shared_case
 
 pytestmark = pytest.mark.gpu
 
@@ -30,9 +30,7 @@ def test_shared_calls_of_different_shapes_on_one_workspace():
     cases = [(n, f) for n in ("large", "drafts", "mha", "many_groups", "chunks", "beams") for f in (False, True)]
     for rnd in range(2):
         for i, (name, fp8) in enumerate(cases):
-            s = shared_case(name, fp8, seed=rnd)
-            if i % 3 != 2:
-                s["groups"], s["shared"] = all_shared(s, SHARED[name][4])
+            s = shared_case(name, fp8, seed=rnd, way=("as_it_is", "large", "tensor")[i % 3])
             if s["q"].shape[0] > 300:
                 continue
             out = torch.zeros_like(s["q"])
@@ -114,11 +112,11 @@ def test_shared_strides():
     assert (back[:, 0] == 5).all() and (back[:, T + 1] == 5).all() and (out[s["cu"][-1]:] == 5).all()
 
 
-@pytest.mark.parametrize("members", [4, 14, 40])
-def test_shared_large_and_rising_scores(members):
-    """Scores whose maxima lie late in the prefix and far above the first ones (the running maximum has to move), for prefixes in
-    four, two and one parts, and own keys far below or above them."""
-    n_kv, n_q, page, prefix, own = 2, 8, 32, 3968, 40
+@pytest.mark.parametrize("members,empty", [(4, 0), (7, 400), (14, 0), (14, 400), (40, 0)])
+def test_shared_large_and_rising_scores(members, empty):
+    """Scores whose maxima lie late in the prefix and far above the first ones (the running maximum has to move), for prefixes of
+    the warps and, in four, two and one parts, of the tensor cores, and own keys far below or above them."""
+    n_kv, n_q, page, prefix, own = 8, 32, 32, 6400, 40
     g = torch.Generator(device=DEV).manual_seed(members)
     c, rows = make_cache([prefix] + [own] * members, n_kv, page, False, g)
     pos = torch.arange(prefix, device=DEV)
@@ -138,7 +136,7 @@ def test_shared_large_and_rising_scores(members):
     q = torch.randn(members, n_q, D, generator=g, device=DEV).bfloat16()
     s = dict(q=q, n=[1] * members, cu=list(range(members + 1)), lens=[prefix + own] * members, table=table, k=c["k"], v=c["v"], ks=None, vs=None,
              groups=[0, members], shared=[prefix], rows=[[torch.cat((rows[0][i], rows[1 + b][i])) for i in range(2)] for b in range(members)])
-    s["groups"], s["shared"] = all_shared(s, n_kv)
+    s["groups"], s["shared"] = s["groups"] + [members] * empty, s["shared"] + [0] * empty
     out = torch.zeros_like(q)
     run_shared(s, out)
     assert ops().device_error() == 0
@@ -148,8 +146,7 @@ def test_shared_large_and_rising_scores(members):
 def test_a_row_depends_on_its_own_query_only():
     """Another member's query changes nothing in a row, to the bit."""
     for name in ("beams", "two_quarters", "large"):
-        s = shared_case(name, False)
-        s["groups"], s["shared"] = all_shared(s, SHARED[name][4])
+        s = shared_case(name, False, way="tensor")
         a, b = torch.zeros_like(s["q"]), torch.zeros_like(s["q"])
         run_shared(s, a)
         q = s["q"].clone()

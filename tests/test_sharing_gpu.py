@@ -417,9 +417,13 @@ SHARED = {   # members and prefix of each group (prefix None: its sequences are 
 }
 
 
-def shared_case(name, fp8, seed=0):
-    """The call's tensors, with their rows in 64 bits: groups' tables name the prefix's pages, other pages hold NaN."""
+def shared_case(name, fp8, seed=0, way="as_it_is"):
+    """The call's tensors, with their rows in 64 bits: groups' tables name the prefix's pages, other pages hold NaN. way "large": with a
+    group of 90 more sequences, which alone saves enough reads for the launch of the large prefixes, so that every large one is read
+    once. "tensor": also with so many empty groups that only prefixes of one block of rows are left to the warps."""
     spec, new, own, n_q, n_kv, page = SHARED[name]
+    if way != "as_it_is":
+        spec = spec + [(90, -(-240_001 // (89 * n_kv)) // 128 * 128 + 128)]
     g = torch.Generator(device=DEV).manual_seed(seed + len(name) + n_q)
     members = [m for m, _ in spec]
     of = [i for i, m in enumerate(members) for _ in range(m)]
@@ -444,25 +448,17 @@ def shared_case(name, fp8, seed=0):
         groups.append(heads[i])
         shared.append(prefix[i] if i in grouped else 0)
     groups.append(B)
+    if way == "tensor":
+        groups, shared = groups + [B] * 420, shared + [0] * 420
     q = (torch.randn(sum(n) + 2, n_q, D, generator=g, device=DEV) * 1.5).to(torch.bfloat16)
     return dict(c, table=table, q=q, n=n, lens=lens, cu=cumulative(n), groups=groups, shared=shared, rows=full, page=page)
 
 
-def all_shared(s, n_kv):
-    """The case's groups, and empty ones behind them: what sharing has to save is a group's part of a sum over the groups, so
-    with enough of them every prefix of 128 keys or more is read once."""
-    saved = [(b - a - 1) * (keys // 128 * 128) * n_kv for a, b, keys in zip(s["groups"], s["groups"][1:], s["shared"])]
-    n = -(-240_001 // min([x for x in saved if x > 0] or [1 << 20]))
-    return s["groups"] + [len(s["n"])] * n, s["shared"] + [0] * n
-
-
-@pytest.mark.parametrize("every", [False, True], ids=["large_ones", "every_prefix"])
+@pytest.mark.parametrize("way", ["as_it_is", "large", "tensor"])
 @pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "e4m3"])
 @pytest.mark.parametrize("name", SHARED)
-def test_shared_attention(name, fp8, every):
-    s = shared_case(name, fp8)
-    if every:
-        s["groups"], s["shared"] = all_shared(s, SHARED[name][4])
+def test_shared_attention(name, fp8, way):
+    s = shared_case(name, fp8, way=way)
     out = torch.full_like(s["q"], 3.0)
     k = ops()
     k.device_error()
