@@ -71,14 +71,14 @@ __device__ __forceinline__ SharedGroup shared_group(const SharedParams& x, const
   if (bad) atomicOr(&g_dev_error, DEVERR_BAD_STATE);
   return s;
 }
+// Reads that a large prefix saves: a sequence's own keys are read once for each 16 of its rows.
+__device__ __forceinline__ long long saved_reads(const SharedGroup& s, const RaggedParams& r) {
+  return s.keys && !s.warps ? (long long)(max(s.end - s.first, s.n * r.group / 16) - 1) * s.keys * r.c.n_kv : 0;
+}
 // Whether what the large prefixes save is worth their launch; a whole warp.
 __device__ __forceinline__ bool large_prefixes(const SharedParams& x, const RaggedParams& r, int lane) {
   long long reads = 0;
-  for (int g = lane; g < x.G; g += 32) {
-    const SharedGroup s = shared_group(x, r, g, true);
-    if (s.keys && !s.warps)                 // (a sequence's own keys are read once for each 16 of its rows)
-      reads += (long long)(max(s.end - s.first, s.n * r.group / 16) - 1) * s.keys * r.c.n_kv;
-  }
+  for (int g = lane; g < x.G; g += 32) reads += saved_reads(shared_group(x, r, g, true), r);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) reads += __shfl_xor_sync(0xffffffffu, reads, o);
   return reads >= SHARED_MIN_READS;
@@ -316,9 +316,14 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
       row0[i] = end[i] = len[i] = 0;
       if (b < r.c.B) row0[i] = __ldg(r.c.cu + b), end[i] = __ldg(r.c.cu + b + 1), len[i] = __ldg(r.c.seq_lens + b);
     }
-    large = large_prefixes(p.x, r, lane);
+    SharedGroup g = {0, 0, 0, 0, 0, false};
+    if (lane < p.x.G) g = shared_group(p.x, r, lane, true);
+    long long reads = saved_reads(g, r);    // (as large_prefixes)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) reads += __shfl_xor_sync(0xffffffffu, reads, o);
+    large = reads >= SHARED_MIN_READS;
+    if (!g.warps && !large) g.keys = 0;
     if (lane < p.x.G) {
-      const SharedGroup g = shared_group(p.x, r, lane, large);   // (the loads are in the L1 cache by now)
       const OwnSeq s = own_prefix(g);
       sm.group[lane] = make_int4(g.first, g.end, g.keys, 0);
       sm.prefix[lane] = make_int4(s.row0, s.n, s.len, s.start);
