@@ -6,8 +6,8 @@
 // Three launches, each of which starts as the one before it leaves the SMs:
 //  * the sequences' own keys. They are few and short beside the prefix, and what costs is each unit's chain of latencies (lengths,
 //    pages, rows of q, the first tile, the sums' way out). So a warp is a CTA of its own here, with a ring of its own: six on an SM
-//    hide each other's chains. (The few-row kernel, whose eight warps take each unit together: 40 us for 64 sequences of up to
-//    500 keys and 8 KV heads out of a cold cache, against XX.)
+//    hide each other's chains. (64 sequences of up to 500 keys and 8 KV heads: 22 us; the few-row kernel, whose eight warps take
+//    each unit together, 40 out of a cold cache.)
 //    Prefixes of groups with few query rows are sequences like these, in blocks of 16 rows.
 //  * the prefixes of larger groups (attention_tc.cuh): a group's rows, as one sequence's, over the keys they share, read once;
 //  * prefix_merge_kernel: a row's sums over its own keys and its prefix, in pieces where CTAs or warps shared them out, become the output.
@@ -204,7 +204,7 @@ struct OwnShape {
   static constexpr int S = FP8 ? 4 : 2;    // 32 KB
 };
 // Up to so many sequences, and groups, are looked up once, side by side, and kept in shared memory: a warp would else come to
-// its first tile by a chain of some ten loads from memory (64 sequences of up to 500 keys: XX us of launch, XX now).
+// its first tile by a chain of some ten loads from memory.
 constexpr int OWN_KEPT = 128, OWN_KEPT_GROUPS = 32;
 
 template <bool FP8, int NT>
