@@ -65,8 +65,9 @@ int qk_set_pdl(int on);
  * capturing a graph (the slots are fixed into a graph at capture). */
 int qk_set_timeline(uint64_t* buf, int n_slots);
 
-/* Read and clear the device-side error word (bit 1: a bounded wait gave up; bit 2: bad step state or
- * token id). Synchronises `stream`. No counterpart in the reference (its waits are unbounded). */
+/* Read and clear the device-side error word (bit 1: a bounded wait gave up; bit 2: bad step state,
+ * position, page, token id or logits; bit 4: a grid-wide wait gave up; bit 8: too few free pages).
+ * Synchronises `stream`. No counterpart in the reference (its waits are unbounded). */
 int qk_get_device_error(int* err, qk_stream_t stream);
 
 /* Exercise the failure path of the bounded waits (no counterpart in the reference, whose waits are unbounded):
@@ -399,7 +400,8 @@ int qk_packed_attention(const qk_ragged_attention_t* args, qk_stream_t stream);
  *   may overlap need one each.
  * qk_shared_attention: qk_paged_attention over sequences of which group g (as above, device data) has its first shared[g] positions in
  *   common: in the same pages, or in pages of equal contents. They are read through the group's first row, once for all its
- *   query rows. Every new token of a group comes after them (lens >= shared: else error word 2, and the group's rows are unspecified).
+ *   query rows. Every new token of a group comes after them (lens >= shared: else error word 2, and the group's rows are
+ *   unspecified).
  *   Sequences in no group are on their own. workspace: qk_shared_attention_workspace_bytes(rows, n_q). */
 typedef struct {
   const int *refs, *lens, *fresh, *block_table, *groups;

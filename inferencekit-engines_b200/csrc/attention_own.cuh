@@ -183,6 +183,8 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const __grid_constant
   }
   __syncthreads();
   if (quarter || (info | own) == 0) return;
+  if (q0 == 0) x.info[at] = x.own_info[at] = 0;
+  if (own == 0) return;                     // a sequence with more rows than max_q says: nobody took its own keys
 #pragma unroll
   for (int k = 1; k < 4; ++k) add(sum_ml[warp + k][lane], sum[warp + k][0][lane], sum[warp + k][1][lane]);
   const float inv = L == 0.f ? 0.f : 1.f / L;
@@ -190,7 +192,6 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const __grid_constant
   uint2* dst = reinterpret_cast<uint2*>(p.out + t * p.out_row + (long long)(at - t * p.n_q) * p.out_head);
   dst[q0] = make_uint2(pack_bf16(o[0].x * inv, o[0].y * inv), pack_bf16(o[0].z * inv, o[0].w * inv));
   dst[q0 + 16] = make_uint2(pack_bf16(o[1].x * inv, o[1].y * inv), pack_bf16(o[1].z * inv, o[1].w * inv));
-  if (q0 == 0) x.info[at] = x.own_info[at] = 0;
 }
 
 // A sequence's part here: up to OWN_MAX_ROWS query rows per KV head, in blocks of 8 or 16.

@@ -202,6 +202,7 @@ int qk_beam_select(const qk_beam_select_t* args, qk_stream_t stream) {
   p.keys = static_cast<unsigned long long*>(a.workspace);
   p.ml = reinterpret_cast<float2*>(p.keys + all * p.K);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  std::lock_guard<std::mutex> together(workspace_mutex(a.workspace));   // (another thread's chunks would take the lists' place)
   if (all) {
     auto k = a.fp32 ? beam_chunk_kernel<float> : beam_chunk_kernel<bf16>;
     if (int r = ensure_smem((const void*)k, (int)sizeof(BeamChunkSmem))) return r;

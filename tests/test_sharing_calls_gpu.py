@@ -2,6 +2,7 @@
 one after another on one workspace, with strides, with inputs that are refused or set the error word. Bounds as in
 test_sharing_gpu.py."""
 import math
+import threading
 
 import pytest
 import torch
@@ -95,6 +96,48 @@ def test_calls_on_two_streams():
     for i in range(2):
         check_shared(cases[i], outs[i])
         check_select(logits[i], scores, [0, 8, 24], 16, [t.tolist() for t in sel[i]])
+
+
+def test_host_threads_share_a_stream():
+    """Calls from two threads on one stream, each of several launches, on the stream's own workspaces."""
+    k = ops()
+    g = torch.Generator(device=DEV).manual_seed(10)
+    logits = [torch.randn(12, 30000, generator=g, device=DEV) for _ in range(2)]
+    scores, cu = torch.zeros(12, device=DEV), ints([0, 5, 12])
+    want = []
+    for x in logits:
+        out = (torch.zeros(2, 16, device=DEV), *(torch.zeros(2, 16, dtype=torch.int32, device=DEV) for _ in range(2)))
+        k.beam_select(x, scores, cu, *out)
+        want.append([t.clone() for t in out])
+    cases, outs = [shared_case("large", False, seed=i) for i in range(2)], []
+    args = []
+    for s in cases:
+        out = torch.zeros_like(s["q"])
+        run_shared(s, out)
+        outs.append(out.clone())
+        args.append((s["q"], ints(s["cu"]), ints(s["lens"]), s["table"], ints(s["groups"]), ints(s["shared"]), s["k"], s["v"]))
+    torch.cuda.synchronize()
+    failed = []
+    stream = torch.cuda.current_stream()
+
+    def work(i):
+        with torch.cuda.stream(stream):
+            res = [(torch.zeros(2, 16, device=DEV), *(torch.zeros(2, 16, dtype=torch.int32, device=DEV) for _ in range(2))) for _ in range(40)]
+            att = [torch.zeros_like(cases[i]["q"]) for _ in range(10)]
+            for n, out in enumerate(res):
+                k.beam_select(logits[i], scores, cu, *out)
+                if n % 4 == 0:
+                    k.shared_attention(*args[i], att[n // 4], D ** -0.5, 1)
+            stream.synchronize()
+            failed.extend(n for n, out in enumerate(res) if not all(torch.equal(a, b) for a, b in zip(out, want[i])))
+            failed.extend(n for n, a in enumerate(att) if not torch.equal(a, outs[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed and k.device_error() == 0
 
 
 def test_shared_strides():
