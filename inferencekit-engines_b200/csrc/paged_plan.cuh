@@ -40,6 +40,12 @@ struct PlanParams {
   int B, width, pages, page_shift, T, G;
 };
 
+// The warps' sums; the arrays over sequences (and pages) lie behind them.
+struct PlanSmem {
+  long long need[PLAN_WARPS], rows[PLAN_WARPS];
+  int free[PLAN_WARPS], copies[PLAN_WARPS], cta_free, pad[3];
+};
+
 // The CTAs of a launch are one cluster (or a single one).
 __device__ __forceinline__ void plan_sync() {
   if (gridDim.x == 1) __syncthreads();
@@ -72,15 +78,16 @@ struct FreePages {
     first = (int)min((long long)pages, (long long)w * per);
     last = (int)min((long long)pages, (long long)(w + 1) * per);
   }
-  // f(page, refs of it, whether it is free, free pages of the range before it): for every page of the range. Returns the free ones.
-  template <typename F>
-  __device__ __forceinline__ int each(const int* refs, int lane, F f) const {
+  // f(page, refs of it, whether it is free, free pages of the range before it): for every page of the range, whose refs are get(page).
+  // Returns the free ones.
+  template <typename G, typename F>
+  __device__ __forceinline__ int each(G get, int lane, F f) const {
     int before = 0, next[4];
     auto load = [&](int p0) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int p = p0 + 32 * k + lane;
-        next[k] = p < last ? __ldcg(refs + p) : 1;
+        next[k] = p < last ? get(p) : 1;
       }
     };
     load(first);
@@ -113,11 +120,13 @@ __device__ __forceinline__ int taker_of(const int* sums, int n, int r) {
 }
 
 __global__ void __launch_bounds__(PLAN_THREADS, 1) paged_plan_kernel(const __grid_constant__ PlanParams p) {
-  extern __shared__ int plan_smem[];
-  int* need_at = plan_smem;                 // [B] pages of the sequences before
-  int* new_at = plan_smem + p.B;            // [B + 1] rows of the sequences before
-  __shared__ long long w_need[PLAN_WARPS], w_new[PLAN_WARPS];
-  __shared__ int w_free[PLAN_WARPS], cta_free;
+  extern __shared__ __align__(16) uint8_t plan_smem[];
+  PlanSmem& sm = *reinterpret_cast<PlanSmem*>(plan_smem);
+  int* need_at = reinterpret_cast<int*>(&sm + 1);   // [B] pages of the sequences before
+  int* new_at = need_at + p.B;              // [B + 1] rows of the sequences before
+  auto &w_need = sm.need, &w_new = sm.rows;
+  auto &w_free = sm.free;
+  int& cta_free = sm.cta_free;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x, ctas = gridDim.x;
   const int all_warps = PLAN_WARPS * ctas, my_warp = cta * PLAN_WARPS + warp;
   const int P = 1 << p.page_shift;
@@ -143,7 +152,8 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) paged_plan_kernel(const __gri
   const long long need_in = warp_scan(need, lane), rows_in = warp_scan(rows, lane);
   if (lane == 31) w_need[warp] = need_in, w_new[warp] = rows_in;
   const FreePages range(p.pages, my_warp, all_warps);
-  const int free_here = range.each(p.refs, lane, [](int, int, bool, int) {});
+  auto refs_of = [&](int page) { return __ldcg(p.refs + page); };
+  const int free_here = range.each(refs_of, lane, [](int, int, bool, int) {});
   if (lane == 0) w_free[warp] = free_here;
   __syncthreads();
   if (ctas > 1 && warp == 0) {
@@ -192,7 +202,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) paged_plan_kernel(const __gri
   // ---- pages: those of rank below the sum go to the sequences ----------------------------------------------------------------
   const int take = fits ? (int)all_need : 0;
   if (p.refs_out != p.refs || (free_before < take && free_here))
-    range.each(p.refs, lane, [&](int page, int refs, bool free, int before) {
+    range.each(refs_of, lane, [&](int page, int refs, bool free, int before) {
       const int rank = free_before + before;
       const bool taken = free && rank < take;
       if (taken) {
@@ -276,10 +286,12 @@ struct ForkParams {
 // The tables and counts of a fork. Row i copies where copied[i]: its parent's last page is partly filled and belongs to an
 // earlier child, or to a sequence outside the call.
 __global__ void __launch_bounds__(PLAN_THREADS, 1) paged_fork_kernel(const __grid_constant__ ForkParams p) {
-  extern __shared__ int plan_smem[];
-  int* first = plan_smem;                   // [B] a row's first child
-  int* copy_at = plan_smem + p.B;           // [N] copies of the rows before
-  __shared__ int w_copies[PLAN_WARPS], w_free[PLAN_WARPS];
+  extern __shared__ __align__(16) uint8_t plan_smem[];
+  PlanSmem& sm = *reinterpret_cast<PlanSmem*>(plan_smem);
+  int* first = reinterpret_cast<int*>(&sm + 1);   // [B] a row's first child
+  int* copy_at = first + p.B;               // [N] copies of the rows before
+  auto refs_of = [&](int page) { return __ldcg(p.refs_out + page); };
+  auto &w_copies = sm.copies, &w_free = sm.free;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int P = 1 << p.page_shift;
   grid_dep_wait();
@@ -312,7 +324,8 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) paged_fork_kernel(const __gri
   };
   for (int b = tid; b < p.B; b += PLAN_THREADS) first[b] = 0x7fffffff;
   if (p.refs_out != p.refs)
-    for (int i = tid; i < p.pages; i += PLAN_THREADS) p.refs_out[i] = __ldg(p.refs + i);
+#pragma unroll 4
+    for (int i = tid; i < p.pages; i += PLAN_THREADS) p.refs_out[i] = __ldcg(p.refs + i);
   __syncthreads();
   for (int b = warp; b < p.B; b += PLAN_WARPS) count(b, pages_of(length(b)), -1);
   for (int i = tid; i < p.N; i += PLAN_THREADS) {
@@ -326,7 +339,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) paged_fork_kernel(const __gri
     if ((n & (P - 1)) == 0) return 0;
     if (first[b] != i) return 1;
     const int page = old_page(b, n >> p.page_shift);
-    return page >= 0 && __ldcg(p.refs_out + page) != 0 ? 1 : 0;
+    return page >= 0 && refs_of(page) != 0 ? 1 : 0;
   };
   const int per = (p.N + PLAN_THREADS - 1) / PLAN_THREADS;
   int mine = 0;
@@ -355,7 +368,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) paged_fork_kernel(const __gri
   }
   __syncthreads();
   const FreePages range(p.pages, warp, PLAN_WARPS);
-  const int free_here = range.each(p.refs_out, lane, [](int, int, bool, int) {});
+  const int free_here = range.each(refs_of, lane, [](int, int, bool, int) {});
   if (lane == 0) w_free[warp] = free_here;
   __syncthreads();
   int free_before = 0, all_free = 0;
@@ -373,7 +386,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) paged_fork_kernel(const __gri
     for (int b = warp; b < p.B; b += PLAN_WARPS) count(b, pages_of(length(b)), 1);
     __syncthreads();
     all_free = 0;
-    const int back = range.each(p.refs_out, lane, [](int, int, bool, int) {});
+    const int back = range.each(refs_of, lane, [](int, int, bool, int) {});
     if (lane == 0) w_free[warp] = back;
     __syncthreads();
     for (int w = 0; w < PLAN_WARPS; ++w) all_free += w_free[w];
@@ -394,7 +407,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) paged_fork_kernel(const __gri
     if (lane == 0) p.lens_out[i] = n;
   }
   if (fits && free_before < wanted && free_here)
-    range.each(p.refs_out, lane, [&](int page, int, bool free, int at) {
+    range.each(refs_of, lane, [&](int page, int, bool free, int at) {
       const int rank = free_before + at;
       if (!free || rank >= wanted) return;
       const int i = taker_of(copy_at, p.N, rank);

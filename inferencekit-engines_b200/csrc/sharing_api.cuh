@@ -128,7 +128,7 @@ int qk_paged_plan(const qk_paged_plan_t* args, qk_stream_t stream) {
   p.slots = a.slots, p.positions = a.positions, p.groups = a.groups, p.shared = a.shared, p.info = a.info;
   p.table_stride = stride, p.out_stride = out;
   p.B = (int)a.batch, p.width = (int)a.table_width, p.pages = (int)a.n_pages, p.T = (int)a.rows, p.G = (int)a.n_groups;
-  const int smem = (2 * p.B + 1) * 4;
+  const int smem = (int)sizeof(PlanSmem) + (2 * p.B + 1) * 4;
   if (int r = ensure_smem((const void*)paged_plan_kernel, smem)) return r;
   return launch_cluster(paged_plan_kernel, plan_ctas(p.pages, p.B, p.T), dim3(PLAN_THREADS), smem, static_cast<cudaStream_t>(stream), p);
 }
@@ -161,13 +161,13 @@ int qk_paged_fork(const qk_paged_fork_t* args, qk_stream_t stream) {
   p.B = (int)a.batch, p.N = (int)a.rows, p.width = (int)a.table_width, p.pages = (int)a.n_pages;
   p.layers = (int)a.layers, p.n_kv = (int)a.n_kv, p.row_bytes = a.kv_fp8 ? HEAD_DIM : 2 * HEAD_DIM;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int smem = (p.B + p.N) * 4;
+  const int smem = (int)sizeof(PlanSmem) + (p.B + p.N) * 4;
   if (int r = ensure_smem((const void*)paged_fork_kernel, smem)) return r;
   if (int r = launch(paged_fork_kernel, dim3(1), dim3(PLAN_THREADS), smem, st, p)) return r;
   if (p.N == 0) return QK_OK;
   // a layer's K or V page at a time, where that leaves 32 CTAs an SM (53 us with 8 for 8 requests of 8 beams and 36 layers, 43 with 32)
   p.parts = (int)std::max(1ll, std::min(2ll * p.layers, 32ll * device_sms() / p.N));
-  return launch(paged_copy_kernel, dim3(p.N, p.parts), dim3(256), 0, st, p);
+  return launch_as(true, paged_copy_kernel, dim3(p.N, p.parts), dim3(256), 0, st, p);   // (its CTAs are there when the tables are)
 }
 
 // The chunks' sums and lists; as many chunks as a call of these sizes may make, of rows of either type.

@@ -76,6 +76,8 @@ PLANS = {   # lens, new, page, free pages, groups
     "mixed": ([1000, 0, 127, 128, 129, 5], [1, 700, 1, 1, 1, 0], 128, 60, [0, 2, 6]),
     "many": ([37 * i % 500 for i in range(1500)], [i % 3 for i in range(1500)], 64, 1600, list(range(0, 1501, 5))),
     "large_pool": ([40, 50], [5000, 3000], 16, 100_000, [0, 2]),
+    "most_sequences": ([i % 40 for i in range(16384)], [1] * 16384, 16, 2000, [0, 16384]),
+    "9000_sequences": ([i % 7 for i in range(9000)], [i % 2 for i in range(9000)], 16, 3000, [0, 3, 9000]),
 }
 
 
@@ -179,6 +181,9 @@ FORKS = {   # lens, parents, page, spare pages, groups of sequences that share
     "swap": ([20, 90, 5], [2, 1, 0, -1], 128, 2, [0, 1, 3]),
     "empty_sequences": ([0, 1, 0], [0, 0, 1, 1, 2], 16, 2, [0, 3]),
     "many": ([37 * (i // 8) % 500 for i in range(800)], [i // 8 * 8 + (i * i) % 8 for i in range(800)], 32, 900, list(range(0, 801, 8))),
+    "large_pool": ([100, 40], [1, 0, 0, 1], 16, 60_000, [0, 2]),
+    "most_rows": ([i % 20 for i in range(16384)], [i ^ 1 if i % 3 else i for i in range(16384)], 16, 9000, [0, 16384]),
+    "6000_rows": ([3] * 6000, list(range(6000)), 16, 10, [0, 6000]),
 }
 
 
