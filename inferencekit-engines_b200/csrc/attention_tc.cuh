@@ -378,6 +378,7 @@ struct TcWalk {
   }
   // of tile x of the pair: its first token, whether it has any, and its key tiles in this piece
   __device__ __forceinline__ int tok0(int x) const { return pair * step + x * (step / 2); }
+  __device__ __forceinline__ bool two() const { return tok0(1) < s.n; }
   __device__ __forceinline__ int end(int x) const {
     if (tok0(x) >= s.n) return t0;
     const int keys = MODE == TC_PREFIX ? s.len : min(s.len, s.len - s.n + min(tok0(x) + step / 2, s.n));
@@ -534,7 +535,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
       for (int unit = 0; w.more() && ok; w.next(), ++unit) {
         if (unit) ok = __all_sync(0xffffffffu, mbar_wait_small(&sm.q_empty, (uint32_t)((unit - 1) & 1)));
         if (!ok) break;
-        const bool two = w.tok0(1) < w.s.n;
+        const bool two = w.two();
         if (lane == 0) {
           mbar_arrive_expect_tx(&sm.q_full, two ? 2 * q_bytes : q_bytes);
           for (int x = 0; x < (two ? 2 : 1); ++x)
@@ -723,7 +724,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
             else sm.k_scale[FP8 ? (it >> 1) % 3 : 0][FP8 ? th : 0] = scales.x;
           }
           if (is_v) scales = ahead;
-          const bool ten = MODE == TC_PREFIX && prefix_parts(w.s.n, tpq) > 1;
+          const bool ten = MODE == TC_PREFIX && !w.two();   // with tile 1's softmax warps, which have no rows
           if (ten) tca_convert<24, 80, TCA_KEYS>(src, dst, th, TCA_KEYS);
           else tca_convert<24, 0, TCA_KEYS>(src, dst, th, tail);
           fence_proxy_async_smem();
@@ -752,7 +753,9 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         const bool valid = (MODE == TC_PREFIX ? own < tpq : row < (step / 2) * r.group) && tok < w.s.n;
         const int first = MODE == TC_PREFIX ? w.s.len - 1 : w.s.len - w.s.n + w.tok0(x);   // the last key that the tile's first row sees
         float m = -INFINITY, l = 0.f, base = 0.f;   // base = -m * sl2 - TCA_SHIFT
-        if (FP8 && MODE == TC_PREFIX && parts > 1 && x == 1) {   // no rows here: most of the tiles' conversion
+        // No rows in tile 1 (a prefix in parts, or a last pair of few rows): its warps do most of the tiles' conversion. That also
+        // keeps them in step with the ring, whose phases they know by parity only: none of them passes a piece without its tiles.
+        if (FP8 && MODE == TC_PREFIX && x == 1 && !w.two()) {
           for (uint32_t it = 2 * kt; it < (uint32_t)(2 * (kt + w.t1 - w.t0)); ++it) {
             const uint32_t rs = it % RAW, st = it % TCA_STAGES;
             ok = ok && mbar_wait_small(&sm.raw_full[rs], (it / RAW) & 1);

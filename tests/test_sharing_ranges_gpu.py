@@ -1,0 +1,38 @@
+"""shared_attention where one CTA's or warp's range of work holds pieces of different kinds: groups of different sizes behind each
+other, units cut between CTAs. Bounds as in test_sharing_gpu.py."""
+import pytest
+import torch
+
+import test_sharing_gpu
+from test_paged_gpu import DEV, ops
+from test_sharing_calls_gpu import check_shared, run_shared
+from test_sharing_gpu import shared_case
+
+pytestmark = pytest.mark.gpu
+
+# as SHARED in test_sharing_gpu.py. A tile pair of the tensor cores holds a prefix's rows in one tile, twice or four times where they are few
+# (up to 16 tokens at 4 heads a KV head), once from there on, and in both tiles from 33 tokens on.
+CHANGES = {
+    "long": ([(22, 8192), (14, 8192), (20, 8192)], [1], [30, 5], 32, 8, 64),
+    "both_tiles": ([(22, 4096), (40, 4096), (7, 4096), (70, 4096), (12, 4096), (33, 4096)], [1], [30, 5], 32, 8, 16),
+    "short": ([(n, 256 + 128 * (i % 2)) for i in range(17) for n in (18, 5, 17, 36, 20, 9)], [1], [1, 7], 16, 4, 128),
+    "short_mha": ([(n, 256) for _ in range(4) for n in (70, 20, 100, 40, 130)], [1], [3], 4, 4, 32),
+    "drafts": ([(6, 2048), (2, 2048), (9, 1024), (3, 4096), (5, 2048)], [4, 1, 3, 5], [40, 6], 32, 8, 32),
+}
+
+
+@pytest.mark.parametrize("way", ["as_it_is", "tensor"])
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "e4m3"])
+@pytest.mark.parametrize("name", CHANGES)
+def test_groups_of_different_sizes_in_one_range(name, fp8, way, monkeypatch):
+    monkeypatch.setitem(test_sharing_gpu.SHARED, name, CHANGES[name])
+    k = ops()
+    s = shared_case(name, fp8, way=way)
+    ws = k.shared_workspace(DEV, *s["q"].shape[:2])
+    outs = [torch.full_like(s["q"], 3.0) for _ in range(5)]
+    k.device_error()
+    for out in outs:
+        run_shared(s, out, ws)
+    assert k.device_error() == 0
+    assert (outs[0][s["cu"][-1]:] == 3).all() and all(torch.equal(out, outs[0]) for out in outs)
+    check_shared(s, outs[0], fp8)
