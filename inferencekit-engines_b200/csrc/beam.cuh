@@ -258,7 +258,10 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) beam_chunk_kernel(const __gri
     since = 0;
     __syncthreads();
     const int vectors = hits;
-    if (!ends && vectors <= BEAM_CAP / 2) continue;
+    if (!ends) {                            // (a warp that goes on adds to them: not before all have read)
+      __syncthreads();
+      if (vectors <= BEAM_CAP / 2) continue;
+    }
     // ---- the vectors' values that reach the border, the k best of them and of those before -----------------------------------------
     for (int i = tid; i < min(vectors, BEAM_CAP); i += BEAM_THREADS) {
       const int first = (int)(sm.hit[i] & 0x7fffffffu) * PER - c.lead;
