@@ -383,11 +383,13 @@ int qk_packed_attention(const qk_ragged_attention_t* args, qk_stream_t stream);
  *   All or nothing: with too few free pages (error word 8), or more rows than `rows` (error word 2; rows -1: any number), nothing is taken,
  *   cu_rows is 0 and seq_lens is lens. info (NULL, or [2]): pages missing (0: done), free pages left. A sequence with a negative length or
  *   one past its table sits the pass out (error word 2). table_out and refs_out may be the inputs (then only what changes is
- *   written) or memory apart from them (copied). At most 16,384 sequences.
+ *   written) or memory apart from them (copied). At most 16,384 sequences. A partly filled page that new tokens go into has to be its
+ *   sequence's own: it is after a qk_paged_fork, which copies what several hold.
  * qk_paged_fork: the sequences in a new order: row i (of `rows`) continues row parents[i] of the old ones (-1: it is empty). table_out and
  *   lens_out (apart from the inputs) are the new rows, -1 behind their pages; refs counts the new rows in place of the old ones. A
- *   partly filled last page stays with its row's first child, unless a sequence outside the call holds it too; the
- *   other children get a free page and a copy of the filled rows, in every layer: pools [layers][n_pages][n_kv][page_size][128].
+ *   partly filled last page stays with the first of the new rows that end in it (several old rows may have ended in one page), unless a
+ *   sequence outside the call, or a new row that goes past it, holds it too. The others get a free page and a copy of the filled
+ *   rows, in every layer: pools [layers][n_pages][n_kv][page_size][128].
  *   With one old row and many new ones it spreads a prompt, with parents -1 it ends sequences. All or nothing: with too few free pages
  *   (error word 8) the refs are as they were and the new rows are empty. At most 16,384 rows on either side.
  * qk_beam_select: request b's beams are the rows cu_rows[b] .. cu_rows[b+1]-1 (at most 128) of logits [rows][vocab] (bf16, or fp32 = 1;

@@ -8,7 +8,7 @@
 //   plan: need_b = ceil((len_b + new_b) / P) - ceil(len_b / P), all of them or none; cu = prefix sums of new; slot of every
 //         new row; per group of sequences the leading positions that lie in the same pages
 //   fork: row i continues row parents[i]: refs of the old rows' pages fall, those of the new rows' rise; a partly filled last page
-//         goes to one child, the others get a page of their own and a copy of the filled rows
+//         goes to the first row that ends in it, the others get a page of their own and a copy of the filled rows
 //
 // Both are chains of short dependent steps (prefix sums over sequences, over pages, then tables, then slots), bound by the
 // latency of each, so each is one launch: a CTA, or a cluster of eight for large batches and pools, which share out the
@@ -283,13 +283,12 @@ struct ForkParams {
   int B, N, width, pages, page_shift, layers, n_kv, row_bytes, parts;
 };
 
-// The tables and counts of a fork. Row i copies where copied[i]: its parent's last page is partly filled and belongs to an
-// earlier child, or to a sequence outside the call.
+// The tables and counts of a fork. Row i copies where copied(i): its parent's last page is partly filled and an earlier new row ends in
+// it too, or something else holds it: a new row that goes past it, or a sequence outside the call.
 __global__ void __launch_bounds__(PLAN_THREADS, 1) paged_fork_kernel(const __grid_constant__ ForkParams p) {
   extern __shared__ __align__(16) uint8_t plan_smem[];
   PlanSmem& sm = *reinterpret_cast<PlanSmem*>(plan_smem);
-  int* first = reinterpret_cast<int*>(&sm + 1);   // [B] a row's first child
-  int* copy_at = first + p.B;               // [N] copies of the rows before
+  int* copy_at = reinterpret_cast<int*>(&sm + 1);   // [N] copies of the rows before
   auto refs_of = [&](int page) { return __ldcg(p.refs_out + page); };
   auto &w_copies = sm.copies, &w_free = sm.free;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -316,35 +315,40 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) paged_fork_kernel(const __gri
     atomicOr(&g_dev_error, DEVERR_BAD_STATE);
     return -1;
   };
+  auto open_page = [&](int i) {             // the partly filled page that row i's parent ends in; -1: none
+    const int b = parent(i), n = b < 0 ? 0 : length(b);
+    return n & (P - 1) ? old_page(b, n >> p.page_shift) : -1;
+  };
   auto count = [&](int b, int entries, int by) {   // a warp: the first entries of an old row
     for (int j = lane; j < entries; j += 32) {
       const int page = old_page(b, j);
       if (page >= 0) atomicAdd(p.refs_out + page, by);
     }
   };
-  for (int b = tid; b < p.B; b += PLAN_THREADS) first[b] = 0x7fffffff;
-  if (p.refs_out != p.refs)
+  if (p.refs_out != p.refs) {
 #pragma unroll 4
     for (int i = tid; i < p.pages; i += PLAN_THREADS) p.refs_out[i] = __ldcg(p.refs + i);
-  __syncthreads();
+    __syncthreads();
+  }
+  // ---- the old rows' pages, and the new rows' but for those partly filled ----------------------------------------------------------
   for (int b = warp; b < p.B; b += PLAN_WARPS) count(b, pages_of(length(b)), -1);
-  for (int i = tid; i < p.N; i += PLAN_THREADS) {
+  for (int i = warp; i < p.N; i += PLAN_WARPS) {
     const int b = parent(i);
-    if (b >= 0) atomicMin(&first[b], i);
+    if (b >= 0) count(b, length(b) >> p.page_shift, 1);
+  }
+  __syncthreads();
+  // ---- a partly filled page that nothing else holds is the first row's that ends in it: i - N, the least, in the place of its count -----
+  const int per = (p.N + PLAN_THREADS - 1) / PLAN_THREADS, i0 = tid * per, i1 = min(p.N, i0 + per);
+  for (int i = i0; i < i1; ++i) {
+    const int page = open_page(i);
+    if (page >= 0 && refs_of(page) <= 0) atomicMin(p.refs_out + page, i - p.N);
   }
   __syncthreads();
   // ---- which rows copy, and the sums of that -----------------------------------------------------------------------------------
-  auto copies = [&](int i) {
-    const int b = parent(i), n = b < 0 ? 0 : length(b);
-    if ((n & (P - 1)) == 0) return 0;
-    if (first[b] != i) return 1;
-    const int page = old_page(b, n >> p.page_shift);
-    return page >= 0 && refs_of(page) != 0 ? 1 : 0;
-  };
-  const int per = (p.N + PLAN_THREADS - 1) / PLAN_THREADS;
   int mine = 0;
-  for (int i = tid * per; i < min(p.N, (tid + 1) * per); ++i) {
-    copy_at[i] = copies(i);                 // (a flag for now)
+  for (int i = i0; i < i1; ++i) {
+    const int page = open_page(i);
+    copy_at[i] = page >= 0 && refs_of(page) != i - p.N;   // (a flag for now)
     mine += copy_at[i];
   }
   const int incl = (int)warp_scan(mine, lane);
@@ -355,18 +359,14 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) paged_fork_kernel(const __gri
     if (w < warp) before += w_copies[w];
     wanted += w_copies[w];
   }
-  for (int i = tid * per; i < min(p.N, (tid + 1) * per); ++i) {
-    const int f = copy_at[i];
+  for (int i = i0; i < i1; ++i) {
+    const int f = copy_at[i], page = f ? -1 : open_page(i);
+    if (page >= 0) p.refs_out[page] = 1;    // its one holder
     copy_at[i] = before;
     before += f;
   }
   __syncthreads();
   auto copied = [&](int i) { return (i + 1 < p.N ? copy_at[i + 1] : wanted) != copy_at[i]; };
-  for (int i = warp; i < p.N; i += PLAN_WARPS) {
-    const int b = parent(i);
-    if (b >= 0) count(b, pages_of(length(b)) - (copied(i) ? 1 : 0), 1);
-  }
-  __syncthreads();
   const FreePages range(p.pages, warp, PLAN_WARPS);
   const int free_here = range.each(refs_of, lane, [](int, int, bool, int) {});
   if (lane == 0) w_free[warp] = free_here;

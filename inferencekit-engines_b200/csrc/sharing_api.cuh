@@ -161,7 +161,7 @@ int qk_paged_fork(const qk_paged_fork_t* args, qk_stream_t stream) {
   p.B = (int)a.batch, p.N = (int)a.rows, p.width = (int)a.table_width, p.pages = (int)a.n_pages;
   p.layers = (int)a.layers, p.n_kv = (int)a.n_kv, p.row_bytes = a.kv_fp8 ? HEAD_DIM : 2 * HEAD_DIM;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int smem = (int)sizeof(PlanSmem) + (p.B + p.N) * 4;
+  const int smem = (int)sizeof(PlanSmem) + p.N * 4;
   if (int r = ensure_smem((const void*)paged_fork_kernel, smem)) return r;
   if (int r = launch(paged_fork_kernel, dim3(1), dim3(PLAN_THREADS), smem, st, p)) return r;
   if (p.N == 0) return QK_OK;

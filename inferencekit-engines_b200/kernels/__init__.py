@@ -677,7 +677,8 @@ class DecodeOps:
                    refs_out=None, info=None):
         """The sequences in a new order: row i of table_out [N, width] and lens_out [N] (not the inputs) continues row parents[i]
         (int32 [N]; -1: an empty row) of block_table [B, width] and lens [B]. Whole pages are shared by count; a partly filled last
-        page stays with its row's first child, the others get a free page and a copy of the filled rows. Pools: [pages, n_kv,
+        page stays with the first new row that ends in it, unless a sequence outside the call or a longer new row holds it too; the
+        others get a free page and a copy of the filled rows. Pools: [pages, n_kv,
         page_size, 128] or [layers, pages, n_kv, page_size, 128] (bf16, or e4m3 with scales of the leading dimensions), whose
         pages are copied in every layer. One row into many spreads a prompt over its beams, parents of -1 end sequences. refs_out:
         where the counts go (default: in place). info (int32 [2]): pages missing (0: done; else refs is as it was and the new rows are
