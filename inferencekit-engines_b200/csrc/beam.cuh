@@ -360,7 +360,10 @@ struct BeamMergeSmem {
   double cand_s[BEAM_CAP];
   unsigned cand_at[BEAM_CAP];
   BeamBorder border;
-  double off[BEAM_MAX_ROWS];               // score - logsumexp; -inf: the row has nothing
+  // A logit x of row r scores (x - max[r]) + off[r], off = score - log of the sum under the maximum; -inf: the row has nothing. (The
+  // difference first: a row of the type's lowest values has its maximum there too, beside which the rest would be lost.)
+  double off[BEAM_MAX_ROWS];
+  float max[BEAM_MAX_ROWS];
   float2 ml[BEAM_MAX_USED];
   BeamBest red[BEAM_WARPS];
   int list_at[BEAM_MAX_ROWS + 4];          // lists of the rows before
@@ -464,8 +467,9 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const __grid_c
     }
     const bool none = score == -INFINITY || (L == 0. && M == -INFINITY), wrong = !none && !(fabsf(score) < INFINITY && L > 0. && L < 1e300);
     if (wrong) atomicOr(&g_dev_error, DEVERR_BAD_STATE);   // a NaN or +infinity among its logits, or as its score
-    const double off = none || wrong ? -INFINITY : (double)score - ((double)M + log(L));
+    const double off = none || wrong ? -INFINITY : (double)score - log(L);
     sm.off[tid] = off;
+    sm.max[tid] = none || wrong ? 0.f : M;
     if (off != -INFINITY) atomicMax(&sm.reach, __float_as_int(fabsf((float)off)));
   }
   __syncthreads();
@@ -478,7 +482,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const __grid_c
       r = row_of(list);
       chunk = chunk_of(r, list);
       const unsigned long long key = key_at(chunk, 0);
-      return key ? beam_value(key) + (float)sm.off[r] : -INFINITY;
+      return key ? (beam_value(key) - sm.max[r]) + (float)sm.off[r] : -INFINITY;
     };
     int r, chunk;
     float top = -INFINITY;
@@ -499,8 +503,8 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const __grid_c
     // ---- their candidates: a warp a list, its first one another lane's in each ------------------------------------------------------
     auto each = [&](auto f) {
       for (int at = warp; at < n_lists; at += BEAM_WARPS) {
-        const float off = (float)sm.off[sm.row[at]];
-        for (int i = (lane - 5 * (at / BEAM_WARPS)) & 31; i < p.K; i += 32) f(at, i, value[at * p.K + i] + off);
+        const float off = (float)sm.off[sm.row[at]], max = sm.max[sm.row[at]];
+        for (int i = (lane - 5 * (at / BEAM_WARPS)) & 31; i < p.K; i += 32) f(at, i, (value[at * p.K + i] - max) + off);
       }
     };
     float top = -INFINITY;
@@ -512,7 +516,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const __grid_c
       if (to >= BEAM_CAP) return;
       const int r = sm.row[at];
       const unsigned long long key = key_at(sm.chunk[at], i);
-      sm.cand_s[to] = (double)beam_value(key) + sm.off[r];
+      sm.cand_s[to] = ((double)beam_value(key) - (double)sm.max[r]) + sm.off[r];
       sm.cand_at[to] = (unsigned)r * (unsigned)p.V + (unsigned)beam_index(key);
     });
   } else if (tid == 0) {
@@ -540,8 +544,8 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const __grid_c
       if (sm.head[i] >= p.K) continue;
       const int r = row_of(i);
       const unsigned long long key = key_at(chunk_of(r, i), sm.head[i]);
-      const BeamBest c = {key ? (double)beam_value(key) + sm.off[r] : -INFINITY, (unsigned)r * (unsigned)p.V + (unsigned)beam_index(key), i};
-      if (c.s > -INFINITY && (best.list < 0 || beam_better(c.s, c.at, best.s, best.at))) best = c;
+      const BeamBest c = {key ? ((double)beam_value(key) - (double)sm.max[r]) + sm.off[r] : -INFINITY, (unsigned)r * (unsigned)p.V + (unsigned)beam_index(key), i};
+      if ((float)c.s > -INFINITY && (best.list < 0 || beam_better(c.s, c.at, best.s, best.at))) best = c;
     }
     return best;
   };
