@@ -394,7 +394,7 @@ int qk_packed_attention(const qk_ragged_attention_t* args, qk_stream_t stream);
  *   (error word 8) the refs are as they were and the new rows are empty. At most 16,384 rows on either side.
  * qk_beam_select: request b's beams are the rows cu_rows[b] .. cu_rows[b+1]-1 (at most 128) of logits [rows][vocab] (bf16, or fp32 = 1;
  *   row_stride elements apart, vocab at most 1,048,576) with their scores so far. Out of all (beam r, token v) the k <= 64 largest
- *   scores[r] + logits[r][v] - logsumexp(logits[r]), in order, equal ones by r, then v: out_scores, out_parents (r) and out_tokens
+ *   scores[r] + logits[r][v] - logsumexp(logits[r]), in order, equal ones by r, then logit and v: out_scores, out_parents (r) and out_tokens
  *   [batch][k]; -inf, -1, -1 where fewer have a score above -inf (in fp32). A logit of -inf excludes a token, a score of -inf a beam (whatever its
  *   logits are). A row with a NaN or +inf in logits or score sets error word 2 and gives no candidates; a request whose
  *   offsets are not within the rows, or of more than 128, sets it too and is empty. Sums of exponentials in fp32,

@@ -1,5 +1,5 @@
 // Beam search's selection: for each request the best k of  s(r, v) = score_r + x_rv - logsumexp_v'(x_rv')  over its beams r
-// and the vocabulary v, ties to the lowest (r, v).
+// and the vocabulary v; of equal scores the lowest r first, in a row the largest logit, then the lowest v.
 //
 // Bound by the logits' bytes, which are read once, and nearly as much by their exponentials (16 a cycle and SM: 70 % of the time
 // that bf16 logits take to arrive).
@@ -349,16 +349,23 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) beam_chunk_kernel(const __gri
 
 constexpr int BEAM_MAX_USED = 256;         // lists that are merged side by side
 
-struct BeamBest {            // a candidate of the merge: its score, then its flat place in the request (row * V + token)
+// What orders candidates whose scores are equal in 64 bits, the larger first: the lower row of the request, in it the larger logit (which
+// a score far larger may have swallowed), then the lower token. 7, 32 and 20 bits.
+__device__ __forceinline__ unsigned long long beam_place(int row, unsigned long long key) {
+  return (unsigned long long)(BEAM_MAX_ROWS - 1 - row) << 52 | key >> 32 << 20 | (BEAM_MAX_VOCAB - 1 - beam_index(key));
+}
+static_assert(BEAM_MAX_ROWS <= 1 << 7 && BEAM_MAX_VOCAB <= 1 << 20, "a candidate's place has 59 bits");
+
+struct BeamBest {            // a candidate of the merge: its score, then its place
   double s;
-  unsigned at;
+  unsigned long long at;
   int list;                 // where it is from; -1: none
 };
-__device__ __forceinline__ bool beam_better(double a, unsigned ia, double b, unsigned ib) { return a > b || (a == b && ia < ib); }
+__device__ __forceinline__ bool beam_better(double a, unsigned long long ia, double b, unsigned long long ib) { return a > b || (a == b && ia > ib); }
 
 struct BeamMergeSmem {
   double cand_s[BEAM_CAP];
-  unsigned cand_at[BEAM_CAP];
+  unsigned long long cand_at[BEAM_CAP];
   BeamBorder border;
   // A logit x of row r scores (x - max[r]) + off[r], off = score - log of the sum under the maximum; -inf: the row has nothing. (The
   // difference first: a row of the type's lowest values has its maximum there too, beside which the rest would be lost.)
@@ -387,11 +394,10 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const __grid_c
     rows = 0;
   }
   const size_t out = (size_t)b * p.K;
-  auto write = [&](int k, bool any, double s, unsigned at) {
-    const unsigned r = at / (unsigned)p.V;
+  auto write = [&](int k, bool any, double s, unsigned long long at) {
     p.out_scores[out + k] = any ? (float)s : -INFINITY;
-    p.out_parents[out + k] = any ? r0 + (int)r : -1;
-    p.out_tokens[out + k] = any ? (int)(at - r * (unsigned)p.V) : -1;
+    p.out_parents[out + k] = any ? r0 + BEAM_MAX_ROWS - 1 - (int)(at >> 52) : -1;
+    p.out_tokens[out + k] = any ? BEAM_MAX_VOCAB - 1 - (int)(at & (BEAM_MAX_VOCAB - 1)) : -1;
   };
   // ---- the rows' parts: row r's lists are list_at[r] .. list_at[r + 1] - 1, one for each CTA that had chunks of it -------------------
   if (warp == 0) {
@@ -517,7 +523,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const __grid_c
       const int r = sm.row[at];
       const unsigned long long key = key_at(sm.chunk[at], i);
       sm.cand_s[to] = ((double)beam_value(key) - (double)sm.max[r]) + sm.off[r];
-      sm.cand_at[to] = (unsigned)r * (unsigned)p.V + (unsigned)beam_index(key);
+      sm.cand_at[to] = beam_place(r, key);
     });
   } else if (tid == 0) {
     sm.count = BEAM_CAP + 1;
@@ -527,24 +533,30 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const __grid_c
   if (n <= BEAM_CAP) {
     for (int i = tid; i < n; i += BEAM_THREADS) {
       const double s = sm.cand_s[i];
-      const unsigned at = sm.cand_at[i];
-      int rank = 0;
+      const unsigned long long at = sm.cand_at[i];
+      int rank = 0, equal = 0;
 #pragma unroll 4
-      for (int j = 0; j < n; ++j) rank += beam_better(sm.cand_s[j], sm.cand_at[j], s, at);
+      for (int j = 0; j < n; ++j) {
+        const double o = sm.cand_s[j];
+        rank += o > s;
+        equal += o == s;
+      }
+      if (equal > 1)                        // (rare: the places' loads beside the scores' took 2 us of 34 for 64 of 8,000)
+        for (int j = 0; j < n; ++j) rank += sm.cand_s[j] == s && sm.cand_at[j] > at;
       if (rank < p.K) write(rank, true, s, at);
     }
-    for (int k = n + tid; k < p.K; k += BEAM_THREADS) write(k, false, 0., 0u);
+    for (int k = n + tid; k < p.K; k += BEAM_THREADS) write(k, false, 0., 0ull);
     return;
   }
   // many equal ones: a round each, among the heads of the lists
   for (int i = tid; i < lists; i += BEAM_THREADS) sm.head[i] = 0;
   auto pick = [&]() {                       // (a thread's own lists)
-    BeamBest best = {-INFINITY, 0xffffffffu, -1};
+    BeamBest best = {-INFINITY, 0, -1};
     for (int i = tid; i < lists; i += BEAM_THREADS) {
       if (sm.head[i] >= p.K) continue;
       const int r = row_of(i);
       const unsigned long long key = key_at(chunk_of(r, i), sm.head[i]);
-      const BeamBest c = {key ? ((double)beam_value(key) - (double)sm.max[r]) + sm.off[r] : -INFINITY, (unsigned)r * (unsigned)p.V + (unsigned)beam_index(key), i};
+      const BeamBest c = {key ? ((double)beam_value(key) - (double)sm.max[r]) + sm.off[r] : -INFINITY, beam_place(r, key), i};
       if ((float)c.s > -INFINITY && (best.list < 0 || beam_better(c.s, c.at, best.s, best.at))) best = c;
     }
     return best;
@@ -555,7 +567,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_merge_kernel(const __grid_c
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const double s = __shfl_xor_sync(0xffffffffu, best.s, o);
-      const unsigned at = __shfl_xor_sync(0xffffffffu, best.at, o);
+      const unsigned long long at = __shfl_xor_sync(0xffffffffu, best.at, o);
       const int list = __shfl_xor_sync(0xffffffffu, best.list, o);
       if (list >= 0 && (best.list < 0 || beam_better(s, at, best.s, best.at))) best = {s, at, list};
     }

@@ -725,7 +725,7 @@ class DecodeOps:
         """The k best continuations of each request: its beams are rows cu[b] .. cu[b+1]-1 (int32 [B+1], at most 128 a request) of
         logits [R, V] (bf16 or fp32, any row stride) with their scores so far (fp32 [R]). out_scores (fp32), out_parents (the
         row) and out_tokens (int32), all [B, k] with k <= 64: the largest scores[r] + log_softmax(logits[r])[v], in order,
-        equal ones by row, then token; -inf, -1, -1 where fewer have a score above -inf. A logit of -inf excludes a token, a score of
+        equal ones by row, then logit and token; -inf, -1, -1 where fewer have a score above -inf. A logit of -inf excludes a token, a score of
         -inf a beam. A NaN or +inf among a row's logits (or as its score) sets the device error word (2) and excludes the row."""
         what, dev = "beam_select", logits.get_device()
         if dev < 0 or logits.dim() != 2 or logits.dtype not in (_BF16, _F32) or (logits.stride(1) != 1 and logits.shape[1] > 1):

@@ -65,3 +65,15 @@ def test_select_beams_of_a_low_score(dtype):
     err, got = select(logits, scores, [0, 4, 8], 20)
     assert err == 0 and all(p[:12] == [r] * 12 for p, r in zip(got[1], (0, 4)))
     check_masked(logits, scores, [0, 4, 8], 20, got)
+
+
+@pytest.mark.parametrize("V", [300, 50000])
+@pytest.mark.parametrize("score", [-1e12, -3e38, -15.0])
+def test_select_scores_that_swallow_the_logits(score, V):
+    """Equal scores in 64 bits, because a beam's score so far or the other logits are far larger: a row keeps the order of its logits."""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    logits = torch.rand(3, V, generator=g, device=DEV) * (1e-7 if score < -100 else 1e-18)
+    scores = torch.full((3,), score, device=DEV)
+    err, got = select(logits, scores, [0, 3], 40)
+    assert err == 0
+    check_masked(logits, scores, [0, 3], 40, got)
