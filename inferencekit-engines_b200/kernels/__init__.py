@@ -506,10 +506,10 @@ class DecodeOps:
             key = ("ragged" if maker == "attention_workspace" else maker, dev, stream)
             ws = self._scratch.get(key)
             if ws is None or ws.numel() < nbytes:
-                if ws is not None:
-                    self._outgrown.append(ws)
-                dest = torch.device("cuda", dev)
-                ws = self._scratch[key] = torch.zeros(nbytes, dtype=torch.uint8, device=dest) if nbytes else self.attention_workspace(dest)
+                # (no graph runs on an outgrown one, and the stream's calls are done with it before its memory is given out again: dropped,
+                # and replaced by half as much again, so that slowly growing calls replace few)
+                dest, grown = torch.device("cuda", dev), 0 if ws is None else ws.numel() * 3 // 2
+                ws = self._scratch[key] = torch.zeros(max(nbytes, grown), dtype=torch.uint8, device=dest) if nbytes else self.attention_workspace(dest)
         elif ws.dtype is not torch.uint8 or ws.get_device() != dev or not ws.is_contiguous():
             raise RuntimeError(f"{what}: workspace must come from {maker}() on the call's device")
         return ws
