@@ -33,6 +33,12 @@ __host__ __device__ constexpr int beam_min_chunks(int V, int size) {
 constexpr int BEAM_MAX_CHUNKS = beam_min_chunks(BEAM_MAX_VOCAB, 4);
 constexpr int BEAM_MAX_LISTS = BEAM_MAX_ROWS * BEAM_MAX_CHUNKS;
 
+// CTAs for `all` chunks on `sms` SMs: two an SM, and no more than that (all + 1) CTAs and chunks multiply within 32 bits. (The most
+// chunks, 65,536 rows of 129, leave 508.)
+inline int beam_grid(long long all, int sms) {
+  return (int)std::max(1ll, std::min(std::min(all, 2ll * sms), 0xffffffffll / (all + 1)));
+}
+
 struct BeamParams {
   const void* logits;   // row r at r * row_stride
   const float* scores;  // [R]
@@ -45,7 +51,7 @@ struct BeamParams {
   long long row_stride;
   int B, R, V, K, chunks, granules, grid;   // granules: 16-byte vectors of a chunk; grid: of the chunks' kernel
 };
-// CTA c has the chunks from beam_first(c) to beam_first(c + 1). (At most 2^23 chunks, 2^9 CTAs.)
+// CTA c has the chunks from beam_first(c) to beam_first(c + 1). (32 bits hold the products: beam_grid.)
 __device__ __forceinline__ int beam_first(const BeamParams& p, int c) { return (int)((unsigned)c * (unsigned)(p.R * p.chunks) / (unsigned)p.grid); }
 __device__ __forceinline__ int beam_owner(const BeamParams& p, int u) {
   return (int)(((unsigned)(u + 1) * (unsigned)p.grid - 1) / (unsigned)(p.R * p.chunks));

@@ -198,7 +198,7 @@ int qk_beam_select(const qk_beam_select_t* args, qk_stream_t stream) {
   p.chunks = beam_min_chunks(p.V, size);
   p.granules = (beam_granules(p.V, size) + p.chunks - 1) / p.chunks;
   const size_t all = (size_t)p.R * p.chunks;
-  p.grid = (int)std::max((size_t)1, std::min(all, (size_t)device_sms() * 2));
+  p.grid = beam_grid((long long)all, device_sms());
   p.keys = static_cast<unsigned long long*>(a.workspace);
   p.ml = reinterpret_cast<float2*>(p.keys + all * p.K);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -40,3 +40,19 @@ def test_dense_chunks_behind_sparse_ones(rows, some, k, dtype):
     scores = torch.randn(rows, generator=g, device=DEV) * 0.5 - 9
     cu = cumulative([min(60, rows - i) for i in range(0, rows, 60)])
     check_select(logits, scores, cu, k, select_again(logits, scores, cu, k, 20))
+
+
+def test_the_most_chunks_of_a_call():
+    """65,536 rows of 1,048,576 fp32 values (one row, at a stride of 0): 8,454,144 chunks, whose products with the CTAs pass 2^31."""
+    rows, V, k = 65536, 1 << 20, 2
+    g = torch.Generator(device=DEV).manual_seed(7)
+    row = torch.randn(1, V, generator=g, device=DEV)
+    scores = torch.randn(rows, generator=g, device=DEV)
+    cu = list(range(0, rows + 1, 128))
+    out = select_again(row.expand(rows, V), scores, cu, k, 1)
+    best = row[0].topk(2)
+    lp = best.values.double() - torch.logsumexp(row[0].double(), 0)
+    s = scores.view(-1, 128).double()
+    for b, (at, want) in enumerate(zip(s.argmax(1).tolist(), (s.amax(1) + lp[0]).tolist())):
+        assert (out[1][b][0], out[2][b][0]) == (cu[b] + at, best.indices[0].item()), b
+        assert abs(out[0][b][0] - want) <= abs(want) * 2.0 ** -24 + 2.0 ** -17
