@@ -36,3 +36,32 @@ def test_groups_of_different_sizes_in_one_range(name, fp8, way, monkeypatch):
     assert k.device_error() == 0
     assert (outs[0][s["cu"][-1]:] == 3).all() and all(torch.equal(out, outs[0]) for out in outs)
     check_shared(s, outs[0], fp8)
+
+
+# Chunks of prompts behind a shared one: sequences with more than 64 query rows a KV head are the tensor cores' for their own keys too, and
+# with 1,000 own keys and more (8 key tiles) they are cut between CTAs, beside sequences that are not cut, and some in no group.
+CHUNKS = {
+    "one_long": ([(2, 1024)], [1024, 1], [1500, 9], 32, 8, 64),
+    "several": ([(3, 512), (2, 1280), (2, None)], [300, 40, 1, 513, 128], [2000, 45, 1100, 1030, 900], 32, 8, 16),
+    "few_rows_of_long_own": ([(4, 2048)], [17, 33, 20, 65], [4000, 1025, 2050, 1200], 32, 8, 128),
+    "mha": ([(3, 640)], [200, 70, 129], [1300, 1100, 129], 4, 4, 32),
+    "one_kv_head": ([(5, 1024), (2, 256)], [64, 3, 90, 5, 400], [3000, 50, 1024, 1700, 400], 16, 1, 64),
+    "group_5": ([(3, 768)], [150, 14, 13], [1500, 1300, 40], 10, 2, 32),
+}
+
+
+@pytest.mark.parametrize("way", ["as_it_is", "large", "tensor"])
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "e4m3"])
+@pytest.mark.parametrize("name", CHUNKS)
+def test_long_chunks_behind_a_shared_prefix(name, fp8, way, monkeypatch):
+    monkeypatch.setitem(test_sharing_gpu.SHARED, name, CHUNKS[name])
+    k = ops()
+    s = shared_case(name, fp8, way=way)
+    ws = k.shared_workspace(DEV, *s["q"].shape[:2])
+    outs = [torch.full_like(s["q"], 3.0) for _ in range(3)]
+    k.device_error()
+    for out in outs:
+        run_shared(s, out, ws)
+    assert k.device_error() == 0
+    assert (outs[0][s["cu"][-1]:] == 3).all() and all(torch.equal(out, outs[0]) for out in outs)
+    check_shared(s, outs[0], fp8)
