@@ -404,7 +404,8 @@ int qk_packed_attention(const qk_ragged_attention_t* args, qk_stream_t stream);
  *   common: in the same pages, or in pages of equal contents. They are read through the group's first row, once for all its
  *   query rows. Every new token of a group comes after them (lens >= shared: else error word 2, and the group's rows are
  *   unspecified).
- *   Sequences in no group are on their own. workspace: qk_shared_attention_workspace_bytes(rows, n_q). */
+ *   Sequences in no group are on their own. workspace: qk_shared_attention_workspace_bytes(rows, n_q) bytes (some 104 MB, and 2.6 KB a
+ *   row and head), otherwise as qk_paged_attention's: zeroed once, and calls of other sizes may take any part of it from its start. */
 typedef struct {
   const int *refs, *lens, *fresh, *block_table, *groups;
   int *refs_out, *table_out, *cu_rows, *seq_lens, *slots, *positions, *shared, *info;

@@ -16,17 +16,26 @@
 
 namespace qk {
 
+// Sums (o under a maximum m in log2 units, and l) of row t, head h at t * n_q + h: over its own keys where one warp or CTA took them
+// all, and over its prefix, in 1, 2 or 4 parts, where one CTA did. In blocks, so that where a row's are goes by its number alone: calls
+// of any shape, on any part of a workspace, find info as the last one left it.
+constexpr int SHARED_BLOCK = 1024;
+struct SharedRows {
+  float own_o[SHARED_BLOCK][HEAD_DIM], o[SHARED_BLOCK][4][HEAD_DIM];
+  float2 own_ml[SHARED_BLOCK], ml[SHARED_BLOCK][4];
+  int own_info[SHARED_BLOCK], info[SHARED_BLOCK];   // what the kernels left (OWN_*, PREFIX_*), zero between launches
+};
 struct SharedParams {
   const int* groups;        // [G + 1]: group g is the sequences groups[g] .. groups[g + 1] - 1
   const int* shared;        // [G]: positions that they have in common
   int G;
-  // Sums (o under a maximum m in log2 units, and l) of row t, head h at t * n_q + h: over its own keys where one warp or CTA took them
-  // all, and over its prefix, in 1, 2 or 4 parts, where one CTA did.
-  float2* own_ml;           // [T][n_q]
-  float* own_o;             // [T][n_q][128]
-  float2* ml;               // [T][n_q][4]
-  float* o;                 // [T][n_q][4][128]
-  int *own_info, *info;     // [T][n_q], what the kernels left (OWN_*, PREFIX_*), zero between launches
+  SharedRows* rows;
+  __device__ __forceinline__ float* own_o(int at) const { return rows[(unsigned)at / SHARED_BLOCK].own_o[(unsigned)at % SHARED_BLOCK]; }
+  __device__ __forceinline__ float* o(int at, int part) const { return rows[(unsigned)at / SHARED_BLOCK].o[(unsigned)at % SHARED_BLOCK][part]; }
+  __device__ __forceinline__ float2* own_ml(int at) const { return &rows[(unsigned)at / SHARED_BLOCK].own_ml[(unsigned)at % SHARED_BLOCK]; }
+  __device__ __forceinline__ float2* ml(int at, int part) const { return &rows[(unsigned)at / SHARED_BLOCK].ml[(unsigned)at % SHARED_BLOCK][part]; }
+  __device__ __forceinline__ int* own_info(int at) const { return &rows[(unsigned)at / SHARED_BLOCK].own_info[(unsigned)at % SHARED_BLOCK]; }
+  __device__ __forceinline__ int* info(int at) const { return &rows[(unsigned)at / SHARED_BLOCK].info[(unsigned)at % SHARED_BLOCK]; }
   float* part;              // the prefixes' pieces, as in the tensor-core kernel, with maxima in log2 units
   float* part_ml;
   float* own_part;          // own keys' pieces: [warp][2][16 rows][128]
@@ -114,7 +123,7 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const __grid_constant
   const int at = (blockIdx.x * 2 + (warp >> 2)) * 2 + (lane & 1), q0 = lane >> 1;
   grid_dep_wait();
   grid_dep_launch();
-  const int info = at < p.rows ? __ldcg(x.info + at) : 0, own = at < p.rows ? __ldcg(x.own_info + at) : 0;
+  const int info = at < p.rows ? __ldcg(x.info(at)) : 0, own = at < p.rows ? __ldcg(x.own_info(at)) : 0;
   if (__syncthreads_or(info | own) == 0) return;
   const bool whole = info & PREFIX_WHOLE && !(info & PREFIX_WARPS);
   const int split = info >> 24 & 3, first = min(info & 255, 159), last = min(info >> 8 & 255, 159), row = info >> 16 & 255;
@@ -160,13 +169,13 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const __grid_constant
         const int k = pre ? i - w_own.parts : i;
         const size_t at_row = (size_t)((w.first + k) * 2 + (k == 0 ? w.code >> 24 & 1 : 0)) * 16 + (w.code >> 20 & 15);
         const bool sums = w.code & OWN_SUMS;
-        ml = !sums ? x.own_part_ml + at_row : pre ? x.ml + (size_t)at * 4 : x.own_ml + at;
-        src = (!sums ? x.own_part + at_row * HEAD_DIM : pre ? x.o + (size_t)at * 4 * HEAD_DIM : x.own_o + (size_t)at * HEAD_DIM) + 4 * q0;
+        ml = !sums ? x.own_part_ml + at_row : pre ? x.ml(at, 0) : x.own_ml(at);
+        src = (!sums ? x.own_part + at_row * HEAD_DIM : pre ? x.o(at, 0) : x.own_o(at)) + 4 * q0;
       } else {
         const int k = i - by_warp, part = k & ((1 << split) - 1), c = first + (k >> split), r = (row & 127) + part * (128 >> split);
         const size_t slot = ((size_t)(c * 2 + (c == first ? 1 : 0)) * 2 + (row >> 7)) * 128;
-        ml = whole ? x.ml + (size_t)at * 4 + part : reinterpret_cast<const float2*>(x.part_ml) + slot + (r & 127);
-        src = whole ? x.o + ((size_t)at * 4 + part) * HEAD_DIM + 4 * q0 : x.part + slot * 128 + (size_t)q0 * 512 + (r & 127) * 4;
+        ml = whole ? x.ml(at, part) : reinterpret_cast<const float2*>(x.part_ml) + slot + (r & 127);
+        src = whole ? x.o(at, part) + 4 * q0 : x.part + slot * 128 + (size_t)q0 * 512 + (r & 127) * 4;
         if (!whole) step = 16 * 512;
       }
       v[j] = __ldcg(ml);
@@ -183,7 +192,7 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const __grid_constant
   }
   __syncthreads();
   if (quarter || (info | own) == 0) return;
-  if (q0 == 0) x.info[at] = x.own_info[at] = 0;
+  if (q0 == 0) *x.info(at) = *x.own_info(at) = 0;
   if (own == 0) return;                     // a sequence with more rows than max_q says: nobody took its own keys
 #pragma unroll
   for (int k = 1; k < 4; ++k) add(sum_ml[warp + k][lane], sum[warp + k][0][lane], sum[warp + k][1][lane]);
@@ -464,10 +473,10 @@ __global__ void __launch_bounds__(32) own_attention_kernel(const __grid_constant
           if (row >= rows) continue;
           const int sum_at = (s.row0 + by_group(from + row, r.group)) * r.n_q + at.g * r.group + from + row - by_group(from + row, r.group) * r.group;
           if (lg == 0) {
-            *(!whole ? p.x.own_part_ml + slot + row : prefix ? p.x.ml + (size_t)sum_at * 4 : p.x.own_ml + sum_at) = make_float2(w.m[nt][e], w.l[nt][e]);
-            if (t0 == 0) *(prefix ? p.x.info + sum_at : p.x.own_info + sum_at) = code | row << 20 | (prefix ? PREFIX_WARPS : 0);
+            *(!whole ? p.x.own_part_ml + slot + row : prefix ? p.x.ml(sum_at, 0) : p.x.own_ml(sum_at)) = make_float2(w.m[nt][e], w.l[nt][e]);
+            if (t0 == 0) *(prefix ? p.x.info(sum_at) : p.x.own_info(sum_at)) = code | row << 20 | (prefix ? PREFIX_WARPS : 0);
           }
-          float* dst = !whole ? p.x.own_part + (slot + row) * HEAD_DIM : prefix ? p.x.o + (size_t)sum_at * 4 * HEAD_DIM : p.x.own_o + (size_t)sum_at * HEAD_DIM;
+          float* dst = !whole ? p.x.own_part + (slot + row) * HEAD_DIM : prefix ? p.x.o(sum_at, 0) : p.x.own_o(sum_at);
 #pragma unroll
           for (int i = 0; i < 8; i += 2) {
             if (FP8) {                      // 16 dims in a row

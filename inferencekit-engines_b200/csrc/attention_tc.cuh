@@ -949,7 +949,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
         const float m2 = m == -INFINITY ? m : m * sl2 + TCA_SHIFT;
         if ((MODE == TC_PREFIX || (MODE == TC_OWN && w.s.start)) && w.t0 == 0 && w.t1 == w.n) {
           if (any) {
-            float* sums = MODE == TC_PREFIX ? p.x.o + ((size_t)row_at * 4 + part) * HEAD_DIM : p.x.own_o + (size_t)row_at * HEAD_DIM;
+            float* sums = MODE == TC_PREFIX ? p.x.o(row_at, part) : p.x.own_o(row_at);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               uint32_t o[32];
@@ -963,9 +963,9 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
               __syncwarp();
             }
             if (valid) {
-              *(MODE == TC_PREFIX ? p.x.ml + (size_t)row_at * 4 + part : p.x.own_ml + row_at) = make_float2(m2, l);
-              if (MODE == TC_OWN) p.x.own_info[row_at] = OWN_SUMS;
-              else if (part == 0) p.x.info[row_at] = PREFIX_WHOLE | split << 24;
+              *(MODE == TC_PREFIX ? p.x.ml(row_at, part) : p.x.own_ml(row_at)) = make_float2(m2, l);
+              if (MODE == TC_OWN) *p.x.own_info(row_at) = OWN_SUMS;
+              else if (part == 0) *p.x.info(row_at) = PREFIX_WHOLE | split << 24;
             }
             __syncwarp();
           }
@@ -1008,7 +1008,7 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
           }
         }
         if (MODE == TC_PREFIX) {              // (the merge adds the pieces)
-          if (valid && w.t0 == 0 && part == 0) p.x.info[row_at] = PREFIX_PIECES | (c_lo - 1) | c_hi << 8 | (x * 128 + row) << 16 | split << 24;
+          if (valid && w.t0 == 0 && part == 0) *p.x.info(row_at) = PREFIX_PIECES | (c_lo - 1) | c_hi << 8 | (x * 128 + row) << 16 | split << 24;
           __syncwarp();
           continue;
         }
@@ -1043,8 +1043,8 @@ __global__ void __launch_bounds__(TcShape<SRC>::THREADS, 1) tc_attention_kernel(
             }
             if (MODE == TC_OWN && w.s.start) {
 #pragma unroll
-              for (int k = 0; k < 64; k += 4) *reinterpret_cast<float4*>(p.x.own_o + (size_t)row_at * HEAD_DIM + col + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-              if (col == 0) p.x.own_ml[row_at] = make_float2(M == -INFINITY ? M : M * sl2 + TCA_SHIFT, L), p.x.own_info[row_at] = OWN_SUMS;
+              for (int k = 0; k < 64; k += 4) *reinterpret_cast<float4*>(p.x.own_o(row_at) + col + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+              if (col == 0) *p.x.own_ml(row_at) = make_float2(M == -INFINITY ? M : M * sl2 + TCA_SHIFT, L), *p.x.own_info(row_at) = OWN_SUMS;
               continue;
             }
             const float inv = L == 0.f ? 0.f : 1.f / L;

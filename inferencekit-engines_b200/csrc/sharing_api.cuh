@@ -36,7 +36,6 @@ struct SharedWorkspace {
   float2 own_ml[OWN_MAX_GRID * 2 * 16];
   float own_part[OWN_MAX_GRID * 2 * 16 * HEAD_DIM];
 };
-constexpr long long SHARED_ROW = 5 * (HEAD_DIM * 4 + 8) + 8;   // bytes of a row and head: sums, and info
 constexpr long long shared_fixed_bytes() { return ((long long)sizeof(SharedWorkspace) + 255) / 256 * 256; }
 
 template <bool FP8, int NT>
@@ -215,7 +214,7 @@ int qk_beam_select(const qk_beam_select_t* args, qk_stream_t stream) {
 
 long long qk_shared_attention_workspace_bytes(long long rows, long long n_q) {
   if (rows < 0 || rows > 0x7fffffffll / 64 || n_q < 1 || n_q > 32768 || rows > 0x7fffffffll / n_q) return -1;
-  return shared_fixed_bytes() + (rows * n_q + 3) / 4 * 4 * SHARED_ROW;
+  return shared_fixed_bytes() + (rows * n_q + SHARED_BLOCK - 1) / SHARED_BLOCK * (long long)sizeof(SharedRows);
 }
 
 int qk_shared_attention(const qk_shared_attention_t* args, qk_stream_t stream) {
@@ -236,14 +235,7 @@ int qk_shared_attention(const qk_shared_attention_t* args, qk_stream_t stream) {
   SharedWorkspace* fixed = static_cast<SharedWorkspace*>(a.att.workspace);
   x.part = fixed->prefix_part, x.part_ml = fixed->prefix_ml;
   x.own_part = fixed->own_part, x.own_part_ml = fixed->own_ml;
-  // where the rows' sums are goes by the workspace's size: calls of any shape find info as the last one left it
-  const size_t room = (size_t)(a.att.workspace_bytes - shared_fixed_bytes()) / (4 * SHARED_ROW) * 4;
-  x.own_o = reinterpret_cast<float*>(ws + shared_fixed_bytes());
-  x.o = x.own_o + room * HEAD_DIM;
-  x.own_ml = reinterpret_cast<float2*>(x.o + room * 4 * HEAD_DIM);
-  x.ml = x.own_ml + room;
-  x.info = reinterpret_cast<int*>(x.ml + room * 4);
-  x.own_info = x.info + room;
+  x.rows = reinterpret_cast<SharedRows*>(ws + shared_fixed_bytes());
   return a.att.cache.kv_fp8 ? shared_launches<true>(p, a.att, x, static_cast<cudaStream_t>(stream))
                             : shared_launches<false>(p, a.att, x, static_cast<cudaStream_t>(stream));
 }

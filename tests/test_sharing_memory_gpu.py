@@ -46,3 +46,20 @@ def test_results_on_a_workspace_that_was_replaced():
         for i in range(3):
             check_shared(cases[i], outs[i])
             check_select(x[i], scores[:len(x[i])], cu[i].tolist(), 16, [t.tolist() for t in sel[i]])
+
+
+def test_calls_take_as_much_of_a_workspace_as_they_need():
+    """One buffer, of which each call is given what it needs for its own rows: larger and smaller calls in turn."""
+    k = ops()
+    cases = [(n, shared_case(n, fp8, seed=i, way=("tensor", "large", "as_it_is")[i % 3]), fp8)
+             for i, (n, fp8) in enumerate((n, fp8) for n in ("beams", "large", "mha", "chunks", "drafts") for fp8 in (False, True))]
+    size = [k.lib.qk_shared_attention_workspace_bytes(*s["q"].shape[:2]) for _, s, _ in cases]
+    assert len(set(size)) > 2
+    ws = torch.zeros(max(size), dtype=torch.uint8, device=DEV)
+    k.device_error()
+    for _ in range(2):
+        for n, (name, s, fp8) in zip(size, cases):
+            out = torch.zeros_like(s["q"])
+            run_shared(s, out, ws[:n])
+            assert k.device_error() == 0, name
+            check_shared(s, out, fp8)
