@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import test_sharing_gpu
-from test_paged_gpu import DEV, ops
+from test_paged_gpu import D, DEV, attend64, check_attention, ints, ops
 from test_sharing_calls_gpu import check_shared, run_shared
 from test_sharing_gpu import shared_case
 
@@ -65,3 +65,28 @@ def test_long_chunks_behind_a_shared_prefix(name, fp8, way, monkeypatch):
     assert k.device_error() == 0
     assert (outs[0][s["cu"][-1]:] == 3).all() and all(torch.equal(out, outs[0]) for out in outs)
     check_shared(s, outs[0], fp8)
+
+
+@pytest.mark.parametrize("max_q", [3, 200])
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "e4m3"])
+def test_rows_that_see_nothing(fp8, max_q, monkeypatch):
+    """Sequences shorter than their new tokens, or empty: the first rows give zeros, as in paged_attention, beside a shared prefix."""
+    monkeypatch.setitem(test_sharing_gpu.SHARED, "short", ([(30, 1280), (5, None)], [1, max_q], [200], 32, 8, 32))
+    k = ops()
+    s = shared_case("short", fp8)
+    n, lens = s["n"], s["lens"]
+    for b, length in ((30, 0), (31, max_q - 2), (33, 1), (34, 0)):
+        lens[b] = length
+        s["rows"][b] = [x[:length] for x in s["rows"][b]]
+    out, want = torch.full_like(s["q"], 3.0), torch.full_like(s["q"], 3.0)
+    k.device_error()
+    run_shared(s, out)
+    k.paged_attention(s["q"], ints(s["cu"]), ints(lens), s["table"], s["k"], s["v"], want, D ** -0.5, max_q, k_scale=s["ks"], v_scale=s["vs"])
+    assert k.device_error() == 0
+    for b, length in ((30, 0), (31, max_q - 2), (33, 1), (34, 0)):
+        a, z = s["cu"][b], s["cu"][b + 1]
+        hidden = z - a - length                     # rows of the sequence that see nothing
+        assert (out[a:a + hidden] == 0).all() and (want[a:a + hidden] == 0).all() and (out[a + hidden:z] != 0).any(-1).all()
+    keep = [b for b in range(30)] + [32]
+    check_attention(torch.cat([out[s["cu"][b]:s["cu"][b + 1]] for b in keep]), *(torch.cat(x) for x in zip(*[
+        attend64(s["q"][s["cu"][b]:s["cu"][b + 1]].double(), *s["rows"][b], lens[b] - n[b], D ** -0.5) for b in keep])), fp8)
