@@ -404,7 +404,10 @@ int qk_packed_attention(const qk_ragged_attention_t* args, qk_stream_t stream);
  *   common: in the same pages, or in pages of equal contents. They are read through the group's first row, once for all its
  *   query rows. Every new token of a group comes after them (lens >= shared: else error word 2, and the group's rows are
  *   unspecified).
- *   Sequences in no group are on their own. workspace: qk_shared_attention_workspace_bytes(rows, n_q) bytes (some 104 MB, and 2.6 KB a
+ *   Sequences in no group are on their own. Roundings: rows whose prefix goes over the tensor cores (which depends on all groups of the
+ *   call, so a row's last bits do too) and sequences of more than 64 query rows a KV head have their weights rounded to bf16, as the larger
+ *   batches of qk_paged_attention; the others keep the remainder too; sums are fp32. An infinity in a V row of the shared positions makes the
+ *   rows that see it infinite or NaN. workspace: qk_shared_attention_workspace_bytes(rows, n_q) bytes (some 104 MB, and 2.6 KB a
  *   row and head), otherwise as qk_paged_attention's: zeroed once, and calls of other sizes may take any part of it from its start. */
 typedef struct {
   const int *refs, *lens, *fresh, *block_table, *groups;

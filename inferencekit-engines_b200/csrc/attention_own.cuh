@@ -52,7 +52,8 @@ constexpr int SHARED_MIN_KEYS = 256;  // shorter ones too
 // The tensor cores' launch pays where it saves so many reads of a key (for one KV head) in all: it and the merge of its sums take some
 // 10 us, and a shared page that is read again comes out of the L2 cache. Measured, shared against not: 16 sequences behind
 // 2,048 keys (246,000 reads) 25 us against 27; 64 behind 512 (258,000) 33 against 32; 8 groups of 8 behind 512 (229,000) 31
-// against 33, behind 1,024 38 against 47; e4m3 pages alike.
+// against 33, behind 1,024 38 against 47; e4m3 pages alike. (So near the border it is wrong by 1 or 2 us either way: the number of reads
+// does not say it all.)
 constexpr long long SHARED_MIN_READS = 240000;
 // A prefix that the warps take is read once for every 16 rows (the second time out of the L2 cache): those of one block of rows, and of
 // up to four where that is few reads in all. Measured, warps against tensor cores: 8 sequences behind 4,096 keys (65,000 reads) 25 us against
